@@ -476,6 +476,68 @@ int q3_greedy_select(int dtype, const void* logits, int64_t ld, int64_t batch, i
  * No counterpart in the reference: it is what lets one captured decode step serve every position. */
 int q3_advance(int64_t* counter, int64_t by, hipStream_t stream);
 
+/* ------------------------------------------------------------------ 8-bit serving
+ * Codes of 8 bits with fp32 scales.  A group of values a with M = max |a| is held as q = the integer nearest to 127 a / M
+ * (ties to even, decided exactly) and a scale of M / 127; a group that holds an infinity or a NaN gets the scale NaN, so
+ * whatever is formed from it is NaN.  dtype is Q3_BF16 or Q3_F16 throughout.  Forward only.  New here: the reference
+ * serves in 16 bits.
+ *
+ * Rows of x [rows, h] (row stride ldx): q [rows, h], scale [rows] = M / 127.  16-byte aligned x and q, ldx % 8 == 0,
+ * h % 16 == 0, h <= 32768.  Also a weight's output channels (rows of W). */
+int q3_quant_rows(int dtype, const void* x, int64_t ldx, int8_t* q, float* scale, int64_t rows, int64_t h,
+                  hipStream_t stream);
+/* RMSNorm with that output: t = round(x + res) to dtype (stored to total [rows, h]; res and total both or neither),
+ * a = t * w, q as above, scale = M / 127 * rsqrt(mean(t^2) + eps).  Same limits. */
+int q3_rmsnorm_quant(int dtype, const void* x, int64_t ldx, const void* res, int64_t ldres, const void* w, int8_t* q,
+                     float* scale, void* total, int64_t rows, int64_t h, float eps, hipStream_t stream);
+/* c[m, n] = round((sum_k a[m, k] b[n, k]) * a_scale[m] * b_scale[n] (+ res[m, n])), the sum exact in int32.
+ *   epilogue Q3_GEMM_PLAIN: up to 3 pieces along n (end[i]: where piece i ends), each with a B, its scales and a C;
+ *   Q3_GEMM_RESIDUAL: one piece, res added before the one rounding (c may be res);
+ *   Q3_GEMM_GATE_UP: b[0], b[1] the gate and up weights [n, k] at one ldb, c = round(silu(g) * u) of the unrounded g, u.
+ * k % 16 == 0, k < 2^17, 16-byte aligned operands with row strides % 16 == 0 and below 2^23; gate/up: n % 8 == 0, c
+ * 16-byte aligned with ldc % 8 == 0. */
+typedef struct q3_int8_gemm_desc {
+  int dtype, pieces, epilogue;
+  int64_t m, n, k, end[3];
+  const int8_t* a;
+  int64_t lda;
+  const float* a_scale;
+  const int8_t* b[3];
+  int64_t ldb[3];
+  const float* b_scale[3];
+  void* c[3];
+  int64_t ldc[3];
+  const void* res;
+  int64_t ldres;
+} q3_int8_gemm_desc;
+size_t q3_gemm_int8_workspace_bytes(const q3_int8_gemm_desc* desc);
+int q3_gemm_int8(const q3_int8_gemm_desc* desc, void* workspace, size_t workspace_bytes, hipStream_t stream);
+/* Key/value cache in 8 bits, d = 128, blocks of 64 positions (Cb = ceil(capacity / 64)) with a scale per block and head:
+ *   cache_k [B, H, 64 Cb, 128], cache_v [B, H, Cb, 128, 64] (transposed within a block), scale_k / scale_v [B, H, Cb],
+ *   tail_k [B, H, 64, 128], tail_v [B, H, 128, 64] in dtype: the positions of the last, unfinished block.
+ * append writes k, v [B, S, H, 128] (strides of batch, position, head; multiples of 8) at positions start .. start + S - 1:
+ * a block is quantised, from its 16-bit values, when its last position comes.  The cache must hold exactly the positions
+ * before start.  With start_dev (S = 1) the position is read from that device int64; positions outside the capacity are
+ * skipped. */
+int q3_kv8_append(int dtype, const void* k, int64_t ksb, int64_t kss, int64_t ksh, const void* v, int64_t vsb, int64_t vss,
+                  int64_t vsh, int8_t* cache_k, int8_t* cache_v, float* scale_k, float* scale_v, void* tail_k, void* tail_v,
+                  int64_t B, int64_t S, int64_t H, int64_t d, int64_t capacity, int64_t start, const int64_t* start_dev,
+                  hipStream_t stream);
+/* k, v [B, H, length, 128] in out_dtype (any): code * scale rounded once, the tail's positions as they are. */
+int q3_kv8_read(int dtype, int out_dtype, const int8_t* cache_k, const int8_t* cache_v, const float* scale_k,
+                const float* scale_v, const void* tail_k, const void* tail_v, void* k, void* v, int64_t B, int64_t H,
+                int64_t d, int64_t capacity, int64_t length, hipStream_t stream);
+/* Causal attention of q [B, S, Hq, 128] (strides, multiples of 8) at positions start .. start + S - 1 over the cache's
+ * positions 0 .. start + S - 1 (already appended); out strides are multiples of 4, out 8-byte aligned.  With start_dev
+ * (S = 1) the position is read from that device int64 and the workspace is sized for span = capacity, else
+ * span = start + S. */
+size_t q3_kv8_attention_workspace_bytes(int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t span);
+int q3_kv8_attention(int dtype, const void* q, int64_t qsb, int64_t qss, int64_t qsh, const int8_t* cache_k,
+                     const int8_t* cache_v, const float* scale_k, const float* scale_v, const void* tail_k,
+                     const void* tail_v, void* out, int64_t osb, int64_t oss, int64_t osh, void* workspace,
+                     size_t workspace_bytes, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t d, int64_t capacity,
+                     int64_t start, const int64_t* start_dev, float scale, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -72,7 +72,18 @@ struct Args {
   const int64_t* tgt;
   float *m_part, *s_part, *pick;
   int64_t part0, ldp, col0;
+  // Q8: scales of the A rows, and of the B rows of each piece (gate/up: of Wg and Wu)
+  const float* rscale;
+  const float* cscale[3];
 };
+
+// Q8: operands are codes of 8 bits, two to a 16-bit element (so M, N, K, row strides and tiles above count pairs along k),
+// and the products exact int32 sums: the same 16-byte fragments, on v_mfma_i32_16x16x64_i8, 128 codes of k per k-tile.
+template <bool Q8> struct AccOf { typedef f32x4 type; };
+template <> struct AccOf<true> { typedef i32x4 type; };
+Q3_DEV void mfma_acc(i32x4& c, bf16x8_t a, bf16x8_t b) {
+  c = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
+}
 
 // Work item -> (tile, split): each XCD (workgroup ids congruent mod 8) takes a contiguous range of items,
 // splits outermost, so its L2 holds one k-range of the shared operand; tiles in groups of 4 tile-rows.
@@ -93,7 +104,7 @@ Q3_DEV void work_coords(int bid, int tiles_m, int tiles_n, int splits, int& tm, 
 // EPI 0: plain / residual / split partials; 2: cross-entropy statistics (per row and 128-column group: the max and the
 // sum of exp(z - max) to m_part / s_part [part0 + group][row], the logit of column tgt[row] - col0 to pick[row]) of
 // the rounded logits, which are stored too; 3: gate/up SwiGLU; 5: SwiGLU backward.  KP: A and B in pieces along K.
-template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool AT, bool BT, int EPI, bool KP>
+template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool AT, bool BT, int EPI, bool KP, bool Q8>
 __global__ __launch_bounds__(WM * WN * 64) void gemm_tile_kernel(Args ar) {
   constexpr int NW = WM * WN;
   constexpr int TMW = BM / WM, TNW = BN / WN, FM = TMW / 16, FN = TNW / 16;
@@ -103,6 +114,8 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile_kernel(Args ar) {
   static_assert(TMW % 16 == 0 && TNW % 16 == 0, "fragments");
   static_assert(!AT || (BM == 64 || BM == 128 || BM == 256), "K-major slots");
   static_assert(!BT || (BN == 64 || BN == 128 || BN == 256), "K-major slots");
+  static_assert(!Q8 || (!AT && !BT && !KP && (EPI == 0 || EPI == 3)), "8-bit codes: two k-contiguous operands");
+  typedef typename AccOf<Q8>::type acc_t;
   constexpr int LPW = (AL + BL) / NW, LA = AL / NW;
   constexpr int ABYTES = tile_bytes<BM, AT>(), STAGE = ABYTES + tile_bytes<BN, BT>();
   constexpr int BMAX = BM * BN * 2;
@@ -120,6 +133,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile_kernel(Args ar) {
   const u16 *pa = ar.a.p[0], *pb = ar.b.p[0];
   int64_t lda = ar.a.ld[0], ldb = ar.b.ld[0], ldc = ar.ldc[0];
   void* cp = ar.c[0];
+  [[maybe_unused]] const float* csc = ar.cscale[0];
   int begm = 0, begn = 0, mrows = M, ncols = N;  // the piece's first row / column, its extent
   if (ar.axis >= 2) {
     int s = 0, t = ar.axis == 2 ? tn : tm, beg = 0;
@@ -130,6 +144,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile_kernel(Args ar) {
     }
     cp = ar.c[s];
     ldc = ar.ldc[s];
+    if constexpr (Q8) csc = ar.cscale[s];
     if (ar.axis == 2) {
       pb = ar.b.p[s];
       ldb = ar.b.ld[s];
@@ -273,11 +288,11 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile_kernel(Args ar) {
     }
   };
 
-  f32x4 acc[FM][FN];
+  acc_t acc[FM][FN];
 #pragma unroll
   for (int i = 0; i < FM; ++i)
 #pragma unroll
-    for (int j = 0; j < FN; ++j) acc[i][j] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int j = 0; j < FN; ++j) acc[i][j] = acc_t{0, 0, 0, 0};
 
 #pragma unroll
   for (int st = 0; st < STAGES - 1; ++st) {
@@ -307,7 +322,10 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile_kernel(Args ar) {
 #pragma unroll
       for (int i = 0; i < FM; ++i)
 #pragma unroll
-        for (int j = 0; j < FN; ++j) acc[i][j] = mfma_16x16x32<T>(bfr[ks][j], af[ks][i], acc[i][j]);
+        for (int j = 0; j < FN; ++j) {
+          if constexpr (Q8) mfma_acc(acc[i][j], bfr[ks][j], af[ks][i]);
+          else acc[i][j] = mfma_16x16x32<T>(bfr[ks][j], af[ks][i], acc[i][j]);
+        }
       // spread the step's memory instructions through its MFMAs (refills first, two MFMAs apart where
       // there are enough of them, then the fragment reads; the other step's reads start after 3/8 of them)
       if constexpr (MF >= 16) {
@@ -369,14 +387,80 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile_kernel(Args ar) {
 #pragma unroll
         for (int j = 0; j < FN; ++j) {
           const int col = nb + wn * TNW + j * 16 + 4 * quarter;  // pieces and N are multiples of 8
-          if (col < ncols) *reinterpret_cast<f32x4*>(P + (int64_t)(begm + row) * N + begn + col) = acc[i][j];
+          if (col < ncols) *reinterpret_cast<acc_t*>(P + (int64_t)(begm + row) * N + begn + col) = acc[i][j];
         }
       }
     }
     return;
   }
   u16* C = reinterpret_cast<u16*>(cp);
-  {
+  // Q8: this lane's element e of block (i, j) in fp32, by its row's and column's scales
+  [[maybe_unused]] auto scaled = [&](int i, int j, const float* cs, int col, int lim, float rs, float (&v)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) v[e] = (float)acc[i][j][e] * rs * cs[min(col + e, lim - 1)];
+  };
+  if constexpr (Q8) {
+    // One rounding: the product scaled, the residual (or SwiGLU) formed in fp32, then staged through LDS as below
+    if (ar.vec || EPI == 3) {
+      constexpr int NC = EPI == 3 ? TNW / 2 : TNW, CH = NC / 8, RPI = 64 / CH, DIV = EPI == 3 ? 2 : 1;
+      static_assert(CH == 2 || CH == 4 || CH == 8 || CH == 16, "16-byte chunks per staged row");
+      char* wl = lds + wave * (TMW * NC * 2);
+      auto swz = [&](int r) { return CH == 16 ? (r & 15) : CH == 8 ? ((r >> 1) & 7) : CH == 4 ? ((r >> 2) & 3) : ((r >> 3) & 1); };
+      const int cb = (nb + wn * TNW) / DIV, clim = ncols / DIV;  // the wave's first output column, their number
+#pragma unroll
+      for (int i = 0; i < FM; ++i) {
+        const int row = min(ma + wm * TMW + i * 16 + j16, mrows - 1);
+        const float rs = ar.rscale[begm + row];
+#pragma unroll
+        for (int j = 0; j < FN; j += DIV) {
+          const int col = cb + j / DIV * 16 + 4 * quarter;
+          float v[4];
+          scaled(i, j, csc, col, clim, rs, v);
+          if constexpr (EPI == 3) {
+            float u[4];
+            scaled(i, j + 1, ar.cscale[1], col, clim, rs, u);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = v[e] * q3_sigmoid(v[e]) * u[e];
+          } else if (ar.res && col < clim) {  // whole 8-column groups: col + 3 is a column too
+            const i32x2 x = *reinterpret_cast<const i32x2*>(ar.res + (int64_t)row * ar.ldres + col);
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] += to_f32<T>((u16)((uint32_t)x[e >> 1] >> (16 * (e & 1))));
+          }
+          const int r = i * 16 + j16, c = (j / DIV * 16 + 4 * quarter) >> 3;
+          *reinterpret_cast<i32x2*>(wl + r * (NC * 2) + ((c ^ swz(r)) << 4) + (quarter & 1) * 8) =
+              i32x2{(int)pack2<T>(v[0], v[1]), (int)pack2<T>(v[2], v[3])};
+        }
+      }
+      lds_wait();
+      __builtin_amdgcn_wave_barrier();
+      const int c = lane % CH, rlim = min(mrows - ma - wm * TMW, TMW);
+#pragma unroll
+      for (int q = 0; q < (TMW + RPI - 1) / RPI; ++q) {
+        const int r = q * RPI + lane / CH;
+        if (r < rlim && cb + c * 8 < clim)
+          *reinterpret_cast<i32x4*>(C + (int64_t)(ma + wm * TMW + r) * ldc + cb + c * 8) =
+              *reinterpret_cast<const i32x4*>(wl + r * (NC * 2) + ((c ^ swz(r)) << 4));
+      }
+      return;
+    }
+#pragma unroll
+    for (int i = 0; i < FM; ++i) {
+      const int row = ma + wm * TMW + i * 16 + j16;
+      if (row >= mrows) continue;
+      const float rs = ar.rscale[begm + row];
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        const int col = nb + wn * TNW + j * 16 + 4 * quarter;
+        float v[4];
+        scaled(i, j, csc, col, ncols, rs, v);
+#pragma unroll
+        for (int e = 0; e < 4; ++e)
+          if (col + e < ncols)
+            C[(int64_t)row * ldc + col + e] =
+                from_f32<T>(ar.res ? v[e] + to_f32<T>(ar.res[(int64_t)row * ar.ldres + col + e]) : v[e]);
+      }
+    }
+  } else {
     // 16-bit outputs: each wave rounds its tile into a private LDS block (16-byte chunks XOR-swizzled by row),
     // then works on whole rows with 16-byte accesses.
     if (ar.vec || EPI != 0) {
@@ -548,7 +632,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile_kernel(Args ar) {
       }
     }
   }
-  if constexpr (EPI == 0) {
+  if constexpr (EPI == 0 && !Q8) {
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       const int row = ma + wm * TMW + i * 16 + j16;
@@ -569,10 +653,10 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile_kernel(Args ar) {
   }
 }
 
-template <typename T, int BM, int BN, int WM, int WN, int ST, bool AT, bool BT, int EPI, bool KP = false>
+template <typename T, int BM, int BN, int WM, int WN, int ST, bool AT, bool BT, int EPI, bool KP = false, bool Q8 = false>
 int launch_tile(const Args& a, hipStream_t s) {
   const int64_t tiles = (int64_t)a.tms * a.tns * a.splits;
-  gemm_tile_kernel<T, BM, BN, WM, WN, ST, AT, BT, EPI, KP><<<(unsigned)tiles, WM * WN * 64, 0, s>>>(a);
+  gemm_tile_kernel<T, BM, BN, WM, WN, ST, AT, BT, EPI, KP, Q8><<<(unsigned)tiles, WM * WN * 64, 0, s>>>(a);
   return (int)hipGetLastError();
 }
 

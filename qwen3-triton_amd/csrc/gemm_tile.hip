@@ -7,6 +7,7 @@ namespace q3gemm {
 int launch_tile_nt(int dtype, int cfg, int epi, const Args& a, hipStream_t s);
 int launch_tile_nn(int dtype, int cfg, int epi, const Args& a, hipStream_t s);
 int launch_tile_tn(int dtype, int cfg, const Args& a, hipStream_t s);
+int launch_tile_q8(int dtype, int cfg, int epi, const Args& a, hipStream_t s);
 }  // namespace q3gemm
 
 namespace {
@@ -132,6 +133,34 @@ template <typename T> __global__ __launch_bounds__(256) void combine_kernel(Args
   store_vec<T>(reinterpret_cast<u16*>(a.c[s]) + r * a.ldc[s] + c, v);
 }
 
+// The partial products of 8-bit codes: int32 sums (exact in any order), the scales, the residual added in fp32, one rounding.
+template <typename T> __global__ __launch_bounds__(256) void combine_q8_kernel(Args a) {
+  const int64_t cols = a.N / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
+  if (i >= a.M * cols) return;
+  const int64_t r = i / cols;
+  int64_t c = (i - r * cols) * 8;
+  const int* p = reinterpret_cast<const int*>(a.part) + r * a.N + c;
+  i32x4 s0 = *reinterpret_cast<const i32x4*>(p), s1 = *reinterpret_cast<const i32x4*>(p + 4);
+  for (int k = 1; k < a.splits; ++k) {
+    p += a.M * a.N;
+    s0 += *reinterpret_cast<const i32x4*>(p);
+    s1 += *reinterpret_cast<const i32x4*>(p + 4);
+  }
+  int s = 0;
+  if (a.axis == 2)
+    while (s + 1 < a.pieces && c >= a.len[s]) c -= a.len[s++];
+  const float rs = a.rscale[r];
+  Vec<T> v;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) v.v[e] = (float)(e < 4 ? s0[e] : s1[e - 4]) * rs * a.cscale[s][c + e];
+  if (a.res) {
+    const Vec<T> b = load_vec<T>(a.res + r * a.ldres + c);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) v.v[e] += b.v[e];
+  }
+  store_vec<T>(reinterpret_cast<u16*>(a.c[s]) + r * a.ldc[s] + c, v);
+}
+
 // The same for one whole row per 512-thread workgroup (N <= 8192), also writing
 // Y = C rsqrt(mean(C^2) + eps) w, the RMSNorm that follows (from the rounded C, one rounding).
 template <typename T>
@@ -178,6 +207,7 @@ struct Call {
   double combine;
   bool at, bt, can_split;
   int epi;
+  bool q8;
 };
 
 bool operand_ok(const void* p, int64_t ld, int64_t rows, int64_t k, bool kmajor) {
@@ -194,6 +224,7 @@ bool parse(const q3_gemm_desc* d, Call& c) {
   if (d->axis < 0 || d->axis > 3 || (d->axis == 0 ? d->pieces != 1 : (d->pieces < 1 || d->pieces > 3))) return false;
   Args& a = c.a;
   a = Args{};
+  c.q8 = false;
   c.at = d->a_kmajor != 0;
   c.bt = d->b_kmajor != 0;
   if (c.at && !c.bt) return false;
@@ -266,6 +297,64 @@ bool parse(const q3_gemm_desc* d, Call& c) {
   return tile_rows(a, 32) * tile_cols(a, 64) < (1ll << 28);
 }
 
+// 8-bit operands: pairs of codes along k are the 16-bit elements of the tiles above.
+bool parse_int8(const q3_int8_gemm_desc* d, Call& c) {
+  if (!d || (d->dtype != Q3_BF16 && d->dtype != Q3_F16)) return false;
+  if (d->m < 1 || d->n < 1 || d->k < 16 || d->m >= (1ll << 31) - 256 || d->n >= (1ll << 30) || d->k >= (1ll << 17) || d->k % 16)
+    return false;
+  const bool gate_up = d->epilogue == Q3_GEMM_GATE_UP, residual = d->epilogue == Q3_GEMM_RESIDUAL;
+  if (!gate_up && !residual && d->epilogue != Q3_GEMM_PLAIN) return false;
+  if (d->pieces < 1 || d->pieces > 3 || ((gate_up || residual) && d->pieces != 1)) return false;
+  Args& a = c.a;
+  a = Args{};
+  c.q8 = true;
+  c.at = c.bt = false;
+  c.epi = gate_up ? 3 : 0;
+  a.axis = d->pieces > 1 ? 2 : 0;
+  a.pieces = d->pieces;
+  a.M = d->m;
+  a.N = gate_up ? 2 * d->n : d->n;
+  a.K = d->k / 2;
+  a.splits = 1;
+  auto operand = [&](const int8_t* p, int64_t ld, int64_t rows) {
+    return ld % 2 == 0 && operand_ok(p, ld / 2, rows, a.K, false);
+  };
+  if (!operand(d->a, d->lda, d->m) || !d->a_scale) return false;
+  bool vec = true;
+  int64_t beg = 0;
+  for (int i = 0; i < (gate_up ? 2 : d->pieces); ++i) {
+    const int64_t end = gate_up || d->pieces == 1 ? d->n : d->end[i], len = end - (gate_up ? 0 : beg);
+    if (len < 1 || end > d->n || (!gate_up && i + 1 == d->pieces && end != d->n)) return false;
+    if (!operand(d->b[i], d->ldb[i], len) || !d->b_scale[i] || (gate_up && d->ldb[i] != d->ldb[0])) return false;
+    const int ic = gate_up ? 0 : i;
+    if (!d->c[ic] || d->ldc[ic] < len) return false;
+    vec = vec && len % 8 == 0 && al16(d->c[ic]) && d->ldc[ic] % 8 == 0;
+    a.len[i] = len;
+    a.b.p[i] = (const u16*)d->b[i];
+    a.b.ld[i] = d->ldb[i] / 2;
+    a.cscale[i] = d->b_scale[i];
+    a.c[ic] = d->c[ic];
+    a.ldc[ic] = d->ldc[ic];
+    beg = end;
+  }
+  for (int i = 0; i < 3; ++i) {  // one A operand, whatever the piece
+    a.a.p[i] = (const u16*)d->a;
+    a.a.ld[i] = d->lda / 2;
+  }
+  a.rscale = d->a_scale;
+  if (residual) {
+    if (!d->res || d->ldres < d->n) return false;
+    a.res = (const u16*)d->res;
+    a.ldres = d->ldres;
+    vec = vec && al16(d->res) && d->ldres % 8 == 0;
+  }
+  if (gate_up && !vec) return false;
+  a.vec = vec;
+  c.can_split = !gate_up && vec;
+  c.combine = 4.5;
+  return tile_rows(a, 32) * tile_cols(a, 64) < (1ll << 28);
+}
+
 // One launch of a call: its arguments (the rows it forms are rows of its own operands), tiles and grid.
 struct Launch {
   Args a;
@@ -280,6 +369,7 @@ void set_grid(Launch& l) {
 }
 
 int launch(const Call& c, const Launch& l, int dtype, hipStream_t s) {
+  if (c.q8) return q3gemm::launch_tile_q8(dtype, l.p.cfg, c.epi, l.a, s);
   if (c.at) return q3gemm::launch_tile_tn(dtype, l.p.cfg, l.a, s);
   if (c.bt) return q3gemm::launch_tile_nn(dtype, l.p.cfg, c.epi, l.a, s);
   return q3gemm::launch_tile_nt(dtype, l.p.cfg, c.epi, l.a, s);
@@ -319,6 +409,7 @@ void drop_rows(Args& a, bool at, int64_t rows) {
     if (a.c[i]) a.c[i] = (u16*)a.c[i] + rows * a.ldc[a.axis == 2 ? i : 0];
   const int64_t out = rows * a.ldc[0], in = rows * a.ldgu;
   if (a.res) a.res += rows * a.ldres;
+  if (a.rscale) a.rscale += rows;
   if (a.g) a.g += out;
   if (a.u) a.u += out;
   if (a.gin) a.gin += in;
@@ -396,6 +487,37 @@ int q3_gemm(const q3_gemm_desc* d, void* workspace, size_t workspace_bytes, hipS
     if (rc != 0) return rc;
   }
   return norm ? q3_rmsnorm_fwd(d->dtype, d->c[0], d->norm_w, d->y, d->m, d->n, d->eps, stream) : 0;
+}
+
+size_t q3_gemm_int8_workspace_bytes(const q3_int8_gemm_desc* d) {
+  Call c;
+  if (!parse_int8(d, c)) return 0;
+  const Plan p = plan_for(c.a, false, false, c.can_split, c.combine);
+  return p.splits > 1 ? (size_t)p.splits * (size_t)c.a.M * (size_t)c.a.N * sizeof(int) : 0;
+}
+
+int q3_gemm_int8(const q3_int8_gemm_desc* d, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  Call c;
+  Q3_REQUIRE(parse_int8(d, c));
+  Launch l[2];
+  const int n = launches(c, l);
+  if (l[0].p.splits > 1) {
+    Args& a = l[0].a;
+    Q3_REQUIRE(workspace && al16(workspace) &&
+               workspace_bytes >= (size_t)a.splits * (size_t)a.M * (size_t)a.N * sizeof(int));
+    a.part = (float*)workspace;
+    const int rc = launch(c, l[0], d->dtype, stream);
+    if (rc != 0) return rc;
+    const unsigned g = (unsigned)cdiv(a.M * (a.N / 8), 256);
+    if (d->dtype == Q3_BF16) combine_q8_kernel<BF16><<<g, 256, 0, stream>>>(a);
+    else combine_q8_kernel<F16><<<g, 256, 0, stream>>>(a);
+    return (int)hipGetLastError();
+  }
+  for (int i = 0; i < n; ++i) {
+    const int rc = launch(c, l[i], d->dtype, stream);
+    if (rc != 0) return rc;
+  }
+  return 0;
 }
 
 // LM-head logits A B^T, stored, with their cross-entropy statistics (q3hip.h): 256 x 256 tiles, 128 x 256 when

@@ -35,6 +35,13 @@ class GemmDesc(ctypes.Structure):
                 ("ldgu", _i64), ("eps", _f32)]
 
 
+class Int8GemmDesc(ctypes.Structure):
+    """``q3_int8_gemm_desc``."""
+    _fields_ = [*((n, _i32) for n in ("dtype", "pieces", "epilogue")), ("m", _i64), ("n", _i64), ("k", _i64),
+                ("end", _i64 * 3), ("a", _p), ("lda", _i64), ("a_scale", _p), ("b", _p * 3), ("ldb", _i64 * 3),
+                ("b_scale", _p * 3), ("c", _p * 3), ("ldc", _i64 * 3), ("res", _p), ("ldres", _i64)]
+
+
 # name -> (restype, argtypes); mirrors include/q3hip.h one-to-one.
 SIGNATURES: dict[str, tuple] = {
     "q3_error_string": (ctypes.c_char_p, [_i32]),
@@ -115,6 +122,16 @@ SIGNATURES: dict[str, tuple] = {
     "q3_gemm_workspace_bytes": (_sz, [_p]),
     "q3_gemm_plan": (_i32, [_p, _p]),
     "q3_gemm": (_i32, [_p, _p, _sz, _p]),
+    "q3_quant_rows": (_i32, [_i32, _p, _i64, _p, _p, _i64, _i64, _p]),
+    "q3_rmsnorm_quant": (_i32, [_i32, _p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _i64, _f32, _p]),
+    "q3_gemm_int8_workspace_bytes": (_sz, [_p]),
+    "q3_gemm_int8": (_i32, [_p, _p, _sz, _p]),
+    "q3_kv8_append": (_i32, [_i32, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64,
+                             _i64, _i64, _i64, _p, _p]),
+    "q3_kv8_read": (_i32, [_i32, _i32, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p]),
+    "q3_kv8_attention_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64]),
+    "q3_kv8_attention": (_i32, [_i32, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _p, _sz, _i64,
+                                _i64, _i64, _i64, _i64, _i64, _i64, _p, _f32, _p]),
     "q3_gemm_strided": (_i32, [_i32, _i32, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _f32, _i32,
                                 _p]),
 }

@@ -1,0 +1,329 @@
+"""Serving in 8 bits: rows, RMSNorm, matrix products and a key/value cache in int8 with fp32 scales, and attention over
+that cache.  Forward only (inputs that require a gradient are refused); bf16 or fp16 around the codes.
+
+One rule for every group of values with one scale (a token's row, a weight's output channel, 64 cached positions of a
+head): with M the largest magnitude, a value is held as the integer nearest to 127 a / M (ties to even) and the scale is
+M / 127.  A group that holds an infinity or a NaN gets the scale NaN, and what is formed from it is NaN.
+
+``TritonQwen3Inference.quantize_weights`` and ``new_cache(..., dtype=torch.int8)`` run the model on these.  The reference
+serves in 16 bits only; nothing here has a counterpart in it.
+"""
+import ctypes
+from dataclasses import dataclass
+
+import torch
+
+from .. import _hip as H
+
+KV_BLOCK = 64     # cached positions that share a scale
+MAX_ROW = 32768   # values that quantize_rows / rms_norm take per row
+MAX_K = 1 << 17   # int32 sums of products of 8-bit codes stay exact below
+
+_FLOATS = (torch.bfloat16, torch.float16)
+
+
+def _forward_only(*tensors):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
+        raise ValueError('int8 operators are forward only: run them under torch.no_grad or detach the inputs')
+
+
+def _require_float(t, what):
+    if t.dtype not in _FLOATS:
+        raise TypeError(f'{what}: bfloat16 or float16 required, not {t.dtype}')
+
+
+def _rows(x, what):
+    """x [..., K] as (rows, row stride): whole rows of 16-byte chunks at one stride."""
+    k = x.shape[-1] if x.ndim else 0
+    if x.ndim < 1 or x.numel() == 0:
+        raise ValueError(f'{what}: nonempty [..., K] required')
+    if x.stride(-1) != 1 and k > 1 or not (x.is_contiguous() or x.ndim == 2):
+        raise ValueError(f'{what}: contiguous, or a matrix of contiguous rows; no hidden layout copy')
+    rows = x.numel() // k
+    ld = x.stride(0) if x.ndim == 2 and rows > 1 else k
+    if ld < k or (ld * x.element_size()) % 16 or x.data_ptr() % 16:
+        raise ValueError(f'{what}: rows must start on 16 bytes and not overlap')
+    return rows, ld
+
+
+# ---------------------------------------------------------------- rows
+def _check_rows(x):
+    H.require_device(x)
+    _require_float(x, 'rows')
+    rows, ld = _rows(x, 'rows')
+    k = x.shape[-1]
+    if k % 16 or k > MAX_ROW:
+        raise ValueError(f'rows: a row length that is a multiple of 16 and at most {MAX_ROW} required, not {k}')
+    return rows, ld, k
+
+
+def quantize_rows(x):
+    """x [..., K] -> (codes int8 [..., K], scales fp32 [...]): each row on its own."""
+    _forward_only(x)
+    rows, ld, k = _check_rows(x)
+    q = torch.empty(x.shape, device=x.device, dtype=torch.int8)
+    scale = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
+    with torch.cuda.device(x.device):
+        H.call("q3_quant_rows", H.code(x.dtype), x.data_ptr(), ld, q.data_ptr(), scale.data_ptr(), rows, k, H.stream())
+    return q, scale
+
+
+def rms_norm(x, weight, eps, *, residual=None):
+    """RMSNorm of x [..., K] in 8 bits: (codes, scales), and with ``residual`` (codes, scales, total) where
+    total = x + residual, rounded once, is what the norm is taken of."""
+    _forward_only(x, weight, residual)
+    rows, ld, k = _check_rows(x)
+    H.require_device(x, weight)
+    if weight.shape != (k,) or weight.dtype != x.dtype or not weight.is_contiguous() or weight.data_ptr() % 16:
+        raise ValueError(f'a contiguous 16-byte aligned weight of {k} {x.dtype} values required')
+    if not float(eps) >= 0.0:
+        raise ValueError('a nonnegative eps required')
+    ldr, total = 0, None
+    if residual is not None:
+        H.require_device(x, residual)
+        if residual.shape != x.shape or residual.dtype != x.dtype:
+            raise ValueError('a residual of the shape and dtype of x required')
+        ldr = _rows(residual, 'residual')[1]
+        total = torch.empty(x.shape, device=x.device, dtype=x.dtype)
+    q = torch.empty(x.shape, device=x.device, dtype=torch.int8)
+    scale = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
+    with torch.cuda.device(x.device):
+        H.call("q3_rmsnorm_quant", H.code(x.dtype), x.data_ptr(), ld, None if residual is None else residual.data_ptr(),
+               ldr, weight.data_ptr(), q.data_ptr(), scale.data_ptr(), None if total is None else total.data_ptr(), rows, k,
+               float(eps), H.stream())
+    return (q, scale) if residual is None else (q, scale, total)
+
+
+# ---------------------------------------------------------------- products
+def _check_codes(q, scale):
+    H.require_device(q, scale)
+    if q.dtype != torch.int8:
+        raise TypeError(f'int8 codes required, not {q.dtype}')
+    rows, ld = _rows(q, 'codes')
+    if scale.dtype != torch.float32 or scale.shape != q.shape[:-1] or not scale.is_contiguous():
+        raise ValueError('contiguous float32 scales, one per row of codes, required')
+    k = q.shape[-1]
+    if k % 16 or k >= MAX_K:
+        raise ValueError(f'a row length that is a multiple of 16 and below {MAX_K} required, not {k}')
+    return rows, ld, k
+
+
+def _check_weight(q, w, ws):
+    H.require_device(q, w, ws)
+    if w.dtype != torch.int8 or w.ndim != 2 or w.shape[1] != q.shape[-1]:
+        raise ValueError('an int8 weight [N, K] of the codes\' K required')
+    if ws.dtype != torch.float32 or ws.shape != (w.shape[0],) or not ws.is_contiguous():
+        raise ValueError('contiguous float32 scales, one per weight row, required')
+    ld = _rows(w, 'weight')[1]
+    if ld >= 1 << 23:
+        raise ValueError('weight rows are too far apart')
+    return ld
+
+
+def _product(q, scale, weights, outs, epilogue, dtype, residual=None):
+    if dtype not in _FLOATS:
+        raise TypeError(f'a bfloat16 or float16 result required, not {dtype}')
+    _forward_only(residual)
+    rows, lda, k = _check_codes(q, scale)
+    d = H.Int8GemmDesc()
+    d.dtype, d.epilogue, d.m, d.k = H.code(dtype), epilogue, rows, k
+    d.a, d.lda, d.a_scale = q.data_ptr(), lda, scale.data_ptr()
+    if lda >= 1 << 23:
+        raise ValueError('rows of codes are too far apart')
+    end = 0
+    for i, (w, ws) in enumerate(weights):
+        d.b[i], d.ldb[i], d.b_scale[i] = w.data_ptr(), _check_weight(q, w, ws), ws.data_ptr()
+        end += w.shape[0]
+        d.end[i] = end
+    d.pieces = len(outs)
+    d.n = end if epilogue != H.GEMM_GATE_UP else weights[0][0].shape[0]
+    for i, y in enumerate(outs):
+        d.c[i], d.ldc[i] = y.data_ptr(), y.shape[-1]
+    if residual is not None:
+        H.require_device(q, residual)
+        if residual.shape != outs[0].shape or residual.dtype != dtype or not residual.is_contiguous():
+            raise ValueError('a contiguous residual of the result\'s shape and dtype required')
+        d.res, d.ldres = residual.data_ptr(), residual.shape[-1]
+    ref = ctypes.addressof(d)
+    with torch.cuda.device(q.device):
+        nbytes = H.query("q3_gemm_int8_workspace_bytes", ref)
+        ws = H.workspace(nbytes, q.device) if nbytes else None
+        H.call("q3_gemm_int8", ref, None if ws is None else ws.data_ptr(), nbytes, H.stream())
+
+
+def _out(q, n, dtype):
+    return torch.empty((*q.shape[:-1], n), device=q.device, dtype=dtype)
+
+
+def linear(q, scale, weight, weight_scale, *, dtype=torch.bfloat16, residual=None):
+    """(codes [..., K], scales [...]) x (weight codes [N, K], scales [N]) -> [..., N] in ``dtype``: exact integer sums,
+    scaled in fp32, plus ``residual`` [..., N], rounded once."""
+    y = _out(q, weight.shape[0], dtype)
+    _product(q, scale, [(weight, weight_scale)], [y], H.GEMM_PLAIN if residual is None else H.GEMM_RESIDUAL, dtype, residual)
+    return y
+
+
+def projections(q, scale, weights, *, dtype=torch.bfloat16):
+    """``linear`` by up to three weights [(codes, scales), ...] of one input in one launch (Q, K and V)."""
+    if not 1 <= len(weights) <= 3:
+        raise ValueError('one to three weights required')
+    outs = [_out(q, w.shape[0], dtype) for w, _ in weights]
+    _product(q, scale, list(weights), outs, H.GEMM_PLAIN, dtype)
+    return outs
+
+
+def gate_up_swiglu(q, scale, gate, gate_scale, up, up_scale, *, dtype=torch.bfloat16):
+    """silu(x Wg^T) * (x Wu^T) of codes x and weights [N, K] (N a multiple of 8), formed in fp32 and rounded once."""
+    if gate.shape != up.shape or gate.stride() != up.stride():
+        raise ValueError('gate and up weights of one shape and layout required')
+    if gate.shape[0] % 8:
+        raise ValueError('a number of gate/up channels that is a multiple of 8 required')
+    y = _out(q, gate.shape[0], dtype)
+    _product(q, scale, [(gate, gate_scale), (up, up_scale)], [y], H.GEMM_GATE_UP, dtype)
+    return y
+
+
+# ---------------------------------------------------------------- cache
+@dataclass
+class LayerCache:
+    """One layer's keys and values in 8 bits, head dim 128, capacity C in blocks of 64 positions (Cb = ceil(C / 64)):
+
+    ``k`` int8 [B, Hkv, 64 Cb, 128]; ``v`` int8 [B, Hkv, Cb, 128, 64], transposed within a block; ``k_scale`` and
+    ``v_scale`` fp32 [B, Hkv, Cb]; ``k_tail`` [B, Hkv, 64, 128] and ``v_tail`` [B, Hkv, 128, 64]: the positions of the last,
+    unfinished block in 16 bits, at slot position % 64.
+
+    A block is quantised once, from its 16-bit values, when its last position is appended; so what the cache holds does
+    not depend on how the tokens were cut into chunks.  Positions are appended in order: the cache cannot be wound back
+    into a block that is already quantised (start again from 0)."""
+    k: torch.Tensor
+    v: torch.Tensor
+    k_scale: torch.Tensor
+    v_scale: torch.Tensor
+    k_tail: torch.Tensor
+    v_tail: torch.Tensor
+
+    @classmethod
+    def empty(cls, batch, heads, capacity, *, device, dtype=torch.bfloat16, head_dim=128):
+        """Buffers for ``capacity`` positions (their contents are whatever the memory held: nothing reads a position that
+        was not appended)."""
+        if head_dim != 128:
+            raise ValueError('head_dim 128 required')
+        if min(batch, heads, capacity) < 1:
+            raise ValueError('a batch, heads and capacity of at least 1 required')
+        if dtype not in _FLOATS:
+            raise TypeError(f'bfloat16 or float16 required, not {dtype}')
+        cb = -(-capacity // KV_BLOCK)
+        i8, f32 = dict(device=device, dtype=torch.int8), dict(device=device, dtype=torch.float32)
+        return cls(torch.empty((batch, heads, cb * KV_BLOCK, 128), **i8), torch.empty((batch, heads, cb, 128, KV_BLOCK), **i8),
+                   torch.empty((batch, heads, cb), **f32), torch.empty((batch, heads, cb), **f32),
+                   torch.empty((batch, heads, KV_BLOCK, 128), device=device, dtype=dtype),
+                   torch.empty((batch, heads, 128, KV_BLOCK), device=device, dtype=dtype))
+
+    @property
+    def capacity(self):
+        return self.k.shape[2]
+
+    @property
+    def nbytes(self):
+        return sum(t.numel() * t.element_size()
+                   for t in (self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail))
+
+    def check(self):
+        """Raise unless the buffers are what the kernels take; returns (batch, heads)."""
+        tensors = (self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail)
+        H.require_device(*tensors)
+        b, h, c, d = self.k.shape if self.k.ndim == 4 else (0, 0, 0, 0)
+        cb = c // KV_BLOCK
+        if d != 128 or c % KV_BLOCK or min(b, h, c) < 1 or self.v.shape != (b, h, cb, d, KV_BLOCK) or \
+                self.k_scale.shape != (b, h, cb) or self.v_scale.shape != (b, h, cb) or \
+                self.k_tail.shape != (b, h, KV_BLOCK, d) or self.v_tail.shape != (b, h, d, KV_BLOCK):
+            raise ValueError('cache buffers of matching shapes (head dim 128, blocks of 64) required')
+        if self.k.dtype != torch.int8 or self.v.dtype != torch.int8 or self.k_scale.dtype != torch.float32 or \
+                self.v_scale.dtype != torch.float32 or self.k_tail.dtype not in _FLOATS or \
+                self.v_tail.dtype != self.k_tail.dtype:
+            raise TypeError('int8 codes, float32 scales and 16-bit tails of one dtype required')
+        if any(not t.is_contiguous() for t in tensors) or any(t.data_ptr() % 16 for t in (self.k, self.v, self.k_tail,
+                                                                                          self.v_tail)):
+            raise ValueError('contiguous, 16-byte aligned cache buffers required')
+        return b, h
+
+    def pointers(self):
+        return (self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
+                self.k_tail.data_ptr(), self.v_tail.data_ptr())
+
+
+def _check_heads(t, cache, what):
+    """t [B, S, heads, 128] of the cache's batch and dtype, every head's row 16 bytes of its own; returns its strides."""
+    b, _ = cache.check()
+    H.require_device(cache.k, t)
+    if t.ndim != 4 or t.shape[0] != b or t.shape[3] != 128 or t.numel() == 0:
+        raise ValueError(f'{what}: [B, S, heads, 128] of the cache\'s batch required')
+    if t.dtype != cache.k_tail.dtype:
+        raise TypeError(f'{what}: {cache.k_tail.dtype} required, not {t.dtype}')
+    strides = [s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape)]   # a lone index's stride is never used
+    if t.stride(3) != 1 or any(s % 8 or s < 0 for s in strides) or t.data_ptr() % 16:
+        raise ValueError(f'{what}: contiguous, 16-byte aligned heads required')
+    return strides
+
+
+def _check_span(start, s, cache, start_dev):
+    if start_dev is not None:
+        if s != 1:
+            raise ValueError('device-resident positions are for single-token decode steps')
+        H.require_device(cache.k, start_dev)
+        if start_dev.dtype != torch.int64 or start_dev.numel() != 1:
+            raise ValueError('a device position is one int64')
+        return 0
+    if type(start) is not int or start < 0 or start + s > cache.capacity:
+        raise ValueError(f'positions {start} .. {start} + {s} - 1 do not fit a cache of {cache.capacity}')
+    return start
+
+
+def append(k, v, cache, start, start_dev=None):
+    """Append k, v [B, S, Hkv, 128] to a ``LayerCache`` that holds the positions before ``start`` (with ``start_dev``, one
+    token at that device int64, read when the kernel runs; positions outside the capacity are skipped)."""
+    _forward_only(k, v)
+    ks, vs = _check_heads(k, cache, 'keys'), _check_heads(v, cache, 'values')
+    b, s, h, d = k.shape
+    if v.shape != k.shape or h != cache.k.shape[1]:
+        raise ValueError('keys and values of one shape, with the cache\'s heads, required')
+    start = _check_span(start, s, cache, start_dev)
+    with torch.cuda.device(k.device):
+        H.call("q3_kv8_append", H.code(k.dtype), k.data_ptr(), *ks, v.data_ptr(), *vs, *cache.pointers(), b, s, h, d,
+               cache.capacity, start, None if start_dev is None else start_dev.data_ptr(), H.stream())
+
+
+def read(cache, length, *, dtype=None):
+    """The first ``length`` positions back as k, v [B, Hkv, length, 128] in ``dtype`` (the tail's by default)."""
+    b, h = cache.check()
+    if type(length) is not int or not 1 <= length <= cache.capacity:
+        raise ValueError(f'length must be an int in [1, {cache.capacity}]')
+    dtype = cache.k_tail.dtype if dtype is None else dtype
+    out = [torch.empty((b, h, length, 128), device=cache.k.device, dtype=dtype) for _ in range(2)]
+    with torch.cuda.device(cache.k.device):
+        H.call("q3_kv8_read", H.code(cache.k_tail.dtype), H.code(dtype), *cache.pointers(), out[0].data_ptr(),
+               out[1].data_ptr(), b, h, 128, cache.capacity, length, H.stream())
+    return out[0], out[1]
+
+
+def attention(q, cache, start, start_dev=None, *, scale=None):
+    """q [B, S, Hq, 128] at positions start .. start + S - 1, causal, against the cache's positions up to each query's own
+    (appended before); returns [B, S, Hq, 128].  With ``start_dev`` (S = 1) the position is read on the device and the
+    launch spans the whole capacity, so a captured step replays at any position."""
+    _forward_only(q)
+    qs = _check_heads(q, cache, 'queries')
+    b, s, hq, d = q.shape
+    hkv = cache.k.shape[1]
+    if hq % hkv:
+        raise ValueError('query heads must be a multiple of key/value heads')
+    start = _check_span(start, s, cache, start_dev)
+    scale = d ** -0.5 if scale is None else float(scale)
+    out = torch.empty((b, s, hq, d), device=q.device, dtype=q.dtype)
+    with torch.cuda.device(q.device):
+        nbytes = H.query("q3_kv8_attention_workspace_bytes", b, s, hq, hkv,
+                         start + s if start_dev is None else cache.capacity)
+        ws = H.workspace(nbytes, q.device) if nbytes else None
+        H.call("q3_kv8_attention", H.code(q.dtype), q.data_ptr(), *qs, *cache.pointers(), out.data_ptr(), *out.stride()[:3],
+               None if ws is None else ws.data_ptr(), nbytes, b, s, hq, hkv, d, cache.capacity, start,
+               None if start_dev is None else start_dev.data_ptr(), scale, H.stream())
+    return out

@@ -1,0 +1,166 @@
+"""The 8-bit serving entry points on the host: what they refuse before any launch, their workspace sizes, and the rule by
+which a value gets its code, in the kernels' own arithmetic against exact rationals."""
+import ctypes
+from fractions import Fraction
+
+import numpy as np
+import pytest
+import torch
+
+from qwen3_triton import _hip as H
+from qwen3_triton.inference import int8 as I8
+
+INVALID = 100000
+P = 1 << 20   # a 16-byte aligned address that no refused call touches
+
+
+def test_quantise_rule_matches_exact_rationals():
+    """a (127 / M) in fp32, nearest, and the exact decision within 1e-4 of a half: the same integer as the rational 127 a / M
+    rounded to nearest even, for 16-bit a and for products of two."""
+    rng = np.random.default_rng(0)
+    f32 = np.float32
+
+    def code(a, m):
+        t = f32(a) * (f32(127) / f32(m))
+        q = np.rint(t)
+        if abs(f32(t - q)) > f32(0.4999):
+            u, k = 127.0 * float(a), np.floor(float(t))
+            mid = (k + 0.5) * float(m)
+            q = k if u < mid else k + 1 if u > mid else 2 * np.rint(0.5 * k + 0.25)
+        return int(q)
+
+    for _ in range(4000):
+        bits = rng.choice([8, 11, 22])
+        m = f32(rng.integers(1 << (bits - 1), 1 << bits)) * f32(2.0) ** int(rng.integers(-30, 30))
+        n = int(rng.integers(-127, 127))
+        near = float(m) * (n + 0.5) / 127   # next to a border
+        a = f32(np.sign(near)) * min(f32(abs(near)), m) if rng.random() < 0.7 else f32(rng.uniform(-1, 1)) * m
+        scale = 2.0 ** np.floor(np.log2(abs(float(a)) + 1e-300))
+        a = f32(np.rint(float(a) / scale * 2 ** (bits - 1)) / 2 ** (bits - 1) * scale)
+        if abs(a) > m:
+            continue
+        assert code(a, m) == round(Fraction(127) * Fraction(float(a)) / Fraction(float(m))), (a, m)
+
+
+def test_rows_refusals():
+    lib = H.load()
+    good = dict(dtype=2, x=P, ldx=64, q=P, s=P, rows=4, h=64)
+
+    def quant(**kw):
+        a = {**good, **kw}
+        return lib.q3_quant_rows(a['dtype'], a['x'], a['ldx'], a['q'], a['s'], a['rows'], a['h'], None)
+    for bad in (dict(dtype=0), dict(dtype=3), dict(x=None), dict(q=None), dict(s=None), dict(rows=0), dict(rows=1 << 31), dict(h=0),
+                dict(h=8), dict(h=40, ldx=40), dict(h=32784, ldx=32784), dict(h=1 << 40, ldx=1 << 40), dict(ldx=48), dict(ldx=68),
+                dict(x=P + 2), dict(q=P + 4), dict(s=P + 2)):
+        assert quant(**bad) == INVALID, bad
+
+    def norm(**kw):
+        a = {**good, 'w': P, 'res': P, 'ldr': 64, 'total': P, 'eps': 1e-6, **kw}
+        return lib.q3_rmsnorm_quant(a['dtype'], a['x'], a['ldx'], a['res'], a['ldr'], a['w'], a['q'], a['s'], a['total'],
+                                    a['rows'], a['h'], a['eps'], None)
+    for bad in (dict(dtype=0), dict(w=None), dict(w=P + 2), dict(res=None), dict(total=None), dict(ldr=32), dict(ldr=68),
+                dict(res=P + 2), dict(total=P + 8), dict(eps=-1.0), dict(eps=float('nan')), dict(h=24), dict(rows=0)):
+        assert norm(**bad) == INVALID, bad
+
+
+def gemm_desc(**kw):
+    d = H.Int8GemmDesc()
+    d.dtype, d.pieces, d.epilogue, d.m, d.n, d.k = 2, 1, 0, 4, 64, 128
+    d.a, d.lda, d.a_scale = P, 128, P
+    for i in range(3):
+        d.end[i] = (i + 1) * 64
+        d.b[i], d.ldb[i], d.b_scale[i], d.c[i], d.ldc[i] = P, 128, P, P, 64
+    for k, v in kw.items():
+        if isinstance(v, tuple):
+            getattr(d, k)[v[0]] = v[1]
+        else:
+            setattr(d, k, v)
+    return d
+
+
+@pytest.mark.parametrize("bad", [dict(dtype=0), dict(m=0), dict(n=0), dict(k=0), dict(k=120), dict(k=1 << 17), dict(m=1 << 31), dict(n=1 << 30),
+                                 dict(pieces=0), dict(pieces=4), dict(pieces=2, epilogue=1, n=128), dict(pieces=2, epilogue=3, n=128),
+                                 dict(epilogue=2), dict(epilogue=4), dict(epilogue=9), dict(a=None), dict(a=P + 8), dict(a_scale=None), dict(lda=120),
+                                 dict(lda=136), dict(lda=1 << 23), dict(b=(0, None)), dict(b_scale=(0, None)), dict(ldb=(0, 64)), dict(c=(0, None)),
+                                 dict(ldc=(0, 63)), dict(epilogue=1), dict(epilogue=1, res=P, ldres=63), dict(epilogue=3, n=60),
+                                 dict(epilogue=3, b=(1, None)), dict(epilogue=3, ldb=(1, 256)), dict(epilogue=3, c=(0, P + 2)),
+                                 dict(pieces=2, n=130), dict(pieces=2, n=128, end=(0, 0)), dict(pieces=2, n=128, end=(0, 128)),
+                                 dict(pieces=3, n=128), dict(pieces=2, n=128, ldc=(1, 63))])
+def test_product_refusals(bad):
+    d = gemm_desc(**bad)
+    assert H.load().q3_gemm_int8(ctypes.addressof(d), P, 1 << 40, None) == INVALID
+    assert H.load().q3_gemm_int8_workspace_bytes(ctypes.addressof(d)) == 0
+    assert H.load().q3_gemm_int8(None, None, 0, None) == INVALID
+
+
+def test_product_refuses_a_short_workspace():
+    d = gemm_desc(m=40, n=4096, k=12288, lda=12288, ldb=(0, 12288), ldc=(0, 4096))
+    need = H.load().q3_gemm_int8_workspace_bytes(ctypes.addressof(d))
+    assert need > 0
+    assert H.load().q3_gemm_int8(ctypes.addressof(d), P, need - 1, None) == INVALID
+    assert H.load().q3_gemm_int8(ctypes.addressof(d), None, need, None) == INVALID
+
+
+def test_cache_refusals():
+    lib = H.load()
+    good = dict(dtype=2, k=P, ks=(1024, 256, 128), v=P, vs=(1024, 256, 128), ck=P, cv=P, sk=P, sv=P, tk=P, tv=P, B=1, S=4, Hh=2, d=128,
+                cap=64, start=0, dev=None)
+
+    def append(**kw):
+        a = {**good, **kw}
+        return lib.q3_kv8_append(a['dtype'], a['k'], *a['ks'], a['v'], *a['vs'], a['ck'], a['cv'], a['sk'], a['sv'], a['tk'], a['tv'],
+                                 a['B'], a['S'], a['Hh'], a['d'], a['cap'], a['start'], a['dev'], None)
+    for bad in (dict(dtype=0), dict(k=None), dict(k=P + 2), dict(v=P + 8), dict(ks=(1024, 252, 128)), dict(vs=(1020, 256, 128)),
+                dict(ck=None), dict(cv=P + 1), dict(sk=None), dict(sv=None), dict(tk=None), dict(tv=P + 4), dict(B=0), dict(B=65536),
+                dict(S=0), dict(Hh=0), dict(Hh=65536), dict(d=64), dict(cap=0), dict(cap=1 << 31), dict(start=-1), dict(start=61),
+                dict(start=1 << 62), dict(S=1 << 62), dict(S=2, dev=P)):
+        assert append(**bad) == INVALID, bad
+
+    def read(**kw):
+        a = {**good, 'out': 2, 'length': 10, **kw}
+        return lib.q3_kv8_read(a['dtype'], a['out'], a['ck'], a['cv'], a['sk'], a['sv'], a['tk'], a['tv'], a['k'], a['v'], a['B'],
+                               a['Hh'], a['d'], a['cap'], a['length'], None)
+    for bad in (dict(dtype=0), dict(out=3), dict(out=-1), dict(ck=None), dict(k=None), dict(v=P + 2), dict(length=0), dict(length=65),
+                dict(d=32), dict(B=0)):
+        assert read(**bad) == INVALID, bad
+
+
+def test_attention_refusals():
+    lib = H.load()
+    good = dict(dtype=2, q=P, qs=(1024, 1024, 128), ck=P, cv=P, sk=P, sv=P, tk=P, tv=P, o=P, os=(1024, 1024, 128), ws=P, wsb=1 << 40, B=1, S=1,
+                Hq=8, Hkv=2, d=128, cap=64, start=0, dev=None)
+
+    def attn(**kw):
+        a = {**good, **kw}
+        return lib.q3_kv8_attention(a['dtype'], a['q'], *a['qs'], a['ck'], a['cv'], a['sk'], a['sv'], a['tk'], a['tv'], a['o'], *a['os'],
+                                    a['ws'], a['wsb'], a['B'], a['S'], a['Hq'], a['Hkv'], a['d'], a['cap'], a['start'], a['dev'], 0.1, None)
+    for bad in (dict(dtype=0), dict(q=None), dict(q=P + 2), dict(qs=(1024, 1024, 124)), dict(ck=None), dict(cv=P + 8), dict(sk=None),
+                dict(sv=None), dict(tk=P + 2), dict(tv=None), dict(o=None), dict(o=P + 4), dict(os=(1024, 1022, 128)), dict(B=0), dict(B=65536),
+                dict(S=0), dict(Hq=1), dict(Hq=7), dict(Hkv=0), dict(B=8192, Hkv=8), dict(d=64), dict(cap=0), dict(cap=1 << 31), dict(start=-1),
+                dict(start=64), dict(S=65), dict(start=1 << 62), dict(S=2, dev=P), dict(cap=4096, start=4095, wsb=16), dict(cap=4096, start=4095, ws=None)):
+        assert attn(**bad) == INVALID, bad
+    assert lib.q3_kv8_attention_workspace_bytes(1, 1, 7, 2, 64) == 0 and lib.q3_kv8_attention_workspace_bytes(0, 1, 8, 2, 64) == 0
+    # a captured step's workspace, sized for the capacity, holds every shorter span's
+    sizes = [lib.q3_kv8_attention_workspace_bytes(1, 1, 32, 8, n) for n in range(64, 65536, 64)]
+    assert sizes == sorted(sizes) and sizes[-1] > 0
+
+
+def test_python_refusals_without_a_device():
+    x = torch.zeros(4, 64, dtype=torch.bfloat16)
+    with pytest.raises(ValueError, match='ROCm device'):
+        I8.quantize_rows(x)
+    with pytest.raises(ValueError, match='forward only'):
+        I8.quantize_rows(x.requires_grad_())
+    with torch.no_grad(), pytest.raises(ValueError, match='ROCm device'):
+        I8.quantize_rows(x)
+    c = I8.LayerCache.empty(1, 2, 70, device='cpu')
+    assert c.capacity == 128 and c.v.shape == (1, 2, 2, 128, 64) and c.k_scale.shape == (1, 2, 2)
+    assert c.nbytes == 2 * 2 * 128 * 128 + 2 * 2 * 2 * 4 + 2 * 2 * 64 * 128 * 2
+    with pytest.raises(ValueError):
+        I8.LayerCache.empty(1, 2, 0, device='cpu')
+    with pytest.raises(ValueError):
+        I8.LayerCache.empty(1, 2, 64, device='cpu', head_dim=64)
+    with pytest.raises(TypeError):
+        I8.LayerCache.empty(1, 2, 64, device='cpu', dtype=torch.float32)
+    with pytest.raises(ValueError, match='one to three'):
+        I8.projections(x, x, [])

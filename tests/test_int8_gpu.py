@@ -1,0 +1,463 @@
+"""The 8-bit serving operators (``inference/int8.py``) against their definitions in 64 bits.
+
+Codes are compared for equality: the rule (the integer nearest to 127 a / M, ties to even) leaves nothing to rounding.
+Tolerances elsewhere count roundings: u = eps / 2 of the output type once, 2^-24 per fp32 operation, and for attention the
+rounding of the probabilities (2^-11 in fp16 over 8-bit blocks; the tail's, in the activation type) on sum p |v|.
+"""
+import math
+
+import pytest
+import torch
+
+from _util import seeded
+
+from qwen3_triton.inference import int8 as I8
+
+pytestmark = pytest.mark.gpu
+
+DT = [torch.bfloat16, torch.float16]
+F64 = torch.float64
+
+
+def randn(*shape, gen, dtype=torch.float32, scale=1.0):
+    return (torch.randn(*shape, generator=gen) * scale).to(dtype)
+
+
+def codes64(a):
+    """a [..., n] in 64 bits -> (codes, M): one scale per row of the last axis."""
+    m = a.abs().amax(-1)
+    return torch.where(m[..., None] > 0, (127.0 * a / m[..., None]).round(), torch.zeros_like(a)), m
+
+
+def close(y, ref, tol):
+    bad = (y.double().cpu() - ref).abs() > tol
+    assert torch.isfinite(y).all() and not bool(bad.any()), \
+        (int(bad.sum()), float(((y.double().cpu() - ref).abs() - tol).max()))
+
+
+# ---------------------------------------------------------------- rows
+def row_cases(h, dtype, gen):
+    """Rows where the rule can go wrong: ordinary, outliers, zeros, ties, tiny and huge magnitudes."""
+    x = randn(9, h, gen=gen)
+    x[1, ::7] *= 40
+    x[2] = 0
+    x[3] = torch.arange(h) % 128 - 0.5      # M 126.5 or 127 with ties
+    x[3, 0] = 127
+    x[4] = (torch.arange(h) % 255 - 127) / 2  # ties at M = 63.5: 127 x / M = 2 x
+    x[4, 1] = 63.5
+    x[5] *= 2.0 ** (-110 if dtype == torch.bfloat16 else -20)
+    x[6] *= 2.0 ** (120 if dtype == torch.bfloat16 else 12)
+    x[7] = 0
+    x[7, h // 2] = -3.0
+    x[8] = -1.5
+    return x.to(dtype)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("h", [16, 48, 128, 512, 528, 1024, 1040, 2048, 4096, 4112, 8192, 12288, 16400, 32768])
+def test_quantize_rows(h, dtype):
+    x = row_cases(h, dtype, seeded(h))
+    q, s = I8.quantize_rows(x.cuda())
+    want, m = codes64(x.double())
+    assert torch.equal(q.cpu().double(), want)
+    assert torch.equal(s.cpu(), m.float() / 127.0)
+    q1, s1 = I8.quantize_rows(x[1:2].cuda().view(1, 1, h))
+    assert torch.equal(q1.view(1, h), q[1:2]) and torch.equal(s1.view(1), s[1:2]) and q1.shape == (1, 1, h)
+
+
+def test_quantize_rows_strided_and_nonfinite():
+    x = randn(7, 256, gen=seeded(1), dtype=torch.bfloat16).cuda()
+    q, s = I8.quantize_rows(x[:, :128])
+    want, wants = I8.quantize_rows(x[:, :128].contiguous())
+    assert torch.equal(q, want) and torch.equal(s, wants)
+    y = x.clone()
+    y[1, 3], y[2, 200], y[3, 0] = math.nan, math.inf, -math.inf
+    q, s = I8.quantize_rows(y)
+    assert torch.isnan(s[1:4]).all() and torch.isfinite(s[[0, 4, 5, 6]]).all()
+    assert torch.equal(q[[0, 4, 5, 6]], I8.quantize_rows(x)[0][[0, 4, 5, 6]])
+
+
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("rows,h", [(1, 4096), (3, 16), (130, 256), (5, 1040), (2, 2048), (33, 4096), (2, 12288), (1, 32768)])
+def test_rms_norm(rows, h, dtype, residual):
+    gen = seeded(rows + h)
+    x, r = randn(rows, h, gen=gen, dtype=dtype), randn(rows, h, gen=gen, dtype=dtype)
+    x[0, ::5] *= 16
+    w = (1 + 0.1 * torch.randn(h, generator=gen)).to(dtype)
+    out = I8.rms_norm(x.cuda(), w.cuda(), 1e-6, residual=r.cuda() if residual else None)
+    t = (x.float() + r.float()).to(dtype) if residual else x
+    if residual:
+        assert torch.equal(out[2].cpu(), t)
+    want, m = codes64(t.double() * w.double())
+    assert torch.equal(out[0].cpu().double(), want)
+    ref = m / 127.0 / (t.double().square().mean(-1) + 1e-6).sqrt()
+    # the sum of squares over h / 8 ... terms a thread, then butterflies; 1 / h, + eps, the root (2 ulp), two products
+    tol = (math.ceil(math.log2(h)) + 40) * 2.0 ** -24
+    assert float(((out[1].double().cpu() - ref) / ref).abs().max()) <= tol
+
+
+def test_rms_norm_zero_row_eps_and_strided_residual():
+    gen = seeded(5)
+    x, r = randn(3, 512, gen=gen, dtype=torch.bfloat16).cuda(), randn(3, 1024, gen=gen, dtype=torch.bfloat16).cuda()
+    w = torch.ones(512, dtype=torch.bfloat16, device="cuda")
+    x[1] = 0
+    q, s = I8.rms_norm(x, w, 0.0)
+    assert not q[1].any() and torch.isnan(s[1])   # 0 * rsqrt(0), as the 16-bit norm's
+    q, s = I8.rms_norm(x, w, 1e-6)
+    assert not q[1].any() and float(s[1]) == 0.0
+    a = I8.rms_norm(x, w, 1e-6, residual=r[:, :512])
+    b = I8.rms_norm(x, w, 1e-6, residual=r[:, :512].contiguous())
+    assert all(torch.equal(p, o) for p, o in zip(a, b))
+
+
+# ---------------------------------------------------------------- products
+def product_inputs(m, n, k, gen):
+    q = torch.randint(-127, 128, (m, k), generator=gen, dtype=torch.int8)
+    w = torch.randint(-127, 128, (n, k), generator=gen, dtype=torch.int8)
+    s, ws = torch.rand(m, generator=gen) * 1e-2 + 1e-3, torch.rand(n, generator=gen) * 1e-3 + 1e-4
+    return q, s, w, ws
+
+
+def product64(q, s, w, ws):
+    return (q.double() @ w.double().t()) * s.double()[:, None] * ws.double()
+
+
+SIZES = [(1, 1, 16), (1, 64, 128), (2, 100, 48), (3, 7, 1040), (8, 256, 4096), (16, 300, 512), (17, 256, 256), (33, 64, 144),
+         (65, 130, 2048), (100, 1000, 80), (128, 128, 128), (200, 512, 12288), (256, 256, 64), (300, 264, 528), (513, 520, 1024)]
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("residual", [False, True])
+@pytest.mark.parametrize("m,n,k", SIZES)
+def test_linear(m, n, k, residual, dtype):
+    gen = seeded(m * 7 + n * 3 + k)
+    q, s, w, ws = product_inputs(m, n, k, gen)
+    res = randn(m, n, gen=gen, dtype=dtype) if residual else None
+    y = I8.linear(q.cuda(), s.cuda(), w.cuda(), ws.cuda(), dtype=dtype, residual=None if res is None else res.cuda())
+    p = product64(q, s, w, ws)
+    ref = p + (res.double() if residual else 0)
+    # int -> fp32, two scales, the residual's sum: four fp32 roundings; one to the output type
+    close(y, ref, ref.abs() * torch.finfo(dtype).eps / 2 * (1 + 2.0 ** -10) + (p.abs() + ref.abs()) * 4 * 2.0 ** -24 + 1e-7)
+
+
+@pytest.mark.parametrize("m", [1, 5, 16, 40, 300])
+def test_linear_largest_sums(m):
+    """Codes of +-127 (and the -128 that a caller's own weights may hold) at the largest K: sums up to 2^31 - 2^18."""
+    k = (1 << 17) - 16
+    q = torch.full((m, k), -128, dtype=torch.int8)
+    w = torch.full((24, k), -128, dtype=torch.int8)
+    w[1] = 127
+    w[2, ::2] = 127
+    s, ws = torch.full((m,), 2.0 ** -20), torch.full((24,), 2.0 ** -10)
+    y = I8.linear(q.cuda(), s.cuda(), w.cuda(), ws.cuda())
+    ref = product64(q, s, w, ws)
+    close(y, ref, ref.abs() * 2.0 ** -8 * (1 + 2.0 ** -10))
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("m", [1, 7, 16, 31, 130, 515])
+def test_projections_in_one_launch(m, dtype):
+    gen = seeded(m)
+    q, s, _, _ = product_inputs(m, 8, 512, gen)
+    ws = [product_inputs(1, n, 512, gen)[2:] for n in (256, 64, 72)]
+    outs = I8.projections(q.cuda(), s.cuda(), [(w.cuda(), x.cuda()) for w, x in ws], dtype=dtype)
+    for y, (w, x) in zip(outs, ws):
+        assert torch.equal(y, I8.linear(q.cuda(), s.cuda(), w.cuda(), x.cuda(), dtype=dtype))
+        ref = product64(q, s, w, x)
+        close(y, ref, ref.abs() * (torch.finfo(dtype).eps / 2 * (1 + 2.0 ** -10) + 2.0 ** -21) + 1e-7)
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("m,n,k", [(1, 8, 16), (1, 688, 256), (5, 104, 1040), (16, 256, 4096), (17, 72, 128), (128, 512, 512),
+                                   (300, 264, 64), (520, 776, 256)])
+def test_gate_up_swiglu(m, n, k, dtype):
+    gen = seeded(m + n + k)
+    q, s, wg, sg = product_inputs(m, n, k, gen)
+    _, _, wu, su = product_inputs(1, n, k, gen)
+    y = I8.gate_up_swiglu(q.cuda(), s.cuda(), wg.cuda(), sg.cuda(), wu.cuda(), su.cuda(), dtype=dtype)
+    g, u = product64(q, s, wg, sg), product64(q, s, wu, su)
+    ref = g * torch.sigmoid(g) * u
+    # g and u carry 3 fp32 roundings each; silu's relative sensitivity to g is at most 1 + |g|; exp2, rcp and its argument
+    # (1.44 g rounded) a few ulp each, again times |g| in the exponent
+    rel = torch.finfo(dtype).eps / 2 * (1 + 2.0 ** -10) + (12 + 6 * g.abs()) * 2.0 ** -23
+    close(y, ref, ref.abs() * rel + 1e-7)
+
+
+def test_linear_strided_and_last_columns_untouched():
+    gen = seeded(9)
+    q, s, w, ws = product_inputs(20, 40, 256, gen)
+    wide = torch.cat([q, torch.full_like(q, 99)], 1).cuda()
+    y = I8.linear(wide[:, :256], s.cuda(), w.cuda(), ws.cuda())
+    assert torch.equal(y, I8.linear(q.cuda(), s.cuda(), w.cuda(), ws.cuda()))
+    wwide = torch.cat([w, torch.full_like(w, 77)], 1).cuda()
+    assert torch.equal(y, I8.linear(q.cuda(), s.cuda(), wwide[:, :256], ws.cuda()))
+    s2 = s.clone()
+    s2[3] = math.nan
+    z = I8.linear(q.cuda(), s2.cuda(), w.cuda(), ws.cuda())
+    keep = [i for i in range(20) if i != 3]
+    assert torch.isnan(z[3]).all() and torch.equal(z[keep], y[keep])
+
+
+# ---------------------------------------------------------------- cache
+def filled(b, h, total, dtype, gen, *, cuts=(), capacity=None, wide=True):
+    """(cache, k, v): ``total`` positions appended in the chunks that ``cuts`` make, into poisoned buffers."""
+    k, v = randn(b, total, h, 128, gen=gen, dtype=dtype), randn(b, total, h, 128, gen=gen, dtype=dtype)
+    if wide:
+        k[..., ::16] *= 6
+        v[:, ::3] *= 0.1
+    c = poisoned(b, h, capacity or total, dtype)
+    at = 0
+    for end in (*cuts, total):
+        I8.append(k[:, at:end].cuda(), v[:, at:end].cuda(), c, at)
+        at = end
+    return c, k, v
+
+
+def poisoned(b, h, capacity, dtype):
+    c = I8.LayerCache.empty(b, h, capacity, device="cuda", dtype=dtype)
+    c.k.fill_(111), c.v.fill_(-111)
+    for t in (c.k_scale, c.v_scale, c.k_tail, c.v_tail):
+        t.fill_(math.nan)
+    return c
+
+
+def held64(k, v):
+    """What a cache holds of k, v [B, T, H, 128], as values [B, H, T, 128] in 64 bits, and the codes and scales."""
+    full = k.shape[1] // 64
+    out, parts = [], []
+    for x in (k, v):
+        x = x.double().transpose(1, 2)
+        b, h, t, d = x.shape
+        blocks = x[:, :, :full * 64].reshape(b, h, full, 64 * d)
+        q, m = codes64(blocks)
+        scale = (m.float() / 127.0)
+        val = (q * scale.double()[..., None]).view(b, h, full * 64, d)
+        out.append(torch.cat([val, x[:, :, full * 64:]], 2))
+        parts.append((q.view(b, h, full, 64, d), scale))
+    return out, parts
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("total,cuts", [(1, ()), (63, ()), (64, ()), (65, ()), (64, (63,)), (128, (1, 2, 64, 127)), (200, (130,)),
+                                        (257, (63, 64, 65, 191, 192)), (300, (100, 200)), (130, tuple(range(1, 130)))])
+def test_append_and_read(total, cuts, dtype):
+    b, h = 2, 3
+    c, k, v = filled(b, h, total, dtype, seeded(total + len(cuts)), cuts=cuts, capacity=total + 70)
+    values, parts = held64(k, v)
+    full, rest = total // 64, total % 64
+    blocks = c.k_scale.shape[2]
+    (qk, sk), (qv, sv) = parts
+    got_k = c.k.cpu().view(b, h, blocks, 64, 128)
+    assert torch.equal(got_k[:, :, :full].double(), qk) and torch.equal(c.v.cpu()[:, :, :full].transpose(3, 4).double(), qv)
+    assert torch.equal(c.k_scale.cpu()[:, :, :full], sk) and torch.equal(c.v_scale.cpu()[:, :, :full], sv)
+    # behind the last position everything is as it was
+    assert (got_k[:, :, full:] == 111).all() and (c.v.cpu()[:, :, full:] == -111).all()
+    assert torch.isnan(c.k_scale[:, :, full:]).all() and torch.isnan(c.v_scale[:, :, full:]).all()
+    if rest:
+        assert torch.equal(c.k_tail.cpu()[:, :, :rest], k.transpose(1, 2)[:, :, full * 64:])
+        assert torch.equal(c.v_tail.cpu()[..., :rest].transpose(2, 3), v.transpose(1, 2)[:, :, full * 64:])
+    for out in (dtype, torch.float32, torch.bfloat16):
+        rk, rv = I8.read(c, total, dtype=out)
+        for got, want in ((rk, values[0]), (rv, values[1])):
+            u = torch.finfo(out).eps / 2
+            tol = want.abs() * (u * (1 + 2.0 ** -10) + 2.0 ** -23) + (2.0 ** -25 if out == torch.float16 else 0)
+            close(got, want, tol)
+
+
+def test_append_strided_sources_and_nonfinite_block():
+    gen = seeded(3)
+    b, s, h = 2, 130, 2
+    qkv = randn(b, s, 4 * h, 128, gen=gen, dtype=torch.bfloat16).cuda()
+    k, v = qkv[:, :, h:2 * h], qkv[:, :, 2 * h:3 * h]
+    c, d = poisoned(b, h, s, torch.bfloat16), poisoned(b, h, s, torch.bfloat16)
+    I8.append(k, v, c, 0)
+    I8.append(k.contiguous(), v.contiguous(), d, 0)
+    for x, y in zip(I8.read(c, s), I8.read(d, s)):
+        assert torch.equal(x, y)
+    k2 = k.clone()
+    k2[0, 70, 1, 5] = math.inf
+    I8.append(k2, v, c, 0)
+    rk, rv = I8.read(c, s)
+    assert torch.isnan(rk[0, 1, 64:128]).all() and torch.equal(rv, I8.read(d, s)[1])
+    rk[0, 1, 64:128] = I8.read(d, s)[0][0, 1, 64:128]
+    assert torch.equal(rk, I8.read(d, s)[0])
+
+
+# ---------------------------------------------------------------- attention
+def attention64(q, k, v, start, scale, full):
+    """In 64 bits, k, v [B, Hkv, T, 128]: o, sum p |v| over the 8-bit blocks and over the tail, the largest score's sum of
+    magnitudes, and (largest p) * sum |v| over the 8-bit blocks that a query sees."""
+    b, s, hq, d = q.shape
+    hkv, t = k.shape[1], k.shape[2]
+    qf = q.double().transpose(1, 2).reshape(b, hkv, hq // hkv, s, d)
+    z = torch.matmul(qf, k[:, :, None].transpose(3, 4)) * scale
+    zerr = torch.matmul(qf.abs(), k[:, :, None].abs().transpose(3, 4)).amax((-1), keepdim=True) * scale
+    mask = torch.arange(t)[None] > start + torch.arange(s)[:, None]
+    p = torch.softmax(z.masked_fill(mask, -math.inf), -1)
+    shape = lambda x: x.reshape(b, hq, s, d).transpose(1, 2)  # noqa: E731
+    o = torch.matmul(p, v[:, :, None])
+    n = full * 64
+    a8 = torch.matmul(p[..., :n], v[:, :, None, :n].abs())
+    at = torch.matmul(p[..., n:], v[:, :, None, n:].abs())
+    seen = torch.matmul((~mask[:, :n]).double().expand(b, hkv, 1, s, n), v[:, :, None, :n].abs()) * p.amax(-1, keepdim=True)
+    return shape(o), shape(a8), shape(at), zerr.reshape(b, hq, s, 1).transpose(1, 2), shape(seen)
+
+
+def check_attention(o, q, values, start, scale, dtype):
+    full = (start + q.shape[1]) // 64
+    ref, a8, at, zerr, seen = attention64(q, *values, start, scale, full)
+    u = torch.finfo(dtype).eps / 2
+    # a score: 128 products summed in fp32 (any order: 128 * 2^-24 of the sum of magnitudes), two scales, log2(e): in the
+    # exponent, twice (numerator and sum).  p (relative to the largest) in fp16: 2^-11 where normal; below, 2^-25 absolute,
+    # of a value scale that is at least 1 / 16 of O's unit.  The tail's p in the activation type, fp16's again 2^-25 absolute.
+    # Sums over t and the joins: 2^-16.
+    dz = zerr * 136 * 2.0 ** -24 * 2
+    tol = ref.abs() * u * (1 + 2.0 ** -8) + (a8 + at) * (dz + 2.0 ** -16) + a8 * 2.0 ** -11 + at * u + seen * 2.0 ** -21 + 2.0 ** -24
+    close(o, ref, tol)
+
+
+ATT = [(1, 4, 4, 1, 0), (1, 4, 1, 1, 62), (2, 8, 2, 1, 63), (1, 8, 2, 1, 64), (3, 8, 2, 1, 200), (1, 5, 1, 1, 127), (1, 16, 1, 1, 300),
+       (1, 32, 1, 1, 500), (2, 12, 4, 1, 1000), (1, 32, 8, 1, 4095), (1, 4, 2, 2, 63), (1, 8, 2, 4, 60), (1, 8, 2, 5, 1000),
+       (2, 4, 1, 16, 0), (1, 8, 2, 64, 0), (1, 8, 2, 65, 0), (1, 8, 2, 100, 30), (1, 4, 4, 300, 0), (2, 8, 2, 129, 500),
+       (1, 7, 1, 70, 100), (1, 64, 2, 9, 77), (1, 8, 2, 700, 100)]
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("b,hq,hkv,s,start", ATT)
+def test_attention(b, hq, hkv, s, start, dtype):
+    gen = seeded(b + hq + s + start)
+    c, k, v = filled(b, hkv, start + s, dtype, gen, cuts=(start,) if start else (), capacity=start + s + 100)
+    q = randn(b, s, hq, 128, gen=gen, dtype=dtype)
+    o = I8.attention(q.cuda(), c, start)
+    check_attention(o, q, held64(k, v)[0], start, 128 ** -0.5, dtype)
+
+
+@pytest.mark.parametrize("dtype", DT)
+def test_attention_value_scales_far_apart(dtype):
+    """Blocks whose value scales differ by up to 2^40: O changes its units, and a block that dominates is exact whatever the
+    others' scales; strided queries and an own softmax scale."""
+    gen = seeded(8)
+    b, h, t = 1, 2, 64 * 9 + 10
+    k, v = randn(b, t, h, 128, gen=gen, dtype=dtype), randn(b, t, h, 128, gen=gen)
+    exps = [0, -3, 5, -6, 3, -7, 8, 0, 4, 0] if dtype == torch.float16 else [0, -20, 5, -40, 17, -13, 18, -22, 20, 0]
+    for i, e in enumerate(exps):
+        v[:, 64 * i:64 * (i + 1)] *= 2.0 ** e
+    v[:, 64:128, 1] = 0   # a block of zeros: scale 0
+    v = v.to(dtype)
+    c = poisoned(b, h, t, dtype)
+    I8.append(k.cuda(), v.cuda(), c, 0)
+    for s in (1, 3, 40):
+        wide = randn(b, s, 6, 256, gen=gen, dtype=dtype, scale=2.0).cuda()
+        q = wide[:, :, 1:5, 64:192]
+        o = I8.attention(q, c, t - s, scale=0.3)
+        check_attention(o, q.cpu(), held64(k, v)[0], t - s, 0.3, dtype)
+
+
+def test_attention_masked_nonfinite_positions():
+    """A NaN key or value reaches the queries that see its position (or, once quantised, its block), no others."""
+    gen = seeded(4)
+    b, hq, h, s, start = 1, 4, 2, 40, 70   # positions 70 .. 109: the tail holds 64 .. 109
+    c, k, v = filled(b, h, start + s, torch.bfloat16, gen, cuts=(start,))
+    q = randn(b, s, hq, 128, gen=gen, dtype=torch.bfloat16).cuda()
+    want = I8.attention(q, c, start)
+    c.k_tail[0, 0, 100 - 64, 3] = math.nan
+    got = I8.attention(q, c, start)
+    assert torch.equal(got[:, :100 - start], want[:, :100 - start]) and torch.equal(got[:, :, 2:], want[:, :, 2:])
+    assert torch.isnan(got[:, 100 - start:, :2]).all()
+    # whole blocks: two of them, queries in both; a NaN scale of the second leaves the queries of the first alone
+    c, k, v = filled(b, h, 128, torch.bfloat16, gen)
+    q = randn(b, 128, hq, 128, gen=gen, dtype=torch.bfloat16).cuda()
+    want = I8.attention(q, c, 0)
+    for scales in (c.k_scale, c.v_scale):
+        keep = scales.clone()
+        scales[0, 1, 1] = math.nan
+        got = I8.attention(q, c, 0)
+        assert torch.equal(got[:, :64], want[:, :64]) and torch.equal(got[:, :, :2], want[:, :, :2])
+        assert torch.isnan(got[:, 64:, 2:]).all()
+        scales.copy_(keep)
+
+
+def test_device_positions_and_graph_replay():
+    """One captured step (append + attention at a device position) replayed over a block's end against eager calls."""
+    gen = seeded(6)
+    b, hq, h, cap, start = 2, 8, 2, 200, 120
+    c, k, v = filled(b, h, start, torch.bfloat16, gen, capacity=cap)
+    d = I8.LayerCache(*(t.clone() for t in (c.k, c.v, c.k_scale, c.v_scale, c.k_tail, c.v_tail)))
+    pos = torch.tensor([start], device="cuda")
+    new = [[randn(b, 1, n, 128, gen=gen, dtype=torch.bfloat16).cuda() for n in (hq, h, h)] for _ in range(20)]
+    q, kk, vv = (t.clone() for t in new[0])
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=stream):
+        I8.append(kk, vv, c, 0, pos)
+        o = I8.attention(q, c, 0, pos)
+        pos += 1
+    torch.cuda.current_stream().wait_stream(stream)
+    for i, (a, bk, bv) in enumerate(new):
+        q.copy_(a), kk.copy_(bk), vv.copy_(bv)
+        graph.replay()
+        I8.append(bk, bv, d, start + i)
+        eager = I8.attention(a, d, start + i)
+        k, v = torch.cat([k, bk.cpu()], 1), torch.cat([v, bv.cpu()], 1)
+        values = held64(k, v)[0]
+        for got in (o, eager):   # the two split the positions differently
+            check_attention(got, a.cpu(), values, start + i, 128 ** -0.5, torch.bfloat16)
+    n = (start + 20) // 64
+    assert torch.equal(c.k[:, :, :n * 64], d.k[:, :, :n * 64]) and torch.equal(c.v[:, :, :n], d.v[:, :, :n])
+    # positions outside the capacity are skipped
+    bits = lambda: [t.clone() for t in (c.k, c.v, c.k_tail.view(torch.int16), c.v_tail.view(torch.int16))]  # noqa: E731
+    keep = bits()
+    for bad in (c.capacity, c.capacity + 5, -1):
+        I8.append(kk, vv, c, 0, torch.tensor([bad], device="cuda"))
+    assert all(torch.equal(x, y) for x, y in zip(keep, bits()))
+
+
+def test_determinism_and_side_stream():
+    gen = seeded(12)
+    c, k, v = filled(1, 2, 700, torch.bfloat16, gen)
+    q = randn(1, 1, 8, 128, gen=gen, dtype=torch.bfloat16).cuda()
+    want = I8.attention(q, c, 699)
+    x = randn(5, 1024, gen=gen, dtype=torch.bfloat16).cuda()
+    w = I8.quantize_rows(randn(300, 1024, gen=gen, dtype=torch.bfloat16).cuda())
+    y = I8.linear(*I8.quantize_rows(x), *w)
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        for _ in range(3):
+            assert torch.equal(I8.attention(q, c, 699), want)
+            assert torch.equal(I8.linear(*I8.quantize_rows(x), *w), y)
+    torch.cuda.current_stream().wait_stream(stream)
+
+
+# ---------------------------------------------------------------- a layer of them together
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("s", [1, 3, 70])
+def test_chain(s, dtype):
+    """norm -> Q/K/V -> cache -> attention -> output projection with its residual -> norm with its residual -> gate/up, each
+    step against its own definition on the step's own inputs."""
+    gen = seeded(s)
+    hid, hq, h, start = 512, 4, 2, 100
+    x = randn(1, s, hid, gen=gen, dtype=dtype).cuda()
+    nw = (1 + 0.1 * torch.randn(hid, generator=gen)).to(dtype).cuda()
+    ws = [I8.quantize_rows(randn(n, k, gen=gen, dtype=dtype, scale=0.05).cuda())
+          for n, k in ((hq * 128, hid), (h * 128, hid), (h * 128, hid), (hid, hq * 128), (1024, hid), (1024, hid))]
+    c, k0, v0 = filled(1, h, start, dtype, gen, capacity=start + s)
+    a, sa = I8.rms_norm(x, nw, 1e-6)
+    q, k, v = I8.projections(a, sa, ws[:3], dtype=dtype)
+    q, k, v = q.view(1, s, hq, 128), k.view(1, s, h, 128), v.view(1, s, h, 128)
+    I8.append(k, v, c, start)
+    o = I8.attention(q, c, start)
+    values = held64(torch.cat([k0, k.cpu()], 1), torch.cat([v0, v.cpu()], 1))[0]
+    check_attention(o, q.cpu(), values, start, 128 ** -0.5, dtype)
+    b, sb = I8.quantize_rows(o.view(1, s, -1))
+    y = I8.linear(b, sb, *ws[3], dtype=dtype, residual=x)
+    p = product64(b.cpu().view(s, -1), sb.cpu().view(s), *(t.cpu() for t in ws[3]))
+    ref = p + x.double().cpu().view(s, hid)
+    close(y.view(s, hid), ref, ref.abs() * torch.finfo(dtype).eps / 2 * (1 + 2.0 ** -10) + (p.abs() + ref.abs()) * 2.0 ** -22)
+    d, sd, total = I8.rms_norm(y, nw, 1e-6, residual=x)
+    assert torch.equal(total, (y.float() + x.float()).to(dtype))
+    z = I8.gate_up_swiglu(d, sd, *ws[4], *ws[5], dtype=dtype)
+    g, u = (product64(d.cpu().view(s, -1), sd.cpu().view(s), *(t.cpu() for t in w)) for w in ws[4:])
+    ref = g * torch.sigmoid(g) * u
+    close(z.view(s, -1), ref, ref.abs() * (torch.finfo(dtype).eps / 2 * (1 + 2.0 ** -10) + (12 + 6 * g.abs()) * 2.0 ** -23) + 1e-7)
