@@ -32,7 +32,7 @@ struct AttnArgs {
   float *po, *pm, *pl;  // split partials: unnormalised O [rows][D], maximum, sum
   int64_t S, start, capacity;
   const int64_t* start_dev;
-  int Hkv, G, splits;
+  int Hkv, G, splits, max_splits, minper;
   float scale2;  // softmax scale * log2(e)
 };
 
@@ -73,85 +73,150 @@ template <typename T, int RT> struct Rows {
   bf16x8_t q[RT][2][2];  // [row tile][64-dim half c][8-dim half h]: dims 64 c + 16 g + 8 h .. + 7
   f32x4 o[RT][8];        // O^T: dims 16 t + 4 g + e
   float m[RT], l[RT];
-  float unit;            // of O
+  float unit, inv;       // of O: a power of two (0: nothing yet), and 1 / unit
 };
 
-// Scores (already S^T) of a block -> P in fp16 operands, with the running maximum, sum and O rescaled.
-// RAW_V: the block's values are 16-bit numbers, not codes (the tail): vscale is 1.
-template <typename T, int RT, bool MASK>
-Q3_DEV void softmax_step(Rows<T, RT>& w, f32x4 (&s)[RT][4], float c, float vscale, int key0, const int (&qpos)[RT],
-                         i32x4 (&p)[RT][2]) {
-  // units: a value scale within 16 times of the unit leaves it; one far below all others adds nothing worth a new unit
-  float ratio = w.unit > 0.f ? vscale / w.unit : 0.f;
-  if (vscale > 0.f && (w.unit == 0.f || ratio > 16.f || (ratio < 0.0625f && ratio > 0x1p-60f))) {
-    const float unit = __uint_as_float(__float_as_uint(vscale) & 0x7f800000u);  // the power of two below
-    const float u = unit > 0.f ? unit : 0x1p-126f;
-    const float f = w.unit > 0.f ? w.unit / u : 0.f;
+Q3_DEV float xmax4(float x) {  // max over lanes {l, l ^ 16, l ^ 32, l ^ 48}
+  auto a = __builtin_amdgcn_permlane16_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  x = fmaxf(__uint_as_float(a[0]), __uint_as_float(a[1]));
+  auto c = __builtin_amdgcn_permlane32_swap(__float_as_uint(x), __float_as_uint(x), false, false);
+  return fmaxf(__uint_as_float(c[0]), __uint_as_float(c[1]));
+}
+
+// Raw scores of a block (S^T) -> p in s: 2^(c s - m) * factor, with the running maximum and sum, and O rescaled, also by
+// `units`, in one place (every branch that touches O costs its registers twice).  The maximum moves only when a score
+// passes it by more than 8 (p <= 2^8 is as exact in every type that P takes), so O is rarely rescaled.
+// mask: positions key0 + 4 t + e past a row's own are hidden.
+template <typename T, int RT>
+Q3_DEV void softmax_step(Rows<T, RT>& w, f32x4 (&s)[RT][4], float c, float log2_factor, float inv_factor, float units,
+                         bool mask, int key0, const int (&qpos)[RT]) {
+  if (mask) {
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[r][t][e] = key0 + 4 * t + e > qpos[r] ? -INFINITY : s[r][t][e];
+  }
+  float mx[RT];
+  bool up = units != 1.f;
+#pragma unroll
+  for (int r = 0; r < RT; ++r) {
+    float x = -INFINITY;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) x = fmaxf(x, s[r][t][e]);
+    mx[r] = xmax4(x) * c;
+    up = up || mx[r] > w.m[r] + 8.f;
+  }
+  if (__any(up)) {
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      const float m = fmaxf(w.m[r], mx[r]), alpha = __builtin_amdgcn_exp2f(w.m[r] - m), f = alpha * units;
+      w.m[r] = m;
+      w.l[r] *= alpha;
+#pragma unroll
       for (int t = 0; t < 8; ++t) w.o[r][t] *= f;
-    w.unit = u;
-    ratio = vscale / u;
-  } else if (vscale != vscale) {
-    ratio = vscale;
+    }
   }
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
-    float mx = w.m[r];
+    const float off = log2_factor - w.m[r];
+    float sum = 0.f;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        s[r][t][e] *= c;
-        if (MASK && key0 + 4 * t + e > qpos[r]) s[r][t][e] = -INFINITY;
-        mx = fmaxf(mx, s[r][t][e]);
+        s[r][t][e] = __builtin_amdgcn_exp2f(fmaf(s[r][t][e], c, off));
+        sum += s[r][t][e];
       }
-    mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-    mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-    const float alpha = __builtin_amdgcn_exp2f(w.m[r] - mx);
-    w.m[r] = mx;
-    float sum = 0.f;
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-#pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const float x = __builtin_amdgcn_exp2f(s[r][t][e] - mx);
-        sum += x;
-        s[r][t][e] = MASK && key0 + 4 * t + e > qpos[r] ? 0.f : x * ratio;
-      }
-      p[r][t >> 1][2 * (t & 1)] = pack_f16x2(s[r][t][0], s[r][t][1]);
-      p[r][t >> 1][2 * (t & 1) + 1] = pack_f16x2(s[r][t][2], s[r][t][3]);
-    }
-    w.l[r] = w.l[r] * alpha + sum;
-#pragma unroll
-    for (int t = 0; t < 8; ++t) w.o[r][t] *= alpha;
+    w.l[r] = fmaf(sum, inv_factor, w.l[r]);
   }
 }
 
-// WK waves share the rows and split the blocks (joined through LDS), 4 / WK groups of waves have rows of their own.
-template <typename T, int RT, int WK> __global__ __launch_bounds__(256) void kv8_attn_kernel(AttnArgs a) {
-  constexpr int WR = 4 / WK, ROWS = 16 * RT;
-  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int g = lane >> 4, j = lane & 15;
-  const int wk = wave % WK, wr = wave / WK;
-  const int b = blockIdx.z / a.Hkv, hk = blockIdx.z % a.Hkv, split = blockIdx.x;
-  const int64_t start = a.start_dev ? *a.start_dev : a.start;
-  const int rows = (int)(a.S * a.G), row0 = ((int)blockIdx.y * WR + wr) * ROWS;
-  const int64_t total = min(start + a.S, a.capacity), cblocks = (a.capacity + BLK - 1) / BLK;
-  const int64_t whole = total / BLK;  // blocks in 8 bits; block `whole` is the tail
-  const int64_t bh = (int64_t)b * a.Hkv + hk;
-  const int8_t* ck = a.ck + bh * cblocks * (BLK * D);
-  const int8_t* cv = a.cv + bh * cblocks * (BLK * D);
-  const float* skp = a.sk + bh * cblocks;
-  const float* svp = a.sv + bh * cblocks;
+// A block in 8 bits: P' = p * scale / unit as fp16 operands.
+template <typename T, int RT>
+Q3_DEV void softmax_codes(Rows<T, RT>& w, f32x4 (&s)[RT][4], float c, float vscale, bool mask, int key0,
+                          const int (&qpos)[RT], i32x4 (&p)[RT][2]) {
+  // a value scale within 16 times of the unit leaves it; one 2^60 below adds nothing worth a new unit
+  const uint32_t vb = __float_as_uint(vscale);  // >= 0, or NaN
+  float ratio = vscale * w.inv, units = 1.f;
+  const uint32_t kMost = 0x41800000u, kLeast = 0x3d800000u, kNone = 0x21800000u;  // 16, 1 / 16, 2^-60
+  uint32_t rb = __float_as_uint(ratio);
+  if (vb < 0x7f800000u && vb > 0 && (w.inv == 0.f || rb > kMost || (rb < kLeast && rb > kNone))) {
+    const uint32_t e = min(max(vb & 0x7f800000u, 0x00800000u), 0x7e000000u);  // the power of two below, 2^-126 .. 2^125
+    const float inv = __uint_as_float(0x7f000000u - e);
+    units = w.unit * inv;
+    w.unit = __uint_as_float(e);
+    w.inv = inv;
+    ratio = vscale * inv;
+    rb = __float_as_uint(ratio);
+  }
+  const bool rides = rb >= kLeast && rb <= kMost;  // the factor rides in the exponent
+  const float lr = rides ? __builtin_amdgcn_logf(ratio) : 0.f;  // base 2
+  softmax_step<T, RT>(w, s, c, lr, __builtin_amdgcn_exp2f(-lr), units, mask, key0, qpos);
+  if (!rides) {  // zero, far below the unit, or NaN, which hidden positions stay clear of
+#pragma unroll
+    for (int r = 0; r < RT; ++r)
+#pragma unroll
+      for (int t = 0; t < 4; ++t)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) s[r][t][e] = s[r][t][e] == 0.f ? 0.f : s[r][t][e] * ratio;
+  }
+#pragma unroll
+  for (int r = 0; r < RT; ++r)
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      p[r][t >> 1][2 * (t & 1)] = pack_f16x2(s[r][t][0], s[r][t][1]);
+      p[r][t >> 1][2 * (t & 1) + 1] = pack_f16x2(s[r][t][2], s[r][t][3]);
+    }
+}
 
-  Rows<T, RT> w;
-  int qpos[RT];  // relative to start: the last visible key is start + qpos
+// What a wave of either kernel knows of its launch.
+struct Span {
+  int64_t start, total, whole, b0, b_end;  // positions before the queries and in all; blocks in 8 bits; this split's blocks
+  int rows, row0;
+  int64_t bh;
+  const int8_t *ck, *cv;
+  const float *sk, *sv;
+  const u16 *tk, *tv;
+};
+
+// Blocks a split takes: at least minper, all of them over at most max_splits.  It follows from the positions alone, not from
+// the span that a launch covers, so a captured step and an eager call of one length form the same sums.
+Q3_DEV int64_t split_blocks(const AttnArgs& a, int64_t total) {
+  const int64_t all = (total + BLK - 1) / BLK, per = (all + a.max_splits - 1) / a.max_splits;
+  return per > a.minper ? per : a.minper;
+}
+
+template <int RT> Q3_DEV Span span_of(const AttnArgs& a, int b, int hk, int split, int row0) {
+  Span p;
+  p.start = a.start_dev ? *a.start_dev : a.start;
+  p.total = min(p.start + a.S, a.capacity);
+  p.whole = p.total / BLK;
+  p.rows = (int)(a.S * a.G);
+  p.row0 = row0;
+  p.bh = (int64_t)b * a.Hkv + hk;
+  const int64_t cblocks = (a.capacity + BLK - 1) / BLK, per = split_blocks(a, p.total);
+  p.b0 = split * per;
+  p.b_end = min(p.b0 + per, (p.total + BLK - 1) / BLK);
+  p.ck = a.ck + p.bh * cblocks * (BLK * D);
+  p.cv = a.cv + p.bh * cblocks * (BLK * D);
+  p.sk = a.sk + p.bh * cblocks;
+  p.sv = a.sv + p.bh * cblocks;
+  p.tk = a.tk + p.bh * (BLK * D);
+  p.tv = a.tv + p.bh * (BLK * D);
+  return p;
+}
+
+// The wave's query rows in registers, nothing summed yet.
+template <typename T, int RT>
+Q3_DEV void load_rows(const AttnArgs& a, const Span& p, int b, int hk, int g, int j, Rows<T, RT>& w, int (&qpos)[RT]) {
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
-    const int rc = min(row0 + 16 * r + j, rows - 1), s = rc / a.G, h = hk * a.G + (rc - s * a.G);
-    qpos[r] = s;
+    const int rc = min(p.row0 + 16 * r + j, p.rows - 1), s = rc / a.G, h = hk * a.G + (rc - s * a.G);
+    qpos[r] = s;  // relative to start: the last visible position is start + qpos
     const u16* qp = a.q + b * a.qb + s * a.qs + h * a.qh + 16 * g;
 #pragma unroll
     for (int c = 0; c < 2; ++c)
@@ -162,153 +227,61 @@ template <typename T, int RT, int WK> __global__ __launch_bounds__(256) void kv8
 #pragma unroll
     for (int t = 0; t < 8; ++t) w.o[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  w.unit = 0.f;
-  // this wave's blocks: those of the split, every WK-th, as far as its last row sees
-  const int64_t last_pos = start + min(row0 + ROWS, rows) / a.G - (min(row0 + ROWS, rows) % a.G ? 0 : 1);
-  const int64_t nblk = row0 < rows ? min(last_pos, total - 1) / BLK + 1 : 0;
-  const int64_t all = (total + BLK - 1) / BLK, per = (all + a.splits - 1) / a.splits;
-  const int64_t b_end = min(nblk, (split + 1) * per), b0 = split * per + wk;
-  const int64_t wend = min(b_end, whole);
-  const int64_t first_pos = start + min(row0, rows - 1) / a.G;  // blocks before it need no mask
+  w.unit = w.inv = 0.f;
+}
 
-  Raw raw;
-  float sk = 0.f, sv = 0.f;
-  const int krow = 16 * (j >> 2) + (j & 3);
-  auto load_k = [&](int64_t blk) {
-    const int8_t* p = ck + blk * (BLK * D) + krow * D + 16 * g;
+// The tail block, in 16 bits: P in T, as V is; slots past the last position hold anything and read as zeros.
+template <typename T, int RT>
+Q3_DEV void tail_block(const AttnArgs& a, const Span& p, int g, int j, Rows<T, RT>& w, const int (&qpos)[RT]) {
+  const int left = (int)(p.total - p.whole * BLK), krow = 16 * (j >> 2) + (j & 3);
+  f32x4 s[RT][4];
 #pragma unroll
-    for (int t = 0; t < 4; ++t)
+  for (int t = 0; t < 4; ++t) {
+    const u16* kp = p.tk + (krow + 4 * t) * D + 16 * g;
 #pragma unroll
-      for (int c = 0; c < 2; ++c) raw.k[t][c] = *reinterpret_cast<const i32x4*>(p + t * 4 * D + 64 * c);
-    sk = skp[blk];
-  };
-  auto load_v = [&](int64_t blk) {
-    const int8_t* p = cv + blk * (BLK * D) + j * BLK + 16 * g;
+    for (int r = 0; r < RT; ++r) s[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
-    for (int t = 0; t < 8; ++t) raw.v[t] = *reinterpret_cast<const i32x4*>(p + t * 16 * BLK);
-    sv = svp[blk];
-  };
-  int64_t blk = b0;
-  if (blk < wend) {
-    load_k(blk);
-    load_v(blk);
-  }
-  for (; blk < wend; blk += WK) {
-    f32x4 s[RT][4];
-    const float c = sk * a.scale2;
+    for (int h = 0; h < 2; ++h)
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      bf16x8_t kf[2][2];
+      for (int e = 0; e < 2; ++e) {
+        const bf16x8_t kf = *reinterpret_cast<const bf16x8_t*>(kp + 64 * h + 8 * e);
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) kf[h][e] = codes16<T>(raw.k[t][h][2 * e], raw.k[t][h][2 * e + 1]);
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        s[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) s[r][t] = mfma_16x16x32<T>(kf[h][e], w.q[r][h][e], s[r][t]);
+        for (int r = 0; r < RT; ++r) s[r][t] = mfma_16x16x32<T>(kf, w.q[r][h][e], s[r][t]);
       }
-    }
-    const float vs = sv;
-    if (blk + WK < wend) load_k(blk + WK);
-    i32x4 p[RT][2];
-    if ((blk + 1) * BLK > first_pos + 1) {
-      softmax_step<T, RT, true>(w, s, c, vs, (int)(blk * BLK - start) + 16 * g, qpos, p);
-    } else {
-      softmax_step<T, RT, false>(w, s, c, vs, 0, qpos, p);
+    __builtin_amdgcn_sched_barrier(0);  // a tile's operands at a time: registers
+  }
+  // O back to plain units: the tail's values are what they are
+  softmax_step<T, RT>(w, s, a.scale2, 0.f, 1.f, w.unit, true, (int)(p.whole * BLK - p.start) + 16 * g, qpos);
+  w.unit = w.inv = 1.f;
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    bf16x8_t pf[RT];
+#pragma unroll
+    for (int r = 0; r < RT; ++r) {
+      i32x4 x;
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        x[e] = (int)pack2<T>(s[r][2 * h + (e >> 1)][2 * (e & 1)], s[r][2 * h + (e >> 1)][2 * (e & 1) + 1]);
+      pf[r] = __builtin_bit_cast(bf16x8_t, x);
     }
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
-      const bf16x8_t v0 = codes16<F16>(raw.v[t][0], raw.v[t][1]), v1 = codes16<F16>(raw.v[t][2], raw.v[t][3]);
+      i32x4 v = *reinterpret_cast<const i32x4*>(p.tv + (16 * t + j) * BLK + 16 * g + 8 * h);
 #pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        w.o[r][t] = mfma_16x16x32<F16>(v0, __builtin_bit_cast(bf16x8_t, p[r][0]), w.o[r][t]);
-        w.o[r][t] = mfma_16x16x32<F16>(v1, __builtin_bit_cast(bf16x8_t, p[r][1]), w.o[r][t]);
-      }
-    }
-    if (blk + WK < wend) load_v(blk + WK);
-  }
-  // the tail, in 16 bits: P is rounded to T here, as V is what it multiplies; slots past the last position hold anything
-  if (blk == whole && blk < b_end) {
-    const u16* tk = a.tk + bh * (BLK * D);
-    const u16* tv = a.tv + bh * (BLK * D);
-    const int left = (int)(total - whole * BLK);  // valid slots
-    f32x4 s[RT][4];
-#pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      const u16* p = tk + (krow + 4 * t) * D + 16 * g;
-      bf16x8_t kf[2][2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h)
-#pragma unroll
-        for (int e = 0; e < 2; ++e) kf[h][e] = *reinterpret_cast<const bf16x8_t*>(p + 64 * h + 8 * e);
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        s[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-        for (int h = 0; h < 2; ++h)
-#pragma unroll
-          for (int e = 0; e < 2; ++e) s[r][t] = mfma_16x16x32<T>(kf[h][e], w.q[r][h][e], s[r][t]);
-      }
-    }
-    const int key0 = (int)(whole * BLK - start) + 16 * g;
-#pragma unroll
-    for (int r = 0; r < RT; ++r) {
-      float mx = w.m[r];
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[r][t][e] = key0 + 4 * t + e > qpos[r] ? -INFINITY : s[r][t][e] * a.scale2;
-          mx = fmaxf(mx, s[r][t][e]);
-        }
-      mx = fmaxf(mx, __shfl_xor(mx, 16, 64));
-      mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-      const float alpha = __builtin_amdgcn_exp2f(w.m[r] - mx);
-      w.m[r] = mx;
-      float sum = 0.f;
-#pragma unroll
-      for (int t = 0; t < 4; ++t)
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[r][t][e] = __builtin_amdgcn_exp2f(s[r][t][e] - mx);
-          sum += s[r][t][e];
-        }
-      w.l[r] = w.l[r] * alpha + sum;
-      const float f = alpha * w.unit;  // O back to plain units: the tail's values are what they are
-#pragma unroll
-      for (int t = 0; t < 8; ++t) w.o[r][t] *= f;
-    }
-    w.unit = 1.f;
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      bf16x8_t p[RT];
-#pragma unroll
-      for (int r = 0; r < RT; ++r) {
-        i32x4 x;
-#pragma unroll
-        for (int e = 0; e < 4; ++e)
-          x[e] = (int)pack2<T>(s[r][2 * h + (e >> 1)][2 * (e & 1)], s[r][2 * h + (e >> 1)][2 * (e & 1) + 1]);
-        p[r] = __builtin_bit_cast(bf16x8_t, x);
+      for (int e = 0; e < 4; ++e) {
+        const int slot = 16 * g + 8 * h + 2 * e;
+        if (slot >= left) v[e] = 0;
+        else if (slot + 1 >= left) v[e] &= 0xffff;
       }
 #pragma unroll
-      for (int t = 0; t < 8; ++t) {
-        i32x4 v = *reinterpret_cast<const i32x4*>(tv + (16 * t + j) * BLK + 16 * g + 8 * h);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int slot = 16 * g + 8 * h + 2 * e;
-          if (slot >= left) v[e] = 0;
-          else if (slot + 1 >= left) v[e] &= 0xffff;
-        }
-#pragma unroll
-        for (int r = 0; r < RT; ++r) w.o[r][t] = mfma_16x16x32<T>(__builtin_bit_cast(bf16x8_t, v), p[r], w.o[r][t]);
-      }
+      for (int r = 0; r < RT; ++r) w.o[r][t] = mfma_16x16x32<T>(__builtin_bit_cast(bf16x8_t, v), pf[r], w.o[r][t]);
+      if (t & 1) __builtin_amdgcn_sched_barrier(0);
     }
   }
-  // row sums over the lane groups, O in plain units
+}
+
+// Row sums over the lane groups, O in plain units.
+template <typename T, int RT> Q3_DEV void close_rows(Rows<T, RT>& w) {
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
     w.l[r] += __shfl_xor(w.l[r], 16, 64);
@@ -316,41 +289,15 @@ template <typename T, int RT, int WK> __global__ __launch_bounds__(256) void kv8
 #pragma unroll
     for (int t = 0; t < 8; ++t) w.o[r][t] *= w.unit;
   }
-  // the waves of one set of rows joined in halves, in a fixed order
-  if constexpr (WK > 1) {
-    __shared__ f32x4 jo[WK / 2][RT][8][64];
-    __shared__ float jm[WK / 2][RT][64], jl[WK / 2][RT][64];
-#pragma unroll
-    for (int half = WK / 2; half >= 1; half >>= 1) {
-      if (wk >= half && wk < 2 * half) {
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          jm[wk - half][r][lane] = w.m[r];
-          jl[wk - half][r][lane] = w.l[r];
-#pragma unroll
-          for (int t = 0; t < 8; ++t) jo[wk - half][r][t][lane] = w.o[r][t];
-        }
-      }
-      __syncthreads();
-      if (wk < half) {
-#pragma unroll
-        for (int r = 0; r < RT; ++r) {
-          const float m2 = jm[wk][r][lane], m = fmaxf(w.m[r], m2);
-          const float f1 = __builtin_amdgcn_exp2f(w.m[r] - m), f2 = __builtin_amdgcn_exp2f(m2 - m);
-          w.l[r] = w.l[r] * f1 + jl[wk][r][lane] * f2;
-          w.m[r] = m;
-#pragma unroll
-          for (int t = 0; t < 8; ++t) w.o[r][t] = w.o[r][t] * f1 + jo[wk][r][t][lane] * f2;
-        }
-      }
-      __syncthreads();
-    }
-    if (wk != 0) return;
-  }
+}
+
+// O / l to the output, or this split's (O, m, l).  A split without a visible position leaves l = 0 and no O.
+template <typename T, int RT>
+Q3_DEV void store_rows(const AttnArgs& a, const Span& p, int b, int hk, int split, int g, int j, const Rows<T, RT>& w) {
 #pragma unroll
   for (int r = 0; r < RT; ++r) {
-    const int row = row0 + 16 * r + j;
-    if (row >= rows) continue;
+    const int row = p.row0 + 16 * r + j;
+    if (row >= p.rows) continue;
     if (a.splits == 1) {
       const int64_t s = row / a.G, h = hk * a.G + (row - s * a.G);
       u16* op = a.o + b * a.ob + s * a.os + h * a.oh + 4 * g;
@@ -360,15 +307,201 @@ template <typename T, int RT, int WK> __global__ __launch_bounds__(256) void kv8
         *reinterpret_cast<i32x2*>(op + 16 * t) = i32x2{(int)pack2<T>(w.o[r][t][0] * inv, w.o[r][t][1] * inv),
                                                        (int)pack2<T>(w.o[r][t][2] * inv, w.o[r][t][3] * inv)};
     } else {
-      const int64_t pr = (bh * rows + row) * a.splits + split;
+      const int64_t pr = (p.bh * p.rows + row) * a.splits + split;
       if (g == 0) {
         a.pm[pr] = w.m[r];
         a.pl[pr] = w.l[r];
       }
+      if (w.l[r] == 0.f) continue;
 #pragma unroll
       for (int t = 0; t < 8; ++t) *reinterpret_cast<f32x4*>(a.po + pr * D + 16 * t + 4 * g) = w.o[r][t];
     }
   }
+}
+
+// Few rows (at most 16 per key/value head: one token of a group, a few of a small one): four waves share the rows and take
+// every fourth block each, their K and V fragments straight from memory, and join through LDS.
+template <typename T> __global__ __launch_bounds__(256) void kv8_attn_rows_kernel(AttnArgs a) {
+  constexpr int RT = 1, WK = 4;
+  const int lane = threadIdx.x & 63, wk = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, j = lane & 15;
+  const int b = blockIdx.x / a.Hkv, hk = blockIdx.x % a.Hkv, split = blockIdx.z;
+  const Span sp = span_of<RT>(a, b, hk, split, 0);
+  Rows<T, RT> w;
+  int qpos[RT];
+  load_rows<T, RT>(a, sp, b, hk, g, j, w, qpos);
+  const int64_t wend = min(sp.b_end, sp.whole);
+  int64_t blk = sp.b0 + wk;
+
+  Raw raw;
+  float sk = 0.f, sv = 0.f;
+  const int krow = 16 * (j >> 2) + (j & 3);
+  auto load_k = [&](int64_t i) {
+    const int8_t* p = sp.ck + i * (BLK * D) + krow * D + 16 * g;
+#pragma unroll
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int c = 0; c < 2; ++c) raw.k[t][c] = *reinterpret_cast<const i32x4*>(p + t * 4 * D + 64 * c);
+    sk = sp.sk[i];
+    sv = sp.sv[i];
+  };
+  auto load_v = [&](int64_t i) {
+    const int8_t* p = sp.cv + i * (BLK * D) + j * BLK + 16 * g;
+#pragma unroll
+    for (int t = 0; t < 8; ++t) raw.v[t] = *reinterpret_cast<const i32x4*>(p + t * 16 * BLK);
+  };
+  if (blk < wend) {
+    load_k(blk);
+    load_v(blk);
+  }
+  for (; blk < wend; blk += WK) {
+    f32x4 s[RT][4];
+    const float c = sk * a.scale2;
+#pragma unroll
+    for (int t = 0; t < 4; ++t) {
+      s[0][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 2; ++e)
+          s[0][t] = mfma_16x16x32<T>(codes16<T>(raw.k[t][h][2 * e], raw.k[t][h][2 * e + 1]), w.q[0][h][e], s[0][t]);
+    }
+    const float vs = sv;
+    if (blk + WK < wend) load_k(blk + WK);
+    i32x4 p[RT][2];
+    softmax_codes<T, RT>(w, s, c, vs, (blk + 1) * BLK > sp.start + 1, (int)(blk * BLK - sp.start) + 16 * g, qpos, p);
+#pragma unroll
+    for (int t = 0; t < 8; ++t) {
+      w.o[0][t] = mfma_16x16x32<F16>(codes16<F16>(raw.v[t][0], raw.v[t][1]), __builtin_bit_cast(bf16x8_t, p[0][0]), w.o[0][t]);
+      w.o[0][t] = mfma_16x16x32<F16>(codes16<F16>(raw.v[t][2], raw.v[t][3]), __builtin_bit_cast(bf16x8_t, p[0][1]), w.o[0][t]);
+    }
+    if (blk + WK < wend) load_v(blk + WK);
+  }
+  if (blk == sp.whole && blk < sp.b_end) tail_block<T, RT>(a, sp, g, j, w, qpos);
+  close_rows<T, RT>(w);
+  // the waves joined in halves, in a fixed order
+  __shared__ f32x4 jo[WK / 2][8][64];
+  __shared__ float jm[WK / 2][64], jl[WK / 2][64];
+#pragma unroll
+  for (int half = WK / 2; half >= 1; half >>= 1) {
+    if (wk >= half && wk < 2 * half) {
+      jm[wk - half][lane] = w.m[0];
+      jl[wk - half][lane] = w.l[0];
+#pragma unroll
+      for (int t = 0; t < 8; ++t) jo[wk - half][t][lane] = w.o[0][t];
+    }
+    __syncthreads();
+    if (wk < half) {
+      const float m2 = jm[wk][lane], m = fmaxf(w.m[0], m2);
+      const float f1 = __builtin_amdgcn_exp2f(w.m[0] - m), f2 = __builtin_amdgcn_exp2f(m2 - m);
+      w.l[0] = w.l[0] * f1 + jl[wk][lane] * f2;
+      w.m[0] = m;
+#pragma unroll
+      for (int t = 0; t < 8; ++t) w.o[0][t] = w.o[0][t] * f1 + jo[wk][t][lane] * f2;
+    }
+    __syncthreads();
+  }
+  if (wk == 0) store_rows<T, RT>(a, sp, b, hk, split, g, j, w);
+}
+
+// Barrier that leaves global loads in flight: this wave's LDS accesses are done, then s_barrier.
+Q3_DEV void lds_barrier() {
+  __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14));  // lgkmcnt(0)
+  asm volatile("" ::: "memory");
+  __builtin_amdgcn_s_barrier();
+  asm volatile("" ::: "memory");
+}
+
+// Many rows: WR waves of 32 rows each share every block.  Its codes become 16-bit fragments once per workgroup, in LDS in
+// the order in which the lanes read them (a wave-wide kilobyte per fragment: no bank conflicts), one block ahead of their
+// use; the codes after that are in flight in registers meanwhile.
+template <typename T, int WR> __global__ __launch_bounds__(WR * 64, 2) void kv8_attn_tile_kernel(AttnArgs a) {
+  constexpr int RT = 2, KT = 16 / (2 * WR);  // 16-byte pieces of K (and of V) that a lane turns into fragments
+  __shared__ __attribute__((aligned(16))) i32x4 lk[2][4][4][64], lv[2][8][2][64];  // [stage][tile][16-byte step][lane]
+  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int g = lane >> 4, j = lane & 15;
+  const int b = blockIdx.x / a.Hkv, hk = blockIdx.x % a.Hkv, split = blockIdx.z;
+  const int rb = gridDim.y - 1 - blockIdx.y;  // the rows that see most first
+  const int wg0 = rb * (16 * RT * WR);
+  const Span sp = span_of<RT>(a, b, hk, split, wg0 + wave * 16 * RT);
+  Rows<T, RT> w;
+  int qpos[RT];
+  load_rows<T, RT>(a, sp, b, hk, g, j, w, qpos);
+  auto seen = [&](int row0, int n) { return sp.start + (min(row0 + n, sp.rows) - 1) / a.G; };  // last position of n rows
+  const int64_t wg_end = min(min(sp.b_end, sp.whole), seen(wg0, 16 * RT * WR) / BLK + 1);
+  const int64_t my_end = sp.row0 < sp.rows ? seen(sp.row0, 16 * RT) / BLK + 1 : 0;  // blocks this wave's rows see
+  const int64_t first_pos = sp.start + min(sp.row0, sp.rows - 1) / a.G;
+
+  i32x4 rk[KT], rv[KT];
+  float sk = 0.f, sv = 0.f, nsk = 0.f, nsv = 0.f;
+  const int krow = 16 * (j >> 2) + (j & 3);
+  auto fetch = [&](int64_t i) {  // this wave's share: pieces KT wave .. of the K tiles' halves and of the V dim tiles
+    const int8_t* kp = sp.ck + i * (BLK * D) + krow * D + 16 * g;
+    const int8_t* vp = sp.cv + i * (BLK * D) + j * BLK + 16 * g;
+#pragma unroll
+    for (int c = 0; c < KT; ++c) {
+      const int q = KT * wave + c;
+      rk[c] = *reinterpret_cast<const i32x4*>(kp + (q >> 1) * 4 * D + 64 * (q & 1));
+      rv[c] = *reinterpret_cast<const i32x4*>(vp + q * 16 * BLK);
+    }
+    nsk = sp.sk[i];
+    nsv = sp.sv[i];
+  };
+  auto spread = [&](int st) {
+#pragma unroll
+    for (int c = 0; c < KT; ++c)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int q = KT * wave + c;
+        lk[st][q >> 1][2 * (q & 1) + e][lane] = __builtin_bit_cast(i32x4, codes16<T>(rk[c][2 * e], rk[c][2 * e + 1]));
+        lv[st][q][e][lane] = __builtin_bit_cast(i32x4, codes16<F16>(rv[c][2 * e], rv[c][2 * e + 1]));
+      }
+    sk = nsk;
+    sv = nsv;
+  };
+  int64_t blk = sp.b0;
+  if (blk < wg_end) {
+    fetch(blk);
+    spread(0);
+    if (blk + 1 < wg_end) fetch(blk + 1);
+  }
+  lds_barrier();
+  for (int st = 0; blk < wg_end; ++blk, st ^= 1) {
+    if (blk < my_end) {
+      const float c = sk * a.scale2;
+      f32x4 s[RT][4];
+#pragma unroll
+      for (int t = 0; t < 4; ++t) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r) s[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const bf16x8_t kf = __builtin_bit_cast(bf16x8_t, lk[st][t][e][lane]);
+#pragma unroll
+          for (int r = 0; r < RT; ++r) s[r][t] = mfma_16x16x32<T>(kf, w.q[r][e >> 1][e & 1], s[r][t]);
+        }
+      }
+      i32x4 p[RT][2];
+      softmax_codes<T, RT>(w, s, c, sv, (blk + 1) * BLK > first_pos + 1, (int)(blk * BLK - sp.start) + 16 * g, qpos, p);
+#pragma unroll
+      for (int t = 0; t < 8; ++t) {
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, lv[st][t][e][lane]);
+#pragma unroll
+          for (int r = 0; r < RT; ++r) w.o[r][t] = mfma_16x16x32<F16>(vf, __builtin_bit_cast(bf16x8_t, p[r][e]), w.o[r][t]);
+        }
+      }
+    }
+    if (blk + 1 < wg_end) {
+      spread(st ^ 1);  // every wave is done with that stage: the barrier of the block before
+      if (blk + 2 < wg_end) fetch(blk + 2);
+    }
+    lds_barrier();
+  }
+  if (sp.b0 <= sp.whole && sp.whole < sp.b_end && sp.whole < my_end) tail_block<T, RT>(a, sp, g, j, w, qpos);
+  close_rows<T, RT>(w);
+  store_rows<T, RT>(a, sp, b, hk, split, g, j, w);
 }
 
 // out = sum_j 2^(m_j - M) o_j / sum_j 2^(m_j - M) l_j over a row's splits, in fixed order: a wave per row, 2 dims a lane.
@@ -384,46 +517,52 @@ template <typename T> __global__ __launch_bounds__(256) void kv8_merge_kernel(At
   float l = 0.f, x = 0.f, y = 0.f;
   for (int k0 = 0; k0 < a.splits; k0 += 64) {
     const int n = min(64, a.splits - k0);
-    const float wgt = lane < n ? __builtin_amdgcn_exp2f(a.pm[p0 + k0 + lane] - mx) : 0.f;
-    l += lane < n ? wgt * a.pl[p0 + k0 + lane] : 0.f;
+    float wgt = 0.f;
+    if (lane < n) {
+      const float pl = a.pl[p0 + k0 + lane];
+      wgt = pl == 0.f ? 0.f : __builtin_amdgcn_exp2f(a.pm[p0 + k0 + lane] - mx);  // l = 0: nothing stored
+      l += wgt * pl;
+    }
     for (int k = 0; k < n; ++k) {
       const float f = __shfl(wgt, k, 64);
+      if (f == 0.f) continue;
       const float* o = a.po + (p0 + k0 + k) * D + 2 * lane;
       x += f * o[0];
       y += f * o[1];
     }
   }
   l = group_sum<64>(l);
+  const float inv = 1.f / l;
   const int64_t s = i / a.G, h = (bh % a.Hkv) * a.G + (i - s * a.G);
-  *reinterpret_cast<uint32_t*>(a.o + (bh / a.Hkv) * a.ob + s * a.os + h * a.oh + 2 * lane) = pack2<T>(x / l, y / l);
+  *reinterpret_cast<uint32_t*>(a.o + (bh / a.Hkv) * a.ob + s * a.os + h * a.oh + 2 * lane) = pack2<T>(x * inv, y * inv);
 }
 
 struct Plan {
-  int wk, splits;
+  int waves;  // of a workgroup of the tile kernel; 0: the rows kernel
+  int max_splits, minper, splits;
   int64_t row_blocks;
 };
 
-// Rows of one key/value head and the positions that a launch may span -> tiling.
+// Rows of one key/value head -> kernel and splits; the positions that a launch may span only bound the grid.
 Plan plan_for(int64_t B, int64_t Hkv, int64_t rows, int64_t span) {
   Plan p;
-  p.wk = rows <= 16 ? 4 : 1;
-  const int64_t per_wg = 16 * (4 / p.wk);
-  p.row_blocks = (rows + per_wg - 1) / per_wg;
-  const int64_t blocks = (span + BLK - 1) / BLK, groups = B * Hkv * p.row_blocks;
-  // enough workgroups for two on every CU, but a block for each wave at least
-  int64_t s = std::max<int64_t>(1, 512 / groups);
-  s = std::min<int64_t>(s, (blocks + p.wk - 1) / p.wk);
-  p.splits = (int)std::min<int64_t>(s, 1024);
+  p.waves = rows <= 16 ? 0 : rows <= 128 ? 4 : 8;
+  p.row_blocks = p.waves ? (rows + 32 * p.waves - 1) / (32 * p.waves) : 1;
+  // eight waves on every CU; a block for each wave of a split (rows), or enough of them to pay for the join (tiles)
+  const int64_t wgs = B * Hkv * p.row_blocks;
+  p.max_splits = (int)std::min<int64_t>(1024, std::max<int64_t>(1, (p.waves == 8 ? 256 : 512) / wgs));
+  p.minper = p.waves ? 16 : 4;
+  const int64_t blocks = (span + BLK - 1) / BLK;
+  p.splits = (int)std::min<int64_t>(p.max_splits, (blocks + p.minper - 1) / p.minper);
   return p;
 }
 
-template <typename T> int launch(const Plan& p, const AttnArgs& a, dim3 g, hipStream_t s) {
-  if (p.wk == 4) kv8_attn_kernel<T, 1, 4><<<g, 256, 0, s>>>(a);
-  else kv8_attn_kernel<T, 1, 1><<<g, 256, 0, s>>>(a);
-  if (p.splits > 1) {
-    const dim3 mg((unsigned)((a.S * a.G + 3) / 4), g.z);
-    kv8_merge_kernel<T><<<mg, 256, 0, s>>>(a);
-  }
+template <typename T> int launch(const Plan& p, const AttnArgs& a, int64_t bh, hipStream_t s) {
+  const dim3 g((unsigned)bh, (unsigned)p.row_blocks, (unsigned)p.splits);
+  if (p.waves == 8) kv8_attn_tile_kernel<T, 8><<<g, 512, 0, s>>>(a);
+  else if (p.waves == 4) kv8_attn_tile_kernel<T, 4><<<g, 256, 0, s>>>(a);
+  else kv8_attn_rows_kernel<T><<<g, 256, 0, s>>>(a);
+  if (p.splits > 1) kv8_merge_kernel<T><<<dim3((unsigned)((a.S * a.G + 3) / 4), (unsigned)bh), 256, 0, s>>>(a);
   return (int)hipGetLastError();
 }
 
@@ -451,6 +590,7 @@ int q3_kv8_attention(int dtype, const void* q, int64_t qsb, int64_t qss, int64_t
   Q3_REQUIRE(start_dev ? S == 1 : (start >= 0 && start <= capacity && S <= capacity - start));
   for (int64_t st : {qsb, qss, qsh}) Q3_REQUIRE(st % 8 == 0);
   for (int64_t st : {osb, oss, osh}) Q3_REQUIRE(st % 4 == 0);
+  Q3_REQUIRE(scale > 0.f && scale < 1e30f);  // the running maximum is of unscaled scores
   const int64_t rows = S * (Hq / Hkv);
   const Plan p = plan_for(B, Hkv, rows, start_dev ? capacity : start + S);
   Q3_REQUIRE(rows < (1ll << 31) - 128 && p.row_blocks < 65536);
@@ -459,9 +599,9 @@ int q3_kv8_attention(int dtype, const void* q, int64_t qsb, int64_t qss, int64_t
   float* ws = (float*)workspace;
   const AttnArgs a{(const u16*)q, qsb, qss, qsh, cache_k, cache_v, scale_k, scale_v, (const u16*)tail_k,
                    (const u16*)tail_v, (u16*)out, osb, oss, osh, ws, ws + parts * D, ws + parts * (D + 1), S, start,
-                   capacity, start_dev, (int)Hkv, (int)(Hq / Hkv), p.splits, scale * 1.4426950408889634f};
-  const dim3 g((unsigned)p.splits, (unsigned)p.row_blocks, (unsigned)(B * Hkv));
-  return dtype == Q3_BF16 ? launch<BF16>(p, a, g, stream) : launch<F16>(p, a, g, stream);
+                   capacity, start_dev, (int)Hkv, (int)(Hq / Hkv), p.splits, p.max_splits, p.minper,
+                   scale * 1.4426950408889634f};
+  return dtype == Q3_BF16 ? launch<BF16>(p, a, B * Hkv, stream) : launch<F16>(p, a, B * Hkv, stream);
 }
 
 }  // extern "C"
