@@ -8,6 +8,7 @@ int launch_tile_nt(int dtype, int cfg, int epi, const Args& a, hipStream_t s);
 int launch_tile_nn(int dtype, int cfg, int epi, const Args& a, hipStream_t s);
 int launch_tile_tn(int dtype, int cfg, const Args& a, hipStream_t s);
 int launch_tile_q8(int dtype, int cfg, int epi, const Args& a, hipStream_t s);
+int launch_rows_q8(int dtype, int epi, const Args& a, hipStream_t s);
 }  // namespace q3gemm
 
 namespace {
@@ -297,6 +298,9 @@ bool parse(const q3_gemm_desc* d, Call& c) {
   return tile_rows(a, 32) * tile_cols(a, 64) < (1ll << 28);
 }
 
+// One token row tile of the matrix cores: the weights are streamed once, by a kernel that has no tiles to fill.
+constexpr int64_t kStreamRows = 16;
+
 // 8-bit operands: pairs of codes along k are the 16-bit elements of the tiles above.
 bool parse_int8(const q3_int8_gemm_desc* d, Call& c) {
   if (!d || (d->dtype != Q3_BF16 && d->dtype != Q3_F16)) return false;
@@ -491,7 +495,7 @@ int q3_gemm(const q3_gemm_desc* d, void* workspace, size_t workspace_bytes, hipS
 
 size_t q3_gemm_int8_workspace_bytes(const q3_int8_gemm_desc* d) {
   Call c;
-  if (!parse_int8(d, c)) return 0;
+  if (!parse_int8(d, c) || c.a.M <= kStreamRows) return 0;
   const Plan p = plan_for(c.a, false, false, c.can_split, c.combine);
   return p.splits > 1 ? (size_t)p.splits * (size_t)c.a.M * (size_t)c.a.N * sizeof(int) : 0;
 }
@@ -499,6 +503,7 @@ size_t q3_gemm_int8_workspace_bytes(const q3_int8_gemm_desc* d) {
 int q3_gemm_int8(const q3_int8_gemm_desc* d, void* workspace, size_t workspace_bytes, hipStream_t stream) {
   Call c;
   Q3_REQUIRE(parse_int8(d, c));
+  if (c.a.M <= kStreamRows) return q3gemm::launch_rows_q8(d->dtype, c.epi, c.a, stream);
   Launch l[2];
   const int n = launches(c, l);
   if (l[0].p.splits > 1) {
