@@ -1,8 +1,12 @@
 """Dense bf16 Qwen3 inference: single device, unpadded equal-length batches, contiguous KV cache,
 greedy decoding.  Mirrors ``qwen3_triton/inference/model.py:26-225`` (``KVCache``,
 ``TritonQwen3Inference``, ``CapturedGreedyRequest``); the arithmetic is the HIP kernels.
+
+New here: serving in 8 bits, each half on its own.  ``TritonQwen3Inference.quantize_weights`` holds the layers'
+projections in int8 and quantises their inputs per token; ``new_cache(..., dtype=torch.int8)`` (``cache_dtype`` of
+``generate``, ``DecodeSession`` and ``CapturedGreedyRequest``) keeps keys and values in int8 (``int8.LayerCache``).
 """
-from dataclasses import dataclass
+from dataclasses import dataclass, field
 from pathlib import Path
 
 import torch
@@ -18,7 +22,7 @@ from ..kernels.embedding import IdRangeError, embedding
 from ..kernels.linear import gemm, gemm_ok
 from ..kernels.mlp_precision import gate_up_swiglu
 from ..kernels.residual import residual_add
-from . import kernels
+from . import int8, kernels
 
 
 def _decode_rows(t, gemv):
@@ -81,6 +85,10 @@ class KVCache:
     def reset(self):
         self.length, self.valid = 0, True
 
+    def quantized(self):
+        """An ``Int8KVCache`` of the same positions (prefilled in 16 bits, decoded in 8)."""
+        return _quantized_cache(self)
+
     def admit(self, owner, batch, tokens):
         """Raise unless ``tokens`` more positions of ``batch`` rows fit this valid cache of ``owner``."""
         problems = [what for bad, what in (
@@ -91,6 +99,54 @@ class KVCache:
              f'has {self.capacity - self.length} free positions, {tokens} needed')) if bad]
         if problems:
             raise ValueError('KV cache ' + '; '.join(problems))
+
+
+@dataclass
+class Int8KVCache(KVCache):
+    """A ``KVCache`` whose keys and values are held in int8, one ``int8.LayerCache`` per layer (``keys`` and ``values``
+    stay empty).  A block of 64 positions is quantised when its last one comes; the unfinished block is in bf16."""
+    layers: list = field(default_factory=list)
+
+    @property
+    def nbytes(self):
+        return sum(layer.nbytes for layer in self.layers)
+
+    def dequantized(self):
+        """A bf16 ``KVCache`` of the same positions (a request that goes on in 16 bits)."""
+        shape = (*self.layers[0].k.shape[:2], self.capacity, 128)
+        out = KVCache([], [], self.capacity, self.batch_size, self.owner, self.length, self.valid)
+        for layer in self.layers:
+            for held, kept in zip((out.keys, out.values),
+                                  int8.read(layer, self.length) if self.length else (None, None)):
+                held.append(torch.empty(shape, device=layer.k.device, dtype=layer.k_tail.dtype))
+                if kept is not None:
+                    held[-1][:, :, :self.length].copy_(kept)
+        return out
+
+
+def _quantized_cache(cache):
+    """An ``Int8KVCache`` of a bf16 cache's positions (a request prefilled in 16 bits that decodes in 8)."""
+    b, h = cache.keys[0].shape[:2]
+    layers = []
+    for k, v in zip(cache.keys, cache.values):
+        layers.append(int8.LayerCache.empty(b, h, cache.capacity, device=k.device, dtype=k.dtype))
+        if cache.length:
+            int8.append(k[:, :, :cache.length].transpose(1, 2), v[:, :, :cache.length].transpose(1, 2), layers[-1], 0)
+    return Int8KVCache([], [], cache.capacity, cache.batch_size, cache.owner, cache.length, cache.valid, layers)
+
+
+class _Int8Layer:
+    """One decoder layer's projections as (codes, channel scales)."""
+
+    def __init__(self, layer):
+        a, m = layer.self_attn, layer.mlp
+        self.q, self.k, self.v, self.o, self.gate, self.up, self.down = (
+            int8.quantize_rows(p.weight.detach()) for p in (a.q_proj, a.k_proj, a.v_proj, a.o_proj, m.gate_proj, m.up_proj,
+                                                            m.down_proj))
+
+    @property
+    def nbytes(self):
+        return sum(t.numel() * t.element_size() for pair in vars(self).values() for t in pair)
 
 
 class TritonQwen3Inference(nn.Module):
@@ -106,6 +162,7 @@ class TritonQwen3Inference(nn.Module):
         self.model, self.lm_head, self.config = core.model, core.lm_head, config
         self.gemv, self.split_decode = gemv, split_decode
         self._cache_owner = object()
+        self._int8 = None   # per layer, once quantize_weights has run
         self.generation_config = _generation_config(config)
         self.eval()
 
@@ -118,6 +175,7 @@ class TritonQwen3Inference(nn.Module):
         if wrong:
             raise ValueError(f'bf16 inference weights required; {wrong[0]} is not bf16')
         self.load_state_dict(state, assign=True, strict=True)
+        self._int8 = None
         if tied:
             self.lm_head.weight = self.model.embed_tokens.weight
         self.model.rotary_emb.inv_freq = self._inv_freq().to(self.lm_head.weight.device)
@@ -160,12 +218,35 @@ class TritonQwen3Inference(nn.Module):
             model.generation_config = GenerationConfig.from_pretrained(path, local_files_only=True)
         return model.load_hf_state_dict(read_checkpoint(path, device))
 
+    @torch.no_grad()
+    def quantize_weights(self):
+        """Hold the layers' seven projections in int8 with a scale per output channel, from now on, and free their bf16
+        weights (the embedding, the norms and the LM head stay in bf16).  Each projection's input is then quantised per
+        token.  ``load_hf_state_dict`` goes back to bf16."""
+        if self._int8 is not None:
+            raise ValueError('the weights are already in int8')
+        if self.device.type != 'cuda':
+            raise ValueError('the weights are not on a ROCm device (load or move them first)')
+        c = self.config
+        for n in (c.hidden_size, c.intermediate_size):
+            if n % 16 or n > int8.MAX_ROW:
+                raise ValueError(f'sizes that are multiples of 16 and at most {int8.MAX_ROW} required for int8, not {n}')
+        held = []
+        for layer in self.model.layers:
+            held.append(_Int8Layer(layer))
+            for part in (layer.self_attn, layer.mlp):
+                for proj in (p for name, p in part.named_children() if name.endswith('_proj')):
+                    proj.weight = nn.Parameter(torch.empty_like(proj.weight, device='meta'), requires_grad=False)
+        self._int8 = held
+        return self
+
     @property
     def device(self):
         return self.lm_head.weight.device
 
-    def new_cache(self, batch_size, max_length):
-        """An empty KV cache of ``max_length`` positions for ``batch_size`` rows on the model's device."""
+    def new_cache(self, batch_size, max_length, *, dtype=torch.bfloat16):
+        """An empty KV cache of ``max_length`` positions for ``batch_size`` rows on the model's device, in bf16 or in int8
+        (``dtype=torch.int8``: an ``Int8KVCache``)."""
         c = self.config
         if type(batch_size) is not int or batch_size < 1:
             raise ValueError('batch_size must be a positive int')
@@ -173,6 +254,12 @@ class TritonQwen3Inference(nn.Module):
             raise ValueError(f'max_length must be an int in [1, {c.max_position_embeddings}]')
         if self.device.type != 'cuda':
             raise ValueError('the weights are not on a ROCm device (load or move them first)')
+        if dtype not in (torch.bfloat16, torch.int8):
+            raise TypeError(f'a KV cache is bfloat16 or int8, not {dtype}')
+        if dtype == torch.int8:
+            layers = [int8.LayerCache.empty(batch_size, c.num_key_value_heads, max_length, device=self.device)
+                      for _ in self.model.layers]
+            return Int8KVCache([], [], max_length, batch_size, self._cache_owner, layers=layers)
         shape = (batch_size, c.num_key_value_heads, max_length, c.head_dim)
 
         def layer_buffers():
@@ -180,6 +267,51 @@ class TritonQwen3Inference(nn.Module):
         return KVCache(layer_buffers(), layer_buffers(), max_length, batch_size, self._cache_owner)
 
     # ------------------------------------------------------------------ forward
+    def _cached_attention(self, a, q, k, v, cos, sin, cache, i, start, start_dev):
+        """Q/K-norm + RoPE, the new positions appended to layer ``i``'s cache, attention against it: q [B,S,Hq,D] and
+        k, v [B,S,Hkv,D] as projected -> [B,S,Hq*D]."""
+        b, s = q.shape[:2]
+        d = a.head_dim
+        in8 = isinstance(cache, Int8KVCache)
+        fits = a.q_norm.eps == a.k_norm.eps and _ops.norm_rope_qk_ok(q, k, d) and all(t.is_contiguous() for t in (q, k, v))
+        if not in8 and start_dev is None and fits:
+            # Q/K-norm + RoPE of both tensors and the K/V cache append in one launch
+            q = _ops.norm_rope_qk_cache_fwd(q, k, v, a.q_norm.weight, a.k_norm.weight, cos, sin, cache.keys[i],
+                                            cache.values[i], start, a.q_norm.eps)
+            return kernels.attention(q, cache.keys[i], cache.values[i], start,
+                                     split_decode=self.split_decode).reshape(b, s, -1)
+        if in8 and fits:
+            q, k = _ops.norm_rope_qk_fwd(q, k, a.q_norm.weight, a.k_norm.weight, cos, sin, a.q_norm.eps)
+        else:
+            q = kernels.norm_rope(q, a.q_norm.weight, cos, sin, a.q_norm.eps)
+            k = kernels.norm_rope(k, a.k_norm.weight, cos, sin, a.k_norm.eps)
+        if in8:
+            int8.append(k, v, cache.layers[i], start, start_dev)
+            return int8.attention(q, cache.layers[i], start, start_dev).reshape(b, s, -1)
+        kernels.append(k, v, cache.keys[i], cache.values[i], start, start_dev)
+        return kernels.attention(q, cache.keys[i], cache.values[i], start, split_decode=self.split_decode,
+                                 start_dev=start_dev).reshape(b, s, -1)
+
+    def _int8_layers(self, x, cos, sin, cache, start, start_dev):
+        """The decoder layers on int8 weights: every projection's input is quantised where it is formed (the norms carry
+        the residual sums)."""
+        b, s, _ = x.shape
+        down = None
+        for i, (layer, w) in enumerate(zip(self.model.layers, self._int8)):
+            a, n1, n2 = layer.self_attn, layer.input_layernorm, layer.post_attention_layernorm
+            d = a.head_dim
+            if down is None:
+                h, hs = int8.rms_norm(x, n1.weight, n1.eps)
+            else:
+                h, hs, x = int8.rms_norm(down, n1.weight, n1.eps, residual=x)
+            q, k, v = int8.projections(h, hs, [w.q, w.k, w.v])
+            y = self._cached_attention(a, q.view(b, s, a.num_heads, d), k.view(b, s, a.num_kv_heads, d),
+                                       v.view(b, s, a.num_kv_heads, d), cos, sin, cache, i, start, start_dev)
+            h, hs, x = int8.rms_norm(int8.linear(*int8.quantize_rows(y), *w.o), n2.weight, n2.eps, residual=x)
+            y = int8.gate_up_swiglu(h, hs, *w.gate, *w.up)
+            down = int8.linear(*int8.quantize_rows(y), *w.down)
+        return residual_add(x, down)
+
     def _forward(self, input_ids, cache, logits_to_keep, *, validate_ids=True, start_dev=None):
         from transformers.modeling_outputs import CausalLMOutputWithPast
         if input_ids.ndim != 2 or input_ids.dtype not in (torch.int32, torch.int64) or \
@@ -214,8 +346,11 @@ class TritonQwen3Inference(nn.Module):
             cos, sin = self.model.rotary_emb(pos, torch.bfloat16)
             fused = self.gemv and kernels.decode_linear_ok(x, self.lm_head.weight)
             layers = self.model.layers
+            in8 = isinstance(cache, Int8KVCache)
             h = None  # the next layer's normed input when the previous down projection formed it
-            for i, layer in enumerate(layers):
+            if self._int8 is not None:
+                x = self._int8_layers(x, cos, sin, cache, start, start_dev)
+            for i, layer in enumerate(layers if self._int8 is None else ()):
                 a = layer.self_attn
                 d = a.head_dim
                 if fused:  # decode step: norms, residual adds and SwiGLU ride in the projections
@@ -225,10 +360,12 @@ class TritonQwen3Inference(nn.Module):
                     q = q.view(b, s, a.num_heads, d)
                     k = k.view(b, s, a.num_kv_heads, d)
                     v = v.view(b, s, a.num_kv_heads, d)
-                    if s == 1 and d == 128 and a.q_norm.eps == a.k_norm.eps:
+                    if s == 1 and d == 128 and a.q_norm.eps == a.k_norm.eps and not in8:
                         y = kernels.decode_step_attention(q, k, v, a.q_norm.weight, a.k_norm.weight, a.q_norm.eps,
                                                           cos, sin, cache.keys[i], cache.values[i], start,
                                                           start_dev).reshape(b, s, -1)
+                    elif in8:
+                        y = self._cached_attention(a, q, k, v, cos, sin, cache, i, start, start_dev)
                     else:
                         q = kernels.norm_rope(q, a.q_norm.weight, cos, sin, a.q_norm.eps)
                         k = kernels.norm_rope(k, a.k_norm.weight, cos, sin, a.k_norm.eps)
@@ -248,17 +385,7 @@ class TritonQwen3Inference(nn.Module):
                 q = q.view(b, s, a.num_heads, d)
                 k = k.view(b, s, a.num_kv_heads, d)
                 v = v.view(b, s, a.num_kv_heads, d)
-                if start_dev is None and a.q_norm.eps == a.k_norm.eps and _ops.norm_rope_qk_ok(q, k, d) and \
-                        all(t.is_contiguous() for t in (q, k, v)):
-                    # Q/K-norm + RoPE of both tensors and the K/V cache append in one launch
-                    q = _ops.norm_rope_qk_cache_fwd(q, k, v, a.q_norm.weight, a.k_norm.weight, cos, sin,
-                                                    cache.keys[i], cache.values[i], start, a.q_norm.eps)
-                else:
-                    q = kernels.norm_rope(q, a.q_norm.weight, cos, sin, a.q_norm.eps)
-                    k = kernels.norm_rope(k, a.k_norm.weight, cos, sin, a.k_norm.eps)
-                    kernels.append(k, v, cache.keys[i], cache.values[i], start, start_dev)
-                y = kernels.attention(q, cache.keys[i], cache.values[i], start, split_decode=self.split_decode,
-                                      start_dev=start_dev).reshape(b, s, -1)
+                y = self._cached_attention(a, q, k, v, cos, sin, cache, i, start, start_dev)
                 x, h = _residual_projection(x, y, a.o_proj.weight, self.gemv, layer.post_attention_layernorm)
                 m = layer.mlp
                 if b * s <= 8 and self.gemv:
@@ -298,9 +425,10 @@ class TritonQwen3Inference(nn.Module):
         return out
 
     @torch.inference_mode()
-    def generate(self, input_ids, *, max_new_tokens=32, eos_token_id=None, pad_token_id=None):
+    def generate(self, input_ids, *, max_new_tokens=32, eos_token_id=None, pad_token_id=None,
+                 cache_dtype=torch.bfloat16):
         """Greedy decoding with per-row EOS, padding and a request-local cache
-        (``inference/model.py:158-188``)."""
+        (``inference/model.py:158-188``), in bf16 or int8 (``cache_dtype``)."""
         if type(max_new_tokens) is not int or max_new_tokens < 0:
             raise ValueError('Nonnegative max_new_tokens required')
         gc = self.generation_config
@@ -321,7 +449,7 @@ class TritonQwen3Inference(nn.Module):
                 raise ValueError('Token ID outside vocabulary')
             return input_ids.clone()
         b, s = input_ids.shape
-        cache = self.new_cache(b, s + max_new_tokens)
+        cache = self.new_cache(b, s + max_new_tokens, dtype=cache_dtype)
         output = torch.empty((b, s + max_new_tokens), device=self.device, dtype=torch.int64)
         output[:, :s].copy_(input_ids)
         done = torch.zeros((b,), device=self.device, dtype=torch.bool)
@@ -359,11 +487,11 @@ class DecodeSession:
     """
 
     @torch.inference_mode()
-    def __init__(self, model, batch, capacity, *, eos=(), pad=0):
+    def __init__(self, model, batch, capacity, *, eos=(), pad=0, cache_dtype=torch.bfloat16):
         self.model, self.batch, self.capacity = model, batch, capacity
         self.eos, self.pad = tuple(eos), pad
         dev = model.device
-        self.cache = model.new_cache(batch, capacity)
+        self.cache = model.new_cache(batch, capacity, dtype=cache_dtype)
         self.ids = torch.zeros((batch, capacity), device=dev, dtype=torch.int64)
         self.current = torch.zeros((batch, 1), device=dev, dtype=torch.int64)
         self.length = torch.zeros((1,), device=dev, dtype=torch.int64)
@@ -440,7 +568,7 @@ class CapturedGreedyRequest:
     """
 
     @torch.inference_mode()
-    def __init__(self, model, input_ids, *, max_new_tokens):
+    def __init__(self, model, input_ids, *, max_new_tokens, cache_dtype=torch.bfloat16):
         if type(max_new_tokens) is not int or max_new_tokens < 1:
             raise ValueError('max_new_tokens must be a positive int (the fixed token budget)')
         if input_ids.ndim != 2 or input_ids.device != model.device or \
@@ -451,7 +579,7 @@ class CapturedGreedyRequest:
         self.model, self.shape, self.budget, self.busy = model, (b, s), max_new_tokens, False
         self.input = input_ids.clone()
         dev = model.device
-        self.cache = model.new_cache(b, s + max_new_tokens)
+        self.cache = model.new_cache(b, s + max_new_tokens, dtype=cache_dtype)
         self.output = torch.zeros((b, s + max_new_tokens), device=dev, dtype=torch.int64)
         self.current = torch.zeros((b, 1), device=dev, dtype=torch.int64)
         self.length = torch.zeros((1,), device=dev, dtype=torch.int64)
