@@ -512,6 +512,11 @@ typedef struct q3_int8_gemm_desc {
 } q3_int8_gemm_desc;
 size_t q3_gemm_int8_workspace_bytes(const q3_int8_gemm_desc* desc);
 int q3_gemm_int8(const q3_int8_gemm_desc* desc, void* workspace, size_t workspace_bytes, hipStream_t stream);
+/* q3_quant_rows of x [m, k] (row stride ldx) or, with norm_w, q3_rmsnorm_quant without a residual, and the product, in one
+ * launch, for the rows of a decode step for which q3_decode_linear_int8_ok is 1 (m <= 2, k <= 16384).  desc as there; its a, lda and a_scale are not used. */
+int q3_decode_linear_int8_ok(int64_t m, int64_t k);
+int q3_decode_linear_int8(const q3_int8_gemm_desc* desc, const void* x, int64_t ldx, const void* norm_w, float eps,
+                          hipStream_t stream);
 /* Key/value cache in 8 bits, d = 128, blocks of 64 positions (Cb = ceil(capacity / 64)) with a scale per block and head:
  *   cache_k [B, H, 64 Cb, 128], cache_v [B, H, Cb, 128, 64] (transposed within a block), scale_k / scale_v [B, H, Cb],
  *   tail_k [B, H, 64, 128], tail_v [B, H, 128, 64] in dtype: the positions of the last, unfinished block.
@@ -523,6 +528,15 @@ int q3_kv8_append(int dtype, const void* k, int64_t ksb, int64_t kss, int64_t ks
                   int64_t vsh, int8_t* cache_k, int8_t* cache_v, float* scale_k, float* scale_v, void* tail_k, void* tail_v,
                   int64_t B, int64_t S, int64_t H, int64_t d, int64_t capacity, int64_t start, const int64_t* start_dev,
                   hipStream_t stream);
+/* The Q/K-norm + rotation of a layer and that append in one launch: q [B, S, Hq, 128], k, v [B, S, H, 128] as projected
+ * (strides, multiples of 8), norm weights wq, wk [128], tables cos, sin [B, S, 128] contiguous -> yq [B, S, Hq, 128]
+ * contiguous, the normed and rotated keys (rounded to dtype first) and the unchanged values appended. */
+int q3_kv8_norm_rope_append(int dtype, const void* q, int64_t qsb, int64_t qss, int64_t qsh, const void* k, int64_t ksb,
+                            int64_t kss, int64_t ksh, const void* v, int64_t vsb, int64_t vss, int64_t vsh, const void* wq,
+                            const void* wk, const void* cos, const void* sin, void* yq, int8_t* cache_k, int8_t* cache_v,
+                            float* scale_k, float* scale_v, void* tail_k, void* tail_v, int64_t B, int64_t S, int64_t Hq,
+                            int64_t H, int64_t d, int64_t capacity, int64_t start, const int64_t* start_dev, float eps,
+                            hipStream_t stream);
 /* k, v [B, H, length, 128] in out_dtype (any): code * scale rounded once, the tail's positions as they are. */
 int q3_kv8_read(int dtype, int out_dtype, const int8_t* cache_k, const int8_t* cache_v, const float* scale_k,
                 const float* scale_v, const void* tail_k, const void* tail_v, void* k, void* v, int64_t B, int64_t H,

@@ -85,6 +85,14 @@ Q3_DEV void mfma_acc(i32x4& c, bf16x8_t a, bf16x8_t b) {
   c = __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, a), __builtin_bit_cast(i32x4, b), c, 0, 0, 0);
 }
 
+// 16-bit rows that a product turns into codes itself (w: through an RMSNorm).
+struct RowIn {
+  const u16* x;
+  int64_t ldx;
+  const u16* w;
+  float eps;
+};
+
 // Work item -> (tile, split): each XCD (workgroup ids congruent mod 8) takes a contiguous range of items,
 // splits outermost, so its L2 holds one k-range of the shared operand; tiles in groups of 4 tile-rows.
 Q3_DEV void work_coords(int bid, int tiles_m, int tiles_n, int splits, int& tm, int& tn, int& sp) {

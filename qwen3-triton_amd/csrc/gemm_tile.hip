@@ -8,7 +8,7 @@ int launch_tile_nt(int dtype, int cfg, int epi, const Args& a, hipStream_t s);
 int launch_tile_nn(int dtype, int cfg, int epi, const Args& a, hipStream_t s);
 int launch_tile_tn(int dtype, int cfg, const Args& a, hipStream_t s);
 int launch_tile_q8(int dtype, int cfg, int epi, const Args& a, hipStream_t s);
-int launch_rows_q8(int dtype, int epi, const Args& a, hipStream_t s);
+int launch_rows_q8(int dtype, int epi, const Args& a, const RowIn& in, hipStream_t s);
 }  // namespace q3gemm
 
 namespace {
@@ -302,7 +302,7 @@ bool parse(const q3_gemm_desc* d, Call& c) {
 constexpr int64_t kStreamRows = 16;
 
 // 8-bit operands: pairs of codes along k are the 16-bit elements of the tiles above.
-bool parse_int8(const q3_int8_gemm_desc* d, Call& c) {
+bool parse_int8(const q3_int8_gemm_desc* d, Call& c, bool codes = true) {
   if (!d || (d->dtype != Q3_BF16 && d->dtype != Q3_F16)) return false;
   if (d->m < 1 || d->n < 1 || d->k < 16 || d->m >= (1ll << 31) - 256 || d->n >= (1ll << 30) || d->k >= (1ll << 17) || d->k % 16)
     return false;
@@ -323,7 +323,7 @@ bool parse_int8(const q3_int8_gemm_desc* d, Call& c) {
   auto operand = [&](const int8_t* p, int64_t ld, int64_t rows) {
     return ld % 2 == 0 && operand_ok(p, ld / 2, rows, a.K, false);
   };
-  if (!operand(d->a, d->lda, d->m) || !d->a_scale) return false;
+  if (codes && (!operand(d->a, d->lda, d->m) || !d->a_scale)) return false;
   bool vec = true;
   int64_t beg = 0;
   for (int i = 0; i < (gate_up ? 2 : d->pieces); ++i) {
@@ -503,7 +503,7 @@ size_t q3_gemm_int8_workspace_bytes(const q3_int8_gemm_desc* d) {
 int q3_gemm_int8(const q3_int8_gemm_desc* d, void* workspace, size_t workspace_bytes, hipStream_t stream) {
   Call c;
   Q3_REQUIRE(parse_int8(d, c));
-  if (c.a.M <= kStreamRows) return q3gemm::launch_rows_q8(d->dtype, c.epi, c.a, stream);
+  if (c.a.M <= kStreamRows) return q3gemm::launch_rows_q8(d->dtype, c.epi, c.a, q3gemm::RowIn{}, stream);
   Launch l[2];
   const int n = launches(c, l);
   if (l[0].p.splits > 1) {
@@ -523,6 +523,18 @@ int q3_gemm_int8(const q3_int8_gemm_desc* d, void* workspace, size_t workspace_b
     if (rc != 0) return rc;
   }
   return 0;
+}
+
+int q3_decode_linear_int8_ok(int64_t m, int64_t k) {
+  return m >= 1 && m <= 2 && k >= 16 && k % 16 == 0 && k <= 16384;  // four 16-byte pieces of a row per thread
+}
+
+int q3_decode_linear_int8(const q3_int8_gemm_desc* d, const void* x, int64_t ldx, const void* norm_w, float eps,
+                          hipStream_t stream) {
+  Call c;
+  Q3_REQUIRE(parse_int8(d, c, false) && q3_decode_linear_int8_ok(d->m, d->k));
+  Q3_REQUIRE(al16(x) && x && ldx >= d->k && ldx % 8 == 0 && (!norm_w || (al16(norm_w) && eps >= 0.f)));
+  return q3gemm::launch_rows_q8(d->dtype, c.epi, c.a, q3gemm::RowIn{(const u16*)x, ldx, (const u16*)norm_w, eps}, stream);
 }
 
 // LM-head logits A B^T, stored, with their cross-entropy statistics (q3hip.h): 256 x 256 tiles, 128 x 256 when

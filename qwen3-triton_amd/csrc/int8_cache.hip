@@ -22,21 +22,81 @@ struct CacheArgs {
   u16 *tk, *tv;
   int64_t S, H, capacity, start;
   const int64_t* start_dev;
+  // with the Q/K-norm and rotation: k as projected, and the query rows beside it
+  const u16 *q, *qw, *kw, *cs, *sn;  // q [B, S, Hq, D], norm weights [D], tables [B, S, D]
+  int64_t qb, qs, qh;
+  u16* yq;  // [B, S, Hq, D]
+  int64_t B, Hq;
+  int blocks;  // workgroups per head and batch row of the cache's part
+  float eps;
 };
+
+// RMSNorm and split-half rotation of a 128-dim row whose dims 32 i .. + 31 sit in lane i of an aligned quad (the partner
+// dims, 64 away, in lane i ^ 2), rounded once: x holds 32 16-bit values.
+template <typename T>
+Q3_DEV void norm_rope_quad(i32x4 (&x)[4], const u16* w, const u16* cs, const u16* sn, float eps, int quarter) {
+  Vec<T> f[4];
+  float ss = 0.f;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    f[c] = unpack_vec<T>(x[c]);
+#pragma unroll
+    for (int e = 0; e < 8; ++e) ss += f[c].v[e] * f[c].v[e];
+  }
+  ss = group_sum<4>(ss);
+  const float inv = rsqrtf(ss * (1.f / (float)D) + eps), sign = quarter < 2 ? -1.f : 1.f;
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const Vec<T> wf = load_vec<T>(w + 8 * c), cf = load_vec<T>(cs + 8 * c), sf = load_vec<T>(sn + 8 * c);
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      float y[2];
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int e = 2 * p + h;
+        const float n = f[c].v[e] * inv * wf.v[e];
+        const float o = __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, n), 0x4E, 0xF, 0xF, true));
+        y[h] = n * cf.v[e] + sign * o * sf.v[e];
+      }
+      x[c][p] = (int)pack2<T>(y[0], y[1]);
+    }
+  }
+}
 
 // One workgroup per (touched block, head, batch row); the one of the first block also writes the last, unfinished block's
 // new positions into the tail (after it has read the tail, which may hold the first block's positions in the same slots).
 // Thread t owns position t / 4 of the block and dims 32 (t % 4) .. + 31.
-template <typename T> __global__ __launch_bounds__(256) void kv8_append_kernel(CacheArgs a) {
+// NR: the rows come as projected and are normed and rotated here (values as they are); the workgroups behind the cache's
+// take the query rows, 64 each.
+template <typename T, bool NR> __global__ __launch_bounds__(256) void kv8_append_kernel(CacheArgs a) {
   __shared__ uint32_t red[2][4];
   __shared__ __attribute__((aligned(16))) int8_t vt[D][BLK + 16];
   const int tid = threadIdx.x, row = tid >> 2, d0 = (tid & 3) * 32;
-  const int h = blockIdx.y, b = blockIdx.z;
+  int64_t job = blockIdx.x;
+  if constexpr (NR) {
+    const int64_t cache_jobs = a.blocks * a.H * a.B;
+    if (job >= cache_jobs) {
+      const int64_t i = (job - cache_jobs) * 64 + row, n = a.B * a.S * a.Hq;  // whole quads: row is a quad's
+      if (i >= n) return;
+      const int64_t bs = i / a.Hq, qh = i - bs * a.Hq, qb = bs / a.S, qs = bs - qb * a.S;
+      const u16* p = a.q + qb * a.qb + qs * a.qs + qh * a.qh + d0;
+      i32x4 x[4];
+#pragma unroll
+      for (int c = 0; c < 4; ++c) x[c] = *reinterpret_cast<const i32x4*>(p + 8 * c);
+      norm_rope_quad<T>(x, a.qw + d0, a.cs + bs * D + d0, a.sn + bs * D + d0, a.eps, tid & 3);
+#pragma unroll
+      for (int c = 0; c < 4; ++c) *reinterpret_cast<i32x4*>(a.yq + i * D + d0 + 8 * c) = x[c];
+      return;
+    }
+  }
+  const int part = (int)(job % a.blocks);
+  job /= a.blocks;
+  const int h = (int)(job % a.H), b = (int)(job / a.H);
   const int64_t start = a.start_dev ? *a.start_dev : a.start;
   const int64_t end = min(start + a.S, a.capacity);
   if (start < 0 || end <= start) return;
   const int64_t first = start / BLK, last = end / BLK;  // last: the first block that is not whole
-  const int64_t blk = first + blockIdx.x;
+  const int64_t blk = first + part;
   const int64_t bh = (int64_t)b * a.H + h, cblocks = (a.capacity + BLK - 1) / BLK;
   u16* tk = a.tk + bh * (BLK * D);
   u16* tv = a.tv + bh * (BLK * D);
@@ -52,6 +112,10 @@ template <typename T> __global__ __launch_bounds__(256) void kv8_append_kernel(C
       for (int c = 0; c < 4; ++c) {
         kr[c] = *reinterpret_cast<const i32x4*>(kq + 8 * c);
         vr[c] = *reinterpret_cast<const i32x4*>(vq + 8 * c);
+      }
+      if constexpr (NR) {
+        const int64_t at = (b * a.S + pos - start) * D + d0;
+        norm_rope_quad<T>(kr, a.kw + d0, a.cs + at, a.sn + at, a.eps, tid & 3);
       }
     } else {
 #pragma unroll
@@ -112,15 +176,22 @@ template <typename T> __global__ __launch_bounds__(256) void kv8_append_kernel(C
       *reinterpret_cast<i32x4*>(cv + chunk * 16) = *reinterpret_cast<const i32x4*>(&vt[chunk >> 2][(chunk & 3) * 16]);
     }
   }
-  if (blockIdx.x != 0) return;
+  if (part != 0) return;
   // the last, unfinished block: every tail read above is done (the barriers), by this workgroup alone
   const int64_t pos = last * BLK + row;
   if (pos < start || pos >= end) return;
   const u16* kq = kp + (pos - start) * a.ks + d0;
   const u16* vq = vp + (pos - start) * a.vs + d0;
+  i32x4 kr[4];
+#pragma unroll
+  for (int c = 0; c < 4; ++c) kr[c] = *reinterpret_cast<const i32x4*>(kq + 8 * c);
+  if constexpr (NR) {
+    const int64_t at = (b * a.S + pos - start) * D + d0;
+    norm_rope_quad<T>(kr, a.kw + d0, a.cs + at, a.sn + at, a.eps, tid & 3);
+  }
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
-    *reinterpret_cast<i32x4*>(tk + row * D + d0 + 8 * c) = *reinterpret_cast<const i32x4*>(kq + 8 * c);
+    *reinterpret_cast<i32x4*>(tk + row * D + d0 + 8 * c) = kr[c];
     const i32x4 x = *reinterpret_cast<const i32x4*>(vq + 8 * c);
 #pragma unroll
     for (int p = 0; p < 4; ++p) {
@@ -198,6 +269,12 @@ bool cache_ok(const void* ck, const void* cv, const float* sk, const float* sv, 
          capacity > 0 && capacity < (1ll << 31) - 64;
 }
 
+// Workgroups per head: the blocks that the new positions complete, at least one (the tail's).
+int append_blocks(const CacheArgs& a) {
+  const int64_t whole = a.start_dev ? 1 : (a.start + a.S) / BLK - a.start / BLK;
+  return (int)(whole > 1 ? whole : 1);
+}
+
 template <typename T> int read_as(int out, const ReadArgs& a, dim3 g, hipStream_t s) {
   switch (out) {
     case Q3_F32: kv8_read_kernel<T, F32><<<g, 256, 0, s>>>(a); break;
@@ -219,13 +296,36 @@ int q3_kv8_append(int dtype, const void* k, int64_t ksb, int64_t kss, int64_t ks
   Q3_REQUIRE(cache_ok(cache_k, cache_v, scale_k, scale_v, tail_k, tail_v, B, H, capacity));
   Q3_REQUIRE(S > 0 && (start_dev ? S == 1 : (start >= 0 && start <= capacity && S <= capacity - start)));
   for (int64_t st : {ksb, kss, ksh, vsb, vss, vsh}) Q3_REQUIRE(st % 8 == 0);
-  const CacheArgs a{(const u16*)k, (const u16*)v, ksb, kss, ksh, vsb, vss, vsh, cache_k, cache_v, scale_k, scale_v,
-                    (u16*)tail_k, (u16*)tail_v, S, H, capacity, start, start_dev};
-  // whole blocks touched, at least one workgroup (the tail's)
-  const int64_t whole = start_dev ? 1 : (start + S) / BLK - start / BLK;
-  const dim3 g((unsigned)(whole > 1 ? whole : 1), (unsigned)H, (unsigned)B);
-  if (dtype == Q3_BF16) kv8_append_kernel<BF16><<<g, 256, 0, stream>>>(a);
-  else kv8_append_kernel<F16><<<g, 256, 0, stream>>>(a);
+  CacheArgs a{(const u16*)k, (const u16*)v, ksb, kss, ksh, vsb, vss, vsh, cache_k, cache_v, scale_k, scale_v,
+              (u16*)tail_k, (u16*)tail_v, S, H, capacity, start, start_dev};
+  a.B = B;
+  a.blocks = append_blocks(a);
+  Q3_REQUIRE(a.blocks * H * B < (1ll << 31));
+  const unsigned g = (unsigned)(a.blocks * H * B);
+  if (dtype == Q3_BF16) kv8_append_kernel<BF16, false><<<g, 256, 0, stream>>>(a);
+  else kv8_append_kernel<F16, false><<<g, 256, 0, stream>>>(a);
+  return (int)hipGetLastError();
+}
+
+int q3_kv8_norm_rope_append(int dtype, const void* q, int64_t qsb, int64_t qss, int64_t qsh, const void* k, int64_t ksb,
+                            int64_t kss, int64_t ksh, const void* v, int64_t vsb, int64_t vss, int64_t vsh, const void* wq,
+                            const void* wk, const void* cos, const void* sin, void* yq, int8_t* cache_k, int8_t* cache_v,
+                            float* scale_k, float* scale_v, void* tail_k, void* tail_v, int64_t B, int64_t S, int64_t Hq,
+                            int64_t H, int64_t d, int64_t capacity, int64_t start, const int64_t* start_dev, float eps,
+                            hipStream_t stream) {
+  Q3_REQUIRE((dtype == Q3_BF16 || dtype == Q3_F16) && d == D && al16(q) && al16(k) && al16(v) && al16(wq) && al16(wk) &&
+             al16(cos) && al16(sin) && al16(yq) && Hq > 0 && Hq < 65536 && eps >= 0.f);
+  Q3_REQUIRE(cache_ok(cache_k, cache_v, scale_k, scale_v, tail_k, tail_v, B, H, capacity));
+  Q3_REQUIRE(S > 0 && (start_dev ? S == 1 : (start >= 0 && start <= capacity && S <= capacity - start)));
+  for (int64_t st : {qsb, qss, qsh, ksb, kss, ksh, vsb, vss, vsh}) Q3_REQUIRE(st % 8 == 0);
+  CacheArgs a{(const u16*)k, (const u16*)v, ksb, kss, ksh, vsb, vss, vsh, cache_k, cache_v, scale_k, scale_v,
+              (u16*)tail_k, (u16*)tail_v, S, H, capacity, start, start_dev, (const u16*)q, (const u16*)wq, (const u16*)wk,
+              (const u16*)cos, (const u16*)sin, qsb, qss, qsh, (u16*)yq, B, Hq, 0, eps};
+  a.blocks = append_blocks(a);
+  const int64_t g = a.blocks * H * B + (B * S * Hq + 63) / 64;
+  Q3_REQUIRE(g < (1ll << 31));
+  if (dtype == Q3_BF16) kv8_append_kernel<BF16, true><<<(unsigned)g, 256, 0, stream>>>(a);
+  else kv8_append_kernel<F16, true><<<(unsigned)g, 256, 0, stream>>>(a);
   return (int)hipGetLastError();
 }
 

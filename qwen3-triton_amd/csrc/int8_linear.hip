@@ -6,13 +6,42 @@
 // operand; its 8 waves take 256-wide k blocks in turn, P of them in flight, and fold their int32 tiles in LDS: exact, so in
 // any order.
 #include "gemm_tile.h"
+#include "int8.h"
 
 namespace q3gemm {
 
-template <typename T, int EPI, int P> __global__ __launch_bounds__(512) void gemm_rows_q8_kernel(Args a) {
-  constexpr int NW = 8, NB = EPI == 3 ? 2 : 1;
+// Largest magnitude over a wave, every lane with the result.
+Q3_DEV uint32_t wave_umax(uint32_t x) {
+  auto dpp = [](uint32_t v, auto ctrl) {
+    const uint32_t y = (uint32_t)__builtin_amdgcn_mov_dpp((int)v, decltype(ctrl)::value, 0xF, 0xF, true);
+    return v > y ? v : y;
+  };
+  x = dpp(x, std::integral_constant<int, 0xB1>{});
+  x = dpp(x, std::integral_constant<int, 0x4E>{});
+  x = dpp(x, std::integral_constant<int, 0x141>{});
+  x = dpp(x, std::integral_constant<int, 0x140>{});
+#pragma unroll
+  for (int o = 16; o < 64; o <<= 1) {
+    const uint32_t y = (uint32_t)__shfl_xor((int)x, o, 64);
+    x = x > y ? x : y;
+  }
+  return x;
+}
+
+// What the rows are: their codes (R = 0), or R 16-bit rows that every workgroup turns into codes itself, in LDS, while its
+// first weights are on their way: quantize_rows, or with NORM rms_norm.  Each workgroup repeats that work on rows that sit
+// in L2; it saves a launch and its wait, and a decode step has one before each of its four products.  One row: 9.5 against
+// 12.1 us (6144 x 4096 after a norm), 14.7 against 16.6 (4096 x 12288); four rows: 13.9 against 13.8 and 20.9 against 18.5,
+// so it stops at two.
+// V: 16-byte pieces of a row per thread.
+template <typename T, int EPI, int P, int R, int V, bool NORM>
+__global__ __launch_bounds__(512) void gemm_rows_q8_kernel(Args a, RowIn in) {
+  constexpr int NW = 8, NB = EPI == 3 ? 2 : 1, PAD = 16;  // PAD: the rows of codes start in different banks
+  extern __shared__ __attribute__((aligned(16))) int8_t xs[];
   __shared__ i32x4 red[NW - 1][NB][64];
-  const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  __shared__ uint32_t red_m[NW][R ? R : 1];
+  __shared__ float red_s[NW][R ? R : 1], xscale[R ? R : 1];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, kq = lane >> 4;
   const int M = (int)a.M, K = (int)a.K * 2;  // codes
   int tile = blockIdx.x, s = 0;
@@ -30,31 +59,121 @@ template <typename T, int EPI, int P> __global__ __launch_bounds__(512) void gem
   i32x4 acc[NB];
 #pragma unroll
   for (int j = 0; j < NB; ++j) acc[j] = i32x4{0, 0, 0, 0};
-  auto blocks = [&](auto qc, int b) {  // k blocks b, b + NW, ...: every load before the first product
-    constexpr int Q = decltype(qc)::value;
-    i32x4 wv[Q][NB][4], xv[Q][4];
+  // 16-bit rows first in the queue, then the first weights behind them
+  [[maybe_unused]] i32x4 rv[R ? R : 1][V], nv[V];
+  if constexpr (R > 0) {
 #pragma unroll
-    for (int p = 0; p < Q; ++p)
+    for (int v = 0; v < V; ++v) {
+      const int at = min((v * 512 + tid) * 8, K - 8);
+#pragma unroll
+      for (int m = 0; m < R; ++m) rv[m][v] = *reinterpret_cast<const i32x4*>(in.x + (int64_t)min(m, M - 1) * in.ldx + at);
+      if constexpr (NORM) nv[v] = *reinterpret_cast<const i32x4*>(in.w + at);
+    }
+  }
+  const int nblk = (K + 255) / 256;
+  i32x4 wv[P][NB][4];
+  auto load = [&](int b) {  // k blocks b, b + NW, ..: P of them, zeros past the end
+#pragma unroll
+    for (int p = 0; p < P; ++p)
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
         const int k = (b + p * NW) * 256 + 64 * c;
-        const bool ok = k + 16 * kq < K;
 #pragma unroll
-        for (int j = 0; j < NB; ++j) wv[p][j][c] = ok ? *reinterpret_cast<const i32x4*>(w[j] + k) : i32x4{0, 0, 0, 0};
-        xv[p][c] = ok && live ? *reinterpret_cast<const i32x4*>(x + k) : i32x4{0, 0, 0, 0};
+        for (int j = 0; j < NB; ++j)
+          wv[p][j][c] = k + 16 * kq < K ? *reinterpret_cast<const i32x4*>(w[j] + k) : i32x4{0, 0, 0, 0};
+      }
+  };
+  int b = wave;
+  load(b);
+  if constexpr (R > 0) {
+    float ss[R];
+    uint32_t mb[R];
+#pragma unroll
+    for (int m = 0; m < R; ++m) {
+      ss[m] = 0.f;
+      mb[m] = 0;
+#pragma unroll
+      for (int v = 0; v < V; ++v) {
+        if ((v * 512 + tid) * 8 >= K) continue;
+        const Vec<T> xf = unpack_vec<T>(rv[m][v]);
+        Vec<T> wf;
+        if constexpr (NORM) wf = unpack_vec<T>(nv[v]);
+#pragma unroll
+        for (int e = 0; e < 8; ++e) {
+          if constexpr (NORM) ss[m] += xf.v[e] * xf.v[e];
+          const uint32_t y = mag_bits(NORM ? xf.v[e] * wf.v[e] : xf.v[e]);
+          mb[m] = mb[m] > y ? mb[m] : y;
+        }
+      }
+      mb[m] = wave_umax(mb[m]);
+      if constexpr (NORM) ss[m] = group_sum<64>(ss[m]);
+    }
+    if (lane == 0) {
+#pragma unroll
+      for (int m = 0; m < R; ++m) {
+        red_m[wave][m] = mb[m];
+        red_s[wave][m] = ss[m];
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14));  // lgkmcnt(0): the weights stay in flight
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+#pragma unroll
+    for (int m = 0; m < R; ++m) {
+      uint32_t top = red_m[0][m];
+      float sum = red_s[0][m];
+#pragma unroll
+      for (int i = 1; i < NW; ++i) {
+        top = top > red_m[i][m] ? top : red_m[i][m];
+        sum += red_s[i][m];
+      }
+      const bool finite = bits_finite(top);
+      const QuantStep st = quant_step(finite ? __uint_as_float(top) : 0.f);
+      if (tid == 0) {
+        float sc = finite ? st.m / 127.f : __uint_as_float(0x7fc00000u);
+        if constexpr (NORM) sc *= rsqrtf(sum * (1.f / (float)K) + in.eps);
+        xscale[m] = sc;
       }
 #pragma unroll
-    for (int p = 0; p < Q; ++p)
+      for (int v = 0; v < V; ++v) {
+        if ((v * 512 + tid) * 8 >= K) continue;
+        const Vec<T> xf = unpack_vec<T>(rv[m][v]);
+        Vec<T> wf;
+        if constexpr (NORM) wf = unpack_vec<T>(nv[v]);
+        float c[8];
+#pragma unroll
+        for (int e = 0; e < 8; ++e) c[e] = finite ? quant_code(NORM ? xf.v[e] * wf.v[e] : xf.v[e], st) : 0.f;
+        *reinterpret_cast<i32x2*>(xs + m * (K + PAD) + (v * 512 + tid) * 8) =
+            i32x2{pack_codes(c[0], c[1], c[2], c[3]), pack_codes(c[4], c[5], c[6], c[7])};
+      }
+    }
+    __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14));
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  }
+  const int8_t* xl = xs + min(r, R ? R - 1 : 0) * (K + PAD) + 16 * kq;
+  for (; b < nblk; b += P * NW) {
+    i32x4 xv[P][4];
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int k = (b + p * NW) * 256 + 64 * c;
+        const bool ok = live && k + 16 * kq < K;
+        if constexpr (R > 0) xv[p][c] = ok ? *reinterpret_cast<const i32x4*>(xl + k) : i32x4{0, 0, 0, 0};
+        else xv[p][c] = ok ? *reinterpret_cast<const i32x4*>(x + k) : i32x4{0, 0, 0, 0};
+      }
+#pragma unroll
+    for (int p = 0; p < P; ++p)
 #pragma unroll
       for (int c = 0; c < 4; ++c)
 #pragma unroll
         for (int j = 0; j < NB; ++j)
           mfma_acc(acc[j], __builtin_bit_cast(bf16x8_t, xv[p][c]), __builtin_bit_cast(bf16x8_t, wv[p][j][c]));
-  };
-  const int nblk = (K + 255) / 256;
-  int b = wave;
-  for (; b + (P - 1) * NW < nblk; b += P * NW) blocks(std::integral_constant<int, P>{}, b);
-  for (; b < nblk; b += NW) blocks(std::integral_constant<int, 1>{}, b);
+    if (b + P * NW < nblk) load(b + P * NW);
+  }
   if (wave > 0) {
 #pragma unroll
     for (int j = 0; j < NB; ++j) red[wave - 1][j][lane] = acc[j];
@@ -75,7 +194,7 @@ template <typename T, int EPI, int P> __global__ __launch_bounds__(512) void gem
   for (int e = 0; e < 4; ++e) {
     const int m = 4 * kq + e;
     if (m >= M) continue;
-    const float rs = a.rscale[m];
+    const float rs = R ? xscale[min(m, R ? R - 1 : 0)] : a.rscale[m];
     float v = (float)acc[0][e] * rs * cs;
     if constexpr (EPI == 3) v = v * q3_sigmoid(v) * ((float)acc[NB - 1][e] * rs * cu);
     else if (a.res) v += to_f32<T>(a.res[m * a.ldres + n]);
@@ -83,19 +202,32 @@ template <typename T, int EPI, int P> __global__ __launch_bounds__(512) void gem
   }
 }
 
-template <typename T> static int rows_q8(int epi, const Args& a, hipStream_t s) {
+template <typename T, int EPI, int R, int V, bool NORM>
+static int launch_rows(const Args& a, const RowIn& in, int64_t tiles, hipStream_t s) {
+  const size_t lds = R ? (size_t)R * (size_t)(2 * a.K + 16) : 0;
+  gemm_rows_q8_kernel<T, EPI, 2, R, V, NORM><<<(unsigned)tiles, 512, lds, s>>>(a, in);
+  return (int)hipGetLastError();
+}
+template <typename T, int EPI, int R>
+static int rows_of(const Args& a, const RowIn& in, int64_t tiles, hipStream_t s) {
+  const bool wide = a.K > 2048;  // more than 4096 codes: four pieces of a row per thread
+  if (in.w) return wide ? launch_rows<T, EPI, R, 4, true>(a, in, tiles, s) : launch_rows<T, EPI, R, 1, true>(a, in, tiles, s);
+  return wide ? launch_rows<T, EPI, R, 4, false>(a, in, tiles, s) : launch_rows<T, EPI, R, 1, false>(a, in, tiles, s);
+}
+template <typename T, int EPI> static int rows_q8(const Args& a, const RowIn& in, int64_t tiles, hipStream_t s) {
+  if (!in.x) return launch_rows<T, EPI, 0, 1, false>(a, in, tiles, s);
+  if (a.M == 1) return rows_of<T, EPI, 1>(a, in, tiles, s);
+  return rows_of<T, EPI, 2>(a, in, tiles, s);
+}
+
+int launch_rows_q8(int dtype, int epi, const Args& a, const RowIn& in, hipStream_t s) {
   int64_t tiles = 0;
   if (epi == 3) tiles = (a.N / 2 + 15) / 16;
   else if (a.axis == 2)
     for (int i = 0; i < a.pieces; ++i) tiles += (a.len[i] + 15) / 16;
   else tiles = (a.N + 15) / 16;
-  if (epi == 3) gemm_rows_q8_kernel<T, 3, 2><<<(unsigned)tiles, 512, 0, s>>>(a);
-  else gemm_rows_q8_kernel<T, 0, 2><<<(unsigned)tiles, 512, 0, s>>>(a);
-  return (int)hipGetLastError();
-}
-
-int launch_rows_q8(int dtype, int epi, const Args& a, hipStream_t s) {
-  return dtype == Q3_BF16 ? rows_q8<BF16>(epi, a, s) : rows_q8<F16>(epi, a, s);
+  if (epi == 3) return dtype == Q3_BF16 ? rows_q8<BF16, 3>(a, in, tiles, s) : rows_q8<F16, 3>(a, in, tiles, s);
+  return dtype == Q3_BF16 ? rows_q8<BF16, 0>(a, in, tiles, s) : rows_q8<F16, 0>(a, in, tiles, s);
 }
 
 }  // namespace q3gemm

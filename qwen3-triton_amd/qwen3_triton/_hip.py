@@ -126,8 +126,11 @@ SIGNATURES: dict[str, tuple] = {
     "q3_rmsnorm_quant": (_i32, [_i32, _p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _i64, _f32, _p]),
     "q3_gemm_int8_workspace_bytes": (_sz, [_p]),
     "q3_gemm_int8": (_i32, [_p, _p, _sz, _p]),
+    "q3_decode_linear_int8_ok": (_i32, [_i64, _i64]),
+    "q3_decode_linear_int8": (_i32, [_p, _p, _i64, _p, _f32, _p]),
     "q3_kv8_append": (_i32, [_i32, _p, _i64, _i64, _i64, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64,
                              _i64, _i64, _i64, _p, _p]),
+    "q3_kv8_norm_rope_append": (_i32, [_i32, *[_p, _i64, _i64, _i64] * 3, *[_p] * 11, *[_i64] * 7, _p, _f32, _p]),
     "q3_kv8_read": (_i32, [_i32, _i32, _p, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _i64, _i64, _p]),
     "q3_kv8_attention_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64]),
     "q3_kv8_attention": (_i32, [_i32, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _p, _sz, _i64,

@@ -120,16 +120,10 @@ def _check_weight(q, w, ws):
     return ld
 
 
-def _product(q, scale, weights, outs, epilogue, dtype, residual=None):
-    if dtype not in _FLOATS:
-        raise TypeError(f'a bfloat16 or float16 result required, not {dtype}')
-    _forward_only(residual)
-    rows, lda, k = _check_codes(q, scale)
+def _desc(q, rows, k, weights, outs, epilogue, dtype, residual):
+    """The product's descriptor without its left operand (``q``: the tensor that names the device and k)."""
     d = H.Int8GemmDesc()
     d.dtype, d.epilogue, d.m, d.k = H.code(dtype), epilogue, rows, k
-    d.a, d.lda, d.a_scale = q.data_ptr(), lda, scale.data_ptr()
-    if lda >= 1 << 23:
-        raise ValueError('rows of codes are too far apart')
     end = 0
     for i, (w, ws) in enumerate(weights):
         d.b[i], d.ldb[i], d.b_scale[i] = w.data_ptr(), _check_weight(q, w, ws), ws.data_ptr()
@@ -144,6 +138,18 @@ def _product(q, scale, weights, outs, epilogue, dtype, residual=None):
         if residual.shape != outs[0].shape or residual.dtype != dtype or not residual.is_contiguous():
             raise ValueError('a contiguous residual of the result\'s shape and dtype required')
         d.res, d.ldres = residual.data_ptr(), residual.shape[-1]
+    return d
+
+
+def _product(q, scale, weights, outs, epilogue, dtype, residual=None):
+    if dtype not in _FLOATS:
+        raise TypeError(f'a bfloat16 or float16 result required, not {dtype}')
+    _forward_only(residual)
+    rows, lda, k = _check_codes(q, scale)
+    if lda >= 1 << 23:
+        raise ValueError('rows of codes are too far apart')
+    d = _desc(q, rows, k, weights, outs, epilogue, dtype, residual)
+    d.a, d.lda, d.a_scale = q.data_ptr(), lda, scale.data_ptr()
     ref = ctypes.addressof(d)
     with torch.cuda.device(q.device):
         nbytes = H.query("q3_gemm_int8_workspace_bytes", ref)
@@ -181,6 +187,42 @@ def gate_up_swiglu(q, scale, gate, gate_scale, up, up_scale, *, dtype=torch.bflo
     y = _out(q, gate.shape[0], dtype)
     _product(q, scale, [(gate, gate_scale), (up, up_scale)], [y], H.GEMM_GATE_UP, dtype)
     return y
+
+
+def decode_linear_ok(x):
+    """Whether ``decode_linear`` takes rows like x [..., K]: at most 2, of at most 16384 values."""
+    k = x.shape[-1]
+    return bool(H.query("q3_decode_linear_int8_ok", x.numel() // k, k))
+
+
+def decode_linear(x, weights, *, norm_weight=None, eps=1e-6, gate_up=False, residual=None):
+    """A decode step's product straight from 16-bit rows x [..., K]: ``quantize_rows`` (with ``norm_weight`` ``rms_norm``) and
+    ``projections`` of up to three weights [(codes, scales), ...] in one launch -> a list; with ``gate_up`` the SwiGLU of
+    two -> one tensor; with ``residual`` [..., N] one weight's product plus it -> one tensor."""
+    _forward_only(x, norm_weight, residual)
+    rows, ld, k = _check_rows(x)
+    if not decode_linear_ok(x):
+        raise ValueError('decode_linear takes at most 2 rows of at most 16384 values')
+    if norm_weight is not None:
+        H.require_device(x, norm_weight)
+        if norm_weight.shape != (k,) or norm_weight.dtype != x.dtype or not norm_weight.is_contiguous() or \
+                norm_weight.data_ptr() % 16 or not float(eps) >= 0.0:
+            raise ValueError(f'a contiguous 16-byte aligned norm weight of {k} {x.dtype} values and a nonnegative eps required')
+    if gate_up:
+        if len(weights) != 2 or residual is not None or weights[0][0].shape != weights[1][0].shape or \
+                weights[0][0].stride() != weights[1][0].stride() or weights[0][0].shape[0] % 8:
+            raise ValueError('gate and up weights of one shape and layout, channels a multiple of 8, and no residual required')
+        outs, epilogue = [_out(x, weights[0][0].shape[0], x.dtype)], H.GEMM_GATE_UP
+    else:
+        if not 1 <= len(weights) <= (3 if residual is None else 1):
+            raise ValueError('one to three weights required, one with a residual')
+        outs = [_out(x, w.shape[0], x.dtype) for w, _ in weights]
+        epilogue = H.GEMM_PLAIN if residual is None else H.GEMM_RESIDUAL
+    d = _desc(x, rows, k, list(weights), outs, epilogue, x.dtype, residual)
+    with torch.cuda.device(x.device):
+        H.call("q3_decode_linear_int8", ctypes.addressof(d), x.data_ptr(), ld,
+               None if norm_weight is None else norm_weight.data_ptr(), float(eps), H.stream())
+    return outs[0] if gate_up or residual is not None else outs
 
 
 # ---------------------------------------------------------------- cache
@@ -293,8 +335,33 @@ def append(k, v, cache, start, start_dev=None):
                cache.capacity, start, None if start_dev is None else start_dev.data_ptr(), H.stream())
 
 
+def norm_rope_append(q, k, v, q_norm_weight, k_norm_weight, cos, sin, cache, start, start_dev=None, *, eps=1e-6):
+    """Per-head RMSNorm and rotation of q [B, S, Hq, 128] and k [B, S, Hkv, 128] as projected (tables cos, sin [B, S, 128])
+    and ``append`` of those keys and v, in one launch; returns the normed and rotated q, contiguous."""
+    _forward_only(q, k, v, q_norm_weight, k_norm_weight)
+    qs, ks, vs = (_check_heads(t, cache, what) for t, what in ((q, 'queries'), (k, 'keys'), (v, 'values')))
+    b, s, hq, d = q.shape
+    h = k.shape[2]
+    if v.shape != k.shape or k.shape[1] != s or h != cache.k.shape[1]:
+        raise ValueError('queries, keys and values of one batch and length, with the cache\'s heads, required')
+    for t, shape in ((q_norm_weight, (d,)), (k_norm_weight, (d,)), (cos, (b, s, d)), (sin, (b, s, d))):
+        H.require_device(q, t)
+        if t.shape != shape or t.dtype != q.dtype or not t.is_contiguous() or t.data_ptr() % 16:
+            raise ValueError(f'contiguous, 16-byte aligned {q.dtype} norm weights [128] and tables [B, S, 128] required')
+    if not float(eps) >= 0.0:
+        raise ValueError('a nonnegative eps required')
+    start = _check_span(start, s, cache, start_dev)
+    out = torch.empty((b, s, hq, d), device=q.device, dtype=q.dtype)
+    with torch.cuda.device(q.device):
+        H.call("q3_kv8_norm_rope_append", H.code(q.dtype), q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(), *vs,
+               q_norm_weight.data_ptr(), k_norm_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(), out.data_ptr(),
+               *cache.pointers(), b, s, hq, h, d, cache.capacity, start,
+               None if start_dev is None else start_dev.data_ptr(), float(eps), H.stream())
+    return out
+
+
 def read(cache, length, *, dtype=None):
-    """The first ``length`` positions back as k, v [B, Hkv, length, 128] in ``dtype`` (the tail's by default)."""
+    """The ``length`` positions that the cache holds back as k, v [B, Hkv, length, 128] in ``dtype`` (the tail's by default)."""
     b, h = cache.check()
     if type(length) is not int or not 1 <= length <= cache.capacity:
         raise ValueError(f'length must be an int in [1, {cache.capacity}]')
@@ -318,6 +385,8 @@ def attention(q, cache, start, start_dev=None, *, scale=None):
         raise ValueError('query heads must be a multiple of key/value heads')
     start = _check_span(start, s, cache, start_dev)
     scale = d ** -0.5 if scale is None else float(scale)
+    if not 0.0 < scale < 1e30:
+        raise ValueError('a positive softmax scale required')
     out = torch.empty((b, s, hq, d), device=q.device, dtype=q.dtype)
     with torch.cuda.device(q.device):
         nbytes = H.query("q3_kv8_attention_workspace_bytes", b, s, hq, hkv,

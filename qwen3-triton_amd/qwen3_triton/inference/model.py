@@ -273,6 +273,9 @@ class TritonQwen3Inference(nn.Module):
         b, s = q.shape[:2]
         d = a.head_dim
         in8 = isinstance(cache, Int8KVCache)
+        if not in8 and self._int8 is not None and s == 1 and a.q_norm.eps == a.k_norm.eps:
+            return kernels.decode_step_attention(q, k, v, a.q_norm.weight, a.k_norm.weight, a.q_norm.eps, cos, sin,
+                                                 cache.keys[i], cache.values[i], start, start_dev).reshape(b, s, -1)
         fits = a.q_norm.eps == a.k_norm.eps and _ops.norm_rope_qk_ok(q, k, d) and all(t.is_contiguous() for t in (q, k, v))
         if not in8 and start_dev is None and fits:
             # Q/K-norm + RoPE of both tensors and the K/V cache append in one launch
@@ -280,11 +283,12 @@ class TritonQwen3Inference(nn.Module):
                                             cache.values[i], start, a.q_norm.eps)
             return kernels.attention(q, cache.keys[i], cache.values[i], start,
                                      split_decode=self.split_decode).reshape(b, s, -1)
-        if in8 and fits:
-            q, k = _ops.norm_rope_qk_fwd(q, k, a.q_norm.weight, a.k_norm.weight, cos, sin, a.q_norm.eps)
-        else:
-            q = kernels.norm_rope(q, a.q_norm.weight, cos, sin, a.q_norm.eps)
-            k = kernels.norm_rope(k, a.k_norm.weight, cos, sin, a.k_norm.eps)
+        if in8 and a.q_norm.eps == a.k_norm.eps:
+            q = int8.norm_rope_append(q, k, v, a.q_norm.weight, a.k_norm.weight, cos, sin, cache.layers[i], start, start_dev,
+                                      eps=a.q_norm.eps)
+            return int8.attention(q, cache.layers[i], start, start_dev).reshape(b, s, -1)
+        q = kernels.norm_rope(q, a.q_norm.weight, cos, sin, a.q_norm.eps)
+        k = kernels.norm_rope(k, a.k_norm.weight, cos, sin, a.k_norm.eps)
         if in8:
             int8.append(k, v, cache.layers[i], start, start_dev)
             return int8.attention(q, cache.layers[i], start, start_dev).reshape(b, s, -1)
@@ -292,10 +296,27 @@ class TritonQwen3Inference(nn.Module):
         return kernels.attention(q, cache.keys[i], cache.values[i], start, split_decode=self.split_decode,
                                  start_dev=start_dev).reshape(b, s, -1)
 
+    def _int8_decode(self, x, cos, sin, cache, start, start_dev):
+        """The same for the one or two token rows of a decode step: norms and quantisation ride in the products, residual
+        sums in their epilogues."""
+        b, s, _ = x.shape
+        for i, (layer, w) in enumerate(zip(self.model.layers, self._int8)):
+            a, n1, n2 = layer.self_attn, layer.input_layernorm, layer.post_attention_layernorm
+            d = a.head_dim
+            q, k, v = int8.decode_linear(x, [w.q, w.k, w.v], norm_weight=n1.weight, eps=n1.eps)
+            y = self._cached_attention(a, q.view(b, s, a.num_heads, d), k.view(b, s, a.num_kv_heads, d),
+                                       v.view(b, s, a.num_kv_heads, d), cos, sin, cache, i, start, start_dev)
+            x = int8.decode_linear(y, [w.o], residual=x)
+            y = int8.decode_linear(x, [w.gate, w.up], norm_weight=n2.weight, eps=n2.eps, gate_up=True)
+            x = int8.decode_linear(y, [w.down], residual=x)
+        return x
+
     def _int8_layers(self, x, cos, sin, cache, start, start_dev):
         """The decoder layers on int8 weights: every projection's input is quantised where it is formed (the norms carry
         the residual sums)."""
         b, s, _ = x.shape
+        if int8.decode_linear_ok(x) and self.config.intermediate_size <= 16384:
+            return self._int8_decode(x, cos, sin, cache, start, start_dev)
         down = None
         for i, (layer, w) in enumerate(zip(self.model.layers, self._int8)):
             a, n1, n2 = layer.self_attn, layer.input_layernorm, layer.post_attention_layernorm

@@ -101,6 +101,20 @@ def test_product_refuses_a_short_workspace():
     assert H.load().q3_gemm_int8(ctypes.addressof(d), None, need, None) == INVALID
 
 
+def test_decode_product_refusals():
+    lib = H.load()
+
+    def call(d, x=P, ldx=128, w=None, eps=1e-6):
+        return lib.q3_decode_linear_int8(ctypes.addressof(d), x, ldx, w, eps, None)
+    assert call(gemm_desc(m=3)) == INVALID and call(gemm_desc(m=2, k=16400)) == INVALID and call(gemm_desc(m=2, k=120)) == INVALID
+    assert call(gemm_desc(m=1), x=None) == INVALID and call(gemm_desc(m=1), x=P + 2) == INVALID
+    assert call(gemm_desc(m=1), ldx=64) == INVALID and call(gemm_desc(m=1), ldx=132) == INVALID
+    assert call(gemm_desc(m=1), w=P + 2) == INVALID and call(gemm_desc(m=1), w=P, eps=-1.0) == INVALID
+    assert call(gemm_desc(m=1, b=(0, None))) == INVALID
+    assert [lib.q3_decode_linear_int8_ok(m, k) for m, k in ((0, 64), (1, 16), (2, 16384), (3, 64), (1, 24), (1, 16400), (1, 0))] == \
+        [0, 1, 1, 0, 0, 0, 0]
+
+
 def test_cache_refusals():
     lib = H.load()
     good = dict(dtype=2, k=P, ks=(1024, 256, 128), v=P, vs=(1024, 256, 128), ck=P, cv=P, sk=P, sv=P, tk=P, tv=P, B=1, S=4, Hh=2, d=128,
@@ -115,6 +129,16 @@ def test_cache_refusals():
                 dict(S=0), dict(Hh=0), dict(Hh=65536), dict(d=64), dict(cap=0), dict(cap=1 << 31), dict(start=-1), dict(start=61),
                 dict(start=1 << 62), dict(S=1 << 62), dict(S=2, dev=P)):
         assert append(**bad) == INVALID, bad
+
+    def fused(**kw):
+        a = {**good, 'q': P, 'qs': (1024, 256, 128), 'w': (P, P, P, P), 'y': P, 'Hq': 4, 'eps': 1e-6, **kw}
+        return lib.q3_kv8_norm_rope_append(a['dtype'], a['q'], *a['qs'], a['k'], *a['ks'], a['v'], *a['vs'], *a['w'], a['y'], a['ck'],
+                                           a['cv'], a['sk'], a['sv'], a['tk'], a['tv'], a['B'], a['S'], a['Hq'], a['Hh'], a['d'], a['cap'],
+                                           a['start'], a['dev'], a['eps'], None)
+    for bad in (dict(dtype=0), dict(q=None), dict(qs=(1024, 250, 128)), dict(w=(None, P, P, P)), dict(w=(P, P + 2, P, P)), dict(w=(P, P, None, P)),
+                dict(w=(P, P, P, P + 8)), dict(y=None), dict(y=P + 2), dict(Hq=0), dict(eps=-1.0), dict(k=None), dict(vs=(1024, 256, 100)),
+                dict(start=61), dict(S=2, dev=P), dict(d=64), dict(tk=None)):
+        assert fused(**bad) == INVALID, bad
 
     def read(**kw):
         a = {**good, 'out': 2, 'length': 10, **kw}
@@ -133,11 +157,12 @@ def test_attention_refusals():
     def attn(**kw):
         a = {**good, **kw}
         return lib.q3_kv8_attention(a['dtype'], a['q'], *a['qs'], a['ck'], a['cv'], a['sk'], a['sv'], a['tk'], a['tv'], a['o'], *a['os'],
-                                    a['ws'], a['wsb'], a['B'], a['S'], a['Hq'], a['Hkv'], a['d'], a['cap'], a['start'], a['dev'], 0.1, None)
+                                    a['ws'], a['wsb'], a['B'], a['S'], a['Hq'], a['Hkv'], a['d'], a['cap'], a['start'], a['dev'], a.get('scale', 0.1), None)
     for bad in (dict(dtype=0), dict(q=None), dict(q=P + 2), dict(qs=(1024, 1024, 124)), dict(ck=None), dict(cv=P + 8), dict(sk=None),
                 dict(sv=None), dict(tk=P + 2), dict(tv=None), dict(o=None), dict(o=P + 4), dict(os=(1024, 1022, 128)), dict(B=0), dict(B=65536),
                 dict(S=0), dict(Hq=1), dict(Hq=7), dict(Hkv=0), dict(B=8192, Hkv=8), dict(d=64), dict(cap=0), dict(cap=1 << 31), dict(start=-1),
-                dict(start=64), dict(S=65), dict(start=1 << 62), dict(S=2, dev=P), dict(cap=4096, start=4095, wsb=16), dict(cap=4096, start=4095, ws=None)):
+                dict(start=64), dict(S=65), dict(start=1 << 62), dict(S=2, dev=P), dict(cap=4096, start=4095, wsb=16), dict(cap=4096, start=4095, ws=None),
+                dict(scale=0.0), dict(scale=-1.0), dict(scale=float('nan')), dict(scale=float('inf'))):
         assert attn(**bad) == INVALID, bad
     assert lib.q3_kv8_attention_workspace_bytes(1, 1, 7, 2, 64) == 0 and lib.q3_kv8_attention_workspace_bytes(0, 1, 8, 2, 64) == 0
     # a captured step's workspace, sized for the capacity, holds every shorter span's

@@ -184,6 +184,44 @@ def test_gate_up_swiglu(m, n, k, dtype):
     close(y, ref, ref.abs() * rel + 1e-7)
 
 
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("norm", [False, True])
+@pytest.mark.parametrize("m,k", [(1, 16), (1, 4096), (2, 4096), (2, 528), (1, 4112), (1, 12288), (2, 12288), (2, 16384), (1, 8208)])
+def test_decode_linear(m, k, norm, dtype):
+    """One launch against quantize_rows / rms_norm and the product: the same codes, so the same bits but for the norm's scale,
+    whose sum of squares is taken in another order."""
+    gen = seeded(m + k)
+    x, nw = randn(m, k, gen=gen, dtype=dtype).cuda(), (1 + 0.1 * torch.randn(k, generator=gen)).to(dtype).cuda()
+    x[0, ::9] *= 20
+    ws = [I8.quantize_rows(randn(n, k, gen=gen, dtype=dtype, scale=0.05).cuda()) for n in (100, 40, 24, 100)]
+    res = randn(m, 100, gen=gen, dtype=dtype).cuda()
+    kw = dict(norm_weight=nw, eps=1e-6) if norm else {}
+    q, s = I8.rms_norm(x, nw, 1e-6) if norm else I8.quantize_rows(x)
+    pairs = list(zip(I8.decode_linear(x, ws[:3], **kw), I8.projections(q, s, ws[:3], dtype=dtype)))
+    pairs.append((I8.decode_linear(x, ws[:1], residual=res, **kw), I8.linear(q, s, *ws[0], dtype=dtype, residual=res)))
+    even = [(w[:96], t[:96].contiguous()) for w, t in (ws[0], ws[3])]
+    pairs.append((I8.decode_linear(x, even, gate_up=True, **kw), I8.gate_up_swiglu(q, s, *even[0], *even[1], dtype=dtype)))
+    for got, want in pairs:
+        if norm:   # one output rounding apart where the scales differ in their last bits (sums below 2^-17 apart)
+            ref = want.double().cpu()
+            close(got, ref, ref.abs() * torch.finfo(dtype).eps * (1 + 2.0 ** -8) + 2.0 ** -16)
+        else:
+            assert torch.equal(got, want)
+
+
+def test_decode_linear_refusals_and_nonfinite_rows():
+    x = randn(3, 64, gen=seeded(1), dtype=torch.bfloat16).cuda()
+    w = I8.quantize_rows(randn(32, 64, gen=seeded(2), dtype=torch.bfloat16).cuda())
+    for bad in (lambda: I8.decode_linear(x, [w]), lambda: I8.decode_linear(x[:1], [w] * 4), lambda: I8.decode_linear(x[:1], []),
+                lambda: I8.decode_linear(x[:1], [w, w, w], gate_up=True), lambda: I8.decode_linear(x[:1], [w, w], residual=x[:1, :32]),
+                lambda: I8.decode_linear(x[:1, :48], [w]), lambda: I8.decode_linear(x[:1], [w], norm_weight=x[0, :32])):
+        with pytest.raises(ValueError):
+            bad()
+    x[1, 5] = math.nan
+    y, = I8.decode_linear(x[:2], [w])
+    assert torch.isnan(y[1]).all() and torch.equal(y[:1], I8.decode_linear(x[:1], [w])[0])
+
+
 def test_linear_strided_and_last_columns_untouched():
     gen = seeded(9)
     q, s, w, ws = product_inputs(20, 40, 256, gen)
@@ -282,6 +320,60 @@ def test_append_strided_sources_and_nonfinite_block():
     assert torch.isnan(rk[0, 1, 64:128]).all() and torch.equal(rv, I8.read(d, s)[1])
     rk[0, 1, 64:128] = I8.read(d, s)[0][0, 1, 64:128]
     assert torch.equal(rk, I8.read(d, s)[0])
+
+
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("b,hq,h,cuts", [(1, 4, 1, (1, 2)), (2, 8, 2, (70, 71, 130)), (3, 5, 5, (64, 65, 128)), (1, 32, 8, (200, 201))])
+def test_norm_rope_append(b, hq, h, cuts, dtype):
+    """Norm + rotation + append in chunks: the keys within their roundings of 64 bits, and the cache bit for bit that of the
+    same keys appended; whatever the chunks."""
+    gen = seeded(sum(cuts))
+    t = cuts[-1]
+    qkv = randn(b, t, hq + 2 * h, 128, gen=gen, dtype=dtype)
+    wq, wk = ((1 + 0.1 * torch.randn(128, generator=gen)).to(dtype) for _ in range(2))
+    ang = torch.rand(b, t, 64, generator=gen) * 6.28
+    cos, sin = (torch.cat([f(ang)] * 2, -1).to(dtype) for f in (torch.cos, torch.sin))
+    dev = qkv.cuda()
+
+    def ref(x, w):
+        x = x.double()
+        n = x / (x.square().mean(-1, keepdim=True) + 1e-6).sqrt() * w.double()
+        rot = torch.cat([-n[..., 64:], n[..., :64]], -1)
+        c, s = cos.double()[:, :, None], sin.double()[:, :, None]
+        return n * c + rot * s, n.abs() * c.abs() + rot.abs() * s.abs()
+
+    def run(cuts):
+        c, qs, at = poisoned(b, h, t + 64, dtype), [], 0
+        for end in cuts:
+            part = dev[:, at:end]
+            qs.append(I8.norm_rope_append(part[:, :, :hq], part[:, :, hq:hq + h], part[:, :, hq + h:], wq.cuda(), wk.cuda(),
+                                          cos[:, at:end].contiguous().cuda(), sin[:, at:end].contiguous().cuda(), c, at))
+            at = end
+        return c, torch.cat(qs, 1)
+    c, q = run(cuts)
+    want, mag = ref(qkv[:, :, :hq], wq)
+    # the norm: a sum of 128 squares, rsqrt, two products; the rotation: two products and a sum
+    close(q, want, want.abs() * torch.finfo(dtype).eps / 2 * (1 + 2.0 ** -8) + mag * 2.0 ** -19 + 2.0 ** -24)
+    whole, qw = run((t,))
+    assert torch.equal(q, qw)
+    # the keys as 16-bit numbers: those of a cache that never fills a block
+    keys = []
+    for at in range(0, t, 63):
+        d, end = poisoned(b, h, 64, dtype), min(t, at + 63)
+        part = dev[:, at:end]
+        I8.norm_rope_append(part[:, :, :hq], part[:, :, hq:hq + h], part[:, :, hq + h:], wq.cuda(), wk.cuda(),
+                            cos[:, at:end].contiguous().cuda(), sin[:, at:end].contiguous().cuda(), d, 0)
+        keys.append(d.k_tail[:, :, :end - at].transpose(1, 2))
+    k = torch.cat(keys, 1)
+    want, mag = ref(qkv[:, :, hq:hq + h], wk)
+    close(k, want, want.abs() * torch.finfo(dtype).eps / 2 * (1 + 2.0 ** -8) + mag * 2.0 ** -19 + 2.0 ** -24)
+    plain = poisoned(b, h, t + 64, dtype)
+    I8.append(k, dev[:, :, hq + h:], plain, 0)
+    n, rest = t // 64, t % 64
+    for x in (c, whole):
+        assert torch.equal(x.k, plain.k) and torch.equal(x.v, plain.v)
+        assert torch.equal(x.k_scale[:, :, :n], plain.k_scale[:, :, :n]) and torch.equal(x.v_scale[:, :, :n], plain.v_scale[:, :, :n])
+        assert torch.equal(x.k_tail[:, :, :rest], plain.k_tail[:, :, :rest]) and torch.equal(x.v_tail[..., :rest], plain.v_tail[..., :rest])
 
 
 # ---------------------------------------------------------------- attention
