@@ -1,0 +1,195 @@
+// The key/value cache in 8 bits: its arguments and the writing of new positions, shared by the append kernel and the decode
+// step's attention.
+//
+// Blocks of 64 positions with one scale per block and key/value head for the keys and one for the values.  A block is
+// quantised once, from the 16-bit values, when its last position is written; until then its positions stay as they are in
+// the tail.  So the stored codes do not depend on how a prompt was cut into chunks, no value is rounded twice, and the newest
+// tokens are exact.  Layout per layer (Cb = capacity / 64 blocks, rounded up):
+//   k [B, H, 64 Cb, 128] int8    v [B, H, Cb, 128, 64] int8: transposed within a block, so that the products of the
+//   attention read 16-byte fragments of both as they lie    k_scale, v_scale [B, H, Cb] fp32
+//   k_tail [B, H, 64, 128]    v_tail [B, H, 128, 64] in the activation type: position p at slot p % 64.
+#pragma once
+#include "int8.h"
+
+namespace q3kv8 {
+
+constexpr int D = 128, BLK = 64;
+
+struct CacheArgs {
+  const u16 *k, *v;                // new tokens [B, S, H, D]
+  int64_t kb, ks, kh, vb, vs, vh;  // element strides (batch, position, head)
+  int8_t *ck, *cv;
+  float *sk, *sv;
+  u16 *tk, *tv;
+  int64_t S, H, capacity, start;
+  const int64_t* start_dev;
+  // with the Q/K-norm and rotation: k as projected, and the query rows beside it
+  const u16 *q, *qw, *kw, *cs, *sn;  // q [B, S, Hq, D], norm weights [D], tables [B, S, D]
+  int64_t qb, qs, qh;
+  u16* yq;  // [B, S, Hq, D]
+  int64_t B, Hq;
+  int blocks;  // workgroups per head and batch row of the cache's part
+  float eps;
+};
+
+// RMSNorm and split-half rotation of a 128-dim row whose dims 8 i .. + 7 sit in lane i of an aligned 16 (the partner dims, 64
+// away, in lane i ^ 8), rounded once.
+template <typename T>
+Q3_DEV i32x4 norm_rope16(i32x4 x, const u16* w, const u16* cs, const u16* sn, float eps, int i) {
+  const Vec<T> f = unpack_vec<T>(x), wf = load_vec<T>(w), cf = load_vec<T>(cs), sf = load_vec<T>(sn);
+  float ss = 0.f;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) ss += f.v[e] * f.v[e];
+  const float inv = rsqrtf(group_sum<16>(ss) * (1.f / (float)D) + eps), sign = i < 8 ? -1.f : 1.f;
+  Vec<T> y;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    const float n = f.v[e] * inv * wf.v[e];
+    const float o = __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, n), 0x128, 0xF, 0xF, true));
+    y.v[e] = fmaf(n, cf.v[e], sign * (o * sf.v[e]));
+  }
+  i32x4 r;
+#pragma unroll
+  for (int p = 0; p < 4; ++p) r[p] = (int)pack2<T>(y.v[2 * p], y.v[2 * p + 1]);
+  return r;
+}
+
+// LDS image of a block's V codes, transposed: word (d, r) holds the codes of dim d at positions 4 r .. + 3.  Dims of one lane
+// group 16 words apart, lane groups 144, and r permuted by the group: the 64 words that a wave writes (or reads) for one dim
+// per lane, and the 16-byte pieces of a dim, touch every bank once.
+constexpr int kVWords = 16 * 144;
+Q3_DEV int vword(int d, int r) { return (d >> 3) * 144 + (d & 7) * 16 + (r ^ (4 * (d >> 5))); }
+
+// The new positions start .. end - 1 as far as block `part` (counted from the first one touched) goes; part 0 also writes the
+// last, unfinished block's into the tail, after it has read the tail, which may hold the first block's positions in the same
+// slots.  256 threads: thread t owns positions 4 (t / 16) .. + 3 of the block and dims 8 (t % 16) .. + 7.
+// NR: the keys come as projected and are normed and rotated here.
+template <typename T, bool NR>
+Q3_DEV void append_part(const CacheArgs& a, int part, int h, int b, int64_t start) {
+  __shared__ __attribute__((aligned(16))) int vt[kVWords];
+  __shared__ uint32_t red[2][4];
+  const int tid = threadIdx.x, r = tid >> 4, i = tid & 15;
+  const int64_t end = min(start + a.S, a.capacity);
+  if (start < 0 || end <= start) return;
+  const int64_t first = start / BLK, last = end / BLK;  // last: the first block that is not whole
+  const int64_t blk = first + part;
+  const int64_t bh = (int64_t)b * a.H + h, cblocks = (a.capacity + BLK - 1) / BLK;
+  u16* tk = a.tk + bh * (BLK * D);
+  u16* tv = a.tv + bh * (BLK * D);
+  const u16* kp = a.k + b * a.kb + h * a.kh + 8 * i;
+  const u16* vp = a.v + b * a.vb + h * a.vh;
+  auto key = [&](int64_t pos) {  // a new position's 8 dims
+    i32x4 x = *reinterpret_cast<const i32x4*>(kp + (pos - start) * a.ks);
+    if constexpr (NR) {
+      const int64_t at = (b * a.S + pos - start) * D + 8 * i;
+      x = norm_rope16<T>(x, a.kw + 8 * i, a.cs + at, a.sn + at, a.eps, i);
+    }
+    return x;
+  };
+  if (blk < last) {
+    const int64_t pos0 = blk * BLK;
+    const bool mixed = pos0 < start;  // positions before start are in the tail, V's transposed already
+    i32x4 kr[4], vr[4];
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const int64_t pos = pos0 + 4 * r + c;
+      if (pos >= start) kr[c] = key(pos);
+      else kr[c] = *reinterpret_cast<const i32x4*>(tk + (4 * r + c) * D + 8 * i);
+    }
+    const int d = tid >> 1, half = (tid & 1) * 32;  // mixed: V of dim d, slots half .. + 31
+    if (mixed) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) vr[c] = *reinterpret_cast<const i32x4*>(tv + d * BLK + half + 8 * c);
+      const int from = (int)(start - pos0);
+      if (from < half + 32) {
+#pragma unroll
+        for (int e = 0; e < 32; ++e)
+          if (half + e >= from) {
+            const uint32_t x = vp[(pos0 + half + e - start) * a.vs + d];
+            const uint32_t w = (uint32_t)vr[e >> 3][(e >> 1) & 3];
+            vr[e >> 3][(e >> 1) & 3] = (int)((e & 1) ? (w & 0xffffu) | (x << 16) : (w & 0xffff0000u) | x);
+          }
+      }
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) vr[c] = *reinterpret_cast<const i32x4*>(vp + (pos0 + 4 * r + c - start) * a.vs + 8 * i);
+    }
+    uint32_t mk = 0, mv = 0;
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const Vec<T> x = unpack_vec<T>(kr[c]), y = unpack_vec<T>(vr[c]);
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        mk = max(mk, mag_bits(x.v[e]));
+        mv = max(mv, mag_bits(y.v[e]));
+      }
+    }
+    mk = group_umax<64>(mk);
+    mv = group_umax<64>(mv);
+    if ((tid & 63) == 0) {
+      red[0][tid >> 6] = mk;
+      red[1][tid >> 6] = mv;
+    }
+    __syncthreads();
+    mk = max(max(red[0][0], red[0][1]), max(red[0][2], red[0][3]));
+    mv = max(max(red[1][0], red[1][1]), max(red[1][2], red[1][3]));
+    const bool fk = bits_finite(mk), fv = bits_finite(mv);
+    const QuantStep sk = quant_step(fk ? __uint_as_float(mk) : 0.f), sv = quant_step(fv ? __uint_as_float(mv) : 0.f);
+    if (tid == 0) {
+      const float nan = __uint_as_float(0x7fc00000u);
+      a.sk[bh * cblocks + blk] = fk ? sk.m / 127.f : nan;
+      a.sv[bh * cblocks + blk] = fv ? sv.m / 127.f : nan;
+    }
+    i32x2 vc[4];  // codes of the thread's V values, in the order of vr
+#pragma unroll
+    for (int c = 0; c < 4; ++c) {
+      const Vec<T> x = unpack_vec<T>(kr[c]), y = unpack_vec<T>(vr[c]);
+      float p[8], q[8];
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        p[e] = fk ? quant_code(x.v[e], sk) : 0.f;
+        q[e] = fv ? quant_code(y.v[e], sv) : 0.f;
+      }
+      *reinterpret_cast<i32x2*>(a.ck + (bh * cblocks * BLK + pos0 + 4 * r + c) * D + 8 * i) =
+          i32x2{pack_codes(p[0], p[1], p[2], p[3]), pack_codes(p[4], p[5], p[6], p[7])};
+      vc[c] = i32x2{pack_codes(q[0], q[1], q[2], q[3]), pack_codes(q[4], q[5], q[6], q[7])};
+    }
+    int8_t* cv = a.cv + (bh * cblocks + blk) * (D * BLK);
+    if (mixed) {
+      *reinterpret_cast<i32x4*>(cv + d * BLK + half) = i32x4{vc[0][0], vc[0][1], vc[1][0], vc[1][1]};
+      *reinterpret_cast<i32x4*>(cv + d * BLK + half + 16) = i32x4{vc[2][0], vc[2][1], vc[3][0], vc[3][1]};
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {  // 4 positions of one dim to a word
+        const int w = e >> 2, s = 8 * (e & 3);
+        uint32_t x = 0;
+#pragma unroll
+        for (int c = 0; c < 4; ++c) x |= (((uint32_t)vc[c][w] >> s) & 0xffu) << (8 * c);
+        vt[vword(8 * i + e, r)] = (int)x;
+      }
+      __syncthreads();
+#pragma unroll
+      for (int c = 0; c < 2; ++c) {
+        const int chunk = tid + 256 * c, vd = chunk >> 2, q = chunk & 3;  // dim, positions 16 q .. + 15
+        *reinterpret_cast<i32x4*>(cv + chunk * 16) = *reinterpret_cast<const i32x4*>(&vt[vword(vd, 4 * q)]);
+      }
+    }
+  }
+  if (part != 0) return;
+  // the last, unfinished block: every tail read above is done (the barrier), by this workgroup alone
+#pragma unroll
+  for (int c = 0; c < 4; ++c) {
+    const int slot = 4 * r + c;
+    const int64_t pos = last * BLK + slot;
+    if (pos < start || pos >= end) continue;
+    *reinterpret_cast<i32x4*>(tk + slot * D + 8 * i) = key(pos);
+    const i32x4 x = *reinterpret_cast<const i32x4*>(vp + (pos - start) * a.vs + 8 * i);
+#pragma unroll
+    for (int p = 0; p < 4; ++p) {
+      tv[(8 * i + 2 * p) * BLK + slot] = (u16)((uint32_t)x[p] & 0xffffu);
+      tv[(8 * i + 2 * p + 1) * BLK + slot] = (u16)((uint32_t)x[p] >> 16);
+    }
+  }
+}
+
+}  // namespace q3kv8

@@ -1,204 +1,30 @@
-// The key/value cache in 8 bits: blocks of 64 positions with one scale per block and key/value head for the keys and one
-// for the values, written as tokens come and read back to 16 or 32 bits.
-//
-// A block is quantised once, from the 16-bit values, when its last position is written; until then its positions stay as
-// they are in the tail.  So the stored codes do not depend on how a prompt was cut into chunks, no value is rounded twice,
-// and the newest tokens are exact.  Layout per layer (Cb = capacity / 64 blocks, rounded up):
-//   k [B, H, 64 Cb, 128] int8    v [B, H, Cb, 128, 64] int8: transposed within a block, so that the products of the
-//   attention read 16-byte fragments of both as they lie    k_scale, v_scale [B, H, Cb] fp32
-//   k_tail [B, H, 64, 128]    v_tail [B, H, 128, 64] in the activation type: position p at slot p % 64.
-// Both kernels are bound by HBM (a prompt's 2 + 1 bytes per value), by latency at one token.
-#include "int8.h"
+// Writing new positions into the key/value cache in 8 bits (int8_cache.h), and reading the cache back to 16 or 32 bits.
+// Bound by HBM (a prompt's 2 + 1 bytes per value, and back), by latency at one token.
+#include "int8_cache.h"
 
 namespace {
 
-constexpr int D = 128, BLK = 64;
+using namespace q3kv8;
 
-struct CacheArgs {
-  const u16 *k, *v;              // new tokens [B, S, H, D]
-  int64_t kb, ks, kh, vb, vs, vh;  // element strides (batch, position, head)
-  int8_t *ck, *cv;
-  float *sk, *sv;
-  u16 *tk, *tv;
-  int64_t S, H, capacity, start;
-  const int64_t* start_dev;
-  // with the Q/K-norm and rotation: k as projected, and the query rows beside it
-  const u16 *q, *qw, *kw, *cs, *sn;  // q [B, S, Hq, D], norm weights [D], tables [B, S, D]
-  int64_t qb, qs, qh;
-  u16* yq;  // [B, S, Hq, D]
-  int64_t B, Hq;
-  int blocks;  // workgroups per head and batch row of the cache's part
-  float eps;
-};
-
-// RMSNorm and split-half rotation of a 128-dim row whose dims 32 i .. + 31 sit in lane i of an aligned quad (the partner
-// dims, 64 away, in lane i ^ 2), rounded once: x holds 32 16-bit values.
-template <typename T>
-Q3_DEV void norm_rope_quad(i32x4 (&x)[4], const u16* w, const u16* cs, const u16* sn, float eps, int quarter) {
-  Vec<T> f[4];
-  float ss = 0.f;
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    f[c] = unpack_vec<T>(x[c]);
-#pragma unroll
-    for (int e = 0; e < 8; ++e) ss += f[c].v[e] * f[c].v[e];
-  }
-  ss = group_sum<4>(ss);
-  const float inv = rsqrtf(ss * (1.f / (float)D) + eps), sign = quarter < 2 ? -1.f : 1.f;
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    const Vec<T> wf = load_vec<T>(w + 8 * c), cf = load_vec<T>(cs + 8 * c), sf = load_vec<T>(sn + 8 * c);
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      float y[2];
-#pragma unroll
-      for (int h = 0; h < 2; ++h) {
-        const int e = 2 * p + h;
-        const float n = f[c].v[e] * inv * wf.v[e];
-        const float o = __builtin_bit_cast(float, __builtin_amdgcn_mov_dpp(__builtin_bit_cast(int, n), 0x4E, 0xF, 0xF, true));
-        y[h] = n * cf.v[e] + sign * o * sf.v[e];
-      }
-      x[c][p] = (int)pack2<T>(y[0], y[1]);
-    }
-  }
-}
-
-// One workgroup per (touched block, head, batch row); the one of the first block also writes the last, unfinished block's
-// new positions into the tail (after it has read the tail, which may hold the first block's positions in the same slots).
-// Thread t owns position t / 4 of the block and dims 32 (t % 4) .. + 31.
-// NR: the rows come as projected and are normed and rotated here (values as they are); the workgroups behind the cache's
-// take the query rows, 64 each.
+// One workgroup per (touched block, head, batch row); with the norm and rotation, the ones behind them take 16 query rows each.
 template <typename T, bool NR> __global__ __launch_bounds__(256) void kv8_append_kernel(CacheArgs a) {
-  __shared__ uint32_t red[2][4];
-  __shared__ __attribute__((aligned(16))) int8_t vt[D][BLK + 16];
-  const int tid = threadIdx.x, row = tid >> 2, d0 = (tid & 3) * 32;
   int64_t job = blockIdx.x;
   if constexpr (NR) {
     const int64_t cache_jobs = a.blocks * a.H * a.B;
     if (job >= cache_jobs) {
-      const int64_t i = (job - cache_jobs) * 64 + row, n = a.B * a.S * a.Hq;  // whole quads: row is a quad's
-      if (i >= n) return;
-      const int64_t bs = i / a.Hq, qh = i - bs * a.Hq, qb = bs / a.S, qs = bs - qb * a.S;
-      const u16* p = a.q + qb * a.qb + qs * a.qs + qh * a.qh + d0;
-      i32x4 x[4];
-#pragma unroll
-      for (int c = 0; c < 4; ++c) x[c] = *reinterpret_cast<const i32x4*>(p + 8 * c);
-      norm_rope_quad<T>(x, a.qw + d0, a.cs + bs * D + d0, a.sn + bs * D + d0, a.eps, tid & 3);
-#pragma unroll
-      for (int c = 0; c < 4; ++c) *reinterpret_cast<i32x4*>(a.yq + i * D + d0 + 8 * c) = x[c];
+      const int tid = threadIdx.x, i = tid & 15;
+      const int64_t at = (job - cache_jobs) * 16 + (tid >> 4);  // a 16-lane row's query
+      if (at >= a.B * a.S * a.Hq) return;
+      const int64_t bs = at / a.Hq, qh = at - bs * a.Hq, qb = bs / a.S, qs = bs - qb * a.S;
+      const i32x4 x = *reinterpret_cast<const i32x4*>(a.q + qb * a.qb + qs * a.qs + qh * a.qh + 8 * i);
+      *reinterpret_cast<i32x4*>(a.yq + at * D + 8 * i) =
+          norm_rope16<T>(x, a.qw + 8 * i, a.cs + bs * D + 8 * i, a.sn + bs * D + 8 * i, a.eps, i);
       return;
     }
   }
   const int part = (int)(job % a.blocks);
   job /= a.blocks;
-  const int h = (int)(job % a.H), b = (int)(job / a.H);
-  const int64_t start = a.start_dev ? *a.start_dev : a.start;
-  const int64_t end = min(start + a.S, a.capacity);
-  if (start < 0 || end <= start) return;
-  const int64_t first = start / BLK, last = end / BLK;  // last: the first block that is not whole
-  const int64_t blk = first + part;
-  const int64_t bh = (int64_t)b * a.H + h, cblocks = (a.capacity + BLK - 1) / BLK;
-  u16* tk = a.tk + bh * (BLK * D);
-  u16* tv = a.tv + bh * (BLK * D);
-  const u16* kp = a.k + b * a.kb + h * a.kh;
-  const u16* vp = a.v + b * a.vb + h * a.vh;
-  if (blk < last) {
-    const int64_t pos = blk * BLK + row;
-    i32x4 kr[4], vr[4];
-    if (pos >= start) {
-      const u16* kq = kp + (pos - start) * a.ks + d0;
-      const u16* vq = vp + (pos - start) * a.vs + d0;
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        kr[c] = *reinterpret_cast<const i32x4*>(kq + 8 * c);
-        vr[c] = *reinterpret_cast<const i32x4*>(vq + 8 * c);
-      }
-      if constexpr (NR) {
-        const int64_t at = (b * a.S + pos - start) * D + d0;
-        norm_rope_quad<T>(kr, a.kw + d0, a.cs + at, a.sn + at, a.eps, tid & 3);
-      }
-    } else {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        kr[c] = *reinterpret_cast<const i32x4*>(tk + row * D + d0 + 8 * c);
-#pragma unroll
-        for (int p = 0; p < 4; ++p)
-          vr[c][p] = (int)((uint32_t)tv[(d0 + 8 * c + 2 * p) * BLK + row] |
-                           ((uint32_t)tv[(d0 + 8 * c + 2 * p + 1) * BLK + row] << 16));
-      }
-    }
-    uint32_t mk = 0, mv = 0;
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const Vec<T> x = unpack_vec<T>(kr[c]), y = unpack_vec<T>(vr[c]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        mk = max(mk, mag_bits(x.v[e]));
-        mv = max(mv, mag_bits(y.v[e]));
-      }
-    }
-    mk = group_umax<64>(mk);
-    mv = group_umax<64>(mv);
-    if ((tid & 63) == 0) {
-      red[0][tid >> 6] = mk;
-      red[1][tid >> 6] = mv;
-    }
-    __syncthreads();
-    mk = max(max(red[0][0], red[0][1]), max(red[0][2], red[0][3]));
-    mv = max(max(red[1][0], red[1][1]), max(red[1][2], red[1][3]));
-    const bool fk = bits_finite(mk), fv = bits_finite(mv);
-    const QuantStep sk = quant_step(fk ? __uint_as_float(mk) : 0.f), sv = quant_step(fv ? __uint_as_float(mv) : 0.f);
-    if (tid == 0) {
-      const float nan = __uint_as_float(0x7fc00000u);
-      a.sk[bh * cblocks + blk] = fk ? sk.m / 127.f : nan;
-      a.sv[bh * cblocks + blk] = fv ? sv.m / 127.f : nan;
-    }
-    int kc[8];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const Vec<T> x = unpack_vec<T>(kr[c]), y = unpack_vec<T>(vr[c]);
-      float q[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) q[e] = fk ? quant_code(x.v[e], sk) : 0.f;
-      kc[2 * c] = pack_codes(q[0], q[1], q[2], q[3]);
-      kc[2 * c + 1] = pack_codes(q[4], q[5], q[6], q[7]);
-#pragma unroll
-      for (int e = 0; e < 8; ++e) vt[d0 + 8 * c + e][row] = (int8_t)(fv ? (int)quant_code(y.v[e], sv) : 0);
-    }
-    int8_t* ck = a.ck + (bh * cblocks * BLK + pos) * D + d0;
-    *reinterpret_cast<i32x4*>(ck) = i32x4{kc[0], kc[1], kc[2], kc[3]};
-    *reinterpret_cast<i32x4*>(ck + 16) = i32x4{kc[4], kc[5], kc[6], kc[7]};
-    __syncthreads();
-    int8_t* cv = a.cv + (bh * cblocks + blk) * (D * BLK);
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int chunk = tid + 256 * i;  // dim chunk / 4, positions 16 (chunk % 4) .. + 15
-      *reinterpret_cast<i32x4*>(cv + chunk * 16) = *reinterpret_cast<const i32x4*>(&vt[chunk >> 2][(chunk & 3) * 16]);
-    }
-  }
-  if (part != 0) return;
-  // the last, unfinished block: every tail read above is done (the barriers), by this workgroup alone
-  const int64_t pos = last * BLK + row;
-  if (pos < start || pos >= end) return;
-  const u16* kq = kp + (pos - start) * a.ks + d0;
-  const u16* vq = vp + (pos - start) * a.vs + d0;
-  i32x4 kr[4];
-#pragma unroll
-  for (int c = 0; c < 4; ++c) kr[c] = *reinterpret_cast<const i32x4*>(kq + 8 * c);
-  if constexpr (NR) {
-    const int64_t at = (b * a.S + pos - start) * D + d0;
-    norm_rope_quad<T>(kr, a.kw + d0, a.cs + at, a.sn + at, a.eps, tid & 3);
-  }
-#pragma unroll
-  for (int c = 0; c < 4; ++c) {
-    *reinterpret_cast<i32x4*>(tk + row * D + d0 + 8 * c) = kr[c];
-    const i32x4 x = *reinterpret_cast<const i32x4*>(vq + 8 * c);
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      tv[(d0 + 8 * c + 2 * p) * BLK + row] = (u16)((uint32_t)x[p] & 0xffffu);
-      tv[(d0 + 8 * c + 2 * p + 1) * BLK + row] = (u16)((uint32_t)x[p] >> 16);
-    }
-  }
+  append_part<T, NR>(a, part, (int)(job % a.H), (int)(job / a.H), a.start_dev ? *a.start_dev : a.start);
 }
 
 struct ReadArgs {
@@ -209,55 +35,72 @@ struct ReadArgs {
   int64_t H, capacity, length;
 };
 
-// out = code * scale, rounded once; tail positions converted as they are.  One workgroup per (block, head, batch row).
+// out = code * scale, rounded once; tail positions converted as they are.  One workgroup per (block, head, batch row), threads
+// and LDS image as in append_part.
 template <typename T, typename O> __global__ __launch_bounds__(256) void kv8_read_kernel(ReadArgs a) {
-  __shared__ __attribute__((aligned(16))) int8_t vt[D][BLK + 16];
+  __shared__ __attribute__((aligned(16))) int vt[kVWords];
   typedef typename O::storage out_t;
-  const int tid = threadIdx.x, row = tid >> 2, d0 = (tid & 3) * 32;
+  const int tid = threadIdx.x, r = tid >> 4, i = tid & 15;
   const int64_t blk = blockIdx.x, bh = (int64_t)blockIdx.z * a.H + blockIdx.y, cblocks = (a.capacity + BLK - 1) / BLK;
-  const int64_t pos = blk * BLK + row;
-  const bool whole = (blk + 1) * BLK <= a.length;
-  float x[32], y[32];
-  if (whole) {
-    const int8_t* cv = a.cv + (bh * cblocks + blk) * (D * BLK);
+  const int64_t pos0 = blk * BLK + 4 * r;
+  out_t* ko = reinterpret_cast<out_t*>(a.k) + (bh * a.length + pos0) * D + 8 * i;
+  out_t* vo = reinterpret_cast<out_t*>(a.v) + (bh * a.length + pos0) * D + 8 * i;
+  auto store = [&](out_t* p, const float (&x)[8]) {
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      const int chunk = tid + 256 * i;
-      *reinterpret_cast<i32x4*>(&vt[chunk >> 2][(chunk & 3) * 16]) = *reinterpret_cast<const i32x4*>(cv + chunk * 16);
+    for (int c = 0; c < 8 / O::vec; ++c) {
+      Vec<O> y;
+#pragma unroll
+      for (int e = 0; e < O::vec; ++e) y.v[e] = x[c * O::vec + e];
+      store_vec<O>(p + c * O::vec, y);
     }
-    const int8_t* ck = a.ck + (bh * cblocks * BLK + pos) * D + d0;
+  };
+  if ((blk + 1) * BLK <= a.length) {
+    const int8_t* cv = a.cv + (bh * cblocks + blk) * (D * BLK);
+    const int8_t* ck = a.ck + (bh * cblocks * BLK + pos0) * D + 8 * i;
+    i32x4 vraw[2];
+    i32x2 kraw[4];
+#pragma unroll
+    for (int c = 0; c < 2; ++c) vraw[c] = *reinterpret_cast<const i32x4*>(cv + (tid + 256 * c) * 16);
+#pragma unroll
+    for (int c = 0; c < 4; ++c) kraw[c] = *reinterpret_cast<const i32x2*>(ck + c * D);
     const float sk = a.sk[bh * cblocks + blk], sv = a.sv[bh * cblocks + blk];
 #pragma unroll
     for (int c = 0; c < 2; ++c) {
-      const i32x4 w = *reinterpret_cast<const i32x4*>(ck + 16 * c);
+      const int chunk = tid + 256 * c;
+      *reinterpret_cast<i32x4*>(&vt[vword(chunk >> 2, 4 * (chunk & 3))]) = vraw[c];
+    }
+    float x[8];
 #pragma unroll
-      for (int e = 0; e < 16; ++e) x[16 * c + e] = (float)(int8_t)((uint32_t)w[e >> 2] >> (8 * (e & 3))) * sk;
+    for (int c = 0; c < 4; ++c) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = (float)(int8_t)((uint32_t)kraw[c][e >> 2] >> (8 * (e & 3))) * sk;
+      store(ko + c * D, x);
     }
     __syncthreads();
+    uint32_t w[8];
 #pragma unroll
-    for (int e = 0; e < 32; ++e) y[e] = (float)vt[d0 + e][row] * sv;
-  } else {
-    if (pos >= a.length) return;
-    const u16* tk = a.tk + bh * (BLK * D) + row * D + d0;
-    const u16* tv = a.tv + bh * (BLK * D) + d0 * BLK + row;
+    for (int e = 0; e < 8; ++e) w[e] = (uint32_t)vt[vword(8 * i + e, r)];
 #pragma unroll
-    for (int e = 0; e < 32; ++e) {
-      x[e] = to_f32<T>(tk[e]);
-      y[e] = to_f32<T>(tv[e * BLK]);
+    for (int c = 0; c < 4; ++c) {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) x[e] = (float)(int8_t)(w[e] >> (8 * c)) * sv;
+      store(vo + c * D, x);
     }
+    return;
   }
-  out_t* ko = reinterpret_cast<out_t*>(a.k) + (bh * a.length + pos) * D + d0;
-  out_t* vo = reinterpret_cast<out_t*>(a.v) + (bh * a.length + pos) * D + d0;
+  const u16* tk = a.tk + bh * (BLK * D) + 4 * r * D + 8 * i;
+  const u16* tv = a.tv + bh * (BLK * D) + 8 * i * BLK + 4 * r;
 #pragma unroll
-  for (int c = 0; c < 32 / O::vec; ++c) {
-    Vec<O> p, q;
+  for (int c = 0; c < 4; ++c) {
+    if (pos0 + c >= a.length) continue;
+    float x[8], y[8];
 #pragma unroll
-    for (int e = 0; e < O::vec; ++e) {
-      p.v[e] = x[c * O::vec + e];
-      q.v[e] = y[c * O::vec + e];
+    for (int e = 0; e < 8; ++e) {
+      x[e] = to_f32<T>(tk[c * D + e]);
+      y[e] = to_f32<T>(tv[e * BLK + c]);
     }
-    store_vec<O>(ko + c * O::vec, p);
-    store_vec<O>(vo + c * O::vec, q);
+    store(ko + c * D, x);
+    store(vo + c * D, y);
   }
 }
 
@@ -322,7 +165,7 @@ int q3_kv8_norm_rope_append(int dtype, const void* q, int64_t qsb, int64_t qss, 
               (u16*)tail_k, (u16*)tail_v, S, H, capacity, start, start_dev, (const u16*)q, (const u16*)wq, (const u16*)wk,
               (const u16*)cos, (const u16*)sin, qsb, qss, qsh, (u16*)yq, B, Hq, 0, eps};
   a.blocks = append_blocks(a);
-  const int64_t g = a.blocks * H * B + (B * S * Hq + 63) / 64;
+  const int64_t g = a.blocks * H * B + (B * S * Hq + 15) / 16;
   Q3_REQUIRE(g < (1ll << 31));
   if (dtype == Q3_BF16) kv8_append_kernel<BF16, true><<<(unsigned)g, 256, 0, stream>>>(a);
   else kv8_append_kernel<F16, true><<<(unsigned)g, 256, 0, stream>>>(a);
