@@ -552,16 +552,6 @@ int q3_kv8_attention(int dtype, const void* q, int64_t qsb, int64_t qss, int64_t
                      size_t workspace_bytes, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t d, int64_t capacity,
                      int64_t start, const int64_t* start_dev, float scale, hipStream_t stream);
 
-/* A decode step's attention from the projections q [B, Hq, 128], k, v [B, Hkv, 128] (strides of batch and head): Q/K-norm,
- * rotation (tables [B, 128]), append at the position and attention over the cache, as q3_kv8_norm_rope_append and
- * q3_kv8_attention with S = 1 but in the attention's launches.  Hq / Hkv <= 16; workspace as q3_kv8_attention's for S = 1. */
-int q3_kv8_step_attention(int dtype, const void* q, int64_t qsb, int64_t qsh, const void* k, int64_t ksb, int64_t ksh,
-                          const void* v, int64_t vsb, int64_t vsh, const void* wq, const void* wk, float eps, const void* cos,
-                          const void* sin, int8_t* cache_k, int8_t* cache_v, float* scale_k, float* scale_v, void* tail_k,
-                          void* tail_v, void* out, int64_t osb, int64_t osh, void* workspace, size_t workspace_bytes, int64_t B,
-                          int64_t Hq, int64_t Hkv, int64_t d, int64_t capacity, int64_t start, const int64_t* start_dev,
-                          float scale, hipStream_t stream);
-
 #ifdef __cplusplus
 }
 #endif

@@ -181,7 +181,6 @@ struct Span {
   int64_t bh;
   const int8_t *ck, *cv;
   const float *sk, *sv;
-  const u16 *tk, *tv;
 };
 
 // Blocks a split takes: at least minper, all of them over at most max_splits.  It follows from the positions alone, not from
@@ -206,8 +205,6 @@ template <int RT> Q3_DEV Span span_of(const AttnArgs& a, int b, int hk, int spli
   p.cv = a.cv + p.bh * cblocks * (BLK * D);
   p.sk = a.sk + p.bh * cblocks;
   p.sv = a.sv + p.bh * cblocks;
-  p.tk = a.tk + p.bh * (BLK * D);
-  p.tv = a.tv + p.bh * (BLK * D);
   return p;
 }
 
@@ -231,53 +228,85 @@ Q3_DEV void load_rows(const AttnArgs& a, const Span& p, int b, int hk, int g, in
   w.unit = w.inv = 0.f;
 }
 
-// The tail block, in 16 bits: P in T, as V is; slots past the last position hold anything and read as zeros.
+// The tail block, in 16 bits: P in T, as V is; slots past the last position hold anything and read as zeros.  One row tile
+// takes all of V before its scores are formed (a wait less); two have no registers for that and take two dim tiles at a time.
 template <typename T, int RT>
 Q3_DEV void tail_block(const AttnArgs& a, const Span& p, int g, int j, Rows<T, RT>& w, const int (&qpos)[RT]) {
   const int left = (int)(p.total - p.whole * BLK), krow = 16 * (j >> 2) + (j & 3);
   f32x4 s[RT][4];
+  constexpr int VT = RT == 1 ? 8 : 2;  // dim tiles of V in registers
+  i32x4 v[VT][2];
+  auto load_v = [&](int t, i32x4 (&x)[2]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h) x[h] = *reinterpret_cast<const i32x4*>(a.tv + p.bh * (BLK * D) + (16 * t + j) * BLK + 16 * g + 8 * h);
+  };
+  bf16x8_t tkf[RT == 1 ? 4 : 1][2][2];
+  auto load_k = [&](int t, bf16x8_t (&x)[2][2]) {
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+        x[h][e] = *reinterpret_cast<const bf16x8_t*>(a.tk + p.bh * (BLK * D) + (krow + 4 * t) * D + 64 * h + 16 * g + 8 * e);
+  };
+  if constexpr (RT == 1) {
+#pragma unroll
+    for (int t = 0; t < 4; ++t) load_k(t, tkf[t]);
+  }
 #pragma unroll
   for (int t = 0; t < 4; ++t) {
-    const u16* kp = p.tk + (krow + 4 * t) * D + 16 * g;
+    if constexpr (RT > 1) load_k(t, tkf[0]);
 #pragma unroll
     for (int r = 0; r < RT; ++r) s[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int e = 0; e < 2; ++e) {
-        const bf16x8_t kf = *reinterpret_cast<const bf16x8_t*>(kp + 64 * h + 8 * e);
+        const bf16x8_t kf = tkf[RT == 1 ? t : 0][h][e];
 #pragma unroll
         for (int r = 0; r < RT; ++r) s[r][t] = mfma_16x16x32<T>(kf, w.q[r][h][e], s[r][t]);
       }
     if constexpr (RT > 1) __builtin_amdgcn_sched_barrier(0);  // a tile's operands at a time: registers
   }
+  if constexpr (VT == 8) {
+#pragma unroll
+    for (int t = 0; t < 8; ++t) load_v(t, v[t]);
+  }
   // O back to plain units: the tail's values are what they are
   softmax_step<T, RT>(w, s, a.scale2, 0.f, 1.f, w.unit, true, (int)(p.whole * BLK - p.start) + 16 * g, qpos);
   w.unit = w.inv = 1.f;
+  bf16x8_t pf[RT][2];
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    bf16x8_t pf[RT];
+  for (int r = 0; r < RT; ++r)
 #pragma unroll
-    for (int r = 0; r < RT; ++r) {
+    for (int h = 0; h < 2; ++h) {
       i32x4 x;
 #pragma unroll
       for (int e = 0; e < 4; ++e)
         x[e] = (int)pack2<T>(s[r][2 * h + (e >> 1)][2 * (e & 1)], s[r][2 * h + (e >> 1)][2 * (e & 1) + 1]);
-      pf[r] = __builtin_bit_cast(bf16x8_t, x);
+      pf[r][h] = __builtin_bit_cast(bf16x8_t, x);
     }
 #pragma unroll
-    for (int t = 0; t < 8; ++t) {
-      i32x4 v = *reinterpret_cast<const i32x4*>(p.tv + (16 * t + j) * BLK + 16 * g + 8 * h);
+  for (int t0 = 0; t0 < 8; t0 += VT) {
+    if constexpr (VT < 8) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) {
-        const int slot = 16 * g + 8 * h + 2 * e;
-        if (slot >= left) v[e] = 0;
-        else if (slot + 1 >= left) v[e] &= 0xffff;
+      for (int t = 0; t < VT; ++t) load_v(t0 + t, v[t]);
+    }
+#pragma unroll
+    for (int t = 0; t < VT; ++t)
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        i32x4 x = v[t][h];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int slot = 16 * g + 8 * h + 2 * e;
+          if (slot >= left) x[e] = 0;
+          else if (slot + 1 >= left) x[e] &= 0xffff;
+        }
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+          w.o[r][t0 + t] = mfma_16x16x32<T>(__builtin_bit_cast(bf16x8_t, x), pf[r][h], w.o[r][t0 + t]);
       }
-#pragma unroll
-      for (int r = 0; r < RT; ++r) w.o[r][t] = mfma_16x16x32<T>(__builtin_bit_cast(bf16x8_t, v), pf[r], w.o[r][t]);
-      if (RT > 1 && (t & 1)) __builtin_amdgcn_sched_barrier(0);
-    }
+    if constexpr (VT < 8) __builtin_amdgcn_sched_barrier(0);
   }
 }
 
@@ -320,57 +349,9 @@ Q3_DEV void store_rows(const AttnArgs& a, const Span& p, int b, int hk, int spli
   }
 }
 
-// RMSNorm and split-half rotation of the lane's query row, in the fragments' order (dims 64 h + 16 g + 8 e .. + 7: a dim's
-// partner, 64 away, is the lane's own), rounded once.
-template <typename T>
-Q3_DEV void norm_rope_frags(bf16x8_t (&q)[2][2], const u16* w, const u16* cs, const u16* sn, float eps, int g) {
-  float n[2][2][8], ss = 0.f;
-#pragma unroll
-  for (int h = 0; h < 2; ++h)
-#pragma unroll
-    for (int e = 0; e < 2; ++e) {
-      const Vec<T> x = unpack_vec<T>(__builtin_bit_cast(i32x4, q[h][e]));
-#pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        n[h][e][k] = x.v[k];
-        ss += x.v[k] * x.v[k];
-      }
-    }
-  ss += __shfl_xor(ss, 16, 64);
-  ss += __shfl_xor(ss, 32, 64);
-  const float inv = rsqrtf(ss * (1.f / (float)D) + eps);
-#pragma unroll
-  for (int e = 0; e < 2; ++e) {
-    Vec<T> c[2], s[2];
-#pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      const int at = 64 * h + 16 * g + 8 * e;
-      const Vec<T> wf = load_vec<T>(w + at);
-      c[h] = load_vec<T>(cs + at);
-      s[h] = load_vec<T>(sn + at);
-#pragma unroll
-      for (int k = 0; k < 8; ++k) n[h][e][k] = n[h][e][k] * inv * wf.v[k];
-    }
-    i32x4 lo, hi;
-#pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      const int k = 2 * p;
-      // the products and sums of norm_rope16, so that a step's queries are those of a prefill
-      lo[p] = (int)pack2<T>(fmaf(n[0][e][k], c[0].v[k], -(n[1][e][k] * s[0].v[k])),
-                            fmaf(n[0][e][k + 1], c[0].v[k + 1], -(n[1][e][k + 1] * s[0].v[k + 1])));
-      hi[p] = (int)pack2<T>(fmaf(n[1][e][k], c[1].v[k], n[0][e][k] * s[1].v[k]),
-                            fmaf(n[1][e][k + 1], c[1].v[k + 1], n[0][e][k + 1] * s[1].v[k + 1]));
-    }
-    q[0][e] = __builtin_bit_cast(bf16x8_t, lo);
-    q[1][e] = __builtin_bit_cast(bf16x8_t, hi);
-  }
-}
-
 // Few rows (at most 16 per key/value head: one token of a group, a few of a small one): four waves share the rows and take
 // every fourth block each, their K and V fragments straight from memory, and join through LDS.
-// STEP: a decode step from the projections: q is normed and rotated here, and the workgroup whose split holds the new
-// position appends it first (k normed and rotated) and then reads it as it lies in memory.
-template <typename T, bool STEP> __global__ __launch_bounds__(256) void kv8_attn_rows_kernel(AttnArgs a, CacheArgs ca) {
+template <typename T> __global__ __launch_bounds__(256) void kv8_attn_rows_kernel(AttnArgs a) {
   constexpr int RT = 1, WK = 4;
   const int lane = threadIdx.x & 63, wk = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, j = lane & 15;
@@ -379,15 +360,6 @@ template <typename T, bool STEP> __global__ __launch_bounds__(256) void kv8_attn
   Rows<T, RT> w;
   int qpos[RT];
   load_rows<T, RT>(a, sp, b, hk, g, j, w, qpos);
-  if constexpr (STEP) {
-    norm_rope_frags<T>(w.q[0], ca.qw, ca.cs + b * D, ca.sn + b * D, ca.eps, g);
-    const int64_t own = sp.start / BLK;  // the new position's block
-    if (own >= sp.b0 && own < sp.b_end) {
-      append_part<T, true>(ca, 0, hk, b, sp.start);
-      __threadfence_block();  // the workgroup's stores before its loads of them
-      __syncthreads();
-    }
-  }
   const int64_t wend = min(sp.b_end, sp.whole);
   int64_t blk = sp.b0 + wk;
 
@@ -611,22 +583,21 @@ Plan plan_for(int64_t B, int64_t Hkv, int64_t rows, int64_t span) {
   Plan p;
   p.waves = rows <= 16 ? 0 : rows <= 128 ? 4 : 8;
   p.row_blocks = p.waves ? (rows + 32 * p.waves - 1) / (32 * p.waves) : 1;
-  // eight waves on every CU; a block for each wave of a split (rows), or enough of them to pay for the join (tiles)
+  // eight waves on every CU; a block for each wave of a split, or enough of them to pay for the join
+  // where the rows fill the CUs without (32 x 300 positions: 13.1 us in two splits, 10.7 in one)
   const int64_t wgs = B * Hkv * p.row_blocks;
   p.max_splits = (int)std::min<int64_t>(1024, std::max<int64_t>(1, (p.waves == 8 ? 256 : 512) / wgs));
-  p.minper = p.waves ? 16 : 4;
+  p.minper = p.waves || wgs >= 256 ? 16 : 4;
   const int64_t blocks = (span + BLK - 1) / BLK;
   p.splits = (int)std::min<int64_t>(p.max_splits, (blocks + p.minper - 1) / p.minper);
   return p;
 }
 
-// ca: a decode step's append.
-template <typename T> int launch(const Plan& p, const AttnArgs& a, const CacheArgs* ca, int64_t bh, hipStream_t s) {
+template <typename T> int launch(const Plan& p, const AttnArgs& a, int64_t bh, hipStream_t s) {
   const dim3 g((unsigned)bh, (unsigned)p.row_blocks, (unsigned)p.splits);
   if (p.waves == 8) kv8_attn_tile_kernel<T, 8><<<g, 512, 0, s>>>(a);
   else if (p.waves == 4) kv8_attn_tile_kernel<T, 4><<<g, 256, 0, s>>>(a);
-  else if (ca) kv8_attn_rows_kernel<T, true><<<g, 256, 0, s>>>(a, *ca);
-  else kv8_attn_rows_kernel<T, false><<<g, 256, 0, s>>>(a, CacheArgs{});
+  else kv8_attn_rows_kernel<T><<<g, 256, 0, s>>>(a);
   if (p.splits > 1) kv8_merge_kernel<T><<<dim3((unsigned)((a.S * a.G + 3) / 4), (unsigned)bh), 256, 0, s>>>(a);
   return (int)hipGetLastError();
 }
@@ -666,40 +637,7 @@ int q3_kv8_attention(int dtype, const void* q, int64_t qsb, int64_t qss, int64_t
                    (const u16*)tail_v, (u16*)out, osb, oss, osh, ws, ws + parts * D, ws + parts * (D + 1), S, start,
                    capacity, start_dev, (int)Hkv, (int)(Hq / Hkv), p.splits, p.max_splits, p.minper,
                    scale * 1.4426950408889634f};
-  return dtype == Q3_BF16 ? launch<BF16>(p, a, nullptr, B * Hkv, stream) : launch<F16>(p, a, nullptr, B * Hkv, stream);
-}
-
-int q3_kv8_step_attention(int dtype, const void* q, int64_t qsb, int64_t qsh, const void* k, int64_t ksb, int64_t ksh,
-                          const void* v, int64_t vsb, int64_t vsh, const void* wq, const void* wk, float eps, const void* cos,
-                          const void* sin, int8_t* cache_k, int8_t* cache_v, float* scale_k, float* scale_v, void* tail_k,
-                          void* tail_v, void* out, int64_t osb, int64_t osh, void* workspace, size_t workspace_bytes, int64_t B,
-                          int64_t Hq, int64_t Hkv, int64_t d, int64_t capacity, int64_t start, const int64_t* start_dev,
-                          float scale, hipStream_t stream) {
-  Q3_REQUIRE((dtype == Q3_BF16 || dtype == Q3_F16) && d == D && al16(q) && al16(k) && al16(v) && out &&
-             ((uintptr_t)out & 7) == 0 && al16(wq) && al16(wk) && al16(cos) && al16(sin) && eps >= 0.f);
-  Q3_REQUIRE(al16(cache_k) && al16(cache_v) && scale_k && scale_v && al16(tail_k) && al16(tail_v));
-  Q3_REQUIRE(B > 0 && Hkv > 0 && Hq >= Hkv && Hq % Hkv == 0 && Hq / Hkv <= 16 && capacity > 0 && capacity < (1ll << 31) - 64);
-  Q3_REQUIRE(B < 65536 && Hq < 65536 && B * Hkv < 65536);
-  Q3_REQUIRE(start_dev || (start >= 0 && start < capacity));
-  for (int64_t st : {qsb, qsh, ksb, ksh, vsb, vsh}) Q3_REQUIRE(st % 8 == 0);
-  for (int64_t st : {osb, osh}) Q3_REQUIRE(st % 4 == 0);
-  Q3_REQUIRE(scale > 0.f && scale < 1e30f);
-  const int64_t rows = Hq / Hkv;
-  const Plan p = plan_for(B, Hkv, rows, start_dev ? capacity : start + 1);
-  const int64_t parts = B * Hkv * rows * p.splits;
-  if (p.splits > 1) Q3_REQUIRE(al16(workspace) && workspace_bytes >= (size_t)parts * (D + 2) * sizeof(float));
-  float* ws = (float*)workspace;
-  const AttnArgs a{(const u16*)q, qsb, 0, qsh, cache_k, cache_v, scale_k, scale_v, (const u16*)tail_k,
-                   (const u16*)tail_v, (u16*)out, osb, 0, osh, ws, ws + parts * D, ws + parts * (D + 1), 1, start,
-                   capacity, start_dev, (int)Hkv, (int)rows, p.splits, p.max_splits, p.minper, scale * 1.4426950408889634f};
-  CacheArgs c{(const u16*)k, (const u16*)v, ksb, 0, ksh, vsb, 0, vsh, cache_k, cache_v, scale_k, scale_v, (u16*)tail_k,
-              (u16*)tail_v, 1, Hkv, capacity, start, start_dev};
-  c.qw = (const u16*)wq;
-  c.kw = (const u16*)wk;
-  c.cs = (const u16*)cos;
-  c.sn = (const u16*)sin;
-  c.eps = eps;
-  return dtype == Q3_BF16 ? launch<BF16>(p, a, &c, B * Hkv, stream) : launch<F16>(p, a, &c, B * Hkv, stream);
+  return dtype == Q3_BF16 ? launch<BF16>(p, a, B * Hkv, stream) : launch<F16>(p, a, B * Hkv, stream);
 }
 
 }  // extern "C"

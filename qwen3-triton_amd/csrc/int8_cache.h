@@ -1,5 +1,4 @@
-// The key/value cache in 8 bits: its arguments and the writing of new positions, shared by the append kernel and the decode
-// step's attention.
+// The key/value cache in 8 bits: its layout, and the writing of new positions.
 //
 // Blocks of 64 positions with one scale per block and key/value head for the keys and one for the values.  A block is
 // quantised once, from the 16-bit values, when its last position is written; until then its positions stay as they are in

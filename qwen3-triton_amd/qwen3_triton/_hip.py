@@ -135,8 +135,6 @@ SIGNATURES: dict[str, tuple] = {
     "q3_kv8_attention_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64]),
     "q3_kv8_attention": (_i32, [_i32, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _p, _sz, _i64,
                                 _i64, _i64, _i64, _i64, _i64, _i64, _p, _f32, _p]),
-    "q3_kv8_step_attention": (_i32, [_i32, *[_p, _i64, _i64] * 3, _p, _p, _f32, *[_p] * 9, _i64, _i64, _p, _sz,
-                                     *[_i64] * 6, _p, _f32, _p]),
     "q3_gemm_strided": (_i32, [_i32, _i32, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _f32, _i32,
                                 _p]),
 }

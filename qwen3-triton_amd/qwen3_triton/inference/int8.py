@@ -401,25 +401,3 @@ def attention(q, cache, start, start_dev=None, *, scale=None):
                None if ws is None else ws.data_ptr(), nbytes, b, s, hq, hkv, d, cache.capacity, start,
                None if start_dev is None else start_dev.data_ptr(), scale, H.stream())
     return out
-
-
-def decode_step_attention(q, k, v, q_norm_weight, k_norm_weight, eps, cos, sin, cache, start, start_dev=None):
-    """A decode step's attention from the raw projections q [B, 1, Hq, 128], k, v [B, 1, Hkv, 128]: ``norm_rope_append`` and
-    ``attention`` in the attention's launches.  At most 16 query heads per key/value head.  Returns [B, 1, Hq, 128]."""
-    _forward_only(q, k, v, q_norm_weight, k_norm_weight)
-    qs, ks, vs = (_check_heads(t, cache, what) for t, what in ((q, 'queries'), (k, 'keys'), (v, 'values')))
-    b, s, hq, d = q.shape
-    hkv = k.shape[2]
-    if s != 1 or v.shape != k.shape or k.shape[1] != 1 or hkv != cache.k.shape[1] or hq % hkv or hq // hkv > 16:
-        raise ValueError('one token of at most 16 query heads per key/value head of the cache required')
-    _check_norm_rope(q, q_norm_weight, k_norm_weight, cos, sin, eps)
-    start = _check_span(start, 1, cache, start_dev)
-    out = torch.empty((b, 1, hq, d), device=q.device, dtype=q.dtype)
-    with torch.cuda.device(q.device):
-        nbytes = H.query("q3_kv8_attention_workspace_bytes", b, 1, hq, hkv, start + 1 if start_dev is None else cache.capacity)
-        ws = H.workspace(nbytes, q.device) if nbytes else None
-        H.call("q3_kv8_step_attention", H.code(q.dtype), q.data_ptr(), qs[0], qs[2], k.data_ptr(), ks[0], ks[2], v.data_ptr(),
-               vs[0], vs[2], q_norm_weight.data_ptr(), k_norm_weight.data_ptr(), float(eps), cos.data_ptr(), sin.data_ptr(),
-               *cache.pointers(), out.data_ptr(), out.stride(0), out.stride(2), None if ws is None else ws.data_ptr(), nbytes, b,
-               hq, hkv, d, cache.capacity, start, None if start_dev is None else start_dev.data_ptr(), d ** -0.5, H.stream())
-    return out

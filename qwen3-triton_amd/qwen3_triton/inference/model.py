@@ -283,9 +283,6 @@ class TritonQwen3Inference(nn.Module):
                                             cache.values[i], start, a.q_norm.eps)
             return kernels.attention(q, cache.keys[i], cache.values[i], start,
                                      split_decode=self.split_decode).reshape(b, s, -1)
-        if in8 and s == 1 and a.q_norm.eps == a.k_norm.eps and a.num_heads <= 16 * a.num_kv_heads:
-            return int8.decode_step_attention(q, k, v, a.q_norm.weight, a.k_norm.weight, a.q_norm.eps, cos, sin,
-                                              cache.layers[i], start, start_dev).reshape(b, s, -1)
         if in8 and a.q_norm.eps == a.k_norm.eps:
             q = int8.norm_rope_append(q, k, v, a.q_norm.weight, a.k_norm.weight, cos, sin, cache.layers[i], start, start_dev,
                                       eps=a.q_norm.eps)

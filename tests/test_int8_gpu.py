@@ -505,39 +505,14 @@ def test_device_positions_and_graph_replay():
     assert all(torch.equal(x, y) for x, y in zip(keep, bits()))
 
 
-@pytest.mark.parametrize("dtype", DT)
-@pytest.mark.parametrize("b,hq,h,start", [(1, 4, 1, 0), (2, 8, 2, 63), (1, 32, 8, 64), (3, 5, 5, 126), (2, 16, 1, 127), (1, 12, 4, 700), (8, 32, 8, 1023)])
-def test_decode_step_attention(b, hq, h, start, dtype):
-    """One call against norm_rope_append and attention: the same bits in the output and the cache.  Projections of small whole
-    numbers, so that their sums of squares are exact in any order; strided sources; host and device positions."""
-    gen = seeded(b + hq + start)
-    c, _, _ = filled(b, h, start, dtype, gen, capacity=start + 70) if start else (poisoned(b, h, 70, dtype), None, None)
-    qkv = torch.randint(-7, 8, (b, 1, hq + 2 * h, 128), generator=gen).to(dtype).cuda()
-    q, k, v = qkv[:, :, :hq], qkv[:, :, hq:hq + h], qkv[:, :, hq + h:]
-    wq, wk = ((1 + 0.1 * torch.randn(128, generator=gen)).to(dtype).cuda() for _ in range(2))
-    ang = torch.rand(b, 1, 64, generator=gen) * 6.28
-    cos, sin = (torch.cat([f(ang)] * 2, -1).to(dtype).cuda() for f in (torch.cos, torch.sin))
-    copies = [I8.LayerCache(*(t.clone() for t in (c.k, c.v, c.k_scale, c.v_scale, c.k_tail, c.v_tail))) for _ in range(2)]
-    want = I8.attention(I8.norm_rope_append(q, k, v, wq, wk, cos, sin, c, start), c, start)
-    bits = lambda x: [t.view(torch.int16 if t.element_size() == 2 else torch.int32 if t.element_size() == 4 else torch.int8)  # noqa: E731
-                      for t in (x.k, x.v, x.k_scale, x.v_scale, x.k_tail, x.v_tail)]
-    for i, d in enumerate(copies):
-        pos = torch.tensor([start], device="cuda") if i else None
-        got = I8.decode_step_attention(q, k, v, wq, wk, 1e-6, cos, sin, d, 0 if i else start, pos)
-        assert torch.isfinite(got).all() and torch.equal(got, want)
-        assert all(torch.equal(x, y) for x, y in zip(bits(d), bits(c)))
-
-
-def test_decode_step_refusals():
+def test_refusals_on_the_device():
     q = torch.zeros(1, 1, 34, 128, dtype=torch.bfloat16, device="cuda")
     w, t = torch.ones(128, dtype=torch.bfloat16, device="cuda"), torch.ones(1, 1, 128, dtype=torch.bfloat16, device="cuda")
     c = poisoned(1, 2, 64, torch.bfloat16)
     kv = q[:, :, :2]
-    for bad in (lambda: I8.decode_step_attention(q, kv, kv, w, w, 1e-6, t, t, c, 0),                         # 17 heads a group
-                lambda: I8.decode_step_attention(q[:, :, :32], kv, kv, w, w, 1e-6, t, t, c, 64),             # past the capacity
-                lambda: I8.decode_step_attention(q[:, :, :32], kv, kv, w, w, -1.0, t, t, c, 0),
-                lambda: I8.decode_step_attention(q[:, :, :32], kv, kv, w[:64], w, 1e-6, t, t, c, 0),
-                lambda: I8.decode_step_attention(q[:, :, :32], q[:, :, :1], q[:, :, :1], w, w, 1e-6, t, t, c, 0),
+    for bad in (lambda: I8.norm_rope_append(q, kv, kv, w, w, t, t, c, 64), lambda: I8.norm_rope_append(q, kv, kv, w, w, t, t, c, 0, eps=-1.0),
+                lambda: I8.norm_rope_append(q, kv, kv, w[:64], w, t, t, c, 0), lambda: I8.norm_rope_append(q, kv, kv, w, w, t[0], t, c, 0),
+                lambda: I8.norm_rope_append(q, q[:, :, :1], q[:, :, :1], w, w, t, t, c, 0),
                 lambda: I8.attention(q[:, :, :32], c, 0, scale=0.0), lambda: I8.attention(q[:, :, :33], c, 0),
                 lambda: I8.attention(q[:, :, :32], c, 64), lambda: I8.attention(q[:, :, :32], c, -1),
                 lambda: I8.append(kv, q[:, :, :1], c, 0), lambda: I8.append(kv.expand(1, 2, 2, 128), kv.expand(1, 2, 2, 128), c, 63),
