@@ -534,42 +534,44 @@ template <typename T, int WR> __global__ __launch_bounds__(WR * 64, 2) void kv8_
   store_rows<T, RT>(a, sp, b, hk, split, g, j, w);
 }
 
-// out = sum_j 2^(m_j - M) o_j / sum_j 2^(m_j - M) l_j over a row's splits, in fixed order: a wave per row, 2 dims a lane.
-template <typename T> __global__ __launch_bounds__(256) void kv8_merge_kernel(AttnArgs a) {
-  const int64_t rows = a.S * a.G, i = (int64_t)blockIdx.x * 4 + (threadIdx.x >> 6);
-  const int lane = threadIdx.x & 63;
-  const int64_t bh = blockIdx.y;
-  if (i >= rows) return;
-  const int64_t p0 = (bh * rows + i) * a.splits;
+// out = sum_j 2^(m_j - M) o_j / sum_j 2^(m_j - M) l_j over a row's splits, in fixed order: 32 lanes per row, 4 dims each; a
+// split's weight sits in lane j % 32.  Bound by the partials' traffic at many rows, by latency at few: NJ splits' outputs are
+// in flight before their weights are known.
+template <typename T, int NJ> __global__ __launch_bounds__(256) void kv8_merge_kernel(AttnArgs a) {
+  const int64_t rows = a.S * a.G, i = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5), bh = blockIdx.y;
+  const int lane = threadIdx.x & 31;
+  const int64_t p0 = (bh * rows + min(i, rows - 1)) * a.splits;
   float mx = kLow;
-  for (int k = lane; k < a.splits; k += 64) mx = fmaxf(mx, a.pm[p0 + k]);
-  mx = group_max<64>(mx);
-  float l = 0.f, x = 0.f, y = 0.f;
-  for (int k0 = 0; k0 < a.splits; k0 += 64) {
-    const int n = min(64, a.splits - k0);
+  for (int k = lane; k < a.splits; k += 32) mx = fmaxf(mx, a.pm[p0 + k]);
+  mx = group_max<32>(mx);
+  float l = 0.f;
+  f32x4 x = {0.f, 0.f, 0.f, 0.f};
+  for (int k0 = 0; k0 < a.splits; k0 += 32) {
+    const int n = min(32, a.splits - k0);
     float wgt = 0.f;
     if (lane < n) {
       const float pl = a.pl[p0 + k0 + lane];
       wgt = pl == 0.f ? 0.f : __builtin_amdgcn_exp2f(a.pm[p0 + k0 + lane] - mx);  // l = 0: nothing stored
       l += wgt * pl;
     }
-    for (int k1 = 0; k1 < n; k1 += 8) {
-      f32x2_t o[8];  // eight loads in flight, before their weights are known
+    for (int k1 = 0; k1 < n; k1 += NJ) {
+      f32x4 o[NJ];
 #pragma unroll
-      for (int k = 0; k < 8; ++k)
-        o[k] = *reinterpret_cast<const f32x2_t*>(a.po + (p0 + k0 + min(k1 + k, n - 1)) * D + 2 * lane);
+      for (int k = 0; k < NJ; ++k) o[k] = *reinterpret_cast<const f32x4*>(a.po + (p0 + k0 + min(k1 + k, n - 1)) * D + 4 * lane);
 #pragma unroll
-      for (int k = 0; k < 8; ++k) {
-        const float f = k1 + k < n ? __shfl(wgt, min(k1 + k, n - 1), 64) : 0.f;
-        x += f == 0.f ? 0.f : f * o[k][0];
-        y += f == 0.f ? 0.f : f * o[k][1];
+      for (int k = 0; k < NJ; ++k) {
+        const float f = k1 + k < n ? __shfl(wgt, min(k1 + k, n - 1), 32) : 0.f;
+#pragma unroll
+        for (int e = 0; e < 4; ++e) x[e] += f == 0.f ? 0.f : f * o[k][e];
       }
     }
   }
-  l = group_sum<64>(l);
+  l = group_sum<32>(l);
+  if (i >= rows) return;
   const float inv = 1.f / l;
   const int64_t s = i / a.G, h = (bh % a.Hkv) * a.G + (i - s * a.G);
-  *reinterpret_cast<uint32_t*>(a.o + (bh / a.Hkv) * a.ob + s * a.os + h * a.oh + 2 * lane) = pack2<T>(x * inv, y * inv);
+  *reinterpret_cast<i32x2*>(a.o + (bh / a.Hkv) * a.ob + s * a.os + h * a.oh + 4 * lane) =
+      i32x2{(int)pack2<T>(x[0] * inv, x[1] * inv), (int)pack2<T>(x[2] * inv, x[3] * inv)};
 }
 
 struct Plan {
@@ -598,7 +600,11 @@ template <typename T> int launch(const Plan& p, const AttnArgs& a, int64_t bh, h
   if (p.waves == 8) kv8_attn_tile_kernel<T, 8><<<g, 512, 0, s>>>(a);
   else if (p.waves == 4) kv8_attn_tile_kernel<T, 4><<<g, 256, 0, s>>>(a);
   else kv8_attn_rows_kernel<T><<<g, 256, 0, s>>>(a);
-  if (p.splits > 1) kv8_merge_kernel<T><<<dim3((unsigned)((a.S * a.G + 3) / 4), (unsigned)bh), 256, 0, s>>>(a);
+  if (p.splits > 1) {
+    const dim3 mg((unsigned)((a.S * a.G + 7) / 8), (unsigned)bh);
+    if (p.splits <= 2) kv8_merge_kernel<T, 2><<<mg, 256, 0, s>>>(a);
+    else kv8_merge_kernel<T, 8><<<mg, 256, 0, s>>>(a);
+  }
   return (int)hipGetLastError();
 }
 

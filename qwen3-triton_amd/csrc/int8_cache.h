@@ -97,17 +97,17 @@ Q3_DEV void append_part(const CacheArgs& a, int part, int h, int b, int64_t star
     }
     const int d = tid >> 1, half = (tid & 1) * 32;  // mixed: V of dim d, slots half .. + 31
     if (mixed) {
+      const int from = (int)(start - pos0) - half;  // the first new one among this thread's slots
 #pragma unroll
       for (int c = 0; c < 4; ++c) vr[c] = *reinterpret_cast<const i32x4*>(tv + d * BLK + half + 8 * c);
-      const int from = (int)(start - pos0);
-      if (from < half + 32) {
+      u16 fresh[32];
 #pragma unroll
-        for (int e = 0; e < 32; ++e)
-          if (half + e >= from) {
-            const uint32_t x = vp[(pos0 + half + e - start) * a.vs + d];
-            const uint32_t w = (uint32_t)vr[e >> 3][(e >> 1) & 3];
-            vr[e >> 3][(e >> 1) & 3] = (int)((e & 1) ? (w & 0xffffu) | (x << 16) : (w & 0xffff0000u) | x);
-          }
+      for (int e = 0; e < 32; ++e) fresh[e] = vp[(int64_t)max(e - from, 0) * a.vs + d];  // (no branch: the first one again)
+#pragma unroll
+      for (int e = 0; e < 32; ++e) {
+        const uint32_t w = (uint32_t)vr[e >> 3][(e >> 1) & 3], x = fresh[e];
+        const uint32_t y = (e & 1) ? (w & 0xffffu) | (x << 16) : (w & 0xffff0000u) | x;
+        vr[e >> 3][(e >> 1) & 3] = (int)(e >= from ? y : w);
       }
     } else {
 #pragma unroll
@@ -115,16 +115,14 @@ Q3_DEV void append_part(const CacheArgs& a, int part, int h, int b, int64_t star
     }
     uint32_t mk = 0, mv = 0;
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const Vec<T> x = unpack_vec<T>(kr[c]), y = unpack_vec<T>(vr[c]);
+    for (int c = 0; c < 4; ++c)
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        mk = max(mk, mag_bits(x.v[e]));
-        mv = max(mv, mag_bits(y.v[e]));
+      for (int p = 0; p < 4; ++p) {
+        mk = mag_max16(mk, (uint32_t)kr[c][p]);
+        mv = mag_max16(mv, (uint32_t)vr[c][p]);
       }
-    }
-    mk = group_umax<64>(mk);
-    mv = group_umax<64>(mv);
+    mk = wave_umax(mag_bits16<T>(mk));
+    mv = wave_umax(mag_bits16<T>(mv));
     if ((tid & 63) == 0) {
       red[0][tid >> 6] = mk;
       red[1][tid >> 6] = mv;
@@ -143,15 +141,9 @@ Q3_DEV void append_part(const CacheArgs& a, int part, int h, int b, int64_t star
 #pragma unroll
     for (int c = 0; c < 4; ++c) {
       const Vec<T> x = unpack_vec<T>(kr[c]), y = unpack_vec<T>(vr[c]);
-      float p[8], q[8];
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        p[e] = fk ? quant_code(x.v[e], sk) : 0.f;
-        q[e] = fv ? quant_code(y.v[e], sv) : 0.f;
-      }
       *reinterpret_cast<i32x2*>(a.ck + (bh * cblocks * BLK + pos0 + 4 * r + c) * D + 8 * i) =
-          i32x2{pack_codes(p[0], p[1], p[2], p[3]), pack_codes(p[4], p[5], p[6], p[7])};
-      vc[c] = i32x2{pack_codes(q[0], q[1], q[2], q[3]), pack_codes(q[4], q[5], q[6], q[7])};
+          fk ? quant_codes(x.v, sk) : i32x2{0, 0};
+      vc[c] = fv ? quant_codes(y.v, sv) : i32x2{0, 0};
     }
     int8_t* cv = a.cv + (bh * cblocks + blk) * (D * BLK);
     if (mixed) {
@@ -159,12 +151,14 @@ Q3_DEV void append_part(const CacheArgs& a, int part, int h, int b, int64_t star
       *reinterpret_cast<i32x4*>(cv + d * BLK + half + 16) = i32x4{vc[2][0], vc[2][1], vc[3][0], vc[3][1]};
     } else {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {  // 4 positions of one dim to a word
-        const int w = e >> 2, s = 8 * (e & 3);
-        uint32_t x = 0;
-#pragma unroll
-        for (int c = 0; c < 4; ++c) x |= (((uint32_t)vc[c][w] >> s) & 0xffu) << (8 * c);
-        vt[vword(8 * i + e, r)] = (int)x;
+      for (int w = 0; w < 2; ++w) {  // 4 dims x 4 positions: 4 positions of one dim to a word
+        const uint32_t x0 = (uint32_t)vc[0][w], x1 = (uint32_t)vc[1][w], x2 = (uint32_t)vc[2][w], x3 = (uint32_t)vc[3][w];
+        const uint32_t a01 = __builtin_amdgcn_perm(x1, x0, 0x05010400u), a23 = __builtin_amdgcn_perm(x3, x2, 0x05010400u);
+        const uint32_t b01 = __builtin_amdgcn_perm(x1, x0, 0x07030602u), b23 = __builtin_amdgcn_perm(x3, x2, 0x07030602u);
+        vt[vword(8 * i + 4 * w, r)] = (int)__builtin_amdgcn_perm(a23, a01, 0x05040100u);
+        vt[vword(8 * i + 4 * w + 1, r)] = (int)__builtin_amdgcn_perm(a23, a01, 0x07060302u);
+        vt[vword(8 * i + 4 * w + 2, r)] = (int)__builtin_amdgcn_perm(b23, b01, 0x05040100u);
+        vt[vword(8 * i + 4 * w + 3, r)] = (int)__builtin_amdgcn_perm(b23, b01, 0x07060302u);
       }
       __syncthreads();
 #pragma unroll

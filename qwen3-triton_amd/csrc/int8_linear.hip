@@ -10,24 +10,6 @@
 
 namespace q3gemm {
 
-// Largest magnitude over a wave, every lane with the result.
-Q3_DEV uint32_t wave_umax(uint32_t x) {
-  auto dpp = [](uint32_t v, auto ctrl) {
-    const uint32_t y = (uint32_t)__builtin_amdgcn_mov_dpp((int)v, decltype(ctrl)::value, 0xF, 0xF, true);
-    return v > y ? v : y;
-  };
-  x = dpp(x, std::integral_constant<int, 0xB1>{});
-  x = dpp(x, std::integral_constant<int, 0x4E>{});
-  x = dpp(x, std::integral_constant<int, 0x141>{});
-  x = dpp(x, std::integral_constant<int, 0x140>{});
-#pragma unroll
-  for (int o = 16; o < 64; o <<= 1) {
-    const uint32_t y = (uint32_t)__shfl_xor((int)x, o, 64);
-    x = x > y ? x : y;
-  }
-  return x;
-}
-
 // What the rows are: their codes (R = 0), or R 16-bit rows that every workgroup turns into codes itself, in LDS, while its
 // first weights are on their way: quantize_rows, or with NORM rms_norm.  Each workgroup repeats that work on rows that sit
 // in L2; it saves a launch and its wait, and a decode step has one before each of its four products.  One row: 9.5 against
@@ -95,16 +77,19 @@ __global__ __launch_bounds__(512) void gemm_rows_q8_kernel(Args a, RowIn in) {
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         if ((v * 512 + tid) * 8 >= K) continue;
-        const Vec<T> xf = unpack_vec<T>(rv[m][v]);
-        Vec<T> wf;
-        if constexpr (NORM) wf = unpack_vec<T>(nv[v]);
+        if constexpr (NORM) {
+          const Vec<T> xf = unpack_vec<T>(rv[m][v]), wf = unpack_vec<T>(nv[v]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-          if constexpr (NORM) ss[m] += xf.v[e] * xf.v[e];
-          const uint32_t y = mag_bits(NORM ? xf.v[e] * wf.v[e] : xf.v[e]);
-          mb[m] = mb[m] > y ? mb[m] : y;
+          for (int e = 0; e < 8; ++e) {
+            ss[m] += xf.v[e] * xf.v[e];
+            mb[m] = max(mb[m], mag_bits(xf.v[e] * wf.v[e]));
+          }
+        } else {
+#pragma unroll
+          for (int p = 0; p < 4; ++p) mb[m] = mag_max16(mb[m], (uint32_t)rv[m][v][p]);
         }
       }
+      if constexpr (!NORM) mb[m] = mag_bits16<T>(mb[m]);
       mb[m] = wave_umax(mb[m]);
       if constexpr (NORM) ss[m] = group_sum<64>(ss[m]);
     }
@@ -138,14 +123,13 @@ __global__ __launch_bounds__(512) void gemm_rows_q8_kernel(Args a, RowIn in) {
 #pragma unroll
       for (int v = 0; v < V; ++v) {
         if ((v * 512 + tid) * 8 >= K) continue;
-        const Vec<T> xf = unpack_vec<T>(rv[m][v]);
-        Vec<T> wf;
-        if constexpr (NORM) wf = unpack_vec<T>(nv[v]);
-        float c[8];
+        Vec<T> xf = unpack_vec<T>(rv[m][v]);
+        if constexpr (NORM) {
+          const Vec<T> wf = unpack_vec<T>(nv[v]);
 #pragma unroll
-        for (int e = 0; e < 8; ++e) c[e] = finite ? quant_code(NORM ? xf.v[e] * wf.v[e] : xf.v[e], st) : 0.f;
-        *reinterpret_cast<i32x2*>(xs + m * (K + PAD) + (v * 512 + tid) * 8) =
-            i32x2{pack_codes(c[0], c[1], c[2], c[3]), pack_codes(c[4], c[5], c[6], c[7])};
+          for (int e = 0; e < 8; ++e) xf.v[e] *= wf.v[e];
+        }
+        *reinterpret_cast<i32x2*>(xs + m * (K + PAD) + (v * 512 + tid) * 8) = finite ? quant_codes(xf.v, st) : i32x2{0, 0};
       }
     }
     __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14));

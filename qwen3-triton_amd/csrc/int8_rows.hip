@@ -63,17 +63,21 @@ __global__ __launch_bounds__(BLOCK) void quant_rows_kernel(RowArgs a) {
       if (in && live) *reinterpret_cast<i32x4*>(a.total + row * a.h + (t + j * TPR) * 8) = tv[j];
     }
     if (in) {
-      Vec<T> w;
-      if constexpr (NORM) w = unpack_vec<T>(wv[j]);
+      if constexpr (NORM) {
+        const Vec<T> w = unpack_vec<T>(wv[j]);
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        if constexpr (NORM) ss += x.v[e] * x.v[e];
-        const uint32_t b = mag_bits(NORM ? x.v[e] * w.v[e] : x.v[e]);
-        mb = mb > b ? mb : b;
+        for (int e = 0; e < 8; ++e) {
+          ss += x.v[e] * x.v[e];
+          mb = max(mb, mag_bits(x.v[e] * w.v[e]));
+        }
+      } else {
+#pragma unroll
+        for (int p = 0; p < 4; ++p) mb = mag_max16(mb, (uint32_t)tv[j][p]);
       }
     }
   }
-  mb = group_umax<64>(mb);
+  if constexpr (!NORM) mb = mag_bits16<T>(mb);
+  mb = wave_umax(mb);
   if constexpr (NORM) ss = group_sum<64>(ss);
   if constexpr (NWR > 1) {
     const int wv_id = threadIdx.x >> 6, w0 = (threadIdx.x / TPR) * NWR;
@@ -102,14 +106,13 @@ __global__ __launch_bounds__(BLOCK) void quant_rows_kernel(RowArgs a) {
 #pragma unroll
   for (int j = 0; j < MAXV; ++j) {
     if (t + j * TPR >= nvec) continue;
-    const Vec<T> x = unpack_vec<T>(tv[j]);
-    Vec<T> w;
-    if constexpr (NORM) w = unpack_vec<T>(wv[j]);
-    float c[8];
+    Vec<T> x = unpack_vec<T>(tv[j]);
+    if constexpr (NORM) {
+      const Vec<T> w = unpack_vec<T>(wv[j]);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) c[e] = finite ? quant_code(NORM ? x.v[e] * w.v[e] : x.v[e], st) : 0.f;
-    *reinterpret_cast<i32x2*>(a.q + row * a.h + (t + j * TPR) * 8) =
-        i32x2{pack_codes(c[0], c[1], c[2], c[3]), pack_codes(c[4], c[5], c[6], c[7])};
+      for (int e = 0; e < 8; ++e) x.v[e] *= w.v[e];
+    }
+    *reinterpret_cast<i32x2*>(a.q + row * a.h + (t + j * TPR) * 8) = finite ? quant_codes(x.v, st) : i32x2{0, 0};
   }
 }
 

@@ -15,19 +15,24 @@ P = 1 << 20   # a 16-byte aligned address that no refused call touches
 
 
 def test_quantise_rule_matches_exact_rationals():
-    """a (127 / M) in fp32, nearest, and the exact decision within 1e-4 of a half: the same integer as the rational 127 a / M
-    rounded to nearest even, for 16-bit a and for products of two."""
+    """a (127 / M) + 1.5 * 2^23 in one fma, and the exact decision within 1e-5 of a half: the same integer as the rational
+    127 a / M rounded to nearest even, for 16-bit a and for products of two."""
     rng = np.random.default_rng(0)
-    f32 = np.float32
+    f32, magic = np.float32, np.float32(12582912.0)
+
+    def fma(x, y, z):   # exact, then one rounding
+        return f32(float(Fraction(float(x)) * Fraction(float(y)) + Fraction(float(z))))
 
     def code(a, m):
-        t = f32(a) * (f32(127) / f32(m))
-        q = np.rint(t)
-        if abs(f32(t - q)) > f32(0.4999):
-            u, k = 127.0 * float(a), np.floor(float(t))
+        inv = f32(127) / f32(m)
+        r = fma(a, inv, magic)
+        d = abs(fma(a, inv, f32(magic - r)))
+        if d > f32(0.49999):
+            u = 127.0 * float(a)
+            k = np.floor(u / float(m))
             mid = (k + 0.5) * float(m)
-            q = k if u < mid else k + 1 if u > mid else 2 * np.rint(0.5 * k + 0.25)
-        return int(q)
+            return int(k if u < mid else k + 1 if u > mid else 2 * np.rint(0.5 * k + 0.25))
+        return int(r - magic)
 
     for _ in range(4000):
         bits = rng.choice([8, 11, 22])
