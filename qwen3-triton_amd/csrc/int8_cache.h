@@ -61,25 +61,25 @@ Q3_DEV int vword(int d, int r) { return (d >> 3) * 144 + (d & 7) * 16 + (r ^ (4 
 
 // The new positions start .. end - 1 as far as block `part` (counted from the first one touched) goes; part 0 also writes the
 // last, unfinished block's into the tail, after it has read the tail, which may hold the first block's positions in the same
-// slots.  256 threads: thread t owns positions 4 (t / 16) .. + 3 of the block and dims 8 (t % 16) .. + 7.
+// slots.  Keys and values are a workgroup's each (V).  256 threads: thread t owns positions 4 (t / 16) .. + 3 of the block and
+// dims 8 (t % 16) .. + 7.
 // NR: the keys come as projected and are normed and rotated here.
-template <typename T, bool NR>
+template <typename T, bool NR, bool V>
 Q3_DEV void append_part(const CacheArgs& a, int part, int h, int b, int64_t start) {
-  __shared__ __attribute__((aligned(16))) int vt[kVWords];
-  __shared__ uint32_t red[2][4];
+  __shared__ __attribute__((aligned(16))) int vt[V ? kVWords : 4];
+  __shared__ uint32_t red[4];
   const int tid = threadIdx.x, r = tid >> 4, i = tid & 15;
   const int64_t end = min(start + a.S, a.capacity);
   if (start < 0 || end <= start) return;
   const int64_t first = start / BLK, last = end / BLK;  // last: the first block that is not whole
   const int64_t blk = first + part;
   const int64_t bh = (int64_t)b * a.H + h, cblocks = (a.capacity + BLK - 1) / BLK;
-  u16* tk = a.tk + bh * (BLK * D);
-  u16* tv = a.tv + bh * (BLK * D);
-  const u16* kp = a.k + b * a.kb + h * a.kh + 8 * i;
-  const u16* vp = a.v + b * a.vb + h * a.vh;
-  auto key = [&](int64_t pos) {  // a new position's 8 dims
-    i32x4 x = *reinterpret_cast<const i32x4*>(kp + (pos - start) * a.ks);
-    if constexpr (NR) {
+  u16* tail = (V ? a.tv : a.tk) + bh * (BLK * D);
+  const u16* src = V ? a.v + b * a.vb + h * a.vh : a.k + b * a.kb + h * a.kh;
+  const int64_t stride = V ? a.vs : a.ks;
+  auto fetch = [&](int64_t pos) {  // a new position's 8 dims
+    i32x4 x = *reinterpret_cast<const i32x4*>(src + (pos - start) * stride + 8 * i);
+    if constexpr (NR && !V) {
       const int64_t at = (b * a.S + pos - start) * D + 8 * i;
       x = norm_rope16<T>(x, a.kw + 8 * i, a.cs + at, a.sn + at, a.eps, i);
     }
@@ -88,71 +88,55 @@ Q3_DEV void append_part(const CacheArgs& a, int part, int h, int b, int64_t star
   if (blk < last) {
     const int64_t pos0 = blk * BLK;
     const bool mixed = pos0 < start;  // positions before start are in the tail, V's transposed already
-    i32x4 kr[4], vr[4];
-#pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const int64_t pos = pos0 + 4 * r + c;
-      if (pos >= start) kr[c] = key(pos);
-      else kr[c] = *reinterpret_cast<const i32x4*>(tk + (4 * r + c) * D + 8 * i);
-    }
-    const int d = tid >> 1, half = (tid & 1) * 32;  // mixed: V of dim d, slots half .. + 31
-    if (mixed) {
+    i32x4 x[4];
+    const int d = tid >> 1, half = (tid & 1) * 32;  // V, mixed: dim d, slots half .. + 31
+    if (V && mixed) {
       const int from = (int)(start - pos0) - half;  // the first new one among this thread's slots
 #pragma unroll
-      for (int c = 0; c < 4; ++c) vr[c] = *reinterpret_cast<const i32x4*>(tv + d * BLK + half + 8 * c);
+      for (int c = 0; c < 4; ++c) x[c] = *reinterpret_cast<const i32x4*>(tail + d * BLK + half + 8 * c);
       u16 fresh[32];
 #pragma unroll
-      for (int e = 0; e < 32; ++e) fresh[e] = vp[(int64_t)max(e - from, 0) * a.vs + d];  // (no branch: the first one again)
+      for (int e = 0; e < 32; ++e) fresh[e] = src[(int64_t)max(e - from, 0) * stride + d];  // (no branch: the first one again)
 #pragma unroll
       for (int e = 0; e < 32; ++e) {
-        const uint32_t w = (uint32_t)vr[e >> 3][(e >> 1) & 3], x = fresh[e];
-        const uint32_t y = (e & 1) ? (w & 0xffffu) | (x << 16) : (w & 0xffff0000u) | x;
-        vr[e >> 3][(e >> 1) & 3] = (int)(e >= from ? y : w);
+        const uint32_t w = (uint32_t)x[e >> 3][(e >> 1) & 3], n = fresh[e];
+        const uint32_t y = (e & 1) ? (w & 0xffffu) | (n << 16) : (w & 0xffff0000u) | n;
+        x[e >> 3][(e >> 1) & 3] = (int)(e >= from ? y : w);
       }
     } else {
 #pragma unroll
-      for (int c = 0; c < 4; ++c) vr[c] = *reinterpret_cast<const i32x4*>(vp + (pos0 + 4 * r + c - start) * a.vs + 8 * i);
+      for (int c = 0; c < 4; ++c) {
+        const int64_t pos = pos0 + 4 * r + c;
+        if (!V && pos < start) x[c] = *reinterpret_cast<const i32x4*>(tail + (4 * r + c) * D + 8 * i);
+        else x[c] = fetch(pos);
+      }
     }
-    uint32_t mk = 0, mv = 0;
+    uint32_t m = 0;
 #pragma unroll
     for (int c = 0; c < 4; ++c)
 #pragma unroll
-      for (int p = 0; p < 4; ++p) {
-        mk = mag_max16(mk, (uint32_t)kr[c][p]);
-        mv = mag_max16(mv, (uint32_t)vr[c][p]);
-      }
-    mk = wave_umax(mag_bits16<T>(mk));
-    mv = wave_umax(mag_bits16<T>(mv));
-    if ((tid & 63) == 0) {
-      red[0][tid >> 6] = mk;
-      red[1][tid >> 6] = mv;
-    }
+      for (int p = 0; p < 4; ++p) m = mag_max16(m, (uint32_t)x[c][p]);
+    m = wave_umax(mag_bits16<T>(m));
+    if ((tid & 63) == 0) red[tid >> 6] = m;
     __syncthreads();
-    mk = max(max(red[0][0], red[0][1]), max(red[0][2], red[0][3]));
-    mv = max(max(red[1][0], red[1][1]), max(red[1][2], red[1][3]));
-    const bool fk = bits_finite(mk), fv = bits_finite(mv);
-    const QuantStep sk = quant_step(fk ? __uint_as_float(mk) : 0.f), sv = quant_step(fv ? __uint_as_float(mv) : 0.f);
-    if (tid == 0) {
-      const float nan = __uint_as_float(0x7fc00000u);
-      a.sk[bh * cblocks + blk] = fk ? sk.m / 127.f : nan;
-      a.sv[bh * cblocks + blk] = fv ? sv.m / 127.f : nan;
-    }
-    i32x2 vc[4];  // codes of the thread's V values, in the order of vr
+    m = max(max(red[0], red[1]), max(red[2], red[3]));
+    const bool finite = bits_finite(m);
+    const QuantStep st = quant_step(finite ? __uint_as_float(m) : 0.f);
+    if (tid == 0) (V ? a.sv : a.sk)[bh * cblocks + blk] = finite ? st.m / 127.f : __uint_as_float(0x7fc00000u);
+    i32x2 q[4];  // the codes, in the order of x
 #pragma unroll
-    for (int c = 0; c < 4; ++c) {
-      const Vec<T> x = unpack_vec<T>(kr[c]), y = unpack_vec<T>(vr[c]);
-      *reinterpret_cast<i32x2*>(a.ck + (bh * cblocks * BLK + pos0 + 4 * r + c) * D + 8 * i) =
-          fk ? quant_codes(x.v, sk) : i32x2{0, 0};
-      vc[c] = fv ? quant_codes(y.v, sv) : i32x2{0, 0};
-    }
-    int8_t* cv = a.cv + (bh * cblocks + blk) * (D * BLK);
-    if (mixed) {
-      *reinterpret_cast<i32x4*>(cv + d * BLK + half) = i32x4{vc[0][0], vc[0][1], vc[1][0], vc[1][1]};
-      *reinterpret_cast<i32x4*>(cv + d * BLK + half + 16) = i32x4{vc[2][0], vc[2][1], vc[3][0], vc[3][1]};
+    for (int c = 0; c < 4; ++c) q[c] = finite ? quant_codes(unpack_vec<T>(x[c]).v, st) : i32x2{0, 0};
+    int8_t* out = (V ? a.cv : a.ck) + (bh * cblocks + blk) * (D * BLK);
+    if (!V) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) *reinterpret_cast<i32x2*>(out + (4 * r + c) * D + 8 * i) = q[c];
+    } else if (mixed) {
+      *reinterpret_cast<i32x4*>(out + d * BLK + half) = i32x4{q[0][0], q[0][1], q[1][0], q[1][1]};
+      *reinterpret_cast<i32x4*>(out + d * BLK + half + 16) = i32x4{q[2][0], q[2][1], q[3][0], q[3][1]};
     } else {
 #pragma unroll
       for (int w = 0; w < 2; ++w) {  // 4 dims x 4 positions: 4 positions of one dim to a word
-        const uint32_t x0 = (uint32_t)vc[0][w], x1 = (uint32_t)vc[1][w], x2 = (uint32_t)vc[2][w], x3 = (uint32_t)vc[3][w];
+        const uint32_t x0 = (uint32_t)q[0][w], x1 = (uint32_t)q[1][w], x2 = (uint32_t)q[2][w], x3 = (uint32_t)q[3][w];
         const uint32_t a01 = __builtin_amdgcn_perm(x1, x0, 0x05010400u), a23 = __builtin_amdgcn_perm(x3, x2, 0x05010400u);
         const uint32_t b01 = __builtin_amdgcn_perm(x1, x0, 0x07030602u), b23 = __builtin_amdgcn_perm(x3, x2, 0x07030602u);
         vt[vword(8 * i + 4 * w, r)] = (int)__builtin_amdgcn_perm(a23, a01, 0x05040100u);
@@ -163,8 +147,8 @@ Q3_DEV void append_part(const CacheArgs& a, int part, int h, int b, int64_t star
       __syncthreads();
 #pragma unroll
       for (int c = 0; c < 2; ++c) {
-        const int chunk = tid + 256 * c, vd = chunk >> 2, q = chunk & 3;  // dim, positions 16 q .. + 15
-        *reinterpret_cast<i32x4*>(cv + chunk * 16) = *reinterpret_cast<const i32x4*>(&vt[vword(vd, 4 * q)]);
+        const int chunk = tid + 256 * c, vd = chunk >> 2, p = chunk & 3;  // dim, positions 16 p .. + 15
+        *reinterpret_cast<i32x4*>(out + chunk * 16) = *reinterpret_cast<const i32x4*>(&vt[vword(vd, 4 * p)]);
       }
     }
   }
@@ -175,12 +159,15 @@ Q3_DEV void append_part(const CacheArgs& a, int part, int h, int b, int64_t star
     const int slot = 4 * r + c;
     const int64_t pos = last * BLK + slot;
     if (pos < start || pos >= end) continue;
-    *reinterpret_cast<i32x4*>(tk + slot * D + 8 * i) = key(pos);
-    const i32x4 x = *reinterpret_cast<const i32x4*>(vp + (pos - start) * a.vs + 8 * i);
+    const i32x4 x = fetch(pos);
+    if (!V) {
+      *reinterpret_cast<i32x4*>(tail + slot * D + 8 * i) = x;
+    } else {
 #pragma unroll
-    for (int p = 0; p < 4; ++p) {
-      tv[(8 * i + 2 * p) * BLK + slot] = (u16)((uint32_t)x[p] & 0xffffu);
-      tv[(8 * i + 2 * p + 1) * BLK + slot] = (u16)((uint32_t)x[p] >> 16);
+      for (int p = 0; p < 4; ++p) {
+        tail[(8 * i + 2 * p) * BLK + slot] = (u16)((uint32_t)x[p] & 0xffffu);
+        tail[(8 * i + 2 * p + 1) * BLK + slot] = (u16)((uint32_t)x[p] >> 16);
+      }
     }
   }
 }

@@ -6,11 +6,11 @@ namespace {
 
 using namespace q3kv8;
 
-// One workgroup per (touched block, head, batch row); with the norm and rotation, the ones behind them take 16 query rows each.
+// Two workgroups per (touched block, head, batch row), for the keys and the values; with the norm and rotation, the ones behind them take 16 query rows each.
 template <typename T, bool NR> __global__ __launch_bounds__(256) void kv8_append_kernel(CacheArgs a) {
   int64_t job = blockIdx.x;
   if constexpr (NR) {
-    const int64_t cache_jobs = a.blocks * a.H * a.B;
+    const int64_t cache_jobs = 2 * a.blocks * a.H * a.B;
     if (job >= cache_jobs) {
       const int tid = threadIdx.x, i = tid & 15;
       const int64_t at = (job - cache_jobs) * 16 + (tid >> 4);  // a 16-lane row's query
@@ -22,9 +22,13 @@ template <typename T, bool NR> __global__ __launch_bounds__(256) void kv8_append
       return;
     }
   }
-  const int part = (int)(job % a.blocks);
-  job /= a.blocks;
-  append_part<T, NR>(a, part, (int)(job % a.H), (int)(job / a.H), a.start_dev ? *a.start_dev : a.start);
+  const bool values = job & 1;
+  job >>= 1;
+  const int h = (int)(job % a.H);  // heads next to each other, as their rows are in memory
+  job /= a.H;
+  const int64_t start = a.start_dev ? *a.start_dev : a.start;
+  if (values) append_part<T, NR, true>(a, (int)(job % a.blocks), h, (int)(job / a.blocks), start);
+  else append_part<T, NR, false>(a, (int)(job % a.blocks), h, (int)(job / a.blocks), start);
 }
 
 struct ReadArgs {
@@ -143,8 +147,8 @@ int q3_kv8_append(int dtype, const void* k, int64_t ksb, int64_t kss, int64_t ks
               (u16*)tail_k, (u16*)tail_v, S, H, capacity, start, start_dev};
   a.B = B;
   a.blocks = append_blocks(a);
-  Q3_REQUIRE(a.blocks * H * B < (1ll << 31));
-  const unsigned g = (unsigned)(a.blocks * H * B);
+  Q3_REQUIRE(2 * a.blocks * H * B < (1ll << 31));
+  const unsigned g = (unsigned)(2 * a.blocks * H * B);
   if (dtype == Q3_BF16) kv8_append_kernel<BF16, false><<<g, 256, 0, stream>>>(a);
   else kv8_append_kernel<F16, false><<<g, 256, 0, stream>>>(a);
   return (int)hipGetLastError();
@@ -165,7 +169,7 @@ int q3_kv8_norm_rope_append(int dtype, const void* q, int64_t qsb, int64_t qss, 
               (u16*)tail_k, (u16*)tail_v, S, H, capacity, start, start_dev, (const u16*)q, (const u16*)wq, (const u16*)wk,
               (const u16*)cos, (const u16*)sin, qsb, qss, qsh, (u16*)yq, B, Hq, 0, eps};
   a.blocks = append_blocks(a);
-  const int64_t g = a.blocks * H * B + (B * S * Hq + 15) / 16;
+  const int64_t g = 2 * a.blocks * H * B + (B * S * Hq + 15) / 16;
   Q3_REQUIRE(g < (1ll << 31));
   if (dtype == Q3_BF16) kv8_append_kernel<BF16, true><<<(unsigned)g, 256, 0, stream>>>(a);
   else kv8_append_kernel<F16, true><<<(unsigned)g, 256, 0, stream>>>(a);
