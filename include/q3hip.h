@@ -497,8 +497,7 @@ int q3_rmsnorm_quant(int dtype, const void* x, int64_t ldx, const void* res, int
  * k % 16 == 0, k < 2^17, 16-byte aligned operands with row strides % 16 == 0 and below 2^23; gate/up: n % 8 == 0, c
  * 16-byte aligned with ldc % 8 == 0. */
 typedef struct q3_int8_gemm_desc {
-  int dtype, pieces, epilogue;
-  int64_t m, n, k, end[3];
+  int64_t dtype, pieces, epilogue, m, n, k, end[3];
   const int8_t* a;
   int64_t lda;
   const float* a_scale;

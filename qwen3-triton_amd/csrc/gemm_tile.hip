@@ -315,7 +315,7 @@ bool parse_int8(const q3_int8_gemm_desc* d, Call& c, bool codes = true) {
   c.at = c.bt = false;
   c.epi = gate_up ? 3 : 0;
   a.axis = d->pieces > 1 ? 2 : 0;
-  a.pieces = d->pieces;
+  a.pieces = (int)d->pieces;
   a.M = d->m;
   a.N = gate_up ? 2 * d->n : d->n;
   a.K = d->k / 2;
@@ -472,7 +472,7 @@ int q3_gemm(const q3_gemm_desc* d, void* workspace, size_t workspace_bytes, hipS
     Q3_REQUIRE(workspace && al16(workspace) &&
                workspace_bytes >= (size_t)a.splits * (size_t)a.M * (size_t)a.N * sizeof(float));
     a.part = (float*)workspace;
-    const int rc = launch(c, l[0], d->dtype, stream);
+    const int rc = launch(c, l[0], (int)d->dtype, stream);
     if (rc != 0) return rc;
     if (norm) {
       if (d->dtype == Q3_BF16)
@@ -487,7 +487,7 @@ int q3_gemm(const q3_gemm_desc* d, void* workspace, size_t workspace_bytes, hipS
     return (int)hipGetLastError();
   }
   for (int i = 0; i < n; ++i) {
-    const int rc = launch(c, l[i], d->dtype, stream);
+    const int rc = launch(c, l[i], (int)d->dtype, stream);
     if (rc != 0) return rc;
   }
   return norm ? q3_rmsnorm_fwd(d->dtype, d->c[0], d->norm_w, d->y, d->m, d->n, d->eps, stream) : 0;
@@ -503,7 +503,7 @@ size_t q3_gemm_int8_workspace_bytes(const q3_int8_gemm_desc* d) {
 int q3_gemm_int8(const q3_int8_gemm_desc* d, void* workspace, size_t workspace_bytes, hipStream_t stream) {
   Call c;
   Q3_REQUIRE(parse_int8(d, c));
-  if (c.a.M <= kStreamRows) return q3gemm::launch_rows_q8(d->dtype, c.epi, c.a, q3gemm::RowIn{}, stream);
+  if (c.a.M <= kStreamRows) return q3gemm::launch_rows_q8((int)d->dtype, c.epi, c.a, q3gemm::RowIn{}, stream);
   Launch l[2];
   const int n = launches(c, l);
   if (l[0].p.splits > 1) {
@@ -511,7 +511,7 @@ int q3_gemm_int8(const q3_int8_gemm_desc* d, void* workspace, size_t workspace_b
     Q3_REQUIRE(workspace && al16(workspace) &&
                workspace_bytes >= (size_t)a.splits * (size_t)a.M * (size_t)a.N * sizeof(int));
     a.part = (float*)workspace;
-    const int rc = launch(c, l[0], d->dtype, stream);
+    const int rc = launch(c, l[0], (int)d->dtype, stream);
     if (rc != 0) return rc;
     const unsigned g = (unsigned)cdiv(a.M * (a.N / 8), 256);
     if (d->dtype == Q3_BF16) combine_q8_kernel<BF16><<<g, 256, 0, stream>>>(a);
@@ -519,7 +519,7 @@ int q3_gemm_int8(const q3_int8_gemm_desc* d, void* workspace, size_t workspace_b
     return (int)hipGetLastError();
   }
   for (int i = 0; i < n; ++i) {
-    const int rc = launch(c, l[i], d->dtype, stream);
+    const int rc = launch(c, l[i], (int)d->dtype, stream);
     if (rc != 0) return rc;
   }
   return 0;
@@ -534,7 +534,7 @@ int q3_decode_linear_int8(const q3_int8_gemm_desc* d, const void* x, int64_t ldx
   Call c;
   Q3_REQUIRE(parse_int8(d, c, false) && q3_decode_linear_int8_ok(d->m, d->k));
   Q3_REQUIRE(al16(x) && x && ldx >= d->k && ldx % 8 == 0 && (!norm_w || (al16(norm_w) && eps >= 0.f)));
-  return q3gemm::launch_rows_q8(d->dtype, c.epi, c.a, q3gemm::RowIn{(const u16*)x, ldx, (const u16*)norm_w, eps}, stream);
+  return q3gemm::launch_rows_q8((int)d->dtype, c.epi, c.a, q3gemm::RowIn{(const u16*)x, ldx, (const u16*)norm_w, eps}, stream);
 }
 
 // LM-head logits A B^T, stored, with their cross-entropy statistics (q3hip.h): 256 x 256 tiles, 128 x 256 when

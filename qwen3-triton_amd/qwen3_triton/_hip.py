@@ -35,11 +35,8 @@ class GemmDesc(ctypes.Structure):
                 ("ldgu", _i64), ("eps", _f32)]
 
 
-class Int8GemmDesc(ctypes.Structure):
-    """``q3_int8_gemm_desc``."""
-    _fields_ = [*((n, _i32) for n in ("dtype", "pieces", "epilogue")), ("m", _i64), ("n", _i64), ("k", _i64),
-                ("end", _i64 * 3), ("a", _p), ("lda", _i64), ("a_scale", _p), ("b", _p * 3), ("ldb", _i64 * 3),
-                ("b_scale", _p * 3), ("c", _p * 3), ("ldc", _i64 * 3), ("res", _p), ("ldres", _i64)]
+# ``q3_int8_gemm_desc``: 8-byte fields throughout, so that a call fills it at once.
+Int8GemmDesc = _i64 * 29
 
 
 # name -> (restype, argtypes); mirrors include/q3hip.h one-to-one.

@@ -8,7 +8,6 @@ M / 127.  A group that holds an infinity or a NaN gets the scale NaN, and what i
 ``TritonQwen3Inference.quantize_weights`` and ``new_cache(..., dtype=torch.int8)`` run the model on these.  The reference
 serves in 16 bits only; nothing here has a counterpart in it.
 """
-import ctypes
 from dataclasses import dataclass
 
 import torch
@@ -23,8 +22,18 @@ _FLOATS = (torch.bfloat16, torch.float16)
 
 
 def _forward_only(*tensors):
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors):
-        raise ValueError('int8 operators are forward only: run them under torch.no_grad or detach the inputs')
+    if torch.is_grad_enabled():
+        for t in tensors:
+            if t is not None and t.requires_grad:
+                raise ValueError('int8 operators are forward only: run them under torch.no_grad or detach the inputs')
+
+
+def _launch(t, name, *args):
+    """Launch on t's device and its current stream (appended to ``args``), whatever device is current."""
+    if t.get_device() == torch._C._cuda_getDevice():
+        return H.call(name, *args, H.stream())
+    with torch.cuda.device(t.device):
+        return H.call(name, *args, H.stream())
 
 
 def _require_float(t, what):
@@ -33,38 +42,48 @@ def _require_float(t, what):
 
 
 def _rows(x, what):
-    """x [..., K] as (rows, row stride): whole rows of 16-byte chunks at one stride."""
-    k = x.shape[-1] if x.ndim else 0
-    if x.ndim < 1 or x.numel() == 0:
+    """x [..., K] as (rows, row stride, K): whole rows of 16-byte chunks at one stride."""
+    k, n = x.shape[-1] if x.ndim else 0, x.numel()
+    if n == 0:
         raise ValueError(f'{what}: nonempty [..., K] required')
-    if x.stride(-1) != 1 and k > 1 or not (x.is_contiguous() or x.ndim == 2):
-        raise ValueError(f'{what}: contiguous, or a matrix of contiguous rows; no hidden layout copy')
-    rows = x.numel() // k
-    ld = x.stride(0) if x.ndim == 2 and rows > 1 else k
+    rows, ld = n // k, k
+    if not x.is_contiguous():
+        if x.ndim != 2 or x.stride(1) != 1 and k > 1:
+            raise ValueError(f'{what}: contiguous, or a matrix of contiguous rows; no hidden layout copy')
+        if rows > 1:
+            ld = x.stride(0)
     if ld < k or (ld * x.element_size()) % 16 or x.data_ptr() % 16:
         raise ValueError(f'{what}: rows must start on 16 bytes and not overlap')
-    return rows, ld
+    return rows, ld, k
 
 
 # ---------------------------------------------------------------- rows
 def _check_rows(x):
     H.require_device(x)
     _require_float(x, 'rows')
-    rows, ld = _rows(x, 'rows')
-    k = x.shape[-1]
+    rows, ld, k = _rows(x, 'rows')
     if k % 16 or k > MAX_ROW:
         raise ValueError(f'rows: a row length that is a multiple of 16 and at most {MAX_ROW} required, not {k}')
     return rows, ld, k
+
+
+def _check_norm(x, weight, eps, k):
+    if weight.shape != (k,) or weight.dtype != x.dtype or not weight.is_contiguous() or weight.data_ptr() % 16 or \
+            not float(eps) >= 0.0:
+        raise ValueError(f'a contiguous 16-byte aligned norm weight of {k} {x.dtype} values and a nonnegative eps required')
+
+
+def _codes_like(x):
+    return torch.empty_like(x, dtype=torch.int8, memory_format=torch.contiguous_format), \
+        x.new_empty(x.shape[:-1], dtype=torch.float32)
 
 
 def quantize_rows(x):
     """x [..., K] -> (codes int8 [..., K], scales fp32 [...]): each row on its own."""
     _forward_only(x)
     rows, ld, k = _check_rows(x)
-    q = torch.empty(x.shape, device=x.device, dtype=torch.int8)
-    scale = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
-    with torch.cuda.device(x.device):
-        H.call("q3_quant_rows", H.code(x.dtype), x.data_ptr(), ld, q.data_ptr(), scale.data_ptr(), rows, k, H.stream())
+    q, scale = _codes_like(x)
+    _launch(x, "q3_quant_rows", H.code(x.dtype), x.data_ptr(), ld, q.data_ptr(), scale.data_ptr(), rows, k)
     return q, scale
 
 
@@ -74,24 +93,21 @@ def rms_norm(x, weight, eps, *, residual=None):
     _forward_only(x, weight, residual)
     rows, ld, k = _check_rows(x)
     H.require_device(x, weight)
-    if weight.shape != (k,) or weight.dtype != x.dtype or not weight.is_contiguous() or weight.data_ptr() % 16:
-        raise ValueError(f'a contiguous 16-byte aligned weight of {k} {x.dtype} values required')
-    if not float(eps) >= 0.0:
-        raise ValueError('a nonnegative eps required')
-    ldr, total = 0, None
-    if residual is not None:
-        H.require_device(x, residual)
-        if residual.shape != x.shape or residual.dtype != x.dtype:
-            raise ValueError('a residual of the shape and dtype of x required')
-        ldr = _rows(residual, 'residual')[1]
-        total = torch.empty(x.shape, device=x.device, dtype=x.dtype)
-    q = torch.empty(x.shape, device=x.device, dtype=torch.int8)
-    scale = torch.empty(x.shape[:-1], device=x.device, dtype=torch.float32)
-    with torch.cuda.device(x.device):
-        H.call("q3_rmsnorm_quant", H.code(x.dtype), x.data_ptr(), ld, None if residual is None else residual.data_ptr(),
-               ldr, weight.data_ptr(), q.data_ptr(), scale.data_ptr(), None if total is None else total.data_ptr(), rows, k,
-               float(eps), H.stream())
-    return (q, scale) if residual is None else (q, scale, total)
+    _check_norm(x, weight, eps, k)
+    if residual is None:
+        q, scale = _codes_like(x)
+        _launch(x, "q3_rmsnorm_quant", H.code(x.dtype), x.data_ptr(), ld, None, 0, weight.data_ptr(), q.data_ptr(),
+                scale.data_ptr(), None, rows, k, float(eps))
+        return q, scale
+    H.require_device(x, residual)
+    if residual.shape != x.shape or residual.dtype != x.dtype:
+        raise ValueError('a residual of the shape and dtype of x required')
+    ldr = _rows(residual, 'residual')[1]
+    q, scale = _codes_like(x)
+    total = torch.empty_like(x, memory_format=torch.contiguous_format)
+    _launch(x, "q3_rmsnorm_quant", H.code(x.dtype), x.data_ptr(), ld, residual.data_ptr(), ldr, weight.data_ptr(),
+            q.data_ptr(), scale.data_ptr(), total.data_ptr(), rows, k, float(eps))
+    return q, scale, total
 
 
 # ---------------------------------------------------------------- products
@@ -99,73 +115,66 @@ def _check_codes(q, scale):
     H.require_device(q, scale)
     if q.dtype != torch.int8:
         raise TypeError(f'int8 codes required, not {q.dtype}')
-    rows, ld = _rows(q, 'codes')
+    rows, ld, k = _rows(q, 'codes')
     if scale.dtype != torch.float32 or scale.shape != q.shape[:-1] or not scale.is_contiguous():
         raise ValueError('contiguous float32 scales, one per row of codes, required')
-    k = q.shape[-1]
-    if k % 16 or k >= MAX_K:
-        raise ValueError(f'a row length that is a multiple of 16 and below {MAX_K} required, not {k}')
+    if k % 16 or k >= MAX_K or ld >= 1 << 23:
+        raise ValueError(f'a row length that is a multiple of 16 and below {MAX_K} required, not {k} ({ld} apart)')
     return rows, ld, k
 
 
-def _check_weight(q, w, ws):
-    H.require_device(q, w, ws)
-    if w.dtype != torch.int8 or w.ndim != 2 or w.shape[1] != q.shape[-1]:
-        raise ValueError('an int8 weight [N, K] of the codes\' K required')
-    if ws.dtype != torch.float32 or ws.shape != (w.shape[0],) or not ws.is_contiguous():
+def _check_weight(x, k, w, ws):
+    H.require_device(x, w, ws)
+    if w.dtype != torch.int8 or w.ndim != 2 or w.shape[1] != k:
+        raise ValueError('an int8 weight [N, K] of the input\'s K required')
+    if ws.dtype != torch.float32 or ws.ndim != 1 or ws.shape[0] != w.shape[0] or not ws.is_contiguous():
         raise ValueError('contiguous float32 scales, one per weight row, required')
     ld = _rows(w, 'weight')[1]
     if ld >= 1 << 23:
         raise ValueError('weight rows are too far apart')
-    return ld
+    return w.data_ptr(), ld, ws.data_ptr()
 
 
-def _desc(q, rows, k, weights, outs, epilogue, dtype, residual):
-    """The product's descriptor without its left operand (``q``: the tensor that names the device and k)."""
-    d = H.Int8GemmDesc()
-    d.dtype, d.epilogue, d.m, d.k = H.code(dtype), epilogue, rows, k
-    end = 0
+def _desc(x, operand, rows, k, weights, outs, epilogue, dtype, residual):
+    """``q3_int8_gemm_desc``; ``operand``: the left one's (codes, row stride, scales), x: a tensor of its device."""
+    p, ld, s, ends, end = [0, 0, 0], [0, 0, 0], [0, 0, 0], [0, 0, 0], 0
     for i, (w, ws) in enumerate(weights):
-        d.b[i], d.ldb[i], d.b_scale[i] = w.data_ptr(), _check_weight(q, w, ws), ws.data_ptr()
+        p[i], ld[i], s[i] = _check_weight(x, k, w, ws)
         end += w.shape[0]
-        d.end[i] = end
-    d.pieces = len(outs)
-    d.n = end if epilogue != H.GEMM_GATE_UP else weights[0][0].shape[0]
+        ends[i] = end
+    n = end if epilogue != H.GEMM_GATE_UP else weights[0][0].shape[0]
+    c, ldc = [0, 0, 0], [0, 0, 0]
     for i, y in enumerate(outs):
-        d.c[i], d.ldc[i] = y.data_ptr(), y.shape[-1]
+        c[i], ldc[i] = y.data_ptr(), y.shape[-1]
+    res = ldres = 0
     if residual is not None:
-        H.require_device(q, residual)
+        H.require_device(x, residual)
         if residual.shape != outs[0].shape or residual.dtype != dtype or not residual.is_contiguous():
             raise ValueError('a contiguous residual of the result\'s shape and dtype required')
-        d.res, d.ldres = residual.data_ptr(), residual.shape[-1]
-    return d
+        res, ldres = residual.data_ptr(), residual.shape[-1]
+    return H.Int8GemmDesc(H.code(dtype), len(outs), epilogue, rows, n, k, *ends, *operand, *p, *ld, *s, *c, *ldc, res, ldres)
 
 
 def _product(q, scale, weights, outs, epilogue, dtype, residual=None):
-    if dtype not in _FLOATS:
-        raise TypeError(f'a bfloat16 or float16 result required, not {dtype}')
     _forward_only(residual)
-    rows, lda, k = _check_codes(q, scale)
-    if lda >= 1 << 23:
-        raise ValueError('rows of codes are too far apart')
-    d = _desc(q, rows, k, weights, outs, epilogue, dtype, residual)
-    d.a, d.lda, d.a_scale = q.data_ptr(), lda, scale.data_ptr()
-    ref = ctypes.addressof(d)
-    with torch.cuda.device(q.device):
-        nbytes = H.query("q3_gemm_int8_workspace_bytes", ref)
-        ws = H.workspace(nbytes, q.device) if nbytes else None
-        H.call("q3_gemm_int8", ref, None if ws is None else ws.data_ptr(), nbytes, H.stream())
+    rows, ld, k = _check_codes(q, scale)
+    d = _desc(q, (q.data_ptr(), ld, scale.data_ptr()), rows, k, weights, outs, epilogue, dtype, residual)
+    nbytes = H.query("q3_gemm_int8_workspace_bytes", d)
+    ws = H.workspace(nbytes, q.device) if nbytes else None
+    _launch(q, "q3_gemm_int8", d, None if ws is None else ws.data_ptr(), nbytes)
 
 
 def _out(q, n, dtype):
-    return torch.empty((*q.shape[:-1], n), device=q.device, dtype=dtype)
+    if dtype not in _FLOATS:
+        raise TypeError(f'a bfloat16 or float16 result required, not {dtype}')
+    return q.new_empty((*q.shape[:-1], n), dtype=dtype)
 
 
 def linear(q, scale, weight, weight_scale, *, dtype=torch.bfloat16, residual=None):
     """(codes [..., K], scales [...]) x (weight codes [N, K], scales [N]) -> [..., N] in ``dtype``: exact integer sums,
     scaled in fp32, plus ``residual`` [..., N], rounded once."""
     y = _out(q, weight.shape[0], dtype)
-    _product(q, scale, [(weight, weight_scale)], [y], H.GEMM_PLAIN if residual is None else H.GEMM_RESIDUAL, dtype, residual)
+    _product(q, scale, ((weight, weight_scale),), (y,), H.GEMM_PLAIN if residual is None else H.GEMM_RESIDUAL, dtype, residual)
     return y
 
 
@@ -174,18 +183,22 @@ def projections(q, scale, weights, *, dtype=torch.bfloat16):
     if not 1 <= len(weights) <= 3:
         raise ValueError('one to three weights required')
     outs = [_out(q, w.shape[0], dtype) for w, _ in weights]
-    _product(q, scale, list(weights), outs, H.GEMM_PLAIN, dtype)
+    _product(q, scale, weights, outs, H.GEMM_PLAIN, dtype)
     return outs
 
 
-def gate_up_swiglu(q, scale, gate, gate_scale, up, up_scale, *, dtype=torch.bfloat16):
-    """silu(x Wg^T) * (x Wu^T) of codes x and weights [N, K] (N a multiple of 8), formed in fp32 and rounded once."""
+def _check_gate_up(gate, up):
     if gate.shape != up.shape or gate.stride() != up.stride():
         raise ValueError('gate and up weights of one shape and layout required')
     if gate.shape[0] % 8:
         raise ValueError('a number of gate/up channels that is a multiple of 8 required')
+
+
+def gate_up_swiglu(q, scale, gate, gate_scale, up, up_scale, *, dtype=torch.bfloat16):
+    """silu(x Wg^T) * (x Wu^T) of codes x and weights [N, K] (N a multiple of 8), formed in fp32 and rounded once."""
+    _check_gate_up(gate, up)
     y = _out(q, gate.shape[0], dtype)
-    _product(q, scale, [(gate, gate_scale), (up, up_scale)], [y], H.GEMM_GATE_UP, dtype)
+    _product(q, scale, ((gate, gate_scale), (up, up_scale)), (y,), H.GEMM_GATE_UP, dtype)
     return y
 
 
@@ -205,28 +218,25 @@ def decode_linear(x, weights, *, norm_weight=None, eps=1e-6, gate_up=False, resi
         raise ValueError('decode_linear takes at most 2 rows of at most 16384 values')
     if norm_weight is not None:
         H.require_device(x, norm_weight)
-        if norm_weight.shape != (k,) or norm_weight.dtype != x.dtype or not norm_weight.is_contiguous() or \
-                norm_weight.data_ptr() % 16 or not float(eps) >= 0.0:
-            raise ValueError(f'a contiguous 16-byte aligned norm weight of {k} {x.dtype} values and a nonnegative eps required')
+        _check_norm(x, norm_weight, eps, k)
     if gate_up:
-        if len(weights) != 2 or residual is not None or weights[0][0].shape != weights[1][0].shape or \
-                weights[0][0].stride() != weights[1][0].stride() or weights[0][0].shape[0] % 8:
-            raise ValueError('gate and up weights of one shape and layout, channels a multiple of 8, and no residual required')
+        if len(weights) != 2 or residual is not None:
+            raise ValueError('gate and up weights and no residual required')
+        _check_gate_up(weights[0][0], weights[1][0])
         outs, epilogue = [_out(x, weights[0][0].shape[0], x.dtype)], H.GEMM_GATE_UP
     else:
         if not 1 <= len(weights) <= (3 if residual is None else 1):
             raise ValueError('one to three weights required, one with a residual')
         outs = [_out(x, w.shape[0], x.dtype) for w, _ in weights]
         epilogue = H.GEMM_PLAIN if residual is None else H.GEMM_RESIDUAL
-    d = _desc(x, rows, k, list(weights), outs, epilogue, x.dtype, residual)
-    with torch.cuda.device(x.device):
-        H.call("q3_decode_linear_int8", ctypes.addressof(d), x.data_ptr(), ld,
-               None if norm_weight is None else norm_weight.data_ptr(), float(eps), H.stream())
+    d = _desc(x, (0, 0, 0), rows, k, weights, outs, epilogue, x.dtype, residual)
+    _launch(x, "q3_decode_linear_int8", d, x.data_ptr(), ld, None if norm_weight is None else norm_weight.data_ptr(),
+            float(eps))
     return outs[0] if gate_up or residual is not None else outs
 
 
 # ---------------------------------------------------------------- cache
-@dataclass
+@dataclass(frozen=True)
 class LayerCache:
     """One layer's keys and values in 8 bits, head dim 128, capacity C in blocks of 64 positions (Cb = ceil(C / 64)):
 
@@ -270,24 +280,21 @@ class LayerCache:
         return sum(t.numel() * t.element_size()
                    for t in (self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail))
 
-    def check(self):
-        """Raise unless the buffers are what the kernels take; returns (batch, heads)."""
-        tensors = (self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail)
-        H.require_device(*tensors)
-        b, h, c, d = self.k.shape if self.k.ndim == 4 else (0, 0, 0, 0)
+    def __post_init__(self):
+        """The buffers are what the kernels take, once and for all (the fields cannot be set again)."""
+        k, v, ks, vs, kt, vt = tensors = (self.k, self.v, self.k_scale, self.v_scale, self.k_tail, self.v_tail)
+        b, h, c, d = k.shape if k.ndim == 4 else (0, 0, 0, 0)
         cb = c // KV_BLOCK
-        if d != 128 or c % KV_BLOCK or min(b, h, c) < 1 or self.v.shape != (b, h, cb, d, KV_BLOCK) or \
-                self.k_scale.shape != (b, h, cb) or self.v_scale.shape != (b, h, cb) or \
-                self.k_tail.shape != (b, h, KV_BLOCK, d) or self.v_tail.shape != (b, h, d, KV_BLOCK):
+        if d != 128 or c % KV_BLOCK or min(b, h, c) < 1 or v.shape != (b, h, cb, d, KV_BLOCK) or ks.shape != (b, h, cb) or \
+                vs.shape != (b, h, cb) or kt.shape != (b, h, KV_BLOCK, d) or vt.shape != (b, h, d, KV_BLOCK):
             raise ValueError('cache buffers of matching shapes (head dim 128, blocks of 64) required')
-        if self.k.dtype != torch.int8 or self.v.dtype != torch.int8 or self.k_scale.dtype != torch.float32 or \
-                self.v_scale.dtype != torch.float32 or self.k_tail.dtype not in _FLOATS or \
-                self.v_tail.dtype != self.k_tail.dtype:
+        if k.dtype != torch.int8 or v.dtype != torch.int8 or ks.dtype != torch.float32 or vs.dtype != torch.float32 or \
+                kt.dtype not in _FLOATS or vt.dtype != kt.dtype:
             raise TypeError('int8 codes, float32 scales and 16-bit tails of one dtype required')
-        if any(not t.is_contiguous() for t in tensors) or any(t.data_ptr() % 16 for t in (self.k, self.v, self.k_tail,
-                                                                                          self.v_tail)):
-            raise ValueError('contiguous, 16-byte aligned cache buffers required')
-        return b, h
+        dev = k.device
+        for t in tensors:
+            if t.device != dev or not t.is_contiguous() or t.data_ptr() % 16 and t.dtype != torch.float32:
+                raise ValueError('contiguous, 16-byte aligned cache buffers on one device required')
 
     def pointers(self):
         return (self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
@@ -296,16 +303,19 @@ class LayerCache:
 
 def _check_heads(t, cache, what):
     """t [B, S, heads, 128] of the cache's batch and dtype, every head's row 16 bytes of its own; returns its strides."""
-    b, _ = cache.check()
     H.require_device(cache.k, t)
-    if t.ndim != 4 or t.shape[0] != b or t.shape[3] != 128 or t.numel() == 0:
+    if t.ndim != 4 or t.numel() == 0:
+        raise ValueError(f'{what}: [B, S, heads, 128] required')
+    b, s, h, d = t.shape
+    if b != cache.k.shape[0] or d != 128:
         raise ValueError(f'{what}: [B, S, heads, 128] of the cache\'s batch required')
     if t.dtype != cache.k_tail.dtype:
         raise TypeError(f'{what}: {cache.k_tail.dtype} required, not {t.dtype}')
-    strides = [s if n > 1 else 0 for s, n in zip(t.stride()[:3], t.shape)]   # a lone index's stride is never used
-    if t.stride(3) != 1 or any(s % 8 or s < 0 for s in strides) or t.data_ptr() % 16:
+    sb, ss, sh, sd = t.stride()
+    sb, ss, sh = sb if b > 1 else 0, ss if s > 1 else 0, sh if h > 1 else 0   # a lone index's stride is never used
+    if sd != 1 or (sb | ss | sh) % 8 or t.data_ptr() % 16:
         raise ValueError(f'{what}: contiguous, 16-byte aligned heads required')
-    return strides
+    return sb, ss, sh
 
 
 def _check_span(start, s, cache, start_dev):
@@ -330,9 +340,8 @@ def append(k, v, cache, start, start_dev=None):
     if v.shape != k.shape or h != cache.k.shape[1]:
         raise ValueError('keys and values of one shape, with the cache\'s heads, required')
     start = _check_span(start, s, cache, start_dev)
-    with torch.cuda.device(k.device):
-        H.call("q3_kv8_append", H.code(k.dtype), k.data_ptr(), *ks, v.data_ptr(), *vs, *cache.pointers(), b, s, h, d,
-               cache.capacity, start, None if start_dev is None else start_dev.data_ptr(), H.stream())
+    _launch(k, "q3_kv8_append", H.code(k.dtype), k.data_ptr(), *ks, v.data_ptr(), *vs, *cache.pointers(), b, s, h, d,
+            cache.capacity, start, None if start_dev is None else start_dev.data_ptr())
 
 
 def _check_norm_rope(q, q_norm_weight, k_norm_weight, cos, sin, eps):
@@ -356,26 +365,25 @@ def norm_rope_append(q, k, v, q_norm_weight, k_norm_weight, cos, sin, cache, sta
         raise ValueError('queries, keys and values of one batch and length, with the cache\'s heads, required')
     _check_norm_rope(q, q_norm_weight, k_norm_weight, cos, sin, eps)
     start = _check_span(start, s, cache, start_dev)
-    out = torch.empty((b, s, hq, d), device=q.device, dtype=q.dtype)
-    with torch.cuda.device(q.device):
-        H.call("q3_kv8_norm_rope_append", H.code(q.dtype), q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(), *vs,
-               q_norm_weight.data_ptr(), k_norm_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(), out.data_ptr(),
-               *cache.pointers(), b, s, hq, h, d, cache.capacity, start,
-               None if start_dev is None else start_dev.data_ptr(), float(eps), H.stream())
+    out = q.new_empty((b, s, hq, d))
+    _launch(q, "q3_kv8_norm_rope_append", H.code(q.dtype), q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(), *vs,
+            q_norm_weight.data_ptr(), k_norm_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(), out.data_ptr(),
+            *cache.pointers(), b, s, hq, h, d, cache.capacity, start, None if start_dev is None else start_dev.data_ptr(),
+            float(eps))
     return out
 
 
 def read(cache, length, *, dtype=None):
     """The ``length`` positions that the cache holds back as k, v [B, Hkv, length, 128] in ``dtype`` (the tail's by default)."""
-    b, h = cache.check()
-    if type(length) is not int or not 1 <= length <= cache.capacity:
-        raise ValueError(f'length must be an int in [1, {cache.capacity}]')
+    H.require_device(cache.k)
+    b, h, capacity, _ = cache.k.shape
+    if type(length) is not int or not 1 <= length <= capacity:
+        raise ValueError(f'length must be an int in [1, {capacity}]')
     dtype = cache.k_tail.dtype if dtype is None else dtype
-    out = [torch.empty((b, h, length, 128), device=cache.k.device, dtype=dtype) for _ in range(2)]
-    with torch.cuda.device(cache.k.device):
-        H.call("q3_kv8_read", H.code(cache.k_tail.dtype), H.code(dtype), *cache.pointers(), out[0].data_ptr(),
-               out[1].data_ptr(), b, h, 128, cache.capacity, length, H.stream())
-    return out[0], out[1]
+    k, v = (cache.k.new_empty((b, h, length, 128), dtype=dtype) for _ in range(2))
+    _launch(k, "q3_kv8_read", H.code(cache.k_tail.dtype), H.code(dtype), *cache.pointers(), k.data_ptr(), v.data_ptr(), b, h,
+            128, capacity, length)
+    return k, v
 
 
 def attention(q, cache, start, start_dev=None, *, scale=None):
@@ -392,12 +400,10 @@ def attention(q, cache, start, start_dev=None, *, scale=None):
     scale = d ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < 1e30:
         raise ValueError('a positive softmax scale required')
-    out = torch.empty((b, s, hq, d), device=q.device, dtype=q.dtype)
-    with torch.cuda.device(q.device):
-        nbytes = H.query("q3_kv8_attention_workspace_bytes", b, s, hq, hkv,
-                         start + s if start_dev is None else cache.capacity)
-        ws = H.workspace(nbytes, q.device) if nbytes else None
-        H.call("q3_kv8_attention", H.code(q.dtype), q.data_ptr(), *qs, *cache.pointers(), out.data_ptr(), *out.stride()[:3],
-               None if ws is None else ws.data_ptr(), nbytes, b, s, hq, hkv, d, cache.capacity, start,
-               None if start_dev is None else start_dev.data_ptr(), scale, H.stream())
+    out = q.new_empty((b, s, hq, d))
+    nbytes = H.query("q3_kv8_attention_workspace_bytes", b, s, hq, hkv, start + s if start_dev is None else cache.capacity)
+    ws = H.workspace(nbytes, q.device) if nbytes else None
+    _launch(q, "q3_kv8_attention", H.code(q.dtype), q.data_ptr(), *qs, *cache.pointers(), out.data_ptr(), s * hq * d, hq * d, d,
+            None if ws is None else ws.data_ptr(), nbytes, b, s, hq, hkv, d, cache.capacity, start,
+            None if start_dev is None else start_dev.data_ptr(), scale)
     return out

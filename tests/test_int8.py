@@ -68,19 +68,21 @@ def test_rows_refusals():
         assert norm(**bad) == INVALID, bad
 
 
+FIELDS = ["dtype", "pieces", "epilogue", "m", "n", "k", "end", "a", "lda", "a_scale", "b", "ldb", "b_scale", "c", "ldc", "res", "ldres"]
+
+
 def gemm_desc(**kw):
-    d = H.Int8GemmDesc()
-    d.dtype, d.pieces, d.epilogue, d.m, d.n, d.k = 2, 1, 0, 4, 64, 128
-    d.a, d.lda, d.a_scale = P, 128, P
-    for i in range(3):
-        d.end[i] = (i + 1) * 64
-        d.b[i], d.ldb[i], d.b_scale[i], d.c[i], d.ldc[i] = P, 128, P, P, 64
+    d = dict(dtype=2, pieces=1, epilogue=0, m=4, n=64, k=128, end=[64, 128, 192], a=P, lda=128, a_scale=P, b=[P] * 3, ldb=[128] * 3,
+             b_scale=[P] * 3, c=[P] * 3, ldc=[64] * 3, res=0, ldres=0)
     for k, v in kw.items():
         if isinstance(v, tuple):
-            getattr(d, k)[v[0]] = v[1]
+            d[k][v[0]] = v[1] or 0
         else:
-            setattr(d, k, v)
-    return d
+            d[k] = v or 0
+    flat = []
+    for f in FIELDS:
+        flat += d[f] if isinstance(d[f], list) else [d[f]]
+    return H.Int8GemmDesc(*flat)
 
 
 @pytest.mark.parametrize("bad", [dict(dtype=0), dict(m=0), dict(n=0), dict(k=0), dict(k=120), dict(k=1 << 17), dict(m=1 << 31), dict(n=1 << 30),
