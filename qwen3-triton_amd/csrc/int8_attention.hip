@@ -136,34 +136,58 @@ Q3_DEV void softmax_step(Rows<T, RT>& w, f32x4 (&s)[RT][4], float c, float log2_
   }
 }
 
+// A value that is the same in every lane, in a scalar register.
+Q3_DEV float uniform(float x) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x))); }
+
+// A block's factor of the raw scores.  Keys that are all zero have scale 0: their raw scores are 0 whatever the factor, and a
+// factor of 0 would turn hidden positions' minus infinity into NaN.
+Q3_DEV float score_factor(float kscale, float scale2) {
+  const float c = uniform(kscale * scale2);
+  return __float_as_uint(c) == 0 ? 1.f : c;
+}
+
+// How a block's value scale meets O's unit: O is to be multiplied by `units`, and P' = p * scale / unit.
+struct UnitStep {
+  float units, ratio, log2_factor, inv_factor;
+  bool rides, nan;  // the factor rides in the exponent; if not, it is 0, far below the unit, or NaN
+};
+template <typename T, int RT> Q3_DEV UnitStep unit_step(Rows<T, RT>& w, float vscale) {
+  // a value scale within 16 times of the unit leaves it; one 2^60 below adds nothing worth a new unit
+  const uint32_t vb = __float_as_uint(uniform(vscale));  // >= 0, or NaN
+  UnitStep u;
+  u.units = 1.f;
+  u.ratio = uniform(vscale * w.inv);
+  const uint32_t kMost = 0x41800000u, kLeast = 0x3d800000u, kNone = 0x21800000u;  // 16, 1 / 16, 2^-60
+  uint32_t rb = __float_as_uint(u.ratio);
+  if (vb < 0x7f800000u && vb > 0 && (w.inv == 0.f || rb > kMost || (rb < kLeast && rb > kNone))) {
+    const uint32_t e = min(max(vb & 0x7f800000u, 0x00800000u), 0x7e000000u);  // the power of two below, 2^-126 .. 2^125
+    const float inv = __uint_as_float(0x7f000000u - e);
+    u.units = uniform(w.unit * inv);
+    w.unit = __uint_as_float(e);
+    w.inv = inv;
+    u.ratio = uniform(vscale * inv);
+    rb = __float_as_uint(u.ratio);
+  }
+  u.rides = rb >= kLeast && rb <= kMost;
+  u.nan = vb > 0x7f800000u;
+  u.log2_factor = u.rides ? uniform(__builtin_amdgcn_logf(u.ratio)) : 0.f;  // base 2
+  u.inv_factor = u.rides ? uniform(__builtin_amdgcn_exp2f(-u.log2_factor)) : 1.f;
+  return u;
+}
+
 // A block in 8 bits: P' = p * scale / unit as fp16 operands.
 template <typename T, int RT>
 Q3_DEV void softmax_codes(Rows<T, RT>& w, f32x4 (&s)[RT][4], float c, float vscale, bool mask, int key0,
                           const int (&qpos)[RT], i32x4 (&p)[RT][2]) {
-  // a value scale within 16 times of the unit leaves it; one 2^60 below adds nothing worth a new unit
-  const uint32_t vb = __float_as_uint(vscale);  // >= 0, or NaN
-  float ratio = vscale * w.inv, units = 1.f;
-  const uint32_t kMost = 0x41800000u, kLeast = 0x3d800000u, kNone = 0x21800000u;  // 16, 1 / 16, 2^-60
-  uint32_t rb = __float_as_uint(ratio);
-  if (vb < 0x7f800000u && vb > 0 && (w.inv == 0.f || rb > kMost || (rb < kLeast && rb > kNone))) {
-    const uint32_t e = min(max(vb & 0x7f800000u, 0x00800000u), 0x7e000000u);  // the power of two below, 2^-126 .. 2^125
-    const float inv = __uint_as_float(0x7f000000u - e);
-    units = w.unit * inv;
-    w.unit = __uint_as_float(e);
-    w.inv = inv;
-    ratio = vscale * inv;
-    rb = __float_as_uint(ratio);
-  }
-  const bool rides = rb >= kLeast && rb <= kMost;  // the factor rides in the exponent
-  const float lr = rides ? __builtin_amdgcn_logf(ratio) : 0.f;  // base 2
-  softmax_step<T, RT>(w, s, c, lr, __builtin_amdgcn_exp2f(-lr), units, mask, key0, qpos);
-  if (!rides) {  // zero, far below the unit, or NaN, which hidden positions stay clear of
+  const UnitStep u = unit_step(w, vscale);
+  softmax_step<T, RT>(w, s, c, u.log2_factor, u.inv_factor, u.units, mask, key0, qpos);
+  if (!u.rides) {  // zero, far below the unit, or NaN, which hidden positions stay clear of
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[r][t][e] = s[r][t][e] == 0.f ? 0.f : s[r][t][e] * ratio;
+        for (int e = 0; e < 4; ++e) s[r][t][e] = s[r][t][e] == 0.f ? 0.f : s[r][t][e] * u.ratio;
   }
 #pragma unroll
   for (int r = 0; r < RT; ++r)
@@ -174,33 +198,29 @@ Q3_DEV void softmax_codes(Rows<T, RT>& w, f32x4 (&s)[RT][4], float c, float vsca
     }
 }
 
-// What a wave of either kernel knows of its launch.
+// What a wave of either kernel knows of its launch (positions and blocks fit 32 bits: capacity does).
 struct Span {
-  int64_t start, total, whole, b0, b_end;  // positions before the queries and in all; blocks in 8 bits; this split's blocks
-  int rows, row0;
-  int64_t bh;
+  int start, total, whole, b0, b_end;  // positions before the queries and in all; blocks in 8 bits; this split's blocks
+  int rows, row0, bh;
   const int8_t *ck, *cv;
   const float *sk, *sv;
 };
 
 // Blocks a split takes: at least minper, all of them over at most max_splits.  It follows from the positions alone, not from
 // the span that a launch covers, so a captured step and an eager call of one length form the same sums.
-Q3_DEV int64_t split_blocks(const AttnArgs& a, int64_t total) {
-  const int64_t all = (total + BLK - 1) / BLK, per = (all + a.max_splits - 1) / a.max_splits;
-  return per > a.minper ? per : a.minper;
-}
-
 template <int RT> Q3_DEV Span span_of(const AttnArgs& a, int b, int hk, int split, int row0) {
   Span p;
-  p.start = a.start_dev ? *a.start_dev : a.start;
-  p.total = min(p.start + a.S, a.capacity);
+  const int cap = (int)a.capacity;
+  p.start = (int)min(max(a.start_dev ? *a.start_dev : a.start, (int64_t)-1), a.capacity);
+  p.total = min(p.start + (int)a.S, cap);
   p.whole = p.total / BLK;
-  p.rows = (int)(a.S * a.G);
+  p.rows = (int)a.S * a.G;
   p.row0 = row0;
-  p.bh = (int64_t)b * a.Hkv + hk;
-  const int64_t cblocks = (a.capacity + BLK - 1) / BLK, per = split_blocks(a, p.total);
+  p.bh = b * a.Hkv + hk;
+  const int64_t cblocks = (cap + BLK - 1) / BLK;
+  const int all = (p.total + BLK - 1) / BLK, per = max((all + a.max_splits - 1) / a.max_splits, a.minper);
   p.b0 = split * per;
-  p.b_end = min(p.b0 + per, (p.total + BLK - 1) / BLK);
+  p.b_end = min(p.b0 + per, all);
   p.ck = a.ck + p.bh * cblocks * (BLK * D);
   p.cv = a.cv + p.bh * cblocks * (BLK * D);
   p.sk = a.sk + p.bh * cblocks;
@@ -232,13 +252,13 @@ Q3_DEV void load_rows(const AttnArgs& a, const Span& p, int b, int hk, int g, in
 // takes all of V before its scores are formed (a wait less); two have no registers for that and take two dim tiles at a time.
 template <typename T, int RT>
 Q3_DEV void tail_block(const AttnArgs& a, const Span& p, int g, int j, Rows<T, RT>& w, const int (&qpos)[RT]) {
-  const int left = (int)(p.total - p.whole * BLK), krow = 16 * (j >> 2) + (j & 3);
+  const int left = p.total - p.whole * BLK, krow = 16 * (j >> 2) + (j & 3);
   f32x4 s[RT][4];
   constexpr int VT = RT == 1 ? 8 : 2;  // dim tiles of V in registers
   i32x4 v[VT][2];
   auto load_v = [&](int t, i32x4 (&x)[2]) {
 #pragma unroll
-    for (int h = 0; h < 2; ++h) x[h] = *reinterpret_cast<const i32x4*>(a.tv + p.bh * (BLK * D) + (16 * t + j) * BLK + 16 * g + 8 * h);
+    for (int h = 0; h < 2; ++h) x[h] = *reinterpret_cast<const i32x4*>(a.tv + (int64_t)p.bh * (BLK * D) + (16 * t + j) * BLK + 16 * g + 8 * h);
   };
   bf16x8_t tkf[RT == 1 ? 4 : 1][2][2];
   auto load_k = [&](int t, bf16x8_t (&x)[2][2]) {
@@ -246,7 +266,7 @@ Q3_DEV void tail_block(const AttnArgs& a, const Span& p, int g, int j, Rows<T, R
     for (int h = 0; h < 2; ++h)
 #pragma unroll
       for (int e = 0; e < 2; ++e)
-        x[h][e] = *reinterpret_cast<const bf16x8_t*>(a.tk + p.bh * (BLK * D) + (krow + 4 * t) * D + 64 * h + 16 * g + 8 * e);
+        x[h][e] = *reinterpret_cast<const bf16x8_t*>(a.tk + (int64_t)p.bh * (BLK * D) + (krow + 4 * t) * D + 64 * h + 16 * g + 8 * e);
   };
   if constexpr (RT == 1) {
 #pragma unroll
@@ -272,7 +292,7 @@ Q3_DEV void tail_block(const AttnArgs& a, const Span& p, int g, int j, Rows<T, R
     for (int t = 0; t < 8; ++t) load_v(t, v[t]);
   }
   // O back to plain units: the tail's values are what they are
-  softmax_step<T, RT>(w, s, a.scale2, 0.f, 1.f, w.unit, true, (int)(p.whole * BLK - p.start) + 16 * g, qpos);
+  softmax_step<T, RT>(w, s, a.scale2, 0.f, 1.f, w.unit, true, p.whole * BLK - p.start + 16 * g, qpos);
   w.unit = w.inv = 1.f;
   bf16x8_t pf[RT][2];
 #pragma unroll
@@ -337,7 +357,7 @@ Q3_DEV void store_rows(const AttnArgs& a, const Span& p, int b, int hk, int spli
         *reinterpret_cast<i32x2*>(op + 16 * t) = i32x2{(int)pack2<T>(w.o[r][t][0] * inv, w.o[r][t][1] * inv),
                                                        (int)pack2<T>(w.o[r][t][2] * inv, w.o[r][t][3] * inv)};
     } else {
-      const int64_t pr = (p.bh * p.rows + row) * a.splits + split;
+      const int64_t pr = ((int64_t)p.bh * p.rows + row) * a.splits + split;
       if (g == 0) {
         a.pm[pr] = w.m[r];
         a.pl[pr] = w.l[r];
@@ -360,14 +380,14 @@ template <typename T> __global__ __launch_bounds__(256) void kv8_attn_rows_kerne
   Rows<T, RT> w;
   int qpos[RT];
   load_rows<T, RT>(a, sp, b, hk, g, j, w, qpos);
-  const int64_t wend = min(sp.b_end, sp.whole);
-  int64_t blk = sp.b0 + wk;
+  const int wend = min(sp.b_end, sp.whole);
+  int blk = sp.b0 + wk;
 
   Raw raw;
   float sk = 0.f, sv = 0.f;
   const int krow = 16 * (j >> 2) + (j & 3);
-  auto load_k = [&](int64_t i) {
-    const int8_t* p = sp.ck + i * (BLK * D) + krow * D + 16 * g;
+  auto load_k = [&](int i) {
+    const int8_t* p = sp.ck + (int64_t)i * (BLK * D) + krow * D + 16 * g;
 #pragma unroll
     for (int t = 0; t < 4; ++t)
 #pragma unroll
@@ -375,8 +395,8 @@ template <typename T> __global__ __launch_bounds__(256) void kv8_attn_rows_kerne
     sk = sp.sk[i];
     sv = sp.sv[i];
   };
-  auto load_v = [&](int64_t i) {
-    const int8_t* p = sp.cv + i * (BLK * D) + j * BLK + 16 * g;
+  auto load_v = [&](int i) {
+    const int8_t* p = sp.cv + (int64_t)i * (BLK * D) + j * BLK + 16 * g;
 #pragma unroll
     for (int t = 0; t < 8; ++t) raw.v[t] = *reinterpret_cast<const i32x4*>(p + t * 16 * BLK);
   };
@@ -386,7 +406,7 @@ template <typename T> __global__ __launch_bounds__(256) void kv8_attn_rows_kerne
   }
   for (; blk < wend; blk += WK) {
     f32x4 s[RT][4];
-    const float c = sk * a.scale2;
+    const float c = score_factor(sk, a.scale2);
 #pragma unroll
     for (int t = 0; t < 4; ++t) {
       s[0][t] = f32x4{0.f, 0.f, 0.f, 0.f};
@@ -399,7 +419,7 @@ template <typename T> __global__ __launch_bounds__(256) void kv8_attn_rows_kerne
     const float vs = sv;
     if (blk + WK < wend) load_k(blk + WK);
     i32x4 p[RT][2];
-    softmax_codes<T, RT>(w, s, c, vs, (blk + 1) * BLK > sp.start + 1, (int)(blk * BLK - sp.start) + 16 * g, qpos, p);
+    softmax_codes<T, RT>(w, s, c, vs, (blk + 1) * BLK > sp.start + 1, blk * BLK - sp.start + 16 * g, qpos, p);
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
       w.o[0][t] = mfma_16x16x32<F16>(codes16<F16>(raw.v[t][0], raw.v[t][1]), __builtin_bit_cast(bf16x8_t, p[0][0]), w.o[0][t]);
@@ -442,11 +462,14 @@ Q3_DEV void lds_barrier() {
   asm volatile("" ::: "memory");
 }
 
-// Many rows: WR waves of 32 rows each share every block.  Its codes become 16-bit fragments once per workgroup, in LDS in
-// the order in which the lanes read them (a wave-wide kilobyte per fragment: no bank conflicts), one block ahead of their
-// use; the codes after that are in flight in registers meanwhile.
-template <typename T, int WR> __global__ __launch_bounds__(WR * 64, 2) void kv8_attn_tile_kernel(AttnArgs a) {
-  constexpr int RT = 2, KT = 16 / (2 * WR);  // 16-byte pieces of K (and of V) that a lane turns into fragments
+// Many rows: eight waves of 32 rows each share every block.  Its codes become 16-bit fragments once per workgroup, in LDS in
+// the order in which the lanes read them (a wave-wide kilobyte per fragment: no bank conflicts).
+// Pipeline: while the exponentials of block n run on the vector units, the matrix cores form P V of block n - 1 and the scores
+// of block n + 1, in eight steps of eight products each, and the codes of K(n + 2) and V(n) become fragments; K and V keep two
+// stages each.  One barrier per block.  O follows a change of the maximum or of its unit a block late (`pend`), between P V of
+// the block before the change and of the block after it.
+template <typename T> __global__ __launch_bounds__(512, 2) void kv8_attn_tile_kernel(AttnArgs a) {
+  constexpr int RT = 2, WR = 8;
   __shared__ __attribute__((aligned(16))) i32x4 lk[2][4][4][64], lv[2][8][2][64];  // [stage][tile][16-byte step][lane]
   const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int g = lane >> 4, j = lane & 15;
@@ -458,77 +481,203 @@ template <typename T, int WR> __global__ __launch_bounds__(WR * 64, 2) void kv8_
   int qpos[RT];
   load_rows<T, RT>(a, sp, b, hk, g, j, w, qpos);
   auto seen = [&](int row0, int n) { return sp.start + (min(row0 + n, sp.rows) - 1) / a.G; };  // last position of n rows
-  const int64_t wg_end = min(min(sp.b_end, sp.whole), seen(wg0, 16 * RT * WR) / BLK + 1);
-  const int64_t my_end = sp.row0 < sp.rows ? seen(sp.row0, 16 * RT) / BLK + 1 : 0;  // blocks this wave's rows see
-  const int64_t first_pos = sp.start + min(sp.row0, sp.rows - 1) / a.G;
+  // blocks of 8 bits: n = 0 .. nb - 1 are the split's, as far as the workgroup's rows see
+  const int nb = min(min(sp.b_end, sp.whole), seen(wg0, 16 * RT * WR) / BLK + 1) - sp.b0;
+  const int first_pos = sp.start + min(sp.row0, sp.rows - 1) / a.G;
+  const int clear = min((first_pos + 1) / BLK - sp.b0, nb);  // blocks before this one need no mask
 
-  i32x4 rk[KT], rv[KT];
-  float sk = 0.f, sv = 0.f, nsk = 0.f, nsv = 0.f;
-  const int krow = 16 * (j >> 2) + (j & 3);
-  auto fetch = [&](int64_t i) {  // this wave's share: pieces KT wave .. of the K tiles' halves and of the V dim tiles
-    const int8_t* kp = sp.ck + i * (BLK * D) + krow * D + 16 * g;
-    const int8_t* vp = sp.cv + i * (BLK * D) + j * BLK + 16 * g;
+  if (nb > 0) {
+    // codes in flight: this wave's 16-byte pieces, K tile wave / 2, half wave % 2, and V dim tile `wave` (past the end: the
+    // last block again)
+    i32x4 rk, rv;
+    const uint32_t klane = ((wave >> 1) * 4 + 16 * (j >> 2) + (j & 3)) * D + 64 * (wave & 1) + 16 * g;
+    const uint32_t vlane = (16 * wave + j) * BLK + 16 * g;
+    auto codes_of = [&](const int8_t* base, int n) { return base + (int64_t)(sp.b0 + min(n, nb - 1)) * (BLK * D); };
+    auto fetch_k = [&](int n) { rk = *reinterpret_cast<const i32x4*>(codes_of(sp.ck, n) + klane); };
+    auto fetch_v = [&](int n) { rv = *reinterpret_cast<const i32x4*>(codes_of(sp.cv, n) + vlane); };
+    auto spread_k = [&](int st) {
 #pragma unroll
-    for (int c = 0; c < KT; ++c) {
-      const int q = KT * wave + c;
-      rk[c] = *reinterpret_cast<const i32x4*>(kp + (q >> 1) * 4 * D + 64 * (q & 1));
-      rv[c] = *reinterpret_cast<const i32x4*>(vp + q * 16 * BLK);
-    }
-    nsk = sp.sk[i];
-    nsv = sp.sv[i];
-  };
-  auto spread = [&](int st) {
+      for (int e = 0; e < 2; ++e)
+        lk[st][wave >> 1][2 * (wave & 1) + e][lane] = __builtin_bit_cast(i32x4, codes16<T>(rk[2 * e], rk[2 * e + 1]));
+    };
+    auto spread_v = [&](int st) {
 #pragma unroll
-    for (int c = 0; c < KT; ++c)
+      for (int e = 0; e < 2; ++e)
+        lv[st][wave][e][lane] = __builtin_bit_cast(i32x4, codes16<F16>(rv[2 * e], rv[2 * e + 1]));
+    };
+    // the operands of step i: two of V (dim tile i) and two of K (half a tile of keys)
+    auto read_v = [&](bf16x8_t (&f)[2], int st, int i) {
 #pragma unroll
-      for (int e = 0; e < 2; ++e) {
-        const int q = KT * wave + c;
-        lk[st][q >> 1][2 * (q & 1) + e][lane] = __builtin_bit_cast(i32x4, codes16<T>(rk[c][2 * e], rk[c][2 * e + 1]));
-        lv[st][q][e][lane] = __builtin_bit_cast(i32x4, codes16<F16>(rv[c][2 * e], rv[c][2 * e + 1]));
+      for (int e = 0; e < 2; ++e) f[e] = __builtin_bit_cast(bf16x8_t, lv[st][i][e][lane]);
+    };
+    auto read_k = [&](bf16x8_t (&f)[2], int st, int i) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) f[e] = __builtin_bit_cast(bf16x8_t, lk[st][i >> 1][2 * (i & 1) + e][lane]);
+    };
+    auto pv_step = [&](const bf16x8_t (&f)[2], const i32x4 (&p)[RT][2], int i) {
+#pragma unroll
+      for (int e = 0; e < 2; ++e)
+#pragma unroll
+        for (int r = 0; r < RT; ++r) w.o[r][i] = mfma_16x16x32<F16>(f[e], __builtin_bit_cast(bf16x8_t, p[r][e]), w.o[r][i]);
+    };
+    auto qk_step = [&](const bf16x8_t (&f)[2], f32x4 (&s)[RT][4], int i) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h) {
+        const int t = i >> 1, e = 2 * (i & 1) + h;
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+          s[r][t] = mfma_16x16x32<T>(f[h], w.q[r][e >> 1][e & 1], e == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : s[r][t]);
       }
-    sk = nsk;
-    sv = nsv;
-  };
-  int64_t blk = sp.b0;
-  if (blk < wg_end) {
-    fetch(blk);
-    spread(0);
-    if (blk + 1 < wg_end) fetch(blk + 1);
-  }
-  lds_barrier();
-  for (int st = 0; blk < wg_end; ++blk, st ^= 1) {
-    if (blk < my_end) {
-      const float c = sk * a.scale2;
-      f32x4 s[RT][4];
+    };
+    float pend[RT] = {1.f, 1.f};
+    bool late = false;
+    auto rescale = [&]() {
+      if (!late) return;
 #pragma unroll
-      for (int t = 0; t < 4; ++t) {
+      for (int r = 0; r < RT; ++r)
 #pragma unroll
-        for (int r = 0; r < RT; ++r) s[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
+        for (int t = 0; t < 8; ++t) w.o[r][t] *= pend[r];
+    };
+    float nsk = sp.sk[sp.b0], nsv = sp.sv[sp.b0];
+    // block n: s its scores, p becomes its P', sn the scores of block n + 1, pp the P' of block n - 1
+    auto block = [&](int n, f32x4 (&s)[RT][4], i32x4 (&p)[RT][2], f32x4 (&sn)[RT][4], const i32x4 (&pp)[RT][2], auto par) {
+      constexpr int W = decltype(par)::value, R = W ^ 1;  // stages written and read
+      lds_barrier();
+      bf16x8_t fv[2][2], fk[2];
+      read_v(fv[0], R, 0);
+      rescale();
+      float c = score_factor(nsk, a.scale2);
+      const UnitStep u = unit_step(w, nsv);
+      if (n >= clear) {
+        const int key0 = (sp.b0 + n) * BLK - sp.start + 16 * g;
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) s[r][t][e] = key0 + 4 * t + e > qpos[r] ? -INFINITY : s[r][t][e];
+      }
+      if (__float_as_uint(c) > 0x7f800000u) {  // keys that were not finite: NaN for the rows that see the block, no others
+        c = 1.f;
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e)
+              if (__float_as_uint(s[r][t][e]) != 0xff800000u) s[r][t][e] = __uint_as_float(0x7fc00000u);
+      }
+      float mx[RT];
+      bool up = u.units != 1.f;
+#pragma unroll
+      for (int r = 0; r < RT; ++r) {
+        float x = -INFINITY;
+#pragma unroll
+        for (int t = 0; t < 4; ++t)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x = fmaxf(x, s[r][t][e]);
+        mx[r] = xmax4(x) * c;
+        up = up || mx[r] > w.m[r] + 8.f;
+      }
+      late = __any(up);
+      if (late) {
+#pragma unroll
+        for (int r = 0; r < RT; ++r) {
+          const float m = fmaxf(w.m[r], mx[r]), alpha = __builtin_amdgcn_exp2f(w.m[r] - m);
+          w.m[r] = m;
+          w.l[r] *= alpha;
+          pend[r] = alpha * u.units;
+        }
+      }
+      if (!u.rides) {  // no values worth a product (or NaN): their part of the sums here, then scores that give P' 0 (or NaN)
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+#pragma unroll
+          for (int t = 0; t < 4; ++t)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              float x = fmaf(s[r][t][e], c, -w.m[r]);
+              asm volatile("" : "+v"(x));  // not the expression of the steps below, or both are formed up here
+              w.l[r] += __builtin_amdgcn_exp2f(x);
+              // hidden positions (minus infinity, by its bits) stay hidden
+              if (__float_as_uint(s[r][t][e]) != 0xff800000u) s[r][t][e] = u.nan ? __uint_as_float(0x7fc00000u) : -INFINITY;
+            }
+      }
+      float off[RT], sum[RT] = {0.f, 0.f};
+#pragma unroll
+      for (int r = 0; r < RT; ++r) off[r] = u.log2_factor - w.m[r];
+      nsk = sp.sk[sp.b0 + min(n + 1, nb - 1)];
+      nsv = sp.sv[sp.b0 + min(n + 1, nb - 1)];
+#pragma unroll
+      for (int i = 0; i < 8; ++i) {
+        __builtin_amdgcn_sched_barrier(0);
+        read_k(fk, R, i);  // V's are here a step early: their products cover the wait for K's
+        if (i < 7) read_v(fv[(i + 1) & 1], R, i + 1);
+        if (i == 0) spread_k(W);
+        if (i == 0) fetch_k(n + 3);
+        if (i == 3) spread_v(W);
+        if (i == 3) fetch_v(n + 1);
+        pv_step(fv[i & 1], pp, i);
+        qk_step(fk, sn, i);
+        const int r = i >> 2, t = i & 3;
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
-          const bf16x8_t kf = __builtin_bit_cast(bf16x8_t, lk[st][t][e][lane]);
-#pragma unroll
-          for (int r = 0; r < RT; ++r) s[r][t] = mfma_16x16x32<T>(kf, w.q[r][e >> 1][e & 1], s[r][t]);
+          s[r][t][e] = __builtin_amdgcn_exp2f(fmaf(s[r][t][e], c, off[r]));
+          sum[r] += s[r][t][e];
         }
+        int lo = pack_f16x2(s[r][t][0], s[r][t][1]), hi = pack_f16x2(s[r][t][2], s[r][t][3]);
+        asm volatile("" : "+v"(lo), "+v"(hi));  // formed here, beside the products, not where the next block uses them
+        p[r][t >> 1][2 * (t & 1)] = lo;
+        p[r][t >> 1][2 * (t & 1) + 1] = hi;
       }
-      i32x4 p[RT][2];
-      softmax_codes<T, RT>(w, s, c, sv, (blk + 1) * BLK > first_pos + 1, (int)(blk * BLK - sp.start) + 16 * g, qpos, p);
+      __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-      for (int t = 0; t < 8; ++t) {
+      for (int r = 0; r < RT; ++r) w.l[r] = fmaf(sum[r], u.inv_factor, w.l[r]);
+    };
+
+    f32x4 sa[RT][4], sb[RT][4];
+    i32x4 pa[RT][2], pb[RT][2];
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const bf16x8_t vf = __builtin_bit_cast(bf16x8_t, lv[st][t][e][lane]);
+    for (int r = 0; r < RT; ++r)
 #pragma unroll
-          for (int r = 0; r < RT; ++r) w.o[r][t] = mfma_16x16x32<F16>(vf, __builtin_bit_cast(bf16x8_t, p[r][e]), w.o[r][t]);
-        }
-      }
-    }
-    if (blk + 1 < wg_end) {
-      spread(st ^ 1);  // every wave is done with that stage: the barrier of the block before
-      if (blk + 2 < wg_end) fetch(blk + 2);
-    }
+      for (int e = 0; e < 2; ++e) pb[r][e] = i32x4{0, 0, 0, 0};
+    fetch_k(0);
+    spread_k(0);
+    fetch_k(1);
+    spread_k(1);
+#pragma unroll
+    for (int e = 0; e < 2; ++e) lv[1][wave][e][lane] = i32x4{0, 0, 0, 0};  // P V "of block -1"
+    fetch_k(2);
+    fetch_v(0);
     lds_barrier();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      bf16x8_t f[2];
+      read_k(f, 0, i);
+      qk_step(f, sa, i);
+    }
+    int n = 0;
+    for (; n + 2 <= nb; n += 2) {
+      block(n, sa, pa, sb, pb, std::integral_constant<int, 0>{});
+      block(n + 1, sb, pb, sa, pa, std::integral_constant<int, 1>{});
+    }
+    if (n < nb) {
+      block(n, sa, pa, sb, pb, std::integral_constant<int, 0>{});
+#pragma unroll
+      for (int r = 0; r < RT; ++r)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) pb[r][e] = pa[r][e];
+    }
+    lds_barrier();  // V of the last block
+    rescale();
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+      bf16x8_t f[2];
+      read_v(f, (nb - 1) & 1, i);
+      pv_step(f, pb, i);
+    }
   }
+  const int my_end = sp.row0 < sp.rows ? seen(sp.row0, 16 * RT) / BLK + 1 : 0;  // blocks this wave's rows see
   if (sp.b0 <= sp.whole && sp.whole < sp.b_end && sp.whole < my_end) tail_block<T, RT>(a, sp, g, j, w, qpos);
   close_rows<T, RT>(w);
   store_rows<T, RT>(a, sp, b, hk, split, g, j, w);
@@ -575,7 +724,7 @@ template <typename T, int NJ> __global__ __launch_bounds__(256) void kv8_merge_k
 }
 
 struct Plan {
-  int waves;  // of a workgroup of the tile kernel; 0: the rows kernel
+  bool tile;
   int max_splits, minper, splits;
   int64_t row_blocks;
 };
@@ -583,13 +732,13 @@ struct Plan {
 // Rows of one key/value head -> kernel and splits; the positions that a launch may span only bound the grid.
 Plan plan_for(int64_t B, int64_t Hkv, int64_t rows, int64_t span) {
   Plan p;
-  p.waves = rows <= 16 ? 0 : rows <= 128 ? 4 : 8;
-  p.row_blocks = p.waves ? (rows + 32 * p.waves - 1) / (32 * p.waves) : 1;
+  p.tile = rows > 16;
+  p.row_blocks = p.tile ? (rows + 255) / 256 : 1;
   // eight waves on every CU; a block for each wave of a split, or enough of them to pay for the join
   // where the rows fill the CUs without (32 x 300 positions: 13.1 us in two splits, 10.7 in one)
   const int64_t wgs = B * Hkv * p.row_blocks;
-  p.max_splits = (int)std::min<int64_t>(1024, std::max<int64_t>(1, (p.waves == 8 ? 256 : 512) / wgs));
-  p.minper = p.waves || wgs >= 256 ? 16 : 4;
+  p.max_splits = (int)std::min<int64_t>(1024, std::max<int64_t>(1, (p.tile ? 256 : 512) / wgs));
+  p.minper = p.tile || wgs >= 256 ? 16 : 4;
   const int64_t blocks = (span + BLK - 1) / BLK;
   p.splits = (int)std::min<int64_t>(p.max_splits, (blocks + p.minper - 1) / p.minper);
   return p;
@@ -597,8 +746,7 @@ Plan plan_for(int64_t B, int64_t Hkv, int64_t rows, int64_t span) {
 
 template <typename T> int launch(const Plan& p, const AttnArgs& a, int64_t bh, hipStream_t s) {
   const dim3 g((unsigned)bh, (unsigned)p.row_blocks, (unsigned)p.splits);
-  if (p.waves == 8) kv8_attn_tile_kernel<T, 8><<<g, 512, 0, s>>>(a);
-  else if (p.waves == 4) kv8_attn_tile_kernel<T, 4><<<g, 256, 0, s>>>(a);
+  if (p.tile) kv8_attn_tile_kernel<T><<<g, 512, 0, s>>>(a);
   else kv8_attn_rows_kernel<T><<<g, 256, 0, s>>>(a);
   if (p.splits > 1) {
     const dim3 mg((unsigned)((a.S * a.G + 7) / 8), (unsigned)bh);

@@ -436,10 +436,12 @@ def test_attention_value_scales_far_apart(dtype):
     for i, e in enumerate(exps):
         v[:, 64 * i:64 * (i + 1)] *= 2.0 ** e
     v[:, 64:128, 1] = 0   # a block of zeros: scale 0
+    k[:, 192:256, 1] = 0
+    k[:, t - 74:t - 10, 0] = 0   # the last whole block, which some of the queries below see in part
     v = v.to(dtype)
     c = poisoned(b, h, t, dtype)
     I8.append(k.cuda(), v.cuda(), c, 0)
-    for s in (1, 3, 40):
+    for s in (1, 3, 40, 100):
         wide = randn(b, s, 6, 256, gen=gen, dtype=dtype, scale=2.0).cuda()
         q = wide[:, :, 1:5, 64:192]
         o = I8.attention(q, c, t - s, scale=0.3)
