@@ -36,6 +36,16 @@ def _launch(t, name, *args):
         return H.call(name, *args, H.stream())
 
 
+def _on_device(x, *others):
+    """x on a ROCm device and the others beside it (the quick form of ``_hip.require_device``, which names what is wrong)."""
+    dev = x.get_device()
+    if dev < 0:
+        H.require_device(x)
+    for t in others:
+        if t.get_device() != dev:
+            H.require_device(x, t)
+
+
 def _require_float(t, what):
     if t.dtype not in _FLOATS:
         raise TypeError(f'{what}: bfloat16 or float16 required, not {t.dtype}')
@@ -59,7 +69,7 @@ def _rows(x, what):
 
 # ---------------------------------------------------------------- rows
 def _check_rows(x):
-    H.require_device(x)
+    _on_device(x)
     _require_float(x, 'rows')
     rows, ld, k = _rows(x, 'rows')
     if k % 16 or k > MAX_ROW:
@@ -92,14 +102,14 @@ def rms_norm(x, weight, eps, *, residual=None):
     total = x + residual, rounded once, is what the norm is taken of."""
     _forward_only(x, weight, residual)
     rows, ld, k = _check_rows(x)
-    H.require_device(x, weight)
+    _on_device(x, weight)
     _check_norm(x, weight, eps, k)
     if residual is None:
         q, scale = _codes_like(x)
         _launch(x, "q3_rmsnorm_quant", H.code(x.dtype), x.data_ptr(), ld, None, 0, weight.data_ptr(), q.data_ptr(),
                 scale.data_ptr(), None, rows, k, float(eps))
         return q, scale
-    H.require_device(x, residual)
+    _on_device(x, residual)
     if residual.shape != x.shape or residual.dtype != x.dtype:
         raise ValueError('a residual of the shape and dtype of x required')
     ldr = _rows(residual, 'residual')[1]
@@ -112,11 +122,11 @@ def rms_norm(x, weight, eps, *, residual=None):
 
 # ---------------------------------------------------------------- products
 def _check_codes(q, scale):
-    H.require_device(q, scale)
+    _on_device(q, scale)
     if q.dtype != torch.int8:
         raise TypeError(f'int8 codes required, not {q.dtype}')
     rows, ld, k = _rows(q, 'codes')
-    if scale.dtype != torch.float32 or scale.shape != q.shape[:-1] or not scale.is_contiguous():
+    if scale.dtype != torch.float32 or scale.numel() != rows or not scale.is_contiguous():
         raise ValueError('contiguous float32 scales, one per row of codes, required')
     if k % 16 or k >= MAX_K or ld >= 1 << 23:
         raise ValueError(f'a row length that is a multiple of 16 and below {MAX_K} required, not {k} ({ld} apart)')
@@ -124,7 +134,7 @@ def _check_codes(q, scale):
 
 
 def _check_weight(x, k, w, ws):
-    H.require_device(x, w, ws)
+    _on_device(x, w, ws)
     if w.dtype != torch.int8 or w.ndim != 2 or w.shape[1] != k:
         raise ValueError('an int8 weight [N, K] of the input\'s K required')
     if ws.dtype != torch.float32 or ws.ndim != 1 or ws.shape[0] != w.shape[0] or not ws.is_contiguous():
@@ -137,6 +147,18 @@ def _check_weight(x, k, w, ws):
 
 def _desc(x, operand, rows, k, weights, outs, epilogue, dtype, residual):
     """``q3_int8_gemm_desc``; ``operand``: the left one's (codes, row stride, scales), x: a tensor of its device."""
+    res = ldres = 0
+    if residual is not None:
+        _on_device(x, residual)
+        if residual.shape != outs[0].shape or residual.dtype != dtype or not residual.is_contiguous():
+            raise ValueError('a contiguous residual of the result\'s shape and dtype required')
+        res, ldres = residual.data_ptr(), residual.shape[-1]
+    if len(weights) == 1:
+        (w, ws), = weights
+        p, ld, s = _check_weight(x, k, w, ws)
+        n = w.shape[0]
+        return H.Int8GemmDesc(H.code(dtype), 1, epilogue, rows, n, k, n, 0, 0, *operand, p, 0, 0, ld, 0, 0, s, 0, 0,
+                              outs[0].data_ptr(), 0, 0, n, 0, 0, res, ldres)
     p, ld, s, ends, end = [0, 0, 0], [0, 0, 0], [0, 0, 0], [0, 0, 0], 0
     for i, (w, ws) in enumerate(weights):
         p[i], ld[i], s[i] = _check_weight(x, k, w, ws)
@@ -146,12 +168,6 @@ def _desc(x, operand, rows, k, weights, outs, epilogue, dtype, residual):
     c, ldc = [0, 0, 0], [0, 0, 0]
     for i, y in enumerate(outs):
         c[i], ldc[i] = y.data_ptr(), y.shape[-1]
-    res = ldres = 0
-    if residual is not None:
-        H.require_device(x, residual)
-        if residual.shape != outs[0].shape or residual.dtype != dtype or not residual.is_contiguous():
-            raise ValueError('a contiguous residual of the result\'s shape and dtype required')
-        res, ldres = residual.data_ptr(), residual.shape[-1]
     return H.Int8GemmDesc(H.code(dtype), len(outs), epilogue, rows, n, k, *ends, *operand, *p, *ld, *s, *c, *ldc, res, ldres)
 
 
@@ -159,7 +175,7 @@ def _product(q, scale, weights, outs, epilogue, dtype, residual=None):
     _forward_only(residual)
     rows, ld, k = _check_codes(q, scale)
     d = _desc(q, (q.data_ptr(), ld, scale.data_ptr()), rows, k, weights, outs, epilogue, dtype, residual)
-    nbytes = H.query("q3_gemm_int8_workspace_bytes", d)
+    nbytes = H.query("q3_gemm_int8_workspace_bytes", d) if rows > 16 else 0   # up to 16 rows never take any
     ws = H.workspace(nbytes, q.device) if nbytes else None
     _launch(q, "q3_gemm_int8", d, None if ws is None else ws.data_ptr(), nbytes)
 
@@ -167,6 +183,8 @@ def _product(q, scale, weights, outs, epilogue, dtype, residual=None):
 def _out(q, n, dtype):
     if dtype not in _FLOATS:
         raise TypeError(f'a bfloat16 or float16 result required, not {dtype}')
+    if q.ndim == 2:
+        return q.new_empty((q.shape[0], n), dtype=dtype)
     return q.new_empty((*q.shape[:-1], n), dtype=dtype)
 
 
@@ -217,7 +235,7 @@ def decode_linear(x, weights, *, norm_weight=None, eps=1e-6, gate_up=False, resi
     if not decode_linear_ok(x):
         raise ValueError('decode_linear takes at most 2 rows of at most 16384 values')
     if norm_weight is not None:
-        H.require_device(x, norm_weight)
+        _on_device(x, norm_weight)
         _check_norm(x, norm_weight, eps, k)
     if gate_up:
         if len(weights) != 2 or residual is not None:
@@ -303,7 +321,7 @@ class LayerCache:
 
 def _check_heads(t, cache, what):
     """t [B, S, heads, 128] of the cache's batch and dtype, every head's row 16 bytes of its own; returns its strides."""
-    H.require_device(cache.k, t)
+    _on_device(cache.k, t)
     if t.ndim != 4 or t.numel() == 0:
         raise ValueError(f'{what}: [B, S, heads, 128] required')
     b, s, h, d = t.shape
@@ -322,7 +340,7 @@ def _check_span(start, s, cache, start_dev):
     if start_dev is not None:
         if s != 1:
             raise ValueError('device-resident positions are for single-token decode steps')
-        H.require_device(cache.k, start_dev)
+        _on_device(cache.k, start_dev)
         if start_dev.dtype != torch.int64 or start_dev.numel() != 1:
             raise ValueError('a device position is one int64')
         return 0
@@ -347,7 +365,7 @@ def append(k, v, cache, start, start_dev=None):
 def _check_norm_rope(q, q_norm_weight, k_norm_weight, cos, sin, eps):
     b, s, _, d = q.shape
     for t, shape in ((q_norm_weight, (d,)), (k_norm_weight, (d,)), (cos, (b, s, d)), (sin, (b, s, d))):
-        H.require_device(q, t)
+        _on_device(q, t)
         if t.shape != shape or t.dtype != q.dtype or not t.is_contiguous() or t.data_ptr() % 16:
             raise ValueError(f'contiguous, 16-byte aligned {q.dtype} norm weights [128] and tables [B, S, 128] required')
     if not float(eps) >= 0.0:
@@ -375,7 +393,7 @@ def norm_rope_append(q, k, v, q_norm_weight, k_norm_weight, cos, sin, cache, sta
 
 def read(cache, length, *, dtype=None):
     """The ``length`` positions that the cache holds back as k, v [B, Hkv, length, 128] in ``dtype`` (the tail's by default)."""
-    H.require_device(cache.k)
+    _on_device(cache.k)
     b, h, capacity, _ = cache.k.shape
     if type(length) is not int or not 1 <= length <= capacity:
         raise ValueError(f'length must be an int in [1, {capacity}]')
