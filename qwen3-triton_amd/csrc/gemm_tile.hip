@@ -29,6 +29,14 @@ constexpr int kNumCfg = 8;
 constexpr Cfg kCfg[kNumCfg] = {{256, 256, 1, 1.27, 1.48}, {128, 256, 1, 0.86, 0.94}, {128, 128, 1, 0.48, 0.62},
                                {64, 128, 1, 0.28, 0.32},  {64, 64, 2, 0.34, 0.70},   {32, 64, 3, 0.27, 1.04},
                                {192, 256, 1, 0.98, 1.25}, {192, 128, 1, 0.61, 0.68}};
+// The same tiles on 8-bit codes, 128 to a k-tile: a k-tile holds the same bytes and matrix instructions, but the scales'
+// epilogue is longer and the small tiles keep up better.  Fitted with estimate()'s other two constants to 70 shapes (M
+// 17-8192, N 152-24576, K 272-12288), and then timed on 40 others: the plan is 2 % slower on average than the best tile and
+// split, 23 % at worst (57 x 9688 x 7792: 32.8 against 26.7 us).  On the first 70 the 16-bit constants were 3.4 % slower on
+// average and 32 % at worst (128 x 6144 x 4096: 18.4 against 14.1 us), these 1 % and 9 %.
+constexpr Cfg kCfgInt8[kNumCfg] = {{256, 256, 1, 1.49, 1.58}, {128, 256, 1, 1.11, 1.25}, {128, 128, 1, 0.77, 0.87},
+                                   {64, 128, 1, 0.38, 0.43},  {64, 64, 2, 0.30, 0.65},   {32, 64, 3, 0.20, 0.80},
+                                   {192, 256, 1, 1.18, 1.30}, {192, 128, 1, 0.77, 0.80}};
 // Instantiated layouts: the 192-row tiles for a k-contiguous A (they fill the CUs where 256 rows would leave the
 // last row of tiles half empty: 1500 x 24576 x 4096 247 against 279 us), 32 rows for two k-contiguous operands.
 bool cfg_for(int c, bool at, bool bt) { return c < 5 || (c == 5 ? !bt : !at); }
@@ -47,14 +55,15 @@ struct Plan {
 // at worst (512 x 1024 x 1024: 8.3 against 6.6 us).  The order matters more than the values: 256 x 256 tiles sustain
 // 1.38-1.45 PFLOP/s once they fill the CUs, smaller tiles and splits keep the CUs busy below that (65 x 4096 x 4096:
 // 15 us against 47 us on 32 tiles of 128 x 128).
-double estimate(int c, int splits, int64_t tiles, int64_t M, int64_t N, int64_t K, double combine) {
-  const Cfg& f = kCfg[c];
+double estimate(int c, bool int8, int splits, int64_t tiles, int64_t M, int64_t N, int64_t K, double combine) {
+  const Cfg& f = int8 ? kCfgInt8[c] : kCfg[c];
+  const double base = int8 ? 3.5 : 5.6, traffic = int8 ? 3.3e6 : 5e6;
   const int64_t w = tiles * splits, slots = 256 * f.conc;
   const int64_t kt = cdiv(cdiv(K, 64), splits), r = w / slots, rem = w % slots;
   const double last = rem ? std::max(f.solo, f.full * (double)rem / (double)slots) : 0.0;
-  double t = 5.6 + (double)kt * ((double)r * f.full + last);
-  t = std::max(t, 5.6 + 2.0 * (double)N * (double)K / 6e6);
-  return splits > 1 ? t + combine + (double)splits * (double)M * (double)N * 4.0 / 5e6 : t;
+  double t = base + (double)kt * ((double)r * f.full + last);
+  t = std::max(t, base + 2.0 * (double)N * (double)K / 6e6);
+  return splits > 1 ? t + combine + (double)splits * (double)M * (double)N * 4.0 / traffic : t;
 }
 
 // Tiles of a call along its rows / columns: every piece starts a tile of its own.
@@ -85,7 +94,7 @@ Plan plan_for(const Args& a, bool at, bool bt, bool can_split, double combine) {
       // a grid that fills the chip by itself is not split: its partial products would outgrow the caches
       // (6144 x 4096 x 8192 in two splits: 390 + 43 us against 300 us in two launches, below)
       if (sp > 1 && (!can_split || a.K / sp < kMinSplitK || tiles >= 256 * kCfg[c].conc)) break;
-      const double t = estimate(c, sp, tiles, a.M, a.N, a.K, combine);
+      const double t = estimate(c, a.rscale != nullptr, sp, tiles, a.M, a.N, a.K, combine);
       if (best_t == 0.0 || t < best_t) {
         best = {c, sp};
         best_t = t;
@@ -142,10 +151,10 @@ template <typename T> __global__ __launch_bounds__(256) void combine_q8_kernel(A
   int64_t c = (i - r * cols) * 8;
   const int* p = reinterpret_cast<const int*>(a.part) + r * a.N + c;
   i32x4 s0 = *reinterpret_cast<const i32x4*>(p), s1 = *reinterpret_cast<const i32x4*>(p + 4);
+#pragma unroll 4
   for (int k = 1; k < a.splits; ++k) {
-    p += a.M * a.N;
-    s0 += *reinterpret_cast<const i32x4*>(p);
-    s1 += *reinterpret_cast<const i32x4*>(p + 4);
+    s0 += *reinterpret_cast<const i32x4*>(p + k * a.M * a.N);
+    s1 += *reinterpret_cast<const i32x4*>(p + k * a.M * a.N + 4);
   }
   int s = 0;
   if (a.axis == 2)
@@ -355,7 +364,7 @@ bool parse_int8(const q3_int8_gemm_desc* d, Call& c, bool codes = true) {
   if (gate_up && !vec) return false;
   a.vec = vec;
   c.can_split = !gate_up && vec;
-  c.combine = 4.5;
+  c.combine = 2.9;
   return tile_rows(a, 32) * tile_cols(a, 64) < (1ll << 28);
 }
 
