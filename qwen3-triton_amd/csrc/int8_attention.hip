@@ -37,6 +37,13 @@ struct AttnArgs {
   float scale2;  // softmax scale * log2(e)
 };
 
+// NaN as a value that the compiler does not know (this file is compiled on the promise that results of arithmetic are not NaN).
+Q3_DEV float quiet_nan() {
+  uint32_t x;
+  asm("v_mov_b32 %0, 0x7fc00000" : "=v"(x));
+  return __uint_as_float(x);
+}
+
 typedef _Float16 f16x2_t __attribute__((ext_vector_type(2)));
 Q3_DEV int pack_f16x2(float lo, float hi) {
   const f32x2_t v = {lo, hi};
@@ -181,13 +188,13 @@ Q3_DEV void softmax_codes(Rows<T, RT>& w, f32x4 (&s)[RT][4], float c, float vsca
                           const int (&qpos)[RT], i32x4 (&p)[RT][2]) {
   const UnitStep u = unit_step(w, vscale);
   softmax_step<T, RT>(w, s, c, u.log2_factor, u.inv_factor, u.units, mask, key0, qpos);
-  if (!u.rides) {  // zero, far below the unit, or NaN, which hidden positions stay clear of
+  if (!u.rides) {  // zero, far below the unit, or NaN, for every row: 16 rows' positions lie closer than a block's
 #pragma unroll
     for (int r = 0; r < RT; ++r)
 #pragma unroll
       for (int t = 0; t < 4; ++t)
 #pragma unroll
-        for (int e = 0; e < 4; ++e) s[r][t][e] = s[r][t][e] == 0.f ? 0.f : s[r][t][e] * u.ratio;
+        for (int e = 0; e < 4; ++e) s[r][t][e] = s[r][t][e] * u.ratio;
   }
 #pragma unroll
   for (int r = 0; r < RT; ++r)
@@ -250,6 +257,8 @@ Q3_DEV void load_rows(const AttnArgs& a, const Span& p, int b, int hk, int g, in
 
 // The tail block, in 16 bits: P in T, as V is; slots past the last position hold anything and read as zeros.  One row tile
 // takes all of V before its scores are formed (a wait less); two have no registers for that and take two dim tiles at a time.
+// An infinity or NaN among the values makes the rows that see its position NaN, as the whole block will be; the others, whose
+// P is 0 there, are kept clear of it (0 times it is NaN) by reading zeros from that slot on.
 template <typename T, int RT>
 Q3_DEV void tail_block(const AttnArgs& a, const Span& p, int g, int j, Rows<T, RT>& w, const int (&qpos)[RT]) {
   const int left = p.total - p.whole * BLK, krow = 16 * (j >> 2) + (j & 3);
@@ -311,6 +320,32 @@ Q3_DEV void tail_block(const AttnArgs& a, const Span& p, int g, int j, Rows<T, R
 #pragma unroll
       for (int t = 0; t < VT; ++t) load_v(t0 + t, v[t]);
     }
+    uint32_t most = 0;
+#pragma unroll
+    for (int t = 0; t < VT; ++t)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+#pragma unroll
+        for (int e = 0; e < 4; ++e) most = mag_max16(most, (uint32_t)v[t][h][e]);
+    int lim = left;
+    if (__any(!bits_finite(mag_bits16<T>(most)))) {
+      uint32_t before = 0;  // 64 - the first slot that is not finite
+#pragma unroll
+      for (int t = 0; t < VT; ++t)
+#pragma unroll
+        for (int h = 0; h < 2; ++h)
+#pragma unroll
+          for (int e = 0; e < 8; ++e)
+            if (!bits_finite(mag_bits(to_f32<T>((u16)((uint32_t)v[t][h][e >> 1] >> (16 * (e & 1)))))))
+              before = max(before, (uint32_t)(64 - (16 * g + 8 * h + e)));
+      const int first = 64 - (int)wave_umax(before);
+      if (first < left) {
+        lim = first;
+#pragma unroll
+        for (int r = 0; r < RT; ++r)
+          if (p.whole * BLK - p.start + first <= qpos[r]) w.l[r] = quiet_nan();
+      }
+    }
 #pragma unroll
     for (int t = 0; t < VT; ++t)
 #pragma unroll
@@ -319,8 +354,8 @@ Q3_DEV void tail_block(const AttnArgs& a, const Span& p, int g, int j, Rows<T, R
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const int slot = 16 * g + 8 * h + 2 * e;
-          if (slot >= left) x[e] = 0;
-          else if (slot + 1 >= left) x[e] &= 0xffff;
+          if (slot >= lim) x[e] = 0;
+          else if (slot + 1 >= lim) x[e] &= 0xffff;
         }
 #pragma unroll
         for (int r = 0; r < RT; ++r)
@@ -558,6 +593,7 @@ template <typename T> __global__ __launch_bounds__(512, 2) void kv8_attn_tile_ke
             for (int e = 0; e < 4; ++e) s[r][t][e] = key0 + 4 * t + e > qpos[r] ? -INFINITY : s[r][t][e];
       }
       if (__float_as_uint(c) > 0x7f800000u) {  // keys that were not finite: NaN for the rows that see the block, no others
+        const float nan = c;
         c = 1.f;
 #pragma unroll
         for (int r = 0; r < RT; ++r)
@@ -565,7 +601,7 @@ template <typename T> __global__ __launch_bounds__(512, 2) void kv8_attn_tile_ke
           for (int t = 0; t < 4; ++t)
 #pragma unroll
             for (int e = 0; e < 4; ++e)
-              if (__float_as_uint(s[r][t][e]) != 0xff800000u) s[r][t][e] = __uint_as_float(0x7fc00000u);
+              if (__float_as_uint(s[r][t][e]) != 0xff800000u) s[r][t][e] = nan;
       }
       float mx[RT];
       bool up = u.units != 1.f;
@@ -600,7 +636,7 @@ template <typename T> __global__ __launch_bounds__(512, 2) void kv8_attn_tile_ke
               asm volatile("" : "+v"(x));  // not the expression of the steps below, or both are formed up here
               w.l[r] += __builtin_amdgcn_exp2f(x);
               // hidden positions (minus infinity, by its bits) stay hidden
-              if (__float_as_uint(s[r][t][e]) != 0xff800000u) s[r][t][e] = u.nan ? __uint_as_float(0x7fc00000u) : -INFINITY;
+              if (__float_as_uint(s[r][t][e]) != 0xff800000u) s[r][t][e] = u.nan ? u.ratio : -INFINITY;
             }
       }
       float off[RT], sum[RT] = {0.f, 0.f};

@@ -472,6 +472,41 @@ def test_attention_masked_nonfinite_positions():
         scales.copy_(keep)
 
 
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16], ids=["bf16", "f16"])
+@pytest.mark.parametrize("s", [4, 40], ids=["few", "many"])
+def test_attention_masked_nonfinite_tail_values(s, dtype):
+    """An infinite or NaN value in the tail: NaN for the queries that see its position, nothing for the others."""
+    gen = seeded(5)
+    b, hq, h, total = 2, 4, 2, 110
+    c, k, v = filled(b, h, total, dtype, gen)
+    q = randn(b, s, hq, 128, gen=gen, dtype=dtype).cuda()
+    start = total - s
+    want = I8.attention(q, c, start)
+    for pos, dim, x in ((total - 1, 0, math.nan), (total - 3, 77, math.inf), (total - 2, 127, -math.inf), (64, 5, math.nan)):
+        keep = c.v_tail[1, 1, dim, pos - 64].clone()
+        c.v_tail[1, 1, dim, pos - 64] = x
+        got = I8.attention(q, c, start)
+        sees = max(pos - start, 0)
+        assert torch.equal(got[0], want[0]) and torch.equal(got[1, :, :2], want[1, :, :2]), (pos, dim)
+        assert torch.equal(got[1, :sees, 2:], want[1, :sees, 2:]) and torch.isnan(got[1, sees:, 2:]).all(), (pos, dim)
+        c.v_tail[1, 1, dim, pos - 64] = keep
+
+
+@pytest.mark.parametrize("s", [1, 70])
+def test_attention_nonfinite_values_of_no_weight(s):
+    """A block of values that were not finite makes a query that sees it NaN, however small the block's weight."""
+    gen = seeded(6)
+    k, v = (randn(1, 192 + s, 1, 128, gen=gen, dtype=torch.float32) for _ in range(2))
+    q = randn(1, s, 2, 128, gen=gen, dtype=torch.float32)
+    k[:, :64] = -40.0   # its scores lie thousands below the others': weights of 0
+    q += 40.0
+    c = poisoned(1, 1, 192 + s, torch.bfloat16)
+    I8.append(k.bfloat16().cuda(), v.bfloat16().cuda(), c, 0)
+    assert torch.isfinite(I8.attention(q.bfloat16().cuda(), c, 192)).all()
+    c.v_scale[0, 0, 0] = math.nan
+    assert torch.isnan(I8.attention(q.bfloat16().cuda(), c, 192)).all()
+
+
 def test_device_positions_and_graph_replay():
     """One captured step (append + attention at a device position) replayed over a block's end against eager calls."""
     gen = seeded(6)
