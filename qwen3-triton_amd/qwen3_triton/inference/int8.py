@@ -172,7 +172,7 @@ def _desc(x, operand, rows, k, weights, outs, epilogue, dtype, residual):
 
 
 def _product(q, scale, weights, outs, epilogue, dtype, residual=None):
-    _forward_only(residual)
+    _forward_only(scale, residual, *(ws for _, ws in weights))
     rows, ld, k = _check_codes(q, scale)
     d = _desc(q, (q.data_ptr(), ld, scale.data_ptr()), rows, k, weights, outs, epilogue, dtype, residual)
     nbytes = H.query("q3_gemm_int8_workspace_bytes", d) if rows > 16 else 0   # up to 16 rows never take any
@@ -222,15 +222,15 @@ def gate_up_swiglu(q, scale, gate, gate_scale, up, up_scale, *, dtype=torch.bflo
 
 def decode_linear_ok(x):
     """Whether ``decode_linear`` takes rows like x [..., K]: at most 2, of at most 16384 values."""
-    k = x.shape[-1]
-    return bool(H.query("q3_decode_linear_int8_ok", x.numel() // k, k))
+    k = x.shape[-1] if x.ndim else 0
+    return k > 0 and bool(H.query("q3_decode_linear_int8_ok", x.numel() // k, k))
 
 
 def decode_linear(x, weights, *, norm_weight=None, eps=1e-6, gate_up=False, residual=None):
     """A decode step's product straight from 16-bit rows x [..., K]: ``quantize_rows`` (with ``norm_weight`` ``rms_norm``) and
     ``projections`` of up to three weights [(codes, scales), ...] in one launch -> a list; with ``gate_up`` the SwiGLU of
     two -> one tensor; with ``residual`` [..., N] one weight's product plus it -> one tensor."""
-    _forward_only(x, norm_weight, residual)
+    _forward_only(x, norm_weight, residual, *(ws for _, ws in weights))
     rows, ld, k = _check_rows(x)
     if not decode_linear_ok(x):
         raise ValueError('decode_linear takes at most 2 rows of at most 16384 values')
@@ -313,6 +313,8 @@ class LayerCache:
         for t in tensors:
             if t.device != dev or not t.is_contiguous() or t.data_ptr() % 16 and t.dtype != torch.float32:
                 raise ValueError('contiguous, 16-byte aligned cache buffers on one device required')
+            if t.requires_grad:
+                raise ValueError('cache buffers take no gradient')
 
     def pointers(self):
         return (self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
@@ -375,7 +377,7 @@ def _check_norm_rope(q, q_norm_weight, k_norm_weight, cos, sin, eps):
 def norm_rope_append(q, k, v, q_norm_weight, k_norm_weight, cos, sin, cache, start, start_dev=None, *, eps=1e-6):
     """Per-head RMSNorm and rotation of q [B, S, Hq, 128] and k [B, S, Hkv, 128] as projected (tables cos, sin [B, S, 128])
     and ``append`` of those keys and v, in one launch; returns the normed and rotated q, contiguous."""
-    _forward_only(q, k, v, q_norm_weight, k_norm_weight)
+    _forward_only(q, k, v, q_norm_weight, k_norm_weight, cos, sin)
     qs, ks, vs = (_check_heads(t, cache, what) for t, what in ((q, 'queries'), (k, 'keys'), (v, 'values')))
     b, s, hq, d = q.shape
     h = k.shape[2]

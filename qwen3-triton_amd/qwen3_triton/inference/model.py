@@ -111,6 +111,9 @@ class Int8KVCache(KVCache):
     def nbytes(self):
         return sum(layer.nbytes for layer in self.layers)
 
+    def quantized(self):
+        raise ValueError('the cache is in int8 already')
+
     def dequantized(self):
         """A bf16 ``KVCache`` of the same positions (a request that goes on in 16 bits)."""
         shape = (*self.layers[0].k.shape[:2], self.capacity, 128)
@@ -163,6 +166,7 @@ class TritonQwen3Inference(nn.Module):
         self.gemv, self.split_decode = gemv, split_decode
         self._cache_owner = object()
         self._int8 = None   # per layer, once quantize_weights has run
+        self._weights = object()   # replaced when the weights that captured steps read are freed
         self.generation_config = _generation_config(config)
         self.eval()
 
@@ -175,7 +179,8 @@ class TritonQwen3Inference(nn.Module):
         if wrong:
             raise ValueError(f'bf16 inference weights required; {wrong[0]} is not bf16')
         self.load_state_dict(state, assign=True, strict=True)
-        self._int8 = None
+        if self._int8 is not None:
+            self._int8, self._weights = None, object()
         if tied:
             self.lm_head.weight = self.model.embed_tokens.weight
         self.model.rotary_emb.inv_freq = self._inv_freq().to(self.lm_head.weight.device)
@@ -222,7 +227,8 @@ class TritonQwen3Inference(nn.Module):
     def quantize_weights(self):
         """Hold the layers' seven projections in int8 with a scale per output channel, from now on, and free their bf16
         weights (the embedding, the norms and the LM head stay in bf16).  Each projection's input is then quantised per
-        token.  ``load_hf_state_dict`` goes back to bf16."""
+        token.  ``load_hf_state_dict`` goes back to bf16.  Steps captured before (``DecodeSession.capture``,
+        ``CapturedGreedyRequest``) read the freed weights: they refuse to replay and have to be captured again."""
         if self._int8 is not None:
             raise ValueError('the weights are already in int8')
         if self.device.type != 'cuda':
@@ -237,8 +243,13 @@ class TritonQwen3Inference(nn.Module):
             for part in (layer.self_attn, layer.mlp):
                 for proj in (p for name, p in part.named_children() if name.endswith('_proj')):
                     proj.weight = nn.Parameter(torch.empty_like(proj.weight, device='meta'), requires_grad=False)
-        self._int8 = held
+        self._int8, self._weights = held, object()
         return self
+
+    def state_dict(self, *args, **kwargs):
+        if self._int8 is not None:
+            raise ValueError('quantize_weights has freed the bf16 weights: no state to save')
+        return super().state_dict(*args, **kwargs)
 
     @property
     def device(self):
@@ -497,6 +508,12 @@ def _generation_config(config):
         return None
 
 
+def _check_captured(session):
+    """Raise if the weights that a captured step reads have been freed since."""
+    if session._weights is not session.model._weights:
+        raise RuntimeError('captured before the model\'s weights were replaced: capture again')
+
+
 class DecodeSession:
     """Greedy decoding with ONE captured HIP graph for the decode step, replayed at every position.
 
@@ -552,7 +569,7 @@ class DecodeSession:
         host_len = self.cache.length
         stream = torch.cuda.Stream(device=self.model.device)
         stream.wait_stream(torch.cuda.current_stream())
-        self.graph = torch.cuda.CUDAGraph()
+        self.graph, self._weights = torch.cuda.CUDAGraph(), self.model._weights
         with torch.cuda.graph(self.graph, stream=stream):
             self._step()
         torch.cuda.current_stream().wait_stream(stream)
@@ -565,6 +582,7 @@ class DecodeSession:
         if self.graph is None:
             self._step()
             return
+        _check_captured(self)
         self.graph.replay()
         self.cache.length += 1
 
@@ -611,7 +629,7 @@ class CapturedGreedyRequest:
             self._prefill()
             if max_new_tokens > 1:
                 self._step()
-        self.prefill_graph = torch.cuda.CUDAGraph()
+        self.prefill_graph, self._weights = torch.cuda.CUDAGraph(), model._weights
         self.cache.reset()
         with torch.cuda.graph(self.prefill_graph, stream=stream):
             self._prefill()
@@ -649,6 +667,7 @@ class CapturedGreedyRequest:
         if tuple(input_ids.shape) != self.shape or input_ids.device != self.model.device or \
                 input_ids.dtype != self.input.dtype:
             raise ValueError(f'prompt must match the captured {self.shape} {self.input.dtype} on {self.model.device}')
+        _check_captured(self)
         self.busy = True
         try:
             _check_vocab(self.model, input_ids)

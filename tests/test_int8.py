@@ -196,3 +196,28 @@ def test_python_refusals_without_a_device():
         I8.LayerCache.empty(1, 2, 64, device='cpu', dtype=torch.float32)
     with pytest.raises(ValueError, match='one to three'):
         I8.projections(x, x, [])
+
+
+def test_gradients_are_refused():
+    x = torch.zeros(1, 32)
+    q, w, one = torch.zeros(1, 32, dtype=torch.int8), torch.zeros(8, 32, dtype=torch.int8), torch.ones(1)
+    learned = torch.ones(8, requires_grad=True)
+    for call in (lambda: I8.linear(q, one, w, learned), lambda: I8.linear(q, one.clone().requires_grad_(), w, torch.ones(8)),
+                 lambda: I8.gate_up_swiglu(q, one, w, torch.ones(8), w, learned),
+                 lambda: I8.projections(q, one, [(w, torch.ones(8)), (w, learned)]),
+                 lambda: I8.decode_linear(x.bfloat16(), [(w, learned)])):
+        with pytest.raises(ValueError, match='forward only'):
+            call()
+    cos = torch.zeros(1, 1, 128, dtype=torch.bfloat16, requires_grad=True)
+    t = torch.zeros(1, 1, 1, 128, dtype=torch.bfloat16)
+    cache = I8.LayerCache.empty(1, 1, 64, device='cpu')
+    with pytest.raises(ValueError, match='forward only'):
+        I8.norm_rope_append(t, t, t, t[0, 0, 0], t[0, 0, 0], cos, cos, cache, 0)
+    with pytest.raises(ValueError, match='no gradient'):
+        I8.LayerCache(cache.k, cache.v, cache.k_scale.requires_grad_(), cache.v_scale, cache.k_tail, cache.v_tail)
+
+
+def test_decode_linear_ok_of_nothing():
+    for shape in ((), (0,), (3, 0), (0, 32)):
+        assert not I8.decode_linear_ok(torch.zeros(shape, dtype=torch.bfloat16))
+    assert I8.decode_linear_ok(torch.zeros(2, 16384)) and not I8.decode_linear_ok(torch.zeros(3, 16384))

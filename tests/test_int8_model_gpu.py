@@ -250,3 +250,33 @@ def test_integer_sums_do_not_depend_on_the_batch():
     whole = int8.linear(q, s, *w)
     for m in (1, 5, 16, 17, 40, 130, 300):
         assert torch.equal(int8.linear(q[:m], s[:m], *w), whole[:m])
+
+
+def test_replaced_weights_end_captured_steps_and_state():
+    """A captured step reads the weights that it was captured with: once they are freed it refuses to replay."""
+    model, params = build(False)
+    ids = torch.arange(12, device='cuda').view(1, 12)
+    session = DecodeSession(model, 1, 32)
+    session.prefill(ids)
+    session.capture()
+    session.step()
+    request = CapturedGreedyRequest(model, ids, max_new_tokens=3)
+    request(ids)
+    assert model.state_dict()
+    model.quantize_weights()
+    with pytest.raises(RuntimeError, match='capture again'):
+        session.step()
+    with pytest.raises(RuntimeError, match='capture again'):
+        request(ids)
+    with pytest.raises(ValueError, match='no state'):
+        model.state_dict()
+    session.capture()
+    session.step()
+    request = CapturedGreedyRequest(model, ids, max_new_tokens=3)
+    assert torch.equal(request(ids), model.generate(ids, max_new_tokens=3, eos_token_id=()))
+    model.load_hf_state_dict({k: v.cuda() for k, v in params.items()})
+    with pytest.raises(RuntimeError, match='capture again'):
+        request(ids)
+    assert model.state_dict()
+    with pytest.raises(ValueError, match='already'):
+        model.new_cache(1, 16, dtype=torch.int8).quantized()
