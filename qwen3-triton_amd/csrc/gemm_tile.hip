@@ -30,13 +30,13 @@ constexpr Cfg kCfg[kNumCfg] = {{256, 256, 1, 1.27, 1.48}, {128, 256, 1, 0.86, 0.
                                {64, 128, 1, 0.28, 0.32},  {64, 64, 2, 0.34, 0.70},   {32, 64, 3, 0.27, 1.04},
                                {192, 256, 1, 0.98, 1.25}, {192, 128, 1, 0.61, 0.68}};
 // The same tiles on 8-bit codes, 128 to a k-tile: a k-tile holds the same bytes and matrix instructions, but the scales'
-// epilogue is longer and the small tiles keep up better.  Fitted with estimate()'s other two constants to 70 shapes (M
-// 17-8192, N 152-24576, K 272-12288), and then timed on 40 others: the plan is 2 % slower on average than the best tile and
-// split, 23 % at worst (57 x 9688 x 7792: 32.8 against 26.7 us).  On the first 70 the 16-bit constants were 3.4 % slower on
-// average and 32 % at worst (128 x 6144 x 4096: 18.4 against 14.1 us), these 1 % and 9 %.
-constexpr Cfg kCfgInt8[kNumCfg] = {{256, 256, 1, 1.49, 1.58}, {128, 256, 1, 1.11, 1.25}, {128, 128, 1, 0.77, 0.87},
-                                   {64, 128, 1, 0.38, 0.43},  {64, 64, 2, 0.30, 0.65},   {32, 64, 3, 0.20, 0.80},
-                                   {192, 256, 1, 1.18, 1.30}, {192, 128, 1, 0.77, 0.80}};
+// epilogue is longer, the waves of some tiles are more and the small tiles keep up better.  Fitted with estimate()'s other two
+// constants to 110 shapes (M 17-8192, N 104-24576, K 256-12288; 1 % slower on average than the best tile and split), then timed
+// on 40 others: 2 % slower on average, 17 % at worst (920 x 12200 x 896: 20.7 against 17.7 us).  The 16-bit constants are 3.4 %
+// slower on average and 32 % at worst on 70 of the first.
+constexpr Cfg kCfgInt8[kNumCfg] = {{256, 256, 1, 1.58, 1.66}, {128, 256, 1, 0.96, 1.03}, {128, 128, 1, 0.63, 0.66},
+                                   {64, 128, 1, 0.40, 0.44},  {64, 64, 2, 0.28, 0.64},   {32, 64, 3, 0.20, 0.80},
+                                   {192, 256, 1, 1.12, 1.77}, {192, 128, 1, 0.78, 0.88}};
 // Instantiated layouts: the 192-row tiles for a k-contiguous A (they fill the CUs where 256 rows would leave the
 // last row of tiles half empty: 1500 x 24576 x 4096 247 against 279 us), 32 rows for two k-contiguous operands.
 bool cfg_for(int c, bool at, bool bt) { return c < 5 || (c == 5 ? !bt : !at); }
@@ -57,7 +57,7 @@ struct Plan {
 // 15 us against 47 us on 32 tiles of 128 x 128).
 double estimate(int c, bool int8, int splits, int64_t tiles, int64_t M, int64_t N, int64_t K, double combine) {
   const Cfg& f = int8 ? kCfgInt8[c] : kCfg[c];
-  const double base = int8 ? 3.5 : 5.6, traffic = int8 ? 3.3e6 : 5e6;
+  const double base = int8 ? 3.5 : 5.6, traffic = int8 ? 3.1e6 : 5e6;
   const int64_t w = tiles * splits, slots = 256 * f.conc;
   const int64_t kt = cdiv(cdiv(K, 64), splits), r = w / slots, rem = w % slots;
   const double last = rem ? std::max(f.solo, f.full * (double)rem / (double)slots) : 0.0;
