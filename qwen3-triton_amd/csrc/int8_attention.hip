@@ -12,6 +12,10 @@
 // scales only when one is more than 16 times off it.  P in fp16 has 11 bits where bf16 has 8, and unit keeps it in range.
 // The running maximum and sum of the softmax are per row, replicated over the 4 lane groups.
 // The unfinished block is read from the 16-bit tail in the same lane order (V tail transposed as well).
+// Bound by HBM at one token over a long cache (8 rows x 20001 positions x 8 heads: 58.8 us, 5.6 TB/s), by latency over a short
+// one (2048 positions: 5.8 us + 2.2 - 3.3 for the join); with many queries by the vector units' exponentials and conversions,
+// the matrix cores and LDS, about 2500, 2050 and 2050 cycles of a 256-row block's 5000 (8192 queries of 32 heads: 537 us, as the
+// 16-bit kernel's 501 - 576; 1024 queries at 3000: 79 - 86 us + 9.5).
 #include <algorithm>
 
 #include "int8_cache.h"
@@ -405,7 +409,9 @@ Q3_DEV void store_rows(const AttnArgs& a, const Span& p, int b, int hk, int spli
 }
 
 // Few rows (at most 16 per key/value head: one token of a group, a few of a small one): four waves share the rows and take
-// every fourth block each, their K and V fragments straight from memory, and join through LDS.
+// every fourth block each, their K and V fragments straight from memory, and join through LDS.  Heads before splits in the
+// grid: a head's splits on one XCD, where the join finds them (2048 positions 8.5 us with the join, splits first 10.5; at
+// 8 x 20001 positions splits first is 5 % faster).
 template <typename T> __global__ __launch_bounds__(256) void kv8_attn_rows_kernel(AttnArgs a) {
   constexpr int RT = 1, WK = 4;
   const int lane = threadIdx.x & 63, wk = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);

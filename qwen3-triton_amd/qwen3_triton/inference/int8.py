@@ -264,7 +264,7 @@ class LayerCache:
 
     A block is quantised once, from its 16-bit values, when its last position is appended; so what the cache holds does
     not depend on how the tokens were cut into chunks.  Positions are appended in order: the cache cannot be wound back
-    into a block that is already quantised (start again from 0)."""
+    into a block that is already quantised (start again from 0 or another multiple of 64)."""
     k: torch.Tensor
     v: torch.Tensor
     k_scale: torch.Tensor

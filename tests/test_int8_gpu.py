@@ -209,6 +209,35 @@ def test_decode_linear(m, k, norm, dtype):
             assert torch.equal(got, want)
 
 
+@pytest.mark.parametrize("m", [1, 2, 9, 16])
+@pytest.mark.parametrize("k", [272, 2048, 4352])
+def test_few_rows_many_channels(m, k):
+    """More channels than the workgroups of a launch take in one go: each goes on to others, over the pieces' borders."""
+    gen = seeded(m + k)
+    dtype = torch.bfloat16
+    x = randn(m, k, gen=gen, dtype=dtype).cuda()
+    q, s = I8.quantize_rows(x)
+    _, _, w, ws = product_inputs(1, 17016, k, gen)
+    wd, wsd = w.cuda(), ws.cuda()
+    ref = product64(q.cpu(), s.cpu(), w, ws)
+    tol = torch.finfo(dtype).eps / 2 * (1 + 2.0 ** -10) + 2.0 ** -21
+    y = I8.linear(q, s, wd, wsd)
+    close(y, ref, ref.abs() * tol + 1e-7)
+    ends = (0, 8216, 8240, 17016)
+    pieces = [(wd[a:b], wsd[a:b]) for a, b in zip(ends, ends[1:])]
+    for got, a, b in zip(I8.projections(q, s, pieces), ends, ends[1:]):
+        assert torch.equal(got, y[:, a:b])
+    even = [(wd[:8504], wsd[:8504]), (wd[8512:], wsd[8512:])]
+    g, u = ref[:, :8504], ref[:, 8512:]
+    z = I8.gate_up_swiglu(q, s, *even[0], *even[1])
+    want = g * torch.sigmoid(g) * u
+    close(z, want, want.abs() * (torch.finfo(dtype).eps / 2 * (1 + 2.0 ** -10) + (12 + 6 * g.abs()) * 2.0 ** -23) + 1e-7)
+    if m <= 2:
+        for got, a, b in zip(I8.decode_linear(x, pieces), ends, ends[1:]):
+            assert torch.equal(got, y[:, a:b])
+        assert torch.equal(I8.decode_linear(x, even, gate_up=True), z)
+
+
 def test_decode_linear_refusals_and_nonfinite_rows():
     x = randn(3, 64, gen=seeded(1), dtype=torch.bfloat16).cuda()
     w = I8.quantize_rows(randn(32, 64, gen=seeded(2), dtype=torch.bfloat16).cuda())
@@ -446,6 +475,21 @@ def test_attention_value_scales_far_apart(dtype):
         q = wide[:, :, 1:5, 64:192]
         o = I8.attention(q, c, t - s, scale=0.3)
         check_attention(o, q.cpu(), held64(k, v)[0], t - s, 0.3, dtype)
+
+
+def test_cache_started_again_at_a_block():
+    """Positions appended again from a multiple of 64 on: as if the earlier ones had never been."""
+    gen = seeded(7)
+    c, k, v = filled(2, 2, 200, torch.bfloat16, gen)
+    k2, v2 = (randn(2, 90, 2, 128, gen=gen, dtype=torch.bfloat16).cuda() for _ in range(2))
+    fresh = poisoned(2, 2, 200, torch.bfloat16)
+    for start in (128, 64, 0):
+        I8.append(k2, v2, c, start)
+        if start:
+            I8.append(k[:, :start].cuda(), v[:, :start].cuda(), fresh, 0)
+        I8.append(k2, v2, fresh, start)
+        for got, want in zip(I8.read(c, start + 90), I8.read(fresh, start + 90)):
+            assert torch.equal(got, want), start
 
 
 def test_attention_masked_nonfinite_positions():
