@@ -776,11 +776,13 @@ Plan plan_for(int64_t B, int64_t Hkv, int64_t rows, int64_t span) {
   Plan p;
   p.tile = rows > 16;
   p.row_blocks = p.tile ? (rows + 255) / 256 : 1;
-  // eight waves on every CU; a block for each wave of a split, or enough of them to pay for the join
-  // where the rows fill the CUs without (32 x 300 positions: 13.1 us in two splits, 10.7 in one)
+  // Eight waves on every CU.  A split takes at least four blocks: one for each wave of the rows kernel, and enough for the tile
+  // kernel's start (17 queries at 2000: 41.8 us at sixteen, 28.1 at eight, 21.6 at four, 19.6 at two; but 200 at 0 16.4, 16.4,
+  // 16.3 and 19.6).  Where the rows fill the CUs without splits, sixteen, to pay for the join (32 x 300 positions: 13.1 us in two
+  // splits, 10.7 in one).
   const int64_t wgs = B * Hkv * p.row_blocks;
   p.max_splits = (int)std::min<int64_t>(1024, std::max<int64_t>(1, (p.tile ? 256 : 512) / wgs));
-  p.minper = p.tile || wgs >= 256 ? 16 : 4;
+  p.minper = wgs >= 256 ? 16 : 4;
   const int64_t blocks = (span + BLK - 1) / BLK;
   p.splits = (int)std::min<int64_t>(p.max_splits, (blocks + p.minper - 1) / p.minper);
   return p;
