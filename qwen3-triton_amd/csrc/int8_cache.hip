@@ -31,8 +31,9 @@ template <typename T, bool NR> __global__ __launch_bounds__(256) void kv8_append
   const int h = (int)(job % a.H);  // heads next to each other, as their rows are in memory
   job /= a.H;
   const int64_t start = a.start_dev ? *a.start_dev : a.start;
-  if (values) append_part<T, NR, true>(a, (int)(job % a.blocks), h, (int)(job / a.blocks), start);
-  else append_part<T, NR, false>(a, (int)(job % a.blocks), h, (int)(job / a.blocks), start);
+  const int b = (int)(job % a.B), part = (int)(job / a.B);  // the parts that may read the tail first: they take longest
+  if (values) append_part<T, NR, true>(a, part, h, b, start);
+  else append_part<T, NR, false>(a, part, h, b, start);
 }
 
 struct ReadArgs {
@@ -98,14 +99,21 @@ template <typename T, typename O> __global__ __launch_bounds__(256) void kv8_rea
   }
   const u16* tk = a.tk + bh * (BLK * D) + 4 * r * D + 8 * i;
   const u16* tv = a.tv + bh * (BLK * D) + 8 * i * BLK + 4 * r;
+  i32x4 kraw[4];
+  i32x2 vraw[8];  // a dim's four positions
+#pragma unroll
+  for (int c = 0; c < 4; ++c) kraw[c] = *reinterpret_cast<const i32x4*>(tk + c * D);
+#pragma unroll
+  for (int e = 0; e < 8; ++e) vraw[e] = *reinterpret_cast<const i32x2*>(tv + e * BLK);
 #pragma unroll
   for (int c = 0; c < 4; ++c) {
     if (pos0 + c >= a.length) continue;
+    const Vec<T> k = unpack_vec<T>(kraw[c]);
     float x[8], y[8];
 #pragma unroll
     for (int e = 0; e < 8; ++e) {
-      x[e] = to_f32<T>(tk[c * D + e]);
-      y[e] = to_f32<T>(tv[e * BLK + c]);
+      x[e] = k.v[e];
+      y[e] = to_f32<T>((u16)((uint32_t)vraw[e][c >> 1] >> (16 * (c & 1))));
     }
     store(ko + c * D, x);
     store(vo + c * D, y);
