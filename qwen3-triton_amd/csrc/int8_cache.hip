@@ -1,7 +1,7 @@
 // Writing new positions into the key/value cache in 8 bits (int8_cache.h), and reading the cache back to 16 or 32 bits.
 // Bound by HBM (a prompt's 2 + 1 bytes per value, and back), by latency at one token.  Measured with 8 heads: 8192 positions
 // appended in 15.8 us (3.2 TB/s; a copy of the same bytes 11.7 us, the quantisation about 4 on top of it), read back in 9.0
-// (5.6 TB/s); one token of 8 rows 2.2 us, 5.6 - 8.2 us where it completes a block, whose 64 positions are then read from the
+// (5.6 TB/s); one token of 8 rows 2.3 us, 5.8 - 8.3 us where it completes a block, whose 64 positions are then read from the
 // tail, in one chain of three waits.
 #include "int8_cache.h"
 
