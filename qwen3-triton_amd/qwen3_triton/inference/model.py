@@ -234,7 +234,7 @@ class TritonQwen3Inference(nn.Module):
         if self.device.type != 'cuda':
             raise ValueError('the weights are not on a ROCm device (load or move them first)')
         c = self.config
-        for n in (c.hidden_size, c.intermediate_size):
+        for n in (c.hidden_size, c.intermediate_size, c.num_attention_heads * c.head_dim):
             if n % 16 or n > int8.MAX_ROW:
                 raise ValueError(f'sizes that are multiples of 16 and at most {int8.MAX_ROW} required for int8, not {n}')
         held = []
@@ -326,7 +326,8 @@ class TritonQwen3Inference(nn.Module):
         """The decoder layers on int8 weights: every projection's input is quantised where it is formed (the norms carry
         the residual sums)."""
         b, s, _ = x.shape
-        if int8.decode_linear_ok(x) and self.config.intermediate_size <= 16384:
+        c = self.config
+        if int8.decode_linear_ok(x) and max(c.intermediate_size, c.num_attention_heads * c.head_dim) <= 16384:
             return self._int8_decode(x, cos, sin, cache, start, start_dev)
         down = None
         for i, (layer, w) in enumerate(zip(self.model.layers, self._int8)):

@@ -551,6 +551,57 @@ def test_attention_nonfinite_values_of_no_weight(s):
     assert torch.isnan(I8.attention(q.bfloat16().cuda(), c, 192)).all()
 
 
+def test_cache_past_32_bits():
+    """2.2 million positions of 8 heads: codes, 16-bit sources and read-back values past 2^31 elements.  The last head against
+    the same calls on a cache of that head alone."""
+    total, h, dtype = 2_200_037, 8, torch.bfloat16
+    gen = torch.Generator(device="cuda").manual_seed(8)
+    k, v = (torch.randn((1, total, h, 128), generator=gen, device="cuda", dtype=dtype) for _ in range(2))
+    c = I8.LayerCache.empty(1, h, total, device="cuda", dtype=dtype)
+    one = I8.LayerCache.empty(1, 1, total, device="cuda", dtype=dtype)
+    at = 0
+    for end in (1_500_000, total):
+        I8.append(k[:, at:end], v[:, at:end], c, at)
+        I8.append(k[:, at:end, 7:], v[:, at:end, 7:], one, at)
+        at = end
+    full, rest = total // 64, total % 64
+    assert torch.equal(c.k[:, 7:, :full * 64], one.k[:, :, :full * 64]) and torch.equal(c.v[:, 7:, :full], one.v[:, :, :full])
+    assert torch.equal(c.k_tail[:, 7:, :rest], one.k_tail[:, :, :rest])
+    for got, want in zip(I8.read(c, total), I8.read(one, total)):
+        assert torch.equal(got[:, 7:], want)
+    del k, got, want
+    top = float(v[:, :, 7].abs().max())
+    for s in (1, 40):
+        q = torch.randn((1, s, 16, 128), generator=gen, device="cuda", dtype=dtype) * 4
+        a = I8.attention(q, c, total - s)[:, :, 14:].double()
+        b = I8.attention(q[:, :, 14:], one, total - s).double()
+        # two splits of one sum: P rounded to fp16 in either (2^-11 of sum p |v| <= top), fp32 sums and joins, an output rounding
+        tol = 2 * top * (2.0 ** -11 + 2.0 ** -15)
+        assert ((a - b).abs() <= tol + b.abs() * torch.finfo(dtype).eps * (1 + 2.0 ** -8)).all()
+        # the outputs stand clear of it, so that another head's would show: scores of deviation 4 leave the largest of 2.2
+        # million (about 5 deviations up) more than a hundredth of the sum, 2.2e6 e^8 against e^20 and more: 0.07 of a value
+        assert float(b.abs().max()) > 10 * tol
+
+
+def test_rows_past_32_bits():
+    """70000 rows of 32768: values and codes past 2^31 elements; rows here and there against calls on those rows alone."""
+    gen = torch.Generator(device="cuda").manual_seed(9)
+    x = torch.randn((70000, 32768), generator=gen, device="cuda", dtype=torch.bfloat16)
+    w = torch.rand(32768, generator=gen, device="cuda").bfloat16()
+    wq, ws = I8.quantize_rows(x[:48])
+    parts = (slice(0, 3), slice(65530, 65545), slice(69990, 70000))
+    q, s = I8.quantize_rows(x)
+    y = I8.linear(q, s, wq, ws)
+    for p in parts:
+        a, b = I8.quantize_rows(x[p])
+        assert torch.equal(q[p], a) and torch.equal(s[p], b) and torch.equal(y[p], I8.linear(a, b, wq, ws))
+    del q, s, y
+    q, s, total = I8.rms_norm(x, w, 1e-6, residual=x)
+    for p in parts:
+        for got, want in zip((q[p], s[p], total[p]), I8.rms_norm(x[p], w, 1e-6, residual=x[p])):
+            assert torch.equal(got, want)
+
+
 def test_device_positions_and_graph_replay():
     """One captured step (append + attention at a device position) replayed over a block's end against eager calls."""
     gen = seeded(6)

@@ -280,3 +280,15 @@ def test_replaced_weights_end_captured_steps_and_state():
     assert model.state_dict()
     with pytest.raises(ValueError, match='already'):
         model.new_cache(1, 16, dtype=torch.int8).quantized()
+
+
+@pytest.mark.parametrize("heads,kv,cache_dtype", [(144, 18, BF), (144, 18, torch.int8), (144, 9, torch.int8), (130, 2, torch.int8)])
+def test_more_heads_than_a_fused_product_takes(heads, kv, cache_dtype):
+    """The output projection's rows (18432 and 16640 values) are longer than decode_linear's.  More than 8 heads of a group
+    decode over the int8 cache only: attention over the 16-bit one refuses them, whatever the weights."""
+    oc = O.OracleConfig(vocab_size=200, hidden_size=128, intermediate_size=256, num_hidden_layers=1, num_attention_heads=heads,
+                        num_key_value_heads=kv, head_dim=128)
+    model = TritonQwen3Inference.random_init(hf_config(oc), seed=3, std=0.05).quantize_weights()
+    ids = torch.arange(9, device='cuda').view(1, 9)
+    out = model.generate(ids, max_new_tokens=4, eos_token_id=(), cache_dtype=cache_dtype)
+    assert torch.equal(out, CapturedGreedyRequest(model, ids, max_new_tokens=4, cache_dtype=cache_dtype)(ids))
