@@ -302,6 +302,42 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile_kernel(Args ar) {
 #pragma unroll
     for (int j = 0; j < FN; ++j) acc[i][j] = acc_t{0, 0, 0, 0};
 
+  // Q8: the scales of this lane's rows and of its columns (four to a block; gate/up: of Wg and Wu in turn); where there are few of
+  // them, with the residual's values, ahead of the first tiles, so that the epilogue need not wait for them
+  [[maybe_unused]] float rsc[Q8 ? FM : 1];
+  [[maybe_unused]] f32x4 col_s[Q8 ? FN : 1];
+  constexpr bool EARLY = Q8 && FM + 4 * FN <= 20;
+  [[maybe_unused]] i32x2 res_v[EARLY && EPI == 0 ? FM : 1][EARLY && EPI == 0 ? FN : 1];
+  [[maybe_unused]] auto load_scales = [&]() {
+    if constexpr (Q8) {
+      typedef float f32x4u __attribute__((ext_vector_type(4), aligned(4)));
+#pragma unroll
+      for (int i = 0; i < FM; ++i) rsc[i] = ar.rscale[begm + min(ma + wm * TMW + i * 16 + j16, mrows - 1)];
+#pragma unroll
+      for (int j = 0; j < FN; ++j) {
+        constexpr int DIV = EPI == 3 ? 2 : 1;
+        const int col = (nb + wn * TNW) / DIV + j / DIV * 16 + 4 * quarter, lim = ncols / DIV;
+        col_s[j] = *reinterpret_cast<const f32x4u*>((EPI == 3 && (j & 1) ? ar.cscale[1] : csc) + min(col, lim - 4));
+      }
+    }
+  };
+  if constexpr (EARLY) {
+    if (ar.splits == 1 && (ar.vec || EPI == 3)) {
+      load_scales();
+      if constexpr (EPI == 0) {
+        if (ar.res) {
+#pragma unroll
+          for (int i = 0; i < FM; ++i)
+#pragma unroll
+            for (int j = 0; j < FN; ++j) {
+              const int row = min(ma + wm * TMW + i * 16 + j16, mrows - 1);
+              const int col = min(nb + wn * TNW + j * 16 + 4 * quarter, ncols - 4);
+              res_v[i][j] = *reinterpret_cast<const i32x2*>(ar.res + (int64_t)row * ar.ldres + col);
+            }
+        }
+      }
+    }
+  }
 #pragma unroll
   for (int st = 0; st < STAGES - 1; ++st) {
     prep();
@@ -402,11 +438,6 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile_kernel(Args ar) {
     return;
   }
   u16* C = reinterpret_cast<u16*>(cp);
-  // Q8: this lane's element e of block (i, j) in fp32, by its row's and column's scales
-  [[maybe_unused]] auto scaled = [&](int i, int j, const float* cs, int col, int lim, float rs, float (&v)[4]) {
-#pragma unroll
-    for (int e = 0; e < 4; ++e) v[e] = (float)acc[i][j][e] * rs * cs[min(col + e, lim - 1)];
-  };
   if constexpr (Q8) {
     // One rounding: the product scaled, the residual (or SwiGLU) formed in fp32, then staged through LDS as below
     if (ar.vec || EPI == 3) {
@@ -415,22 +446,23 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile_kernel(Args ar) {
       char* wl = lds + wave * (TMW * NC * 2);
       auto swz = [&](int r) { return CH == 16 ? (r & 15) : CH == 8 ? ((r >> 1) & 7) : CH == 4 ? ((r >> 2) & 3) : ((r >> 3) & 1); };
       const int cb = (nb + wn * TNW) / DIV, clim = ncols / DIV;  // the wave's first output column, their number
+      if constexpr (!EARLY) load_scales();
 #pragma unroll
-      for (int i = 0; i < FM; ++i) {
-        const int row = min(ma + wm * TMW + i * 16 + j16, mrows - 1);
-        const float rs = ar.rscale[begm + row];
+      for (int j = 0; j < FN; j += DIV) {
+        const int col = cb + j / DIV * 16 + 4 * quarter;
 #pragma unroll
-        for (int j = 0; j < FN; j += DIV) {
-          const int col = cb + j / DIV * 16 + 4 * quarter;
+        for (int i = 0; i < FM; ++i) {
           float v[4];
-          scaled(i, j, csc, col, clim, rs, v);
-          if constexpr (EPI == 3) {
-            float u[4];
-            scaled(i, j + 1, ar.cscale[1], col, clim, rs, u);
 #pragma unroll
-            for (int e = 0; e < 4; ++e) v[e] = v[e] * q3_sigmoid(v[e]) * u[e];
+          for (int e = 0; e < 4; ++e) v[e] = (float)acc[i][j][e] * rsc[i] * col_s[j][e];
+          if constexpr (EPI == 3) {
+#pragma unroll
+            for (int e = 0; e < 4; ++e) v[e] = v[e] * q3_sigmoid(v[e]) * ((float)acc[i][j + 1][e] * rsc[i] * col_s[j + 1][e]);
           } else if (ar.res && col < clim) {  // whole 8-column groups: col + 3 is a column too
-            const i32x2 x = *reinterpret_cast<const i32x2*>(ar.res + (int64_t)row * ar.ldres + col);
+            const int row = min(ma + wm * TMW + i * 16 + j16, mrows - 1);
+            i32x2 x;
+            if constexpr (EARLY) x = res_v[i][j];
+            else x = *reinterpret_cast<const i32x2*>(ar.res + (int64_t)row * ar.ldres + col);
 #pragma unroll
             for (int e = 0; e < 4; ++e) v[e] += to_f32<T>((u16)((uint32_t)x[e >> 1] >> (16 * (e & 1))));
           }
@@ -459,13 +491,12 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile_kernel(Args ar) {
 #pragma unroll
       for (int j = 0; j < FN; ++j) {
         const int col = nb + wn * TNW + j * 16 + 4 * quarter;
-        float v[4];
-        scaled(i, j, csc, col, ncols, rs, v);
 #pragma unroll
-        for (int e = 0; e < 4; ++e)
-          if (col + e < ncols)
-            C[(int64_t)row * ldc + col + e] =
-                from_f32<T>(ar.res ? v[e] + to_f32<T>(ar.res[(int64_t)row * ar.ldres + col + e]) : v[e]);
+        for (int e = 0; e < 4; ++e) {
+          if (col + e >= ncols) continue;
+          const float v = (float)acc[i][j][e] * rs * csc[col + e];
+          C[(int64_t)row * ldc + col + e] = from_f32<T>(ar.res ? v + to_f32<T>(ar.res[(int64_t)row * ar.ldres + col + e]) : v);
+        }
       }
     }
   } else {
