@@ -31,9 +31,9 @@ constexpr Cfg kCfg[kNumCfg] = {{256, 256, 1, 1.27, 1.48}, {128, 256, 1, 0.86, 0.
                                {192, 256, 1, 0.98, 1.25}, {192, 128, 1, 0.61, 0.68}};
 // The same tiles on 8-bit codes, 128 to a k-tile: a k-tile holds the same bytes and matrix instructions, but the scales'
 // epilogue is longer, the waves of some tiles are more and the small tiles keep up better.  Fitted with estimate()'s other two
-// constants to 110 shapes (M 17-8192, N 104-24576, K 256-12288; 1 % slower on average than the best tile and split), then timed
-// on 40 others: 2 % slower on average, 17 % at worst (920 x 12200 x 896: 20.7 against 17.7 us).  The 16-bit constants are 3.4 %
-// slower on average and 32 % at worst on 70 of the first.
+// constants to 110 shapes (M 17-8192, N 104-24576, K 256-12288), then timed on 40 others: 2 % slower on average than the best
+// tile and split, 17 % at worst (920 x 12200 x 896: 20.7 against 17.7 us); on the 110 again, with weights from HBM and the
+// present epilogue, 1.3 % and 15 %.  The 16-bit constants were 3.4 % slower on average and 32 % at worst on 70 of them.
 constexpr Cfg kCfgInt8[kNumCfg] = {{256, 256, 1, 1.58, 1.66}, {128, 256, 1, 0.96, 1.03}, {128, 128, 1, 0.63, 0.66},
                                    {64, 128, 1, 0.40, 0.44},  {64, 64, 2, 0.28, 0.64},   {32, 64, 3, 0.20, 0.80},
                                    {192, 256, 1, 1.12, 1.77}, {192, 128, 1, 0.78, 0.88}};

@@ -1,5 +1,5 @@
 // gemm_tile.h instantiated for codes of 8 bits (two k-contiguous operands): Y = X W^T with a scale per row of each, and its
-// gate/up form.  Bound by the matrix cores at many rows (8192 x 24576 x 4096 with SwiGLU: 659 - 715 us, 2.3 - 2.5 POP/s, where a
+// gate/up form.  Bound by the matrix cores at many rows (8192 x 24576 x 4096 with SwiGLU: 651 - 693 us, 2.4 - 2.5 POP/s, where a
 // plain library product of 16384 cubed reaches 2.4), by the weights' stream and a k-tile's latency at few (32 x 4096 x 12288:
 // 11.3 - 12.0 us and 3 - 4 for the join, 4.4 TB/s).
 #include "gemm_tile.h"
