@@ -54,6 +54,21 @@ Q3_DEV int pack_f16x2(float lo, float hi) {
   return __builtin_bit_cast(int, __builtin_convertvector(v, f16x2_t));
 }
 
+// P with 11 bits is as close as bf16 outputs can tell; to fp16 outputs it adds as much error as their own rounding (1.4 - 1.6
+// times a 32-bit P's in all), so the kernel of few rows, which waits for memory, takes the remainder p - fp16(p) in a second
+// product.  The kernel of many rows has no registers for it (85 spilled); its sums are of the rounded P, which leaves 1.25 - 1.4.
+template <typename T> constexpr bool kTwoTerms = T::code == Q3_F16;
+Q3_DEV int pack_rest_f16x2(float lo, float hi, int packed) {
+  const f16x2_t h = __builtin_bit_cast(f16x2_t, packed);
+  return pack_f16x2(lo - (float)h[0], hi - (float)h[1]);
+}
+
+// Both halves onto a sum in fp32 (subnormal halves count: 40000 weights of e^-11 beside one of 1 are summed right).
+Q3_DEV float sum_f16x2(int x, float sum) {
+  const f16x2_t one = {(_Float16)1.f, (_Float16)1.f};
+  return __builtin_amdgcn_fdot2(__builtin_bit_cast(f16x2_t, x), one, sum, false);
+}
+
 // 8 codes -> 8 exact 16-bit numbers.  fp16: the code + 128 as the low bits of 1024 + x, less 1152.
 template <typename T> Q3_DEV bf16x8_t codes16(int lo, int hi) {
   i32x4 r;
@@ -189,7 +204,7 @@ template <typename T, int RT> Q3_DEV UnitStep unit_step(Rows<T, RT>& w, float vs
 // A block in 8 bits: P' = p * scale / unit as fp16 operands.
 template <typename T, int RT>
 Q3_DEV void softmax_codes(Rows<T, RT>& w, f32x4 (&s)[RT][4], float c, float vscale, bool mask, int key0,
-                          const int (&qpos)[RT], i32x4 (&p)[RT][2]) {
+                          const int (&qpos)[RT], i32x4 (&p)[RT][2], i32x4 (&rest)[RT][2]) {
   const UnitStep u = unit_step(w, vscale);
   softmax_step<T, RT>(w, s, c, u.log2_factor, u.inv_factor, u.units, mask, key0, qpos);
   if (!u.rides) {  // zero, far below the unit, or NaN, for every row: 16 rows' positions lie closer than a block's
@@ -203,10 +218,13 @@ Q3_DEV void softmax_codes(Rows<T, RT>& w, f32x4 (&s)[RT][4], float c, float vsca
 #pragma unroll
   for (int r = 0; r < RT; ++r)
 #pragma unroll
-    for (int t = 0; t < 4; ++t) {
-      p[r][t >> 1][2 * (t & 1)] = pack_f16x2(s[r][t][0], s[r][t][1]);
-      p[r][t >> 1][2 * (t & 1) + 1] = pack_f16x2(s[r][t][2], s[r][t][3]);
-    }
+    for (int t = 0; t < 4; ++t)
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int x = pack_f16x2(s[r][t][2 * e], s[r][t][2 * e + 1]);
+        p[r][t >> 1][2 * (t & 1) + e] = x;
+        if constexpr (kTwoTerms<T>) rest[r][t >> 1][2 * (t & 1) + e] = pack_rest_f16x2(s[r][t][2 * e], s[r][t][2 * e + 1], x);
+      }
 }
 
 // What a wave of either kernel knows of its launch (positions and blocks fit 32 bits: capacity does).
@@ -307,16 +325,20 @@ Q3_DEV void tail_block(const AttnArgs& a, const Span& p, int g, int j, Rows<T, R
   // O back to plain units: the tail's values are what they are
   softmax_step<T, RT>(w, s, a.scale2, 0.f, 1.f, w.unit, true, p.whole * BLK - p.start + 16 * g, qpos);
   w.unit = w.inv = 1.f;
-  bf16x8_t pf[RT][2];
+  bf16x8_t pf[RT][2], prest[RT][2];
 #pragma unroll
   for (int r = 0; r < RT; ++r)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      i32x4 x;
+      i32x4 x, y = {0, 0, 0, 0};
 #pragma unroll
-      for (int e = 0; e < 4; ++e)
-        x[e] = (int)pack2<T>(s[r][2 * h + (e >> 1)][2 * (e & 1)], s[r][2 * h + (e >> 1)][2 * (e & 1) + 1]);
+      for (int e = 0; e < 4; ++e) {
+        const float lo = s[r][2 * h + (e >> 1)][2 * (e & 1)], hi = s[r][2 * h + (e >> 1)][2 * (e & 1) + 1];
+        x[e] = (int)pack2<T>(lo, hi);
+        if constexpr (kTwoTerms<T>) y[e] = pack_rest_f16x2(lo, hi, x[e]);
+      }
       pf[r][h] = __builtin_bit_cast(bf16x8_t, x);
+      prest[r][h] = __builtin_bit_cast(bf16x8_t, y);
     }
 #pragma unroll
   for (int t0 = 0; t0 < 8; t0 += VT) {
@@ -363,8 +385,10 @@ Q3_DEV void tail_block(const AttnArgs& a, const Span& p, int g, int j, Rows<T, R
 #pragma unroll
         for (int e = 0; e < 4; ++e) x[e] &= (int)keep[h][e];
 #pragma unroll
-        for (int r = 0; r < RT; ++r)
+        for (int r = 0; r < RT; ++r) {
           w.o[r][t0 + t] = mfma_16x16x32<T>(__builtin_bit_cast(bf16x8_t, x), pf[r][h], w.o[r][t0 + t]);
+          if constexpr (kTwoTerms<T>) w.o[r][t0 + t] = mfma_16x16x32<T>(__builtin_bit_cast(bf16x8_t, x), prest[r][h], w.o[r][t0 + t]);
+        }
       }
     if constexpr (VT < 8) __builtin_amdgcn_sched_barrier(0);
   }
@@ -460,12 +484,16 @@ template <typename T> __global__ __launch_bounds__(256) void kv8_attn_rows_kerne
     }
     const float vs = sv;
     if (blk + WK < wend) load_k(blk + WK);
-    i32x4 p[RT][2];
-    softmax_codes<T, RT>(w, s, c, vs, (blk + 1) * BLK > sp.start + 1, blk * BLK - sp.start + 16 * g, qpos, p);
+    i32x4 p[RT][2], rest[RT][2];
+    softmax_codes<T, RT>(w, s, c, vs, (blk + 1) * BLK > sp.start + 1, blk * BLK - sp.start + 16 * g, qpos, p, rest);
 #pragma unroll
     for (int t = 0; t < 8; ++t) {
-      w.o[0][t] = mfma_16x16x32<F16>(codes16<F16>(raw.v[t][0], raw.v[t][1]), __builtin_bit_cast(bf16x8_t, p[0][0]), w.o[0][t]);
-      w.o[0][t] = mfma_16x16x32<F16>(codes16<F16>(raw.v[t][2], raw.v[t][3]), __builtin_bit_cast(bf16x8_t, p[0][1]), w.o[0][t]);
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const bf16x8_t v = codes16<F16>(raw.v[t][2 * e], raw.v[t][2 * e + 1]);
+        w.o[0][t] = mfma_16x16x32<F16>(v, __builtin_bit_cast(bf16x8_t, p[0][e]), w.o[0][t]);
+        if constexpr (kTwoTerms<T>) w.o[0][t] = mfma_16x16x32<F16>(v, __builtin_bit_cast(bf16x8_t, rest[0][e]), w.o[0][t]);
+      }
     }
     if (blk + WK < wend) load_v(blk + WK);
   }
@@ -664,12 +692,10 @@ template <typename T> __global__ __launch_bounds__(512, 2) void kv8_attn_tile_ke
         qk_step(fk, sn, i);
         const int r = i >> 2, t = i & 3;
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-          s[r][t][e] = __builtin_amdgcn_exp2f(fmaf(s[r][t][e], c, off[r]));
-          sum[r] += s[r][t][e];
-        }
+        for (int e = 0; e < 4; ++e) s[r][t][e] = __builtin_amdgcn_exp2f(fmaf(s[r][t][e], c, off[r]));
         int lo = pack_f16x2(s[r][t][0], s[r][t][1]), hi = pack_f16x2(s[r][t][2], s[r][t][3]);
         asm volatile("" : "+v"(lo), "+v"(hi));  // formed here, beside the products, not where the next block uses them
+        sum[r] = sum_f16x2(hi, sum_f16x2(lo, sum[r]));
         p[r][t >> 1][2 * (t & 1)] = lo;
         p[r][t >> 1][2 * (t & 1) + 1] = hi;
       }

@@ -536,6 +536,27 @@ def test_attention_masked_nonfinite_tail_values(s, dtype):
         c.v_tail[1, 1, dim, pos - 64] = keep
 
 
+@pytest.mark.parametrize("dtype", DT)
+@pytest.mark.parametrize("s", [1, 20])
+def test_attention_many_tiny_weights(s, dtype):
+    """One strong key beside 40000 weak ones, whose weights of about e^-11 are subnormal in fp16 where the strong one's is 1."""
+    total = 40000
+    gen = seeded(11)
+    k, v = torch.zeros(1, total, 1, 128), 1 + 0.01 * torch.randn(1, total, 1, 128, generator=gen)
+    k[..., 0] = -11 * 128 ** 0.5 / 8
+    k[0, 70], v[0, 70] = 0, -1
+    q = torch.zeros(1, s, 4, 128)
+    q[..., 0] = 8
+    c = I8.LayerCache.empty(1, 1, total, device="cuda", dtype=dtype)
+    I8.append(k.to(dtype).cuda(), v.to(dtype).cuda(), c, 0)
+    y = I8.attention(q.to(dtype).cuda(), c, total - s)[0, -1].double().cpu()
+    kk, vv = (x[0, 0].double().cpu() for x in I8.read(c, total, dtype=torch.float32))
+    w = torch.softmax(8.0 * kk[:, 0] * 128 ** -0.5, 0) @ vv
+    # P and its sum each rounded by at most 2^-11 (fp16; here the weak ones all alike), subnormal ones by 2^-25 of a weight of
+    # 2^-16: 2^-9; |v| is 1; the output's own rounding
+    assert ((y - w).abs() <= 2 * (2.0 ** -11 + 2.0 ** -9) + w.abs() * torch.finfo(dtype).eps / 2).all()
+
+
 @pytest.mark.parametrize("s", [1, 70])
 def test_attention_nonfinite_values_of_no_weight(s):
     """A block of values that were not finite makes a query that sees it NaN, however small the block's weight."""
