@@ -62,6 +62,10 @@ Q3_DEV int pack_rest_f16x2(float lo, float hi, int packed) {
   const f16x2_t h = __builtin_bit_cast(f16x2_t, packed);
   return pack_f16x2(lo - (float)h[0], hi - (float)h[1]);
 }
+// The same in the activation type, for the tail's P.
+template <typename T> Q3_DEV int pack_rest2(float lo, float hi, int packed) {
+  return (int)pack2<T>(lo - to_f32<T>((u16)((uint32_t)packed & 0xffffu)), hi - to_f32<T>((u16)((uint32_t)packed >> 16)));
+}
 
 // Both halves onto a sum in fp32 (subnormal halves count: 40000 weights of e^-11 beside one of 1 are summed right).
 Q3_DEV float sum_f16x2(int x, float sum) {
@@ -277,7 +281,9 @@ Q3_DEV void load_rows(const AttnArgs& a, const Span& p, int b, int hk, int g, in
   w.unit = w.inv = 0.f;
 }
 
-// The tail block, in 16 bits: P in T, as V is; slots past the last position hold anything and read as zeros.  One row tile
+// The tail block, in 16 bits: P in T, as V is, in two terms: its rounding and the remainder's (over the first 63 positions of
+// a request the tail is all there is, and one bf16 term there left outputs 1.2 - 1.3 times as far from 64 bits as a 32-bit P's;
+// it is one block in a row's pass).  Slots past the last position hold anything and read as zeros.  One row tile
 // takes all of V before its scores are formed (a wait less); two have no registers for that and take two dim tiles at a time.
 // An infinity or NaN among the values makes the rows that see its position NaN, as the whole block will be; the others, whose
 // P is 0 there, are kept clear of it (0 times it is NaN) by reading zeros from that slot on.
@@ -330,12 +336,12 @@ Q3_DEV void tail_block(const AttnArgs& a, const Span& p, int g, int j, Rows<T, R
   for (int r = 0; r < RT; ++r)
 #pragma unroll
     for (int h = 0; h < 2; ++h) {
-      i32x4 x, y = {0, 0, 0, 0};
+      i32x4 x, y;
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
         const float lo = s[r][2 * h + (e >> 1)][2 * (e & 1)], hi = s[r][2 * h + (e >> 1)][2 * (e & 1) + 1];
         x[e] = (int)pack2<T>(lo, hi);
-        if constexpr (kTwoTerms<T>) y[e] = pack_rest_f16x2(lo, hi, x[e]);
+        y[e] = pack_rest2<T>(lo, hi, x[e]);
       }
       pf[r][h] = __builtin_bit_cast(bf16x8_t, x);
       prest[r][h] = __builtin_bit_cast(bf16x8_t, y);
@@ -387,7 +393,7 @@ Q3_DEV void tail_block(const AttnArgs& a, const Span& p, int g, int j, Rows<T, R
 #pragma unroll
         for (int r = 0; r < RT; ++r) {
           w.o[r][t0 + t] = mfma_16x16x32<T>(__builtin_bit_cast(bf16x8_t, x), pf[r][h], w.o[r][t0 + t]);
-          if constexpr (kTwoTerms<T>) w.o[r][t0 + t] = mfma_16x16x32<T>(__builtin_bit_cast(bf16x8_t, x), prest[r][h], w.o[r][t0 + t]);
+          w.o[r][t0 + t] = mfma_16x16x32<T>(__builtin_bit_cast(bf16x8_t, x), prest[r][h], w.o[r][t0 + t]);
         }
       }
     if constexpr (VT < 8) __builtin_amdgcn_sched_barrier(0);

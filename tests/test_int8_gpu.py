@@ -724,3 +724,16 @@ def test_chain(s, dtype):
     g, u = (product64(d.cpu().view(s, -1), sd.cpu().view(s), *(t.cpu() for t in w)) for w in ws[4:])
     ref = g * torch.sigmoid(g) * u
     close(z.view(s, -1), ref, ref.abs() * (torch.finfo(dtype).eps / 2 * (1 + 2.0 ** -10) + (12 + 6 * g.abs()) * 2.0 ** -23) + 1e-7)
+
+
+@pytest.mark.parametrize("t,s", [(2, 1), (5, 5), (40, 1), (63, 1), (17, 17), (63, 40), (63, 63)])
+def test_attention_short_contexts(t, s):
+    """Below 64 positions every one of them is in the tail: outputs as near to 64 bits as their own rounding to bf16 lets them."""
+    gen = seeded(t + s)
+    c, k, v = filled(2, 2, t, torch.bfloat16, gen, wide=False)
+    q = randn(2, s, 8, 128, gen=gen, dtype=torch.bfloat16, scale=0.3)
+    o = I8.attention(q.cuda(), c, t - s)
+    ref, _, at, zerr, _ = attention64(q, *held64(k, v)[0], t - s, 128 ** -0.5, 0)
+    # scores and sums as in check_attention; P in two bf16 terms: what the first leaves (2^-8 of it) is rounded by 2^-8
+    dz = zerr * 136 * 2.0 ** -24 * 2
+    close(o, ref, ref.abs() * 2.0 ** -8 * (1 + 2.0 ** -8) + at * (dz + 2.0 ** -16 + 2.0 ** -16) + 2.0 ** -24)
