@@ -105,6 +105,7 @@ template <typename T, int RT> struct Rows {
   f32x4 o[RT][8];        // O^T: dims 16 t + 4 g + e
   float m[RT], l[RT];
   float unit, inv;       // of O: a power of two (0: nothing yet), and 1 / unit
+  float least;           // 2^-76 of the largest unit so far
 };
 
 Q3_DEV float xmax4(float x) {  // max over lanes {l, l ^ 16, l ^ 32, l ^ 48}
@@ -182,19 +183,22 @@ struct UnitStep {
   bool rides, nan;  // the factor rides in the exponent; if not, it is 0, far below the unit, or NaN
 };
 template <typename T, int RT> Q3_DEV UnitStep unit_step(Rows<T, RT>& w, float vscale) {
-  // a value scale within 16 times of the unit leaves it; one 2^60 below adds nothing worth a new unit
+  // A value scale within 16 times of the unit leaves it; one 2^76 below the largest unit so far adds nothing worth a new one.
+  // (Below the largest, not the last: O grows by old unit / new unit with each fall, and passes 2^128 after a few.  |O| is at
+  // most 128 * 16 * 2^8 a position in its unit, 2^50 at 2^31 positions, so a fall by 2^76 in all leaves it finite.)
   const uint32_t vb = __float_as_uint(uniform(vscale));  // >= 0, or NaN
   UnitStep u;
   u.units = 1.f;
   u.ratio = uniform(vscale * w.inv);
-  const uint32_t kMost = 0x41800000u, kLeast = 0x3d800000u, kNone = 0x21800000u;  // 16, 1 / 16, 2^-60
+  const uint32_t kMost = 0x41800000u, kLeast = 0x3d800000u;  // 16, 1 / 16
   uint32_t rb = __float_as_uint(u.ratio);
-  if (vb < 0x7f800000u && vb > 0 && (w.inv == 0.f || rb > kMost || (rb < kLeast && rb > kNone))) {
+  if (vb < 0x7f800000u && vb > 0 && (w.inv == 0.f || rb > kMost || (rb < kLeast && vb > __float_as_uint(w.least)))) {
     const uint32_t e = min(max(vb & 0x7f800000u, 0x00800000u), 0x7e000000u);  // the power of two below, 2^-126 .. 2^125
     const float inv = __uint_as_float(0x7f000000u - e);
     u.units = uniform(w.unit * inv);
     w.unit = __uint_as_float(e);
     w.inv = inv;
+    w.least = fmaxf(w.least, uniform(w.unit * 0x1p-76f));
     u.ratio = uniform(vscale * inv);
     rb = __float_as_uint(u.ratio);
   }
@@ -278,7 +282,7 @@ Q3_DEV void load_rows(const AttnArgs& a, const Span& p, int b, int hk, int g, in
 #pragma unroll
     for (int t = 0; t < 8; ++t) w.o[r][t] = f32x4{0.f, 0.f, 0.f, 0.f};
   }
-  w.unit = w.inv = 0.f;
+  w.unit = w.inv = w.least = 0.f;
 }
 
 // The tail block, in 16 bits: P in T, as V is, in two terms: its rounding and the remainder's (over the first 63 positions of

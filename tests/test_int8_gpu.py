@@ -737,3 +737,38 @@ def test_attention_short_contexts(t, s):
     # scores and sums as in check_attention; P in two bf16 terms: what the first leaves (2^-8 of it) is rounded by 2^-8
     dz = zerr * 136 * 2.0 ** -24 * 2
     close(o, ref, ref.abs() * 2.0 ** -8 * (1 + 2.0 ** -8) + at * (dz + 2.0 ** -16 + 2.0 ** -16) + 2.0 ** -24)
+
+
+@pytest.mark.parametrize("exps", [(0, -55, -110), (0, -40, -80, -120), (0, -30, -60, -90, -120), (0, -55, -110, 4, -70, -100), (-60, 0, -110)])
+@pytest.mark.parametrize("s", [1, 40])
+def test_attention_value_scales_that_keep_falling(s, exps):
+    """Blocks whose values fall by more in all than a 32-bit sum in one unit could follow: the large ones' values stay finite."""
+    gen = seeded(len(exps))
+    for tail in (0, 10):
+        t = 64 * len(exps) + tail
+        k, v = randn(1, t, 2, 128, gen=gen, dtype=torch.bfloat16), randn(1, t, 2, 128, gen=gen)
+        for i, e in enumerate(exps):
+            v[:, 64 * i:64 * (i + 1)] *= 2.0 ** e
+        v[:, 64 * len(exps):] *= 2.0 ** exps[-1]
+        v = v.bfloat16()
+        c = poisoned(1, 2, t, torch.bfloat16)
+        I8.append(k.cuda(), v.cuda(), c, 0)
+        q = randn(1, s, 4, 128, gen=gen, dtype=torch.bfloat16)
+        check_attention(I8.attention(q.cuda(), c, t - s), q, held64(k, v)[0], t - s, 128 ** -0.5, torch.bfloat16)
+
+
+def test_attention_value_scales_that_keep_falling_over_a_full_launch():
+    """The same where the rows fill the CUs, so that each wave goes over several of the blocks."""
+    gen = seeded(3)
+    exps, b = (20, -36, -92, -118), 512
+    t = 64 * 4 * len(exps)
+    k, v = randn(1, t, 1, 128, gen=gen, dtype=torch.bfloat16), randn(1, t, 1, 128, gen=gen)
+    for i, e in enumerate(exps):   # four waves take every fourth block each
+        v[:, 256 * i:256 * (i + 1)] *= 2.0 ** e
+    v = v.bfloat16()
+    c = poisoned(b, 1, t, torch.bfloat16)
+    I8.append(k.cuda().expand(b, t, 1, 128), v.cuda().expand(b, t, 1, 128), c, 0)
+    q = randn(1, 1, 2, 128, gen=gen, dtype=torch.bfloat16)
+    o = I8.attention(q.cuda().expand(b, 1, 2, 128), c, t - 1)
+    check_attention(o[:1], q, held64(k, v)[0], t - 1, 128 ** -0.5, torch.bfloat16)
+    assert torch.equal(o, o[:1].expand_as(o))
