@@ -170,11 +170,12 @@ Q3_DEV void softmax_step(Rows<T, RT>& w, f32x4 (&s)[RT][4], float c, float log2_
 // A value that is the same in every lane, in a scalar register.
 Q3_DEV float uniform(float x) { return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x))); }
 
-// A block's factor of the raw scores.  Keys that are all zero have scale 0: their raw scores are 0 whatever the factor, and a
-// factor of 0 would turn hidden positions' minus infinity into NaN.
+// A block's factor of the raw scores.  A factor of 0 would turn hidden positions' minus infinity into NaN.  Keys that are all zero
+// have scale 0, and their raw scores are 0 whatever the factor; a product that fell below 2^-149 makes scores of 0 too (raw scores
+// stay below 2^30 for queries below 2^16).
 Q3_DEV float score_factor(float kscale, float scale2) {
   const float c = uniform(kscale * scale2);
-  return __float_as_uint(c) == 0 ? 1.f : c;
+  return __float_as_uint(c) == 0 ? 0x1p-126f : c;
 }
 
 // How a block's value scale meets O's unit: O is to be multiplied by `units`, and P' = p * scale / unit.

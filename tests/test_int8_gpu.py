@@ -772,3 +772,15 @@ def test_attention_value_scales_that_keep_falling_over_a_full_launch():
     o = I8.attention(q.cuda().expand(b, 1, 2, 128), c, t - 1)
     check_attention(o[:1], q, held64(k, v)[0], t - 1, 128 ** -0.5, torch.bfloat16)
     assert torch.equal(o, o[:1].expand_as(o))
+
+
+@pytest.mark.parametrize("s", [1, 40])
+def test_attention_key_scales_that_vanish(s):
+    """Keys so small that their scale times the softmax scale is below the least 32-bit number: every score is 0."""
+    gen = seeded(2)
+    t = 64 * 3
+    k, v = randn(1, t, 2, 128, gen=gen, scale=2.0 ** -100).bfloat16(), randn(1, t, 2, 128, gen=gen, dtype=torch.bfloat16)
+    c = poisoned(1, 2, t, torch.bfloat16)
+    I8.append(k.cuda(), v.cuda(), c, 0)
+    q = randn(1, s, 4, 128, gen=gen, dtype=torch.bfloat16, scale=4.0)
+    check_attention(I8.attention(q.cuda(), c, t - s, scale=1e-20), q, held64(k, v)[0], t - s, 1e-20, torch.bfloat16)
