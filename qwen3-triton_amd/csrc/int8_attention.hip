@@ -199,7 +199,7 @@ template <typename T, int RT> Q3_DEV UnitStep unit_step(Rows<T, RT>& w, float vs
     u.units = uniform(w.unit * inv);
     w.unit = __uint_as_float(e);
     w.inv = inv;
-    w.least = fmaxf(w.least, uniform(w.unit * 0x1p-76f));
+    w.least = uniform(fmaxf(w.least, w.unit * 0x1p-76f));
     u.ratio = uniform(vscale * inv);
     rb = __float_as_uint(u.ratio);
   }
