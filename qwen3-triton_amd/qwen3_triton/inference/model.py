@@ -166,7 +166,7 @@ class TritonQwen3Inference(nn.Module):
         self.gemv, self.split_decode = gemv, split_decode
         self._cache_owner = object()
         self._int8 = None   # per layer, once quantize_weights has run
-        self._weights = object()   # replaced when the weights that captured steps read are freed
+        self._weights = object()   # replaced when the tensors that captured steps read are
         self.generation_config = _generation_config(config)
         self.eval()
 
@@ -179,12 +179,18 @@ class TritonQwen3Inference(nn.Module):
         if wrong:
             raise ValueError(f'bf16 inference weights required; {wrong[0]} is not bf16')
         self.load_state_dict(state, assign=True, strict=True)
-        if self._int8 is not None:
-            self._int8, self._weights = None, object()
+        self._int8 = None
         if tied:
             self.lm_head.weight = self.model.embed_tokens.weight
         self.model.rotary_emb.inv_freq = self._inv_freq().to(self.lm_head.weight.device)
         return self
+
+    def load_state_dict(self, state_dict, strict=True, assign=False):
+        """``nn.Module.load_state_dict``.  With ``assign`` the tensors are replaced: steps captured before read the old ones,
+        and refuse to replay (also after a load that failed half-way)."""
+        if assign:
+            self._weights = object()
+        return super().load_state_dict(state_dict, strict=strict, assign=assign)
 
     def _inv_freq(self):
         c = self.config
@@ -510,7 +516,7 @@ def _generation_config(config):
 
 
 def _check_captured(session):
-    """Raise if the weights that a captured step reads have been freed since."""
+    """Raise if the weights that a captured step reads have been replaced or freed since."""
     if session._weights is not session.model._weights:
         raise RuntimeError('captured before the model\'s weights were replaced: capture again')
 

@@ -221,3 +221,30 @@ def test_decode_linear_ok_of_nothing():
     for shape in ((), (0,), (3, 0), (0, 32)):
         assert not I8.decode_linear_ok(torch.zeros(shape, dtype=torch.bfloat16))
     assert I8.decode_linear_ok(torch.zeros(2, 16384)) and not I8.decode_linear_ok(torch.zeros(3, 16384))
+
+
+def tiny_model():
+    """A small inference model on the CPU (no kernel runs)."""
+    import oracle as O
+    from transformers import Qwen3Config
+    from qwen3_triton.inference import TritonQwen3Inference
+    sizes = dict(vocab_size=64, hidden_size=128, intermediate_size=256, num_hidden_layers=2, num_attention_heads=2,
+                 num_key_value_heads=1, head_dim=128)
+    state = {k: v.bfloat16() for k, v in O.init_params(O.OracleConfig(**sizes), seed=2, std=0.05).items()}
+    config = Qwen3Config(**sizes, tie_word_embeddings=False, max_position_embeddings=256)
+    return TritonQwen3Inference(config).load_hf_state_dict(state), state
+
+
+def test_replaced_weights_end_captured_steps():
+    from types import SimpleNamespace
+    from qwen3_triton.inference.model import _check_captured
+    model, state = tiny_model()
+    step = SimpleNamespace(model=model, _weights=model._weights)
+    model.load_state_dict(state)   # copied in place
+    _check_captured(step)
+    for load in (lambda: model.load_hf_state_dict(state), lambda: model.load_state_dict(state, assign=True),
+                 lambda: model.load_state_dict({k: v for k, v in state.items() if 'norm' in k}, strict=False, assign=True)):
+        step._weights = model._weights
+        load()
+        with pytest.raises(RuntimeError, match='capture again'):
+            _check_captured(step)

@@ -292,3 +292,34 @@ def test_more_heads_than_a_fused_product_takes(heads, kv, cache_dtype):
     ids = torch.arange(9, device='cuda').view(1, 9)
     out = model.generate(ids, max_new_tokens=4, eos_token_id=(), cache_dtype=cache_dtype)
     assert torch.equal(out, CapturedGreedyRequest(model, ids, max_new_tokens=4, cache_dtype=cache_dtype)(ids))
+
+
+@pytest.mark.parametrize("load", ["load_hf_state_dict", "load_state_dict", "half a load"])
+def test_a_reload_ends_captured_steps(load):
+    """Without int8 too: the old tensors are gone, and a step captured on them refuses to replay."""
+    model, params = build(False)
+    ids = torch.arange(12, device='cuda').view(1, 12)
+    session = DecodeSession(model, 1, 32)
+    session.prefill(ids)
+    session.capture()
+    session.step()
+    request = CapturedGreedyRequest(model, ids, max_new_tokens=3)
+    want = request(ids).clone()
+    state = {k: v.cuda() for k, v in params.items()}
+    if load == "load_hf_state_dict":
+        model.load_hf_state_dict(state)
+    elif load == "load_state_dict":
+        model.load_state_dict(state, assign=True)
+    else:
+        del state["lm_head.weight"]
+        with pytest.raises((KeyError, RuntimeError)):
+            model.load_hf_state_dict(state)
+    with pytest.raises(RuntimeError, match='capture again'):
+        session.step()
+    with pytest.raises(RuntimeError, match='capture again'):
+        request(ids)
+    assert torch.equal(CapturedGreedyRequest(model, ids, max_new_tokens=3)(ids), want)
+    # weights copied into the tensors that are there: what a captured step reads is the new ones
+    request = CapturedGreedyRequest(model, ids, max_new_tokens=3)
+    model.load_state_dict({k: v.cuda() for k, v in params.items()})
+    assert torch.equal(request(ids), want)
