@@ -138,6 +138,33 @@ def _quantized_cache(cache):
     return Int8KVCache([], [], cache.capacity, cache.batch_size, cache.owner, cache.length, cache.valid, layers)
 
 
+class _Int8Weights(list):
+    """A model's layers in int8 (``_Int8Layer`` each), with the empty parameters that stand for the projections' bf16 weights
+    meanwhile.  The codes are the weights only as long as those are in place."""
+
+    def __init__(self, model):
+        super().__init__()
+        self.names, self._empty = set(), []
+        for i, layer in enumerate(model.layers):
+            self.append(_Int8Layer(layer))
+            for part in ('self_attn', 'mlp'):
+                for name, proj in getattr(layer, part).named_children():
+                    if name.endswith('_proj'):
+                        proj.weight = nn.Parameter(torch.empty_like(proj.weight, device='meta'), requires_grad=False)
+                        self.names.add(f'model.layers.{i}.{part}.{name}.weight')
+                        self._empty.append((proj._parameters, proj.weight))
+
+    def in_place(self):
+        for held, empty in self._empty:   # a plain loop: this runs before every step
+            if held['weight'] is not empty:
+                return False
+        return True
+
+    def check(self):
+        if not self.in_place():
+            raise RuntimeError('a projection was given weights beside its int8 ones: load_hf_state_dict goes back to bf16')
+
+
 class _Int8Layer:
     """One decoder layer's projections as (codes, channel scales)."""
 
@@ -178,8 +205,13 @@ class TritonQwen3Inference(nn.Module):
         wrong = sorted(k for k, v in state.items() if v.dtype != torch.bfloat16 and not k.endswith('inv_freq'))
         if wrong:
             raise ValueError(f'bf16 inference weights required; {wrong[0]} is not bf16')
-        self.load_state_dict(state, assign=True, strict=True)
-        self._int8 = None
+        held, self._int8 = self._int8, None
+        try:
+            self.load_state_dict(state, assign=True, strict=True)
+        except BaseException:
+            if held is not None and held.in_place():   # nothing reached the projections: they are in int8 still
+                self._int8 = held
+            raise
         if tied:
             self.lm_head.weight = self.model.embed_tokens.weight
         self.model.rotary_emb.inv_freq = self._inv_freq().to(self.lm_head.weight.device)
@@ -187,7 +219,10 @@ class TritonQwen3Inference(nn.Module):
 
     def load_state_dict(self, state_dict, strict=True, assign=False):
         """``nn.Module.load_state_dict``.  With ``assign`` the tensors are replaced: steps captured before read the old ones,
-        and refuse to replay (also after a load that failed half-way)."""
+        and refuse to replay (also after a load that failed half-way).  After ``quantize_weights`` the projections cannot be
+        loaded this way (``load_hf_state_dict`` goes back to bf16)."""
+        if self._int8 is not None and any(name in state_dict for name in self._int8.names):
+            raise ValueError('the projections are in int8: load_hf_state_dict goes back to bf16')
         if assign:
             self._weights = object()
         return super().load_state_dict(state_dict, strict=strict, assign=assign)
@@ -243,13 +278,7 @@ class TritonQwen3Inference(nn.Module):
         for n in (c.hidden_size, c.intermediate_size, c.num_attention_heads * c.head_dim):
             if n % 16 or n > int8.MAX_ROW:
                 raise ValueError(f'sizes that are multiples of 16 and at most {int8.MAX_ROW} required for int8, not {n}')
-        held = []
-        for layer in self.model.layers:
-            held.append(_Int8Layer(layer))
-            for part in (layer.self_attn, layer.mlp):
-                for proj in (p for name, p in part.named_children() if name.endswith('_proj')):
-                    proj.weight = nn.Parameter(torch.empty_like(proj.weight, device='meta'), requires_grad=False)
-        self._int8, self._weights = held, object()
+        self._int8, self._weights = _Int8Weights(self.model), object()
         return self
 
     def state_dict(self, *args, **kwargs):
@@ -362,6 +391,8 @@ class TritonQwen3Inference(nn.Module):
         cache.admit(self._cache_owner, b, s)
         if type(logits_to_keep) is not int or not 0 <= logits_to_keep <= s:
             raise ValueError('logits_to_keep must be 0 or within current sequence length')
+        if self._int8 is not None:
+            self._int8.check()
         start = cache.length
         if start_dev is not None and s != 1:
             raise ValueError('device-resident positions are for single-token decode steps')
@@ -519,6 +550,8 @@ def _check_captured(session):
     """Raise if the weights that a captured step reads have been replaced or freed since."""
     if session._weights is not session.model._weights:
         raise RuntimeError('captured before the model\'s weights were replaced: capture again')
+    if session.model._int8 is not None:
+        session.model._int8.check()
 
 
 class DecodeSession:

@@ -248,3 +248,62 @@ def test_replaced_weights_end_captured_steps():
         load()
         with pytest.raises(RuntimeError, match='capture again'):
             _check_captured(step)
+
+
+def tiny_int8_model(monkeypatch):
+    from qwen3_triton.inference import TritonQwen3Inference
+    model, state = tiny_model()
+    with monkeypatch.context() as m:   # the codes' values do not matter here
+        m.setattr(TritonQwen3Inference, 'device', property(lambda self: torch.device('cuda')))
+        m.setattr(I8, 'quantize_rows', lambda w: (w.to(torch.int8), w.float().abs().amax(1) / 127))
+        model.quantize_weights()
+    return model, state
+
+
+def test_weights_loaded_beside_int8_are_refused(monkeypatch):
+    """The codes stand for the projections until load_hf_state_dict takes them away: no other load is left without effect."""
+    from types import SimpleNamespace
+    from qwen3_triton.inference import KVCache
+    from qwen3_triton.inference.model import _check_captured
+    model, state = tiny_int8_model(monkeypatch)
+    step = SimpleNamespace(model=model, _weights=model._weights)
+    before = dict(model.named_parameters())
+    for kw in (dict(assign=True), dict(), dict(strict=False, assign=True)):
+        with pytest.raises(ValueError, match='load_hf_state_dict'):
+            model.load_state_dict(state, **kw)
+    assert all(p is before[n] for n, p in model.named_parameters()) and len(model._int8) == 2
+    _check_captured(step)
+    # what is not in int8 can be loaded
+    rest = {k: v + 1 for k, v in state.items() if '_proj' not in k}
+    model.load_state_dict(rest, strict=False)
+    assert torch.equal(model.lm_head.weight, rest['lm_head.weight'])
+    # a part of the model, or one weight, behind its back
+    ids, up = torch.zeros(1, 3, dtype=torch.int64), 'layers.1.mlp.up_proj.weight'
+
+    def set_one(m):
+        m.model.layers[0].self_attn.k_proj.weight = torch.nn.Parameter(state['model.layers.0.self_attn.k_proj.weight'])
+    for change in (lambda m: m.model.load_state_dict({up: state['model.' + up]}, strict=False, assign=True), set_one):
+        model, _ = tiny_int8_model(monkeypatch)
+        step = SimpleNamespace(model=model, _weights=model._weights)
+        _check_captured(step)
+        change(model)
+        with pytest.raises(RuntimeError, match='beside its int8'):
+            model(ids, past_key_values=KVCache([], [], 16, 1, model._cache_owner))
+        with pytest.raises(RuntimeError, match='beside its int8'):
+            _check_captured(step)
+        model.load_hf_state_dict(state)
+        assert model._int8 is None and all(torch.equal(p, state[n]) for n, p in model.named_parameters())
+
+
+def test_a_failed_load_over_int8(monkeypatch):
+    """Names that fit nothing leave the model in int8; a load that reached the projections does not leave the old codes."""
+    model, state = tiny_int8_model(monkeypatch)
+    with pytest.raises(RuntimeError):
+        model.load_hf_state_dict({'x.' + k: v for k, v in state.items()})
+    assert len(model._int8) == 2
+    model._int8.check()
+    with pytest.raises(RuntimeError):
+        model.load_hf_state_dict({k: v for k, v in state.items() if 'layers.1' not in k})
+    assert model._int8 is None
+    model.load_hf_state_dict(state)
+    assert all(torch.equal(p, state[n]) for n, p in model.named_parameters())

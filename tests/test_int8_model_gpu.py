@@ -323,3 +323,21 @@ def test_a_reload_ends_captured_steps(load):
     request = CapturedGreedyRequest(model, ids, max_new_tokens=3)
     model.load_state_dict({k: v.cuda() for k, v in params.items()})
     assert torch.equal(request(ids), want)
+
+
+def test_weights_beside_int8_are_refused():
+    model, params = build(True)
+    state = {k: v.cuda() for k, v in params.items()}
+    ids = torch.arange(12, device='cuda').view(1, 12)
+    want = model(ids).logits
+    request = CapturedGreedyRequest(model, ids, max_new_tokens=3)
+    with pytest.raises(ValueError, match='load_hf_state_dict'):
+        model.load_state_dict(state, assign=True)
+    assert torch.equal(model(ids).logits, want)
+    model.model.layers[1].mlp.up_proj.load_state_dict({'weight': state['model.layers.1.mlp.up_proj.weight']}, assign=True)
+    for call in (lambda: model(ids), lambda: request(ids), lambda: model.generate(ids, max_new_tokens=2)):
+        with pytest.raises(RuntimeError, match='beside its int8'):
+            call()
+    model.load_hf_state_dict(state)
+    assert torch.equal(model(ids).logits, build(False)[0](ids).logits)
+    assert torch.equal(model.quantize_weights()(ids).logits, want)
