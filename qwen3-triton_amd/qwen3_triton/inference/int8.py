@@ -68,7 +68,8 @@ def _rows(x, what):
 
 
 # ---------------------------------------------------------------- rows
-def _check_rows(x):
+def check_rows(x):
+    """Rows that ``quantize_rows`` takes, as (rows, row stride, row length); what it refuses is raised."""
     _on_device(x)
     _require_float(x, 'rows')
     rows, ld, k = _rows(x, 'rows')
@@ -91,7 +92,7 @@ def _codes_like(x):
 def quantize_rows(x):
     """x [..., K] -> (codes int8 [..., K], scales fp32 [...]): each row on its own."""
     _forward_only(x)
-    rows, ld, k = _check_rows(x)
+    rows, ld, k = check_rows(x)
     q, scale = _codes_like(x)
     _launch(x, "q3_quant_rows", H.code(x.dtype), x.data_ptr(), ld, q.data_ptr(), scale.data_ptr(), rows, k)
     return q, scale
@@ -101,7 +102,7 @@ def rms_norm(x, weight, eps, *, residual=None):
     """RMSNorm of x [..., K] in 8 bits: (codes, scales), and with ``residual`` (codes, scales, total) where
     total = x + residual, rounded once, is what the norm is taken of."""
     _forward_only(x, weight, residual)
-    rows, ld, k = _check_rows(x)
+    rows, ld, k = check_rows(x)
     _on_device(x, weight)
     _check_norm(x, weight, eps, k)
     if residual is None:
@@ -231,7 +232,7 @@ def decode_linear(x, weights, *, norm_weight=None, eps=1e-6, gate_up=False, resi
     ``projections`` of up to three weights [(codes, scales), ...] in one launch -> a list; with ``gate_up`` the SwiGLU of
     two -> one tensor; with ``residual`` [..., N] one weight's product plus it -> one tensor."""
     _forward_only(x, norm_weight, residual, *(ws for _, ws in weights))
-    rows, ld, k = _check_rows(x)
+    rows, ld, k = check_rows(x)
     if not decode_linear_ok(x):
         raise ValueError('decode_linear takes at most 2 rows of at most 16384 values')
     if norm_weight is not None:

@@ -145,14 +145,18 @@ class _Int8Weights(list):
     def __init__(self, model):
         super().__init__()
         self.names, self._empty = set(), []
-        for i, layer in enumerate(model.layers):
+        projections = [{f'{part}.{name}': proj for part in ('self_attn', 'mlp')
+                        for name, proj in getattr(layer, part).named_children() if name.endswith('_proj')}
+                       for layer in model.layers]
+        for held in projections:   # all of them, before the first one's bf16 weights are gone
+            for proj in held.values():
+                int8.check_rows(proj.weight)
+        for i, (layer, held) in enumerate(zip(model.layers, projections)):
             self.append(_Int8Layer(layer))
-            for part in ('self_attn', 'mlp'):
-                for name, proj in getattr(layer, part).named_children():
-                    if name.endswith('_proj'):
-                        proj.weight = nn.Parameter(torch.empty_like(proj.weight, device='meta'), requires_grad=False)
-                        self.names.add(f'model.layers.{i}.{part}.{name}.weight')
-                        self._empty.append((proj._parameters, proj.weight))
+            for name, proj in held.items():
+                proj.weight = nn.Parameter(torch.empty_like(proj.weight, device='meta'), requires_grad=False)
+                self.names.add(f'model.layers.{i}.{name}.weight')
+                self._empty.append((proj._parameters, proj.weight))
 
     def in_place(self):
         for held, empty in self._empty:   # a plain loop: this runs before every step

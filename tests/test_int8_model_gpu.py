@@ -341,3 +341,21 @@ def test_weights_beside_int8_are_refused():
     model.load_hf_state_dict(state)
     assert torch.equal(model(ids).logits, build(False)[0](ids).logits)
     assert torch.equal(model.quantize_weights()(ids).logits, want)
+
+
+def test_weights_that_cannot_be_quantised_leave_the_model_as_it_was():
+    """One weight of the last layer does not start on 16 bytes: quantize_weights refuses before any bf16 weight is gone."""
+    model, params = build(False)
+    ids = torch.arange(12, device='cuda').view(1, 12)
+    want = model(ids).logits
+    proj = model.model.layers[-1].mlp.down_proj
+    good = proj.weight
+    flat = torch.empty(good.numel() + 1, dtype=BF, device='cuda')
+    flat[1:].copy_(good.detach().flatten())
+    proj.weight = torch.nn.Parameter(flat[1:].view_as(good), requires_grad=False)
+    with pytest.raises(ValueError, match='16 bytes'):
+        model.quantize_weights()
+    proj.weight = good
+    assert model._int8 is None and torch.equal(model(ids).logits, want)
+    model.quantize_weights()
+    assert max_rel(model(ids).logits, want.float()) <= 0.1
