@@ -1,5 +1,5 @@
 """Serving in 8 bits: rows, RMSNorm, matrix products and a key/value cache in int8 with fp32 scales, and attention over
-that cache.  Forward only (inputs that require a gradient are refused); bf16 or fp16 around the codes.
+that cache.  Forward only (inputs that require a gradient or carry a tangent are refused); bf16 or fp16 around the codes.
 
 One rule for every group of values with one scale (a token's row, a weight's output channel, 64 cached positions of a
 head): with M the largest magnitude, a value is held as the integer nearest to 127 a / M (ties to even) and the scale is
@@ -11,6 +11,7 @@ serves in 16 bits only; nothing here has a counterpart in it.
 from dataclasses import dataclass
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 
 from .. import _hip as H
 
@@ -21,10 +22,15 @@ MAX_K = 1 << 17   # int32 sums of products of 8-bit codes stay exact below
 _FLOATS = (torch.bfloat16, torch.float16)
 
 
+def _dual(t):
+    """Whether t carries a tangent of forward-mode differentiation (which torch.no_grad does not end)."""
+    return _forward_ad._current_level >= 0 and _forward_ad.unpack_dual(t).tangent is not None
+
+
 def _forward_only(*tensors):
-    if torch.is_grad_enabled():
+    if torch.is_grad_enabled() or _forward_ad._current_level >= 0:
         for t in tensors:
-            if t is not None and t.requires_grad:
+            if t is not None and (t.requires_grad and torch.is_grad_enabled() or _dual(t)):
                 raise ValueError('int8 operators are forward only: run them under torch.no_grad or detach the inputs')
 
 
@@ -314,7 +320,7 @@ class LayerCache:
         for t in tensors:
             if t.device != dev or not t.is_contiguous() or t.data_ptr() % 16 and t.dtype != torch.float32:
                 raise ValueError('contiguous, 16-byte aligned cache buffers on one device required')
-            if t.requires_grad:
+            if t.requires_grad or _dual(t):
                 raise ValueError('cache buffers take no gradient')
 
     def pointers(self):

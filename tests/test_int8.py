@@ -308,3 +308,26 @@ def test_a_failed_load_over_int8(monkeypatch):
     assert model._int8 is None
     model.load_hf_state_dict(state)
     assert all(torch.equal(p, state[n]) for n, p in model.named_parameters())
+
+
+@pytest.mark.parametrize("grad", [True, False])
+def test_tangents_are_refused(grad):
+    """Inputs of forward-mode differentiation, whose tangents the outputs would not carry."""
+    import torch.autograd.forward_ad as fw
+    x, q, w, one = torch.ones(1, 32).bfloat16(), torch.zeros(1, 32, dtype=torch.int8), torch.zeros(8, 32, dtype=torch.int8), torch.ones(1)
+    t = torch.zeros(1, 1, 1, 128, dtype=torch.bfloat16)
+    cache = I8.LayerCache.empty(1, 1, 64, device='cpu')
+    with fw.dual_level(), torch.set_grad_enabled(grad):
+        dual = lambda a: fw.make_dual(a, torch.ones_like(a))  # noqa: E731
+        for call in (lambda: I8.quantize_rows(dual(x)), lambda: I8.rms_norm(x, dual(x[0]), 1e-6), lambda: I8.rms_norm(x, x[0], 1e-6, residual=dual(x)),
+                     lambda: I8.linear(q, one, w, dual(torch.ones(8))), lambda: I8.linear(q, dual(one), w, torch.ones(8)),
+                     lambda: I8.linear(q, one, w, torch.ones(8), residual=dual(torch.ones(1, 8).bfloat16())),
+                     lambda: I8.decode_linear(dual(x), [(w, torch.ones(8))]), lambda: I8.append(dual(t), t, cache, 0),
+                     lambda: I8.norm_rope_append(t, t, t, t[0, 0, 0], t[0, 0, 0], dual(t[0]), t[0], cache, 0),
+                     lambda: I8.attention(dual(t), cache, 0)):
+            with pytest.raises(ValueError, match='forward only'):
+                call()
+        with pytest.raises(ValueError, match='no gradient'):
+            I8.LayerCache(cache.k, cache.v, dual(cache.k_scale), cache.v_scale, cache.k_tail, cache.v_tail)
+        with pytest.raises(ValueError, match='ROCm device'):   # no tangent among them: the next check's turn
+            I8.quantize_rows(x)
