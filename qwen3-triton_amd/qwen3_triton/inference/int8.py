@@ -271,7 +271,10 @@ class LayerCache:
 
     A block is quantised once, from its 16-bit values, when its last position is appended; so what the cache holds does
     not depend on how the tokens were cut into chunks.  Positions are appended in order: the cache cannot be wound back
-    into a block that is already quantised (start again from 0 or another multiple of 64)."""
+    into a block that is already quantised (start again from 0 or another multiple of 64), nor read there, since the tail
+    holds another block's positions by then.  The object knows how far its own ``append`` calls went and refuses both; it does
+    not know what a captured or device-positioned call appends (after one it checks nothing more), nor what its buffers
+    held before or are given through another object."""
     k: torch.Tensor
     v: torch.Tensor
     k_scale: torch.Tensor
@@ -322,6 +325,18 @@ class LayerCache:
                 raise ValueError('contiguous, 16-byte aligned cache buffers on one device required')
             if t.requires_grad or _dual(t):
                 raise ValueError('cache buffers take no gradient')
+        self._appended(None)
+
+    def _appended(self, end):
+        """Note that the cache holds the positions before ``end`` (None: not known; -1: not known from now on)."""
+        object.__setattr__(self, '_end', end)
+
+    def require_whole(self, n):
+        """Raise if n, where an append is to start or a read to end, lies inside a block that is quantised already."""
+        end = self._end
+        if n % KV_BLOCK and end is not None and n < end // KV_BLOCK * KV_BLOCK:
+            raise ValueError(f'position {n} lies inside a quantised block of a cache of {end} positions: only a multiple of '
+                             f'{KV_BLOCK}, or a position of the unfinished block, can be gone back to')
 
     def pointers(self):
         return (self.k.data_ptr(), self.v.data_ptr(), self.k_scale.data_ptr(), self.v_scale.data_ptr(),
@@ -345,7 +360,8 @@ def _check_heads(t, cache, what):
     return sb, ss, sh
 
 
-def _check_span(start, s, cache, start_dev):
+def _check_span(start, s, cache, start_dev, new):
+    """``new``: whether the s positions are to be appended or are there."""
     if start_dev is not None:
         if s != 1:
             raise ValueError('device-resident positions are for single-token decode steps')
@@ -355,7 +371,16 @@ def _check_span(start, s, cache, start_dev):
         return 0
     if type(start) is not int or start < 0 or start + s > cache.capacity:
         raise ValueError(f'positions {start} .. {start} + {s} - 1 do not fit a cache of {cache.capacity}')
+    cache.require_whole(start if new else start + s)
     return start
+
+
+def _note(cache, start, s, start_dev):
+    """After an append.  What a captured one appends, and when, is not known here."""
+    if start_dev is not None or cache._end == -1 or torch.cuda.is_current_stream_capturing():
+        cache._appended(-1)
+    else:
+        cache._appended(start + s)
 
 
 def append(k, v, cache, start, start_dev=None):
@@ -366,9 +391,10 @@ def append(k, v, cache, start, start_dev=None):
     b, s, h, d = k.shape
     if v.shape != k.shape or h != cache.k.shape[1]:
         raise ValueError('keys and values of one shape, with the cache\'s heads, required')
-    start = _check_span(start, s, cache, start_dev)
+    start = _check_span(start, s, cache, start_dev, True)
     _launch(k, "q3_kv8_append", H.code(k.dtype), k.data_ptr(), *ks, v.data_ptr(), *vs, *cache.pointers(), b, s, h, d,
             cache.capacity, start, None if start_dev is None else start_dev.data_ptr())
+    _note(cache, start, s, start_dev)
 
 
 def _check_norm_rope(q, q_norm_weight, k_norm_weight, cos, sin, eps):
@@ -391,21 +417,24 @@ def norm_rope_append(q, k, v, q_norm_weight, k_norm_weight, cos, sin, cache, sta
     if v.shape != k.shape or k.shape[1] != s or h != cache.k.shape[1]:
         raise ValueError('queries, keys and values of one batch and length, with the cache\'s heads, required')
     _check_norm_rope(q, q_norm_weight, k_norm_weight, cos, sin, eps)
-    start = _check_span(start, s, cache, start_dev)
+    start = _check_span(start, s, cache, start_dev, True)
     out = q.new_empty((b, s, hq, d))
     _launch(q, "q3_kv8_norm_rope_append", H.code(q.dtype), q.data_ptr(), *qs, k.data_ptr(), *ks, v.data_ptr(), *vs,
             q_norm_weight.data_ptr(), k_norm_weight.data_ptr(), cos.data_ptr(), sin.data_ptr(), out.data_ptr(),
             *cache.pointers(), b, s, hq, h, d, cache.capacity, start, None if start_dev is None else start_dev.data_ptr(),
             float(eps))
+    _note(cache, start, s, start_dev)
     return out
 
 
 def read(cache, length, *, dtype=None):
-    """The ``length`` positions that the cache holds back as k, v [B, Hkv, length, 128] in ``dtype`` (the tail's by default)."""
+    """The ``length`` positions that the cache holds back as k, v [B, Hkv, length, 128] in ``dtype`` (the tail's by default).
+    Fewer than it holds can be read up to a multiple of 64, or to a position of its unfinished block."""
     _on_device(cache.k)
     b, h, capacity, _ = cache.k.shape
     if type(length) is not int or not 1 <= length <= capacity:
         raise ValueError(f'length must be an int in [1, {capacity}]')
+    cache.require_whole(length)
     dtype = cache.k_tail.dtype if dtype is None else dtype
     k, v = (cache.k.new_empty((b, h, length, 128), dtype=dtype) for _ in range(2))
     _launch(k, "q3_kv8_read", H.code(cache.k_tail.dtype), H.code(dtype), *cache.pointers(), k.data_ptr(), v.data_ptr(), b, h,
@@ -415,7 +444,7 @@ def read(cache, length, *, dtype=None):
 
 def attention(q, cache, start, start_dev=None, *, scale=None):
     """q [B, S, Hq, 128] at positions start .. start + S - 1, causal, against the cache's positions up to each query's own
-    (appended before); returns [B, S, Hq, 128].  With ``start_dev`` (S = 1) the position is read on the device and the
+    (appended before; where the cache holds more, ``start + S`` as ``read``'s length); returns [B, S, Hq, 128].  With ``start_dev`` (S = 1) the position is read on the device and the
     launch spans the whole capacity, so a captured step replays at any position."""
     _forward_only(q)
     qs = _check_heads(q, cache, 'queries')
@@ -423,7 +452,7 @@ def attention(q, cache, start, start_dev=None, *, scale=None):
     hkv = cache.k.shape[1]
     if hq % hkv:
         raise ValueError('query heads must be a multiple of key/value heads')
-    start = _check_span(start, s, cache, start_dev)
+    start = _check_span(start, s, cache, start_dev, False)
     scale = d ** -0.5 if scale is None else float(scale)
     if not 0.0 < scale < 1e30:
         raise ValueError('a positive softmax scale required')

@@ -104,8 +104,14 @@ class KVCache:
 @dataclass
 class Int8KVCache(KVCache):
     """A ``KVCache`` whose keys and values are held in int8, one ``int8.LayerCache`` per layer (``keys`` and ``values``
-    stay empty).  A block of 64 positions is quantised when its last one comes; the unfinished block is in bf16."""
+    stay empty).  A block of 64 positions is quantised when its last one comes; the unfinished block is in bf16.  So
+    ``length`` can be set back to 0, another multiple of 64 or a position of the unfinished block only."""
     layers: list = field(default_factory=list)
+
+    def admit(self, owner, batch, tokens):
+        super().admit(owner, batch, tokens)
+        for layer in self.layers[:1]:
+            layer.require_whole(self.length)
 
     @property
     def nbytes(self):

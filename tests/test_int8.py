@@ -331,3 +331,25 @@ def test_tangents_are_refused(grad):
             I8.LayerCache(cache.k, cache.v, dual(cache.k_scale), cache.v_scale, cache.k_tail, cache.v_tail)
         with pytest.raises(ValueError, match='ROCm device'):   # no tangent among them: the next check's turn
             I8.quantize_rows(x)
+
+
+def test_cache_knows_its_quantised_blocks():
+    from qwen3_triton.inference import Int8KVCache
+    c = I8.LayerCache.empty(1, 1, 256, device='cpu')
+    for n in range(257):
+        c.require_whole(n)   # nothing known yet
+    c._appended(200)
+    for n in range(257):
+        if n % 64 and n < 192:
+            with pytest.raises(ValueError, match='quantised block'):
+                c.require_whole(n)
+        else:
+            c.require_whole(n)
+    owner = object()
+    cache = Int8KVCache([], [], 256, 1, owner, 100, layers=[c])
+    with pytest.raises(ValueError, match='quantised block'):
+        cache.admit(owner, 1, 1)
+    cache.reset()
+    cache.admit(owner, 1, 1)
+    c._appended(-1)
+    c.require_whole(100)

@@ -784,3 +784,49 @@ def test_attention_key_scales_that_vanish(s):
     I8.append(k.cuda(), v.cuda(), c, 0)
     q = randn(1, s, 4, 128, gen=gen, dtype=torch.bfloat16, scale=4.0)
     check_attention(I8.attention(q.cuda(), c, t - s, scale=1e-20), q, held64(k, v)[0], t - s, 1e-20, torch.bfloat16)
+
+
+def test_going_back_into_a_quantised_block_is_refused():
+    """The tail holds the unfinished block alone: shorter reads and earlier appends go to a whole block or to a tail position."""
+    gen = seeded(9)
+    c, k, v = filled(1, 2, 200, torch.bfloat16, gen, cuts=(100,))   # tail: positions 192 .. 199
+    q = randn(1, 3, 4, 128, gen=gen, dtype=torch.bfloat16).cuda()
+    new = randn(1, 3, 2, 128, gen=gen, dtype=torch.bfloat16).cuda()
+    w, t = torch.ones(128, dtype=torch.bfloat16, device="cuda"), torch.ones(1, 3, 128, dtype=torch.bfloat16, device="cuda")
+    bits = lambda: [x.clone() for x in (c.k, c.v, c.k_tail.view(torch.int16), c.v_tail.view(torch.int16))]  # noqa: E731
+    keep = bits()
+    for bad in (lambda: I8.read(c, 50), lambda: I8.read(c, 191), lambda: I8.attention(q, c, 100), lambda: I8.attention(q, c, 188),
+                lambda: I8.append(new, new, c, 70), lambda: I8.append(new, new, c, 191),
+                lambda: I8.norm_rope_append(q, new, new, w, w, t, t, c, 1)):
+        with pytest.raises(ValueError, match='quantised block'):
+            bad()
+    assert all(torch.equal(a, b) for a, b in zip(keep, bits()))
+    values = held64(k, v)[0]
+    for n in (64, 128, 192, 195, 200):   # what it holds still
+        for got, want in zip(I8.read(c, n, dtype=torch.float32), values):
+            close(got, want[:, :, :n], want[:, :, :n].abs() * 2.0 ** -22)
+        check_attention(I8.attention(q, c, n - 3), q.cpu(), [x[:, :, :n] for x in values], n - 3, 128 ** -0.5, torch.bfloat16)
+    I8.append(new, new, c, 194)   # over the tail's own positions
+    k[:, 194:197], v[:, 194:197] = new.cpu(), new.cpu()
+    for got, want in zip(I8.read(c, 197, dtype=torch.float32), held64(k[:, :197], v[:, :197])[0]):
+        close(got, want, want.abs() * 2.0 ** -22)
+    I8.append(new, new, c, 128)   # back to a block: the positions from there on are others
+    with pytest.raises(ValueError, match='quantised block'):
+        I8.read(c, 120)
+    assert torch.equal(I8.read(c, 131)[0][:, :, 128:], new.transpose(1, 2))
+    # device positions, and captured calls, are not known on the host
+    I8.append(new[:, :1], new[:, :1], c, 0, torch.tensor([131], device="cuda"))
+    assert torch.equal(I8.read(c, 132)[0][:, :, 131:], new[:, :1].transpose(1, 2))
+    d, stream, graph = poisoned(1, 2, 200, torch.bfloat16), torch.cuda.Stream(), torch.cuda.CUDAGraph()
+    stream.wait_stream(torch.cuda.current_stream())
+    kd, vd = k.cuda(), v.cuda()
+    with torch.cuda.graph(graph, stream=stream):
+        I8.append(kd, vd, d, 0)
+    torch.cuda.current_stream().wait_stream(stream)
+    I8.append(kd[:, :10], vd[:, :10], d, 0)
+    assert torch.equal(I8.read(d, 10)[0], kd[:, :10].transpose(1, 2))
+    for _ in range(2):
+        graph.replay()
+        for got, want in zip(I8.read(d, 200, dtype=torch.float32), held64(k, v)[0]):
+            close(got, want, want.abs() * 2.0 ** -22)
+        I8.append(kd[:, :10], vd[:, :10], d, 0)

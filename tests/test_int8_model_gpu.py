@@ -359,3 +359,26 @@ def test_weights_that_cannot_be_quantised_leave_the_model_as_it_was():
     assert model._int8 is None and torch.equal(model(ids).logits, want)
     model.quantize_weights()
     assert max_rel(model(ids).logits, want.float()) <= 0.1
+
+
+def test_an_int8_cache_is_not_wound_back_into_a_block(model):
+    """Its length can go back to a multiple of 64 or within the unfinished block; elsewhere the next step refuses."""
+    m, _, _ = model
+    ids = torch.randint(0, CFG.vocab_size, (1, 150), generator=seeded(8)).cuda()
+    cache = m.new_cache(1, 200, dtype=torch.int8)
+    m(ids, past_key_values=cache)
+    want = m(ids[:, 140:145].contiguous(), past_key_values=cache).logits
+    for back in (100, 127):
+        cache.length = back
+        with pytest.raises(ValueError, match='quantised block'):
+            m(ids[:, :1].contiguous(), past_key_values=cache)
+        with pytest.raises(ValueError, match='quantised block'):
+            cache.dequantized()
+        assert cache.valid
+    cache.length = 150   # a tail position: the same tokens again
+    assert torch.equal(m(ids[:, 140:145].contiguous(), past_key_values=cache).logits, want)
+    cache.length = 128
+    m(ids[:, 128:].contiguous(), past_key_values=cache)
+    cache.reset()
+    m(ids[:, :70].contiguous(), past_key_values=cache)
+    assert cache.length == 70
