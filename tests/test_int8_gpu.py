@@ -830,3 +830,31 @@ def test_going_back_into_a_quantised_block_is_refused():
         for got, want in zip(I8.read(d, 200, dtype=torch.float32), held64(k, v)[0]):
             close(got, want, want.abs() * 2.0 ** -22)
         I8.append(kd[:, :10], vd[:, :10], d, 0)
+
+
+@pytest.mark.parametrize("b,hq,h", [(1, 8, 2), (3, 32, 8)])
+@pytest.mark.parametrize("dtype", DT)
+def test_captured_step_over_several_splits(b, hq, h, dtype):
+    """A captured step in a long capacity, at lengths of several splits (which follow from the position alone): the bits of the
+    eager call, and both against 64 bits."""
+    gen = seeded(b)
+    lengths, cap = (255, 300, 769, 1500, 3000), 6000
+    k, v = randn(b, lengths[-1] + 1, h, 128, gen=gen, dtype=dtype), randn(b, lengths[-1] + 1, h, 128, gen=gen, dtype=dtype)
+    kd, vd = k.cuda(), v.cuda()
+    c, pos = poisoned(b, h, cap, dtype), torch.zeros(1, dtype=torch.int64, device="cuda")
+    q, kk, vv = (torch.zeros(b, 1, n, 128, dtype=dtype, device="cuda") for n in (hq, h, h))
+    graph, stream = torch.cuda.CUDAGraph(), torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.graph(graph, stream=stream):
+        I8.append(kk, vv, c, 0, pos)
+        o = I8.attention(q, c, 0, pos)
+    torch.cuda.current_stream().wait_stream(stream)
+    for n in lengths:
+        I8.append(kd[:, :n], vd[:, :n], c, 0)
+        d = I8.LayerCache(*(t.clone() for t in (c.k, c.v, c.k_scale, c.v_scale, c.k_tail, c.v_tail)))
+        new = randn(b, 1, hq, 128, gen=gen, dtype=dtype)
+        q.copy_(new), kk.copy_(kd[:, n:n + 1]), vv.copy_(vd[:, n:n + 1]), pos.fill_(n)
+        graph.replay()
+        I8.append(kd[:, n:n + 1], vd[:, n:n + 1], d, n)
+        assert torch.equal(o, I8.attention(q, d, n)), n
+        check_attention(o, new, held64(k[:, :n + 1], v[:, :n + 1])[0], n, 128 ** -0.5, dtype)

@@ -382,3 +382,58 @@ def test_an_int8_cache_is_not_wound_back_into_a_block(model):
     cache.reset()
     m(ids[:, :70].contiguous(), past_key_values=cache)
     assert cache.length == 70
+
+
+def test_chunked_prefill_holds_alike_blocks(model):
+    """With bf16 weights too: a projection's sums depend on the number of its rows (the kernel that forms them), so its bf16
+    result may lie one rounding aside (2^-7 of it).  Values follow it; keys by twice that of either dim after the norm, 2^-6 of
+    |n c| + |r s| <= sqrt(2) of the block's largest, and round once more (2^-7).  Each side's code is half a step from its value."""
+    m, _, _ = model
+    ids = torch.randint(0, CFG.vocab_size, (2, 200), generator=seeded(1)).cuda()
+    held = []
+    for cuts in ((200,), (1, 63, 64, 65, 190, 200), (100, 200)):
+        cache, at = m.new_cache(2, 200, dtype=torch.int8), 0
+        for end in cuts:
+            m(ids[:, at:end].contiguous(), past_key_values=cache)
+            at = end
+        held.append([t[:, :, :192].double() for t in int8.read(cache.layers[0], 200, dtype=torch.float32)])
+    for other in held[1:]:
+        for a, b in zip(held[0], other):
+            block = a.view(2, -1, 3, 64 * 128)
+            most = block.abs().amax(-1, keepdim=True) * (1 + 2.0 ** -5)   # either side's M
+            step = most * (2.0 ** -6 * 2 ** 0.5 + 2.0 ** -7 + 1 / 127)
+            assert bool(((block - b.view_as(block)).abs() <= step).all())
+
+
+@pytest.mark.parametrize("b", [1, 2, 3, 17])
+def test_decode_steps_over_a_16_bit_cache(model, b):
+    """Teacher-forced decode steps, every projection at its few-row forms, against the whole sequence in 64 bits."""
+    m, params, weights8 = model
+    ids = torch.randint(0, CFG.vocab_size, (b, 75), generator=seeded(b + 40))
+    cache = m.new_cache(b, 75)
+    m(ids[:, :60].cuda(), past_key_values=cache)
+    got = torch.cat([m(ids[:, t:t + 1].cuda(), past_key_values=cache).logits for t in range(60, 75)], 1)
+    assert max_rel(got, forward64(params, ids, weights8, False)[:, 60:]) <= GATE[weights8]
+
+
+def test_head_norms_with_an_eps_each(model):
+    """Norms whose eps were set apart: the int8 cache's tail holds the keys that the 16-bit cache holds."""
+    m, _, _ = model
+    ids = torch.randint(0, CFG.vocab_size, (1, 40), generator=seeded(4)).cuda()
+    norms = [layer.self_attn.k_norm for layer in m.model.layers]
+    keys = []
+    eps = norms[0].eps
+    try:
+        for e in (eps, 1.0):
+            for norm in norms:
+                norm.eps = e
+            c8, c16 = m.new_cache(1, 64, dtype=torch.int8), m.new_cache(1, 64)
+            a, b = (m(ids, past_key_values=c).logits for c in (c8, c16))
+            assert torch.equal(c8.layers[0].k_tail[:, :, :40], c16.keys[0][:, :, :40]) and max_rel(a, b.float()) <= GATE[True]
+            step = [m(ids[:, :1].contiguous(), past_key_values=c).logits for c in (c8, c16)]
+            assert max_rel(step[0], step[1].float()) <= GATE[True]
+            keys.append(c16.keys[0][:, :, :40].clone())
+    finally:
+        for norm in norms:
+            norm.eps = eps
+    assert not torch.equal(*keys)
