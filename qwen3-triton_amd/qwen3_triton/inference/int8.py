@@ -325,16 +325,20 @@ class LayerCache:
                 raise ValueError('contiguous, 16-byte aligned cache buffers on one device required')
             if t.requires_grad or _dual(t):
                 raise ValueError('cache buffers take no gradient')
-        self._appended(None)
+        self._know(None, 0)
 
-    def _appended(self, end):
-        """Note that the cache holds the positions before ``end`` (None: not known; -1: not known from now on)."""
+    def _know(self, end, tail):
+        """Note that the cache holds the positions before ``end`` (None: not known; -1: not known from now on), and the tail
+        those of its block before ``tail`` (a block's last append leaves there what was before it)."""
         object.__setattr__(self, '_end', end)
+        object.__setattr__(self, '_tail', tail)
 
     def require_whole(self, n):
-        """Raise if n, where an append is to start or a read to end, lies inside a block that is quantised already."""
+        """Raise if n, where an append is to start or a read to end, lies inside a block that is quantised already (and no
+        longer in the tail)."""
         end = self._end
-        if n % KV_BLOCK and end is not None and n < end // KV_BLOCK * KV_BLOCK:
+        if n % KV_BLOCK and end is not None and n < end // KV_BLOCK * KV_BLOCK and \
+                not self._tail // KV_BLOCK * KV_BLOCK < n <= self._tail:
             raise ValueError(f'position {n} lies inside a quantised block of a cache of {end} positions: only a multiple of '
                              f'{KV_BLOCK}, or a position of the unfinished block, can be gone back to')
 
@@ -378,9 +382,16 @@ def _check_span(start, s, cache, start_dev, new):
 def _note(cache, start, s, start_dev):
     """After an append.  What a captured one appends, and when, is not known here."""
     if start_dev is not None or cache._end == -1 or torch.cuda.is_current_stream_capturing():
-        cache._appended(-1)
-    else:
-        cache._appended(start + s)
+        cache._know(-1, 0)
+        return
+    end, tail = start + s, cache._tail
+    if end % KV_BLOCK:
+        tail = end
+    elif start % KV_BLOCK:
+        tail = start
+    elif tail > start:   # the positions that it held are others now
+        tail = 0
+    cache._know(end, tail)
 
 
 def append(k, v, cache, start, start_dev=None):

@@ -333,23 +333,35 @@ def test_tangents_are_refused(grad):
             I8.quantize_rows(x)
 
 
-def test_cache_knows_its_quantised_blocks():
+def test_cache_knows_its_quantised_blocks(monkeypatch):
     from qwen3_triton.inference import Int8KVCache
+    monkeypatch.setattr(torch.cuda, 'is_current_stream_capturing', lambda: False)
     c = I8.LayerCache.empty(1, 1, 256, device='cpu')
-    for n in range(257):
-        c.require_whole(n)   # nothing known yet
-    c._appended(200)
-    for n in range(257):
-        if n % 64 and n < 192:
-            with pytest.raises(ValueError, match='quantised block'):
+
+    def check(ok):
+        for n in range(257):
+            if ok(n):
                 c.require_whole(n)
-        else:
-            c.require_whole(n)
+            else:
+                with pytest.raises(ValueError, match='quantised block'):
+                    c.require_whole(n)
+    check(lambda n: True)   # nothing known yet
+    I8._note(c, 0, 200, None)
+    check(lambda n: n % 64 == 0 or n > 192)
     owner = object()
     cache = Int8KVCache([], [], 256, 1, owner, 100, layers=[c])
     with pytest.raises(ValueError, match='quantised block'):
         cache.admit(owner, 1, 1)
     cache.reset()
     cache.admit(owner, 1, 1)
-    c._appended(-1)
-    c.require_whole(100)
+    I8._note(c, 200, 20, None)
+    I8._note(c, 220, 36, None)   # the block's end: the tail still holds 192 .. 219
+    check(lambda n: n % 64 == 0 or 192 < n <= 220)
+    I8._note(c, 210, 46, None)   # other positions from 210 on
+    check(lambda n: n % 64 == 0 or 192 < n <= 210)
+    I8._note(c, 64, 64, None)   # started again at 64: what lies behind 128 is no longer held
+    check(lambda n: n % 64 == 0 or n > 128)
+    I8._note(c, 128, 127, None)
+    check(lambda n: n % 64 == 0 or n > 192)
+    I8._note(c, 255, 1, torch.zeros(1, dtype=torch.int64))
+    check(lambda n: True)

@@ -858,3 +858,19 @@ def test_captured_step_over_several_splits(b, hq, h, dtype):
         I8.append(kd[:, n:n + 1], vd[:, n:n + 1], d, n)
         assert torch.equal(o, I8.attention(q, d, n)), n
         check_attention(o, new, held64(k[:, :n + 1], v[:, :n + 1])[0], n, 128 ** -0.5, dtype)
+
+
+def test_going_back_over_a_block_s_last_token():
+    """A block's last append leaves the tail as it was: that token can be taken back, and another one appended."""
+    gen = seeded(10)
+    for cut in (127, 100):
+        c, k, v = filled(1, 2, 128, torch.bfloat16, gen, cuts=(cut,))
+        close(I8.read(c, cut, dtype=torch.float32)[0], held64(k[:, :cut], v[:, :cut])[0][0], 2.0 ** -22 * k.double().transpose(1, 2)[:, :, :cut].abs() + 2.0 ** -22)
+        k2, v2 = (randn(1, 128 - cut, 2, 128, gen=gen, dtype=torch.bfloat16, scale=0.5) for _ in range(2))
+        I8.append(k2.cuda(), v2.cuda(), c, cut)
+        fresh = poisoned(1, 2, 128, torch.bfloat16)
+        I8.append(torch.cat([k[:, :cut], k2], 1).cuda(), torch.cat([v[:, :cut], v2], 1).cuda(), fresh, 0)
+        for got, want in zip(I8.read(c, 128), I8.read(fresh, 128)):
+            assert torch.equal(got, want)
+        with pytest.raises(ValueError, match='quantised block'):
+            I8.append(k2.cuda()[:, :1], v2.cuda()[:, :1], c, {127: 62, 100: 101}[cut])
