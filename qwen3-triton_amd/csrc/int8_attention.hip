@@ -13,9 +13,9 @@
 // The running maximum and sum of the softmax are per row, replicated over the 4 lane groups.
 // The unfinished block is read from the 16-bit tail in the same lane order (V tail transposed as well).
 // Bound by HBM at one token over a long cache (8 rows x 20001 positions x 8 heads: 58.8 us, 5.6 TB/s), by latency over a short
-// one (2048 positions: 5.8 us + 2.2 - 3.3 for the join); with many queries by the vector units' exponentials and conversions,
-// the matrix cores and LDS, about 2500, 2050 and 2050 cycles of a 256-row block's 5000 (8192 queries of 32 heads: 537 - 575 us, as
-// the 16-bit kernel's 501 - 576; 1024 queries at 3000: 79 - 86 us + 9.5).
+// one (2048 positions: 5.8 us + 2.2 - 3.3 for the join); with many queries by the vector units (exponentials, conversions) beside
+// the matrix cores: by counters 2490 and 2050 of the 4600 cycles that a CU takes for a 256-row block, LDS 1290 without bank
+// conflicts (8192 queries of 32 heads: 537 - 575 us, as the 16-bit kernel's 501 - 576; 1024 queries at 3000: 79 - 86 us + 9.5).
 #include <algorithm>
 
 #include "int8_cache.h"

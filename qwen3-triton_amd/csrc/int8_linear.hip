@@ -21,7 +21,8 @@ namespace q3gemm {
 // first weights are on their way: quantize_rows, or with NORM rms_norm.  Each workgroup repeats that work on rows that sit
 // in L2; it saves a launch and its wait, and a decode step has one before each of its four products.  One row: 9.2 against
 // 12.0 us (6144 x 4096 after a norm), 13.0 against 16.0 (4096 x 12288), 20.6 against 25.1 (gate/up); two rows 9.9, 14.3 and 22.1
-// against 12.1, 16.0 and 25.4.  Four rows, with a tile per workgroup, were level (13.9 and 13.8, 20.9 and 18.5): it stops at two.
+// against 12.1, 16.0 and 25.4.  Four rows are level (11.6 against 12.5, 19.5 against 18.4, 29.4 against 27.6; 4096 x 4096 9.7 and
+// 10.9), three likewise: it stops at two.
 // V: 16-byte pieces of a row per thread.
 template <typename T, int EPI, int P, int R, int V, bool NORM>
 __global__ __launch_bounds__(512) void gemm_rows_q8_kernel(Args a, RowIn in, int tiles) {
