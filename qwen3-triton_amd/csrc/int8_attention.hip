@@ -54,9 +54,11 @@ Q3_DEV int pack_f16x2(float lo, float hi) {
   return __builtin_bit_cast(int, __builtin_convertvector(v, f16x2_t));
 }
 
-// P with 11 bits is as close as bf16 outputs can tell; to fp16 outputs it adds as much error as their own rounding (1.4 - 1.6
-// times a 32-bit P's in all), so the kernel of few rows, which waits for memory, takes the remainder p - fp16(p) in a second
-// product.  The kernel of many rows has no registers for it (85 spilled); its sums are of the rounded P, which leaves 1.25 - 1.4.
+// P with 11 bits leaves bf16 outputs 0.6 % farther from 64 bits than a 32-bit P (their own rounding is 8 times as large); its
+// remainder in a second product would cost few rows 2 - 4 % (2048 positions 7.7 -> 8.1 us, 8 x 20001 57.2 -> 58.2).  To fp16
+// outputs 11 bits add as much error as their own rounding (1.4 - 1.6 times a 32-bit P's in all), so there the kernel of few
+// rows, which waits for memory, takes the remainder p - fp16(p).  The kernel of many rows has no registers for it (85 spilled);
+// its sums are of the rounded P, which leaves 1.25 - 1.4.
 template <typename T> constexpr bool kTwoTerms = T::code == Q3_F16;
 Q3_DEV int pack_rest_f16x2(float lo, float hi, int packed) {
   const f16x2_t h = __builtin_bit_cast(f16x2_t, packed);
