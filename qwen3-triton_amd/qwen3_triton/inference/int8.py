@@ -455,8 +455,9 @@ def read(cache, length, *, dtype=None):
 
 def attention(q, cache, start, start_dev=None, *, scale=None):
     """q [B, S, Hq, 128] at positions start .. start + S - 1, causal, against the cache's positions up to each query's own
-    (appended before; where the cache holds more, ``start + S`` as ``read``'s length); returns [B, S, Hq, 128].  With ``start_dev`` (S = 1) the position is read on the device and the
-    launch spans the whole capacity, so a captured step replays at any position."""
+    (appended before; where the cache holds more, ``start + S`` as ``read``'s length); returns [B, S, Hq, 128].  With
+    ``start_dev`` (S = 1) the position is read on the device and the launch spans the whole capacity, so a captured step
+    replays at any position."""
     _forward_only(q)
     qs = _check_heads(q, cache, 'queries')
     b, s, hq, d = q.shape
