@@ -551,6 +551,42 @@ int q3_kv8_attention(int dtype, const void* q, int64_t qsb, int64_t qss, int64_t
                      size_t workspace_bytes, int64_t B, int64_t S, int64_t Hq, int64_t Hkv, int64_t d, int64_t capacity,
                      int64_t start, const int64_t* start_dev, float scale, hipStream_t stream);
 
+/* ------------------------------------------------------------------ log probabilities of tokens
+ * New: no counterpart in the reference.  Of rows z [rows, vocab] (row stride ld >= vocab, any alignment) at a temperature
+ * (inv_temperature = 1 / it): logprob[r] = log softmax(z[r] / temperature)[tokens[r]], entropy[r] of that softmax, and the top
+ * (0 .. 32) largest log probabilities with their tokens, [rows, top], in falling order (equal logits: the lower token first;
+ * NaN first of all).  row_max and row_log [rows] keep what the gradient needs.  All results are fp32 / int64.
+ * A row whose token is ignore_index is left out: zeros, and none of its logits is read.  Any other token outside
+ * [0, vocab) gets NaN.  A row of -inf only, or with a NaN or +inf, gets NaN.  vocab < 2^30, with top <= 2^21. */
+size_t q3_token_logprobs_workspace_bytes(int dtype, int64_t rows, int64_t vocab, int64_t top);
+int q3_token_logprobs(int dtype, const void* z, int64_t ld, int64_t rows, int64_t vocab, const int64_t* tokens,
+                      int64_t ignore_index, float inv_temperature, int64_t top, float* logprob, float* entropy,
+                      float* row_max, float* row_log, float* top_logprob, int64_t* top_token, void* workspace,
+                      size_t workspace_bytes, hipStream_t stream);
+/* dz [rows, vocab] (row stride ldo; out_dtype: dtype, or a 16-bit type from fp32 logits) of upstream gradients g of logprob, gh of entropy [rows] and gtop of top_logprob
+ * [rows, top], each or NULL; rows left out get zeros. */
+int q3_token_logprobs_bwd(int dtype, int out_dtype, const void* z, int64_t ld, int64_t rows, int64_t vocab, const int64_t* tokens,
+                          int64_t ignore_index, float inv_temperature, int64_t top, const int64_t* top_token,
+                          const float* row_max, const float* row_log, const float* entropy, const float* g,
+                          const float* gh, const float* gtop, void* dz, int64_t ldo, hipStream_t stream);
+
+/* ------------------------------------------------------------------ attention over a shared prefix
+ * New: no counterpart in the reference.  B rows in R groups of B / R; queries q [B, S, Hq, 128] of row b stand at its own
+ * positions start_b .. start_b + S - 1 and see all P positions of prefix b / (B / R) (prefix_k, prefix_v [R, Hkv, P, 128];
+ * P = 0: none) and its own up to theirs (cache_k, cache_v [B, Hkv, C, 128], appended before).  A query that sees no position
+ * (P = 0 and a negative end) gets zeros.  Strides in elements, of batch, head and position (keys and values alike): multiples
+ * of 8 with 16-byte aligned bases, position strides in [128, 2^24); of out multiples of 4, 8-byte aligned.
+ * start_dev: that device int64 (starts = 1) or one a row (starts = B) instead of start, read when the kernel runs; positions
+ * outside the capacity are not there.  The workspace is sized for span = C then, else for span = start + S. */
+size_t q3_prefix_attention_workspace_bytes(int64_t B, int64_t R, int64_t S, int64_t Hq, int64_t Hkv, int64_t P,
+                                           int64_t span);
+int q3_prefix_attention(int dtype, const void* q, int64_t qsb, int64_t qss, int64_t qsh, const void* prefix_k,
+                        const void* prefix_v, int64_t psb, int64_t psh, int64_t pss, const void* cache_k,
+                        const void* cache_v, int64_t csb, int64_t csh, int64_t css, void* out, int64_t osb, int64_t oss,
+                        int64_t osh, void* workspace, size_t workspace_bytes, int64_t B, int64_t R, int64_t S, int64_t Hq,
+                        int64_t Hkv, int64_t d, int64_t P, int64_t C, int64_t start, const int64_t* start_dev,
+                        int64_t starts, float scale, hipStream_t stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -132,6 +132,13 @@ SIGNATURES: dict[str, tuple] = {
     "q3_kv8_attention_workspace_bytes": (_sz, [_i64, _i64, _i64, _i64, _i64]),
     "q3_kv8_attention": (_i32, [_i32, _p, _i64, _i64, _i64, _p, _p, _p, _p, _p, _p, _p, _i64, _i64, _i64, _p, _sz, _i64,
                                 _i64, _i64, _i64, _i64, _i64, _i64, _p, _f32, _p]),
+    "q3_token_logprobs_workspace_bytes": (_sz, [_i32, _i64, _i64, _i64]),
+    "q3_token_logprobs": (_i32, [_i32, _p, _i64, _i64, _i64, _p, _i64, _f32, _i64, _p, _p, _p, _p, _p, _p, _p, _sz, _p]),
+    "q3_token_logprobs_bwd": (_i32, [_i32, _i32, _p, _i64, _i64, _i64, _p, _i64, _f32, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _i64,
+                                     _p]),
+    "q3_prefix_attention_workspace_bytes": (_sz, [_i64] * 7),
+    "q3_prefix_attention": (_i32, [_i32, _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _i64,
+                                   _i64, _i64, _p, _sz, *[_i64] * 9, _p, _i64, _f32, _p]),
     "q3_gemm_strided": (_i32, [_i32, _i32, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _f32, _i32,
                                 _p]),
 }
@@ -170,6 +177,14 @@ def call(name: str, *args) -> None:
     if rc != 0:
         msg = load().q3_error_string(rc).decode()
         raise RuntimeError(f"{name} failed: {msg} (code {rc})")
+
+
+def launch(t: torch.Tensor, name: str, *args) -> None:
+    """``call`` on t's device and its current stream (appended to ``args``), whatever device is current."""
+    if t.get_device() == torch._C._cuda_getDevice():
+        return call(name, *args, stream())
+    with torch.cuda.device(t.device):
+        return call(name, *args, stream())
 
 
 def query(name: str, *args) -> int:

@@ -1,0 +1,231 @@
+"""Log probabilities of given tokens, with the entropy of their distributions and the most likely alternatives, from logits or
+straight from hidden states and the LM head's weight; differentiable.
+
+Of each row, with p = softmax(logits / temperature): log p[token], -sum p log p, and the ``top`` largest log p with their tokens
+(equal logits: the lower token first).  Everything is formed and returned in fp32.  The reference has a mean cross-entropy and
+an argmax only; nothing here has a counterpart in it.
+"""
+from typing import NamedTuple, Optional
+
+import torch
+from torch.autograd.function import once_differentiable
+
+from .. import _hip as H
+from ._ops import cast
+from .linear import gemm, gemm_nt_into, gemm_ok, matmul_into
+
+MAX_TOP = 32
+IGNORE_INDEX = -100
+_FLOATS = (torch.float32, torch.bfloat16, torch.float16)
+
+
+class TokenLogprobs(NamedTuple):
+    """Of tokens [...]: ``logprobs`` and ``entropy`` fp32 [...], and with ``top`` = K > 0 the K most likely tokens in order,
+    ``top_logprobs`` fp32 and ``top_tokens`` int64 [..., K] (else None)."""
+    logprobs: torch.Tensor
+    entropy: torch.Tensor
+    top_logprobs: Optional[torch.Tensor] = None
+    top_tokens: Optional[torch.Tensor] = None
+
+
+def _check_options(vocab, top, temperature, ignore_index):
+    if type(top) is not int or not 0 <= top <= min(MAX_TOP, vocab):
+        raise ValueError(f'top must be an int in [0, {min(MAX_TOP, vocab)}]')
+    if vocab >= 1 << 30 or (top and vocab > 1 << 21):
+        raise ValueError('fewer than 2^30 tokens, with top at most 2^21, required')
+    if not 1e-6 <= float(temperature) <= 1e6:
+        raise ValueError('a temperature in [1e-6, 1e6] required')
+    if type(ignore_index) is not int:
+        raise ValueError('ignore_index must be an int')
+
+
+def _check_tokens(tokens, shape, device):
+    if tokens.dtype != torch.int64 or tokens.shape != shape or tokens.device != device or not tokens.is_contiguous():
+        raise ValueError(f'contiguous int64 tokens {tuple(shape)} on the same device required')
+
+
+def _logit_rows(logits):
+    """logits [..., V] as (rows, row stride, V): rows at one stride, each contiguous."""
+    v = logits.shape[-1]
+    rows = logits.numel() // v
+    if logits.is_contiguous():
+        return rows, v, v
+    try:
+        m = logits.view(rows, v)
+    except RuntimeError:
+        raise ValueError('logits whose rows lie at one stride required; no hidden layout copy') from None
+    if v > 1 and m.stride(1) != 1 or rows > 1 and m.stride(0) < v:
+        raise ValueError('contiguous rows of logits that do not overlap required; no hidden layout copy')
+    return rows, m.stride(0) if rows > 1 else v, v
+
+
+def _forward(z, rows, ld, v, tokens, ignore_index, temperature, top, outs=None, at=0):
+    """q3_token_logprobs of rows of z; into rows ``at`` .. of ``outs`` where those are given."""
+    if outs is None:
+        outs = _outputs(z, rows, top)
+    lp, ent, m, ls, tlp, tid = (None if t is None else t[at:] for t in outs)
+    nbytes = H.query("q3_token_logprobs_workspace_bytes", H.code(z.dtype), rows, v, top)
+    ws = H.workspace(nbytes, z.device)
+    H.launch(z, "q3_token_logprobs", H.code(z.dtype), z.data_ptr(), ld, rows, v, tokens.data_ptr() + 8 * at, ignore_index,
+             1.0 / float(temperature), top, lp.data_ptr(), ent.data_ptr(), m.data_ptr(), ls.data_ptr(),
+             None if tlp is None else tlp.data_ptr(), None if tid is None else tid.data_ptr(), ws.data_ptr(), nbytes)
+    return outs
+
+
+def _outputs(ref, rows, top):
+    """(log probability, entropy, row maximum, row log, alternatives' log probabilities, their tokens)"""
+    f = dict(device=ref.device, dtype=torch.float32)
+    outs = torch.empty(rows, **f), torch.empty(rows, **f), *torch.empty((2, rows), **f).unbind(0)
+    if not top:
+        return (*outs, None, None)
+    return (*outs, torch.empty((rows, top), **f), torch.empty((rows, top), device=ref.device, dtype=torch.int64))
+
+
+def _backward(z, rows, ld, v, tokens, ignore_index, temperature, top, top_tokens, m, ls, ent, g, gh, gtop, dz, ldo, at=0):
+    """q3_token_logprobs_bwd of rows ``at`` .. ``at`` + rows - 1 (z and dz start there)."""
+    def p(t, width=4):
+        return None if t is None else t.data_ptr() + at * width
+    H.launch(z, "q3_token_logprobs_bwd", H.code(z.dtype), H.code(dz.dtype), z.data_ptr(), ld, rows, v, p(tokens, 8), ignore_index,
+             1.0 / float(temperature), top, p(top_tokens, 8 * top), p(m), p(ls), p(ent), p(g), p(gh), p(gtop, 4 * top),
+             dz.data_ptr(), ldo)
+
+
+def _upstream(g):
+    return None if g is None else g.float().contiguous()
+
+
+class _TokenLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, logits, tokens, ignore_index, temperature, top):
+        rows, ld, v = _logit_rows(logits)
+        lp, ent, m, ls, tlp, tid = _forward(logits, rows, ld, v, tokens, ignore_index, temperature, top)
+        shape = logits.shape[:-1]
+        ctx.save_for_backward(logits, tokens, m, ls, ent, tid)
+        ctx.rest = ignore_index, temperature, top
+        ctx.set_materialize_grads(False)
+        if not top:
+            return lp.view(shape), ent.view(shape)
+        tid = tid.view(*shape, top)
+        ctx.mark_non_differentiable(tid)
+        return lp.view(shape), ent.view(shape), tlp.view(*shape, top), tid
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, gh, gtop=None, _=None):
+        logits, tokens, m, ls, ent, tid = ctx.saved_tensors
+        ignore_index, temperature, top = ctx.rest
+        rows, ld, v = _logit_rows(logits)
+        dz = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
+        _backward(logits, rows, ld, v, tokens, ignore_index, temperature, top, tid, m, ls, ent, _upstream(g), _upstream(gh),
+                  _upstream(gtop), dz, v)
+        return dz, None, None, None, None
+
+
+def token_logprobs(logits, tokens, *, top=0, temperature=1.0, ignore_index=IGNORE_INDEX):
+    """``TokenLogprobs`` of tokens [...] (int64) under logits [..., V] in fp32, bf16 or fp16 (rows at one stride, such as
+    ``logits[:, -1]``); nothing is shifted: row i's token is what row i's logits predict.
+
+    A position whose token is ``ignore_index`` is left out: zeros, and no gradient.  Any other token outside [0, V) has the log
+    probability NaN (it is not looked for on the host: nothing here synchronises), and so has every token of a row that holds
+    a NaN or +inf or only -inf.  Logits of -inf (tokens ruled out) have probability 0.  The gradient reaches the logits from all
+    of ``logprobs``, ``entropy`` and ``top_logprobs``."""
+    if logits.ndim < 1 or logits.numel() < 1:
+        raise ValueError('nonempty [..., V] logits required')
+    H.require_device(logits)
+    if logits.dtype not in _FLOATS:
+        raise TypeError(f'float32, bfloat16 or float16 logits required, not {logits.dtype}')
+    _check_options(logits.shape[-1], top, temperature, ignore_index)
+    _check_tokens(tokens, logits.shape[:-1], logits.device)
+    _logit_rows(logits)
+    return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, ignore_index, float(temperature), top))
+
+
+# ---------------------------------------------------------------- from hidden states
+_CHUNK_BYTES = 1 << 30   # of fp32 logits at a time
+
+
+def _chunks(rows, v):
+    step = max(1, min(rows, _CHUNK_BYTES // (4 * v)))
+    step = step if step == rows or step < 256 else step // 256 * 256
+    return [(r, min(r + step, rows)) for r in range(0, rows, step)]
+
+
+def _logits(x, w, z):
+    """z = x w^T in fp32."""
+    if x.dtype != torch.float32 and x.shape[1] % 8 == 0 and x.data_ptr() % 16 == 0 and w.data_ptr() % 16 == 0:
+        gemm_nt_into(x, x.shape[1], w, w.shape[1], z, x.shape[0], w.shape[0], x.shape[1])
+    else:
+        matmul_into(x, w.t(), z)
+
+
+class _LMHeadLogprobs(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, hidden, weight, tokens, ignore_index, temperature, top):
+        v, h = weight.shape
+        x = hidden.view(-1, h)
+        t = x.shape[0]
+        with torch.cuda.device(x.device):
+            outs = _outputs(x, t, top)
+            chunks = _chunks(t, v)
+            z = torch.empty((chunks[0][1], v), device=x.device, dtype=torch.float32)
+            for r, end in chunks:
+                _logits(x[r:end], weight, z[:end - r])
+                _forward(z, end - r, v, v, tokens, ignore_index, temperature, top, outs, r)
+        lp, ent, m, ls, tlp, tid = outs
+        shape = hidden.shape[:-1]
+        ctx.save_for_backward(hidden, weight, tokens, m, ls, ent, tid)
+        ctx.rest = ignore_index, temperature, top
+        ctx.set_materialize_grads(False)
+        if not top:
+            return lp.view(shape), ent.view(shape)
+        tid = tid.view(*shape, top)
+        ctx.mark_non_differentiable(tid)
+        return lp.view(shape), ent.view(shape), tlp.view(*shape, top), tid
+
+    @staticmethod
+    @once_differentiable
+    def backward(ctx, g, gh, gtop=None, _=None):
+        hidden, weight, tokens, m, ls, ent, tid = ctx.saved_tensors
+        ignore_index, temperature, top = ctx.rest
+        v, h = weight.shape
+        x = hidden.view(-1, h)
+        t = x.shape[0]
+        g, gh, gtop = _upstream(g), _upstream(gh), _upstream(gtop)
+        with torch.cuda.device(x.device):
+            whole = gemm_ok(x, weight) and v % 8 == 0   # dW = dz^T x and dX = dz W from one dz [T, V]
+            chunks = _chunks(t, v)
+            z = torch.empty((chunks[0][1], v), device=x.device, dtype=torch.float32)
+            dz = torch.empty((t if whole else chunks[0][1], v), device=x.device, dtype=x.dtype)
+            dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
+            dw = torch.empty((v, h), device=x.device, dtype=x.dtype if whole else torch.float32) if ctx.needs_input_grad[1] else None
+            for r, end in chunks:
+                n, at = end - r, r if whole else 0
+                _logits(x[r:end], weight, z[:n])
+                _backward(z, n, v, v, tokens, ignore_index, temperature, top, tid, m, ls, ent, g, gh, gtop, dz[at:], v, r)
+                if not whole:
+                    if dx is not None:
+                        matmul_into(dz[:n], weight, dx[r:end])
+                    if dw is not None:
+                        matmul_into(dz[:n].t(), x[r:end], dw, accumulate=r > 0)
+            if whole and dx is not None:
+                gemm([dz], [weight], [dx], t, h, v, kmajor=(False, True))
+            if whole and dw is not None:
+                gemm([dz], [x], [dw], v, h, t, kmajor=(True, True))
+            if dw is not None:
+                dw = cast(dw, weight.dtype) if dw.dtype != weight.dtype else dw
+        return None if dx is None else dx.view(hidden.shape), dw, None, None, None, None
+
+
+def lm_head_logprobs(hidden, weight, tokens, *, top=0, temperature=1.0, ignore_index=IGNORE_INDEX):
+    """``token_logprobs`` of the logits ``hidden @ weight.T`` (hidden [..., H], weight [V, H], both fp32, bf16 or fp16), which
+    are formed in fp32 and never rounded; the gradient reaches hidden and weight."""
+    if hidden.ndim < 1 or weight.ndim != 2 or hidden.numel() < 1 or weight.numel() < 1 or hidden.shape[-1] != weight.shape[1]:
+        raise ValueError('nonempty hidden [..., H] and weight [V, H] required')
+    H.require_device(hidden, weight)
+    if hidden.dtype not in _FLOATS or weight.dtype != hidden.dtype:
+        raise TypeError(f'hidden and weight of one dtype, float32, bfloat16 or float16, required, not {hidden.dtype} and {weight.dtype}')
+    if not hidden.is_contiguous() or not weight.is_contiguous():
+        raise ValueError('contiguous hidden and weight required; no hidden layout copy')
+    _check_options(weight.shape[0], top, temperature, ignore_index)
+    _check_tokens(tokens, hidden.shape[:-1], hidden.device)
+    return TokenLogprobs(*_LMHeadLogprobs.apply(hidden, weight, tokens, ignore_index, float(temperature), top))
