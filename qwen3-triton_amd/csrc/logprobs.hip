@@ -11,9 +11,9 @@
 // -expm1(log p_i).
 //
 // Bound by the logits, read once (forward) or read and written once (backward).  A workgroup holds its slice of a row in
-// registers: the slice's maximum, then the sums, then the alternatives are taken from them.  Many rows take slices of 64 values a
+// registers: the slice's maximum, then the sums, then the alternatives are taken from them.  Many rows take slices of 32 values (fp32: 16) a
 // thread; few rows small ones, so that one row's latency is spread over many CUs.  A second launch joins a row's slices.
-#include <type_traits>
+#include <algorithm>
 
 #include "common.h"
 
@@ -21,90 +21,170 @@ namespace {
 
 constexpr int kThreads = 256;
 constexpr int kMaxTop = 32;
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kGradVectors = 4;  // 16-byte vectors of logits a thread
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 
-// Statistics of a part of a row.  m = -inf: nothing but -inf there (rest 0, or NaN where there is a NaN too).
+// Statistics of a part of a row: its maximum m, rest = the sum of e^d over all but one element that is m, and u = the sum of
+// e^d d, d counted from m in base 2.  m = -inf: nothing but -inf there (rest 0, or NaN where there is a NaN too).
 struct Part {
   float m, rest, u;
 };
 Q3_DEV float part_total(const Part& a) { return a.m == -INFINITY ? a.rest : 1.f + a.rest; }
-// c2 = c log2(e)
+// c2 = log2(e) / temperature
 Q3_DEV Part join(const Part& a, const Part& b, float c2) {
   const bool first = a.m >= b.m;
   const Part &hi = first ? a : b, &lo = first ? b : a;
   if (lo.m == -INFINITY) return Part{hi.m, hi.rest + lo.rest, hi.u};
-  const float d = lo.m - hi.m, w = __builtin_amdgcn_exp2f(d * c2), t = 1.f + lo.rest;
+  const float d = (lo.m - hi.m) * c2, w = __builtin_amdgcn_exp2f(d), t = 1.f + lo.rest;
   return Part{hi.m, fmaf(t, w, hi.rest), fmaf(w, fmaf(t, fmaxf(d, -1e30f), lo.u), hi.u)};
 }
 
+// Statistics of N values of a thread.  One element that is the maximum is taken out on the way to it (each step keeps the larger
+// and stores the smaller), in four chains.  d comes as fma(x, c2, -m c2): one rounding, and what the product m c2 lost to its own is
+// the same factor of every term.  Maxima and minima here hand NaN on.
+template <int N> Q3_DEV Part part_of(const float (&v)[N], float c2) {
+  static_assert(N % 4 == 0, "four chains");
+  float x[N], top[4];
+#pragma unroll
+  for (int k = 0; k < 4; ++k) {
+    top[k] = v[k];
+#pragma unroll
+    for (int i = k + 4; i < N; i += 4) {
+      x[i] = __builtin_elementwise_minimum(top[k], v[i]);
+      top[k] = __builtin_elementwise_maximum(top[k], v[i]);
+    }
+  }
+  Part p{top[0], 0.f, 0.f};
+#pragma unroll
+  for (int k = 1; k < 4; ++k) {
+    x[k] = __builtin_elementwise_minimum(p.m, top[k]);
+    p.m = __builtin_elementwise_maximum(p.m, top[k]);
+  }
+  const bool nan = p.m != p.m;
+  if (nan) p.m = -INFINITY;
+  if (__any(fabsf(p.m) > 1e30f && p.m != -INFINITY)) {  // m c2 might overflow (rows of the type's lowest value)
+    const float ref = p.m == -INFINITY ? 0.f : p.m;
+#pragma unroll
+    for (int i = 1; i < N; ++i) {
+      const float d = (x[i] - ref) * c2, e = __builtin_amdgcn_exp2f(d);
+      p.rest += e;
+      p.u = fmaf(e, fmaxf(d, -1e30f), p.u);
+    }
+  } else {
+    const float mc = p.m == -INFINITY ? 0.f : p.m * c2, lost = p.m == -INFINITY ? 0.f : fmaf(p.m, c2, -mc);
+    float rest[2] = {0.f, 0.f}, u[2] = {0.f, 0.f};
+#pragma unroll
+    for (int i = 1; i < N; ++i) {
+      const float d = fmaf(x[i], c2, -mc), e = __builtin_amdgcn_exp2f(d);
+      rest[i & 1] += e;
+      u[i & 1] = fmaf(e, fmaxf(d, -1e30f), u[i & 1]);
+    }
+    const float k = __builtin_amdgcn_exp2f(-lost), r = rest[0] + rest[1];
+    p.rest = r * k;
+    p.u = k * fmaf(-lost, r, u[0] + u[1]);
+  }
+  if (nan || p.m == INFINITY) p.rest = NAN;  // inf - inf
+  return p;
+}
+
 // ---------------------------------------------------------------- the largest k
-// Values as whole numbers in their order, NaN above all, the lower index first among equals.  A slice of 16-bit values fits
-// value and place into 32 bits; otherwise 64.
+// Values as whole numbers in their order, NaN above all, 0 below all; keys: the value's order, then the lower index first.
 Q3_DEV uint32_t order32(float x) {
   const uint32_t u = __float_as_uint(x + 0.f);  // -0 as +0
-  return x != x ? 0xffffffffu : (u & 0x80000000u) ? ~u : (u | 0x80000000u);
+  return x != x ? 0xffffffffu : u ^ ((uint32_t)((int)u >> 31) | 0x80000000u);
 }
-Q3_DEV float unorder32(uint32_t k) { return __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k); }
-template <typename T> Q3_DEV uint32_t order16(float x) {  // of a value of a 16-bit type
-  const uint32_t h = from_f32<T>(x + 0.f);
-  return x != x ? 0xffffu : (h & 0x8000u) ? (~h & 0xffffu) : (h | 0x8000u);
+Q3_DEV float unorder32(uint32_t k) {
+  return k == 0xffffffffu ? NAN : __uint_as_float((k & 0x80000000u) ? (k & 0x7fffffffu) : ~k);
 }
-Q3_DEV uint64_t key64(float x, uint32_t index) { return ((uint64_t)order32(x) << 32) | (uint32_t)~index; }
-
-template <typename K> Q3_DEV K shfl_key(K x, int mask) {
-  if constexpr (sizeof(K) == 4) return (K)__shfl_xor((int)x, mask, 64);
-  else return ((K)(uint32_t)__shfl_xor((int)(uint32_t)(x >> 32), mask, 64) << 32) | (uint32_t)__shfl_xor((int)(uint32_t)x, mask, 64);
+Q3_DEV uint64_t key_of(uint32_t order, uint32_t index) { return ((uint64_t)order << 32) | (uint32_t)~index; }
+Q3_DEV uint64_t key_xor(uint64_t x, int mask) {
+  return ((uint64_t)(uint32_t)__shfl_xor((int)(x >> 32), mask, 64) << 32) | (uint32_t)__shfl_xor((int)(uint32_t)x, mask, 64);
 }
 
-// The k largest of a workgroup's keys (all different; 0: none), in order, to emit(rank, key) by some thread each; ranks that no
-// key takes get 0.  `each(f)` calls f with every key of the calling thread.
-//  * The 64 maxima of groups of 4 threads: the k-th largest of those is a bound that at least k keys reach (k <= 64), and only
-//    keys of k groups do, so what passes it fits `cand` (k x 4 threads' keys), whatever the data.
-//  * What passes is ranked by counting the larger ones.
-template <typename K> struct TopScratch {
-  alignas(16) K group[64];
-  K bound;
+// The k largest (k <= kMaxTop) of a workgroup's values in order, to emit(rank, key) by some thread each; ranks that no value
+// takes get key 0.  most: the order of the thread's largest value (0: it has none); scan(f) calls f(order, index) for each of
+// its values, order 0 for none, and may read them again: few threads call it.
+//  * The 64 maxima of groups of 4 threads: the k-th largest of those is a bound that at least k values reach.  Of random
+//    values about 1.3 k do; they are collected and ranked by counting the larger ones.
+//  * More than kCand may reach it (ties, a row that rises, few values that are not -inf): then k rounds, each the largest key
+//    left, whose thread looks for its next one.
+constexpr int kCand = 2 * kThreads;
+struct TopScratch {
+  alignas(16) uint64_t cand[kCand];
+  alignas(16) uint32_t group[64];
+  uint64_t wave[kThreads / 64];
+  uint32_t bound;
   int count;
 };
-template <typename K, typename Each, typename Emit>
-Q3_DEV void block_top(TopScratch<K>& sc, K* cand, int k, Each&& each, Emit&& emit) {
+template <typename Scan, typename Emit>
+Q3_DEV void block_top(TopScratch& sc, int k, uint32_t most, Scan&& scan, Emit&& emit) {
   const int tid = threadIdx.x;
-  K best = 0;
-  each([&](K x) { best = x > best ? x : best; });
-  K g = best;
-#pragma unroll
-  for (int o = 1; o <= 2; o <<= 1) {
-    const K y = shfl_key(g, o);
-    g = y > g ? y : g;
-  }
+  uint32_t g = max(most, (uint32_t)__shfl_xor((int)most, 1, 64));
+  g = max(g, (uint32_t)__shfl_xor((int)g, 2, 64));
   if ((tid & 3) == 0) sc.group[tid >> 2] = g;
   if (tid == 0) sc.count = 0;
   __syncthreads();
   if (tid < 64) {
-    const K mine = sc.group[tid];
+    const uint32_t mine = sc.group[tid];
     int larger = 0;
-#pragma unroll 8
+#pragma unroll
     for (int i = 0; i < 64; ++i) {
-      const K o = sc.group[i];
-      larger += (o > mine || (o == mine && i < tid)) ? 1 : 0;  // equal ones are all 0: no key
+      const uint32_t o = sc.group[i];
+      larger += (o > mine || (o == mine && i < tid)) ? 1 : 0;
     }
     if (larger == k - 1) sc.bound = mine;
   }
   __syncthreads();
-  const K bound = sc.bound;
-  if (best >= bound && best != 0)
-    each([&](K x) {
-      if (x >= bound && x != 0) cand[atomicAdd(&sc.count, 1)] = x;
+  const uint32_t bound = sc.bound;
+  if (most >= bound && most != 0)
+    scan([&](uint32_t o, uint32_t i) {
+      if (o >= bound && o != 0) {
+        const int at = atomicAdd(&sc.count, 1);
+        if (at < kCand) sc.cand[at] = key_of(o, i);
+      }
     });
   __syncthreads();
   const int n = sc.count;
-  for (int i = tid; i < n; i += kThreads) {
-    const K mine = cand[i];
-    int larger = 0;
-    for (int j = 0; j < n; ++j) larger += cand[j] > mine ? 1 : 0;
-    if (larger < k) emit(larger, mine);
+  if (n <= kCand) {
+    for (int i = tid; i < n; i += kThreads) {
+      const uint64_t mine = sc.cand[i];
+      int larger = 0, j = 0;
+      for (; j + 16 <= n; j += 16)  // 16 reads in flight together
+#pragma unroll
+        for (int e = 0; e < 16; ++e) larger += sc.cand[j + e] > mine ? 1 : 0;
+#pragma unroll 4
+      for (; j < n; ++j) larger += sc.cand[j] > mine ? 1 : 0;
+      if (larger < k) emit(larger, mine);
+    }
+    if (tid >= n && tid < k) emit(tid, (uint64_t)0);
+    return;
   }
-  for (int r = n + tid; r < k; r += kThreads) emit(r, (K)0);
+  uint64_t best = 0, below = ~0ull;
+  for (int r = 0; r < k; ++r) {
+    if (most != 0 && (r == 0 || best == 0)) {  // look for the thread's largest key below its last one
+      scan([&](uint32_t o, uint32_t i) {
+        const uint64_t x = o ? key_of(o, i) : 0;
+        best = x > best && x < below ? x : best;
+      });
+      if (best == 0) most = 0;  // it has no more
+    }
+    uint64_t w = best;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+      const uint64_t y = key_xor(w, o);
+      w = y > w ? y : w;
+    }
+    __syncthreads();  // the last round's maxima are read
+    if ((tid & 63) == 0) sc.wave[tid >> 6] = w;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < kThreads / 64; ++i) w = sc.wave[i] > w ? sc.wave[i] : w;
+    if (w == 0 ? tid == 0 : w == best) {
+      emit(r, w);
+      below = best;
+      best = 0;
+    }
+  }
 }
 
 // ---------------------------------------------------------------- one slice of a row
@@ -114,73 +194,114 @@ struct Fwd {
   const int64_t* tok;
   int64_t ignore;
   float c;      // 1 / temperature
-  int top, slices;
-  Part* part;   // [rows][slices]
-  uint64_t* key;  // [rows][slices][top]
+  int top, slices, span, per, parts;  // slices of a row, their elements, slices of a workgroup, workgroups of a row
+  Part* part;   // [rows][parts]
+  uint64_t* key;  // [rows][parts][top]
   float *logprob, *entropy, *m, *ls;  // ls: log1p(rest)
   float* top_logprob;
   int64_t* top_token;
 };
 
-// 16 bytes from element i0 of a row of n on, whatever the row's alignment: i0 counts from a 16-byte boundary at or before the
-// row, so only a row's first and last vectors are not whole; elements outside the row are -inf.
-template <typename T> Q3_DEV Vec<T> load_edge(const typename T::storage* row, int64_t i0, int64_t n) {
-  if (i0 >= 0 && i0 + T::vec <= n) return load_vec<T>(row + i0);
-  Vec<T> v;
-#pragma unroll
-  for (int e = 0; e < T::vec; ++e) v.v[e] = i0 + e >= 0 && i0 + e < n ? to_f32<T>(row[i0 + e]) : -INFINITY;
-  return v;
-}
 // Elements between the 16-byte boundary before a row and its start.
 template <typename T> Q3_DEV int misaligned(const typename T::storage* row) {
   return (int)(((uintptr_t)row & 15) / sizeof(typename T::storage));
+}
+template <typename T> constexpr uint32_t kLowest = T::code == Q3_F32 ? 0xff800000u : T::code == Q3_F16 ? 0xfc00fc00u : 0xff80ff80u;
+
+// 16 bytes from element i0 of a row of n on: i0 counts from a 16-byte boundary at or before the row, so only a row's first and
+// last vectors are not whole; elements outside the row are -inf.
+template <typename T> Q3_DEV i32x4 load_edge(const typename T::storage* row, int64_t i0, int64_t n) {
+  if (i0 >= 0 && i0 + T::vec <= n) return *reinterpret_cast<const i32x4*>(row + i0);
+  i32x4 v;
+#pragma unroll
+  for (int w = 0; w < 4; ++w) {
+    uint32_t x = kLowest<T>;
+    if constexpr (T::vec == 4) {
+      if (i0 + w >= 0 && i0 + w < n) x = __float_as_uint(row[i0 + w]);
+    } else {
+#pragma unroll
+      for (int e = 0; e < 2; ++e) {
+        const int64_t i = i0 + 2 * w + e;
+        if (i >= 0 && i < n) x = (x & ~(0xffffu << (16 * e))) | ((uint32_t)row[i] << (16 * e));
+      }
+    }
+    v[w] = (int)x;
+  }
+  return v;
+}
+// C vectors a thread of the slice that starts at element `base`, 256 threads side by side.
+template <typename T, int C> Q3_DEV void load_slice(i32x4 (&v)[C], const typename T::storage* row, int64_t base, int64_t n) {
+  constexpr int V = T::vec;
+  if (base >= 0 && base + kThreads * V * C <= n) {
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i] = *reinterpret_cast<const i32x4*>(row + base + (i * kThreads + (int)threadIdx.x) * V);
+  } else {
+#pragma unroll
+    for (int i = 0; i < C; ++i) v[i] = load_edge<T>(row, base + (i * kThreads + (int)threadIdx.x) * V, n);
+  }
+}
+template <typename T, int C> Q3_DEV void unpack(float (&x)[C * T::vec], const i32x4 (&v)[C]) {
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    const Vec<T> f = unpack_vec<T>(v[i]);
+#pragma unroll
+    for (int e = 0; e < T::vec; ++e) x[i * T::vec + e] = f.v[e];
+  }
 }
 
 template <typename T, int C, bool TOP>
 __global__ __launch_bounds__(kThreads) void slice_kernel(Fwd a) {
   typedef typename T::storage S;
-  constexpr int V = T::vec, N = kThreads * V * C;
-  typedef typename std::conditional<V == 8, uint32_t, uint64_t>::type K;
-  const int64_t r = blockIdx.x / a.slices;
-  const int sl = (int)(blockIdx.x - r * a.slices), tid = threadIdx.x;
+  constexpr int V = T::vec;
+  const int N = a.span;
+  const int64_t r = blockIdx.x / (unsigned)a.parts;
+  const int part = (int)(blockIdx.x - (unsigned)(r * a.parts)), tid = threadIdx.x;
   if (a.tok[r] == a.ignore) return;  // the whole workgroup: nothing of the row is read
   const S* row = (const S*)a.z + r * a.ld;
-  const int64_t base = (int64_t)sl * N - misaligned<T>(row);
-  Vec<T> x[C];
-#pragma unroll
-  for (int i = 0; i < C; ++i) x[i] = load_edge<T>(row, base + (int64_t)(i * kThreads + tid) * V, a.vocab);
-
-  Part p{-INFINITY, 0.f, 0.f};
-#pragma unroll
-  for (int i = 0; i < C; ++i)
-#pragma unroll
-    for (int e = 0; e < V; ++e) p.m = fmaxf(p.m, x[i].v[e]);
+  const int mis = misaligned<T>(row);
   const float c2 = a.c * kLog2e;
-  {
-    const float ref = p.m == -INFINITY ? 0.f : p.m;  // only -inf (e^d = 0) and NaN then
-    int same = 0;
+  const int first = part * a.per, last = min(first + a.per, a.slices);
+  Part p{-INFINITY, 0.f, 0.f};
+  i32x4 raw[C];
+  auto load = [&](int sl) {
+    const int64_t base = (int64_t)sl * N - mis;
+    load_slice<T, C>(raw, row, base, min(a.vocab, base + N));
+  };
+  load(first);
+  for (int sl = first; sl < last; ++sl) {
+    float x[C * V];
+    unpack<T, C>(x, raw);
+    if (sl + 1 < last) load(sl + 1);  // in flight meanwhile
+    const Part q = part_of(x, c2);
+    p = sl == first ? q : join(p, q, c2);
+  }
+  if constexpr (TOP) {
+    __shared__ TopScratch sc;
+    uint64_t* out = a.key + (r * a.parts + part) * a.top;
+    const int64_t begin = (int64_t)first * N - mis + tid * V;  // of the thread's first vector
+    const bool any = begin < a.vocab && begin + V > 0 && tid * V < N;
+    const uint32_t most = !any ? 0 : p.rest != p.rest ? order32(NAN) : order32(p.m);
+    block_top(sc, a.top, most, [&](auto&& f) {
+      for (int sl = last - 1; sl >= first; --sl) {
+        if (last - first > 1) load(sl);
+        float x[C * V];
+        unpack<T, C>(x, raw);
 #pragma unroll
-    for (int i = 0; i < C; ++i)
-#pragma unroll
-      for (int e = 0; e < V; ++e) {
-        const float d = x[i].v[e] - ref;
-        const bool top = d == 0.f;
-        const float w = top ? 0.f : __builtin_amdgcn_exp2f(d * c2);
-        same += top ? 1 : 0;
-        p.rest += w;
-        p.u = fmaf(w, fmaxf(d, -1e30f), p.u);
+        for (int i = 0; i < C * V; ++i) {
+          const int at = (i / V * kThreads + tid) * V + i % V;
+          const int64_t j = (int64_t)sl * N - mis + at;
+          f(j >= 0 && j < a.vocab && at < N ? order32(x[i]) : 0, (uint32_t)j);
+        }
       }
-    if (p.m != -INFINITY) p.rest += (float)(same - 1);
-    if (p.m == INFINITY) p.rest = NAN;  // inf - inf
+    }, [&](int rank, uint64_t k) { out[rank] = k; });
   }
   // over the wave: one lane that holds the maximum gives its rest, the others their totals
   const float wm = group_max<64>(p.m);
   {
     const uint64_t at = __ballot(p.m == wm);
     const bool one = (threadIdx.x & 63) == (unsigned)__builtin_ctzll(at | (1ull << 63));
-    const float d = p.m - wm, w = p.m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(d * c2);
-    const float t = one ? p.rest : part_total(p);
-    const float full = part_total(p);
+    const float d = (p.m - wm) * c2, w = p.m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(d);
+    const float full = part_total(p), t = one ? p.rest : full;
     p.u = group_sum<64>(p.m == -INFINITY ? 0.f : w * fmaf(full, fmaxf(d, -1e30f), p.u));
     p.rest = group_sum<64>(t * w);
     p.m = wm;
@@ -192,38 +313,7 @@ __global__ __launch_bounds__(kThreads) void slice_kernel(Fwd a) {
     p = wave_part[0];
 #pragma unroll
     for (int w = 1; w < kThreads / 64; ++w) p = join(p, wave_part[w], c2);
-    a.part[r * a.slices + sl] = p;
-  }
-  if constexpr (TOP) {
-    __shared__ TopScratch<K> sc;
-    extern __shared__ uint64_t cand_mem[];  // top x 4 threads' keys
-    K* cand = (K*)cand_mem;
-    uint64_t* out = a.key + (r * a.slices + sl) * a.top;
-    auto each = [&](auto&& f) {
-#pragma unroll
-      for (int i = 0; i < C; ++i) {
-        const int at = (i * kThreads + tid) * V;
-#pragma unroll
-        for (int e = 0; e < V; ++e) {
-          const int64_t j = base + at + e;
-          const bool in = j >= 0 && j < a.vocab;
-          if constexpr (V == 8) {
-            const uint32_t k = (order16<T>(x[i].v[e]) << 16) | (uint32_t)(0xffff - (at + e));
-            f(in ? k : 0u);
-          } else {
-            f(in ? key64(x[i].v[e], (uint32_t)j) : (uint64_t)0);
-          }
-        }
-      }
-    };
-    block_top<K>(sc, cand, a.top, each, [&](int rank, K k) {
-      if constexpr (V == 8) {
-        const int64_t j = base + (0xffff - (int)(k & 0xffffu));
-        out[rank] = k == 0 ? 0 : key64(to_f32<T>(row[j]), (uint32_t)j);
-      } else {
-        out[rank] = k;
-      }
-    });
+    a.part[r * a.parts + part] = p;
   }
 }
 
@@ -232,7 +322,7 @@ Q3_DEV void finish_row(const Fwd& a, int64_t r, const Part& p, float picked, boo
   const float ls = log1pf(p.rest), d = picked - p.m;
   const bool none = p.m == -INFINITY;
   a.logprob[r] = valid ? fmaf(d, a.c, -ls) : NAN;
-  a.entropy[r] = none ? NAN : fmaf(-a.c, p.u / (1.f + p.rest), ls);
+  a.entropy[r] = none ? NAN : fmaf(-kLn2, p.u / (1.f + p.rest), ls);
   a.m[r] = p.m;
   a.ls[r] = none ? NAN : ls;
 }
@@ -255,7 +345,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void finish_kernel(
   const float picked = valid ? to_f32<T>(((const typename T::storage*)a.z)[r * a.ld + t]) : 0.f;
   const float c2 = a.c * kLog2e;
   Part p{-INFINITY, 0.f, 0.f};
-  for (int i = lane; i < a.slices; i += 64) p = join(p, a.part[r * a.slices + i], c2);
+  for (int i = lane; i < a.parts; i += 64) p = join(p, a.part[r * a.parts + i], c2);
 #pragma unroll
   for (int o = 1; o < 64; o <<= 1)
     p = join(p, Part{__shfl_xor(p.m, o, 64), __shfl_xor(p.rest, o, 64), __shfl_xor(p.u, o, 64)}, c2);
@@ -264,13 +354,18 @@ template <typename T> __global__ __launch_bounds__(kThreads) void finish_kernel(
 
 // One workgroup a row: the alternatives are the largest of its slices' largest.
 template <typename T> __global__ __launch_bounds__(kThreads) void finish_top_kernel(Fwd a) {
-  __shared__ TopScratch<uint64_t> sc;
-  extern __shared__ uint64_t cand_mem[];
-  uint64_t* cand = cand_mem;
+  __shared__ TopScratch sc;
   __shared__ Part row_part;
+  constexpr int R = 8;  // keys of a thread in registers
   const int64_t r = blockIdx.x;
-  const int tid = threadIdx.x;
+  const int tid = threadIdx.x, n = a.parts * a.top;
   const int64_t t = a.tok[r];
+  const uint64_t* key = a.key + r * n;
+  uint64_t mine[R];
+  if (t != a.ignore) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) mine[i] = tid + i * kThreads < n ? key[tid + i * kThreads] : 0;
+  }
   if (t == a.ignore) {
     if (tid == 0) left_out(a, r);
     if (tid < a.top) {
@@ -284,7 +379,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void finish_top_ker
     const float picked = valid ? to_f32<T>(((const typename T::storage*)a.z)[r * a.ld + t]) : 0.f;
     const float c2 = a.c * kLog2e;
     Part p{-INFINITY, 0.f, 0.f};
-    for (int i = tid; i < a.slices; i += 64) p = join(p, a.part[r * a.slices + i], c2);
+    for (int i = tid; i < a.parts; i += 64) p = join(p, a.part[r * a.parts + i], c2);
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1)
       p = join(p, Part{__shfl_xor(p.m, o, 64), __shfl_xor(p.rest, o, 64), __shfl_xor(p.u, o, 64)}, c2);
@@ -293,14 +388,17 @@ template <typename T> __global__ __launch_bounds__(kThreads) void finish_top_ker
       row_part = p;
     }
   }
-  const uint64_t* key = a.key + r * a.slices * a.top;
-  const int n = a.slices * a.top;
-  block_top<uint64_t>(sc, cand, a.top, [&](auto&& f) {
-    for (int i = tid; i < n; i += kThreads) f(key[i]);
+  uint32_t most = 0;
+#pragma unroll
+  for (int i = 0; i < R; ++i) most = max(most, (uint32_t)(mine[i] >> 32));
+  for (int i = tid + R * kThreads; i < n; i += kThreads) most = max(most, (uint32_t)(key[i] >> 32));
+  block_top(sc, a.top, most, [&](auto&& f) {
+#pragma unroll
+    for (int i = 0; i < R; ++i) f((uint32_t)(mine[i] >> 32), ~(uint32_t)mine[i]);
+    for (int i = tid + R * kThreads; i < n; i += kThreads) f((uint32_t)(key[i] >> 32), ~(uint32_t)key[i]);
   }, [&](int rank, uint64_t k) {  // behind barriers: row_part is there
     a.top_token[r * a.top + rank] = (int64_t)(uint32_t)~(uint32_t)k;
-    const uint32_t o = (uint32_t)(k >> 32);
-    const float x = o == 0xffffffffu ? NAN : unorder32(o);
+    const float x = unorder32((uint32_t)(k >> 32));
     a.top_logprob[r * a.top + rank] = row_part.m == -INFINITY ? NAN : fmaf(x - row_part.m, a.c, -log1pf(row_part.rest));
   });
 }
@@ -332,30 +430,40 @@ struct Bwd {
   int64_t ldo;
 };
 
-// 16 values a thread, in vectors of 16 bytes of logits.  Rows left out are zeros, and nothing of them is read.
+// 32 (fp32: 16) values a thread.  Rows left out are zeros, and nothing of them is read.
 template <typename T, typename O> __global__ __launch_bounds__(kThreads) void grad_kernel(Bwd a, int slices) {
   typedef typename T::storage S;
   typedef typename O::storage SO;
-  constexpr int V = T::vec, C = 16 / V;
-  const int64_t r = blockIdx.x / slices;
-  const int sl = (int)(blockIdx.x - r * slices), tid = threadIdx.x;
+  constexpr int V = T::vec, C = kGradVectors, N = kThreads * V * C;
+  const int64_t r = blockIdx.x / (unsigned)slices;
+  const int sl = (int)(blockIdx.x - (unsigned)(r * slices)), tid = threadIdx.x;
   const int64_t t = a.tok[r];
   const bool live = t != a.ignore;
   const S* row = (const S*)a.z + r * a.ld;
   SO* out = (SO*)a.dz + r * a.ldo;
   const int mis = (int)(((uintptr_t)out & (V * sizeof(SO) - 1)) / sizeof(SO));
-  const bool same = misaligned<T>(row) == mis;
-  const int64_t base = (int64_t)sl * (kThreads * V * C) - mis;
-  Vec<T> x[C];
+  const int64_t base = (int64_t)sl * N - mis;
+  const bool whole = base >= 0 && base + N <= a.vocab;
+  i32x4 raw[C];
   if (live) {
+    if (misaligned<T>(row) == mis) {
+      load_slice<T, C>(raw, row, base, a.vocab);
+    } else {  // the gradient's rows begin elsewhere between 16-byte boundaries
 #pragma unroll
-    for (int i = 0; i < C; ++i) {
-      const int64_t i0 = base + (int64_t)(i * kThreads + tid) * V;
-      if (same) {
-        x[i] = load_edge<T>(row, i0, a.vocab);
-      } else {
+      for (int i = 0; i < C; ++i) {
+        const int64_t i0 = base + (i * kThreads + tid) * V;
 #pragma unroll
-        for (int e = 0; e < V; ++e) x[i].v[e] = i0 + e >= 0 && i0 + e < a.vocab ? to_f32<T>(row[i0 + e]) : -INFINITY;
+        for (int w = 0; w < 4; ++w) {
+          uint32_t x = kLowest<T>;
+#pragma unroll
+          for (int e = 0; e < V / 4; ++e) {
+            const int64_t j = i0 + w * (V / 4) + e;
+            if (j < 0 || j >= a.vocab) continue;
+            if constexpr (V == 4) x = __float_as_uint(row[j]);
+            else x = (x & ~(0xffffu << (16 * e))) | ((uint32_t)row[j] << (16 * e));
+          }
+          raw[i][w] = (int)x;
+        }
       }
     }
   }
@@ -373,16 +481,17 @@ template <typename T, typename O> __global__ __launch_bounds__(kThreads) void gr
   const float c2 = a.c * kLog2e, l2 = ls * kLog2e;
 #pragma unroll
   for (int i = 0; i < C; ++i) {
-    const int64_t i0 = base + (int64_t)(i * kThreads + tid) * V;
-    if (i0 + V <= 0 || i0 >= a.vocab) continue;
-    struct { float v[V]; } o;
+    const int64_t i0 = base + (i * kThreads + tid) * V;
+    float o[V];
     if (live) {
+      const Vec<T> x = unpack_vec<T>(raw[i]);
+      // -c p (all + h (log p + entropy)), log p = d c - ls
 #pragma unroll
       for (int e = 0; e < V; ++e) {
-        const float d = x[i].v[e] - m;
+        const float d = x.v[e] - m;
         const float p = __builtin_amdgcn_exp2f(fmaf(d, c2, -l2));
         const float lp = fmaxf(fmaf(d, a.c, -ls), -1e30f);
-        o.v[e] = -a.c * p * fmaf(gh, lp + ent, all);
+        o[e] = -a.c * p * fmaf(gh, lp + ent, all);
       }
       // the given token, and the alternatives
       for (int j = -1; j < (a.gtop ? a.top : 0); ++j) {
@@ -394,20 +503,20 @@ template <typename T, typename O> __global__ __launch_bounds__(kThreads) void gr
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           if (e != at) continue;
-          const float lp = fmaf(x[i].v[e] - m, a.c, -ls), p = __builtin_amdgcn_exp2f(fmaf(x[i].v[e] - m, c2, -l2));
-          o.v[e] = a.c * (-expm1f(lp) * mine - p * fmaf(gh, fmaxf(lp, -1e30f) + ent, all - mine));
+          const float lp = fmaf(x.v[e] - m, a.c, -ls), p = __builtin_amdgcn_exp2f(fmaf(x.v[e] - m, c2, -l2));
+          o[e] = a.c * (-expm1f(lp) * mine - p * fmaf(gh, fmaxf(lp, -1e30f) + ent, all - mine));
         }
       }
     } else {
 #pragma unroll
-      for (int e = 0; e < V; ++e) o.v[e] = 0.f;
+      for (int e = 0; e < V; ++e) o[e] = 0.f;
     }
-    if (i0 >= 0 && i0 + V <= a.vocab) {
-      store_values<O, V>(out + i0, o.v);
+    if (whole || (i0 >= 0 && i0 + V <= a.vocab)) {
+      store_values<O, V>(out + i0, o);
     } else {
 #pragma unroll
       for (int e = 0; e < V; ++e)
-        if (i0 + e >= 0 && i0 + e < a.vocab) out[i0 + e] = from_f32<O>(o.v[e]);
+        if (i0 + e >= 0 && i0 + e < a.vocab) out[i0 + e] = from_f32<O>(o[e]);
     }
   }
 }
@@ -417,9 +526,9 @@ bool dtype_ok(int dt) { return dt == Q3_F32 || dt == Q3_F16 || dt == Q3_BF16; }
 int vec_of(int dtype) { return dtype == Q3_F32 ? 4 : 8; }
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Vectors of a slice per thread: 8 where that leaves enough workgroups for the chip (or a row has very many values), else 1.
+// Vectors of a slice per thread: 4 where that leaves enough workgroups for the chip (or a row has very many values), else 1.
 int chunks_for(int dtype, int64_t rows, int64_t vocab) {
-  return vocab > (1 << 18) || rows * cdiv(vocab, (int64_t)kThreads * vec_of(dtype) * 8) >= 1024 ? 8 : 1;
+  return vocab > (1 << 18) || rows * cdiv(vocab, (int64_t)kThreads * vec_of(dtype) * 4) >= 1024 ? 4 : 1;
 }
 // A row may start up to a vector before its first element's boundary.
 int64_t slices_for(int dtype, int64_t rows, int64_t vocab) {
@@ -427,26 +536,29 @@ int64_t slices_for(int dtype, int64_t rows, int64_t vocab) {
 }
 bool sizes_ok(int dtype, int64_t rows, int64_t vocab, int64_t top) {
   if (!dtype_ok(dtype) || rows < 1 || vocab < 1 || vocab >= (1ll << 30) || top < 0 || top > kMaxTop || top > vocab) return false;
-  if (rows >= (1ll << 31) || (top > 0 && vocab > (1 << 21))) return false;
+  if (rows >= (1ll << 31)) return false;
   return rows * cdiv(vocab + 16, kThreads * vec_of(dtype)) < (1ll << 31) - 1;
 }
 
+// Slices of a workgroup: as many as leave 4096 workgroups; where alternatives are wanted at most 6, so that what is read again for
+// them is still in a cache.
+int per_for(int64_t rows, int64_t slices, int64_t top) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>(top > 0 ? std::min<int64_t>(slices, 6) : slices, rows * slices / 4096));
+}
+
 template <typename T, int C> void slices(const Fwd& a, hipStream_t s) {
-  const unsigned n = (unsigned)(a.rows * a.slices);
-  const size_t lds = (size_t)a.top * 4 * C * T::vec * (T::vec == 8 ? 4 : 8);
-  if (a.top) slice_kernel<T, C, true><<<n, kThreads, lds, s>>>(a);
+  const unsigned n = (unsigned)(a.rows * a.parts);
+  if (a.top) slice_kernel<T, C, true><<<n, kThreads, 0, s>>>(a);
   else slice_kernel<T, C, false><<<n, kThreads, 0, s>>>(a);
 }
 
 template <typename T> int forward(const Fwd& a, int chunks, hipStream_t s) {
-  if (chunks == 8) slices<T, 8>(a, s);
+  if (chunks == 4) slices<T, 4>(a, s);
   else slices<T, 1>(a, s);
   const int rc = (int)hipGetLastError();
   if (rc != 0) return rc;
   if (a.top) {
-    // a thread of the joining workgroup takes its share of the slices' keys: at most 64 of them (2^21 values of 8192 a slice)
-    const size_t lds = (size_t)a.top * 4 * (size_t)cdiv((int64_t)a.slices * a.top, kThreads) * sizeof(uint64_t);
-    finish_top_kernel<T><<<(unsigned)a.rows, kThreads, lds, s>>>(a);
+    finish_top_kernel<T><<<(unsigned)a.rows, kThreads, 0, s>>>(a);
   } else {
     finish_kernel<T><<<(unsigned)cdiv(a.rows, kThreads / 64), kThreads, 0, s>>>(a);
   }
@@ -454,7 +566,7 @@ template <typename T> int forward(const Fwd& a, int chunks, hipStream_t s) {
 }
 
 template <typename T, typename O> int backward(const Bwd& a, hipStream_t s) {
-  const int64_t n = cdiv(a.vocab + T::vec - 1, kThreads * 16);
+  const int64_t n = cdiv(a.vocab + T::vec - 1, (int64_t)kThreads * T::vec * kGradVectors);
   grad_kernel<T, O><<<(unsigned)(a.rows * n), kThreads, 0, s>>>(a, (int)n);
   return (int)hipGetLastError();
 }
@@ -477,10 +589,13 @@ int q3_token_logprobs(int dtype, const void* z, int64_t ld, int64_t rows, int64_
   Q3_REQUIRE((top == 0 || (top_logprob && top_token)) && inv_temperature > 0.f && inv_temperature < INFINITY);
   Q3_REQUIRE(((uintptr_t)z & (dtype == Q3_F32 ? 3 : 1)) == 0 && workspace && ((uintptr_t)workspace & 15) == 0 &&
              workspace_bytes >= q3_token_logprobs_workspace_bytes(dtype, rows, vocab, top));
-  Fwd a{z, ld, rows, vocab, tokens, ignore_index, inv_temperature, (int)top, (int)slices_for(dtype, rows, vocab),
+  const int n = (int)slices_for(dtype, rows, vocab), per = per_for(rows, n, top), c = chunks_for(dtype, rows, vocab), v = vec_of(dtype);
+  // one vector a thread: slices of a size (a short last one would have many candidates for its alternatives: T = 1, top 20
+  // 19 -> 9 us)
+  const int span = c == 1 ? (int)cdiv(cdiv(vocab + v - 1, v), n) * v : kThreads * v * c;
+  Fwd a{z, ld, rows, vocab, tokens, ignore_index, inv_temperature, (int)top, n, span, per, (int)cdiv(n, per),
         (Part*)workspace, nullptr, logprob, entropy, row_max, row_log, top_logprob, top_token};
-  a.key = (uint64_t*)((char*)workspace + ((size_t)rows * a.slices * sizeof(Part) + 7) / 8 * 8);
-  const int c = chunks_for(dtype, rows, vocab);
+  a.key = (uint64_t*)((char*)workspace + ((size_t)rows * n * sizeof(Part) + 7) / 8 * 8);
   if (dtype == Q3_BF16) return forward<BF16>(a, c, stream);
   if (dtype == Q3_F16) return forward<F16>(a, c, stream);
   return forward<F32>(a, c, stream);

@@ -8,6 +8,7 @@ an argmax only; nothing here has a counterpart in it.
 from typing import NamedTuple, Optional
 
 import torch
+import torch.autograd.forward_ad as _forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import _hip as H
@@ -31,16 +32,16 @@ class TokenLogprobs(NamedTuple):
 def _check_options(vocab, top, temperature, ignore_index):
     if type(top) is not int or not 0 <= top <= min(MAX_TOP, vocab):
         raise ValueError(f'top must be an int in [0, {min(MAX_TOP, vocab)}]')
-    if vocab >= 1 << 30 or (top and vocab > 1 << 21):
-        raise ValueError('fewer than 2^30 tokens, with top at most 2^21, required')
-    if not 1e-6 <= float(temperature) <= 1e6:
+    if vocab >= 1 << 30:
+        raise ValueError('fewer than 2^30 tokens required')
+    if not 1e-6 <= temperature <= 1e6:
         raise ValueError('a temperature in [1e-6, 1e6] required')
     if type(ignore_index) is not int:
         raise ValueError('ignore_index must be an int')
 
 
-def _check_tokens(tokens, shape, device):
-    if tokens.dtype != torch.int64 or tokens.shape != shape or tokens.device != device or not tokens.is_contiguous():
+def _check_tokens(tokens, shape, ref):
+    if tokens.dtype != torch.int64 or tokens.shape != shape or tokens.get_device() != ref.get_device() or not tokens.is_contiguous():
         raise ValueError(f'contiguous int64 tokens {tuple(shape)} on the same device required')
 
 
@@ -59,34 +60,43 @@ def _logit_rows(logits):
     return rows, m.stride(0) if rows > 1 else v, v
 
 
-def _forward(z, rows, ld, v, tokens, ignore_index, temperature, top, outs=None, at=0):
-    """q3_token_logprobs of rows of z; into rows ``at`` .. of ``outs`` where those are given."""
+def _forward(z, rows, ld, v, tokens, ignore_index, temperature, top, keep, outs=None, at=0):
+    """q3_token_logprobs of rows of z -> (log probability, entropy, alternatives' log probabilities, their tokens, [row maximum, row
+    log] where ``keep`` says that a gradient needs them); into rows ``at`` .. of ``outs`` where those are given."""
     if outs is None:
-        outs = _outputs(z, rows, top)
-    lp, ent, m, ls, tlp, tid = (None if t is None else t[at:] for t in outs)
+        outs = _outputs(z, rows, top, keep)
+    lp, ent, tlp, tid, kept = outs
     nbytes = H.query("q3_token_logprobs_workspace_bytes", H.code(z.dtype), rows, v, top)
-    ws = H.workspace(nbytes, z.device)
+    ws = H.workspace(nbytes + (0 if kept is not None else 8 * rows), z.device)
+    w = ws.data_ptr()
+    m, ls = (w + nbytes, w + nbytes + 4 * rows) if kept is None else (kept.data_ptr() + 4 * at, kept.data_ptr() + 4 * (kept.shape[1] + at))
     H.launch(z, "q3_token_logprobs", H.code(z.dtype), z.data_ptr(), ld, rows, v, tokens.data_ptr() + 8 * at, ignore_index,
-             1.0 / float(temperature), top, lp.data_ptr(), ent.data_ptr(), m.data_ptr(), ls.data_ptr(),
-             None if tlp is None else tlp.data_ptr(), None if tid is None else tid.data_ptr(), ws.data_ptr(), nbytes)
+             1.0 / temperature, top, lp.data_ptr() + 4 * at, ent.data_ptr() + 4 * at, m, ls,
+             None if tlp is None else tlp.data_ptr() + 4 * top * at, None if tid is None else tid.data_ptr() + 8 * top * at, w, nbytes)
     return outs
 
 
-def _outputs(ref, rows, top):
-    """(log probability, entropy, row maximum, row log, alternatives' log probabilities, their tokens)"""
-    f = dict(device=ref.device, dtype=torch.float32)
-    outs = torch.empty(rows, **f), torch.empty(rows, **f), *torch.empty((2, rows), **f).unbind(0)
-    if not top:
-        return (*outs, None, None)
-    return (*outs, torch.empty((rows, top), **f), torch.empty((rows, top), device=ref.device, dtype=torch.int64))
+def _outputs(ref, rows, top, keep):
+    f = torch.float32
+    return (ref.new_empty(rows, dtype=f), ref.new_empty(rows, dtype=f), ref.new_empty((rows, top), dtype=f) if top else None,
+            ref.new_empty((rows, top), dtype=torch.int64) if top else None, ref.new_empty((2, rows), dtype=f) if keep else None)
 
 
-def _backward(z, rows, ld, v, tokens, ignore_index, temperature, top, top_tokens, m, ls, ent, g, gh, gtop, dz, ldo, at=0):
+def _shaped(shape, top, lp, ent, tlp, tid, _=None):
+    """The results for tokens of ``shape``."""
+    if len(shape) != 1:
+        lp, ent = lp.view(shape), ent.view(shape)
+        if top:
+            tlp, tid = tlp.view(*shape, top), tid.view(*shape, top)
+    return lp, ent, tlp, tid
+
+
+def _backward(z, rows, ld, v, tokens, ignore_index, temperature, top, top_tokens, kept, ent, g, gh, gtop, dz, ldo, at=0):
     """q3_token_logprobs_bwd of rows ``at`` .. ``at`` + rows - 1 (z and dz start there)."""
     def p(t, width=4):
         return None if t is None else t.data_ptr() + at * width
     H.launch(z, "q3_token_logprobs_bwd", H.code(z.dtype), H.code(dz.dtype), z.data_ptr(), ld, rows, v, p(tokens, 8), ignore_index,
-             1.0 / float(temperature), top, p(top_tokens, 8 * top), p(m), p(ls), p(ent), p(g), p(gh), p(gtop, 4 * top),
+             1.0 / temperature, top, p(top_tokens, 8 * top), p(kept), p(kept[1]), p(ent), p(g), p(gh), p(gtop, 4 * top),
              dz.data_ptr(), ldo)
 
 
@@ -98,27 +108,31 @@ class _TokenLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, logits, tokens, ignore_index, temperature, top):
         rows, ld, v = _logit_rows(logits)
-        lp, ent, m, ls, tlp, tid = _forward(logits, rows, ld, v, tokens, ignore_index, temperature, top)
-        shape = logits.shape[:-1]
-        ctx.save_for_backward(logits, tokens, m, ls, ent, tid)
+        outs = _forward(logits, rows, ld, v, tokens, ignore_index, temperature, top, True)
+        ctx.save_for_backward(logits, tokens, outs[4], outs[1], outs[3])
         ctx.rest = ignore_index, temperature, top
         ctx.set_materialize_grads(False)
+        lp, ent, tlp, tid = _shaped(logits.shape[:-1], top, *outs)
         if not top:
-            return lp.view(shape), ent.view(shape)
-        tid = tid.view(*shape, top)
+            return lp, ent
         ctx.mark_non_differentiable(tid)
-        return lp.view(shape), ent.view(shape), tlp.view(*shape, top), tid
+        return lp, ent, tlp, tid
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g, gh, gtop=None, _=None):
-        logits, tokens, m, ls, ent, tid = ctx.saved_tensors
+        logits, tokens, kept, ent, tid = ctx.saved_tensors
         ignore_index, temperature, top = ctx.rest
         rows, ld, v = _logit_rows(logits)
         dz = torch.empty(logits.shape, device=logits.device, dtype=logits.dtype)
-        _backward(logits, rows, ld, v, tokens, ignore_index, temperature, top, tid, m, ls, ent, _upstream(g), _upstream(gh),
+        _backward(logits, rows, ld, v, tokens, ignore_index, temperature, top, tid, kept, ent, _upstream(g), _upstream(gh),
                   _upstream(gtop), dz, v)
         return dz, None, None, None, None
+
+
+def _recorded(*tensors):
+    """Whether autograd has to see a call on these (a forward-mode tangent has to, to be refused)."""
+    return torch.is_grad_enabled() and any(t.requires_grad for t in tensors) or _forward_ad._current_level >= 0
 
 
 def token_logprobs(logits, tokens, *, top=0, temperature=1.0, ignore_index=IGNORE_INDEX):
@@ -134,10 +148,13 @@ def token_logprobs(logits, tokens, *, top=0, temperature=1.0, ignore_index=IGNOR
     H.require_device(logits)
     if logits.dtype not in _FLOATS:
         raise TypeError(f'float32, bfloat16 or float16 logits required, not {logits.dtype}')
+    shape, temperature = logits.shape[:-1], float(temperature)
     _check_options(logits.shape[-1], top, temperature, ignore_index)
-    _check_tokens(tokens, logits.shape[:-1], logits.device)
-    _logit_rows(logits)
-    return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, ignore_index, float(temperature), top))
+    _check_tokens(tokens, shape, logits)
+    rows, ld, v = _logit_rows(logits)
+    if _recorded(logits):
+        return TokenLogprobs(*_TokenLogprobs.apply(logits, tokens, ignore_index, temperature, top))
+    return TokenLogprobs(*_shaped(shape, top, *_forward(logits, rows, ld, v, tokens, ignore_index, temperature, top, False)))
 
 
 # ---------------------------------------------------------------- from hidden states
@@ -158,34 +175,35 @@ def _logits(x, w, z):
         matmul_into(x, w.t(), z)
 
 
+def _head_forward(x, weight, tokens, ignore_index, temperature, top, keep):
+    t, v = x.shape[0], weight.shape[0]
+    with torch.cuda.device(x.device):
+        outs = _outputs(x, t, top, keep)
+        chunks = _chunks(t, v)
+        z = torch.empty((chunks[0][1], v), device=x.device, dtype=torch.float32)
+        for r, end in chunks:
+            _logits(x[r:end], weight, z[:end - r])
+            _forward(z, end - r, v, v, tokens, ignore_index, temperature, top, keep, outs, r)
+    return outs
+
+
 class _LMHeadLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, tokens, ignore_index, temperature, top):
-        v, h = weight.shape
-        x = hidden.view(-1, h)
-        t = x.shape[0]
-        with torch.cuda.device(x.device):
-            outs = _outputs(x, t, top)
-            chunks = _chunks(t, v)
-            z = torch.empty((chunks[0][1], v), device=x.device, dtype=torch.float32)
-            for r, end in chunks:
-                _logits(x[r:end], weight, z[:end - r])
-                _forward(z, end - r, v, v, tokens, ignore_index, temperature, top, outs, r)
-        lp, ent, m, ls, tlp, tid = outs
-        shape = hidden.shape[:-1]
-        ctx.save_for_backward(hidden, weight, tokens, m, ls, ent, tid)
+        outs = _head_forward(hidden.view(-1, weight.shape[1]), weight, tokens, ignore_index, temperature, top, True)
+        ctx.save_for_backward(hidden, weight, tokens, outs[4], outs[1], outs[3])
         ctx.rest = ignore_index, temperature, top
         ctx.set_materialize_grads(False)
+        lp, ent, tlp, tid = _shaped(hidden.shape[:-1], top, *outs)
         if not top:
-            return lp.view(shape), ent.view(shape)
-        tid = tid.view(*shape, top)
+            return lp, ent
         ctx.mark_non_differentiable(tid)
-        return lp.view(shape), ent.view(shape), tlp.view(*shape, top), tid
+        return lp, ent, tlp, tid
 
     @staticmethod
     @once_differentiable
     def backward(ctx, g, gh, gtop=None, _=None):
-        hidden, weight, tokens, m, ls, ent, tid = ctx.saved_tensors
+        hidden, weight, tokens, kept, ent, tid = ctx.saved_tensors
         ignore_index, temperature, top = ctx.rest
         v, h = weight.shape
         x = hidden.view(-1, h)
@@ -201,7 +219,7 @@ class _LMHeadLogprobs(torch.autograd.Function):
             for r, end in chunks:
                 n, at = end - r, r if whole else 0
                 _logits(x[r:end], weight, z[:n])
-                _backward(z, n, v, v, tokens, ignore_index, temperature, top, tid, m, ls, ent, g, gh, gtop, dz[at:], v, r)
+                _backward(z, n, v, v, tokens, ignore_index, temperature, top, tid, kept, ent, g, gh, gtop, dz[at:], v, r)
                 if not whole:
                     if dx is not None:
                         matmul_into(dz[:n], weight, dx[r:end])
@@ -226,6 +244,10 @@ def lm_head_logprobs(hidden, weight, tokens, *, top=0, temperature=1.0, ignore_i
         raise TypeError(f'hidden and weight of one dtype, float32, bfloat16 or float16, required, not {hidden.dtype} and {weight.dtype}')
     if not hidden.is_contiguous() or not weight.is_contiguous():
         raise ValueError('contiguous hidden and weight required; no hidden layout copy')
+    temperature = float(temperature)
     _check_options(weight.shape[0], top, temperature, ignore_index)
-    _check_tokens(tokens, hidden.shape[:-1], hidden.device)
-    return TokenLogprobs(*_LMHeadLogprobs.apply(hidden, weight, tokens, ignore_index, float(temperature), top))
+    _check_tokens(tokens, hidden.shape[:-1], hidden)
+    if _recorded(hidden, weight):
+        return TokenLogprobs(*_LMHeadLogprobs.apply(hidden, weight, tokens, ignore_index, temperature, top))
+    return TokenLogprobs(*_shaped(hidden.shape[:-1], top, *_head_forward(hidden.view(-1, weight.shape[1]), weight, tokens, ignore_index,
+                                                                         temperature, top, False)))
