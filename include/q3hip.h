@@ -569,6 +569,23 @@ int q3_token_logprobs_bwd(int dtype, int out_dtype, const void* z, int64_t ld, i
                           int64_t ignore_index, float inv_temperature, int64_t top, const int64_t* top_token,
                           const float* row_max, const float* row_log, const float* entropy, const float* g,
                           const float* gh, const float* gtop, void* dz, int64_t ldo, hipStream_t stream);
+/* The same of the logits A . B^T (A [M, K] hidden states, B [N, K] the LM head's weight, N % 8 == 0, K % 64 == 0, 16-byte
+ * aligned K-contiguous rows), which stay in fp32 registers: per row and group of 128 columns the maximum, rest and u of
+ * csrc/logprobs.h to m_part, rest_part, u_part [ceil(N / 128)][ldp], and the logit of a row's token to pick [M].  z, or NULL: the
+ * logits' distances to their group's maximum in 16 bits [M, N] (row stride ldz), for the gradient. */
+int q3_gemm_nt_logprobs(int dtype, const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N, int64_t K,
+                        const int64_t* tokens, float inv_temperature, float* m_part, float* rest_part, float* u_part,
+                        float* pick, int64_t ldp, void* z, int64_t ldz, hipStream_t stream);
+/* Those groups joined: the results of q3_token_logprobs. */
+int q3_head_logprobs_finish(const float* m_part, const float* rest_part, const float* u_part, int64_t ldp, const float* pick,
+                            int64_t rows, int64_t vocab, const int64_t* tokens, int64_t ignore_index,
+                            float inv_temperature, float* logprob, float* entropy, float* row_max, float* row_log,
+                            hipStream_t stream);
+/* The logits' gradient (dtype) in place of q3_gemm_nt_logprobs' z. */
+int q3_head_logprobs_bwd(int dtype, void* z, int64_t ldz, int64_t rows, int64_t vocab, const int64_t* tokens,
+                         int64_t ignore_index, float inv_temperature, const float* m_part, int64_t ldp,
+                         const float* row_max, const float* row_log, const float* logprob, const float* entropy,
+                         const float* g, const float* gh, hipStream_t stream);
 
 /* ------------------------------------------------------------------ attention over a shared prefix
  * New: no counterpart in the reference.  B rows in R groups of B / R; queries q [B, S, Hq, 128] of row b stand at its own

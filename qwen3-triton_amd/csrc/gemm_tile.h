@@ -17,7 +17,7 @@
 #pragma once
 #include <type_traits>
 
-#include "common.h"
+#include "logprobs.h"
 
 namespace q3gemm {
 
@@ -72,6 +72,8 @@ struct Args {
   const int64_t* tgt;
   float *m_part, *s_part, *pick;
   int64_t part0, ldp, col0;
+  float* u_part;  // log probability statistics: with m_part, s_part (rest) and log2(e) / temperature
+  float c2;
   // Q8: scales of the A rows, and of the B rows of each piece (gate/up: of Wg and Wu)
   const float* rscale;
   const float* cscale[3];
@@ -111,7 +113,9 @@ Q3_DEV void work_coords(int bid, int tiles_m, int tiles_n, int splits, int& tm, 
 
 // EPI 0: plain / residual / split partials; 2: cross-entropy statistics (per row and 128-column group: the max and the
 // sum of exp(z - max) to m_part / s_part [part0 + group][row], the logit of column tgt[row] - col0 to pick[row]) of
-// the rounded logits, which are stored too; 3: gate/up SwiGLU; 5: SwiGLU backward.  KP: A and B in pieces along K.
+// the rounded logits, which are stored too; 3: gate/up SwiGLU; 5: SwiGLU backward; 6: log probability statistics
+// (logprobs.h) of the fp32 logits per row and 128-column group, to m_part, s_part and u_part, with the logit of column tgt[row]
+// to pick[row], and where c[0] is set the logits' distances to their group's maximum in 16 bits (q3lp::kGapRange).  KP: A and B in pieces along K.
 template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool AT, bool BT, int EPI, bool KP, bool Q8>
 __global__ __launch_bounds__(WM * WN * 64) void gemm_tile_kernel(Args ar) {
   constexpr int NW = WM * WN;
@@ -514,7 +518,59 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile_kernel(Args ar) {
       const int c = lane % CH;
       const int rlim = mrows - ma - wm * TMW;  // valid rows / columns of the wave's block
       auto row_chunk = [&](int r) { return *reinterpret_cast<const i32x4*>(wl + r * (NC * 2) + ((c ^ swz(r)) << 4)); };
-      if constexpr (EPI == 2) {
+      if constexpr (EPI == 6) {
+        // A lane's 32 values of a row, then the row's four lanes; each row block's accumulators are dead before the next's.
+        static_assert(TNW == 128 && CH == 16, "one statistics partial per wave and row");
+        const int col0 = nb + wn * TNW, clim = ncols - col0;
+        if (clim <= 0) return;  // a wave past the last column
+        const int64_t part = col0 / 128 * ar.ldp;
+#pragma unroll
+        for (int i = 0; i < FM; ++i) {
+          const int row = ma + wm * TMW + i * 16 + j16;
+          float v[4 * FN];
+#pragma unroll
+          for (int j = 0; j < FN; ++j)
+#pragma unroll
+            for (int e = 0; e < 4; ++e) {
+              v[4 * j + e] = acc[i][j][e];
+              if (clim < 128 && j * 16 + 4 * quarter + e >= clim) v[4 * j + e] = -INFINITY;
+            }
+          if (row < mrows) {
+            const int64_t t = ar.tgt[row] - col0;
+            if (t >= 0 && t < min(clim, 128) && ((int)t & 12) == 4 * quarter) {
+#pragma unroll
+              for (int j = 0; j < FN; ++j)
+#pragma unroll
+                for (int e = 0; e < 4; ++e)
+                  if ((int)t == j * 16 + 4 * quarter + e) ar.pick[row] = v[4 * j + e];
+            }
+          }
+          q3lp::Part p = q3lp::part_of(v, ar.c2);
+#pragma unroll
+          for (int o = 16; o < 64; o <<= 1)
+            p = q3lp::join(p, q3lp::Part{__shfl_xor(p.m, o, 64), __shfl_xor(p.rest, o, 64), __shfl_xor(p.u, o, 64)}, ar.c2);
+          if (quarter == 0 && row < mrows) {
+            ar.m_part[part + row] = p.m;
+            ar.s_part[part + row] = p.rest;
+            ar.u_part[part + row] = p.u;
+          }
+          if (C) {
+#pragma unroll
+            for (int j = 0; j < FN; ++j)
+              stage_out(i, j, q3lp::gap2(v[4 * j], v[4 * j + 1], p.m, ar.c2), q3lp::gap2(v[4 * j + 2], v[4 * j + 3], p.m, ar.c2));
+          }
+        }
+        if (!C) return;
+        lds_wait();
+        __builtin_amdgcn_wave_barrier();
+#pragma unroll
+        for (int q = 0; q < TMW / RPI; ++q) {
+          const int r = q * RPI + lane / CH;
+          if (r < rlim && c * 8 < clim)
+            *reinterpret_cast<i32x4*>(C + (int64_t)(ma + wm * TMW + r) * ldc + col0 + c * 8) = row_chunk(r);
+        }
+        return;
+      } else if constexpr (EPI == 2) {
         // The logits are rounded into the staged block first, so their accumulators are dead before the statistics'
         // temporaries are live; then each row's 16 chunks (16 lanes) are read once, for the store and the statistics.
         static_assert(TNW == 128 && CH == 16, "one statistics partial per wave and row");

@@ -580,4 +580,39 @@ int q3_gemm_nt_ce_stats_store(int dtype, const void* A, int64_t lda, const void*
   return q3gemm::launch_tile_nt(dtype, big ? 0 : 1, 2, a, stream);
 }
 
+// LM-head logits A B^T and their log probability statistics (q3hip.h), stored less their groups' maxima where z is set: 256 x 256
+// tiles, 128 x 256 as above, 32 x 256 with a deeper ring for few rows, which wait for the weight.
+int q3_gemm_nt_logprobs(int dtype, const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N, int64_t K,
+                        const int64_t* tokens, float inv_temperature, float* m_part, float* rest_part, float* u_part, float* pick,
+                        int64_t ldp, void* z, int64_t ldz, hipStream_t stream) {
+  Q3_REQUIRE((dtype == Q3_BF16 || dtype == Q3_F16) && tokens && m_part && rest_part && u_part && pick);
+  Q3_REQUIRE(M > 0 && N > 0 && K > 0 && M < (1ll << 31) - 256 && N < (1ll << 30) && N % 8 == 0 && K < (1ll << 31) && K % 64 == 0);
+  Q3_REQUIRE(operand_ok(A, lda, M, K, false) && operand_ok(B, ldb, N, K, false) && ldp >= M);
+  Q3_REQUIRE(inv_temperature > 0.f && inv_temperature < INFINITY && (!z || (ldz >= N && ldz % 8 == 0 && al16(z))));
+  Args a{};
+  a.a.p[0] = (const u16*)A;
+  a.a.ld[0] = lda;
+  a.b.p[0] = (const u16*)B;
+  a.b.ld[0] = ldb;
+  a.M = M;
+  a.N = N;
+  a.K = K;
+  a.pieces = a.splits = 1;
+  a.c[0] = z;
+  a.ldc[0] = ldz;
+  a.tgt = tokens;
+  a.m_part = m_part;
+  a.s_part = rest_part;
+  a.u_part = u_part;
+  a.pick = pick;
+  a.ldp = ldp;
+  a.c2 = inv_temperature * q3lp::kLog2e;
+  const bool big = M > 128 && (M % 256 == 0 || M % 256 > 128 || M > 2048);
+  const int bm = big ? 256 : M > 32 ? 128 : 32;
+  a.tms = (int)cdiv(M, bm);
+  a.tns = (int)cdiv(N, 256);
+  Q3_REQUIRE((int64_t)a.tms * a.tns < (1ll << 31));
+  return q3gemm::launch_tile_nt(dtype, big ? 0 : M > 32 ? 1 : 2, 6, a, stream);
+}
+
 }  // extern "C"

@@ -15,77 +15,15 @@
 // thread; few rows small ones, so that one row's latency is spread over many CUs.  A second launch joins a row's slices.
 #include <algorithm>
 
-#include "common.h"
+#include "logprobs.h"
 
 namespace {
+
+using namespace q3lp;
 
 constexpr int kThreads = 256;
 constexpr int kMaxTop = 32;
 constexpr int kGradVectors = 4;  // 16-byte vectors of logits a thread
-constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
-
-// Statistics of a part of a row: its maximum m, rest = the sum of e^d over all but one element that is m, and u = the sum of
-// e^d d, d counted from m in base 2.  m = -inf: nothing but -inf there (rest 0, or NaN where there is a NaN too).
-struct Part {
-  float m, rest, u;
-};
-Q3_DEV float part_total(const Part& a) { return a.m == -INFINITY ? a.rest : 1.f + a.rest; }
-// c2 = log2(e) / temperature
-Q3_DEV Part join(const Part& a, const Part& b, float c2) {
-  const bool first = a.m >= b.m;
-  const Part &hi = first ? a : b, &lo = first ? b : a;
-  if (lo.m == -INFINITY) return Part{hi.m, hi.rest + lo.rest, hi.u};
-  const float d = (lo.m - hi.m) * c2, w = __builtin_amdgcn_exp2f(d), t = 1.f + lo.rest;
-  return Part{hi.m, fmaf(t, w, hi.rest), fmaf(w, fmaf(t, fmaxf(d, -1e30f), lo.u), hi.u)};
-}
-
-// Statistics of N values of a thread.  One element that is the maximum is taken out on the way to it (each step keeps the larger
-// and stores the smaller), in four chains.  d comes as fma(x, c2, -m c2): one rounding, and what the product m c2 lost to its own is
-// the same factor of every term.  Maxima and minima here hand NaN on.
-template <int N> Q3_DEV Part part_of(const float (&v)[N], float c2) {
-  static_assert(N % 4 == 0, "four chains");
-  float x[N], top[4];
-#pragma unroll
-  for (int k = 0; k < 4; ++k) {
-    top[k] = v[k];
-#pragma unroll
-    for (int i = k + 4; i < N; i += 4) {
-      x[i] = __builtin_elementwise_minimum(top[k], v[i]);
-      top[k] = __builtin_elementwise_maximum(top[k], v[i]);
-    }
-  }
-  Part p{top[0], 0.f, 0.f};
-#pragma unroll
-  for (int k = 1; k < 4; ++k) {
-    x[k] = __builtin_elementwise_minimum(p.m, top[k]);
-    p.m = __builtin_elementwise_maximum(p.m, top[k]);
-  }
-  const bool nan = p.m != p.m;
-  if (nan) p.m = -INFINITY;
-  if (__any(fabsf(p.m) > 1e30f && p.m != -INFINITY)) {  // m c2 might overflow (rows of the type's lowest value)
-    const float ref = p.m == -INFINITY ? 0.f : p.m;
-#pragma unroll
-    for (int i = 1; i < N; ++i) {
-      const float d = (x[i] - ref) * c2, e = __builtin_amdgcn_exp2f(d);
-      p.rest += e;
-      p.u = fmaf(e, fmaxf(d, -1e30f), p.u);
-    }
-  } else {
-    const float mc = p.m == -INFINITY ? 0.f : p.m * c2, lost = p.m == -INFINITY ? 0.f : fmaf(p.m, c2, -mc);
-    float rest[2] = {0.f, 0.f}, u[2] = {0.f, 0.f};
-#pragma unroll
-    for (int i = 1; i < N; ++i) {
-      const float d = fmaf(x[i], c2, -mc), e = __builtin_amdgcn_exp2f(d);
-      rest[i & 1] += e;
-      u[i & 1] = fmaf(e, fmaxf(d, -1e30f), u[i & 1]);
-    }
-    const float k = __builtin_amdgcn_exp2f(-lost), r = rest[0] + rest[1];
-    p.rest = r * k;
-    p.u = k * fmaf(-lost, r, u[0] + u[1]);
-  }
-  if (nan || p.m == INFINITY) p.rest = NAN;  // inf - inf
-  return p;
-}
 
 // ---------------------------------------------------------------- the largest k
 // Values as whole numbers in their order, NaN above all, 0 below all; keys: the value's order, then the lower index first.
@@ -521,6 +459,106 @@ template <typename T, typename O> __global__ __launch_bounds__(kThreads) void gr
   }
 }
 
+// ---------------------------------------------------------------- the LM head's rows
+// Statistics of 128-column groups [group][ldp] from the LM head's product joined: 16 rows a workgroup, 16 threads a row, each a
+// fixed set of groups (as many loads in flight as there are threads).
+struct Head {
+  const float *m, *rest, *u, *pick;
+  int64_t ldp;
+  int groups;
+};
+__global__ __launch_bounds__(kThreads) void head_finish_kernel(Head h, Fwd a) {
+  constexpr int R = 16, G = kThreads / R;
+  __shared__ Part part[G][R];
+  const int lr = threadIdx.x % R, sl = threadIdx.x / R;
+  const int64_t r = (int64_t)blockIdx.x * R + lr, rc = min(r, a.rows - 1);
+  const float c2 = a.c * kLog2e;
+  Part p{-INFINITY, 0.f, 0.f};
+  int i = sl;
+  for (; i + 3 * G < h.groups; i += 4 * G) {
+    Part q[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int64_t at = (int64_t)(i + k * G) * h.ldp + rc;
+      q[k] = Part{h.m[at], h.rest[at], h.u[at]};
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) p = join(p, q[k], c2);
+  }
+  for (; i < h.groups; i += G) {
+    const int64_t at = (int64_t)i * h.ldp + rc;
+    p = join(p, Part{h.m[at], h.rest[at], h.u[at]}, c2);
+  }
+  part[sl][lr] = p;
+  __syncthreads();
+  if (sl != 0 || r >= a.rows) return;
+  for (int k = 1; k < G; ++k) p = join(p, part[k][lr], c2);
+  const int64_t t = a.tok[r];
+  if (t == a.ignore) {
+    left_out(a, r);
+    return;
+  }
+  const bool valid = t >= 0 && t < a.vocab;
+  finish_row(a, r, p, valid ? h.pick[r] : 0.f, valid);
+}
+
+// dz in the place of what the product left of the logits (their distances to their group's maximum): as grad_kernel, with
+// log2 p = (c2 (m_group - M) - ls log2(e)) - distance; the given token's log p is the result itself.
+template <typename O> __global__ __launch_bounds__(kThreads) void head_grad_kernel(Head h, Bwd a, const float* logprob, int slices) {
+  constexpr int C = kGradVectors, N = kThreads * 8 * C;
+  const int64_t r = blockIdx.x / (unsigned)slices;
+  const int base = (int)(blockIdx.x - (unsigned)(r * slices)) * N + (int)threadIdx.x * 8, vocab = (int)a.vocab;
+  const int64_t t = a.tok[r];
+  u16* row = (u16*)a.dz + r * a.ldo;
+  const bool live = t != a.ignore;
+  i32x4 raw[C];
+  float gm[C];
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    const int i0 = base + i * (kThreads * 8);
+    if (live && i0 < vocab) {
+      raw[i] = *reinterpret_cast<const i32x4*>(row + i0);
+      gm[i] = h.m[(int64_t)(i0 >> 7) * h.ldp + r];
+    }
+  }
+  float m = 0.f, ls = 0.f, g = 0.f, gh = 0.f, ent = 0.f, tlp = 0.f;
+  if (live) {
+    m = a.m[r];
+    ls = a.ls[r];
+    ent = a.entropy[r];
+    tlp = logprob[r];
+    g = a.g ? (t >= 0 && t < vocab ? a.g[r] : NAN) : 0.f;
+    gh = a.gh ? a.gh[r] : 0.f;
+  }
+#pragma unroll
+  for (int i = 0; i < C; ++i) {
+    const int i0 = base + i * (kThreads * 8);
+    if (i0 >= vocab) continue;
+    float o[8];
+    if (live) {
+      const float at = fmaf(gm[i] - m, a.c, -ls) * kLog2e;
+#pragma unroll
+      for (int e = 0; e < 8; ++e) {
+        const float gap = (float)(((uint32_t)raw[i][e >> 1] >> (16 * (e & 1))) & 0xffffu);
+        const float l2 = fmaf(gap, -kGapStep, at);
+        o[e] = -a.c * __builtin_amdgcn_exp2f(l2) * fmaf(gh, fmaf(l2, kLn2, ent), g);
+      }
+      const int64_t mine = t - i0;
+      if (mine >= 0 && mine < 8) {
+        const float p = __builtin_amdgcn_exp2f(tlp * kLog2e);
+        const float v = a.c * (-expm1f(tlp) * g - p * gh * (fmaxf(tlp, -1e30f) + ent));
+#pragma unroll
+        for (int e = 0; e < 8; ++e)
+          if (e == mine) o[e] = v;
+      }
+    } else {
+#pragma unroll
+      for (int e = 0; e < 8; ++e) o[e] = 0.f;
+    }
+    store_values<O, 8>(row + i0, o);
+  }
+}
+
 // ---------------------------------------------------------------- host
 bool dtype_ok(int dt) { return dt == Q3_F32 || dt == Q3_F16 || dt == Q3_BF16; }
 int vec_of(int dtype) { return dtype == Q3_F32 ? 4 : 8; }
@@ -616,6 +654,40 @@ int q3_token_logprobs_bwd(int dtype, int out_dtype, const void* z, int64_t ld, i
   if (out_dtype == Q3_BF16) return backward<F32, BF16>(a, stream);
   if (out_dtype == Q3_F16) return backward<F32, F16>(a, stream);
   return backward<F32, F32>(a, stream);
+}
+
+int q3_head_logprobs_finish(const float* m_part, const float* rest_part, const float* u_part, int64_t ldp, const float* pick,
+                            int64_t rows, int64_t vocab, const int64_t* tokens, int64_t ignore_index, float inv_temperature,
+                            float* logprob, float* entropy, float* row_max, float* row_log, hipStream_t stream) {
+  Q3_REQUIRE(m_part && rest_part && u_part && pick && tokens && logprob && entropy && row_max && row_log && rows > 0 &&
+             rows < (1ll << 31) && vocab > 0 && vocab < (1ll << 30) && ldp >= rows && inv_temperature > 0.f && inv_temperature < INFINITY);
+  Fwd a{};
+  a.rows = rows;
+  a.vocab = vocab;
+  a.tok = tokens;
+  a.ignore = ignore_index;
+  a.c = inv_temperature;
+  a.logprob = logprob;
+  a.entropy = entropy;
+  a.m = row_max;
+  a.ls = row_log;
+  head_finish_kernel<<<(unsigned)cdiv(rows, 16), kThreads, 0, stream>>>(Head{m_part, rest_part, u_part, pick, ldp, (int)cdiv(vocab, 128)}, a);
+  return (int)hipGetLastError();
+}
+
+int q3_head_logprobs_bwd(int dtype, void* z, int64_t ldz, int64_t rows, int64_t vocab, const int64_t* tokens, int64_t ignore_index,
+                         float inv_temperature, const float* m_part, int64_t ldp, const float* row_max, const float* row_log,
+                         const float* logprob, const float* entropy, const float* g, const float* gh, hipStream_t stream) {
+  Q3_REQUIRE((dtype == Q3_BF16 || dtype == Q3_F16) && z && ((uintptr_t)z & 15) == 0 && vocab > 0 && vocab < (1ll << 30) - (1 << 16) &&
+             vocab % 8 == 0 && ldz >= vocab && ldz % 8 == 0 && rows > 0 && rows < (1ll << 31) && ldp >= rows && tokens && m_part &&
+             row_max && row_log && logprob && entropy && inv_temperature > 0.f && inv_temperature < INFINITY);
+  const int64_t n = cdiv(vocab, (int64_t)kThreads * 8 * kGradVectors);
+  Q3_REQUIRE(rows * n < (1ll << 31));
+  const Bwd a{nullptr, 0, rows, vocab, tokens, ignore_index, inv_temperature, 0, nullptr, row_max, row_log, entropy, g, gh, nullptr, z, ldz};
+  const Head h{m_part, nullptr, nullptr, nullptr, ldp, 0};
+  if (dtype == Q3_BF16) head_grad_kernel<BF16><<<(unsigned)(rows * n), kThreads, 0, stream>>>(h, a, logprob, (int)n);
+  else head_grad_kernel<F16><<<(unsigned)(rows * n), kThreads, 0, stream>>>(h, a, logprob, (int)n);
+  return (int)hipGetLastError();
 }
 
 }  // extern "C"

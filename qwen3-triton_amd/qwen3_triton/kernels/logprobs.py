@@ -13,7 +13,7 @@ from torch.autograd.function import once_differentiable
 
 from .. import _hip as H
 from ._ops import cast
-from .linear import gemm, gemm_nt_into, gemm_ok, matmul_into
+from .linear import MAX_LD, gemm, gemm_nt_into, gemm_ok, matmul_into
 
 MAX_TOP = 32
 IGNORE_INDEX = -100
@@ -175,23 +175,50 @@ def _logits(x, w, z):
         matmul_into(x, w.t(), z)
 
 
+def _fused_ok(x, w, top):
+    """The logits' product with their statistics in its epilogue (matrix cores; alternatives need whole rows of logits)."""
+    return not top and x.shape[1] % 64 == 0 and gemm_ok(x, w) and w.shape[0] % 8 == 0 and w.shape[0] < MAX_LD and x.shape[0] < (1 << 31) - 256
+
+
+def _fused_product(x, w, tokens, temperature, store):
+    """(statistics [3, groups of 128 columns, rows], logits of the tokens, 16 bits of each logit [T, V] for the gradient or None)"""
+    t, h = x.shape
+    v = w.shape[0]
+    stats = x.new_empty((3, -(-v // 128), t), dtype=torch.float32)
+    pick = x.new_empty(t, dtype=torch.float32)
+    z = x.new_empty((t, v)) if store else None   # 16 bits; the gradient takes its place
+    p, step = stats.data_ptr(), 4 * stats[0].numel()
+    H.call("q3_gemm_nt_logprobs", H.code(x.dtype), x.data_ptr(), h, w.data_ptr(), h, t, v, h, tokens.data_ptr(), 1.0 / temperature,
+           p, p + step, p + 2 * step, pick.data_ptr(), t, None if z is None else z.data_ptr(), v, H.stream())
+    return stats, pick, z
+
+
 def _head_forward(x, weight, tokens, ignore_index, temperature, top, keep):
+    """(``_forward``'s results, [statistics, stored logits] of the fused form with ``keep``)"""
     t, v = x.shape[0], weight.shape[0]
     with torch.cuda.device(x.device):
+        if _fused_ok(x, weight, top):
+            outs = _outputs(x, t, 0, True)
+            stats, pick, z = _fused_product(x, weight, tokens, temperature, keep)
+            p, step = stats.data_ptr(), 4 * stats[0].numel()
+            H.call("q3_head_logprobs_finish", p, p + step, p + 2 * step, t, pick.data_ptr(), t, v, tokens.data_ptr(), ignore_index,
+                   1.0 / temperature, outs[0].data_ptr(), outs[1].data_ptr(), outs[4].data_ptr(), outs[4].data_ptr() + 4 * t, H.stream())
+            return outs, (stats[0].clone() if keep else None, z)
         outs = _outputs(x, t, top, keep)
         chunks = _chunks(t, v)
         z = torch.empty((chunks[0][1], v), device=x.device, dtype=torch.float32)
         for r, end in chunks:
             _logits(x[r:end], weight, z[:end - r])
             _forward(z, end - r, v, v, tokens, ignore_index, temperature, top, keep, outs, r)
-    return outs
+    return outs, (None, None)
 
 
 class _LMHeadLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, tokens, ignore_index, temperature, top):
-        outs = _head_forward(hidden.view(-1, weight.shape[1]), weight, tokens, ignore_index, temperature, top, True)
-        ctx.save_for_backward(hidden, weight, tokens, outs[4], outs[1], outs[3])
+        outs, (groups, ctx.z) = _head_forward(hidden.view(-1, weight.shape[1]), weight, tokens, ignore_index, temperature, top, True)
+        # the results are the caller's: what the gradient needs of them is kept apart
+        ctx.save_for_backward(hidden, weight, tokens, outs[4], outs[1], outs[3], groups, outs[0] if groups is not None else None)
         ctx.rest = ignore_index, temperature, top
         ctx.set_materialize_grads(False)
         lp, ent, tlp, tid = _shaped(hidden.shape[:-1], top, *outs)
@@ -203,40 +230,64 @@ class _LMHeadLogprobs(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g, gh, gtop=None, _=None):
-        hidden, weight, tokens, kept, ent, tid = ctx.saved_tensors
+        hidden, weight, tokens, kept, ent, tid, groups, lp = ctx.saved_tensors
         ignore_index, temperature, top = ctx.rest
         v, h = weight.shape
         x = hidden.view(-1, h)
         t = x.shape[0]
         g, gh, gtop = _upstream(g), _upstream(gh), _upstream(gtop)
+        z, ctx.z = ctx.z, None   # consumed: the gradient takes the stored logits' place
         with torch.cuda.device(x.device):
-            whole = gemm_ok(x, weight) and v % 8 == 0   # dW = dz^T x and dX = dz W from one dz [T, V]
-            chunks = _chunks(t, v)
-            z = torch.empty((chunks[0][1], v), device=x.device, dtype=torch.float32)
-            dz = torch.empty((t if whole else chunks[0][1], v), device=x.device, dtype=x.dtype)
             dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
-            dw = torch.empty((v, h), device=x.device, dtype=x.dtype if whole else torch.float32) if ctx.needs_input_grad[1] else None
-            for r, end in chunks:
-                n, at = end - r, r if whole else 0
-                _logits(x[r:end], weight, z[:n])
-                _backward(z, n, v, v, tokens, ignore_index, temperature, top, tid, kept, ent, g, gh, gtop, dz[at:], v, r)
-                if not whole:
-                    if dx is not None:
+            if groups is not None:
+                if z is None:   # a second backward: the same logits again
+                    z = _fused_product(x, weight, tokens, temperature, True)[2]
+                H.call("q3_head_logprobs_bwd", H.code(x.dtype), z.data_ptr(), v, t, v, tokens.data_ptr(), ignore_index, 1.0 / temperature,
+                       groups.data_ptr(), t, kept.data_ptr(), kept.data_ptr() + 4 * t, lp.data_ptr(), ent.data_ptr(),
+                       None if g is None else g.data_ptr(), None if gh is None else gh.data_ptr(), H.stream())
+                dw = _products(z, x, weight, dx, ctx.needs_input_grad[1])
+            else:
+                whole = gemm_ok(x, weight) and v % 8 == 0   # dW = dz^T x and dX = dz W from one dz [T, V]
+                chunks = _chunks(t, v)
+                z = torch.empty((chunks[0][1], v), device=x.device, dtype=torch.float32)
+                dz = torch.empty((t if whole else chunks[0][1], v), device=x.device, dtype=x.dtype)
+                dw = None
+                if not whole and ctx.needs_input_grad[1]:
+                    dw = torch.empty((v, h), device=x.device, dtype=torch.float32)
+                for r, end in chunks:
+                    n, at = end - r, r if whole else 0
+                    _logits(x[r:end], weight, z[:n])
+                    _backward(z, n, v, v, tokens, ignore_index, temperature, top, tid, kept, ent, g, gh, gtop, dz[at:], v, r)
+                    if not whole and dx is not None:
                         matmul_into(dz[:n], weight, dx[r:end])
                     if dw is not None:
                         matmul_into(dz[:n].t(), x[r:end], dw, accumulate=r > 0)
-            if whole and dx is not None:
-                gemm([dz], [weight], [dx], t, h, v, kmajor=(False, True))
-            if whole and dw is not None:
-                gemm([dz], [x], [dw], v, h, t, kmajor=(True, True))
-            if dw is not None:
-                dw = cast(dw, weight.dtype) if dw.dtype != weight.dtype else dw
+                if whole:
+                    dw = _products(dz, x, weight, dx, ctx.needs_input_grad[1])
+                elif dw is not None and dw.dtype != weight.dtype:
+                    dw = cast(dw, weight.dtype)
         return None if dx is None else dx.view(hidden.shape), dw, None, None, None, None
+
+
+def _products(dz, x, weight, dx, need_dw):
+    """dX = dz W into ``dx`` (None: not wanted); returns dW = dz^T x or None."""
+    (t, v), h = dz.shape, x.shape[1]
+    if dx is not None:
+        gemm([dz], [weight], [dx], t, h, v, kmajor=(False, True))
+    if not need_dw:
+        return None
+    dw = torch.empty_like(weight)
+    gemm([dz], [x], [dw], v, h, t, kmajor=(True, True))
+    return dw
 
 
 def lm_head_logprobs(hidden, weight, tokens, *, top=0, temperature=1.0, ignore_index=IGNORE_INDEX):
     """``token_logprobs`` of the logits ``hidden @ weight.T`` (hidden [..., H], weight [V, H], both fp32, bf16 or fp16), which
-    are formed in fp32 and never rounded; the gradient reaches hidden and weight."""
+    are formed in fp32; the gradient reaches hidden and weight.
+
+    16-bit operands with H a multiple of 64 and V of 8, without alternatives: the results are formed beside the product, and no
+    logits are written unless a gradient is wanted; then 16 bits of each are kept for it (their distance to the largest of 128),
+    which its own rounding takes the place of.  Otherwise the logits are written in fp32, 1 GiB of rows at a time."""
     if hidden.ndim < 1 or weight.ndim != 2 or hidden.numel() < 1 or weight.numel() < 1 or hidden.shape[-1] != weight.shape[1]:
         raise ValueError('nonempty hidden [..., H] and weight [V, H] required')
     H.require_device(hidden, weight)
@@ -250,4 +301,4 @@ def lm_head_logprobs(hidden, weight, tokens, *, top=0, temperature=1.0, ignore_i
     if _recorded(hidden, weight):
         return TokenLogprobs(*_LMHeadLogprobs.apply(hidden, weight, tokens, ignore_index, temperature, top))
     return TokenLogprobs(*_shaped(hidden.shape[:-1], top, *_head_forward(hidden.view(-1, weight.shape[1]), weight, tokens, ignore_index,
-                                                                         temperature, top, False)))
+                                                                         temperature, top, False)[0]))

@@ -125,3 +125,35 @@ def test_logprob_workspace():
     assert q(2, 0, 10, 0) == q(3, 1, 10, 0) == q(2, 1, 10, 11) == q(2, 1, 0, 0) == 0
     assert 0 < q(2, 1, 151936, 0) <= q(2, 1, 151936, 20) <= 1 << 20
     assert q(2, 4096, 151936, 0) <= 4096 * 24 * 12
+
+
+def head_call(**kw):
+    a = dict(dtype=2, a=P, lda=128, b=P, ldb=128, M=10, N=1000, K=128, tok=P, inv=1.0, m=P, rest=P, u=P, pick=P, ldp=10, z=P, ldz=1000)
+    a.update(kw)
+    return H.load().q3_gemm_nt_logprobs(a['dtype'], a['a'], a['lda'], a['b'], a['ldb'], a['M'], a['N'], a['K'], a['tok'], a['inv'], a['m'],
+                                        a['rest'], a['u'], a['pick'], a['ldp'], a['z'], a['ldz'], None)
+
+
+@pytest.mark.parametrize("bad", [dict(dtype=0), dict(a=None), dict(a=P + 8), dict(lda=120), dict(lda=132), dict(b=None), dict(ldb=1 << 22), dict(M=0),
+                                 dict(M=1 << 31, ldp=1 << 31), dict(N=0), dict(N=1001, ldz=1008), dict(N=1 << 30, ldz=1 << 30), dict(K=0),
+                                 dict(K=100), dict(tok=None), dict(inv=0.0), dict(inv=float('inf')), dict(m=None), dict(rest=None), dict(u=None),
+                                 dict(pick=None), dict(ldp=9), dict(z=P + 8), dict(ldz=992), dict(ldz=1004)])
+def test_head_product_refusals(bad):
+    assert head_call(**bad) == INVALID
+
+
+@pytest.mark.parametrize("bad", [dict(m=None), dict(rest=None), dict(u=None), dict(pick=None), dict(rows=0), dict(rows=11), dict(vocab=0),
+                                 dict(tok=None), dict(inv=-1.0), dict(lp=None), dict(ent=None), dict(rm=None), dict(rl=None)])
+def test_head_finish_refusals(bad):
+    a = dict(m=P, rest=P, u=P, ldp=10, pick=P, rows=10, vocab=1000, tok=P, ign=-100, inv=1.0, lp=P, ent=P, rm=P, rl=P)
+    a.update(bad)
+    assert H.load().q3_head_logprobs_finish(*a.values(), None) == INVALID
+
+
+@pytest.mark.parametrize("bad", [dict(dtype=0), dict(z=None), dict(z=P + 8), dict(ldz=992), dict(ldz=1004), dict(rows=0), dict(rows=11), dict(vocab=0),
+                                 dict(vocab=999), dict(vocab=1 << 30, ldz=1 << 30), dict(tok=None), dict(inv=0.0), dict(m=None), dict(rm=None),
+                                 dict(rl=None), dict(lp=None), dict(ent=None)])
+def test_head_gradient_refusals(bad):
+    a = dict(dtype=2, z=P, ldz=1000, rows=10, vocab=1000, tok=P, ign=-100, inv=1.0, m=P, ldp=10, rm=P, rl=P, lp=P, ent=P, g=None, gh=None)
+    a.update(bad)
+    assert H.load().q3_head_logprobs_bwd(*a.values(), None) == INVALID

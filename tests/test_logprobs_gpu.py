@@ -274,7 +274,9 @@ def head(t, h, v, dtype, seed=0):
 def test_lm_head(t, h, v, dtype):
     """Against 64 bits.  A logit is a sum of h products: off by at most (h + 8) 2^-24 sum |x w|, which moves a log probability or
     an entropy (times its largest |log p| + entropy) by at most twice that.  The gradient of a logit is rounded to the type
-    before the products with it; every product rounds its sum once."""
+    before the products with it; every product rounds its sum once.  For 16-bit types it is formed from the logit's distance to a
+    maximum in steps of 64 / 65535 in base 2: half of one moves a probability by 0.5 ln 2 64 / 65535 (3.4e-4) of itself, and
+    probabilities below 2^-64 of another may be 2^-64 of it."""
     print(f"lm head {t} {h} {v} {dtype}", flush=True)
     x, w, ids = head(t, h, v, dtype)
     z = x.double() @ w.double().t()
@@ -295,7 +297,8 @@ def test_lm_head(t, h, v, dtype):
     wide = (g.abs()[:, None] + gh.abs()[:, None] * (3 + lp.abs() + ent[:, None])) / 0.9
     u = torch.finfo(dtype).eps / 2
     tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
-    tol = tol + u * dz.abs() + tiny + (p + one * (1 - p)) * wide * e[:, None]
+    step = 0.0 if dtype == torch.float32 else 0.5 * 0.6931472 * 64 / 65535 * 1.01
+    tol = tol + u * dz.abs() + tiny + (p + one * (1 - p)) * wide * e[:, None] + p * wide * step + 2.0 ** -64 * wide * (step > 0)
     tol = torch.where((ids == -100)[:, None], 0.0, tol)
     for got, exact, bound in ((dx, dz @ w.double(), tol @ w.double().abs() + (v + 8) * E * (dz.abs() @ w.double().abs())),
                               (dw, dz.t() @ x.double(), tol.t() @ x.double().abs() + (t + 8) * E * (dz.abs().t() @ x.double().abs()))):
