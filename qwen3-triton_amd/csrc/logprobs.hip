@@ -460,39 +460,38 @@ template <typename T, typename O> __global__ __launch_bounds__(kThreads) void gr
 }
 
 // ---------------------------------------------------------------- the LM head's rows
-// Statistics of 128-column groups [group][ldp] from the LM head's product joined: 16 rows a workgroup, 16 threads a row, each a
-// fixed set of groups (as many loads in flight as there are threads).
+// Statistics of 128-column groups [group][ldp] from the LM head's product joined: R rows a workgroup, NT / R threads a row, each a
+// fixed set of groups.  16 rows side by side read whole lines; few rows take a workgroup each.
 struct Head {
   const float *m, *rest, *u, *pick;
   int64_t ldp;
   int groups;
 };
-__global__ __launch_bounds__(kThreads) void head_finish_kernel(Head h, Fwd a) {
-  constexpr int R = 16, G = kThreads / R;
-  __shared__ Part part[G][R];
-  const int lr = threadIdx.x % R, sl = threadIdx.x / R;
+template <int R, int NT> __global__ __launch_bounds__(NT) void head_finish_kernel(Head h, Fwd a) {
+  constexpr int G = NT / R, W = NT / 64;
+  __shared__ Part part[W][R];
+  const int lr = threadIdx.x % R, sl = threadIdx.x / R, lane = threadIdx.x & 63;
   const int64_t r = (int64_t)blockIdx.x * R + lr, rc = min(r, a.rows - 1);
   const float c2 = a.c * kLog2e;
   Part p{-INFINITY, 0.f, 0.f};
-  int i = sl;
-  for (; i + 3 * G < h.groups; i += 4 * G) {
+  for (int i = sl; i < h.groups; i += 4 * G) {
     Part q[4];
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int64_t at = (int64_t)(i + k * G) * h.ldp + rc;
+      const int64_t at = (int64_t)min(i + k * G, h.groups - 1) * h.ldp + rc;
       q[k] = Part{h.m[at], h.rest[at], h.u[at]};
     }
 #pragma unroll
-    for (int k = 0; k < 4; ++k) p = join(p, q[k], c2);
+    for (int k = 0; k < 4; ++k)
+      if (i + k * G < h.groups) p = join(p, q[k], c2);
   }
-  for (; i < h.groups; i += G) {
-    const int64_t at = (int64_t)i * h.ldp + rc;
-    p = join(p, Part{h.m[at], h.rest[at], h.u[at]}, c2);
-  }
-  part[sl][lr] = p;
+#pragma unroll
+  for (int o = R; o < 64; o <<= 1)
+    p = join(p, Part{__shfl_xor(p.m, o, 64), __shfl_xor(p.rest, o, 64), __shfl_xor(p.u, o, 64)}, c2);
+  if (lane < R) part[threadIdx.x >> 6][lr] = p;
   __syncthreads();
   if (sl != 0 || r >= a.rows) return;
-  for (int k = 1; k < G; ++k) p = join(p, part[k][lr], c2);
+  for (int k = 1; k < W; ++k) p = join(p, part[k][lr], c2);
   const int64_t t = a.tok[r];
   if (t == a.ignore) {
     left_out(a, r);
@@ -671,7 +670,9 @@ int q3_head_logprobs_finish(const float* m_part, const float* rest_part, const f
   a.entropy = entropy;
   a.m = row_max;
   a.ls = row_log;
-  head_finish_kernel<<<(unsigned)cdiv(rows, 16), kThreads, 0, stream>>>(Head{m_part, rest_part, u_part, pick, ldp, (int)cdiv(vocab, 128)}, a);
+  const Head h{m_part, rest_part, u_part, pick, ldp, (int)cdiv(vocab, 128)};
+  if (rows <= 256) head_finish_kernel<1, 256><<<(unsigned)rows, 256, 0, stream>>>(h, a);
+  else head_finish_kernel<16, 1024><<<(unsigned)cdiv(rows, 16), 1024, 0, stream>>>(h, a);
   return (int)hipGetLastError();
 }
 

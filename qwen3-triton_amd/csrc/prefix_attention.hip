@@ -2,17 +2,19 @@
 // positions of prefix b / n (keys and values held once per group) and its own positions 0 .. start_b + s.  Head dim 128.
 //
 // A query row is one (row b, position s, head j of the G that share a key/value head).  The rows of all n continuations are one
-// operand of the prefix's products, so a prefix is read once per 32 NW query rows, not once per continuation:
-//   S^T = K Q^T and O^T += V^T P on v_mfma_f32_16x16x32, a wave holding 32 query rows (a lane two of them: its 16-row tiles'
-//   rows lane % 16), 64 keys at a time.  The K row that feeds matrix row r is chosen so that P is the second product's operand
+// operand of the prefix's products, so a prefix is read once per 128 query rows, not once per continuation:
+//   S^T = K Q^T and O^T += V^T P on v_mfma_f32_16x16x32, a wave holding 16 or 32 query rows (a lane one of each 16: its rows
+//   lane % 16), 64 keys at a time.  The K row that feeds matrix row r is chosen so that P is the second product's operand
 //   as it comes out of the exponentials; V^T comes from transpose reads of V's rows in LDS.  The running maximum moves only
 //   when a score passes it by more than a factor 2^8; row sums are of the rounded P, by a product with ones.
-// K and V go to LDS in direct loads, one 64-key block ahead.
 //
-// Work is cut into jobs (row tile, key/value head, range of 64-key blocks).  Few queries: jobs over ranges of the prefix with
-// the rows of all continuations, and jobs over ranges of one row's own positions, each leaving unnormalised O, maximum and sum,
-// which a second launch joins in a fixed order.  Many queries (enough row tiles of one row b to fill the chip): a job goes through
-// the prefix and then its row's own positions, and writes the result.
+// Work is cut into jobs (query rows, key/value head, range of 64-key blocks), a workgroup each:
+//  * more than 32 query rows: waves take 32 rows each and share K and V tiles in LDS, loaded a block ahead;
+//  * up to 32: waves take every fourth block of the range each (K straight into the operand's registers, V into a tile of the
+//    wave's own), without waiting for each other, and their sums are joined in LDS.  A decode step's own positions are such jobs:
+//    they wait for memory beside the prefix's jobs, which are bound by the matrix cores.
+// Jobs leave unnormalised O, maximum and sum, which a second launch joins in a fixed order.  Where the queries of single rows fill
+// tiles and the tiles the chip, a job goes through the prefix and then its row's own positions, and writes the result.
 #include <algorithm>
 
 #include "common.h"
@@ -43,7 +45,7 @@ struct Args {
   int start_step;  // 0: one start for all rows
   float scale2;    // scale * log2(e)
   // plan
-  int fused, pjobs, ptiles, psplits, pper, stiles, ssplits, max_splits, min_per, slots;
+  int fused, pjobs, pfew, ptiles, psplits, pper, sfew, stiles, ssplits, max_splits, min_per, slots;
 };
 
 Q3_DEV float xmax4(float x) {  // over lanes {l, l ^ 16, l ^ 32, l ^ 48}
@@ -67,7 +69,10 @@ Q3_DEV int row_start(const Args& a, int b) {
 Q3_DEV int own_end(const Args& a, int start, int s) { return min(max(start + s + 1, 0), a.C); }
 // Blocks of own positions per split: from the number of positions alone, so that a captured step and an eager call of the same
 // length form the same sums.
-Q3_DEV int own_per(const Args& a, int blocks) { return max((blocks + a.max_splits - 1) / a.max_splits, a.min_per); }
+Q3_DEV int own_per(const Args& a, int blocks) {
+  const int per = max((blocks + a.max_splits - 1) / a.max_splits, a.min_per);
+  return a.sfew ? (per + 3) & ~3 : per;  // as many for each wave
+}
 
 // LDS: K rows of 256 bytes, 16-byte chunk c of row r at c ^ kswz(r); V in 16 slots of 4 rows (keys s, s + 16, s + 32, s + 48)
 // at a pitch of 1056 bytes, which spreads a transpose read over all banks.
@@ -84,135 +89,234 @@ template <typename T> Q3_DEV uint32_t only_finite2(uint32_t x) {
   return ((x & E) == E ? 0u : x & 0xffffu) | (((x >> 16) & E) == E ? 0u : x & 0xffff0000u);
 }
 
-template <typename T, int NW>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefix_attn_kernel(Args a) {
-  __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
-  constexpr int RT = 32 * NW;  // query rows of a job
-  const int tid = threadIdx.x, lane = tid & 63, g = lane >> 4, r16 = lane & 15;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int SG = a.S * a.G;
+// A wave's 16 U query rows: operands, O^T (lane: dims 16 dt + 4 g + i of rows 16 u + r16), maxima and sums.
+template <int U> struct Rows {
+  bf16x8_t qf[U][4];
+  f32x4 o[8][U], l[U];
+  float m[U];
+  int lim[U];  // own positions that the row sees
+};
 
-  // ---- the job
-  int b0, hk, tile, slot = 0;       // first row b of the job's rows
-  int rows;                         // query rows from b0's first on
-  int pb = 0, pe = 0, sb = 0, se = 0;  // 64-key blocks of the prefix and of b0's own positions
-  int own = 0, start = 0;           // own positions that the tile's last row sees
-  const int pblocks = (a.P + BLK - 1) / BLK;
-  if ((int)blockIdx.x < a.pjobs) {
-    // each XCD (workgroup ids congruent mod 8) takes a contiguous range of jobs, row tiles innermost: the tiles that read the
-    // same keys share an L2
-    const int xcd = blockIdx.x & 7, per = a.pjobs >> 3, rem = a.pjobs & 7;
-    int w = xcd * per + min(xcd, rem) + ((int)blockIdx.x >> 3);
-    tile = w % a.ptiles;
-    w /= a.ptiles;
-    slot = w % a.psplits;
-    w /= a.psplits;
-    hk = w % a.Hkv;
-    b0 = w / a.Hkv * a.n;
-    rows = a.n * SG;
-    pb = slot * a.pper;
-    pe = min(pb + a.pper, pblocks);
-  } else {
-    int w = (int)blockIdx.x - a.pjobs;
-    tile = w % a.stiles;
-    w /= a.stiles;
-    hk = w % a.Hkv;
-    w /= a.Hkv;
-    const int split = w % a.ssplits;
-    b0 = w / a.ssplits;
-    rows = SG;
-    start = __builtin_amdgcn_readfirstlane(row_start(a, b0));
-    const int all = (own_end(a, start, a.S - 1) + BLK - 1) / BLK;
-    own = own_end(a, start, min(tile * RT + RT - 1, rows - 1) / a.G);
-    const int blocks = (own + BLK - 1) / BLK;
-    if (a.fused) {
-      pe = pblocks;
-      se = blocks;
-    } else {
-      const int per = own_per(a, all);
-      sb = split * per;
-      if (split > 0 && sb >= all) return;  // no such split: the joining launch knows
-      se = min(sb + per, blocks);
-      sb = min(sb, se);
-      slot = a.psplits + split;
+// Where in a key block an element of S^T stands: matrix row r16 of key tile kt is key tile_key(kt) + row_key(r16), element i of
+// that tile in lane group g is key tile_key(kt) + group_key(g) + i.
+Q3_DEV constexpr int tile_key(int kt) { return 32 * (kt >> 1) + 8 * (kt & 1); }
+Q3_DEV int row_key(int r16) { return 4 * ((r16 >> 2) & 1) + 16 * (r16 >> 3) + (r16 & 3); }
+Q3_DEV int group_key(int g) { return 4 * (g & 1) + 16 * (g >> 1); }
+
+// Query rows m0 .. of the job's `rows`, which start at row b0's first; rows past the last are copies of it.
+template <int U> Q3_DEV void load_rows(const Args& a, Rows<U>& w, int m0, int rows, int b0, int hk, int start, int g, int r16) {
+  const int SG = a.S * a.G;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const int m = min(m0 + 16 * u + r16, rows - 1), b = b0 + m / SG, x = m % SG, s = x / a.G, h = hk * a.G + x % a.G;
+    w.lim[u] = own_end(a, start, s);
+    const u16* qp = a.q + b * a.ql.b + h * a.ql.h + s * a.ql.s + 8 * g;
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks) w.qf[u][ks] = *reinterpret_cast<const bf16x8_t*>(qp + 32 * ks);
+    w.l[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+    w.m[u] = -INFINITY;
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt) w.o[dt][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+  }
+}
+
+// Scores of a block -> P, with O, maxima and sums brought along.  mask: keys from `end` on (the prefix) or from the row's own
+// limit on (end < 0) are hidden.
+template <typename T, int U>
+Q3_DEV void softmax_block(Rows<U>& w, f32x4 (&S)[4][U], i32x4 (&P)[U][2], float scale2, bool mask, int key0, int end, int g) {
+  if (mask) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int rel = (end >= 0 ? end : w.lim[u]) - key0 - group_key(g);
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int i = 0; i < 4; ++i) S[kt][u][i] = tile_key(kt) + i < rel ? S[kt][u][i] : -INFINITY;
     }
   }
-  const int npre = pe - pb, nblk = npre + (se - sb);
-  const u16* pk = a.pk + b0 / a.n * a.pl.b + hk * a.pl.h;
-  const u16* pv = a.pv + b0 / a.n * a.pl.b + hk * a.pl.h;
-  const u16* ck = a.ck + b0 * a.cl.b + hk * a.cl.h;
-  const u16* cv = a.cv + b0 * a.cl.b + hk * a.cl.h;
-
-  // ---- this lane's query rows
-  const int m0 = tile * RT + wave * 32;
-  const bool work = m0 < rows;  // a wave without rows only loads
-  int lim[2];                   // own positions that the row sees
-  int64_t orow[2], ooff[2];     // its place among the partials, and in the output
-  bf16x8_t qf[2][4];
+  const float thr = 8.f / scale2;
+  bool any = false;
+  float alpha[U], ms[U];
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    const int m = min(m0 + 16 * u + r16, rows - 1), b = b0 + m / SG, x = m % SG, s = x / a.G, h = hk * a.G + x % a.G;
-    lim[u] = own_end(a, start, s);
-    const u16* qp = a.q + b * a.ql.b + h * a.ql.h + s * a.ql.s;
-    ooff[u] = b * a.ol.b + h * a.ol.h + s * a.ol.s;
-    orow[u] = ((int64_t)b * a.S + s) * (a.Hkv * a.G) + h;
+  for (int u = 0; u < U; ++u) {
+    float x = S[0][u][0];
 #pragma unroll
-    for (int ks = 0; ks < 4; ++ks)
-      qf[u][ks] = *reinterpret_cast<const bf16x8_t*>(qp + 32 * ks + 8 * g);
+    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+      for (int i = 0; i < 4; ++i) x = __builtin_fmaxf(x, S[kt][u][i]);
+    x = xmax4(x);
+    const bool need = x > w.m[u] + thr || w.m[u] == -INFINITY;
+    const float mn = need ? x : w.m[u];
+    alpha[u] = w.m[u] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((w.m[u] - mn) * scale2);
+    w.m[u] = mn;
+    ms[u] = mn == -INFINITY ? 0.f : mn * scale2;
+    any = any || need;
   }
-  // the first own position that some row of the wave does not see
-  const int lim_w = own_end(a, start, min(m0, rows - 1) / a.G);
-
-  // ---- global -> LDS
-  uint32_t krow[16 / NW], kchk[16 / NW], vrow[16 / NW];
+  if (__any(any)) {
 #pragma unroll
-  for (int i = 0; i < 16 / NW; ++i) {
-    const int w = wave + NW * i, r = 4 * w + g;
-    krow[i] = (uint32_t)r;
-    kchk[i] = (uint32_t)((r16 ^ kswz(r)) * 16);
-    vrow[i] = (uint32_t)(w + 16 * g);
+    for (int u = 0; u < U; ++u) {
+      w.l[u] *= alpha[u];
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt) w.o[dt][u] *= alpha[u];
+    }
   }
-  auto issue = [&](int j) {
-    if (j >= nblk) return;
-    const bool pre = j < npre;
-    const int key0 = (pre ? pb + j : sb + j - npre) * BLK, count = (pre ? a.P : own) - key0;
-    const int64_t st = pre ? a.pl.s : a.cl.s;
-    const int bytes = (min(count, BLK) - 1) * (int)st * 2 + 2 * D;
-    const u16 *kp = (pre ? pk : ck) + key0 * st, *vp = (pre ? pv : cv) + key0 * st;
-    char* base = lds + (j & 1) * kStage;
 #pragma unroll
-    for (int i = 0; i < 16 / NW; ++i)
-      buffer_to_lds(kp, bytes, krow[i] * (uint32_t)(st * 2) + kchk[i], base + (wave + NW * i) * 1024);
+  for (int u = 0; u < U; ++u)
 #pragma unroll
-    for (int i = 0; i < 16 / NW; ++i)
-      buffer_to_lds(vp, bytes, vrow[i] * (uint32_t)(st * 2) + r16 * 16, base + kKTile + (wave + NW * i) * kSlot);
-  };
+    for (int kt = 0; kt < 4; ++kt) {
+#pragma unroll
+      for (int i = 0; i < 4; ++i) S[kt][u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[kt][u][i], scale2, -ms[u]));
+      P[u][kt >> 1][2 * (kt & 1)] = (int)pack2<T>(S[kt][u][0], S[kt][u][1]);
+      P[u][kt >> 1][2 * (kt & 1) + 1] = (int)pack2<T>(S[kt][u][2], S[kt][u][3]);
+    }
+}
 
-  // ---- LDS -> fragments.  Matrix row r16 of key tile kt reads K row 32 (kt / 2) + 8 (kt % 2) + krow0; element i of that tile in
-  // lane group g is then key 32 (kt / 2) + 8 (kt % 2) + kbase + i.
-  const int krow0 = 4 * ((r16 >> 2) & 1) + 16 * (r16 >> 3) + (r16 & 3);
-  const int kbase = 4 * (g & 1) + 16 * (g >> 1);
-  int koff[4], voff[2];
-#pragma unroll
-  for (int ks = 0; ks < 4; ++ks) koff[ks] = krow0 * 256 + (((4 * ks + g) ^ r16) << 4);
+// O^T += V^T P and the sums of P, V's tile at vb.  A value that is not finite would spoil the rows that do not see its position too
+// (0 times it is NaN): blocks that some row sees in part (look) are looked through first, and then such values are kept out of
+// the product and added to the rows that do see them.
+template <typename T, int U>
+Q3_DEV void value_block(Rows<U>& w, const i32x4 (&P)[U][2], const char* vb, bool look, int key0, int g, int r16) {
+  const int lane = 16 * g + r16;
+  int voff[2];
 #pragma unroll
   for (int kc = 0; kc < 2; ++kc) voff[kc] = (4 * (g & 1) + (r16 >> 2)) * kSlot + (g >> 1) * 256 + 8 * (r16 & 3) + kc * 512;
-  constexpr int ktoff[4] = {0, 8 * 256, 32 * 256, 40 * 256};
-
-  f32x4 oacc[8][2], lsum[2];
-  float m[2] = {-INFINITY, -INFINITY};
+  bool clean = true;
+  if (look) {
+    uint32_t ok = 1;
+#pragma unroll 4
+    for (int i = 0; i < 16; ++i) {
+      const i32x4 x = *reinterpret_cast<const i32x4*>(vb + i * kSlot + lane * 16);
 #pragma unroll
-  for (int u = 0; u < 2; ++u) {
-    lsum[u] = f32x4{0.f, 0.f, 0.f, 0.f};
+      for (int e = 0; e < 4; ++e) ok &= finite2<T>((uint32_t)x[e]) ? 1u : 0u;
+    }
+    clean = !__any(ok == 0);
+  }
+  if (clean) {
 #pragma unroll
-    for (int dt = 0; dt < 8; ++dt) oacc[dt][u] = f32x4{0.f, 0.f, 0.f, 0.f};
+    for (int dt = 0; dt < 8; ++dt)
+#pragma unroll
+      for (int kc = 0; kc < 2; ++kc) {
+        const i32x4 v = lds_frag_tr(vb + voff[kc] + dt * 32, 8 * kSlot);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          w.o[dt][u] = mfma_16x16x32<T>(__builtin_bit_cast(bf16x8_t, v), __builtin_bit_cast(bf16x8_t, P[u][kc]), w.o[dt][u]);
+      }
+  } else {
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt)
+#pragma unroll
+      for (int kc = 0; kc < 2; ++kc) {
+        i32x4 v = lds_frag_tr(vb + voff[kc] + dt * 32, 8 * kSlot);
+#pragma unroll
+        for (int e = 0; e < 4; ++e) v[e] = (int)only_finite2<T>((uint32_t)v[e]);
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          w.o[dt][u] = mfma_16x16x32<T>(__builtin_bit_cast(bf16x8_t, v), __builtin_bit_cast(bf16x8_t, P[u][kc]), w.o[dt][u]);
+      }
+#pragma unroll 1
+    for (int key = 0; key < BLK; ++key) {
+      const char* row = vb + (key & 15) * kSlot + (key >> 4) * 256 + 8 * g;
+#pragma unroll
+      for (int dt = 0; dt < 8; ++dt) {
+        const i32x2 x = *reinterpret_cast<const i32x2*>(row + dt * 32);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const uint32_t bits = ((uint32_t)x[i >> 1] >> (16 * (i & 1))) & 0xffffu;
+          const float bad = finite2<T>(bits) ? 0.f : to_f32<T>((u16)bits);
+#pragma unroll
+          for (int u = 0; u < U; ++u) w.o[dt][u][i] += key0 + key < w.lim[u] ? bad : 0.f;
+        }
+      }
+    }
   }
   const uint32_t one2 = pack2<T>(1.f, 1.f);
   const i32x4 ones = i32x4{(int)one2, (int)one2, (int)one2, (int)one2};
-  const float thr = 8.f / a.scale2;
+#pragma unroll
+  for (int kc = 0; kc < 2; ++kc)
+#pragma unroll
+    for (int u = 0; u < U; ++u)
+      w.l[u] = mfma_16x16x32<T>(__builtin_bit_cast(bf16x8_t, ones), __builtin_bit_cast(bf16x8_t, P[u][kc]), w.l[u]);
+}
+
+// The range of a job: blocks of the prefix, then of b0's own positions.
+struct Job {
+  int b0, hk, tile, slot;  // first row b of the job's query rows
+  int rows;                // query rows from b0's first on
+  int pb, npre, sb, nblk;
+  int own, all, start;     // own positions that the job's last query row sees
+  const u16 *pk, *pv, *ck, *cv;
+};
+struct Block {  // one of them: 64 positions from key0 on, `count` of them there
+  int key0, count;
+  int64_t st;
+  const u16 *k, *v;
+};
+Q3_DEV Block block_of(const Args& a, const Job& job, int j) {
+  const bool pre = j < job.npre;
+  Block x;
+  x.key0 = (pre ? job.pb + j : job.sb + j - job.npre) * BLK;
+  x.count = min((pre ? a.P : job.own) - x.key0, BLK);
+  x.st = pre ? a.pl.s : a.cl.s;
+  x.k = (pre ? job.pk : job.ck) + x.key0 * x.st;
+  x.v = (pre ? job.pv : job.cv) + x.key0 * x.st;
+  return x;
+}
+Q3_DEV int block_bytes(const Block& x) { return (x.count - 1) * (int)x.st * 2 + 2 * D; }
+Q3_DEV bool block_masked(const Args& a, const Job& job, int j, const Block& x, int lim) {
+  return x.key0 + BLK > (j < job.npre ? a.P : lim);
+}
+
+// A query row's place among the partials, and in the output.
+Q3_DEV void row_place(const Args& a, const Job& job, int m, int64_t& part, int64_t& out) {
+  const int SG = a.S * a.G, b = job.b0 + m / SG, x = m % SG, s = x / a.G, h = job.hk * a.G + x % a.G;
+  part = (((int64_t)b * a.S + s) * (a.Hkv * a.G) + h) * a.slots + job.slot;
+  out = b * a.ol.b + h * a.ol.h + s * a.ol.s;
+}
+template <typename T> Q3_DEV void store4(const Args& a, int64_t part, int64_t out, int d, f32x4 o, float l, bool none) {
+  if (a.slots == 1) {
+    const float inv = none ? 0.f : 1.f / l;  // no position to see: zeros
+    *reinterpret_cast<i32x2*>(a.o + out + d) =
+        i32x2{(int)pack2<T>(o[0] * inv, o[1] * inv), (int)pack2<T>(o[2] * inv, o[3] * inv)};
+  } else {
+    *reinterpret_cast<f32x4*>(a.po + part * D + d) = o;
+  }
+}
+
+// More than 32 query rows: 32 a wave.
+template <typename T, int NW> Q3_DEV void tile_job(const Args& a, const Job& job, char* lds, int wave, int g, int r16) {
+  constexpr int RT = 32 * NW;
+  const int m0 = job.tile * RT + wave * 32;
+  const bool work = m0 < job.rows;  // a wave without rows only loads
+  Rows<2> w;
+  load_rows(a, w, m0, job.rows, job.b0, job.hk, job.start, g, r16);
+  const int lim_w = own_end(a, job.start, min(m0, job.rows - 1) / a.G);  // of the wave's first row, the lowest
+
+  uint32_t krow[16 / NW], kchk[16 / NW], vrow[16 / NW];
+#pragma unroll
+  for (int i = 0; i < 16 / NW; ++i) {
+    const int x = wave + NW * i, r = 4 * x + g;
+    krow[i] = (uint32_t)r;
+    kchk[i] = (uint32_t)((r16 ^ kswz(r)) * 16);
+    vrow[i] = (uint32_t)(x + 16 * g);
+  }
+  auto issue = [&](int j) {
+    if (j >= job.nblk) return;
+    const Block x = block_of(a, job, j);
+    const int bytes = block_bytes(x);
+    char* base = lds + (j & 1) * kStage;
+#pragma unroll
+    for (int i = 0; i < 16 / NW; ++i)
+      buffer_to_lds(x.k, bytes, krow[i] * (uint32_t)(x.st * 2) + kchk[i], base + (wave + NW * i) * 1024);
+#pragma unroll
+    for (int i = 0; i < 16 / NW; ++i)
+      buffer_to_lds(x.v, bytes, vrow[i] * (uint32_t)(x.st * 2) + r16 * 16, base + kKTile + (wave + NW * i) * kSlot);
+  };
+  int koff[4];
+#pragma unroll
+  for (int ks = 0; ks < 4; ++ks) koff[ks] = row_key(r16) * 256 + (((4 * ks + g) ^ r16) << 4);
 
   issue(0);
-  for (int j = 0; j < nblk; ++j) {
+  for (int j = 0; j < job.nblk; ++j) {
     __builtin_amdgcn_s_waitcnt((0 & 15) | (7 << 4) | (0 << 8));  // vmcnt(0) lgkmcnt(0)
     asm volatile("" ::: "memory");
     __builtin_amdgcn_s_barrier();  // block j is there, and every wave is done with block j - 1
@@ -220,169 +324,254 @@ __global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2)))
     issue(j + 1);
     if (!work) continue;
     const char* kb = lds + (j & 1) * kStage;
-    const char* vb = kb + kKTile;
-    const bool pre = j < npre;
-    const int key0 = (pre ? pb + j : sb + j - npre) * BLK;
+    const Block x = block_of(a, job, j);
     f32x4 S[4][2];
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt) {
-        const bf16x8_t kf = *reinterpret_cast<const bf16x8_t*>(kb + koff[ks] + ktoff[kt]);
+        const bf16x8_t kf = *reinterpret_cast<const bf16x8_t*>(kb + koff[ks] + tile_key(kt) * 256);
 #pragma unroll
         for (int u = 0; u < 2; ++u)
-          S[kt][u] = mfma_16x16x32<T>(kf, qf[u][ks], ks == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : S[kt][u]);
+          S[kt][u] = mfma_16x16x32<T>(kf, w.qf[u][ks], ks == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : S[kt][u]);
       }
-    const bool mask = key0 + BLK > (pre ? a.P : lim_w);
-    if (mask) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        const int rel = (pre ? a.P : lim[u]) - key0 - kbase;
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-          for (int i = 0; i < 4; ++i) S[kt][u][i] = 32 * (kt >> 1) + 8 * (kt & 1) + i < rel ? S[kt][u][i] : -INFINITY;
-      }
-    }
-    // ---- online softmax
-    bool need[2];
-    float alpha[2], ms[2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u) {
-      float x = S[0][u][0];
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) x = __builtin_fmaxf(x, S[kt][u][i]);
-      x = xmax4(x);
-      need[u] = x > m[u] + thr || m[u] == -INFINITY;
-      const float mn = need[u] ? x : m[u];
-      alpha[u] = m[u] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((m[u] - mn) * a.scale2);
-      m[u] = mn;
-      ms[u] = mn == -INFINITY ? 0.f : mn * a.scale2;
-    }
-    if (__any(need[0] || need[1])) {
-#pragma unroll
-      for (int u = 0; u < 2; ++u) {
-        lsum[u] *= alpha[u];
-#pragma unroll
-        for (int dt = 0; dt < 8; ++dt) oacc[dt][u] *= alpha[u];
-      }
-    }
+    const bool pre = j < job.npre, mask = block_masked(a, job, j, x, lim_w);
     i32x4 P[2][2];
-#pragma unroll
-    for (int u = 0; u < 2; ++u)
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt) {
-#pragma unroll
-        for (int i = 0; i < 4; ++i)
-          S[kt][u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[kt][u][i], a.scale2, -ms[u]));
-        P[u][kt >> 1][2 * (kt & 1)] = (int)pack2<T>(S[kt][u][0], S[kt][u][1]);
-        P[u][kt >> 1][2 * (kt & 1) + 1] = (int)pack2<T>(S[kt][u][2], S[kt][u][3]);
-      }
-    // ---- O^T += V^T P.  A value that is not finite would spoil the rows that do not see its position too (0 times it is NaN):
-    // blocks that some row sees in part are looked through first, and then such values are kept out of the product and added
-    // to the rows that do see them.
-    bool clean = true;
-    if (mask && !pre && a.S > 1) {
-      uint32_t ok = 1;
-#pragma unroll 4
-      for (int i = 0; i < 16; ++i) {
-        const i32x4 x = *reinterpret_cast<const i32x4*>(vb + i * kSlot + lane * 16);
-#pragma unroll
-        for (int e = 0; e < 4; ++e) ok &= finite2<T>((uint32_t)x[e]) ? 1u : 0u;
-      }
-      clean = !__any(ok == 0);
-    }
-    if (clean) {
-#pragma unroll
-      for (int dt = 0; dt < 8; ++dt)
-#pragma unroll
-        for (int kc = 0; kc < 2; ++kc) {
-          const i32x4 v = lds_frag_tr(vb + voff[kc] + dt * 32, 8 * kSlot);
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-            oacc[dt][u] = mfma_16x16x32<T>(__builtin_bit_cast(bf16x8_t, v), __builtin_bit_cast(bf16x8_t, P[u][kc]), oacc[dt][u]);
-        }
-    } else {
-#pragma unroll
-      for (int dt = 0; dt < 8; ++dt)
-#pragma unroll
-        for (int kc = 0; kc < 2; ++kc) {
-          i32x4 v = lds_frag_tr(vb + voff[kc] + dt * 32, 8 * kSlot);
-#pragma unroll
-          for (int e = 0; e < 4; ++e) v[e] = (int)only_finite2<T>((uint32_t)v[e]);
-#pragma unroll
-          for (int u = 0; u < 2; ++u)
-            oacc[dt][u] = mfma_16x16x32<T>(__builtin_bit_cast(bf16x8_t, v), __builtin_bit_cast(bf16x8_t, P[u][kc]), oacc[dt][u]);
-        }
-      for (int key = 0; key < BLK; ++key) {
-        const char* row = vb + (key & 15) * kSlot + (key >> 4) * 256 + 8 * g;
-#pragma unroll
-        for (int dt = 0; dt < 8; ++dt) {
-          const i32x2 x = *reinterpret_cast<const i32x2*>(row + dt * 32);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const uint32_t bits = ((uint32_t)x[i >> 1] >> (16 * (i & 1))) & 0xffffu;
-            if (finite2<T>(bits)) continue;
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-              if (key0 + key < lim[u]) oacc[dt][u][i] += to_f32<T>((u16)bits);
-          }
-        }
-      }
-    }
-#pragma unroll
-    for (int kc = 0; kc < 2; ++kc)
-#pragma unroll
-      for (int u = 0; u < 2; ++u)
-        lsum[u] = mfma_16x16x32<T>(__builtin_bit_cast(bf16x8_t, ones), __builtin_bit_cast(bf16x8_t, P[u][kc]), lsum[u]);
+    softmax_block<T, 2>(w, S, P, a.scale2, mask, x.key0, pre ? a.P : -1, g);
+    value_block<T, 2>(w, P, kb + kKTile, mask && !pre && a.S > 1, x.key0, g, r16);
   }
 
-  // ---- out: lane holds O[row 16 u + r16][16 dt + 4 g + i]
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
-    if (m0 + 16 * u + r16 >= rows) continue;
-    if (a.slots == 1) {
-      const float inv = a.P == 0 && lim[u] == 0 ? 0.f : 1.f / lsum[u][0];  // no position to see: zeros
-      u16* out = a.o + ooff[u];
+    const int m = m0 + 16 * u + r16;
+    if (m >= job.rows) continue;
+    int64_t part, out;
+    row_place(a, job, m, part, out);
 #pragma unroll
-      for (int dt = 0; dt < 8; ++dt)
-        *reinterpret_cast<i32x2*>(out + 16 * dt + 4 * g) =
-            i32x2{(int)pack2<T>(oacc[dt][u][0] * inv, oacc[dt][u][1] * inv),
-                  (int)pack2<T>(oacc[dt][u][2] * inv, oacc[dt][u][3] * inv)};
-    } else {
-      const int64_t at = orow[u] * a.slots + slot;
-#pragma unroll
-      for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<f32x4*>(a.po + at * D + 16 * dt + 4 * g) = oacc[dt][u];
-      if (g == 0) {
-        a.pm[at] = m[u] == -INFINITY ? -INFINITY : m[u] * a.scale2;
-        a.ps[at] = lsum[u][0];
-      }
+    for (int dt = 0; dt < 8; ++dt)
+      store4<T>(a, part, out, 16 * dt + 4 * g, w.o[dt][u], w.l[u][0], a.P == 0 && w.lim[u] == 0);
+    if (a.slots > 1 && g == 0) {
+      a.pm[part] = w.m[u] == -INFINITY ? -INFINITY : w.m[u] * a.scale2;
+      a.ps[part] = w.l[u][0];
     }
   }
 }
 
-// o = sum_j 2^(m_j - M) O_j / sum_j 2^(m_j - M) s_j over a query row's slots, in slot order: the prefix's splits, then those of
-// its own positions.  32 lanes a row, 4 dims each.
-template <typename T> __global__ __launch_bounds__(256) void prefix_join_kernel(Args a, int64_t rows) {
-  const int64_t row = (int64_t)blockIdx.x * 8 + (threadIdx.x >> 5);
-  if (row >= rows) return;
-  const int l = threadIdx.x & 31, Hq = a.Hkv * a.G;
+// Up to 16 U query rows: each wave takes every fourth block.
+template <typename T, int U> Q3_DEV void few_job(const Args& a, const Job& job, char* lds, int wave, int g, int r16) {
+  constexpr int NW = 4, R = 16 * U;
+  char* const vt = lds + wave * kVTile;
+  Rows<U> w;
+  i32x4 kf[4][4];
+  auto load_k = [&](int j) {
+    const Block x = block_of(a, job, j);
+    const auto d = __builtin_amdgcn_make_buffer_rsrc((void*)x.k, 0, block_bytes(x), 0x00027000);
+    const uint32_t off = (uint32_t)row_key(r16) * (uint32_t)(x.st * 2) + 16 * g;
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+      for (int ks = 0; ks < 4; ++ks)
+        kf[kt][ks] = __builtin_bit_cast(i32x4, __builtin_amdgcn_raw_buffer_load_b128(d, off + (uint32_t)tile_key(kt) * (uint32_t)(x.st * 2) + 64 * ks, 0, 0));
+  };
+  auto load_v = [&](int j) {
+    const Block x = block_of(a, job, j);
+    const int bytes = block_bytes(x);
+#pragma unroll
+    for (int i = 0; i < 16; ++i)
+      buffer_to_lds(x.v, bytes, (uint32_t)(i + 16 * g) * (uint32_t)(x.st * 2) + r16 * 16, vt + i * kSlot);
+  };
+  auto fence = [&]() {
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_sched_barrier(0);
+  };
+  if (wave < job.nblk) {
+    load_k(wave);
+    load_v(wave);
+  }
+  load_rows(a, w, 0, job.rows, job.b0, job.hk, job.start, g, r16);
+  const int lim_w = own_end(a, job.start, 0);
+  for (int j = wave; j < job.nblk; j += NW) {
+    const Block x = block_of(a, job, j);
+    f32x4 S[4][U];
+#pragma unroll
+    for (int ks = 0; ks < 4; ++ks)
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+        for (int u = 0; u < U; ++u)
+          S[kt][u] = mfma_16x16x32<T>(__builtin_bit_cast(bf16x8_t, kf[kt][ks]), w.qf[u][ks], ks == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : S[kt][u]);
+    const bool more = j + NW < job.nblk;
+    fence();
+    if (more) load_k(j + NW);
+    fence();
+    const bool pre = j < job.npre, mask = block_masked(a, job, j, x, lim_w);
+    i32x4 P[U][2];
+    softmax_block<T, U>(w, S, P, a.scale2, mask, x.key0, pre ? a.P : -1, g);
+    // this block's V: everything older than the next K's 16 loads
+    fence();
+    if (more) __builtin_amdgcn_s_waitcnt((16 & 15) | ((16 >> 4) << 14) | (7 << 4) | (15 << 8));
+    else __builtin_amdgcn_s_waitcnt((0 & 15) | (7 << 4) | (15 << 8));
+    fence();
+    value_block<T, U>(w, P, vt, mask && !pre && a.S > 1, x.key0, g, r16);
+    if (more) {
+      __builtin_amdgcn_s_waitcnt((15) | (3 << 14) | (7 << 4) | (0 << 8));  // the tile is read
+      fence();
+      load_v(j + NW);
+    }
+  }
+  // The waves' sums joined: wave i's O [R][128], maxima and sums at its tile.  What is left there is read by the wave itself.
+  __builtin_amdgcn_s_waitcnt((15) | (3 << 14) | (7 << 4) | (0 << 8));
+  fence();
+  constexpr int kRow = D * 4 + 16;  // 16 bytes of padding a row
+  static_assert(R * kRow + 8 * R <= kVTile + 8 * 32, "fits the tile with its end");
+  float* const stat = (float*)(lds + NW * kVTile);  // [wave][2][R]
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+#pragma unroll
+    for (int dt = 0; dt < 8; ++dt)
+      *reinterpret_cast<f32x4*>(vt + (16 * u + r16) * kRow + (16 * dt + 4 * g) * 4) = w.o[dt][u];
+    if (g == 0) {
+      stat[(wave * 2 + 0) * R + 16 * u + r16] = w.m[u] == -INFINITY ? -INFINITY : w.m[u] * a.scale2;
+      stat[(wave * 2 + 1) * R + 16 * u + r16] = w.l[u][0];
+    }
+  }
+  __syncthreads();
+  // 32 lanes a row, 4 dims each
+  const int t = wave * 64 + 16 * g + r16, l = t & 31;
+  for (int m = t >> 5; m < job.rows; m += 8) {
+    float M = -INFINITY, sum = 0.f;
+#pragma unroll
+    for (int i = 0; i < NW; ++i) M = __builtin_fmaxf(M, stat[(i * 2) * R + m]);
+    f32x4 o = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+    for (int i = 0; i < NW; ++i) {
+      const float mi = stat[(i * 2) * R + m], e = mi == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(mi - M);
+      sum = __builtin_fmaf(e, stat[(i * 2 + 1) * R + m], sum);
+      o += e * *reinterpret_cast<const f32x4*>(lds + i * kVTile + m * kRow + l * 16);
+    }
+    int64_t part, out;
+    row_place(a, job, m, part, out);
+    store4<T>(a, part, out, 4 * l, o, sum, a.P == 0 && own_end(a, job.start, m / a.G) == 0);
+    if (a.slots > 1 && l == 0) {
+      a.pm[part] = M;
+      a.ps[part] = sum;
+    }
+  }
+}
+
+constexpr int kFewLds = 4 * kVTile + 4 * 2 * 32 * 4;
+
+template <typename T, int NW>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefix_attn_kernel(Args a) {
+  constexpr int kLds = NW == 4 && kFewLds > 2 * kStage ? kFewLds : 2 * kStage;
+  __shared__ __attribute__((aligned(1024))) char lds[kLds];
+  constexpr int RT = 32 * NW;  // query rows of a tile
+  const int tid = threadIdx.x, g = (tid & 63) >> 4, r16 = tid & 15;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  const int SG = a.S * a.G, pblocks = (a.P + BLK - 1) / BLK;
+
+  Job job{};
+  bool few;
+  if ((int)blockIdx.x < a.pjobs) {
+    // each XCD (workgroup ids congruent mod 8) takes a contiguous range of jobs, row tiles innermost: the tiles that read the
+    // same keys share an L2
+    const int xcd = blockIdx.x & 7, per = a.pjobs >> 3, rem = a.pjobs & 7;
+    int w = xcd * per + min(xcd, rem) + ((int)blockIdx.x >> 3);
+    job.tile = w % a.ptiles;
+    w /= a.ptiles;
+    job.slot = w % a.psplits;
+    w /= a.psplits;
+    job.hk = w % a.Hkv;
+    job.b0 = w / a.Hkv * a.n;
+    job.rows = a.n * SG;
+    job.pb = job.slot * a.pper;
+    job.npre = job.nblk = min(a.pper, pblocks - job.pb);
+    few = a.pfew;
+  } else {
+    int w = (int)blockIdx.x - a.pjobs;
+    job.tile = w % a.stiles;
+    w /= a.stiles;
+    job.hk = w % a.Hkv;
+    w /= a.Hkv;
+    const int split = w % a.ssplits;
+    job.b0 = w / a.ssplits;
+    job.rows = SG;
+    job.start = __builtin_amdgcn_readfirstlane(row_start(a, job.b0));
+    const int all = (own_end(a, job.start, a.S - 1) + BLK - 1) / BLK;
+    job.own = own_end(a, job.start, min(job.tile * RT + RT - 1, SG - 1) / a.G);
+    const int blocks = (job.own + BLK - 1) / BLK;
+    if (a.fused) {
+      job.npre = pblocks;
+      job.nblk = pblocks + blocks;
+    } else {
+      const int per = own_per(a, all);
+      job.sb = split * per;
+      if (split > 0 && job.sb >= all) return;  // no such split: the joining launch knows
+      job.nblk = max(min(per, blocks - job.sb), 0);
+      job.slot = a.psplits + split;
+    }
+    few = a.sfew;
+  }
+  job.pk = a.pk + job.b0 / a.n * a.pl.b + job.hk * a.pl.h;
+  job.pv = a.pv + job.b0 / a.n * a.pl.b + job.hk * a.pl.h;
+  job.ck = a.ck + job.b0 * a.cl.b + job.hk * a.cl.h;
+  job.cv = a.cv + job.b0 * a.cl.b + job.hk * a.cl.h;
+  if constexpr (NW == 4) {
+    if (few) {
+      if (job.rows <= 16) few_job<T, 1>(a, job, lds, wave, g, r16);
+      else few_job<T, 2>(a, job, lds, wave, g, r16);
+      return;
+    }
+  }
+  tile_job<T, NW>(a, job, lds, wave, g, r16);
+}
+
+// o = sum_j 2^(m_j - M) O_j / sum_j 2^(m_j - M) s_j over a query row's slots: the prefix's splits, then those of its own positions.
+// GR groups of 32 lanes (4 dims a lane) take every GR-th slot each, four loads in flight, and are added in order.
+template <typename T, int GR> __global__ __launch_bounds__(256) void prefix_join_kernel(Args a, int64_t rows) {
+  constexpr int RB = 8 / GR;  // rows a workgroup
+  __shared__ f32x4 part[RB][GR][32];
+  __shared__ float psum[RB][GR];
+  const int l = threadIdx.x & 31, grp = (threadIdx.x >> 5) % GR, rb = (threadIdx.x >> 5) / GR, Hq = a.Hkv * a.G;
+  const int64_t row = min((int64_t)blockIdx.x * RB + rb, rows - 1);
   const int64_t bs = row / Hq;
   const int h = (int)(row - bs * Hq), b = (int)(bs / a.S), s = (int)(bs - (int64_t)b * a.S);
+  const float *pm = a.pm + row * a.slots, *ps = a.ps + row * a.slots, *po = a.po + row * a.slots * D + 4 * l;
   const int start = row_start(a, b), all = (own_end(a, start, a.S - 1) + BLK - 1) / BLK;
   const int per = own_per(a, all);
   const int used = a.psplits + max((all + per - 1) / per, 1);
-  const float *pm = a.pm + row * a.slots, *ps = a.ps + row * a.slots, *po = a.po + row * a.slots * D + 4 * l;
   float M = -INFINITY;
-  for (int j = 0; j < used; ++j) M = __builtin_fmaxf(M, pm[j]);
+  for (int j = l; j < used; j += 32) M = __builtin_fmaxf(M, pm[j]);
+#pragma unroll
+  for (int o = 1; o < 32; o <<= 1) M = __builtin_fmaxf(M, __shfl_xor(M, o, 64));
   float sum = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
-  for (int j = 0; j < used; ++j) {
-    const float w = pm[j] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(pm[j] - M);
-    sum = __builtin_fmaf(w, ps[j], sum);
-    o += w * *reinterpret_cast<const f32x4*>(po + (int64_t)j * D);
+  for (int j0 = grp; j0 < used; j0 += 4 * GR) {
+    f32x4 x[4];
+    float m[4], sj[4];
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int j = min(j0 + k * GR, used - 1);
+      x[k] = *reinterpret_cast<const f32x4*>(po + (int64_t)j * D);
+      m[k] = pm[j];
+      sj[k] = ps[j];
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      if (j0 + k * GR >= used || m[k] == -INFINITY) continue;
+      const float w = __builtin_amdgcn_exp2f(m[k] - M);
+      sum = __builtin_fmaf(w, sj[k], sum);
+      o += w * x[k];
+    }
+  }
+  part[rb][grp][l] = o;
+  if (l == 0) psum[rb][grp] = sum;
+  __syncthreads();
+  if (grp != 0 || (int64_t)blockIdx.x * RB + rb >= rows) return;
+#pragma unroll
+  for (int k = 1; k < GR; ++k) {
+    o += part[rb][k][l];
+    sum += psum[rb][k];
   }
   const float inv = a.P == 0 && own_end(a, start, s) == 0 ? 0.f : 1.f / sum;
   u16* out = a.o + b * a.ol.b + s * a.ol.s + h * a.ol.h + 4 * l;
@@ -394,38 +583,38 @@ int64_t cdiv(int64_t x, int64_t y) { return (x + y - 1) / y; }
 bool al(const void* p, int n) { return ((uintptr_t)p & (n - 1)) == 0; }
 bool lay_ok(const void* p, const Strides& l) { return p && al(p, 16) && l.b % 8 == 0 && l.h % 8 == 0 && l.s % 8 == 0; }
 
-constexpr int kMinPer = 4;  // own blocks of a split at least
-
 // The jobs of a call; span: own positions that the launch has to cover.
 struct Plan {
-  int nw, fused, ptiles, psplits, pper, stiles, ssplits, max_splits, slots;
+  int fused, pfew, ptiles, psplits, pper, sfew, stiles, ssplits, max_splits, min_per, slots;
   int64_t pjobs, sjobs;
 };
 Plan plan_for(int64_t R, int64_t n, int64_t S, int64_t Hkv, int64_t G, int64_t P, int64_t span) {
   Plan p{};
   const int64_t B = R * n, SG = S * G, pblocks = cdiv(P, BLK);
-  auto waves = [](int64_t rows) { return rows <= 32 ? 1 : rows <= 64 ? 2 : rows <= 128 ? 4 : 8; };
   // one pass over everything where a row's own queries fill tiles and the tiles fill the chip
   if (SG >= 128 && B * Hkv * cdiv(SG, 256) >= 192) {
-    p.nw = 8;
-    p.fused = 1;
+    p.fused = p.ptiles = 1;
     p.stiles = (int)cdiv(SG, 256);
-    p.ssplits = p.max_splits = p.slots = 1;
+    p.ssplits = p.max_splits = p.slots = p.min_per = 1;
     p.sjobs = B * Hkv * p.stiles;
     return p;
   }
-  p.nw = waves(P > 0 ? n * SG : SG);
-  const int64_t rt = 32 * p.nw, target = p.nw == 8 ? 256 : 512;
+  constexpr int64_t kJobs = 512;  // two workgroups a CU
+  p.ptiles = 1;
   if (P > 0) {
-    p.ptiles = (int)cdiv(n * SG, rt);
-    const int64_t want = std::max<int64_t>(1, target / (R * Hkv * p.ptiles));
-    p.pper = (int)std::max<int64_t>(cdiv(pblocks, want), 2);
+    p.pfew = n * SG <= 32;
+    p.ptiles = p.pfew ? 1 : (int)cdiv(n * SG, 128);
+    const int64_t want = std::max<int64_t>(1, kJobs / (R * Hkv * p.ptiles));
+    p.pper = (int)std::max<int64_t>(cdiv(pblocks, want), 4);
+    if (p.pfew) p.pper = (p.pper + 3) & ~3;
     p.psplits = (int)cdiv(pblocks, p.pper);
     p.pjobs = R * Hkv * p.ptiles * p.psplits;
   }
-  p.stiles = (int)cdiv(SG, rt);
-  p.max_splits = (int)std::max<int64_t>(1, target / (B * Hkv * p.stiles));
-  p.ssplits = (int)std::max<int64_t>(1, std::min<int64_t>(p.max_splits, cdiv(cdiv(span, BLK), kMinPer)));
+  p.sfew = SG <= 32;
+  p.stiles = p.sfew ? 1 : (int)cdiv(SG, 128);
+  p.min_per = 4;
+  p.max_splits = (int)std::max<int64_t>(1, kJobs / (B * Hkv * p.stiles));
+  p.ssplits = (int)std::max<int64_t>(1, std::min<int64_t>(p.max_splits, cdiv(cdiv(span, BLK), p.min_per)));
   p.sjobs = B * Hkv * p.stiles * p.ssplits;
   p.slots = p.psplits + p.ssplits;
   return p;
@@ -441,15 +630,13 @@ size_t bytes_for(const Plan& p, int64_t rows) {
 
 template <typename T> int run(const Plan& p, const Args& a, int64_t rows, hipStream_t s) {
   const unsigned grid = (unsigned)(p.pjobs + p.sjobs);
-  switch (p.nw) {
-    case 1: prefix_attn_kernel<T, 1><<<grid, 64, 0, s>>>(a); break;
-    case 2: prefix_attn_kernel<T, 2><<<grid, 128, 0, s>>>(a); break;
-    case 4: prefix_attn_kernel<T, 4><<<grid, 256, 0, s>>>(a); break;
-    default: prefix_attn_kernel<T, 8><<<grid, 512, 0, s>>>(a); break;
-  }
+  if (p.fused) prefix_attn_kernel<T, 8><<<grid, 512, 0, s>>>(a);
+  else prefix_attn_kernel<T, 4><<<grid, 256, 0, s>>>(a);
   const int rc = (int)hipGetLastError();
   if (rc != 0 || p.slots == 1) return rc;
-  prefix_join_kernel<T><<<(unsigned)cdiv(rows, 8), 256, 0, s>>>(a, rows);
+  // many slots: a workgroup a row (by what the sizes allow, not by the span: the order of the sums)
+  if (p.psplits + p.max_splits > 8) prefix_join_kernel<T, 8><<<(unsigned)rows, 256, 0, s>>>(a, rows);
+  else prefix_join_kernel<T, 2><<<(unsigned)cdiv(rows, 4), 256, 0, s>>>(a, rows);
   return (int)hipGetLastError();
 }
 
@@ -504,13 +691,15 @@ int q3_prefix_attention(int dtype, const void* q, int64_t qsb, int64_t qss, int6
   a.scale2 = scale * kLog2e;
   a.fused = p.fused;
   a.pjobs = (int)p.pjobs;
+  a.pfew = p.pfew;
+  a.sfew = p.sfew;
   a.ptiles = p.ptiles;
   a.psplits = p.psplits;
   a.pper = p.pper;
   a.stiles = p.stiles;
   a.ssplits = p.ssplits;
   a.max_splits = p.max_splits;
-  a.min_per = kMinPer;
+  a.min_per = p.min_per;
   a.slots = p.slots;
   return dtype == Q3_BF16 ? run<BF16>(p, a, rows, stream) : run<F16>(p, a, rows, stream);
 }
