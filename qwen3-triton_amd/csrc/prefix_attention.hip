@@ -16,6 +16,7 @@
 // Jobs leave unnormalised O, maximum and sum, which a second launch joins in a fixed order.  Where the queries of single rows fill
 // tiles and the tiles the chip, a job goes through the prefix and then its row's own positions, and writes the result.
 #include <algorithm>
+#include <type_traits>
 
 #include "common.h"
 
@@ -45,7 +46,7 @@ struct Args {
   int start_step;  // 0: one start for all rows
   float scale2;    // scale * log2(e)
   // plan
-  int fused, pjobs, pfew, ptiles, psplits, pper, sfew, stiles, ssplits, max_splits, min_per, slots;
+  int fused, pjobs, ptiles, psplits, pper, sfew, stiles, ssplits, max_splits, min_per, slots;
 };
 
 Q3_DEV float xmax4(float x) {  // over lanes {l, l ^ 16, l ^ 32, l ^ 48}
@@ -74,10 +75,27 @@ Q3_DEV int own_per(const Args& a, int blocks) {
   return a.sfew ? (per + 3) & ~3 : per;  // as many for each wave
 }
 
+// Wait until at most `tiles` tiles of L loads each are on their way, and for this wave's LDS reads.
+template <int L> Q3_DEV void loads_left(int tiles) {
+  auto wait = [](auto n) {
+    constexpr int N = decltype(n)::value;
+    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (0 << 8));
+  };
+  switch (tiles) {
+    case 0: wait(std::integral_constant<int, 0>{}); break;
+    case 1: wait(std::integral_constant<int, L>{}); break;
+    case 2: wait(std::integral_constant<int, 2 * L>{}); break;
+    case 3: wait(std::integral_constant<int, 3 * L>{}); break;
+    case 4: wait(std::integral_constant<int, 4 * L>{}); break;
+    default: wait(std::integral_constant<int, 5 * L>{}); break;
+  }
+}
+
 // LDS: K rows of 256 bytes, 16-byte chunk c of row r at c ^ kswz(r); V in 16 slots of 4 rows (keys s, s + 16, s + 32, s + 48)
 // at a pitch of 1056 bytes, which spreads a transpose read over all banks.
 Q3_DEV int kswz(int r) { return (r & 7) | (((r >> 4) & 1) << 3); }
-constexpr int kSlot = 1056, kKTile = BLK * D * 2, kVTile = 16 * kSlot, kStage = kKTile + kVTile;
+constexpr int kSlot = 1056, kKTile = BLK * D * 2, kVTile = 16 * kSlot;
+constexpr int kStages = 4;  // of the rings of K and of V tiles
 
 // Whether both 16-bit halves are finite numbers of type T.
 template <typename T> Q3_DEV bool finite2(uint32_t x) {
@@ -87,6 +105,11 @@ template <typename T> Q3_DEV bool finite2(uint32_t x) {
 template <typename T> Q3_DEV uint32_t only_finite2(uint32_t x) {
   constexpr uint32_t E = T::code == Q3_F16 ? 0x7c00u : 0x7f80u;
   return ((x & E) == E ? 0u : x & 0xffffu) | (((x >> 16) & E) == E ? 0u : x & 0xffff0000u);
+}
+
+// A lane's offset in a V tile of the fragments of key half kc.
+Q3_DEV int value_offset(int g, int r16, int kc) {
+  return (4 * (g & 1) + (r16 >> 2)) * kSlot + (g >> 1) * 256 + 8 * (r16 & 3) + kc * 512;
 }
 
 // A wave's 16 U query rows: operands, O^T (lane: dims 16 dt + 4 g + i of rows 16 u + r16), maxima and sums.
@@ -120,55 +143,76 @@ template <int U> Q3_DEV void load_rows(const Args& a, Rows<U>& w, int m0, int ro
   }
 }
 
-// Scores of a block -> P, with O, maxima and sums brought along.  mask: keys from `end` on (the prefix) or from the row's own
-// limit on (end < 0) are hidden.
-template <typename T, int U>
-Q3_DEV void softmax_block(Rows<U>& w, f32x4 (&S)[4][U], i32x4 (&P)[U][2], float scale2, bool mask, int key0, int end, int g) {
-  if (mask) {
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int rel = (end >= 0 ? end : w.lim[u]) - key0 - group_key(g);
-#pragma unroll
-      for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-        for (int i = 0; i < 4; ++i) S[kt][u][i] = tile_key(kt) + i < rel ? S[kt][u][i] : -INFINITY;
-    }
-  }
-  const float thr = 8.f / scale2;
-  bool any = false;
-  float alpha[U], ms[U];
+// keys from `end` on (the prefix) or from the row's own limit on (end < 0) are hidden
+template <int U> Q3_DEV void mask_block(const Rows<U>& w, f32x4 (&S)[4][U], int key0, int end, int g) {
 #pragma unroll
   for (int u = 0; u < U; ++u) {
-    float x = S[0][u][0];
+    const int rel = (end >= 0 ? end : w.lim[u]) - key0 - group_key(g);
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt)
 #pragma unroll
-      for (int i = 0; i < 4; ++i) x = __builtin_fmaxf(x, S[kt][u][i]);
-    x = xmax4(x);
-    const bool need = x > w.m[u] + thr || w.m[u] == -INFINITY;
-    const float mn = need ? x : w.m[u];
-    alpha[u] = w.m[u] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((w.m[u] - mn) * scale2);
+      for (int i = 0; i < 4; ++i) S[kt][u][i] = tile_key(kt) + i < rel ? S[kt][u][i] : -INFINITY;
+  }
+}
+template <int U> Q3_DEV float row_max(const f32x4 (&S)[4][U], int u) {
+  float x = __builtin_fmaxf(__builtin_fmaxf(S[0][u][0], S[0][u][1]), __builtin_fmaxf(S[0][u][2], S[0][u][3]));
+#pragma unroll
+  for (int kt = 1; kt < 4; ++kt)
+    x = __builtin_fmaxf(__builtin_fmaxf(x, __builtin_fmaxf(S[kt][u][0], S[kt][u][1])), __builtin_fmaxf(S[kt][u][2], S[kt][u][3]));
+  return xmax4(x);
+}
+// The maxima moved where a block's pass them by more than 2^8; O and the sums are to be multiplied by alpha if some row's did.
+template <int U> struct Step {
+  float alpha[U], ms[U];
+  bool moved;
+};
+template <int U> Q3_DEV void move_max(Rows<U>& w, Step<U>& t, const float (&x)[U], float scale2, float thr) {
+  bool any = false;
+#pragma unroll
+  for (int u = 0; u < U; ++u) {
+    const bool need = x[u] > w.m[u] + thr || w.m[u] == -INFINITY;
+    const float mn = need ? x[u] : w.m[u];
+    t.alpha[u] = w.m[u] == -INFINITY ? 1.f : __builtin_amdgcn_exp2f((w.m[u] - mn) * scale2);
     w.m[u] = mn;
-    ms[u] = mn == -INFINITY ? 0.f : mn * scale2;
+    t.ms[u] = mn == -INFINITY ? 0.f : mn * scale2;
     any = any || need;
   }
-  if (__any(any)) {
+  t.moved = __any(any);
+}
+template <int U> Q3_DEV void rescale(Rows<U>& w, const Step<U>& t) {
+  if (!t.moved) return;
 #pragma unroll
-    for (int u = 0; u < U; ++u) {
-      w.l[u] *= alpha[u];
+  for (int u = 0; u < U; ++u) {
+    w.l[u] *= t.alpha[u];
 #pragma unroll
-      for (int dt = 0; dt < 8; ++dt) w.o[dt][u] *= alpha[u];
-    }
+    for (int dt = 0; dt < 8; ++dt) w.o[dt][u] *= t.alpha[u];
   }
+}
+template <int U> Q3_DEV void exp_tile(f32x4 (&S)[4][U], const Step<U>& t, float scale2, int u, int kt) {
+#pragma unroll
+  for (int i = 0; i < 4; ++i) S[kt][u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[kt][u][i], scale2, -t.ms[u]));
+}
+template <typename T, int U> Q3_DEV void pack_block(const f32x4 (&S)[4][U], i32x4 (&P)[U][2]) {
 #pragma unroll
   for (int u = 0; u < U; ++u)
 #pragma unroll
     for (int kt = 0; kt < 4; ++kt) {
-#pragma unroll
-      for (int i = 0; i < 4; ++i) S[kt][u][i] = __builtin_amdgcn_exp2f(__builtin_fmaf(S[kt][u][i], scale2, -ms[u]));
       P[u][kt >> 1][2 * (kt & 1)] = (int)pack2<T>(S[kt][u][0], S[kt][u][1]);
       P[u][kt >> 1][2 * (kt & 1) + 1] = (int)pack2<T>(S[kt][u][2], S[kt][u][3]);
     }
+}
+// Scores of a block -> P and the step that O has to take before it.
+template <typename T, int U>
+Q3_DEV void softmax_block(Rows<U>& w, Step<U>& t, f32x4 (&S)[4][U], i32x4 (&P)[U][2], float scale2, float thr) {
+  float x[U];
+#pragma unroll
+  for (int u = 0; u < U; ++u) x[u] = row_max<U>(S, u);
+  move_max(w, t, x, scale2, thr);
+#pragma unroll
+  for (int u = 0; u < U; ++u)
+#pragma unroll
+    for (int kt = 0; kt < 4; ++kt) exp_tile<U>(S, t, scale2, u, kt);
+  pack_block<T, U>(S, P);
 }
 
 // O^T += V^T P and the sums of P, V's tile at vb.  A value that is not finite would spoil the rows that do not see its position too
@@ -177,9 +221,7 @@ Q3_DEV void softmax_block(Rows<U>& w, f32x4 (&S)[4][U], i32x4 (&P)[U][2], float 
 template <typename T, int U>
 Q3_DEV void value_block(Rows<U>& w, const i32x4 (&P)[U][2], const char* vb, bool look, int key0, int g, int r16) {
   const int lane = 16 * g + r16;
-  int voff[2];
-#pragma unroll
-  for (int kc = 0; kc < 2; ++kc) voff[kc] = (4 * (g & 1) + (r16 >> 2)) * kSlot + (g >> 1) * 256 + 8 * (r16 & 3) + kc * 512;
+  const int voff[2] = {value_offset(g, r16, 0), value_offset(g, r16, 1)};
   bool clean = true;
   if (look) {
     uint32_t ok = 1;
@@ -251,10 +293,12 @@ struct Block {  // one of them: 64 positions from key0 on, `count` of them there
   int64_t st;
   const u16 *k, *v;
 };
+// The prefix's blocks come last first: its unfinished block is the job's first, so blocks with hidden keys are the first and the last ones.
+Q3_DEV int block_key(const Job& job, int j) { return (j < job.npre ? job.pb + job.npre - 1 - j : job.sb + j - job.npre) * BLK; }
 Q3_DEV Block block_of(const Args& a, const Job& job, int j) {
   const bool pre = j < job.npre;
   Block x;
-  x.key0 = (pre ? job.pb + j : job.sb + j - job.npre) * BLK;
+  x.key0 = block_key(job, j);
   x.count = min((pre ? a.P : job.own) - x.key0, BLK);
   x.st = pre ? a.pl.s : a.cl.s;
   x.k = (pre ? job.pk : job.ck) + x.key0 * x.st;
@@ -282,63 +326,174 @@ template <typename T> Q3_DEV void store4(const Args& a, int64_t part, int64_t ou
   }
 }
 
-// More than 32 query rows: 32 a wave.
+// More than 32 query rows: 32 a wave.  Per block j, P(j - 1) V(j - 1) and S(j + 1) = K(j + 1) Q^T run on the matrix cores beside the
+// softmax of S(j): blocks without hidden keys, both neighbours likewise there, in eight fenced steps of 8 products each with the
+// next step's four operand fragments and a part of the softmax (64 rows behind 32768: a block 2950 -> XXXX cycles a wave
+// against one thing after the other).
 template <typename T, int NW> Q3_DEV void tile_job(const Args& a, const Job& job, char* lds, int wave, int g, int r16) {
-  constexpr int RT = 32 * NW;
-  const int m0 = job.tile * RT + wave * 32;
+  constexpr int RT = 32 * NW, ST = kStages, L = 16 / NW;  // L: a wave's loads of a tile
+  char* const kring = lds;
+  char* const vring = lds + ST * kKTile;
+  const int m0 = job.tile * RT + wave * 32, nblk = job.nblk;
   const bool work = m0 < job.rows;  // a wave without rows only loads
   Rows<2> w;
   load_rows(a, w, m0, job.rows, job.b0, job.hk, job.start, g, r16);
   const int lim_w = own_end(a, job.start, min(m0, job.rows - 1) / a.G);  // of the wave's first row, the lowest
 
-  uint32_t krow[16 / NW], kchk[16 / NW], vrow[16 / NW];
+  uint32_t krow[L], kchk[L], vrow[L];
 #pragma unroll
-  for (int i = 0; i < 16 / NW; ++i) {
+  for (int i = 0; i < L; ++i) {
     const int x = wave + NW * i, r = 4 * x + g;
     krow[i] = (uint32_t)r;
     kchk[i] = (uint32_t)((r16 ^ kswz(r)) * 16);
     vrow[i] = (uint32_t)(x + 16 * g);
   }
-  auto issue = [&](int j) {
-    if (j >= job.nblk) return;
+  auto issue_k = [&](int j) {
+    if (j >= nblk) return;
     const Block x = block_of(a, job, j);
     const int bytes = block_bytes(x);
-    char* base = lds + (j & 1) * kStage;
 #pragma unroll
-    for (int i = 0; i < 16 / NW; ++i)
-      buffer_to_lds(x.k, bytes, krow[i] * (uint32_t)(x.st * 2) + kchk[i], base + (wave + NW * i) * 1024);
-#pragma unroll
-    for (int i = 0; i < 16 / NW; ++i)
-      buffer_to_lds(x.v, bytes, vrow[i] * (uint32_t)(x.st * 2) + r16 * 16, base + kKTile + (wave + NW * i) * kSlot);
+    for (int i = 0; i < L; ++i)
+      buffer_to_lds(x.k, bytes, krow[i] * (uint32_t)(x.st * 2) + kchk[i], kring + (j % ST) * kKTile + (wave + NW * i) * 1024);
   };
+  auto issue_v = [&](int j) {
+    if (j < 0 || j >= nblk) return;
+    const Block x = block_of(a, job, j);
+    const int bytes = block_bytes(x);
+#pragma unroll
+    for (int i = 0; i < L; ++i)
+      buffer_to_lds(x.v, bytes, vrow[i] * (uint32_t)(x.st * 2) + r16 * 16, vring + (j % ST) * kVTile + (wave + NW * i) * kSlot);
+  };
+  auto masked = [&](int j) { return block_key(job, j) + BLK > (j < job.npre ? a.P : lim_w); };
+  // The start of block j: K(j + 1) and V(j - 1), both issued ST - 1 starts before, are there; what left its stage in block j - 1
+  // is refilled.  `younger` loads of tiles may still be on their way.
+  auto sync = [&](int younger) {
+    loads_left<L>(younger);
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();
+    asm volatile("" ::: "memory");
+  };
+  auto top = [&](int j) {
+    sync(max(min(j + ST - 1, nblk - 1) - (j + 1), 0) + max(min(j + ST - 3, nblk - 1) - (j - 1), 0));
+    issue_k(j + ST);
+    issue_v(j + ST - 2);
+  };
+  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
+  const uint32_t one2 = pack2<T>(1.f, 1.f);
+  const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, i32x4{(int)one2, (int)one2, (int)one2, (int)one2});
+  const float thr = 8.f / a.scale2;
   int koff[4];
 #pragma unroll
   for (int ks = 0; ks < 4; ++ks) koff[ks] = row_key(r16) * 256 + (((4 * ks + g) ^ r16) << 4);
-
-  issue(0);
-  for (int j = 0; j < job.nblk; ++j) {
-    __builtin_amdgcn_s_waitcnt((0 & 15) | (7 << 4) | (0 << 8));  // vmcnt(0) lgkmcnt(0)
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();  // block j is there, and every wave is done with block j - 1
-    asm volatile("" ::: "memory");
-    issue(j + 1);
-    if (!work) continue;
-    const char* kb = lds + (j & 1) * kStage;
-    const Block x = block_of(a, job, j);
-    f32x4 S[4][2];
+  const int voff[2] = {value_offset(g, r16, 0), value_offset(g, r16, 1)};
+  f32x4 S[4][2];
+  i32x4 P[2][2];
+  Step<2> step;
+  step.moved = false;
+  auto frag = [](i32x4 x) { return __builtin_bit_cast(bf16x8_t, x); };
+  auto scores = [&](int j) {
+    const char* kb = kring + (j % ST) * kKTile;
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt) {
         const bf16x8_t kf = *reinterpret_cast<const bf16x8_t*>(kb + koff[ks] + tile_key(kt) * 256);
 #pragma unroll
-        for (int u = 0; u < 2; ++u)
-          S[kt][u] = mfma_16x16x32<T>(kf, w.qf[u][ks], ks == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : S[kt][u]);
+        for (int u = 0; u < 2; ++u) S[kt][u] = mfma_16x16x32<T>(kf, w.qf[u][ks], ks == 0 ? zero : S[kt][u]);
       }
-    const bool pre = j < job.npre, mask = block_masked(a, job, j, x, lim_w);
-    i32x4 P[2][2];
-    softmax_block<T, 2>(w, S, P, a.scale2, mask, x.key0, pre ? a.P : -1, g);
-    value_block<T, 2>(w, P, kb + kKTile, mask && !pre && a.S > 1, x.key0, g, r16);
+  };
+  auto values = [&](int j) {
+    rescale(w, step);
+    const bool pre = j < job.npre;
+    value_block<T, 2>(w, P, vring + (j % ST) * kVTile, !pre && a.S > 1 && masked(j), block_key(job, j), g, r16);
+  };
+  auto generic = [&](int j) {
+    if (j > 0) values(j - 1);
+    if (masked(j)) {
+      mask_block<2>(w, S, block_key(job, j), j < job.npre ? a.P : -1, g);
+    }
+    softmax_block<T, 2>(w, step, S, P, a.scale2, thr);
+    if (j + 1 < nblk) scores(j + 1);
+  };
+  auto pipelined = [&](int j) {
+    const char* vb = vring + ((j - 1) % ST) * kVTile;
+    const char* kb = kring + ((j + 1) % ST) * kKTile;
+    auto fetch = [&](int st, i32x4 (&F)[4]) {
+      if (st < 4) {
+#pragma unroll
+        for (int dd = 0; dd < 2; ++dd)
+#pragma unroll
+          for (int kc = 0; kc < 2; ++kc) F[2 * dd + kc] = lds_frag_tr(vb + voff[kc] + (2 * st + dd) * 32, 8 * kSlot);
+      } else {
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt) F[kt] = *reinterpret_cast<const i32x4*>(kb + koff[st - 4] + tile_key(kt) * 256);
+      }
+    };
+    i32x4 F[2][4];
+    fetch(0, F[0]);
+#pragma unroll
+    for (int st = 0; st < 8; ++st) {
+      i32x4(&f)[4] = F[st & 1];
+      if (st + 1 < 8) fetch(st + 1, F[(st + 1) & 1]);
+      if (st == 0) {
+        const float x[2] = {row_max<2>(S, 0), row_max<2>(S, 1)};
+        move_max(w, step, x, a.scale2, thr);
+      } else if (st == 1) {
+        exp_tile<2>(S, step, a.scale2, 0, 0), exp_tile<2>(S, step, a.scale2, 0, 1), exp_tile<2>(S, step, a.scale2, 0, 2);
+      } else if (st == 2) {
+        exp_tile<2>(S, step, a.scale2, 0, 3), exp_tile<2>(S, step, a.scale2, 1, 0), exp_tile<2>(S, step, a.scale2, 1, 1);
+      } else if (st == 3) {
+        exp_tile<2>(S, step, a.scale2, 1, 2), exp_tile<2>(S, step, a.scale2, 1, 3);
+      }
+      if (st < 4) {
+#pragma unroll
+        for (int dd = 0; dd < 2; ++dd)
+#pragma unroll
+          for (int kc = 0; kc < 2; ++kc)
+#pragma unroll
+            for (int u = 0; u < 2; ++u)
+              w.o[2 * st + dd][u] = mfma_16x16x32<T>(frag(f[2 * dd + kc]), frag(P[u][kc]), w.o[2 * st + dd][u]);
+        w.l[st >> 1] = mfma_16x16x32<T>(ones, frag(P[st >> 1][st & 1]), w.l[st >> 1]);
+      } else {
+        if (st == 4) pack_block<T, 2>(S, P);
+#pragma unroll
+        for (int kt = 0; kt < 4; ++kt)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) S[kt][u] = mfma_16x16x32<T>(frag(f[kt]), w.qf[u][st - 4], st == 4 ? zero : S[kt][u]);
+      }
+      __builtin_amdgcn_sched_barrier(0);
+    }
+  };
+
+  if (nblk > 0) {
+#pragma unroll
+    for (int j = 0; j < ST; ++j) {
+      issue_k(j);
+      issue_v(j - 2);
+    }
+    sync(min(ST, nblk) - 1 + min(ST - 2, nblk));
+    if (work) {
+      scores(0);
+      // From the second block on to the first with hidden keys, in a loop of its own (one body for both kinds costs registers).
+      const int hidden = lim_w / BLK - job.sb + job.npre;  // the first own block with hidden keys
+      const int full = max(1, min(hidden, nblk - 1));
+      top(0);
+      generic(0);
+      int j = 1;
+      for (; j < full; ++j) {
+        top(j);
+        rescale(w, step);
+        pipelined(j);
+      }
+      for (; j < nblk; ++j) {
+        top(j);
+        generic(j);
+      }
+    } else {
+      for (int j = 0; j < nblk; ++j) top(j);
+    }
+    sync(0);
+    if (work) values(nblk - 1);
   }
 
 #pragma unroll
@@ -359,6 +514,8 @@ template <typename T, int NW> Q3_DEV void tile_job(const Args& a, const Job& job
 
 // Up to 16 U query rows: each wave takes every fourth block.
 template <typename T, int U> Q3_DEV void few_job(const Args& a, const Job& job, char* lds, int wave, int g, int r16) {
+  // 16 rows: the next K on its way beside the softmax and V's product; 32 have no registers for it.
+  constexpr bool EARLY = U == 1;
   constexpr int NW = 4, R = 16 * U;
   char* const vt = lds + wave * kVTile;
   Rows<U> w;
@@ -402,20 +559,24 @@ template <typename T, int U> Q3_DEV void few_job(const Args& a, const Job& job, 
           S[kt][u] = mfma_16x16x32<T>(__builtin_bit_cast(bf16x8_t, kf[kt][ks]), w.qf[u][ks], ks == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : S[kt][u]);
     const bool more = j + NW < job.nblk;
     fence();
-    if (more) load_k(j + NW);
+    if (EARLY && more) load_k(j + NW);
     fence();
     const bool pre = j < job.npre, mask = block_masked(a, job, j, x, lim_w);
     i32x4 P[U][2];
-    softmax_block<T, U>(w, S, P, a.scale2, mask, x.key0, pre ? a.P : -1, g);
+    Step<U> step;
+    if (mask) mask_block<U>(w, S, x.key0, pre ? a.P : -1, g);
+    softmax_block<T, U>(w, step, S, P, a.scale2, 8.f / a.scale2);
+    rescale(w, step);
     // this block's V: everything older than the next K's 16 loads
     fence();
-    if (more) __builtin_amdgcn_s_waitcnt((16 & 15) | ((16 >> 4) << 14) | (7 << 4) | (15 << 8));
+    if (EARLY && more) __builtin_amdgcn_s_waitcnt((16 & 15) | ((16 >> 4) << 14) | (7 << 4) | (15 << 8));
     else __builtin_amdgcn_s_waitcnt((0 & 15) | (7 << 4) | (15 << 8));
     fence();
     value_block<T, U>(w, P, vt, mask && !pre && a.S > 1, x.key0, g, r16);
     if (more) {
       __builtin_amdgcn_s_waitcnt((15) | (3 << 14) | (7 << 4) | (0 << 8));  // the tile is read
       fence();
+      if (!EARLY) load_k(j + NW);
       load_v(j + NW);
     }
   }
@@ -423,7 +584,7 @@ template <typename T, int U> Q3_DEV void few_job(const Args& a, const Job& job, 
   __builtin_amdgcn_s_waitcnt((15) | (3 << 14) | (7 << 4) | (0 << 8));
   fence();
   constexpr int kRow = D * 4 + 16;  // 16 bytes of padding a row
-  static_assert(R * kRow + 8 * R <= kVTile + 8 * 32, "fits the tile with its end");
+  static_assert(R * kRow <= kVTile, "fits the wave's tile");
   float* const stat = (float*)(lds + NW * kVTile);  // [wave][2][R]
 #pragma unroll
   for (int u = 0; u < U; ++u) {
@@ -459,71 +620,76 @@ template <typename T, int U> Q3_DEV void few_job(const Args& a, const Job& job, 
   }
 }
 
-constexpr int kFewLds = 4 * kVTile + 4 * 2 * 32 * 4;
-
-template <typename T, int NW>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefix_attn_kernel(Args a) {
-  constexpr int kLds = NW == 4 && kFewLds > 2 * kStage ? kFewLds : 2 * kStage;
-  __shared__ __attribute__((aligned(1024))) char lds[kLds];
-  constexpr int RT = 32 * NW;  // query rows of a tile
-  const int tid = threadIdx.x, g = (tid & 63) >> 4, r16 = tid & 15;
-  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  const int SG = a.S * a.G, pblocks = (a.P + BLK - 1) / BLK;
-
-  Job job{};
-  bool few;
-  if ((int)blockIdx.x < a.pjobs) {
-    // each XCD (workgroup ids congruent mod 8) takes a contiguous range of jobs, row tiles innermost: the tiles that read the
-    // same keys share an L2
-    const int xcd = blockIdx.x & 7, per = a.pjobs >> 3, rem = a.pjobs & 7;
-    int w = xcd * per + min(xcd, rem) + ((int)blockIdx.x >> 3);
-    job.tile = w % a.ptiles;
-    w /= a.ptiles;
-    job.slot = w % a.psplits;
-    w /= a.psplits;
-    job.hk = w % a.Hkv;
-    job.b0 = w / a.Hkv * a.n;
-    job.rows = a.n * SG;
-    job.pb = job.slot * a.pper;
-    job.npre = job.nblk = min(a.pper, pblocks - job.pb);
-    few = a.pfew;
-  } else {
-    int w = (int)blockIdx.x - a.pjobs;
-    job.tile = w % a.stiles;
-    w /= a.stiles;
-    job.hk = w % a.Hkv;
-    w /= a.Hkv;
-    const int split = w % a.ssplits;
-    job.b0 = w / a.ssplits;
-    job.rows = SG;
-    job.start = __builtin_amdgcn_readfirstlane(row_start(a, job.b0));
-    const int all = (own_end(a, job.start, a.S - 1) + BLK - 1) / BLK;
-    job.own = own_end(a, job.start, min(job.tile * RT + RT - 1, SG - 1) / a.G);
-    const int blocks = (job.own + BLK - 1) / BLK;
-    if (a.fused) {
-      job.npre = pblocks;
-      job.nblk = pblocks + blocks;
-    } else {
-      const int per = own_per(a, all);
-      job.sb = split * per;
-      if (split > 0 && job.sb >= all) return;  // no such split: the joining launch knows
-      job.nblk = max(min(per, blocks - job.sb), 0);
-      job.slot = a.psplits + split;
-    }
-    few = a.sfew;
-  }
+// Pointers to a job's keys and values.
+Q3_DEV void job_pointers(const Args& a, Job& job) {
   job.pk = a.pk + job.b0 / a.n * a.pl.b + job.hk * a.pl.h;
   job.pv = a.pv + job.b0 / a.n * a.pl.b + job.hk * a.pl.h;
   job.ck = a.ck + job.b0 * a.cl.b + job.hk * a.cl.h;
   job.cv = a.cv + job.b0 * a.cl.b + job.hk * a.cl.h;
-  if constexpr (NW == 4) {
-    if (few) {
-      if (job.rows <= 16) few_job<T, 1>(a, job, lds, wave, g, r16);
-      else few_job<T, 2>(a, job, lds, wave, g, r16);
-      return;
-    }
+}
+// Job w of the prefix: row tiles innermost.
+Q3_DEV void prefix_job(const Args& a, Job& job, int w) {
+  job.tile = w % a.ptiles;
+  w /= a.ptiles;
+  job.slot = w % a.psplits;
+  w /= a.psplits;
+  job.hk = w % a.Hkv;
+  job.b0 = w / a.Hkv * a.n;
+  job.rows = a.n * a.S * a.G;
+  job.pb = job.slot * a.pper;
+  job.npre = job.nblk = min(a.pper, (a.P + BLK - 1) / BLK - job.pb);
+}
+// Job w of the rows' own positions, with tiles of RT query rows; false: there is no such split (the joining launch knows).
+Q3_DEV bool own_job(const Args& a, Job& job, int w, int RT) {
+  const int SG = a.S * a.G;
+  job.tile = w % a.stiles;
+  w /= a.stiles;
+  job.hk = w % a.Hkv;
+  w /= a.Hkv;
+  const int split = w % a.ssplits;
+  job.b0 = w / a.ssplits;
+  job.rows = SG;
+  job.start = __builtin_amdgcn_readfirstlane(row_start(a, job.b0));
+  const int all = (own_end(a, job.start, a.S - 1) + BLK - 1) / BLK;
+  job.own = own_end(a, job.start, min(job.tile * RT + RT - 1, SG - 1) / a.G);
+  const int blocks = (job.own + BLK - 1) / BLK;
+  if (a.fused) {
+    job.npre = (a.P + BLK - 1) / BLK;
+    job.nblk = job.npre + blocks;
+    return true;
   }
-  tile_job<T, NW>(a, job, lds, wave, g, r16);
+  const int per = own_per(a, all);
+  job.sb = split * per;
+  job.nblk = max(min(per, blocks - job.sb), 0);
+  job.slot = a.psplits + split;
+  return split == 0 || job.sb < all;
+}
+
+// 4 waves: one a SIMD, with all of its registers.
+template <typename T, int NW>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4, NW / 4))) void prefix_tile_kernel(Args a) {
+  __shared__ __attribute__((aligned(1024))) char lds[kStages * (kKTile + kVTile)];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  Job job{};
+  if ((int)blockIdx.x < a.pjobs) {
+    // each XCD (workgroup ids congruent mod 8) takes a contiguous range of jobs: the tiles that read the same keys share an L2
+    const int xcd = blockIdx.x & 7, per = a.pjobs >> 3, rem = a.pjobs & 7;
+    prefix_job(a, job, xcd * per + min(xcd, rem) + ((int)blockIdx.x >> 3));
+  } else if (!own_job(a, job, (int)blockIdx.x - a.pjobs, 32 * NW)) {
+    return;
+  }
+  job_pointers(a, job);
+  tile_job<T, NW>(a, job, lds, wave, (tid & 63) >> 4, tid & 15);
+}
+
+template <typename T, int U> __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefix_few_kernel(Args a) {
+  __shared__ __attribute__((aligned(1024))) char lds[4 * kVTile + 4 * 2 * 16 * U * 4];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  Job job{};
+  if ((int)blockIdx.x < a.pjobs) prefix_job(a, job, blockIdx.x);
+  else if (!own_job(a, job, (int)blockIdx.x - a.pjobs, 32)) return;
+  job_pointers(a, job);
+  few_job<T, U>(a, job, lds, wave, (tid & 63) >> 4, tid & 15);
 }
 
 // o = sum_j 2^(m_j - M) O_j / sum_j 2^(m_j - M) s_j over a query row's slots: the prefix's splits, then those of its own positions.
@@ -583,38 +749,42 @@ int64_t cdiv(int64_t x, int64_t y) { return (x + y - 1) / y; }
 bool al(const void* p, int n) { return ((uintptr_t)p & (n - 1)) == 0; }
 bool lay_ok(const void* p, const Strides& l) { return p && al(p, 16) && l.b % 8 == 0 && l.h % 8 == 0 && l.s % 8 == 0; }
 
-// The jobs of a call; span: own positions that the launch has to cover.
+// The jobs of a call; span: own positions that the launches have to cover.
 struct Plan {
-  int fused, pfew, ptiles, psplits, pper, sfew, stiles, ssplits, max_splits, min_per, slots;
+  int fused, pfew, sfew, nw, ptiles, psplits, pper, stiles, ssplits, max_splits, slots;
   int64_t pjobs, sjobs;
 };
+constexpr int kMinPer = 4;  // blocks of a split at least
 Plan plan_for(int64_t R, int64_t n, int64_t S, int64_t Hkv, int64_t G, int64_t P, int64_t span) {
   Plan p{};
   const int64_t B = R * n, SG = S * G, pblocks = cdiv(P, BLK);
   // one pass over everything where a row's own queries fill tiles and the tiles fill the chip
   if (SG >= 128 && B * Hkv * cdiv(SG, 256) >= 192) {
     p.fused = p.ptiles = 1;
+    p.nw = 8;
     p.stiles = (int)cdiv(SG, 256);
-    p.ssplits = p.max_splits = p.slots = p.min_per = 1;
+    p.ssplits = p.max_splits = p.slots = 1;
     p.sjobs = B * Hkv * p.stiles;
     return p;
   }
-  constexpr int64_t kJobs = 512;  // two workgroups a CU
+  // Jobs of few rows: two workgroups a CU; of tiles: one.  Where both kinds of positions are in one launch, half of it each.
+  p.pfew = P > 0 && n * SG <= 32;
+  p.sfew = SG <= 32;
+  p.nw = (P > 0 ? n * SG : SG) <= 128 ? 4 : 8;
+  const bool both = P > 0 && p.pfew == p.sfew;
+  const int64_t tile_jobs = 256, few_jobs = 512;
   p.ptiles = 1;
   if (P > 0) {
-    p.pfew = n * SG <= 32;
-    p.ptiles = p.pfew ? 1 : (int)cdiv(n * SG, 128);
-    const int64_t want = std::max<int64_t>(1, kJobs / (R * Hkv * p.ptiles));
-    p.pper = (int)std::max<int64_t>(cdiv(pblocks, want), 4);
+    p.ptiles = p.pfew ? 1 : (int)cdiv(n * SG, 32 * p.nw);
+    const int64_t want = std::max<int64_t>(1, (p.pfew ? few_jobs / 2 : tile_jobs) / (R * Hkv * p.ptiles));
+    p.pper = (int)std::max<int64_t>(cdiv(pblocks, want), kMinPer);
     if (p.pfew) p.pper = (p.pper + 3) & ~3;
     p.psplits = (int)cdiv(pblocks, p.pper);
     p.pjobs = R * Hkv * p.ptiles * p.psplits;
   }
-  p.sfew = SG <= 32;
-  p.stiles = p.sfew ? 1 : (int)cdiv(SG, 128);
-  p.min_per = 4;
-  p.max_splits = (int)std::max<int64_t>(1, kJobs / (B * Hkv * p.stiles));
-  p.ssplits = (int)std::max<int64_t>(1, std::min<int64_t>(p.max_splits, cdiv(cdiv(span, BLK), p.min_per)));
+  p.stiles = p.sfew ? 1 : (int)cdiv(SG, 32 * p.nw);
+  p.max_splits = (int)std::max<int64_t>(1, (p.sfew ? few_jobs : tile_jobs) / (both ? 2 : 1) / (B * Hkv * p.stiles));
+  p.ssplits = (int)std::max<int64_t>(1, std::min<int64_t>(p.max_splits, cdiv(cdiv(span, BLK), kMinPer)));
   p.sjobs = B * Hkv * p.stiles * p.ssplits;
   p.slots = p.psplits + p.ssplits;
   return p;
@@ -628,12 +798,25 @@ size_t bytes_for(const Plan& p, int64_t rows) {
   return p.slots == 1 ? 0 : (size_t)rows * p.slots * (D + 2) * sizeof(float);
 }
 
-template <typename T> int run(const Plan& p, const Args& a, int64_t rows, hipStream_t s) {
-  const unsigned grid = (unsigned)(p.pjobs + p.sjobs);
-  if (p.fused) prefix_attn_kernel<T, 8><<<grid, 512, 0, s>>>(a);
-  else prefix_attn_kernel<T, 4><<<grid, 256, 0, s>>>(a);
-  const int rc = (int)hipGetLastError();
-  if (rc != 0 || p.slots == 1) return rc;
+template <typename T> int run(const Plan& p, Args a, int64_t rows, hipStream_t s) {
+  // the jobs of tiles, then those of few rows
+  const int64_t tp = p.pfew ? 0 : p.pjobs, ts = p.sfew ? 0 : p.sjobs;
+  int rc = 0;
+  if (tp + ts > 0) {
+    a.pjobs = (int)tp;
+    if (p.nw == 8) prefix_tile_kernel<T, 8><<<(unsigned)(tp + ts), 512, 0, s>>>(a);
+    else prefix_tile_kernel<T, 4><<<(unsigned)(tp + ts), 256, 0, s>>>(a);
+    if ((rc = (int)hipGetLastError()) != 0) return rc;
+  }
+  const int64_t fp = p.pjobs - tp, fs = p.sjobs - ts;
+  if (fp + fs > 0) {
+    a.pjobs = (int)fp;
+    const int most = (fp > 0 ? a.n : 1) * a.S * a.G;
+    if (most <= 16) prefix_few_kernel<T, 1><<<(unsigned)(fp + fs), 256, 0, s>>>(a);
+    else prefix_few_kernel<T, 2><<<(unsigned)(fp + fs), 256, 0, s>>>(a);
+    if ((rc = (int)hipGetLastError()) != 0) return rc;
+  }
+  if (p.slots == 1) return rc;
   // many slots: a workgroup a row (by what the sizes allow, not by the span: the order of the sums)
   if (p.psplits + p.max_splits > 8) prefix_join_kernel<T, 8><<<(unsigned)rows, 256, 0, s>>>(a, rows);
   else prefix_join_kernel<T, 2><<<(unsigned)cdiv(rows, 4), 256, 0, s>>>(a, rows);
@@ -690,8 +873,6 @@ int q3_prefix_attention(int dtype, const void* q, int64_t qsb, int64_t qss, int6
   a.start_step = start_dev && starts == B && B > 1 ? 1 : 0;
   a.scale2 = scale * kLog2e;
   a.fused = p.fused;
-  a.pjobs = (int)p.pjobs;
-  a.pfew = p.pfew;
   a.sfew = p.sfew;
   a.ptiles = p.ptiles;
   a.psplits = p.psplits;
@@ -699,7 +880,7 @@ int q3_prefix_attention(int dtype, const void* q, int64_t qsb, int64_t qss, int6
   a.stiles = p.stiles;
   a.ssplits = p.ssplits;
   a.max_splits = p.max_splits;
-  a.min_per = p.min_per;
+  a.min_per = kMinPer;
   a.slots = p.slots;
   return dtype == Q3_BF16 ? run<BF16>(p, a, rows, stream) : run<F16>(p, a, rows, stream);
 }
