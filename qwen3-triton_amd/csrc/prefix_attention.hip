@@ -46,7 +46,7 @@ struct Args {
   int start_step;  // 0: one start for all rows
   float scale2;    // scale * log2(e)
   // plan
-  int fused, pjobs, ptiles, psplits, pper, sfew, stiles, ssplits, max_splits, min_per, slots;
+  int fused, pjobs, sjobs, ptiles, psplits, pper, sfew, stiles, ssplits, max_splits, min_per, slots;
 };
 
 Q3_DEV float xmax4(float x) {  // over lanes {l, l ^ 16, l ^ 32, l ^ 48}
@@ -75,27 +75,10 @@ Q3_DEV int own_per(const Args& a, int blocks) {
   return a.sfew ? (per + 3) & ~3 : per;  // as many for each wave
 }
 
-// Wait until at most `tiles` tiles of L loads each are on their way, and for this wave's LDS reads.
-template <int L> Q3_DEV void loads_left(int tiles) {
-  auto wait = [](auto n) {
-    constexpr int N = decltype(n)::value;
-    __builtin_amdgcn_s_waitcnt((N & 15) | ((N >> 4) << 14) | (7 << 4) | (0 << 8));
-  };
-  switch (tiles) {
-    case 0: wait(std::integral_constant<int, 0>{}); break;
-    case 1: wait(std::integral_constant<int, L>{}); break;
-    case 2: wait(std::integral_constant<int, 2 * L>{}); break;
-    case 3: wait(std::integral_constant<int, 3 * L>{}); break;
-    case 4: wait(std::integral_constant<int, 4 * L>{}); break;
-    default: wait(std::integral_constant<int, 5 * L>{}); break;
-  }
-}
-
 // LDS: K rows of 256 bytes, 16-byte chunk c of row r at c ^ kswz(r); V in 16 slots of 4 rows (keys s, s + 16, s + 32, s + 48)
 // at a pitch of 1056 bytes, which spreads a transpose read over all banks.
 Q3_DEV int kswz(int r) { return (r & 7) | (((r >> 4) & 1) << 3); }
-constexpr int kSlot = 1056, kKTile = BLK * D * 2, kVTile = 16 * kSlot;
-constexpr int kStages = 4;  // of the rings of K and of V tiles
+constexpr int kSlot = 1056, kKTile = BLK * D * 2, kVTile = 16 * kSlot, kStage = kKTile + kVTile;
 
 // Whether both 16-bit halves are finite numbers of type T.
 template <typename T> Q3_DEV bool finite2(uint32_t x) {
@@ -216,14 +199,15 @@ Q3_DEV void softmax_block(Rows<U>& w, Step<U>& t, f32x4 (&S)[4][U], i32x4 (&P)[U
 }
 
 // O^T += V^T P and the sums of P, V's tile at vb.  A value that is not finite would spoil the rows that do not see its position too
-// (0 times it is NaN): blocks that some row sees in part (look) are looked through first, and then such values are kept out of
-// the product and added to the rows that do see them.
-template <typename T, int U>
-Q3_DEV void value_block(Rows<U>& w, const i32x4 (&P)[U][2], const char* vb, bool look, int key0, int g, int r16) {
+// (0 times it is NaN): blocks that some row sees in part (LOOK; the last of a job, in a loop of their own, since the second way
+// through the product costs copies of O) are looked through first, and then such values are kept out of the product and
+// added to the rows that do see them.
+template <typename T, int U, bool LOOK>
+Q3_DEV void value_block(Rows<U>& w, const i32x4 (&P)[U][2], const char* vb, int key0, int g, int r16) {
   const int lane = 16 * g + r16;
   const int voff[2] = {value_offset(g, r16, 0), value_offset(g, r16, 1)};
   bool clean = true;
-  if (look) {
+  if constexpr (LOOK) {
     uint32_t ok = 1;
 #pragma unroll 4
     for (int i = 0; i < 16; ++i) {
@@ -306,8 +290,10 @@ Q3_DEV Block block_of(const Args& a, const Job& job, int j) {
   return x;
 }
 Q3_DEV int block_bytes(const Block& x) { return (x.count - 1) * (int)x.st * 2 + 2 * D; }
-Q3_DEV bool block_masked(const Args& a, const Job& job, int j, const Block& x, int lim) {
-  return x.key0 + BLK > (j < job.npre ? a.P : lim);
+// The first of a job's blocks that queries of a wave see in part while others of it see it whole; lim: own positions that its first
+// row sees.  One query a row sees all that is there.
+Q3_DEV int first_partial(const Args& a, const Job& job, int lim) {
+  return a.S == 1 ? job.nblk : min(max(lim / BLK - job.sb, 0) + job.npre, job.nblk);
 }
 
 // A query row's place among the partials, and in the output.
@@ -326,14 +312,9 @@ template <typename T> Q3_DEV void store4(const Args& a, int64_t part, int64_t ou
   }
 }
 
-// More than 32 query rows: 32 a wave.  Per block j, P(j - 1) V(j - 1) and S(j + 1) = K(j + 1) Q^T run on the matrix cores beside the
-// softmax of S(j): blocks without hidden keys, both neighbours likewise there, in eight fenced steps of 8 products each with the
-// next step's four operand fragments and a part of the softmax (64 rows behind 32768: a block 2950 -> XXXX cycles a wave
-// against one thing after the other).
+// More than 32 query rows: 32 a wave.
 template <typename T, int NW> Q3_DEV void tile_job(const Args& a, const Job& job, char* lds, int wave, int g, int r16) {
-  constexpr int RT = 32 * NW, ST = kStages, L = 16 / NW;  // L: a wave's loads of a tile
-  char* const kring = lds;
-  char* const vring = lds + ST * kKTile;
+  constexpr int RT = 32 * NW, L = 16 / NW;  // L: a wave's loads of a tile
   const int m0 = job.tile * RT + wave * 32, nblk = job.nblk;
   const bool work = m0 < job.rows;  // a wave without rows only loads
   Rows<2> w;
@@ -348,153 +329,55 @@ template <typename T, int NW> Q3_DEV void tile_job(const Args& a, const Job& job
     kchk[i] = (uint32_t)((r16 ^ kswz(r)) * 16);
     vrow[i] = (uint32_t)(x + 16 * g);
   }
-  auto issue_k = [&](int j) {
+  auto issue = [&](int j) {
     if (j >= nblk) return;
     const Block x = block_of(a, job, j);
     const int bytes = block_bytes(x);
+    char* base = lds + (j & 1) * kStage;
 #pragma unroll
     for (int i = 0; i < L; ++i)
-      buffer_to_lds(x.k, bytes, krow[i] * (uint32_t)(x.st * 2) + kchk[i], kring + (j % ST) * kKTile + (wave + NW * i) * 1024);
-  };
-  auto issue_v = [&](int j) {
-    if (j < 0 || j >= nblk) return;
-    const Block x = block_of(a, job, j);
-    const int bytes = block_bytes(x);
+      buffer_to_lds(x.k, bytes, krow[i] * (uint32_t)(x.st * 2) + kchk[i], base + (wave + NW * i) * 1024);
 #pragma unroll
     for (int i = 0; i < L; ++i)
-      buffer_to_lds(x.v, bytes, vrow[i] * (uint32_t)(x.st * 2) + r16 * 16, vring + (j % ST) * kVTile + (wave + NW * i) * kSlot);
+      buffer_to_lds(x.v, bytes, vrow[i] * (uint32_t)(x.st * 2) + r16 * 16, base + kKTile + (wave + NW * i) * kSlot);
   };
-  auto masked = [&](int j) { return block_key(job, j) + BLK > (j < job.npre ? a.P : lim_w); };
-  // The start of block j: K(j + 1) and V(j - 1), both issued ST - 1 starts before, are there; what left its stage in block j - 1
-  // is refilled.  `younger` loads of tiles may still be on their way.
-  auto sync = [&](int younger) {
-    loads_left<L>(younger);
-    asm volatile("" ::: "memory");
-    __builtin_amdgcn_s_barrier();
-    asm volatile("" ::: "memory");
-  };
-  auto top = [&](int j) {
-    sync(max(min(j + ST - 1, nblk - 1) - (j + 1), 0) + max(min(j + ST - 3, nblk - 1) - (j - 1), 0));
-    issue_k(j + ST);
-    issue_v(j + ST - 2);
-  };
-  const f32x4 zero = {0.f, 0.f, 0.f, 0.f};
-  const uint32_t one2 = pack2<T>(1.f, 1.f);
-  const bf16x8_t ones = __builtin_bit_cast(bf16x8_t, i32x4{(int)one2, (int)one2, (int)one2, (int)one2});
-  const float thr = 8.f / a.scale2;
   int koff[4];
 #pragma unroll
   for (int ks = 0; ks < 4; ++ks) koff[ks] = row_key(r16) * 256 + (((4 * ks + g) ^ r16) << 4);
-  const int voff[2] = {value_offset(g, r16, 0), value_offset(g, r16, 1)};
-  f32x4 S[4][2];
-  i32x4 P[2][2];
-  Step<2> step;
-  step.moved = false;
-  auto frag = [](i32x4 x) { return __builtin_bit_cast(bf16x8_t, x); };
-  auto scores = [&](int j) {
-    const char* kb = kring + (j % ST) * kKTile;
+  const float thr = 8.f / a.scale2;
+
+  auto block = [&](int j, auto look) {
+    __builtin_amdgcn_s_waitcnt((0 & 15) | (7 << 4) | (0 << 8));  // vmcnt(0) lgkmcnt(0)
+    asm volatile("" ::: "memory");
+    __builtin_amdgcn_s_barrier();  // block j is there, and every wave is done with block j - 1
+    asm volatile("" ::: "memory");
+    issue(j + 1);
+    if (!work) return;
+    const char* kb = lds + (j & 1) * kStage;
+    f32x4 S[4][2];
 #pragma unroll
     for (int ks = 0; ks < 4; ++ks)
 #pragma unroll
       for (int kt = 0; kt < 4; ++kt) {
         const bf16x8_t kf = *reinterpret_cast<const bf16x8_t*>(kb + koff[ks] + tile_key(kt) * 256);
 #pragma unroll
-        for (int u = 0; u < 2; ++u) S[kt][u] = mfma_16x16x32<T>(kf, w.qf[u][ks], ks == 0 ? zero : S[kt][u]);
+        for (int u = 0; u < 2; ++u)
+          S[kt][u] = mfma_16x16x32<T>(kf, w.qf[u][ks], ks == 0 ? f32x4{0.f, 0.f, 0.f, 0.f} : S[kt][u]);
       }
-  };
-  auto values = [&](int j) {
-    rescale(w, step);
     const bool pre = j < job.npre;
-    value_block<T, 2>(w, P, vring + (j % ST) * kVTile, !pre && a.S > 1 && masked(j), block_key(job, j), g, r16);
-  };
-  auto generic = [&](int j) {
-    if (j > 0) values(j - 1);
-    if (masked(j)) {
-      mask_block<2>(w, S, block_key(job, j), j < job.npre ? a.P : -1, g);
-    }
+    const int key0 = block_key(job, j);
+    const bool mask = key0 + BLK > (pre ? a.P : lim_w);
+    if (mask) mask_block<2>(w, S, key0, pre ? a.P : -1, g);
+    i32x4 P[2][2];
+    Step<2> step;
     softmax_block<T, 2>(w, step, S, P, a.scale2, thr);
-    if (j + 1 < nblk) scores(j + 1);
+    rescale(w, step);
+    value_block<T, 2, decltype(look)::value>(w, P, kb + kKTile, key0, g, r16);
   };
-  auto pipelined = [&](int j) {
-    const char* vb = vring + ((j - 1) % ST) * kVTile;
-    const char* kb = kring + ((j + 1) % ST) * kKTile;
-    auto fetch = [&](int st, i32x4 (&F)[4]) {
-      if (st < 4) {
-#pragma unroll
-        for (int dd = 0; dd < 2; ++dd)
-#pragma unroll
-          for (int kc = 0; kc < 2; ++kc) F[2 * dd + kc] = lds_frag_tr(vb + voff[kc] + (2 * st + dd) * 32, 8 * kSlot);
-      } else {
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt) F[kt] = *reinterpret_cast<const i32x4*>(kb + koff[st - 4] + tile_key(kt) * 256);
-      }
-    };
-    i32x4 F[2][4];
-    fetch(0, F[0]);
-#pragma unroll
-    for (int st = 0; st < 8; ++st) {
-      i32x4(&f)[4] = F[st & 1];
-      if (st + 1 < 8) fetch(st + 1, F[(st + 1) & 1]);
-      if (st == 0) {
-        const float x[2] = {row_max<2>(S, 0), row_max<2>(S, 1)};
-        move_max(w, step, x, a.scale2, thr);
-      } else if (st == 1) {
-        exp_tile<2>(S, step, a.scale2, 0, 0), exp_tile<2>(S, step, a.scale2, 0, 1), exp_tile<2>(S, step, a.scale2, 0, 2);
-      } else if (st == 2) {
-        exp_tile<2>(S, step, a.scale2, 0, 3), exp_tile<2>(S, step, a.scale2, 1, 0), exp_tile<2>(S, step, a.scale2, 1, 1);
-      } else if (st == 3) {
-        exp_tile<2>(S, step, a.scale2, 1, 2), exp_tile<2>(S, step, a.scale2, 1, 3);
-      }
-      if (st < 4) {
-#pragma unroll
-        for (int dd = 0; dd < 2; ++dd)
-#pragma unroll
-          for (int kc = 0; kc < 2; ++kc)
-#pragma unroll
-            for (int u = 0; u < 2; ++u)
-              w.o[2 * st + dd][u] = mfma_16x16x32<T>(frag(f[2 * dd + kc]), frag(P[u][kc]), w.o[2 * st + dd][u]);
-        w.l[st >> 1] = mfma_16x16x32<T>(ones, frag(P[st >> 1][st & 1]), w.l[st >> 1]);
-      } else {
-        if (st == 4) pack_block<T, 2>(S, P);
-#pragma unroll
-        for (int kt = 0; kt < 4; ++kt)
-#pragma unroll
-          for (int u = 0; u < 2; ++u) S[kt][u] = mfma_16x16x32<T>(frag(f[kt]), w.qf[u][st - 4], st == 4 ? zero : S[kt][u]);
-      }
-      __builtin_amdgcn_sched_barrier(0);
-    }
-  };
-
-  if (nblk > 0) {
-#pragma unroll
-    for (int j = 0; j < ST; ++j) {
-      issue_k(j);
-      issue_v(j - 2);
-    }
-    sync(min(ST, nblk) - 1 + min(ST - 2, nblk));
-    if (work) {
-      scores(0);
-      // From the second block on to the first with hidden keys, in a loop of its own (one body for both kinds costs registers).
-      const int hidden = lim_w / BLK - job.sb + job.npre;  // the first own block with hidden keys
-      const int full = max(1, min(hidden, nblk - 1));
-      top(0);
-      generic(0);
-      int j = 1;
-      for (; j < full; ++j) {
-        top(j);
-        rescale(w, step);
-        pipelined(j);
-      }
-      for (; j < nblk; ++j) {
-        top(j);
-        generic(j);
-      }
-    } else {
-      for (int j = 0; j < nblk; ++j) top(j);
-    }
-    sync(0);
-    if (work) values(nblk - 1);
-  }
+  issue(0);
+  const int seen = first_partial(a, job, lim_w);
+  for (int j = 0; j < seen; ++j) block(j, std::false_type{});
+  for (int j = seen; j < nblk; ++j) block(j, std::true_type{});
 
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
@@ -513,11 +396,12 @@ template <typename T, int NW> Q3_DEV void tile_job(const Args& a, const Job& job
 }
 
 // Up to 16 U query rows: each wave takes every fourth block.
-template <typename T, int U> Q3_DEV void few_job(const Args& a, const Job& job, char* lds, int wave, int g, int r16) {
+template <typename T, int U, bool LOOK> Q3_DEV void few_job(const Args& a, const Job& job, char* lds, int wave, int g, int r16) {
   // 16 rows: the next K on its way beside the softmax and V's product; 32 have no registers for it.
   constexpr bool EARLY = U == 1;
   constexpr int NW = 4, R = 16 * U;
   char* const vt = lds + wave * kVTile;
+  const int lim_w = own_end(a, job.start, 0);
   Rows<U> w;
   i32x4 kf[4][4];
   auto load_k = [&](int j) {
@@ -541,13 +425,7 @@ template <typename T, int U> Q3_DEV void few_job(const Args& a, const Job& job, 
     asm volatile("" ::: "memory");
     __builtin_amdgcn_sched_barrier(0);
   };
-  if (wave < job.nblk) {
-    load_k(wave);
-    load_v(wave);
-  }
-  load_rows(a, w, 0, job.rows, job.b0, job.hk, job.start, g, r16);
-  const int lim_w = own_end(a, job.start, 0);
-  for (int j = wave; j < job.nblk; j += NW) {
+  auto block = [&](int j) {
     const Block x = block_of(a, job, j);
     f32x4 S[4][U];
 #pragma unroll
@@ -561,7 +439,7 @@ template <typename T, int U> Q3_DEV void few_job(const Args& a, const Job& job, 
     fence();
     if (EARLY && more) load_k(j + NW);
     fence();
-    const bool pre = j < job.npre, mask = block_masked(a, job, j, x, lim_w);
+    const bool pre = j < job.npre, mask = x.key0 + BLK > (pre ? a.P : lim_w);
     i32x4 P[U][2];
     Step<U> step;
     if (mask) mask_block<U>(w, S, x.key0, pre ? a.P : -1, g);
@@ -572,14 +450,20 @@ template <typename T, int U> Q3_DEV void few_job(const Args& a, const Job& job, 
     if (EARLY && more) __builtin_amdgcn_s_waitcnt((16 & 15) | ((16 >> 4) << 14) | (7 << 4) | (15 << 8));
     else __builtin_amdgcn_s_waitcnt((0 & 15) | (7 << 4) | (15 << 8));
     fence();
-    value_block<T, U>(w, P, vt, mask && !pre && a.S > 1, x.key0, g, r16);
+    value_block<T, U, LOOK>(w, P, vt, x.key0, g, r16);
     if (more) {
       __builtin_amdgcn_s_waitcnt((15) | (3 << 14) | (7 << 4) | (0 << 8));  // the tile is read
       fence();
       if (!EARLY) load_k(j + NW);
       load_v(j + NW);
     }
+  };
+  if (wave < job.nblk) {
+    load_k(wave);
+    load_v(wave);
   }
+  load_rows(a, w, 0, job.rows, job.b0, job.hk, job.start, g, r16);
+  for (int j = wave; j < job.nblk; j += NW) block(j);
   // The waves' sums joined: wave i's O [R][128], maxima and sums at its tile.  What is left there is read by the wave itself.
   __builtin_amdgcn_s_waitcnt((15) | (3 << 14) | (7 << 4) | (0 << 8));
   fence();
@@ -622,6 +506,9 @@ template <typename T, int U> Q3_DEV void few_job(const Args& a, const Job& job, 
 
 // Pointers to a job's keys and values.
 Q3_DEV void job_pointers(const Args& a, Job& job) {
+  // in scalar registers, whatever way they came: the tiles' descriptors are formed from them
+  for (int* x : {&job.b0, &job.hk, &job.tile, &job.slot, &job.rows, &job.pb, &job.npre, &job.sb, &job.nblk, &job.own, &job.start})
+    *x = __builtin_amdgcn_readfirstlane(*x);
   job.pk = a.pk + job.b0 / a.n * a.pl.b + job.hk * a.pl.h;
   job.pv = a.pv + job.b0 / a.n * a.pl.b + job.hk * a.pl.h;
   job.ck = a.ck + job.b0 * a.cl.b + job.hk * a.cl.h;
@@ -652,44 +539,66 @@ Q3_DEV bool own_job(const Args& a, Job& job, int w, int RT) {
   job.start = __builtin_amdgcn_readfirstlane(row_start(a, job.b0));
   const int all = (own_end(a, job.start, a.S - 1) + BLK - 1) / BLK;
   job.own = own_end(a, job.start, min(job.tile * RT + RT - 1, SG - 1) / a.G);
-  const int blocks = (job.own + BLK - 1) / BLK;
-  if (a.fused) {
-    job.npre = (a.P + BLK - 1) / BLK;
-    job.nblk = job.npre + blocks;
-    return true;
-  }
-  const int per = own_per(a, all);
-  job.sb = split * per;
-  job.nblk = max(min(per, blocks - job.sb), 0);
+  const int blocks = (job.own + BLK - 1) / BLK, per = own_per(a, all);
+  const int pre = a.fused ? (a.P + BLK - 1) / BLK : 0;
+  job.sb = a.fused ? 0 : split * per;
+  job.npre = pre;
+  job.nblk = pre + (a.fused ? blocks : max(min(per, blocks - job.sb), 0));
   job.slot = a.psplits + split;
   return split == 0 || job.sb < all;
 }
 
-// 4 waves: one a SIMD, with all of its registers.
-template <typename T, int NW>
-__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(NW / 4, NW / 4))) void prefix_tile_kernel(Args a) {
-  __shared__ __attribute__((aligned(1024))) char lds[kStages * (kKTile + kVTile)];
-  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-  Job job{};
-  if ((int)blockIdx.x < a.pjobs) {
-    // each XCD (workgroup ids congruent mod 8) takes a contiguous range of jobs: the tiles that read the same keys share an L2
-    const int xcd = blockIdx.x & 7, per = a.pjobs >> 3, rem = a.pjobs & 7;
-    prefix_job(a, job, xcd * per + min(xcd, rem) + ((int)blockIdx.x >> 3));
-  } else if (!own_job(a, job, (int)blockIdx.x - a.pjobs, 32 * NW)) {
-    return;
+// A workgroup's job.  The launch has pjobs jobs of the prefix and sjobs of the rows' own positions, 256 of each in turn as long as
+// there are such: workgroups that many apart share a CU, and the first kind keeps the matrix cores busy, the second the memory.
+// Jobs of the prefix: each XCD (workgroup ids congruent mod 8) takes a contiguous range, so that row tiles that read the same keys share
+// an L2.  false: nothing to do.
+Q3_DEV bool find_job(const Args& a, Job& job, int RT, bool& own) {
+  const int id = blockIdx.x, both = min(a.pjobs, a.sjobs) & ~255;
+  int w;
+  if (id < 2 * both) {
+    own = (id >> 8) & 1;
+    w = (id >> 9) * 256 + (id & 255);
+  } else {
+    w = id - both;  // the rest of the prefix's jobs, then of the others
+    own = w >= a.pjobs;
+    if (own) w = id - a.pjobs;
+  }
+  if (own) {
+    if (!own_job(a, job, w, RT)) return false;
+  } else {
+    const int xcd = w & 7, per = a.pjobs >> 3, rem = a.pjobs & 7;
+    prefix_job(a, job, xcd * per + min(xcd, rem) + (w >> 3));
   }
   job_pointers(a, job);
+  return true;
+}
+
+template <typename T, int NW>
+__global__ __launch_bounds__(NW * 64) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefix_tile_kernel(Args a) {
+  __shared__ __attribute__((aligned(1024))) char lds[2 * kStage];
+  const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  Job job{};
+  bool own;
+  if (!find_job(a, job, 32 * NW, own)) return;
   tile_job<T, NW>(a, job, lds, wave, (tid & 63) >> 4, tid & 15);
 }
 
-template <typename T, int U> __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefix_few_kernel(Args a) {
-  __shared__ __attribute__((aligned(1024))) char lds[4 * kVTile + 4 * 2 * 16 * U * 4];
+// Jobs of up to 16 U rows, and with TILES the prefix's of more.  LOOK: several queries a row.
+template <typename T, int U, bool TILES, bool LOOK>
+__global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) void prefix_few_kernel(Args a) {
+  constexpr int kFew = 4 * kVTile + 4 * 2 * 16 * U * 4, kTiles = 2 * kStage;
+  __shared__ __attribute__((aligned(1024))) char lds[TILES && kTiles > kFew ? kTiles : kFew];
   const int tid = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   Job job{};
-  if ((int)blockIdx.x < a.pjobs) prefix_job(a, job, blockIdx.x);
-  else if (!own_job(a, job, (int)blockIdx.x - a.pjobs, 32)) return;
-  job_pointers(a, job);
-  few_job<T, U>(a, job, lds, wave, (tid & 63) >> 4, tid & 15);
+  bool own;
+  if (!find_job(a, job, 32, own)) return;
+  if constexpr (TILES) {
+    if (!own) {
+      tile_job<T, 4>(a, job, lds, wave, (tid & 63) >> 4, tid & 15);
+      return;
+    }
+  }
+  few_job<T, U, LOOK>(a, job, lds, wave, (tid & 63) >> 4, tid & 15);
 }
 
 // o = sum_j 2^(m_j - M) O_j / sum_j 2^(m_j - M) s_j over a query row's slots: the prefix's splits, then those of its own positions.
@@ -700,28 +609,33 @@ template <typename T, int GR> __global__ __launch_bounds__(256) void prefix_join
   __shared__ float psum[RB][GR];
   const int l = threadIdx.x & 31, grp = (threadIdx.x >> 5) % GR, rb = (threadIdx.x >> 5) / GR, Hq = a.Hkv * a.G;
   const int64_t row = min((int64_t)blockIdx.x * RB + rb, rows - 1);
+  const float *pm = a.pm + row * a.slots, *ps = a.ps + row * a.slots, *po = a.po + row * a.slots * D + 4 * l;
+  f32x4 x[4];
+  float m[4], sj[4];
+  auto load = [&](int j0) {  // slots that the row has not are loaded too (they are there), and not used
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int j = min(j0 + k * GR, a.slots - 1);
+      x[k] = *reinterpret_cast<const f32x4*>(po + (int64_t)j * D);
+      m[k] = pm[j];
+      sj[k] = ps[j];
+    }
+  };
+  load(grp);
+  const float m0 = pm[min(l, a.slots - 1)];
   const int64_t bs = row / Hq;
   const int h = (int)(row - bs * Hq), b = (int)(bs / a.S), s = (int)(bs - (int64_t)b * a.S);
-  const float *pm = a.pm + row * a.slots, *ps = a.ps + row * a.slots, *po = a.po + row * a.slots * D + 4 * l;
   const int start = row_start(a, b), all = (own_end(a, start, a.S - 1) + BLK - 1) / BLK;
   const int per = own_per(a, all);
   const int used = a.psplits + max((all + per - 1) / per, 1);
-  float M = -INFINITY;
-  for (int j = l; j < used; j += 32) M = __builtin_fmaxf(M, pm[j]);
+  float M = l < used ? m0 : -INFINITY;
+  for (int j = l + 32; j < used; j += 32) M = __builtin_fmaxf(M, pm[j]);
 #pragma unroll
   for (int o = 1; o < 32; o <<= 1) M = __builtin_fmaxf(M, __shfl_xor(M, o, 64));
   float sum = 0.f;
   f32x4 o = {0.f, 0.f, 0.f, 0.f};
   for (int j0 = grp; j0 < used; j0 += 4 * GR) {
-    f32x4 x[4];
-    float m[4], sj[4];
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int j = min(j0 + k * GR, used - 1);
-      x[k] = *reinterpret_cast<const f32x4*>(po + (int64_t)j * D);
-      m[k] = pm[j];
-      sj[k] = ps[j];
-    }
+    if (j0 != grp) load(j0);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
       if (j0 + k * GR >= used || m[k] == -INFINITY) continue;
@@ -767,23 +681,23 @@ Plan plan_for(int64_t R, int64_t n, int64_t S, int64_t Hkv, int64_t G, int64_t P
     p.sjobs = B * Hkv * p.stiles;
     return p;
   }
-  // Jobs of few rows: two workgroups a CU; of tiles: one.  Where both kinds of positions are in one launch, half of it each.
+  // About a workgroup a CU for each kind of position, two in all, if that leaves kMinPer blocks a job.  More would fill the CUs in
+  // finer pieces, but every one writes its rows' O for the second launch (64 rows behind 32768: 256 jobs 80 us, 512 85, 1024 100).
+  constexpr int64_t kJobs = 256;
   p.pfew = P > 0 && n * SG <= 32;
   p.sfew = SG <= 32;
-  p.nw = (P > 0 ? n * SG : SG) <= 128 ? 4 : 8;
-  const bool both = P > 0 && p.pfew == p.sfew;
-  const int64_t tile_jobs = 256, few_jobs = 512;
+  p.nw = 4;
   p.ptiles = 1;
   if (P > 0) {
-    p.ptiles = p.pfew ? 1 : (int)cdiv(n * SG, 32 * p.nw);
-    const int64_t want = std::max<int64_t>(1, (p.pfew ? few_jobs / 2 : tile_jobs) / (R * Hkv * p.ptiles));
+    p.ptiles = p.pfew ? 1 : (int)cdiv(n * SG, 128);
+    const int64_t want = std::max<int64_t>(1, kJobs / (R * Hkv * p.ptiles));
     p.pper = (int)std::max<int64_t>(cdiv(pblocks, want), kMinPer);
     if (p.pfew) p.pper = (p.pper + 3) & ~3;
     p.psplits = (int)cdiv(pblocks, p.pper);
     p.pjobs = R * Hkv * p.ptiles * p.psplits;
   }
-  p.stiles = p.sfew ? 1 : (int)cdiv(SG, 32 * p.nw);
-  p.max_splits = (int)std::max<int64_t>(1, (p.sfew ? few_jobs : tile_jobs) / (both ? 2 : 1) / (B * Hkv * p.stiles));
+  p.stiles = p.sfew ? 1 : (int)cdiv(SG, 128);
+  p.max_splits = (int)std::max<int64_t>(1, kJobs / (B * Hkv * p.stiles));
   p.ssplits = (int)std::max<int64_t>(1, std::min<int64_t>(p.max_splits, cdiv(cdiv(span, BLK), kMinPer)));
   p.sjobs = B * Hkv * p.stiles * p.ssplits;
   p.slots = p.psplits + p.ssplits;
@@ -798,24 +712,21 @@ size_t bytes_for(const Plan& p, int64_t rows) {
   return p.slots == 1 ? 0 : (size_t)rows * p.slots * (D + 2) * sizeof(float);
 }
 
-template <typename T> int run(const Plan& p, Args a, int64_t rows, hipStream_t s) {
-  // the jobs of tiles, then those of few rows
-  const int64_t tp = p.pfew ? 0 : p.pjobs, ts = p.sfew ? 0 : p.sjobs;
-  int rc = 0;
-  if (tp + ts > 0) {
-    a.pjobs = (int)tp;
-    if (p.nw == 8) prefix_tile_kernel<T, 8><<<(unsigned)(tp + ts), 512, 0, s>>>(a);
-    else prefix_tile_kernel<T, 4><<<(unsigned)(tp + ts), 256, 0, s>>>(a);
-    if ((rc = (int)hipGetLastError()) != 0) return rc;
-  }
-  const int64_t fp = p.pjobs - tp, fs = p.sjobs - ts;
-  if (fp + fs > 0) {
-    a.pjobs = (int)fp;
-    const int most = (fp > 0 ? a.n : 1) * a.S * a.G;
-    if (most <= 16) prefix_few_kernel<T, 1><<<(unsigned)(fp + fs), 256, 0, s>>>(a);
-    else prefix_few_kernel<T, 2><<<(unsigned)(fp + fs), 256, 0, s>>>(a);
-    if ((rc = (int)hipGetLastError()) != 0) return rc;
-  }
+template <typename T> int run(const Plan& p, const Args& a, int64_t rows, hipStream_t s) {
+  const unsigned grid = (unsigned)(p.pjobs + p.sjobs);
+  const bool one = a.S * a.G * (p.pfew ? a.n : 1) <= 16;  // 16 rows a job at most
+  auto few = [&](auto tiles) {
+    constexpr bool TILES = decltype(tiles)::value;
+    if (a.S == 1)
+      one ? prefix_few_kernel<T, 1, TILES, false><<<grid, 256, 0, s>>>(a) : prefix_few_kernel<T, 2, TILES, false><<<grid, 256, 0, s>>>(a);
+    else
+      one ? prefix_few_kernel<T, 1, TILES, true><<<grid, 256, 0, s>>>(a) : prefix_few_kernel<T, 2, TILES, true><<<grid, 256, 0, s>>>(a);
+  };
+  if (p.fused) prefix_tile_kernel<T, 8><<<grid, 512, 0, s>>>(a);
+  else if (!p.sfew) prefix_tile_kernel<T, 4><<<grid, 256, 0, s>>>(a);
+  else if (p.pfew || a.P == 0) few(std::false_type{});
+  else few(std::true_type{});
+  const int rc = (int)hipGetLastError();
   if (p.slots == 1) return rc;
   // many slots: a workgroup a row (by what the sizes allow, not by the span: the order of the sums)
   if (p.psplits + p.max_splits > 8) prefix_join_kernel<T, 8><<<(unsigned)rows, 256, 0, s>>>(a, rows);
@@ -873,6 +784,8 @@ int q3_prefix_attention(int dtype, const void* q, int64_t qsb, int64_t qss, int6
   a.start_step = start_dev && starts == B && B > 1 ? 1 : 0;
   a.scale2 = scale * kLog2e;
   a.fused = p.fused;
+  a.pjobs = (int)p.pjobs;
+  a.sjobs = (int)p.sjobs;
   a.sfew = p.sfew;
   a.ptiles = p.ptiles;
   a.psplits = p.psplits;

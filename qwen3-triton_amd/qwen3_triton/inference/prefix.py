@@ -7,7 +7,7 @@ nothing here has a counterpart in it.
 import torch
 
 from .. import _hip as H
-from .int8 import _forward_only
+from .int8 import _FLOATS, _forward_only, _on_device
 
 HEAD_DIM = 128
 MAX_STRIDE = 1 << 24   # elements between positions, below
@@ -15,21 +15,19 @@ MAX_STRIDE = 1 << 24   # elements between positions, below
 
 def _cache_strides(k, v, what):
     """Strides (batch, head, position) of keys and values [.., heads, positions, 128] that lie alike."""
-    if k.ndim != 4 or v.shape != k.shape or k.shape[3] != HEAD_DIM:
+    shape = k.shape
+    if len(shape) != 4 or v.shape != shape or shape[3] != HEAD_DIM:
         raise ValueError(f'{what}: keys and values [batch, heads, positions, {HEAD_DIM}] of one shape required')
-    H.require_device(k, v)
-    b, h, n, _ = k.shape
-    out = []
-    for t in (k, v):
-        sb, sh, ss, sd = t.stride()
-        # the stride of a lone index is never used
-        st = sb if b > 1 else 0, sh if h > 1 else 0, ss if n > 1 else HEAD_DIM
-        if t.numel() and (sd != 1 or (st[0] | st[1] | st[2]) % 8 or t.data_ptr() % 16 or not HEAD_DIM <= st[2] < MAX_STRIDE):
+    b, h, n, _ = shape
+    # the stride of a lone index is never used
+    out = [(sb if b > 1 else 0, sh if h > 1 else 0, ss if n > 1 else HEAD_DIM, sd) for sb, sh, ss, sd in (k.stride(), v.stride())]
+    if b and h and n:
+        sb, sh, ss, sd = out[0]
+        if out[0] != out[1]:
+            raise ValueError(f'{what}: keys and values of one layout required')
+        if sd != 1 or (sb | sh | ss) % 8 or k.data_ptr() % 16 or v.data_ptr() % 16 or not HEAD_DIM <= ss < MAX_STRIDE:
             raise ValueError(f'{what}: contiguous, 16-byte aligned positions required; no hidden layout copy')
-        out.append(st)
-    if out[0] != out[1] and k.numel():
-        raise ValueError(f'{what}: keys and values of one layout required')
-    return out[0]
+    return out[0][:3]
 
 
 def attention(q, prefix_k, prefix_v, cache_k, cache_v, start, start_dev=None, *, scale=None):
@@ -43,14 +41,14 @@ def attention(q, prefix_k, prefix_v, cache_k, cache_v, start, start_dev=None, *,
     _forward_only(q, prefix_k, prefix_v, cache_k, cache_v)
     if q.ndim != 4 or q.numel() == 0 or q.shape[3] != HEAD_DIM:
         raise ValueError(f'queries: [B, S, heads, {HEAD_DIM}] required')
-    H.require_device(q, prefix_k, cache_k)
+    _on_device(q, prefix_k, prefix_v, cache_k, cache_v)
     ps, cs = _cache_strides(prefix_k, prefix_v, 'prefix'), _cache_strides(cache_k, cache_v, 'own positions')
     b, s, hq, d = q.shape
     r, hkv, p, _ = prefix_k.shape
     c = cache_k.shape[2]
-    if q.dtype not in (torch.bfloat16, torch.float16) or \
-            any(t.dtype != q.dtype for t in (prefix_k, prefix_v, cache_k, cache_v)):
-        raise TypeError(f'bfloat16 or float16 queries, keys and values of one dtype required, not {q.dtype}')
+    dt = q.dtype
+    if dt not in _FLOATS or prefix_k.dtype != dt or prefix_v.dtype != dt or cache_k.dtype != dt or cache_v.dtype != dt:
+        raise TypeError(f'bfloat16 or float16 queries, keys and values of one dtype required, not {dt}')
     if r < 1 or b % r or cache_k.shape[:2] != (b, hkv) or hkv < 1 or hq % hkv:
         raise ValueError('a whole number of rows per prefix, own positions of every row, and query heads that are a multiple of '
                          'the key/value heads required')
@@ -65,7 +63,7 @@ def attention(q, prefix_k, prefix_v, cache_k, cache_v, start, start_dev=None, *,
         if type(start) is not int or start < 0 or start + s > c:
             raise ValueError(f'positions {start} .. {start} + {s} - 1 do not fit {c}')
     else:
-        H.require_device(q, start_dev)
+        _on_device(q, start_dev)
         starts, start = start_dev.numel(), 0
         if start_dev.dtype != torch.int64 or starts not in (1, b) or not start_dev.is_contiguous():
             raise ValueError(f'device positions are one int64, or one for each of the {b} rows')
@@ -77,7 +75,7 @@ def attention(q, prefix_k, prefix_v, cache_k, cache_v, start, start_dev=None, *,
     out = q.new_empty((b, s, hq, d))
     nbytes = H.query("q3_prefix_attention_workspace_bytes", b, r, s, hq, hkv, p, start + s if start_dev is None else c)
     ws = H.workspace(nbytes, q.device) if nbytes else None
-    H.launch(q, "q3_prefix_attention", H.code(q.dtype), q.data_ptr(), qb, qs, qh, prefix_k.data_ptr(), prefix_v.data_ptr(), *ps,
+    H.launch(q, "q3_prefix_attention", H.code(dt), q.data_ptr(), qb, qs, qh, prefix_k.data_ptr(), prefix_v.data_ptr(), *ps,
              cache_k.data_ptr(), cache_v.data_ptr(), *cs, out.data_ptr(), s * hq * d, hq * d, d,
              None if ws is None else ws.data_ptr(), nbytes, b, r, s, hq, hkv, d, p, c, start,
              None if start_dev is None else start_dev.data_ptr(), starts, scale)
