@@ -531,18 +531,21 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile_kernel(Args ar) {
 #pragma unroll
           for (int j = 0; j < FN; ++j)
 #pragma unroll
-            for (int e = 0; e < 4; ++e) {
-              v[4 * j + e] = acc[i][j][e];
-              if (clim < 128 && j * 16 + 4 * quarter + e >= clim) v[4 * j + e] = -INFINITY;
-            }
+            for (int e = 0; e < 4; ++e) v[4 * j + e] = acc[i][j][e];
+          if (clim < 128) {  // the last group: columns that are not there
+            int lim = clim - 4 * quarter;
+            asm volatile("" : "+v"(lim));  // compared anew for each row block: 32 masks kept for all of them do not fit the scalars
+#pragma unroll
+            for (int k = 0; k < 4 * FN; ++k) v[k] = (k >> 2) * 16 + (k & 3) >= lim ? -INFINITY : v[k];
+          }
           if (row < mrows) {
             const int64_t t = ar.tgt[row] - col0;
             if (t >= 0 && t < min(clim, 128) && ((int)t & 12) == 4 * quarter) {
+              const int at = ((int)t >> 4) * 4 + ((int)t & 3);
+              float z = 0.f;
 #pragma unroll
-              for (int j = 0; j < FN; ++j)
-#pragma unroll
-                for (int e = 0; e < 4; ++e)
-                  if ((int)t == j * 16 + 4 * quarter + e) ar.pick[row] = v[4 * j + e];
+              for (int k = 0; k < 4 * FN; ++k) z = at == k ? v[k] : z;
+              ar.pick[row] = z;
             }
           }
           q3lp::Part p = q3lp::part_of(v, ar.c2);

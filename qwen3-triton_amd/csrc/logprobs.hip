@@ -224,11 +224,14 @@ __global__ __launch_bounds__(kThreads) void slice_kernel(Fwd a) {
         if (last - first > 1) load(sl);
         float x[C * V];
         unpack<T, C>(x, raw);
+        const int64_t base = (int64_t)sl * N - mis;
+        int lo = (int)max(-base, (int64_t)0);
+        const int n = max((int)min(a.vocab - base, (int64_t)N) - lo, 0);  // the row's part of the slice
 #pragma unroll
         for (int i = 0; i < C * V; ++i) {
+          if (i % V == 0) asm volatile("" : "+v"(lo));  // compared as needed: masks kept for all values do not fit the scalars
           const int at = (i / V * kThreads + tid) * V + i % V;
-          const int64_t j = (int64_t)sl * N - mis + at;
-          f(j >= 0 && j < a.vocab && at < N ? order32(x[i]) : 0, (uint32_t)j);
+          f((unsigned)(at - lo) < (unsigned)n ? order32(x[i]) : 0, (uint32_t)((int)base + at));
         }
       }
     }, [&](int rank, uint64_t k) { out[rank] = k; });

@@ -296,6 +296,13 @@ Q3_DEV int first_partial(const Args& a, const Job& job, int lim) {
   return a.S == 1 ? job.nblk : min(max(lim / BLK - job.sb, 0) + job.npre, job.nblk);
 }
 
+// The launch's arguments read again where a job ends: kept from its start, they would crowd its loop's scalars out of registers.
+Q3_DEV const Args& args_again() {
+  auto p = (const __attribute__((address_space(4))) Args*)__builtin_amdgcn_kernarg_segment_ptr();
+  asm volatile("" : "+s"(p));
+  return *(const Args*)p;
+}
+
 // A query row's place among the partials, and in the output.
 Q3_DEV void row_place(const Args& a, const Job& job, int m, int64_t& part, int64_t& out) {
   const int SG = a.S * a.G, b = job.b0 + m / SG, x = m % SG, s = x / a.G, h = job.hk * a.G + x % a.G;
@@ -379,18 +386,19 @@ template <typename T, int NW> Q3_DEV void tile_job(const Args& a, const Job& job
   for (int j = 0; j < seen; ++j) block(j, std::false_type{});
   for (int j = seen; j < nblk; ++j) block(j, std::true_type{});
 
+  const Args& e = args_again();
 #pragma unroll
   for (int u = 0; u < 2; ++u) {
     const int m = m0 + 16 * u + r16;
     if (m >= job.rows) continue;
     int64_t part, out;
-    row_place(a, job, m, part, out);
+    row_place(e, job, m, part, out);
 #pragma unroll
     for (int dt = 0; dt < 8; ++dt)
-      store4<T>(a, part, out, 16 * dt + 4 * g, w.o[dt][u], w.l[u][0], a.P == 0 && w.lim[u] == 0);
-    if (a.slots > 1 && g == 0) {
-      a.pm[part] = w.m[u] == -INFINITY ? -INFINITY : w.m[u] * a.scale2;
-      a.ps[part] = w.l[u][0];
+      store4<T>(e, part, out, 16 * dt + 4 * g, w.o[dt][u], w.l[u][0], e.P == 0 && w.lim[u] == 0);
+    if (e.slots > 1 && g == 0) {
+      e.pm[part] = w.m[u] == -INFINITY ? -INFINITY : w.m[u] * e.scale2;
+      e.ps[part] = w.l[u][0];
     }
   }
 }
@@ -482,6 +490,7 @@ template <typename T, int U, bool LOOK> Q3_DEV void few_job(const Args& a, const
   }
   __syncthreads();
   // 32 lanes a row, 4 dims each
+  const Args& out_args = args_again();
   const int t = wave * 64 + 16 * g + r16, l = t & 31;
   for (int m = t >> 5; m < job.rows; m += 8) {
     float M = -INFINITY, sum = 0.f;
@@ -495,11 +504,11 @@ template <typename T, int U, bool LOOK> Q3_DEV void few_job(const Args& a, const
       o += e * *reinterpret_cast<const f32x4*>(lds + i * kVTile + m * kRow + l * 16);
     }
     int64_t part, out;
-    row_place(a, job, m, part, out);
-    store4<T>(a, part, out, 4 * l, o, sum, a.P == 0 && own_end(a, job.start, m / a.G) == 0);
-    if (a.slots > 1 && l == 0) {
-      a.pm[part] = M;
-      a.ps[part] = sum;
+    row_place(out_args, job, m, part, out);
+    store4<T>(out_args, part, out, 4 * l, o, sum, out_args.P == 0 && own_end(out_args, job.start, m / out_args.G) == 0);
+    if (out_args.slots > 1 && l == 0) {
+      out_args.pm[part] = M;
+      out_args.ps[part] = sum;
     }
   }
 }

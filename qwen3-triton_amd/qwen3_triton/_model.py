@@ -20,6 +20,7 @@ from .kernels.attention import causal_attention_bshd
 from .kernels.embedding import embedding
 from .kernels.linear import linear
 from .kernels.lm_head_ce import lm_head_cross_entropy
+from .kernels.logprobs import shifted_logprobs
 from .kernels.loss import causal_cross_entropy
 from .kernels.norm import rms_norm, rms_norm_fork
 from .kernels.residual import residual_add
@@ -216,3 +217,16 @@ class TritonQwen3ForCausalLM(nn.Module):
         if return_dict:
             return CausalLMOutputWithPast(loss=loss, logits=logits)
         return (logits,) if labels is None else (loss, logits)
+
+    def logprobs(self, input_ids, labels=None, *, position_ids=None, temperature=1.0, ignore_index=-100):
+        """Log probabilities and entropies (``TokenLogprobs``, fp32 [B, S - 1], differentiable) of labels[:, 1:] (int64 [B, S];
+        input_ids by default), each after the tokens of input_ids before it; positions whose label is ``ignore_index`` are left
+        out.  The logits are not kept (``kernels.logprobs.lm_head_logprobs``): what policy-gradient losses are made of."""
+        if input_ids.ndim != 2 or input_ids.dtype not in (torch.int32, torch.int64) or input_ids.shape[1] < 2:
+            raise ValueError('input_ids must be an integer [batch, sequence] tensor of at least 2 positions')
+        if labels is None:
+            labels = input_ids.to(torch.int64)
+        if labels.shape != input_ids.shape or labels.dtype != torch.int64 or not labels.is_contiguous():
+            raise ValueError('contiguous int64 labels of the shape of input_ids required')
+        hidden = self.model(input_ids, position_ids)
+        return shifted_logprobs(hidden, self.lm_head.weight, labels, temperature=temperature, ignore_index=ignore_index)

@@ -5,9 +5,13 @@ greedy decoding.  Mirrors ``qwen3_triton/inference/model.py:26-225`` (``KVCache`
 New here: serving in 8 bits, each half on its own.  ``TritonQwen3Inference.quantize_weights`` holds the layers'
 projections in int8 and quantises their inputs per token; ``new_cache(..., dtype=torch.int8)`` (``cache_dtype`` of
 ``generate``, ``DecodeSession`` and ``CapturedGreedyRequest``) keeps keys and values in int8 (``int8.LayerCache``).
+
+Also new: many continuations of one prompt.  ``KVCache.fork`` makes a cache of rows that share the positions of another one, held
+and read once (``prefix.attention``), and ``TritonQwen3Inference.score`` says how likely given tokens are.
 """
 from dataclasses import dataclass, field
 from pathlib import Path
+from typing import Optional
 
 import torch
 from torch import nn
@@ -20,9 +24,10 @@ from ..kernels import _ops
 from ..kernels.activation import swiglu
 from ..kernels.embedding import IdRangeError, embedding
 from ..kernels.linear import gemm, gemm_ok
+from ..kernels.logprobs import shifted_logprobs
 from ..kernels.mlp_precision import gate_up_swiglu
 from ..kernels.residual import residual_add
-from . import int8, kernels
+from . import int8, kernels, prefix
 
 
 def _decode_rows(t, gemv):
@@ -77,13 +82,34 @@ class KVCache:
     owner: object
     length: int = 0
     valid: bool = True
+    resets: int = field(default=0, init=False)
+
+    prefix_length = 0   # of the positions, those that are another cache's
 
     @property
     def nbytes(self):
         return sum(t.numel() * t.element_size() for t in (*self.keys, *self.values))
 
     def reset(self):
-        self.length, self.valid = 0, True
+        self.length, self.valid = self.prefix_length, True
+        self.resets += 1
+
+    def fork(self, rows, max_length):
+        """A cache for ``rows`` continuations of each of this cache's rows (row b continues row b // rows), of up to ``max_length``
+        positions of their own.  The positions that this cache holds now are shared, not copied: it has to keep them (it may
+        grow)."""
+        if type(rows) is not int or rows < 1 or type(max_length) is not int or max_length < 1:
+            raise ValueError('a positive number of rows and of positions required')
+        if not self.valid:
+            raise ValueError('KV cache was invalidated by a failed forward (reset it)')
+        if not self.length:
+            raise ValueError('the cache holds no positions to share')
+        _, h, _, d = self.keys[0].shape
+
+        def layer_buffers(like):
+            return [t.new_empty((self.batch_size * rows, h, max_length, d)) for t in like]
+        return SharedPrefixCache(layer_buffers(self.keys), layer_buffers(self.values), self.length + max_length,
+                                 self.batch_size * rows, self.owner, self.length, prefix=self)
 
     def quantized(self):
         """An ``Int8KVCache`` of the same positions (prefilled in 16 bits, decoded in 8)."""
@@ -102,6 +128,32 @@ class KVCache:
 
 
 @dataclass
+class SharedPrefixCache(KVCache):
+    """A ``KVCache`` whose first positions are those of another one, ``prefix``, shared by the rows that continue one of its rows
+    (``KVCache.fork``).  ``keys`` and ``values`` hold the rows' own positions only; ``length`` and ``capacity`` count both.
+    ``reset`` goes back to the shared ones."""
+    prefix: Optional[KVCache] = None
+
+    def __post_init__(self):
+        self.prefix_length, self._prefix_resets = self.length, self.prefix.resets
+
+    def admit(self, owner, batch, tokens):
+        super().admit(owner, batch, tokens)
+        if self.prefix.resets != self._prefix_resets or not self.prefix.valid or self.prefix.length < self.prefix_length:
+            raise ValueError('the cache that holds the shared positions no longer does')
+
+    def shared(self, i):
+        """Layer i's shared keys and values [prefixes, heads, positions, 128]."""
+        return self.prefix.keys[i][:, :, :self.prefix_length], self.prefix.values[i][:, :, :self.prefix_length]
+
+    def fork(self, rows, max_length):
+        raise ValueError('fork the cache that holds the shared positions')
+
+    def quantized(self):
+        raise ValueError('a cache with shared positions stays in 16 bits')
+
+
+@dataclass
 class Int8KVCache(KVCache):
     """A ``KVCache`` whose keys and values are held in int8, one ``int8.LayerCache`` per layer (``keys`` and ``values``
     stay empty).  A block of 64 positions is quantised when its last one comes; the unfinished block is in bf16.  So
@@ -116,6 +168,9 @@ class Int8KVCache(KVCache):
     @property
     def nbytes(self):
         return sum(layer.nbytes for layer in self.layers)
+
+    def fork(self, rows, max_length):
+        raise ValueError('an int8 cache shares no positions: fork dequantized()')
 
     def quantized(self):
         raise ValueError('the cache is in int8 already')
@@ -329,10 +384,20 @@ class TritonQwen3Inference(nn.Module):
         b, s = q.shape[:2]
         d = a.head_dim
         in8 = isinstance(cache, Int8KVCache)
+        fits = a.q_norm.eps == a.k_norm.eps and _ops.norm_rope_qk_ok(q, k, d) and all(t.is_contiguous() for t in (q, k, v))
+        if cache.prefix_length:
+            own = start - cache.prefix_length   # start_dev counts the rows' own positions
+            if start_dev is None and fits:
+                q = _ops.norm_rope_qk_cache_fwd(q, k, v, a.q_norm.weight, a.k_norm.weight, cos, sin, cache.keys[i],
+                                                cache.values[i], own, a.q_norm.eps)
+            else:
+                q = kernels.norm_rope(q, a.q_norm.weight, cos, sin, a.q_norm.eps)
+                k = kernels.norm_rope(k, a.k_norm.weight, cos, sin, a.k_norm.eps)
+                kernels.append(k, v, cache.keys[i], cache.values[i], own, start_dev)
+            return prefix.attention(q, *cache.shared(i), cache.keys[i], cache.values[i], own, start_dev).reshape(b, s, -1)
         if not in8 and self._int8 is not None and s == 1 and a.q_norm.eps == a.k_norm.eps:
             return kernels.decode_step_attention(q, k, v, a.q_norm.weight, a.k_norm.weight, a.q_norm.eps, cos, sin,
                                                  cache.keys[i], cache.values[i], start, start_dev).reshape(b, s, -1)
-        fits = a.q_norm.eps == a.k_norm.eps and _ops.norm_rope_qk_ok(q, k, d) and all(t.is_contiguous() for t in (q, k, v))
         if not in8 and start_dev is None and fits:
             # Q/K-norm + RoPE of both tensors and the K/V cache append in one launch
             q = _ops.norm_rope_qk_cache_fwd(q, k, v, a.q_norm.weight, a.k_norm.weight, cos, sin, cache.keys[i],
@@ -390,7 +455,9 @@ class TritonQwen3Inference(nn.Module):
             down = int8.linear(*int8.quantize_rows(y), *w.down)
         return residual_add(x, down)
 
-    def _forward(self, input_ids, cache, logits_to_keep, *, validate_ids=True, start_dev=None):
+    def _forward(self, input_ids, cache, logits_to_keep, *, validate_ids=True, start_dev=None, head=True):
+        """``start_dev``: the positions of the rows' own that are there before this step's, on the device.  Without ``head`` the
+        normed hidden states take the logits' place."""
         from transformers.modeling_outputs import CausalLMOutputWithPast
         if input_ids.ndim != 2 or input_ids.dtype not in (torch.int32, torch.int64) or \
                 input_ids.device != self.device or not input_ids.is_contiguous():
@@ -419,7 +486,7 @@ class TritonQwen3Inference(nn.Module):
                 x = embedding(input_ids, table)
             except IdRangeError:
                 raise ValueError('Token ID outside vocabulary') from None
-        pos = kernels.positions(b, s, start, self.device, start_dev)
+        pos = _ops.positions(b, s, start if start_dev is None else cache.prefix_length, self.device, start_dev)
         try:
             if x is None:
                 x = embedding(input_ids, self.model.embed_tokens.weight)
@@ -440,11 +507,11 @@ class TritonQwen3Inference(nn.Module):
                     q = q.view(b, s, a.num_heads, d)
                     k = k.view(b, s, a.num_kv_heads, d)
                     v = v.view(b, s, a.num_kv_heads, d)
-                    if s == 1 and d == 128 and a.q_norm.eps == a.k_norm.eps and not in8:
+                    if s == 1 and d == 128 and a.q_norm.eps == a.k_norm.eps and not in8 and not cache.prefix_length:
                         y = kernels.decode_step_attention(q, k, v, a.q_norm.weight, a.k_norm.weight, a.q_norm.eps,
                                                           cos, sin, cache.keys[i], cache.values[i], start,
                                                           start_dev).reshape(b, s, -1)
-                    elif in8:
+                    elif in8 or cache.prefix_length:
                         y = self._cached_attention(a, q, k, v, cos, sin, cache, i, start, start_dev)
                     else:
                         q = kernels.norm_rope(q, a.q_norm.weight, cos, sin, a.q_norm.eps)
@@ -480,7 +547,9 @@ class TritonQwen3Inference(nn.Module):
                     x, h = _residual_projection(x, y, m.down_proj.weight, self.gemv), None
             if logits_to_keep:
                 x = x[:, -logits_to_keep:, :].contiguous()
-            if fused:
+            if not head:
+                logits = kernels.rms_norm(x, self.model.norm.weight, self.model.norm.eps)
+            elif fused:
                 logits = kernels.decode_linear(x, [self.lm_head.weight], norm_weight=self.model.norm.weight,
                                                eps=self.model.norm.eps)[0]
             else:
@@ -505,10 +574,29 @@ class TritonQwen3Inference(nn.Module):
         return out
 
     @torch.inference_mode()
+    def score(self, input_ids, *, past_key_values=None, labels=None, top=0, temperature=1.0, ignore_index=-100):
+        """How likely the tokens of input_ids [B, S] are, each after those before it: ``TokenLogprobs`` [B, S - 1] (log
+        probabilities, entropies and with ``top`` the most likely alternatives) of input_ids[:, 1:], or of ``labels[:, 1:]``
+        (int64 [B, S], ``ignore_index`` leaves a position out).  The chunk is appended to ``past_key_values`` where one is given, such
+        as a forked cache: its first token then only follows what the cache holds."""
+        if input_ids.ndim != 2 or input_ids.shape[1] < 2:
+            raise ValueError('[B, S] token ids with at least 2 positions required')
+        if labels is None:
+            labels = input_ids.to(torch.int64)
+        elif labels.shape != input_ids.shape or labels.dtype != torch.int64 or labels.device != input_ids.device or \
+                not labels.is_contiguous():
+            raise ValueError('contiguous int64 labels of the shape of input_ids required')
+        cache = past_key_values or self.new_cache(*input_ids.shape)
+        hidden = self._forward(input_ids, cache, 0, head=False).logits
+        weight = self.lm_head.weight[:self.config.vocab_size]
+        return shifted_logprobs(hidden, weight, labels, ignore_index=ignore_index, top=top, temperature=temperature)
+
+    @torch.inference_mode()
     def generate(self, input_ids, *, max_new_tokens=32, eos_token_id=None, pad_token_id=None,
-                 cache_dtype=torch.bfloat16):
+                 cache_dtype=torch.bfloat16, past_key_values=None):
         """Greedy decoding with per-row EOS, padding and a request-local cache
-        (``inference/model.py:158-188``), in bf16 or int8 (``cache_dtype``)."""
+        (``inference/model.py:158-188``), in bf16 or int8 (``cache_dtype``), or after what ``past_key_values`` holds (the rows of
+        ``input_ids`` continue it, and it keeps the new positions)."""
         if type(max_new_tokens) is not int or max_new_tokens < 0:
             raise ValueError('Nonnegative max_new_tokens required')
         gc = self.generation_config
@@ -529,7 +617,11 @@ class TritonQwen3Inference(nn.Module):
                 raise ValueError('Token ID outside vocabulary')
             return input_ids.clone()
         b, s = input_ids.shape
-        cache = self.new_cache(b, s + max_new_tokens, dtype=cache_dtype)
+        cache = past_key_values
+        if cache is None:
+            cache = self.new_cache(b, s + max_new_tokens, dtype=cache_dtype)
+        else:
+            cache.admit(self._cache_owner, b, s + max_new_tokens - 1)
         output = torch.empty((b, s + max_new_tokens), device=self.device, dtype=torch.int64)
         output[:, :s].copy_(input_ids)
         done = torch.zeros((b,), device=self.device, dtype=torch.bool)
@@ -572,14 +664,24 @@ class DecodeSession:
     device-side increment, so the same graph serves the whole request.  Prefill runs eagerly.
     No counterpart in the reference (its captured request bakes every position into one graph,
     ``inference/model.py:191-225``); the tokens match ``generate``.
+
+    With ``prefix``, a cache of the model, the rows continue its rows (``batch // prefix.batch_size`` each): prompts and generated
+    tokens are the rows' own, up to ``capacity``, after the shared positions.
     """
 
     @torch.inference_mode()
-    def __init__(self, model, batch, capacity, *, eos=(), pad=0, cache_dtype=torch.bfloat16):
+    def __init__(self, model, batch, capacity, *, eos=(), pad=0, cache_dtype=torch.bfloat16, prefix=None):
         self.model, self.batch, self.capacity = model, batch, capacity
         self.eos, self.pad = tuple(eos), pad
         dev = model.device
-        self.cache = model.new_cache(batch, capacity, dtype=cache_dtype)
+        if prefix is None:
+            self.cache = model.new_cache(batch, capacity, dtype=cache_dtype)
+        else:
+            if cache_dtype != torch.bfloat16 or batch % prefix.batch_size or prefix.owner is not model._cache_owner:
+                raise ValueError('a prefix is a 16-bit cache of this model with a whole number of the rows for each of its rows')
+            if prefix.length + capacity > model.config.max_position_embeddings:
+                raise ValueError(f'{prefix.length} shared and {capacity} own positions are more than the model has')
+            self.cache = prefix.fork(batch // prefix.batch_size, capacity)
         self.ids = torch.zeros((batch, capacity), device=dev, dtype=torch.int64)
         self.current = torch.zeros((batch, 1), device=dev, dtype=torch.int64)
         self.length = torch.zeros((1,), device=dev, dtype=torch.int64)
@@ -596,10 +698,14 @@ class DecodeSession:
         self.done.zero_()
         self.prompt_len = 0
 
+    def _own(self):
+        """Positions of the rows' own (the device's ``length``)."""
+        return self.cache.length - self.cache.prefix_length
+
     @torch.inference_mode()
     def prefill(self, input_ids):
         b, s = input_ids.shape
-        if b != self.batch or s + 1 > self.capacity or self.cache.length:
+        if b != self.batch or s + 1 > self.capacity or self._own():
             raise ValueError('Prompt does not fit this session')
         self.ids[:, :s].copy_(input_ids)
         logits = self.model._forward(input_ids, self.cache, 1).logits[:, 0, :]
@@ -627,18 +733,19 @@ class DecodeSession:
 
     @torch.inference_mode()
     def step(self):
-        if self.cache.length + 1 > self.capacity:
+        if self._own() + 1 > self.capacity:
             raise ValueError('KV cache exhausted')
         if self.graph is None:
             self._step()
             return
         _check_captured(self)
+        self.cache.admit(self.model._cache_owner, self.batch, 1)
         self.graph.replay()
         self.cache.length += 1
 
     def tokens(self):
-        """Prompt plus generated tokens so far ([B, cache.length + 1])."""
-        return self.ids[:, :self.cache.length + 1]
+        """Prompt plus generated tokens so far (the rows' own, [B, positions + 1])."""
+        return self.ids[:, :self._own() + 1]
 
 
 class CapturedGreedyRequest:

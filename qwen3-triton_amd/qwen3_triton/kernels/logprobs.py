@@ -12,7 +12,7 @@ import torch.autograd.forward_ad as _forward_ad
 from torch.autograd.function import once_differentiable
 
 from .. import _hip as H
-from ._ops import cast
+from ._ops import cast, ce_shift_labels
 from .linear import MAX_LD, gemm, gemm_nt_into, gemm_ok, matmul_into
 
 MAX_TOP = 32
@@ -302,3 +302,12 @@ def lm_head_logprobs(hidden, weight, tokens, *, top=0, temperature=1.0, ignore_i
         return TokenLogprobs(*_LMHeadLogprobs.apply(hidden, weight, tokens, ignore_index, temperature, top))
     return TokenLogprobs(*_shaped(hidden.shape[:-1], top, *_head_forward(hidden.view(-1, weight.shape[1]), weight, tokens, ignore_index,
                                                                          temperature, top, False)[0]))
+
+
+def shifted_logprobs(hidden, weight, labels, *, ignore_index=IGNORE_INDEX, **options):
+    """``lm_head_logprobs`` of a causal model: of labels[:, 1:] (labels int64 [B, S]) after hidden[:, :-1], [B, S - 1].  ``options``: its
+    others.  The hidden states are taken as they lie; the last ones of each row are left out."""
+    with torch.cuda.device(labels.device):
+        tokens = ce_shift_labels(labels, ignore_index).view(labels.shape)
+    out = lm_head_logprobs(hidden, weight, tokens, ignore_index=ignore_index, **options)
+    return TokenLogprobs(*(None if t is None else t[:, :-1] for t in out))

@@ -157,3 +157,40 @@ def test_head_gradient_refusals(bad):
     a = dict(dtype=2, z=P, ldz=1000, rows=10, vocab=1000, tok=P, ign=-100, inv=1.0, m=P, ldp=10, rm=P, rl=P, lp=P, ent=P, g=None, gh=None)
     a.update(bad)
     assert H.load().q3_head_logprobs_bwd(*a.values(), None) == INVALID
+
+
+def test_forked_caches():
+    """What a fork shares, counts and refuses, with tensors on the host."""
+    from qwen3_triton.inference import KVCache, SharedPrefixCache
+    owner = object()
+    k, v = ([torch.zeros((2, 3, 50, 128), dtype=torch.bfloat16) for _ in range(2)] for _ in range(2))
+    cache = KVCache(k, v, 50, 2, owner)
+    with pytest.raises(ValueError):
+        cache.fork(4, 10)
+    cache.length = 30
+    forked = cache.fork(4, 10)
+    assert isinstance(forked, SharedPrefixCache) and forked.keys[1].shape == (8, 3, 10, 128) and forked.capacity == 40
+    assert forked.length == forked.prefix_length == 30 and cache.prefix_length == 0
+    assert forked.shared(1)[0].shape == (2, 3, 30, 128) and forked.shared(1)[0].data_ptr() == k[1].data_ptr()
+    forked.admit(owner, 8, 10)
+    cache.length = 45   # it may grow
+    forked.admit(owner, 8, 10)
+    for bad in ((owner, 8, 11), (owner, 2, 1), (object(), 8, 1)):
+        with pytest.raises(ValueError):
+            forked.admit(*bad)
+    forked.length = 37
+    forked.reset()
+    assert forked.length == 30
+    with pytest.raises(ValueError):
+        forked.fork(1, 1)
+    with pytest.raises(ValueError):
+        forked.quantized()
+    cache.valid = False
+    with pytest.raises(ValueError, match='no longer'):
+        forked.admit(owner, 8, 1)
+    with pytest.raises(ValueError):
+        cache.fork(1, 1)
+    cache.reset()
+    cache.length = 45   # other positions by now
+    with pytest.raises(ValueError, match='no longer'):
+        forked.admit(owner, 8, 1)
