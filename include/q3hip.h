@@ -294,6 +294,9 @@ size_t q3_gemm_workspace_bytes(const q3_gemm_desc* desc);
  * launch {first row, rows, tile rows, tile columns, k splits} in out[0..4] and out[5..9]. */
 int q3_gemm_plan(const q3_gemm_desc* desc, int64_t* out);
 int q3_gemm(const q3_gemm_desc* desc, void* workspace, size_t workspace_bytes, hipStream_t stream);
+/* The same plain product (no pieces, no epilogue) where k is far longer than m x n is large: k may be cut into up to 64 parts. */
+size_t q3_gemm_long_k_workspace_bytes(const q3_gemm_desc* desc);
+int q3_gemm_long_k(const q3_gemm_desc* desc, void* workspace, size_t workspace_bytes, hipStream_t stream);
 /* Same product for arbitrary element strides: A(m,k) = A[m*sam + k*sak], B(k,n) = B[k*sbk + n*sbn];
  * any dtype (fp32 included).  SIMT path for shapes the matrix-core kernel does not take.
  * Replaces: kernels/linear.py:13-42 (_gemm with arbitrary strides). */

@@ -40,8 +40,9 @@ constexpr Cfg kCfgInt8[kNumCfg] = {{256, 256, 1, 1.58, 1.66}, {128, 256, 1, 0.96
 // Instantiated layouts: the 192-row tiles for a k-contiguous A (they fill the CUs where 256 rows would leave the
 // last row of tiles half empty: 1500 x 24576 x 4096 247 against 279 us), 32 rows for two k-contiguous operands.
 bool cfg_for(int c, bool at, bool bt) { return c < 5 || (c == 5 ? !bt : !at); }
-constexpr int kSplits[6] = {1, 2, 3, 4, 6, 8};
-constexpr int64_t kMinSplitK = 512;  // k per split
+constexpr int kSplits[9] = {1, 2, 3, 4, 6, 8, 16, 32, 64};
+constexpr int kMost = 8, kMostLong = 64;  // K splits of a call, of a long-K call
+constexpr int64_t kMinSplitK = 512;       // k per split
 
 struct Plan {
   int cfg, splits;
@@ -82,8 +83,8 @@ int64_t tile_cols(const Args& a, int bn) {
 
 // combine: what the combining pass adds besides its traffic (us): a launch (4.5 measured on small products), or
 // next to nothing where the pass also forms the norm that an unsplit product would leave to a launch of its own.
-// can_split: the product may be formed as partial products (plain or residual epilogue, 16-byte columns).
-Plan plan_for(const Args& a, bool at, bool bt, bool can_split, double combine) {
+// most: the splits allowed: 1 unless the product may be formed as partial products (plain or residual epilogue, 16-byte columns).
+Plan plan_for(const Args& a, bool at, bool bt, int most, double combine) {
   Plan best{0, 1};
   double best_t = 0.0;
   for (int c = 0; c < kNumCfg; ++c) {
@@ -93,10 +94,13 @@ Plan plan_for(const Args& a, bool at, bool bt, bool can_split, double combine) {
     for (int sp : kSplits) {
       // a grid that fills the chip by itself is not split: its partial products would outgrow the caches
       // (6144 x 4096 x 8192 in two splits: 390 + 43 us against 300 us in two launches, below)
-      if (sp > 1 && (!can_split || a.K / sp < kMinSplitK || tiles >= 256 * kCfg[c].conc)) break;
-      const double t = estimate(c, a.rscale != nullptr, sp, tiles, a.M, a.N, a.K, combine);
+      if (sp > 1 && (sp > most || a.K / sp < kMinSplitK || tiles >= 256 * kCfg[c].conc)) break;
+      // every split has a k-tile (with k-tiles of at least as many to a split as there are splits, it has anyway)
+      const int64_t nk = cdiv(a.K, 64);
+      const int used = sp > kMost ? (int)cdiv(nk, cdiv(nk, sp)) : sp;
+      const double t = estimate(c, a.rscale != nullptr, used, tiles, a.M, a.N, a.K, combine);
       if (best_t == 0.0 || t < best_t) {
-        best = {c, sp};
+        best = {c, used};
         best_t = t;
       }
     }
@@ -141,6 +145,28 @@ template <typename T> __global__ __launch_bounds__(256) void combine_kernel(Args
   }
   if (a.res) add_res<T>(v, a.res + r * a.ldres + c);
   store_vec<T>(reinterpret_cast<u16*>(a.c[s]) + r * a.ldc[s] + c, v);
+}
+
+// The sum of more than kMost partial products: eight lanes take every eighth of a chunk's, since one after the other their
+// latencies would be the time (16 x 256 in 63 parts 4.7 us against 21, 300 x 512 in 16 5.6 against 12).
+template <typename T> __global__ __launch_bounds__(256) void combine_many_kernel(Args a) {
+  const int64_t cols = a.N / 8, i = (int64_t)blockIdx.x * 32 + (threadIdx.x >> 3);
+  const bool on = i < a.M * cols;
+  const int64_t r = on ? i / cols : 0, c = on ? (i - r * cols) * 8 : 0;
+  f32x4 s0{}, s1{};
+  for (int k = threadIdx.x & 7; k < a.splits; k += 8) {
+    const float* p = a.part + (int64_t)k * a.M * a.N + r * a.N + c;
+    s0 += *reinterpret_cast<const f32x4*>(p);
+    s1 += *reinterpret_cast<const f32x4*>(p + 4);
+  }
+  Vec<T> v;
+#pragma unroll
+  for (int e = 0; e < 8; ++e) {
+    float x = e < 4 ? s0[e] : s1[e - 4];
+    for (int o = 1; o < 8; o <<= 1) x += __shfl_xor(x, o, 8);
+    v.v[e] = x;
+  }
+  if (on && (threadIdx.x & 7) == 0) store_vec<T>(reinterpret_cast<u16*>(a.c[0]) + r * a.ldc[0] + c, v);
 }
 
 // The partial products of 8-bit codes: int32 sums (exact in any order), the scales, the residual added in fp32, one rounding.
@@ -215,7 +241,8 @@ __global__ __launch_bounds__(512) void combine_norm_kernel(Args a, const u16* __
 struct Call {
   Args a;
   double combine;
-  bool at, bt, can_split;
+  bool at, bt;
+  int most;  // splits
   int epi;
   bool q8;
 };
@@ -301,7 +328,7 @@ bool parse(const q3_gemm_desc* d, Call& c) {
     a.ldgu = d->ldgu;
   }
   a.vec = vec;
-  c.can_split = c.epi == 0 && vec;
+  c.most = c.epi == 0 && vec ? kMost : 1;
   c.combine = d->epilogue == Q3_GEMM_RESIDUAL_NORM ? 0.5 : 4.5;
   // the smallest tiles, times the most splits, still number fewer than 2^31
   return tile_rows(a, 32) * tile_cols(a, 64) < (1ll << 28);
@@ -363,7 +390,7 @@ bool parse_int8(const q3_int8_gemm_desc* d, Call& c, bool codes = true) {
   }
   if (gate_up && !vec) return false;
   a.vec = vec;
-  c.can_split = !gate_up && vec;
+  c.most = !gate_up && vec ? kMost : 1;
   c.combine = 2.9;
   return tile_rows(a, 32) * tile_cols(a, 64) < (1ll << 28);
 }
@@ -432,7 +459,7 @@ void drop_rows(Args& a, bool at, int64_t rows) {
 // The launches of a call, one or two.
 int launches(const Call& c, Launch* l) {
   l[0].a = c.a;
-  l[0].p = plan_for(c.a, c.at, c.bt, c.can_split, c.combine);
+  l[0].p = plan_for(c.a, c.at, c.bt, c.most, c.combine);
   l[0].a.splits = l[0].p.splits;
   const int64_t m1 = whole_round_rows(c, l[0].p);
   l[0].rows = m1 > 0 ? m1 : c.a.M;
@@ -440,10 +467,85 @@ int launches(const Call& c, Launch* l) {
   if (m1 == 0) return 1;
   l[1].a = c.a;
   drop_rows(l[1].a, c.at, m1);
-  l[1].p = plan_for(l[1].a, c.at, c.bt, false, c.combine);
+  l[1].p = plan_for(l[1].a, c.at, c.bt, 1, c.combine);
   l[1].rows = l[1].a.M;
   set_grid(l[1]);
   return 2;
+}
+
+// Tiles of the log probability statistics.  Up to 64 rows the weights' stream is the time, and two workgroups of 64 x 128 with
+// three stages each on a CU keep the most loads in flight (8 x 151936 x 4096 205 us, 6.1 TB/s, 64 rows 209; 32 x 256 with four
+// stages 220 and 255, 128 x 256 247 and 265).  Above, the tile of the fewest rounds of 256 workgroups, each weighed by a
+// round's time at K = 4096 (256 x 256 73 us, 128 x 256 46, 128 x 128 34): 512 x 16000 x 4096 takes 94, 65 and 82 us,
+// 200 x 8000 x 4096 74, 46 and 34, 999 x 50000 x 768 93, 102 and 124.
+struct LogprobTile {
+  int bm, bn;
+  double round;
+};
+constexpr LogprobTile kLogprobTile[4] = {{256, 256, 73.0}, {128, 256, 46.0}, {128, 128, 34.0}, {64, 128, 0.0}};
+int logprob_tile(int64_t M, int64_t N) {
+  if (M <= 64) return 3;
+  int best = 0;
+  double best_t = 0.0;
+  for (int c = 0; c < 3; ++c) {
+    const LogprobTile& f = kLogprobTile[c];
+    const double t = (double)cdiv(cdiv(M, f.bm) * cdiv(N, f.bn), 256) * f.round;
+    if (c == 0 || t < best_t) {
+      best = c;
+      best_t = t;
+    }
+  }
+  return best;
+}
+
+}  // namespace
+
+namespace {
+
+// A plain product of one piece whose long K may be cut more often.
+bool parse_long_k(const q3_gemm_desc* d, Call& c) {
+  if (!parse(d, c) || c.epi != 0 || c.a.axis != 0 || c.a.res) return false;
+  if (c.most > 1) c.most = kMostLong;
+  return true;
+}
+
+size_t split_bytes(const Call& c) {
+  const Plan p = plan_for(c.a, c.at, c.bt, c.most, c.combine);
+  return p.splits > 1 ? (size_t)p.splits * (size_t)c.a.M * (size_t)c.a.N * sizeof(float) : 0;
+}
+
+int run(const q3_gemm_desc* d, const Call& c, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  Launch l[2];
+  const int n = launches(c, l);
+  const bool norm = d->epilogue == Q3_GEMM_RESIDUAL_NORM;
+  if (l[0].p.splits > 1) {
+    Args& a = l[0].a;
+    Q3_REQUIRE(workspace && al16(workspace) &&
+               workspace_bytes >= (size_t)a.splits * (size_t)a.M * (size_t)a.N * sizeof(float));
+    a.part = (float*)workspace;
+    const int rc = launch(c, l[0], (int)d->dtype, stream);
+    if (rc != 0) return rc;
+    if (norm) {
+      if (d->dtype == Q3_BF16)
+        combine_norm_kernel<BF16><<<(unsigned)a.M, 512, 0, stream>>>(a, (const u16*)d->norm_w, d->eps, (u16*)d->y, d->ldy);
+      else
+        combine_norm_kernel<F16><<<(unsigned)a.M, 512, 0, stream>>>(a, (const u16*)d->norm_w, d->eps, (u16*)d->y, d->ldy);
+    } else if (a.splits > kMost) {
+      const unsigned g = (unsigned)cdiv(a.M * (a.N / 8), 32);
+      if (d->dtype == Q3_BF16) combine_many_kernel<BF16><<<g, 256, 0, stream>>>(a);
+      else combine_many_kernel<F16><<<g, 256, 0, stream>>>(a);
+    } else {
+      const unsigned g = (unsigned)cdiv(a.M * (a.N / 8), 256);
+      if (d->dtype == Q3_BF16) combine_kernel<BF16><<<g, 256, 0, stream>>>(a);
+      else combine_kernel<F16><<<g, 256, 0, stream>>>(a);
+    }
+    return (int)hipGetLastError();
+  }
+  for (int i = 0; i < n; ++i) {
+    const int rc = launch(c, l[i], (int)d->dtype, stream);
+    if (rc != 0) return rc;
+  }
+  return norm ? q3_rmsnorm_fwd(d->dtype, d->c[0], d->norm_w, d->y, d->m, d->n, d->eps, stream) : 0;
 }
 
 }  // namespace
@@ -452,9 +554,12 @@ extern "C" {
 
 size_t q3_gemm_workspace_bytes(const q3_gemm_desc* d) {
   Call c;
-  if (!parse(d, c)) return 0;
-  const Plan p = plan_for(c.a, c.at, c.bt, c.can_split, c.combine);
-  return p.splits > 1 ? (size_t)p.splits * (size_t)c.a.M * (size_t)c.a.N * sizeof(float) : 0;
+  return parse(d, c) ? split_bytes(c) : 0;
+}
+
+size_t q3_gemm_long_k_workspace_bytes(const q3_gemm_desc* d) {
+  Call c;
+  return parse_long_k(d, c) ? split_bytes(c) : 0;
 }
 
 int q3_gemm_plan(const q3_gemm_desc* d, int64_t* out) {
@@ -473,39 +578,19 @@ int q3_gemm_plan(const q3_gemm_desc* d, int64_t* out) {
 int q3_gemm(const q3_gemm_desc* d, void* workspace, size_t workspace_bytes, hipStream_t stream) {
   Call c;
   Q3_REQUIRE(parse(d, c));
-  Launch l[2];
-  const int n = launches(c, l);
-  const bool norm = d->epilogue == Q3_GEMM_RESIDUAL_NORM;
-  if (l[0].p.splits > 1) {
-    Args& a = l[0].a;
-    Q3_REQUIRE(workspace && al16(workspace) &&
-               workspace_bytes >= (size_t)a.splits * (size_t)a.M * (size_t)a.N * sizeof(float));
-    a.part = (float*)workspace;
-    const int rc = launch(c, l[0], (int)d->dtype, stream);
-    if (rc != 0) return rc;
-    if (norm) {
-      if (d->dtype == Q3_BF16)
-        combine_norm_kernel<BF16><<<(unsigned)a.M, 512, 0, stream>>>(a, (const u16*)d->norm_w, d->eps, (u16*)d->y, d->ldy);
-      else
-        combine_norm_kernel<F16><<<(unsigned)a.M, 512, 0, stream>>>(a, (const u16*)d->norm_w, d->eps, (u16*)d->y, d->ldy);
-    } else {
-      const unsigned g = (unsigned)cdiv(a.M * (a.N / 8), 256);
-      if (d->dtype == Q3_BF16) combine_kernel<BF16><<<g, 256, 0, stream>>>(a);
-      else combine_kernel<F16><<<g, 256, 0, stream>>>(a);
-    }
-    return (int)hipGetLastError();
-  }
-  for (int i = 0; i < n; ++i) {
-    const int rc = launch(c, l[i], (int)d->dtype, stream);
-    if (rc != 0) return rc;
-  }
-  return norm ? q3_rmsnorm_fwd(d->dtype, d->c[0], d->norm_w, d->y, d->m, d->n, d->eps, stream) : 0;
+  return run(d, c, workspace, workspace_bytes, stream);
+}
+
+int q3_gemm_long_k(const q3_gemm_desc* d, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  Call c;
+  Q3_REQUIRE(parse_long_k(d, c));
+  return run(d, c, workspace, workspace_bytes, stream);
 }
 
 size_t q3_gemm_int8_workspace_bytes(const q3_int8_gemm_desc* d) {
   Call c;
   if (!parse_int8(d, c) || c.a.M <= kStreamRows) return 0;
-  const Plan p = plan_for(c.a, false, false, c.can_split, c.combine);
+  const Plan p = plan_for(c.a, false, false, c.most, c.combine);
   return p.splits > 1 ? (size_t)p.splits * (size_t)c.a.M * (size_t)c.a.N * sizeof(int) : 0;
 }
 
@@ -607,12 +692,12 @@ int q3_gemm_nt_logprobs(int dtype, const void* A, int64_t lda, const void* B, in
   a.pick = pick;
   a.ldp = ldp;
   a.c2 = inv_temperature * q3lp::kLog2e;
-  const bool big = M > 128 && (M % 256 == 0 || M % 256 > 128 || M > 2048);
-  const int bm = big ? 256 : M > 32 ? 128 : 32;
-  a.tms = (int)cdiv(M, bm);
-  a.tns = (int)cdiv(N, 256);
-  Q3_REQUIRE((int64_t)a.tms * a.tns < (1ll << 31));
-  return q3gemm::launch_tile_nt(dtype, big ? 0 : M > 32 ? 1 : 2, 6, a, stream);
+  const int cfg = logprob_tile(M, N);
+  const int64_t tms = cdiv(M, kLogprobTile[cfg].bm), tns = cdiv(N, kLogprobTile[cfg].bn);
+  Q3_REQUIRE(tms * tns < (1ll << 31));
+  a.tms = (int)tms;
+  a.tns = (int)tns;
+  return q3gemm::launch_tile_nt(dtype, cfg, 6, a, stream);
 }
 
 }  // extern "C"

@@ -24,8 +24,9 @@ template <typename T> static int stats(int cfg, const Args& a, hipStream_t s) {
 template <typename T> static int logprobs(int cfg, const Args& a, hipStream_t s) {
   switch (cfg) {
     case 0: return launch_tile<T, 256, 256, 4, 2, 2, false, false, 6>(a, s);
-    case 1: return launch_tile<T, 128, 256, 4, 2, 2, false, false, 6>(a, s);
-    default: return launch_tile<T, 32, 256, 2, 2, 4, false, false, 6>(a, s);
+    case 1: return launch_tile<T, 128, 256, 4, 2, 3, false, false, 6>(a, s);
+    case 2: return launch_tile<T, 128, 128, 8, 1, 3, false, false, 6>(a, s);
+    default: return launch_tile<T, 64, 128, 4, 1, 3, false, false, 6>(a, s);
   }
 }
 

@@ -6,6 +6,7 @@ a tensor is not on a ROCm device, the call raises.
 """
 from __future__ import annotations
 
+import contextlib
 import ctypes
 import os
 
@@ -119,6 +120,8 @@ SIGNATURES: dict[str, tuple] = {
     "q3_gemm_workspace_bytes": (_sz, [_p]),
     "q3_gemm_plan": (_i32, [_p, _p]),
     "q3_gemm": (_i32, [_p, _p, _sz, _p]),
+    "q3_gemm_long_k_workspace_bytes": (_sz, [_p]),
+    "q3_gemm_long_k": (_i32, [_p, _p, _sz, _p]),
     "q3_quant_rows": (_i32, [_i32, _p, _i64, _p, _p, _i64, _i64, _p]),
     "q3_rmsnorm_quant": (_i32, [_i32, _p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _i64, _f32, _p]),
     "q3_gemm_int8_workspace_bytes": (_sz, [_p]),
@@ -182,11 +185,17 @@ def call(name: str, *args) -> None:
         raise RuntimeError(f"{name} failed: {msg} (code {rc})")
 
 
+_HERE_ALREADY = contextlib.nullcontext()
+
+
+def on(t: torch.Tensor):
+    """A context in which t's device is the current one."""
+    return _HERE_ALREADY if t.get_device() == torch._C._cuda_getDevice() else torch.cuda.device(t.device)
+
+
 def launch(t: torch.Tensor, name: str, *args) -> None:
     """``call`` on t's device and its current stream (appended to ``args``), whatever device is current."""
-    if t.get_device() == torch._C._cuda_getDevice():
-        return call(name, *args, stream())
-    with torch.cuda.device(t.device):
+    with on(t):
         return call(name, *args, stream())
 
 

@@ -24,7 +24,7 @@ from ..kernels import _ops
 from ..kernels.activation import swiglu
 from ..kernels.embedding import IdRangeError, embedding
 from ..kernels.linear import gemm, gemm_ok
-from ..kernels.logprobs import shifted_logprobs
+from ..kernels.logprobs import _check_options, shifted_logprobs
 from ..kernels.mlp_precision import gate_up_swiglu
 from ..kernels.residual import residual_add
 from . import int8, kernels, prefix
@@ -471,6 +471,8 @@ class TritonQwen3Inference(nn.Module):
         if self._int8 is not None:
             self._int8.check()
         start = cache.length
+        if cache.prefix_length and start + s > self.config.max_position_embeddings:   # other caches are made no longer
+            raise ValueError(f'the model has {self.config.max_position_embeddings} positions')
         if start_dev is not None and s != 1:
             raise ValueError('device-resident positions are for single-token decode steps')
         x = None
@@ -586,6 +588,7 @@ class TritonQwen3Inference(nn.Module):
         elif labels.shape != input_ids.shape or labels.dtype != torch.int64 or labels.device != input_ids.device or \
                 not labels.is_contiguous():
             raise ValueError('contiguous int64 labels of the shape of input_ids required')
+        _check_options(self.config.vocab_size, top, float(temperature), ignore_index)   # before the cache takes the chunk
         cache = past_key_values or self.new_cache(*input_ids.shape)
         hidden = self._forward(input_ids, cache, 0, head=False).logits
         weight = self.lm_head.weight[:self.config.vocab_size]

@@ -41,7 +41,7 @@ def _check_options(vocab, top, temperature, ignore_index):
 
 
 def _check_tokens(tokens, shape, ref):
-    if tokens.dtype != torch.int64 or tokens.shape != shape or tokens.get_device() != ref.get_device() or not tokens.is_contiguous():
+    if tokens.dtype != torch.int64 or tokens.shape != shape or tokens.device != ref.device or not tokens.is_contiguous():
         raise ValueError(f'contiguous int64 tokens {tuple(shape)} on the same device required')
 
 
@@ -181,29 +181,31 @@ def _fused_ok(x, w, top):
 
 
 def _fused_product(x, w, tokens, temperature, store):
-    """(statistics [3, groups of 128 columns, rows], logits of the tokens, 16 bits of each logit [T, V] for the gradient or None)"""
+    """(maxima [groups of 128 columns, T], the groups' other two statistics, logits of the tokens, 16 bits of each logit [T, V]
+    for the gradient or None)"""
     t, h = x.shape
     v = w.shape[0]
-    stats = x.new_empty((3, -(-v // 128), t), dtype=torch.float32)
-    pick = x.new_empty(t, dtype=torch.float32)
+    f = torch.float32
+    groups = x.new_empty((-(-v // 128), t), dtype=f)
+    rest = x.new_empty((2 * groups.numel() + t,), dtype=f)
     z = x.new_empty((t, v)) if store else None   # 16 bits; the gradient takes its place
-    p, step = stats.data_ptr(), 4 * stats[0].numel()
+    p, step = rest.data_ptr(), 4 * groups.numel()
     H.call("q3_gemm_nt_logprobs", H.code(x.dtype), x.data_ptr(), h, w.data_ptr(), h, t, v, h, tokens.data_ptr(), 1.0 / temperature,
-           p, p + step, p + 2 * step, pick.data_ptr(), t, None if z is None else z.data_ptr(), v, H.stream())
-    return stats, pick, z
+           groups.data_ptr(), p, p + step, p + 2 * step, t, None if z is None else z.data_ptr(), v, H.stream())
+    return groups, rest, z
 
 
 def _head_forward(x, weight, tokens, ignore_index, temperature, top, keep):
-    """(``_forward``'s results, [statistics, stored logits] of the fused form with ``keep``)"""
+    """(``_forward``'s results, the fused form's (groups' maxima, stored logits))"""
     t, v = x.shape[0], weight.shape[0]
-    with torch.cuda.device(x.device):
+    with H.on(x):
         if _fused_ok(x, weight, top):
             outs = _outputs(x, t, 0, True)
-            stats, pick, z = _fused_product(x, weight, tokens, temperature, keep)
-            p, step = stats.data_ptr(), 4 * stats[0].numel()
-            H.call("q3_head_logprobs_finish", p, p + step, p + 2 * step, t, pick.data_ptr(), t, v, tokens.data_ptr(), ignore_index,
-                   1.0 / temperature, outs[0].data_ptr(), outs[1].data_ptr(), outs[4].data_ptr(), outs[4].data_ptr() + 4 * t, H.stream())
-            return outs, (stats[0].clone() if keep else None, z)
+            groups, rest, z = _fused_product(x, weight, tokens, temperature, keep)
+            p, step, kept = rest.data_ptr(), 4 * groups.numel(), outs[4].data_ptr()
+            H.call("q3_head_logprobs_finish", groups.data_ptr(), p, p + step, t, p + 2 * step, t, v, tokens.data_ptr(), ignore_index,
+                   1.0 / temperature, outs[0].data_ptr(), outs[1].data_ptr(), kept, kept + 4 * t, H.stream())
+            return outs, (groups, z)
         outs = _outputs(x, t, top, keep)
         chunks = _chunks(t, v)
         z = torch.empty((chunks[0][1], v), device=x.device, dtype=torch.float32)
@@ -217,7 +219,6 @@ class _LMHeadLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, tokens, ignore_index, temperature, top):
         outs, (groups, ctx.z) = _head_forward(hidden.view(-1, weight.shape[1]), weight, tokens, ignore_index, temperature, top, True)
-        # the results are the caller's: what the gradient needs of them is kept apart
         ctx.save_for_backward(hidden, weight, tokens, outs[4], outs[1], outs[3], groups, outs[0] if groups is not None else None)
         ctx.rest = ignore_index, temperature, top
         ctx.set_materialize_grads(False)
@@ -237,7 +238,7 @@ class _LMHeadLogprobs(torch.autograd.Function):
         t = x.shape[0]
         g, gh, gtop = _upstream(g), _upstream(gh), _upstream(gtop)
         z, ctx.z = ctx.z, None   # consumed: the gradient takes the stored logits' place
-        with torch.cuda.device(x.device):
+        with H.on(x):
             dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
             if groups is not None:
                 if z is None:   # a second backward: the same logits again
@@ -273,7 +274,7 @@ def _products(dz, x, weight, dx, need_dw):
     """dX = dz W into ``dx`` (None: not wanted); returns dW = dz^T x or None."""
     (t, v), h = dz.shape, x.shape[1]
     if dx is not None:
-        gemm([dz], [weight], [dx], t, h, v, kmajor=(False, True))
+        gemm([dz], [weight], [dx], t, h, v, kmajor=(False, True), long_k=True)
     if not need_dw:
         return None
     dw = torch.empty_like(weight)
@@ -307,7 +308,11 @@ def lm_head_logprobs(hidden, weight, tokens, *, top=0, temperature=1.0, ignore_i
 def shifted_logprobs(hidden, weight, labels, *, ignore_index=IGNORE_INDEX, **options):
     """``lm_head_logprobs`` of a causal model: of labels[:, 1:] (labels int64 [B, S]) after hidden[:, :-1], [B, S - 1].  ``options``: its
     others.  The hidden states are taken as they lie; the last ones of each row are left out."""
-    with torch.cuda.device(labels.device):
+    H.require_device(hidden, weight)
+    if hidden.ndim != 3:
+        raise ValueError('hidden states [B, S, H] required')
+    _check_tokens(labels, hidden.shape[:2], hidden)
+    with H.on(labels):
         tokens = ce_shift_labels(labels, ignore_index).view(labels.shape)
     out = lm_head_logprobs(hidden, weight, tokens, ignore_index=ignore_index, **options)
     return TokenLogprobs(*(None if t is None else t[:, :-1] for t in out))

@@ -1,5 +1,7 @@
 """Attention over a shared prefix and log probabilities of tokens on the host: what they refuse before any launch, and their
 workspace sizes."""
+import ctypes
+
 import pytest
 import torch
 
@@ -79,6 +81,16 @@ def test_options(kw):
     LP._check_options(**{**args, 'vocab': (1 << 30) - 1, 'top': 32})
     with pytest.raises(ValueError):
         LP._check_options(**{**args, 'vocab': 1 << 30})
+
+
+def test_shifted_labels():
+    x, w, y = torch.zeros(2, 3, 8), torch.zeros(5, 8), torch.zeros(2, 3, dtype=torch.int64)
+    with pytest.raises(ValueError, match='ROCm'):
+        LP.shifted_logprobs(x, w, y)
+    for bad in (y.int(), y[:, :2], y.t().contiguous().t(), y.to('meta')):
+        with pytest.raises(ValueError, match='int64'):
+            LP._check_tokens(bad, x.shape[:2], x)
+    LP._check_tokens(y, x.shape[:2], x)
 
 
 def test_rows_of_logits():
@@ -194,3 +206,33 @@ def test_forked_caches():
     cache.length = 45   # other positions by now
     with pytest.raises(ValueError, match='no longer'):
         forked.admit(owner, 8, 1)
+
+
+def long_k(m, n, k, **kw):
+    d = H.GemmDesc()
+    d.dtype, d.pieces, d.m, d.n, d.k, d.b_kmajor = 2, 1, m, n, k, 1
+    d.a[0], d.lda[0], d.b[0], d.ldb[0], d.c[0], d.ldc[0] = P, k, P, n, P, n
+    for name, value in kw.items():
+        setattr(d, name, value)
+    return d
+
+
+def test_products_of_a_long_k():
+    """The workspace holds fp32 partial products, at most 64 of them and at least 512 of k in each; a product that the other entry
+    cuts into up to 8 needs no more here when its tiles fill the chip."""
+    lib = H.load()
+    size = lambda d: lib.q3_gemm_long_k_workspace_bytes(ctypes.addressof(d))
+    few = lambda d: lib.q3_gemm_workspace_bytes(ctypes.addressof(d))
+    for m, n, k in ((16, 256, 151936), (64, 1024, 151936), (1, 64, 40000), (300, 512, 50000), (1, 8, 8), (64, 1024, 512), (1, 4096, 1 << 18)):
+        d = long_k(m, n, k)
+        parts = size(d) / (4 * m * n)
+        assert parts == int(parts) and 0 <= parts <= 64 and parts * 512 <= max(k, 512 * (parts < 2)) and few(d) / (4 * m * n) <= 8
+    assert size(long_k(16, 256, 151936)) > 8 * 4 * 16 * 256
+    assert size(long_k(8192, 8192, 8192)) == few(long_k(8192, 8192, 8192)) == 0
+    for bad in (dict(axis=1), dict(epilogue=1, res=P, ldres=1024), dict(pieces=2), dict(m=0), dict(dtype=0), dict(k=151935)):
+        d = long_k(**{**dict(m=64, n=1024, k=151936), **bad})
+        assert size(d) == 0 and lib.q3_gemm_long_k(ctypes.addressof(d), P, 1 << 30, None) == INVALID
+    d = long_k(64, 1024, 151936)
+    assert lib.q3_gemm_long_k(None, P, 1 << 30, None) == INVALID
+    assert lib.q3_gemm_long_k(ctypes.addressof(d), None, 1 << 30, None) == INVALID
+    assert lib.q3_gemm_long_k(ctypes.addressof(d), P, size(d) - 1, None) == INVALID

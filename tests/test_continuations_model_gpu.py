@@ -174,6 +174,14 @@ def test_refusals(model):
         model.score(ids_of(2, 1, 0).cuda())
     with pytest.raises(ValueError, match='labels'):
         model.score(ids_of(2, 5, 0).cuda(), labels=ids_of(2, 4, 0).cuda())
+    for bad in (dict(top=33), dict(temperature=0.0), dict(ignore_index=None)):   # refused before the cache takes the chunk
+        with pytest.raises(ValueError):
+            model.score(ids_of(4, 3, 0).cuda(), past_key_values=forked, **bad)
+    assert forked.valid and forked.length == forked.prefix_length
+    long = cache.fork(1, model.config.max_position_embeddings)
+    with pytest.raises(ValueError, match='positions'):
+        model(ids_of(2, model.config.max_position_embeddings - 9, 0).cuda(), past_key_values=long)
+    assert long.valid and long.length == long.prefix_length
 
 
 @pytest.mark.parametrize("dtype", [torch.float32, BF])

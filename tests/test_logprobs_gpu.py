@@ -5,6 +5,8 @@ for |c d| up to 20 (below, it is less than 2^-28 of the sum), and two of its own
 thread, 8 over the workgroup and 8 over the slices.  Together the sum is off by less than 160 e of itself, and so is its logarithm in
 absolute terms.  A log probability adds two roundings of c d: 4 e c |d|.  The entropy's second part is off by 160 + 4 c |d| (20 of
 them at most) e of itself, and it is at most the entropy."""
+import math
+
 import pytest
 import torch
 
@@ -279,22 +281,30 @@ def test_lm_head(t, h, v, dtype):
     probabilities below 2^-64 of another may be 2^-64 of it."""
     print(f"lm head {t} {h} {v} {dtype}", flush=True)
     x, w, ids = head(t, h, v, dtype)
+    g, gh = torch.randn(t, generator=seeded(1)).cuda(), 0.2 * torch.randn(t, generator=seeded(2)).cuda()
+    check_head(x, w, ids, g, gh, 0.9, t)
+
+
+def check_head(x, w, ids, g, gh, temperature, n):
+    """The last n rows; the others have no upstream gradient."""
+    (t, h), v, dtype = x.shape, w.shape[0], x.dtype
+    xr, wr = x.clone().requires_grad_(), w.clone().requires_grad_()
+    out = lm_head_logprobs(xr, wr, ids, temperature=temperature)
+    dx, dw = torch.autograd.grad([out.logprobs, out.entropy], [xr, wr], [g, gh])
+    assert dx.shape == x.shape and not bool(dx[:t - n].any())
+    x, ids, g, gh, dx = x[-n:], ids[-n:], g[-n:], gh[-n:], dx[-n:]
     z = x.double() @ w.double().t()
     dot = (h + 8) * E * (x.double().abs() @ w.double().abs().t())
-    lp, want, ent, t_lp, t_h = reference(z, ids, 0.9)
-    e = 2 * dot.amax(-1) / 0.9
-    xr, wr = x.clone().requires_grad_(), w.clone().requires_grad_()
-    out = lm_head_logprobs(xr, wr, ids, temperature=0.9)
-    near(out.logprobs, want, t_lp + e)
+    lp, want, ent, t_lp, t_h = reference(z, ids, temperature)
+    e = 2 * dot.amax(-1) / temperature
+    near(out.logprobs[-n:], want, t_lp + e)
     span = (-lp.min(-1).values) + ent + 1
-    near(out.entropy, ent, t_h + e * span)
-    g, gh = torch.randn(t, generator=seeded(1)).cuda(), 0.2 * torch.randn(t, generator=seeded(2)).cuda()
-    dx, dw = torch.autograd.grad([out.logprobs, out.entropy], [xr, wr], [g, gh])
-    none = torch.zeros((t, 0), device='cuda')
-    dz, tol = grads(z, ids, g, gh, none, none.long(), 0.9)
+    near(out.entropy[-n:], ent, t_h + e * span)
+    none = torch.zeros((n, 0), device='cuda')
+    dz, tol = grads(z, ids, g, gh, none, none.long(), temperature)
     p = lp.exp()
     one = torch.zeros_like(z).scatter_(-1, ids.clamp(0)[:, None], 1.0)
-    wide = (g.abs()[:, None] + gh.abs()[:, None] * (3 + lp.abs() + ent[:, None])) / 0.9
+    wide = (g.abs()[:, None] + gh.abs()[:, None] * (3 + lp.abs() + ent[:, None])) / temperature
     u = torch.finfo(dtype).eps / 2
     tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
     step = 0.0 if dtype == torch.float32 else 0.5 * 0.6931472 * 64 / 65535 * 1.01
@@ -327,6 +337,93 @@ def test_lm_head_alternatives_and_needs(dtype):
         assert torch.equal(o.logprobs, plain.logprobs)
         (got,) = torch.autograd.grad(o.entropy.sum(), xr if need[0] else wr)
         assert bool(got.isfinite().all())
+
+
+# a tile of each kind above 64 rows, and dX with its sum over the vocabulary in more than eight parts
+@pytest.mark.parametrize("t,h,v", [(200, 64, 32008), (1000, 64, 16376), (100, 192, 9000), (16, 256, 70000), (40, 128, 36000)])
+def test_lm_head_of_other_sizes(t, h, v):
+    test_lm_head(t, h, v, torch.bfloat16)
+
+
+@pytest.mark.parametrize("h", [128, 72])   # with the statistics beside the product, and without
+def test_lm_head_backward_again_and_of_one_result(h):
+    """A second backward of one forward gives the first one's bits (the first takes the stored logits' place), and the gradients of the
+    log probabilities alone and of the entropies alone are those with zeros for the other."""
+    x, w, ids = head(70, h, 1000, torch.bfloat16)
+    g = torch.randn(70, generator=seeded(1)).cuda()
+    xr, wr = x.clone().requires_grad_(), w.clone().requires_grad_()
+    out = lm_head_logprobs(xr, wr, ids)
+    runs = [torch.autograd.grad([out.logprobs, out.entropy], (xr, wr), [g, g], retain_graph=True) for _ in range(3)]
+    for run in runs[1:]:
+        assert all(torch.equal(a, b) for a, b in zip(run, runs[0]))
+    zero = torch.zeros_like(g)
+    for i in range(2):
+        one = torch.autograd.grad(out[i], (xr, wr), g, retain_graph=True)
+        both = torch.autograd.grad([out.logprobs, out.entropy], (xr, wr), [zero if j != i else g for j in range(2)], retain_graph=True)
+        assert all(torch.equal(a, b) for a, b in zip(one, both))
+    with torch.no_grad():
+        xr.mul_(2)
+    with pytest.raises(RuntimeError, match='modified'):
+        torch.autograd.grad(out.entropy.sum(), wr)
+
+
+def test_lm_head_captured():
+    """Forward and backward in captured graphs, replayed on other inputs beside eager calls."""
+    def make(t, h, v):
+        x, w = (torch.zeros(s, dtype=torch.bfloat16, device='cuda', requires_grad=True) for s in ((t, h), (v, h)))
+        ids = torch.zeros(t, dtype=torch.int64, device='cuda')
+        up = torch.ones(t, device='cuda')
+        stream = torch.cuda.Stream()
+        stream.wait_stream(torch.cuda.current_stream())
+        g = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(g, stream=stream):
+            out = lm_head_logprobs(x, w, ids)
+            grads = torch.autograd.grad([out.logprobs, out.entropy], (x, w), [up, up])
+        torch.cuda.current_stream().wait_stream(stream)
+        return g, x, w, ids, [out.logprobs.detach(), out.entropy.detach(), *grads], up
+    graphs = [make(9, 64, 40000), make(130, 72, 904), make(300, 128, 1032)]
+    for i in range(3):
+        for g, x, w, ids, outs, up in graphs:
+            xi, wi, ii = head(*x.shape, w.shape[0], torch.bfloat16, seed=i)
+            with torch.no_grad():
+                x.copy_(xi)
+                w.copy_(wi)
+            ids.copy_(ii)
+            g.replay()
+            torch.cuda.synchronize()
+            xr, wr = xi.clone().requires_grad_(), wi.clone().requires_grad_()
+            out = lm_head_logprobs(xr, wr, ii)
+            grads = torch.autograd.grad([out.logprobs, out.entropy], (xr, wr), [up, up])
+            for a, b in zip(outs, [out.logprobs.detach(), out.entropy.detach(), *grads]):
+                assert torch.equal(a, b)
+            del out, grads, xr, wr
+
+
+def test_offsets_beyond_32_bits():
+    """More than 2^31 logits: the last rows against 64 bits, none of the gradient before them."""
+    t, v, n = 16640, 131080, 300
+    ids = torch.randint(0, v, (t,), generator=seeded(0)).cuda()
+    up = torch.zeros(t, device='cuda')
+    up[-n:] = torch.randn(n, generator=seeded(1)).cuda()
+    z = torch.zeros((t, v), dtype=torch.float16, device='cuda')
+    assert z.numel() > 1 << 31
+    z[-n:] = torch.randn((n, v), generator=seeded(2)).half().cuda()
+    z.requires_grad_()
+    out = token_logprobs(z, ids, top=3)
+    (dz,) = torch.autograd.grad([out.logprobs, out.entropy], z, [up, up])
+    near(out.logprobs[:-n], torch.full((t - n,), -math.log(v), dtype=torch.float64, device='cuda'), E * (160 + 4 * math.log(v)))
+    assert not bool(dz[:-n].any()) and torch.equal(out.top_tokens[0], torch.arange(3, device='cuda'))
+    lp, want, h, t_lp, t_h = reference(z.detach()[-n:], ids[-n:])
+    near(out.logprobs[-n:], want, t_lp)
+    near(out.entropy[-n:], h, t_h)
+    assert torch.equal(out.top_tokens[-n:], lp.sort(dim=-1, descending=True, stable=True).indices[:, :3])
+    none = torch.zeros((n, 0), device='cuda')
+    want, tol = grads(z.detach()[-n:], ids[-n:], up[-n:], up[-n:], none, none.long(), 1.0)
+    u, tiny = torch.finfo(z.dtype).eps / 2, 2.0 ** -25
+    near(dz[-n:], want, u * want.abs() + tol + tiny)
+    del out, z, dz, lp, want, tol
+    x, w, _ = head(t, 64, v, torch.bfloat16)
+    check_head(x, w, ids, up, up, 1.0, n)
 
 
 def test_lm_head_calls_alike_give_the_same_bits():
