@@ -9,8 +9,8 @@
 //   when a score passes it by more than a factor 2^8; row sums are of the rounded P, by a product with ones.
 //
 // Work is cut into jobs (query rows, key/value head, range of 64-key blocks), a workgroup each:
-//  * more than 32 query rows: waves take 32 rows each and share K and V tiles in LDS, loaded a block ahead;
-//  * up to 32: waves take every fourth block of the range each (K straight into the operand's registers, V into a tile of the
+//  * more than 32 query rows (16 of chunks): waves take 32 rows each and share K and V tiles in LDS, loaded a block ahead;
+//  * fewer: waves take every fourth block of the range each (K straight into the operand's registers, V into a tile of the
 //    wave's own), without waiting for each other, and their sums are joined in LDS.  A decode step's own positions are such jobs:
 //    they wait for memory beside the prefix's jobs, which are bound by the matrix cores.
 // Jobs leave unnormalised O, maximum and sum, which a second launch joins in a fixed order.  Where the queries of single rows fill
@@ -681,8 +681,12 @@ constexpr int kMinPer = 4;  // blocks of a split at least
 Plan plan_for(int64_t R, int64_t n, int64_t S, int64_t Hkv, int64_t G, int64_t P, int64_t span) {
   Plan p{};
   const int64_t B = R * n, SG = S * G, pblocks = cdiv(P, BLK);
-  // one pass over everything where a row's own queries fill tiles and the tiles fill the chip
-  if (SG >= 128 && B * Hkv * cdiv(SG, 256) >= 192) {
+  // One pass over everything, a row's own queries in tiles of 256, a tile a CU: where the queries fill more than 11 / 20 of the
+  // CUs' tiles in its rounds.  No partial sums are written, but a CU without a tile and a tile's missing rows are lost: 8 heads of
+  // 4 queries, 100 own positions, behind 4001: 8 x 200 (0.78) 136 against 162 us in jobs, 6 x 200 (0.59) 133 against 154,
+  // 5 x 200 (0.49) 133 against 113; behind 3000: 24 x 64 (0.75) 103 against 130, 40 x 40 (0.39) 185 against 132.
+  const int64_t tiles = B * Hkv * cdiv(SG, 256);
+  if (20 * B * Hkv * SG > 11 * 256 * 256 * cdiv(tiles, 256)) {
     p.fused = p.ptiles = 1;
     p.nw = 8;
     p.stiles = (int)cdiv(SG, 256);
@@ -693,8 +697,12 @@ Plan plan_for(int64_t R, int64_t n, int64_t S, int64_t Hkv, int64_t G, int64_t P
   // About a workgroup a CU for each kind of position, two in all, if that leaves kMinPer blocks a job.  More would fill the CUs in
   // finer pieces, but every one writes its rows' O for the second launch (64 rows behind 32768: 256 jobs 80 us, 512 85, 1024 100).
   constexpr int64_t kJobs = 256;
-  p.pfew = P > 0 && n * SG <= 32;
-  p.sfew = SG <= 32;
+  // Few rows to a job: 32 of single queries (8 x 4 behind 8192 22.9 us and 22.2 in tiles, 5 x 4 behind 32768 34.5 and 36.8, 7 x 4
+  // behind 1000 17.1 and 18.1), 16 of longer chunks, whose products look at values (4 x 8 behind 8192 24.6 and 22.3 in tiles, 1 x 32
+  // 23.6 and 20.4).
+  const int64_t few = S == 1 ? 32 : 16;
+  p.pfew = P > 0 && n * SG <= few;
+  p.sfew = SG <= few;
   p.nw = 4;
   p.ptiles = 1;
   if (P > 0) {
@@ -729,7 +737,7 @@ template <typename T> int run(const Plan& p, const Args& a, int64_t rows, hipStr
     if (a.S == 1)
       one ? prefix_few_kernel<T, 1, TILES, false><<<grid, 256, 0, s>>>(a) : prefix_few_kernel<T, 2, TILES, false><<<grid, 256, 0, s>>>(a);
     else
-      one ? prefix_few_kernel<T, 1, TILES, true><<<grid, 256, 0, s>>>(a) : prefix_few_kernel<T, 2, TILES, true><<<grid, 256, 0, s>>>(a);
+      prefix_few_kernel<T, 1, TILES, true><<<grid, 256, 0, s>>>(a);
   };
   if (p.fused) prefix_tile_kernel<T, 8><<<grid, 512, 0, s>>>(a);
   else if (!p.sfew) prefix_tile_kernel<T, 4><<<grid, 256, 0, s>>>(a);

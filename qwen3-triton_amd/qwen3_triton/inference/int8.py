@@ -31,7 +31,7 @@ def _forward_only(*tensors):
     if torch.is_grad_enabled() or _forward_ad._current_level >= 0:
         for t in tensors:
             if t is not None and (t.requires_grad and torch.is_grad_enabled() or _dual(t)):
-                raise ValueError('int8 operators are forward only: run them under torch.no_grad or detach the inputs')
+                raise ValueError('operators of inference are forward only: run them under torch.no_grad or detach the inputs')
 
 
 def _launch(t, name, *args):

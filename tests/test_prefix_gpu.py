@@ -73,7 +73,8 @@ def check(got, q, pk, pv, ck, cv, starts, scale=None):
     (1, 9, 1, 8, 1, 63, 1000), (4, 2, 1, 16, 4, 700, 128), (1, 40, 1, 8, 2, 1000, 33), (1, 1, 1, 32, 8, 5000, 3000),
     (1, 33, 1, 4, 1, 257, 0), (3, 1, 1, 3, 1, 100, 100), (1, 4, 1, 14, 2, 70, 5),
     (1, 2, 2, 8, 2, 100, 0), (1, 3, 17, 8, 2, 64, 50), (2, 2, 33, 4, 4, 130, 64), (1, 1, 300, 8, 2, 77, 100), (1, 2, 65, 16, 2, 1, 1),
-    (1, 8, 100, 32, 8, 333, 10), (1, 24, 40, 32, 8, 90, 3), (1, 1, 64, 4, 1, 64, 0), (2, 16, 130, 16, 8, 65, 77)])
+    (1, 8, 100, 32, 8, 333, 10), (1, 24, 40, 32, 8, 90, 3), (1, 1, 64, 4, 1, 64, 0), (2, 16, 130, 16, 8, 65, 77),
+    (1, 24, 56, 32, 8, 90, 3), (2, 16, 250, 16, 8, 65, 77), (1, 4, 2, 32, 8, 300, 9), (1, 1, 8, 32, 8, 700, 100)])
 def test_against_64_bits(r, n, s, hq, hkv, p, start, dtype):
     print(f"prefix {r}x{n} S{s} {hq}/{hkv} P{p} start {start} {dtype}", flush=True)
     t = inputs(r, n, s, hq, hkv, p, start + s + 9, dtype)
@@ -88,13 +89,13 @@ def test_without_a_prefix(n, s, start, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("r,n,s,p", [(1, 6, 1, 200), (2, 3, 1, 64), (1, 6, 3, 31), (1, 6, 1, 0), (1, 6, 140, 10), (1, 24, 140, 70)])
+@pytest.mark.parametrize("r,n,s,p", [(1, 6, 1, 200), (2, 3, 1, 64), (1, 6, 3, 31), (1, 6, 1, 0), (1, 6, 140, 10), (1, 24, 140, 70), (1, 24, 190, 70), (1, 4, 4, 100)])
 def test_a_position_for_each_row_read_on_the_device(r, n, s, p, dtype):
     b, c = r * n, 700
     t = inputs(r, n, s, 16, 8, p, c, dtype)
     starts = torch.randint(0, c - s + 1, (b,), generator=seeded(n + s)).tolist()
     # the first position, the last, one before the capacity's end, rows without own positions, one far outside either way
-    starts[:5] = [0, c - s, -s, -s - 3, -1]
+    starts[:5] = [0, c - s, -s, -s - 3, -1][:b]
     check(PX.attention(*t, 0, torch.tensor(starts).cuda()), *t, starts)
     far = list(starts)
     far[0], far[1] = c + 5, -(1 << 40)
@@ -107,12 +108,12 @@ def test_a_position_for_each_row_read_on_the_device(r, n, s, p, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("s", [1, 3, 150])
-def test_what_lies_behind_the_last_position_counts_for_nothing(s, dtype):
+@pytest.mark.parametrize("s,n", [(1, 4), (3, 4), (150, 4), (70, 20)])
+def test_what_lies_behind_the_last_position_counts_for_nothing(s, n, dtype):
     """Infinities, NaN and the type's lowest value behind the prefix and behind each row's own positions."""
-    p, c, n = 77, 400, 4
-    q, pk, pv, ck, cv = inputs(1, n, s, 8, 2, 200, c, dtype)
-    starts = [0, 100, 63, c - s - 1]
+    p, c = 77, 400
+    q, pk, pv, ck, cv = inputs(1, n, s, *((8, 2) if n == 4 else (32, 8)), 200, c, dtype)
+    starts = [0, 100, 63, c - s - 1] * (n // 4)
     want = PX.attention(q, pk[:, :, :p], pv[:, :, :p], ck, cv, 0, torch.tensor(starts).cuda())
     check(want, q, pk[:, :, :p], pv[:, :, :p], ck, cv, starts)
     for bad in (float('nan'), float('inf'), -float('inf'), torch.finfo(dtype).min):
@@ -124,7 +125,7 @@ def test_what_lies_behind_the_last_position_counts_for_nothing(s, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("n,s", [(2, 40), (24, 40)])
+@pytest.mark.parametrize("n,s", [(2, 40), (24, 40), (2, 18), (24, 56)])
 def test_a_value_that_is_not_finite_stays_with_the_queries_that_see_it(n, s, dtype):
     t = inputs(1, n, s, 32, 8, 70, 120, dtype)
     cv = t[4]
