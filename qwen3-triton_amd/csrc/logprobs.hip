@@ -13,6 +13,8 @@
 // Bound by the logits, read once (forward) or read and written once (backward).  A workgroup holds its slice of a row in
 // registers: the slice's maximum, then the sums, then the alternatives are taken from them.  Many rows take slices of 32 values (fp32: 16) a
 // thread; few rows small ones, so that one row's latency is spread over many CUs.  A second launch joins a row's slices.
+// On MI355X (kernels alone, 151936 logits a row): 4096 rows of bf16 212 + 5 us (5.9 TB/s), 777 of fp32 with 5 alternatives 101 + 7
+// (4.7 TB/s), one row with 20 alternatives 7.3 + 6.3; the gradient of 2048 bf16 rows 270 us (4.6 TB/s).
 #include <algorithm>
 
 #include "logprobs.h"
@@ -187,6 +189,8 @@ template <typename T, int C> Q3_DEV void unpack(float (&x)[C * T::vec], const i3
   }
 }
 
+// Bound by the logits where rows are many (the next slice is on its way beside the sums: with part_of's four chains of 32 values
+// these take about as long as the loads), by one trip to memory and the reductions where they are few.
 template <typename T, int C, bool TOP>
 __global__ __launch_bounds__(kThreads) void slice_kernel(Fwd a) {
   typedef typename T::storage S;
@@ -272,7 +276,7 @@ Q3_DEV void left_out(const Fwd& a, int64_t r) {
   a.logprob[r] = a.entropy[r] = a.m[r] = a.ls[r] = 0.f;
 }
 
-// One wave a row, no alternatives.
+// One wave a row, no alternatives (4096 rows 5 us: a launch).
 template <typename T> __global__ __launch_bounds__(kThreads) void finish_kernel(Fwd a) {
   const int64_t r = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;
@@ -293,7 +297,8 @@ template <typename T> __global__ __launch_bounds__(kThreads) void finish_kernel(
   if (lane == 0) finish_row(a, r, p, picked, valid);
 }
 
-// One workgroup a row: the alternatives are the largest of its slices' largest.
+// One workgroup a row: the alternatives are the largest of its slices' largest.  Bound by latencies: a load of the keys, the bound, the
+// ranks, 6.3 us for one row's 75 slices of 20.
 template <typename T> __global__ __launch_bounds__(kThreads) void finish_top_kernel(Fwd a) {
   __shared__ TopScratch sc;
   __shared__ Part row_part;
@@ -371,7 +376,8 @@ struct Bwd {
   int64_t ldo;
 };
 
-// 32 (fp32: 16) values a thread.  Rows left out are zeros, and nothing of them is read.
+// 32 (fp32: 16) values a thread, all loads before the first use; bound by the logits' read and the gradient's write (2048 x 151936
+// bf16: 1.24 GB in 270 us).  Rows left out are zeros, and nothing of them is read.
 template <typename T, typename O> __global__ __launch_bounds__(kThreads) void grad_kernel(Bwd a, int slices) {
   typedef typename T::storage S;
   typedef typename O::storage SO;
@@ -464,7 +470,9 @@ template <typename T, typename O> __global__ __launch_bounds__(kThreads) void gr
 
 // ---------------------------------------------------------------- the LM head's rows
 // Statistics of 128-column groups [group][ldp] from the LM head's product joined: R rows a workgroup, NT / R threads a row, each a
-// fixed set of groups.  16 rows side by side read whole lines; few rows take a workgroup each.
+// fixed set of groups.  16 rows side by side read whole lines (4096 rows of 1187 groups: 58 MB in 25 us); up to 256 rows take a
+// workgroup each, which reads a part of each line but spreads over the CUs (8 rows 6 us and 10, 256 8 and
+// 10, 400 14 and 10).
 struct Head {
   const float *m, *rest, *u, *pick;
   int64_t ldp;
@@ -505,7 +513,8 @@ template <int R, int NT> __global__ __launch_bounds__(NT) void head_finish_kerne
 }
 
 // dz in the place of what the product left of the logits (their distances to their group's maximum): as grad_kernel, with
-// log2 p = (c2 (m_group - M) - ls log2(e)) - distance; the given token's log p is the result itself.
+// log2 p = (c2 (m_group - M) - ls log2(e)) - distance; the given token's log p is the result itself.  Bound by z, read and written
+// (4096 x 151936: 2.5 GB in 442 us, 5.6 TB/s).
 template <typename O> __global__ __launch_bounds__(kThreads) void head_grad_kernel(Head h, Bwd a, const float* logprob, int slices) {
   constexpr int C = kGradVectors, N = kThreads * 8 * C;
   const int64_t r = blockIdx.x / (unsigned)slices;
@@ -566,7 +575,9 @@ bool dtype_ok(int dt) { return dt == Q3_F32 || dt == Q3_F16 || dt == Q3_BF16; }
 int vec_of(int dtype) { return dtype == Q3_F32 ? 4 : 8; }
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
-// Vectors of a slice per thread: 4 where that leaves enough workgroups for the chip (or a row has very many values), else 1.
+// Vectors of a slice per thread: 4 where that leaves 1024 workgroups (or a row has very many values), else 1, which spreads the search
+// for alternatives (rows of 151936, 20 of one row 14.5 us and 17.1 with 4, 5 of 64 rows 25.8 and 22.3).  Without alternatives the
+// rule is the same, for the same bits with and without (one row 8.1 us and 7.6 with 4, 64 rows 13.7 and 10.7).
 int chunks_for(int dtype, int64_t rows, int64_t vocab) {
   return vocab > (1 << 18) || rows * cdiv(vocab, (int64_t)kThreads * vec_of(dtype) * 4) >= 1024 ? 4 : 1;
 }
@@ -580,10 +591,12 @@ bool sizes_ok(int dtype, int64_t rows, int64_t vocab, int64_t top) {
   return rows * cdiv(vocab + 16, kThreads * vec_of(dtype)) < (1ll << 31) - 1;
 }
 
-// Slices of a workgroup: as many as leave 4096 workgroups; where alternatives are wanted at most 6, so that what is read again for
+// Slices of a workgroup: as many as leave 4096 workgroups, dealt out evenly (4096 rows of 151936 226 us, 2048 117, 777 of fp32 with 5 alternatives 112; one slice each
+// 229, 118 and 158; 2048 rows in parts of 9, 9 and 1 121); where alternatives are wanted at most 6, so that what is read again for
 // them is still in a cache.
 int per_for(int64_t rows, int64_t slices, int64_t top) {
-  return (int)std::max<int64_t>(1, std::min<int64_t>(top > 0 ? std::min<int64_t>(slices, 6) : slices, rows * slices / 4096));
+  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(top > 0 ? std::min<int64_t>(slices, 6) : slices, rows * slices / 4096));
+  return (int)cdiv(slices, cdiv(slices, most));
 }
 
 template <typename T, int C> void slices(const Fwd& a, hipStream_t s) {

@@ -319,7 +319,10 @@ template <typename T> Q3_DEV void store4(const Args& a, int64_t part, int64_t ou
   }
 }
 
-// More than 32 query rows: 32 a wave.
+// More query rows: 32 a wave.  Bound by the matrix cores and the softmax between them: 8 x 200 queries of 32 heads behind 4001 (all
+// CUs, a tenth of the work on rows that are not there) 125 us, 0.87 PFLOP/s; 64 single queries behind 32768, with
+// up to 1000 positions of the rows' own in jobs beside, 67 us (265 MB, 4.0 TB/s).  A third K and V tile in flight, or the softmax of one block beside the products of
+// the next, gave nothing more (138 and 134 us where this took 134).
 template <typename T, int NW> Q3_DEV void tile_job(const Args& a, const Job& job, char* lds, int wave, int g, int r16) {
   constexpr int RT = 32 * NW, L = 16 / NW;  // L: a wave's loads of a tile
   const int m0 = job.tile * RT + wave * 32, nblk = job.nblk;
@@ -403,7 +406,8 @@ template <typename T, int NW> Q3_DEV void tile_job(const Args& a, const Job& job
   }
 }
 
-// Up to 16 U query rows: each wave takes every fourth block.
+// Up to 16 U query rows: each wave takes every fourth block.  Bound by the loads' latency until many jobs share a CU: 32 single queries
+// behind 8192 and 511 of their own 21 us (4.8 TB/s), 4 x 8 behind 2047 20.8 (3.9 TB/s), 4 behind 200 6.9.
 template <typename T, int U, bool LOOK> Q3_DEV void few_job(const Args& a, const Job& job, char* lds, int wave, int g, int r16) {
   // 16 rows: the next K on its way beside the softmax and V's product; 32 have no registers for it.
   constexpr bool EARLY = U == 1;
@@ -611,7 +615,8 @@ __global__ __launch_bounds__(256) __attribute__((amdgpu_waves_per_eu(2, 2))) voi
 }
 
 // o = sum_j 2^(m_j - M) O_j / sum_j 2^(m_j - M) s_j over a query row's slots: the prefix's splits, then those of its own positions.
-// GR groups of 32 lanes (4 dims a lane) take every GR-th slot each, four loads in flight, and are added in order.
+// GR groups of 32 lanes (4 dims a lane) take every GR-th slot each, four loads in flight, and are added in order.  Bound by its
+// launch and one trip to the caches: 4 x 32 query rows of 2 slots 2.6 us, 64 x 32 of 17 6.8.
 template <typename T, int GR> __global__ __launch_bounds__(256) void prefix_join_kernel(Args a, int64_t rows) {
   constexpr int RB = 8 / GR;  // rows a workgroup
   __shared__ f32x4 part[RB][GR][32];
