@@ -12,6 +12,7 @@ import torch
 
 from _util import seeded
 
+from qwen3_triton.kernels import logprobs
 from qwen3_triton.kernels.logprobs import MAX_TOP, lm_head_logprobs, token_logprobs
 
 pytestmark = pytest.mark.gpu
@@ -285,12 +286,13 @@ def test_lm_head(t, h, v, dtype):
     check_head(x, w, ids, g, gh, 0.9, t)
 
 
-def check_head(x, w, ids, g, gh, temperature, n):
-    """The last n rows; the others have no upstream gradient."""
+def check_head(x, w, ids, g, gh, temperature, n, top=0):
+    """The last n rows; the others have no upstream gradient.  With ``top`` the alternatives have one too."""
     (t, h), v, dtype = x.shape, w.shape[0], x.dtype
     xr, wr = x.clone().requires_grad_(), w.clone().requires_grad_()
-    out = lm_head_logprobs(xr, wr, ids, temperature=temperature)
-    dx, dw = torch.autograd.grad([out.logprobs, out.entropy], [xr, wr], [g, gh])
+    out = lm_head_logprobs(xr, wr, ids, temperature=temperature, top=top)
+    gtop = torch.randn((t, top), generator=seeded(3)).cuda()
+    dx, dw = torch.autograd.grad([x for x in out[:3] if x is not None], [xr, wr], [g, gh, gtop][:3 if top else 2])
     assert dx.shape == x.shape and not bool(dx[:t - n].any())
     x, ids, g, gh, dx = x[-n:], ids[-n:], g[-n:], gh[-n:], dx[-n:]
     z = x.double() @ w.double().t()
@@ -300,11 +302,13 @@ def check_head(x, w, ids, g, gh, temperature, n):
     near(out.logprobs[-n:], want, t_lp + e)
     span = (-lp.min(-1).values) + ent + 1
     near(out.entropy[-n:], ent, t_h + e * span)
-    none = torch.zeros((n, 0), device='cuda')
-    dz, tol = grads(z, ids, g, gh, none, none.long(), temperature)
+    tid = out.top_tokens if top else torch.zeros((n, 0), dtype=torch.int64, device='cuda')
+    if top:
+        near(out.top_logprobs, torch.where((ids == -100)[:, None], 0.0, lp.gather(-1, tid)), (t_lp + e)[:, None] + 4 * E * lp.abs().amax())
+    dz, tol = grads(z, ids, g, gh, gtop[-n:], tid, temperature)
     p = lp.exp()
-    one = torch.zeros_like(z).scatter_(-1, ids.clamp(0)[:, None], 1.0)
-    wide = (g.abs()[:, None] + gh.abs()[:, None] * (3 + lp.abs() + ent[:, None])) / temperature
+    one = torch.zeros_like(z).scatter_(-1, ids.clamp(0)[:, None], 1.0).scatter_(-1, tid, 1.0)
+    wide = (g.abs()[:, None] + gtop[-n:].abs().sum(-1, keepdim=True) + gh.abs()[:, None] * (3 + lp.abs() + ent[:, None])) / temperature
     u = torch.finfo(dtype).eps / 2
     tiny = torch.finfo(dtype).smallest_normal * torch.finfo(dtype).eps / 2
     step = 0.0 if dtype == torch.float32 else 0.5 * 0.6931472 * 64 / 65535 * 1.01
@@ -343,6 +347,18 @@ def test_lm_head_alternatives_and_needs(dtype):
 @pytest.mark.parametrize("t,h,v", [(200, 64, 32008), (1000, 64, 16376), (100, 192, 9000), (16, 256, 70000), (40, 128, 36000)])
 def test_lm_head_of_other_sizes(t, h, v):
     test_lm_head(t, h, v, torch.bfloat16)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("v", [1000, 1001])   # dX and dW from one dz, and chunk by chunk
+@pytest.mark.parametrize("top", [0, 4])
+def test_lm_head_in_chunks(v, top, dtype, monkeypatch):
+    """Logits a few rows at a time."""
+    monkeypatch.setattr(logprobs, '_CHUNK_BYTES', 4 * v * 30)
+    t = 70
+    assert logprobs._chunks(t, v) == [(0, 30), (30, 60), (60, 70)]
+    x, w, ids = head(t, 72, v, dtype)
+    check_head(x, w, ids, torch.randn(t, generator=seeded(1)).cuda(), torch.randn(t, generator=seeded(2)).cuda(), 0.9, t, top)
 
 
 @pytest.mark.parametrize("h", [128, 72])   # with the statistics beside the product, and without
