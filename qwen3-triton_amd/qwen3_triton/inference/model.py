@@ -105,6 +105,8 @@ class KVCache:
         if not self.length:
             raise ValueError('the cache holds no positions to share')
         _, h, _, d = self.keys[0].shape
+        if d != prefix.HEAD_DIM:
+            raise ValueError(f'shared positions need heads of {prefix.HEAD_DIM}')
 
         def layer_buffers(like):
             return [t.new_empty((self.batch_size * rows, h, max_length, d)) for t in like]
@@ -589,7 +591,7 @@ class TritonQwen3Inference(nn.Module):
                 not labels.is_contiguous():
             raise ValueError('contiguous int64 labels of the shape of input_ids required')
         _check_options(self.config.vocab_size, top, float(temperature), ignore_index)   # before the cache takes the chunk
-        cache = past_key_values or self.new_cache(*input_ids.shape)
+        cache = self.new_cache(*input_ids.shape) if past_key_values is None else past_key_values
         hidden = self._forward(input_ids, cache, 0, head=False).logits
         weight = self.lm_head.weight[:self.config.vocab_size]
         return shifted_logprobs(hidden, weight, labels, ignore_index=ignore_index, top=top, temperature=temperature)
@@ -624,6 +626,8 @@ class TritonQwen3Inference(nn.Module):
         if cache is None:
             cache = self.new_cache(b, s + max_new_tokens, dtype=cache_dtype)
         else:
+            if cache_dtype == torch.int8 and not isinstance(cache, Int8KVCache):
+                raise ValueError('past_key_values is not in int8')
             cache.admit(self._cache_owner, b, s + max_new_tokens - 1)
         output = torch.empty((b, s + max_new_tokens), device=self.device, dtype=torch.int64)
         output[:, :s].copy_(input_ids)

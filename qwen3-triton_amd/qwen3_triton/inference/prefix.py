@@ -18,16 +18,20 @@ def _cache_strides(k, v, what):
     shape = k.shape
     if len(shape) != 4 or v.shape != shape or shape[3] != HEAD_DIM:
         raise ValueError(f'{what}: keys and values [batch, heads, positions, {HEAD_DIM}] of one shape required')
-    b, h, n, _ = shape
-    # the stride of a lone index is never used
-    out = [(sb if b > 1 else 0, sh if h > 1 else 0, ss if n > 1 else HEAD_DIM, sd) for sb, sh, ss, sd in (k.stride(), v.stride())]
-    if b and h and n:
-        sb, sh, ss, sd = out[0]
-        if out[0] != out[1]:
+    sk, sv = k.stride(), v.stride()
+    if sk != sv or not _strides_ok(*sk):   # maybe that of an index that is alone (never used), or nothing is there
+        sk, sv = ([s if n > 1 else d for n, s, d in zip(shape, t, (0, 0, HEAD_DIM, 1))] for t in (sk, sv))
+        if 0 in shape:
+            return 0, 0, HEAD_DIM
+        if sk != sv:
             raise ValueError(f'{what}: keys and values of one layout required')
-        if sd != 1 or (sb | sh | ss) % 8 or k.data_ptr() % 16 or v.data_ptr() % 16 or not HEAD_DIM <= ss < MAX_STRIDE:
-            raise ValueError(f'{what}: contiguous, 16-byte aligned positions required; no hidden layout copy')
-    return out[0][:3]
+    if not _strides_ok(*sk) or (k.data_ptr() | v.data_ptr()) % 16:
+        raise ValueError(f'{what}: contiguous, 16-byte aligned positions required; no hidden layout copy')
+    return sk[0], sk[1], sk[2]
+
+
+def _strides_ok(sb, sh, ss, sd):
+    return sd == 1 and not (sb | sh | ss) % 8 and HEAD_DIM <= ss < MAX_STRIDE
 
 
 def attention(q, prefix_k, prefix_v, cache_k, cache_v, start, start_dev=None, *, scale=None):

@@ -180,6 +180,9 @@ def test_forked_caches():
     with pytest.raises(ValueError):
         cache.fork(4, 10)
     cache.length = 30
+    small = KVCache([t[..., :64] for t in k], [t[..., :64] for t in v], 50, 2, owner, 30)
+    with pytest.raises(ValueError, match='heads of 128'):
+        small.fork(4, 10)
     forked = cache.fork(4, 10)
     assert isinstance(forked, SharedPrefixCache) and forked.keys[1].shape == (8, 3, 10, 128) and forked.capacity == 40
     assert forked.length == forked.prefix_length == 30 and cache.prefix_length == 0

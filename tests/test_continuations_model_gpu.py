@@ -163,6 +163,8 @@ def test_refusals(model):
             what()
     with pytest.raises(ValueError, match='free positions'):
         model.generate(ids_of(4, 3, 0).cuda(), max_new_tokens=4, eos_token_id=[], past_key_values=forked)
+    with pytest.raises(ValueError, match='int8'):
+        model.generate(ids_of(4, 1, 0).cuda(), max_new_tokens=2, past_key_values=forked, cache_dtype=torch.int8)
     other, _ = build()
     with pytest.raises(ValueError, match='another model'):
         other(ids_of(4, 1, 0).cuda(), past_key_values=forked)
