@@ -93,6 +93,12 @@ int q3_norm_rope_qk_cache_fwd(int dtype, const void* q, const void* k, const voi
                               const void* cos, const void* sin, void* yq, void* cache_k, void* cache_v, int64_t B,
                               int64_t S, int64_t hq, int64_t hk, int64_t d, int64_t capacity, int64_t start, float eps,
                               hipStream_t stream);
+/* The same with start read from start_dev when the kernel runs (null: start counts); keys and values that would lie outside
+ * the caches are not written. */
+int q3_norm_rope_qk_cache_dev_fwd(int dtype, const void* q, const void* k, const void* v, const void* wq, const void* wk,
+                                  const void* cos, const void* sin, void* yq, void* cache_k, void* cache_v, int64_t B,
+                                  int64_t S, int64_t hq, int64_t hk, int64_t d, int64_t capacity, int64_t start,
+                                  const int64_t* start_dev, float eps, hipStream_t stream);
 size_t q3_norm_rope_qk_bwd_workspace_bytes(int64_t tokens, int64_t hq, int64_t hk, int64_t d);
 int q3_norm_rope_qk_bwd(int dtype, const void* q, const void* k, const void* wq, const void* wk, const void* cos,
                         const void* sin, const void* dyq, const void* dyk, void* dxq, void* dxk, void* dw,

@@ -516,8 +516,10 @@ template <typename S> struct NrPair {
   int blocks[3];  // workgroups per segment
   // Prefill form of the forward (CACHE): segment 1's normed + rotated keys and segment 2's values
   // (copied unchanged) go straight into the [B, heads, cap, D] caches at positions start + s of
-  // [B, seq] token rows, instead of a [tokens, heads, D] output.
+  // [B, seq] token rows, instead of a [tokens, heads, D] output; start_dev: start, read when the kernel runs, and rows outside the
+  // caches are left out.
   int64_t cap, start, seq;
+  const int64_t* start_dev;
 };
 
 template <typename T, int TPR, bool CACHE>
@@ -535,18 +537,19 @@ __global__ __launch_bounds__(kBlock) void norm_rope_qk_fwd_kernel(NrPair<typenam
   const int64_t rows = p.rows[seg];
   const int heads = p.heads[seg];
   const int t = threadIdx.x % TPR, g = threadIdx.x / TPR;
-  // output offset of a [tokens, heads] row: row-major, or its cache slot (b, head, start + s)
+  const int64_t start = CACHE && p.start_dev ? *p.start_dev : p.start;
+  // output offset of a [tokens, heads] row: row-major, or its cache slot (b, head, start + s), -1 outside the cache
   auto out_off = [&](int64_t row) -> int64_t {
     if (!CACHE || seg == 0) return row * D;
     const int64_t tok = row / heads, h = row % heads, b = tok / p.seq, s = tok % p.seq;
-    return ((b * heads + h) * p.cap + p.start + s) * D;
+    return start < -s || start >= p.cap - s ? -1 : ((b * heads + h) * p.cap + start + s) * D;
   };
   if constexpr (CACHE) {
     if (seg == 2) {  // values: copied into the cache unchanged
       for (int64_t base = (int64_t)blk * RPB; base < rows; base += (int64_t)nblk * RPB) {
         const int64_t row = base + g;
-        if (row < rows)
-          *reinterpret_cast<i32x4*>(y + out_off(row) + t * V) = *reinterpret_cast<const i32x4*>(x + row * D + t * V);
+        const int64_t at = row < rows ? out_off(row) : -1;
+        if (at >= 0) *reinterpret_cast<i32x4*>(y + at + t * V) = *reinterpret_cast<const i32x4*>(x + row * D + t * V);
       }
       return;
     }
@@ -574,7 +577,8 @@ __global__ __launch_bounds__(kBlock) void norm_rope_qk_fwd_kernel(NrPair<typenam
       const float np = partner<TPR>(n);
       o.v[e] = n * cv.v[e] + sign * np * sv.v[e];
     }
-    if (valid) store_vec<T>(y + out_off(row) + t * V, o);
+    const int64_t at = valid ? out_off(row) : -1;
+    if (at >= 0) store_vec<T>(y + at + t * V, o);
   }
 }
 
@@ -879,7 +883,7 @@ int nr_qk_bwd_dispatch(const NrPair<typename T::storage>& p, const void* cs, con
 template <typename T>
 int nr_qk_cache_fwd_t(const void* q, const void* k, const void* v, const void* wq, const void* wk, const void* cs,
                       const void* sn, void* yq, void* ck, void* cv, int64_t B, int64_t S_, int64_t hq, int64_t hk,
-                      int64_t d, int64_t cap, int64_t start, float eps, hipStream_t s) {
+                      int64_t d, int64_t cap, int64_t start, const int64_t* start_dev, float eps, hipStream_t s) {
   typedef typename T::storage S;
   NrPair<S> p{};
   p.x[0] = (const S*)q;
@@ -896,6 +900,7 @@ int nr_qk_cache_fwd_t(const void* q, const void* k, const void* v, const void* w
   p.heads[1] = p.heads[2] = (int)hk;
   p.cap = cap;
   p.start = start;
+  p.start_dev = start_dev;
   p.seq = S_;
   return nr_qk_fwd_dispatch<T>(p, cs, sn, d, eps, s);
 }
@@ -1009,13 +1014,21 @@ int q3_norm_rope_qk_cache_fwd(int dtype, const void* q, const void* k, const voi
                               const void* cos, const void* sin, void* yq, void* cache_k, void* cache_v, int64_t B,
                               int64_t S, int64_t hq, int64_t hk, int64_t d, int64_t capacity, int64_t start, float eps,
                               hipStream_t stream) {
+  return q3_norm_rope_qk_cache_dev_fwd(dtype, q, k, v, wq, wk, cos, sin, yq, cache_k, cache_v, B, S, hq, hk, d, capacity, start,
+                                       nullptr, eps, stream);
+}
+
+int q3_norm_rope_qk_cache_dev_fwd(int dtype, const void* q, const void* k, const void* v, const void* wq, const void* wk,
+                                  const void* cos, const void* sin, void* yq, void* cache_k, void* cache_v, int64_t B,
+                                  int64_t S, int64_t hq, int64_t hk, int64_t d, int64_t capacity, int64_t start,
+                                  const int64_t* start_dev, float eps, hipStream_t stream) {
   Q3_REQUIRE(dtype_ok(dtype) && q && k && v && wq && wk && cos && sin && yq && cache_k && cache_v && B > 0 && S > 0 &&
-             hq > 0 && hk > 0 && d > 0 && d % 2 == 0 && d <= 4096 && eps > 0.f && start >= 0 && start + S <= capacity &&
-             B * S * (hq + hk) < (1ll << 40) && B * hk * capacity * d < (1ll << 40));
+             hq > 0 && hk > 0 && d > 0 && d % 2 == 0 && d <= 4096 && eps > 0.f && S <= capacity &&
+             (start_dev || (start >= 0 && start + S <= capacity)) && B * S * (hq + hk) < (1ll << 40) && B * hk * capacity * d < (1ll << 40));
   Q3_REQUIRE((((uintptr_t)q | (uintptr_t)k | (uintptr_t)v | (uintptr_t)yq | (uintptr_t)cache_k |
                (uintptr_t)cache_v) & 15) == 0);
   return Q3_DISPATCH(dtype, nr_qk_cache_fwd_t, q, k, v, wq, wk, cos, sin, yq, cache_k, cache_v, B, S, hq, hk, d,
-                     capacity, start, eps, stream);
+                     capacity, start, start_dev, eps, stream);
 }
 
 size_t q3_norm_rope_qk_bwd_workspace_bytes(int64_t tokens, int64_t hq, int64_t hk, int64_t d) {

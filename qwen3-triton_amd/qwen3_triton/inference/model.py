@@ -389,9 +389,9 @@ class TritonQwen3Inference(nn.Module):
         fits = a.q_norm.eps == a.k_norm.eps and _ops.norm_rope_qk_ok(q, k, d) and all(t.is_contiguous() for t in (q, k, v))
         if cache.prefix_length:
             own = start - cache.prefix_length   # start_dev counts the rows' own positions
-            if start_dev is None and fits:
+            if fits:
                 q = _ops.norm_rope_qk_cache_fwd(q, k, v, a.q_norm.weight, a.k_norm.weight, cos, sin, cache.keys[i],
-                                                cache.values[i], own, a.q_norm.eps)
+                                                cache.values[i], own, a.q_norm.eps, start_dev)
             else:
                 q = kernels.norm_rope(q, a.q_norm.weight, cos, sin, a.q_norm.eps)
                 k = kernels.norm_rope(k, a.k_norm.weight, cos, sin, a.k_norm.eps)

@@ -146,6 +146,27 @@ def test_scores_of_continuations(model):
     assert bool((some.logprobs[:, :9] == 0).all()) and torch.equal(some.logprobs[:, 9:], out.logprobs[:, 9:])
 
 
+@pytest.mark.parametrize("s", [1, 3])
+def test_positions_appended_where_the_device_says(s):
+    """Norm, rotation and append with a start that is read on the device: the bits of the host's start, and nothing outside the caches."""
+    from qwen3_triton.kernels import _ops
+    b, hq, hk, d, c = 3, 8, 2, 128, 20
+    gen = seeded(s)
+    q, k, v = (torch.randn((b, s, h, d), generator=gen).to(BF).cuda() for h in (hq, hk, hk))
+    wq, wk = (torch.rand(d, generator=gen).to(BF).cuda() for _ in range(2))
+    cos, sin = (torch.randn((b, s, d), generator=gen).to(BF).cuda() for _ in range(2))
+    fresh = torch.randn((2, b, hk, c, d), generator=gen).to(BF).cuda()
+    for start in (0, 7, c - s, c - 1, c, c + 5, -1, -s, 1 << 40, -(1 << 40)):
+        got, want = fresh.clone(), fresh.clone()
+        y = _ops.norm_rope_qk_cache_fwd(q, k, v, wq, wk, cos, sin, got[0], got[1], 0, 1e-6, torch.tensor([start]).cuda())
+        big = torch.zeros((2, b, hk, c + 2 * s, d), dtype=BF, device='cuda')   # room on both sides
+        inside = max(-s, min(start, c))
+        x = _ops.norm_rope_qk_cache_fwd(q, k, v, wq, wk, cos, sin, big[0], big[1], inside + s, 1e-6)
+        lo, hi = max(inside, 0), min(inside + s, c)
+        want[:, :, :, lo:hi] = big[:, :, :, lo + s:hi + s]
+        assert torch.equal(y, x) and torch.equal(got, want), start
+
+
 def test_refusals(model):
     model, _ = model
     cache = model.new_cache(2, 20)
