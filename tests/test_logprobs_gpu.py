@@ -383,6 +383,34 @@ def test_lm_head_backward_again_and_of_one_result(h):
         torch.autograd.grad(out.entropy.sum(), wr)
 
 
+def test_lm_head_gradient_against_differences():
+    """As test_gradient_against_differences, along directions of hidden states and of the weight that move no logit by more than 1 a
+    unit; a logit's own sum (and the rounding of the moved operand) is off by at most (h + 8) 2^-24 sum |x w|, which moves a log
+    probability by twice that and an entropy by its largest |log p| + entropy + 1 <= 15 times as much."""
+    t, h, v = 6, 48, 40
+    x, w, ids = head(t, h, v, torch.float32)
+    gen = seeded(5)
+    g, gh, gt = (torch.randn(s, generator=gen).cuda() for s in ((t,), (t,), (t, 3)))
+
+    def loss(x, w):
+        out = lm_head_logprobs(x, w, ids, top=3)
+        return ((out.logprobs * g).sum().double() + (out.entropy * gh).sum().double() + (out.top_logprobs * gt).sum().double())
+    xr, wr = x.clone().requires_grad_(), w.clone().requires_grad_()
+    dx, dw = torch.autograd.grad(loss(xr, wr), (xr, wr))
+    step = 2.0 ** -7
+    size = float(g.abs().sum() + 15 * gh.abs().sum() + gt.abs().sum())
+    e = 2 * (h + 8) * E * float((x.double().abs() @ w.double().abs().t()).amax())
+    tol = size * 8 * step ** 2 / 6 + size * (400 * E * 10 + e) / step
+    for i in range(4):
+        vx, vw = ((torch.rand(s.shape, generator=seeded(10 * i + j)) * 2 - 1).cuda() for j, s in enumerate((x, w)))
+        vx /= (vx @ w.t()).abs().amax()
+        vw /= (x @ vw.t()).abs().amax()
+        fd = (loss(x + step * vx, w) - loss(x - step * vx, w)) / (2 * step)
+        assert abs(float(fd) - float((dx.double() * vx).sum())) <= tol
+        fd = (loss(x, w + step * vw) - loss(x, w - step * vw)) / (2 * step)
+        assert abs(float(fd) - float((dw.double() * vw).sum())) <= tol
+
+
 def test_lm_head_captured():
     """Forward and backward in captured graphs, replayed on other inputs beside eager calls."""
     def make(t, h, v):
