@@ -540,7 +540,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile_kernel(Args ar) {
             for (int k = 0; k < 4 * FN; ++k) v[k] = (k >> 2) * 16 + (k & 3) >= lim ? -INFINITY : v[k];
           }
           if (row < mrows) {
-            const int64_t t = ar.tgt[row] - col0;
+            const int64_t t = ar.tgt[row] - ar.col0 - col0;
             if (t >= 0 && t < min(clim, 128) && ((int)t & 12) == 4 * quarter) {
               const int at = ((int)t >> 4) * 4 + ((int)t & 3);
               float z = 0.f;

@@ -483,19 +483,37 @@ struct LogprobTile {
   double round;
 };
 constexpr LogprobTile kLogprobTile[4] = {{256, 256, 73.0}, {128, 256, 46.0}, {128, 128, 34.0}, {64, 128, 0.0}};
-int logprob_tile(int64_t M, int64_t N) {
-  if (M <= 64) return 3;
-  int best = 0;
-  double best_t = 0.0;
+// Whole rounds of one tile and the columns left in another as a second launch, where that is less than the rounds of one
+// (500 x 40000 x 2048 84 us and 99, 100 x 151936 x 4096 227 and 240, 999 x 151936 x 4096 974 and 996).
+struct LogprobPlan {
+  int cfg, rest;  // tiles of the first `cols` columns, and of those left
+  int64_t cols;
+};
+LogprobPlan logprob_plan(int64_t M, int64_t N, int64_t K) {
+  if (M <= 64) return {3, 3, N};
+  auto rounds = [&](int c, int64_t n) {
+    const LogprobTile& f = kLogprobTile[c];
+    return (double)cdiv(cdiv(M, f.bm) * cdiv(n, f.bn), 256) * f.round;
+  };
+  auto fewest = [&](int64_t n) {
+    int best = 0;
+    for (int c = 1; c < 3; ++c) best = rounds(c, n) < rounds(best, n) ? c : best;
+    return best;
+  };
+  LogprobPlan p{fewest(N), 0, N};
+  double t = rounds(p.cfg, N);
   for (int c = 0; c < 3; ++c) {
     const LogprobTile& f = kLogprobTile[c];
-    const double t = (double)cdiv(cdiv(M, f.bm) * cdiv(N, f.bn), 256) * f.round;
-    if (c == 0 || t < best_t) {
-      best = c;
-      best_t = t;
+    const int64_t tms = cdiv(M, f.bm), full = tms * cdiv(N, f.bn) / 256, cols = full * 256 / tms * f.bn;
+    if (cols <= 0 || cols >= N) continue;
+    const int rest = fewest(N - cols);
+    const double both = rounds(c, cols) + rounds(rest, N - cols) + 6.0 * 4096.0 / (double)K;  // the second launch's start and end
+    if (both < t) {
+      p = {c, rest, cols};
+      t = both;
     }
   }
-  return best;
+  return p;
 }
 
 }  // namespace
@@ -692,12 +710,26 @@ int q3_gemm_nt_logprobs(int dtype, const void* A, int64_t lda, const void* B, in
   a.pick = pick;
   a.ldp = ldp;
   a.c2 = inv_temperature * q3lp::kLog2e;
-  const int cfg = logprob_tile(M, N);
-  const int64_t tms = cdiv(M, kLogprobTile[cfg].bm), tns = cdiv(N, kLogprobTile[cfg].bn);
-  Q3_REQUIRE(tms * tns < (1ll << 31));
-  a.tms = (int)tms;
-  a.tns = (int)tns;
-  return q3gemm::launch_tile_nt(dtype, cfg, 6, a, stream);
+  const LogprobPlan p = logprob_plan(M, N, K);
+  for (int64_t at = 0; at < N; at += p.cols) {
+    const int cfg = at == 0 ? p.cfg : p.rest;
+    Args l = a;
+    l.N = at == 0 ? p.cols : N - at;
+    l.b.p[0] += at * ldb;
+    l.col0 = at;
+    l.m_part += at / 128 * ldp;
+    l.s_part += at / 128 * ldp;
+    l.u_part += at / 128 * ldp;
+    if (z) l.c[0] = (u16*)z + at;
+    const int64_t tms = cdiv(M, kLogprobTile[cfg].bm), tns = cdiv(l.N, kLogprobTile[cfg].bn);
+    Q3_REQUIRE(tms * tns < (1ll << 31));
+    l.tms = (int)tms;
+    l.tns = (int)tns;
+    const int rc = q3gemm::launch_tile_nt(dtype, cfg, 6, l, stream);
+    if (rc != 0) return rc;
+    if (at > 0) break;
+  }
+  return 0;
 }
 
 }  // extern "C"
