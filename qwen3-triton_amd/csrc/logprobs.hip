@@ -169,12 +169,13 @@ template <typename T> Q3_DEV i32x4 load_edge(const typename T::storage* row, int
   }
   return v;
 }
-// C vectors a thread of the slice that starts at element `base`, 256 threads side by side.
+// C vectors a thread of the slice that starts at element `base`, 256 threads side by side; past the caches, since each is read once
+// (4096 x 151936 bf16 206 us and 226 without, 1000 x 32000 19.5 either way; alternatives' second look takes as long).
 template <typename T, int C> Q3_DEV void load_slice(i32x4 (&v)[C], const typename T::storage* row, int64_t base, int64_t n) {
   constexpr int V = T::vec;
   if (base >= 0 && base + kThreads * V * C <= n) {
 #pragma unroll
-    for (int i = 0; i < C; ++i) v[i] = *reinterpret_cast<const i32x4*>(row + base + (i * kThreads + (int)threadIdx.x) * V);
+    for (int i = 0; i < C; ++i) v[i] = ld_nt(row + base + (i * kThreads + (int)threadIdx.x) * V);
   } else {
 #pragma unroll
     for (int i = 0; i < C; ++i) v[i] = load_edge<T>(row, base + (i * kThreads + (int)threadIdx.x) * V, n);
@@ -350,16 +351,19 @@ template <typename T> __global__ __launch_bounds__(kThreads) void finish_top_ker
 }
 
 // ---------------------------------------------------------------- gradient
-// N values as one store of N elements.
-template <typename O, int N> Q3_DEV void store_values(typename O::storage* p, const float (&v)[N]) {
+// N values as one store of N elements; FAR: past the caches.
+template <typename O, int N, bool FAR> Q3_DEV void store_values(typename O::storage* p, const float (&v)[N]) {
   if constexpr (N == O::vec) {
     Vec<O> o;
 #pragma unroll
     for (int e = 0; e < N; ++e) o.v[e] = v[e];
-    store_vec<O>(p, o);
+    if constexpr (FAR) st_nt<O>(p, o);
+    else store_vec<O>(p, o);
   } else {
     static_assert(N == 4 && O::vec == 8, "fp32 logits, 16-bit gradient");
-    *reinterpret_cast<i32x2*>(p) = i32x2{(int)pack2<O>(v[0], v[1]), (int)pack2<O>(v[2], v[3])};
+    const i32x2 o = {(int)pack2<O>(v[0], v[1]), (int)pack2<O>(v[2], v[3])};
+    if constexpr (FAR) __builtin_nontemporal_store(o, reinterpret_cast<i32x2*>(p));
+    else *reinterpret_cast<i32x2*>(p) = o;
   }
 }
 
@@ -377,8 +381,8 @@ struct Bwd {
 };
 
 // 32 (fp32: 16) values a thread, all loads before the first use; bound by the logits' read and the gradient's write (2048 x 151936
-// bf16: 1.24 GB in 270 us).  Rows left out are zeros, and nothing of them is read.
-template <typename T, typename O> __global__ __launch_bounds__(kThreads) void grad_kernel(Bwd a, int slices) {
+// bf16: 1.24 GB in 260 us).  Rows left out are zeros, and nothing of them is read.
+template <typename T, typename O, bool FAR> __global__ __launch_bounds__(kThreads) void grad_kernel(Bwd a, int slices) {
   typedef typename T::storage S;
   typedef typename O::storage SO;
   constexpr int V = T::vec, C = kGradVectors, N = kThreads * V * C;
@@ -459,7 +463,7 @@ template <typename T, typename O> __global__ __launch_bounds__(kThreads) void gr
       for (int e = 0; e < V; ++e) o[e] = 0.f;
     }
     if (whole || (i0 >= 0 && i0 + V <= a.vocab)) {
-      store_values<O, V>(out + i0, o);
+      store_values<O, V, FAR>(out + i0, o);
     } else {
 #pragma unroll
       for (int e = 0; e < V; ++e)
@@ -566,7 +570,7 @@ template <typename O> __global__ __launch_bounds__(kThreads) void head_grad_kern
 #pragma unroll
       for (int e = 0; e < 8; ++e) o[e] = 0.f;
     }
-    store_values<O, 8>(row + i0, o);
+    store_values<O, 8, false>(row + i0, o);
   }
 }
 
@@ -620,7 +624,12 @@ template <typename T> int forward(const Fwd& a, int chunks, hipStream_t s) {
 
 template <typename T, typename O> int backward(const Bwd& a, hipStream_t s) {
   const int64_t n = cdiv(a.vocab + T::vec - 1, (int64_t)kThreads * T::vec * kGradVectors);
-  grad_kernel<T, O><<<(unsigned)(a.rows * n), kThreads, 0, s>>>(a, (int)n);
+  // A gradient of more than 256 MiB does not pass through the caches (2048 x 151936 bf16 276 us and 288 through them, 777 fp32 157 and
+  // 170); a smaller one is there for who reads it next.
+  if (a.rows * a.vocab * (int64_t)sizeof(typename O::storage) > (256 << 20))
+    grad_kernel<T, O, true><<<(unsigned)(a.rows * n), kThreads, 0, s>>>(a, (int)n);
+  else
+    grad_kernel<T, O, false><<<(unsigned)(a.rows * n), kThreads, 0, s>>>(a, (int)n);
   return (int)hipGetLastError();
 }
 
