@@ -116,7 +116,8 @@ Q3_DEV void work_coords(int bid, int tiles_m, int tiles_n, int splits, int& tm, 
 // the rounded logits, which are stored too; 3: gate/up SwiGLU; 5: SwiGLU backward; 6: log probability statistics
 // (logprobs.h) of the fp32 logits per row and 128-column group, to m_part, s_part and u_part, with the logit of column tgt[row]
 // to pick[row], and where c[0] is set the logits' distances to their group's maximum in 16 bits (q3lp::kGapRange).  4096 x 151936 x 4096 takes 3.71 ms
-// with the statistics alone and 3.91 with the distances (1.30 PFLOP/s), as a plain product that writes its logits 3.76.  KP: A and B in pieces along K.
+// with the statistics alone and 3.91 with the distances (1.30 PFLOP/s), as a plain product that writes its logits 3.76.  7: as 6, and B
+// is read past the caches (non-temporal).  KP: A and B in pieces along K.
 template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool AT, bool BT, int EPI, bool KP, bool Q8>
 __global__ __launch_bounds__(WM * WN * 64) void gemm_tile_kernel(Args ar) {
   constexpr int NW = WM * WN;
@@ -266,7 +267,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile_kernel(Args ar) {
         char* dst = st + ABYTES + (BT ? slot_base(q) : q * 1024);
         const int rr = EPI == 3 ? ((q >> 2) * 2 + (q & 1)) * 16 : q * (BT ? 2 : 16);  // row offset x 2 bytes
         __builtin_amdgcn_raw_ptr_buffer_load_lds(db, (__attribute__((address_space(3))) void*)dst, 16,
-                                                 vb + (uint32_t)(rr * (int)ldb), 0, 0, 0);
+                                                 vb + (uint32_t)(rr * (int)ldb), 0, 0, EPI == 7 ? 2 : 0);
       }
     }
   };
@@ -519,7 +520,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile_kernel(Args ar) {
       const int c = lane % CH;
       const int rlim = mrows - ma - wm * TMW;  // valid rows / columns of the wave's block
       auto row_chunk = [&](int r) { return *reinterpret_cast<const i32x4*>(wl + r * (NC * 2) + ((c ^ swz(r)) << 4)); };
-      if constexpr (EPI == 6) {
+      if constexpr (EPI == 6 || EPI == 7) {
         // A lane's 32 values of a row, then the row's four lanes; each row block's accumulators are dead before the next's.
         static_assert(TNW == 128 && CH == 16, "one statistics partial per wave and row");
         const int col0 = nb + wn * TNW, clim = ncols - col0;

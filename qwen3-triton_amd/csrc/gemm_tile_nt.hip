@@ -30,9 +30,19 @@ template <typename T> static int logprobs(int cfg, const Args& a, hipStream_t s)
   }
 }
 
+// Weights that are read once, past the caches: tiles of up to 128 rows.
+template <typename T> static int logprobs_once(int cfg, const Args& a, hipStream_t s) {
+  switch (cfg) {
+    case 1: return launch_tile<T, 128, 256, 4, 2, 3, false, false, 7>(a, s);
+    case 2: return launch_tile<T, 128, 128, 8, 1, 3, false, false, 7>(a, s);
+    default: return launch_tile<T, 64, 128, 4, 1, 3, false, false, 7>(a, s);
+  }
+}
+
 int launch_tile_nt(int dtype, int cfg, int epi, const Args& a, hipStream_t s) {
   if (epi == 2) return dtype == Q3_BF16 ? stats<BF16>(cfg, a, s) : stats<F16>(cfg, a, s);
   if (epi == 6) return dtype == Q3_BF16 ? logprobs<BF16>(cfg, a, s) : logprobs<F16>(cfg, a, s);
+  if (epi == 7) return dtype == Q3_BF16 ? logprobs_once<BF16>(cfg, a, s) : logprobs_once<F16>(cfg, a, s);
   if (epi == 3) return dtype == Q3_BF16 ? nt<BF16, 3>(cfg, a, s) : nt<F16, 3>(cfg, a, s);
   return dtype == Q3_BF16 ? nt<BF16, 0>(cfg, a, s) : nt<F16, 0>(cfg, a, s);
 }

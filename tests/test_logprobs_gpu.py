@@ -343,8 +343,8 @@ def test_lm_head_alternatives_and_needs(dtype):
         assert bool(got.isfinite().all())
 
 
-# a tile of each kind above 64 rows, two of them beside each other, and dX with its sum over the vocabulary in more than eight parts
-@pytest.mark.parametrize("t,h,v", [(200, 64, 32008), (1000, 64, 16376), (100, 192, 9000), (500, 1024, 40000), (16, 256, 70000), (40, 128, 36000)])
+# a tile of each kind above 64 rows, two of them beside each other, weights beyond the caches, and dX with its sum over the vocabulary in more than eight parts
+@pytest.mark.parametrize("t,h,v", [(200, 64, 32008), (1000, 64, 16376), (100, 192, 9000), (500, 1024, 40000), (8, 1024, 140000), (100, 1024, 140000), (16, 256, 70000), (40, 128, 36000)])
 def test_lm_head_of_other_sizes(t, h, v):
     test_lm_head(t, h, v, torch.bfloat16)
 
