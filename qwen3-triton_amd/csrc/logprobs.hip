@@ -13,8 +13,8 @@
 // Bound by the logits, read once (forward) or read and written once (backward).  A workgroup holds its slice of a row in
 // registers: the slice's maximum, then the sums, then the alternatives are taken from them.  Many rows take slices of 32 values (fp32: 16) a
 // thread; few rows small ones, so that one row's latency is spread over many CUs.  A second launch joins a row's slices.
-// On MI355X (kernels alone, 151936 logits a row): 4096 rows of bf16 212 + 5 us (5.9 TB/s), 777 of fp32 with 5 alternatives 101 + 7
-// (4.7 TB/s), one row with 20 alternatives 7.3 + 6.3; the gradient of 2048 bf16 rows 270 us (4.6 TB/s).
+// On MI355X (kernels alone, 151936 logits a row): 4096 rows of bf16 197 + 5 us (6.3 TB/s), 777 of fp32 with 5 alternatives 75 + 7 (6.2 TB/s),
+// one row with 20 alternatives 7.3 + 6.3; the gradient of 2048 bf16 rows 260 us (4.8 TB/s).
 #include <algorithm>
 
 #include "logprobs.h"
@@ -43,7 +43,8 @@ Q3_DEV uint64_t key_xor(uint64_t x, int mask) {
 
 // The k largest (k <= kMaxTop) of a workgroup's values in order, to emit(rank, key) by some thread each; ranks that no value
 // takes get key 0.  most: the order of the thread's largest value (0: it has none); scan(f) calls f(order, index) for each of
-// its values, order 0 for none, and may read them again: few threads call it.
+// its values, order 0 for none, and may read them again; collect(reaches, f), called by all threads, does so for at least the values
+// of the threads for which `reaches`.
 //  * The 64 maxima of groups of 4 threads: the k-th largest of those is a bound that at least k values reach.  Of random
 //    values about 1.3 k do; they are collected and ranked by counting the larger ones.
 //  * More than kCand may reach it (ties, a row that rises, few values that are not -inf): then k rounds, each the largest key
@@ -56,8 +57,8 @@ struct TopScratch {
   uint32_t bound;
   int count;
 };
-template <typename Scan, typename Emit>
-Q3_DEV void block_top(TopScratch& sc, int k, uint32_t most, Scan&& scan, Emit&& emit) {
+template <typename Collect, typename Scan, typename Emit>
+Q3_DEV void block_top(TopScratch& sc, int k, uint32_t most, Collect&& collect, Scan&& scan, Emit&& emit) {
   const int tid = threadIdx.x;
   uint32_t g = max(most, (uint32_t)__shfl_xor((int)most, 1, 64));
   g = max(g, (uint32_t)__shfl_xor((int)g, 2, 64));
@@ -76,13 +77,12 @@ Q3_DEV void block_top(TopScratch& sc, int k, uint32_t most, Scan&& scan, Emit&& 
   }
   __syncthreads();
   const uint32_t bound = sc.bound;
-  if (most >= bound && most != 0)
-    scan([&](uint32_t o, uint32_t i) {
-      if (o >= bound && o != 0) {
-        const int at = atomicAdd(&sc.count, 1);
-        if (at < kCand) sc.cand[at] = key_of(o, i);
-      }
-    });
+  collect(most >= bound && most != 0, [&](uint32_t o, uint32_t i) {
+    if (o >= bound && o != 0) {
+      const int at = atomicAdd(&sc.count, 1);
+      if (at < kCand) sc.cand[at] = key_of(o, i);
+    }
+  });
   __syncthreads();
   const int n = sc.count;
   if (n <= kCand) {
@@ -220,11 +220,26 @@ __global__ __launch_bounds__(kThreads) void slice_kernel(Fwd a) {
   }
   if constexpr (TOP) {
     __shared__ TopScratch sc;
+    __shared__ int who[kThreads], whos;
     uint64_t* out = a.key + (r * a.parts + part) * a.top;
     const int64_t begin = (int64_t)first * N - mis + tid * V;  // of the thread's first vector
     const bool any = begin < a.vocab && begin + V > 0 && tid * V < N;
     const uint32_t most = !any ? 0 : p.rest != p.rest ? order32(NAN) : order32(p.m);
-    block_top(sc, a.top, most, [&](auto&& f) {
+    if (tid == 0) whos = 0;
+    // The threads whose maximum reaches the bound are few, but one in most waves: all threads read a vector of theirs each (5 of 777 bf16
+    // rows 66 us, 10 of 2000 133; each such thread its own, one after the other, 100 and 225).
+    block_top(sc, a.top, most, [&](bool reaches, auto&& f) {
+      if (reaches) who[atomicAdd(&whos, 1)] = tid;
+      __syncthreads();
+      const int each = (last - first) * C, n = whos * each;
+      for (int j = tid; j < n; j += kThreads) {
+        const int v = j % each;
+        const int64_t base = (int64_t)(first + v / C) * N - mis, i0 = base + (v % C * kThreads + who[j / each]) * V, end = min(a.vocab, base + N);
+        const Vec<T> x = unpack_vec<T>(load_edge<T>(row, i0, end));
+#pragma unroll
+        for (int e = 0; e < V; ++e) f(i0 + e >= 0 && i0 + e < end ? order32(x.v[e]) : 0, (uint32_t)(i0 + e));
+      }
+    }, [&](auto&& f) {
       for (int sl = last - 1; sl >= first; --sl) {
         if (last - first > 1) load(sl);
         float x[C * V];
@@ -339,11 +354,14 @@ template <typename T> __global__ __launch_bounds__(kThreads) void finish_top_ker
 #pragma unroll
   for (int i = 0; i < R; ++i) most = max(most, (uint32_t)(mine[i] >> 32));
   for (int i = tid + R * kThreads; i < n; i += kThreads) most = max(most, (uint32_t)(key[i] >> 32));
-  block_top(sc, a.top, most, [&](auto&& f) {
+  auto scan = [&](auto&& f) {
 #pragma unroll
     for (int i = 0; i < R; ++i) f((uint32_t)(mine[i] >> 32), ~(uint32_t)mine[i]);
     for (int i = tid + R * kThreads; i < n; i += kThreads) f((uint32_t)(key[i] >> 32), ~(uint32_t)key[i]);
-  }, [&](int rank, uint64_t k) {  // behind barriers: row_part is there
+  };
+  block_top(sc, a.top, most, [&](bool reaches, auto&& f) {
+    if (reaches) scan(f);
+  }, scan, [&](int rank, uint64_t k) {  // behind barriers: row_part is there
     a.top_token[r * a.top + rank] = (int64_t)(uint32_t)~(uint32_t)k;
     const float x = unorder32((uint32_t)(k >> 32));
     a.top_logprob[r * a.top + rank] = row_part.m == -INFINITY ? NAN : fmaf(x - row_part.m, a.c, -log1pf(row_part.rest));
@@ -595,12 +613,12 @@ bool sizes_ok(int dtype, int64_t rows, int64_t vocab, int64_t top) {
   return rows * cdiv(vocab + 16, kThreads * vec_of(dtype)) < (1ll << 31) - 1;
 }
 
-// Slices of a workgroup: as many as leave 4096 workgroups, dealt out evenly (4096 rows of 151936 226 us, 2048 117, 777 of fp32 with 5 alternatives 112; one slice each
-// 229, 118 and 158; 2048 rows in parts of 9, 9 and 1 121); where alternatives are wanted at most 6, so that what is read again for
-// them is still in a cache.
+// Slices of a workgroup, dealt out evenly.  Without alternatives as many as leave 4096 workgroups (rows of 151936 bf16: 4096 of them 206
+// us, 229 with one slice each, 2048 108).  With them as many as leave 2048, at most 6, since each workgroup ends with a search (5 of
+// 777 rows 59 us, leaving 4096 66; 20 of 300 41 and 54; 5 of 777 fp32 rows 89, with up to 13 slices 93).
 int per_for(int64_t rows, int64_t slices, int64_t top) {
-  const int64_t most = std::max<int64_t>(1, std::min<int64_t>(top > 0 ? std::min<int64_t>(slices, 6) : slices, rows * slices / 4096));
-  return (int)cdiv(slices, cdiv(slices, most));
+  const int64_t most = top > 0 ? std::min<int64_t>(std::min<int64_t>(slices, 6), rows * slices / 2048) : std::min(slices, rows * slices / 4096);
+  return (int)cdiv(slices, cdiv(slices, std::max<int64_t>(1, most)));
 }
 
 template <typename T, int C> void slices(const Fwd& a, hipStream_t s) {
