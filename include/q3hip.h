@@ -603,9 +603,9 @@ int q3_head_logprobs_bwd(int dtype, void* z, int64_t ldz, int64_t rows, int64_t 
  * (P = 0 and a negative end) gets zeros.  Strides in elements, of batch, head and position (keys and values alike): multiples
  * of 8 with 16-byte aligned bases, position strides in [128, 2^24); of out multiples of 4, 8-byte aligned.
  * start_dev: that device int64 (starts = 1) or one a row (starts = B) instead of start, read when the kernel runs; positions
- * outside the capacity are not there.  The workspace is sized for span = C then, else for span = start + S. */
+ * outside the capacity are not there.  The workspace is sized for span = C then, else for span = start + S; it may be empty. */
 size_t q3_prefix_attention_workspace_bytes(int64_t B, int64_t R, int64_t S, int64_t Hq, int64_t Hkv, int64_t P,
-                                           int64_t span);
+                                           int64_t C, int64_t span);
 int q3_prefix_attention(int dtype, const void* q, int64_t qsb, int64_t qss, int64_t qsh, const void* prefix_k,
                         const void* prefix_v, int64_t psb, int64_t psh, int64_t pss, const void* cache_k,
                         const void* cache_v, int64_t csb, int64_t csh, int64_t css, void* out, int64_t osb, int64_t oss,

@@ -14,7 +14,8 @@
 //    wave's own), without waiting for each other, and their sums are joined in LDS.  A decode step's own positions are such jobs:
 //    they wait for memory beside the prefix's jobs, which are bound by the matrix cores.
 // Jobs leave unnormalised O, maximum and sum, which a second launch joins in a fixed order.  Where the queries of single rows fill
-// tiles and the tiles the chip, a job goes through the prefix and then its row's own positions, and writes the result.
+// tiles and the tiles the chip, and where there are few positions in all, a job goes through the prefix and then its row's own
+// positions, and writes the result.
 #include <algorithm>
 #include <type_traits>
 
@@ -683,7 +684,7 @@ struct Plan {
   int64_t pjobs, sjobs;
 };
 constexpr int kMinPer = 4;  // blocks of a split at least
-Plan plan_for(int64_t R, int64_t n, int64_t S, int64_t Hkv, int64_t G, int64_t P, int64_t span) {
+Plan plan_for(int64_t R, int64_t n, int64_t S, int64_t Hkv, int64_t G, int64_t P, int64_t C, int64_t span) {
   Plan p{};
   const int64_t B = R * n, SG = S * G, pblocks = cdiv(P, BLK);
   // One pass over everything, a row's own queries in tiles of 256, a tile a CU: where the queries fill more than 11 / 20 of the
@@ -710,6 +711,19 @@ Plan plan_for(int64_t R, int64_t n, int64_t S, int64_t Hkv, int64_t G, int64_t P
   p.sfew = SG <= few;
   p.nw = 4;
   p.ptiles = 1;
+  // One pass a row and head over its prefix and its own positions where few blocks of both fit (counted by the capacity, so that a captured
+  // step goes the way of an eager call): no second launch and no partial sums, but a prefix is read once a row.  By the rounds of a
+  // job's four waves (2.2 us each) against the two launches (us, single queries behind 200 and 500 positions, a position block of
+  // their own): 1 row 7.1 and 8.7, 9.5 and 9.0; 8 rows of 8 heads 7.3 and 10.9, 9.6 and 11.3; 32 7.4 and 14.1, 9.7 and 14.3; 64 9.8
+  // and 14.5, 14.9 and 14.8.  Four rounds: 8 rows 11.8 and 11.3, 32 14.5 and 17.9, 64 23.7 and 23.7.
+  const int64_t rounds = cdiv(pblocks + cdiv(C, BLK), 4), jobs = B * Hkv;
+  if (p.sfew && jobs <= 512 && rounds <= (jobs > 256 ? 2 : jobs >= 64 ? 4 : 3)) {
+    p.fused = 1;
+    p.stiles = p.ssplits = p.max_splits = p.slots = 1;
+    p.sjobs = jobs;
+    p.pfew = 0;
+    return p;
+  }
   if (P > 0) {
     p.ptiles = p.pfew ? 1 : (int)cdiv(n * SG, 128);
     const int64_t want = std::max<int64_t>(1, kJobs / (R * Hkv * p.ptiles));
@@ -744,9 +758,9 @@ template <typename T> int run(const Plan& p, const Args& a, int64_t rows, hipStr
     else
       prefix_few_kernel<T, 1, TILES, true><<<grid, 256, 0, s>>>(a);
   };
-  if (p.fused) prefix_tile_kernel<T, 8><<<grid, 512, 0, s>>>(a);
+  if (p.nw == 8) prefix_tile_kernel<T, 8><<<grid, 512, 0, s>>>(a);
   else if (!p.sfew) prefix_tile_kernel<T, 4><<<grid, 256, 0, s>>>(a);
-  else if (p.pfew || a.P == 0) few(std::false_type{});
+  else if (p.pfew || p.fused || a.P == 0) few(std::false_type{});
   else few(std::true_type{});
   const int rc = (int)hipGetLastError();
   if (p.slots == 1) return rc;
@@ -760,9 +774,10 @@ template <typename T> int run(const Plan& p, const Args& a, int64_t rows, hipStr
 
 extern "C" {
 
-size_t q3_prefix_attention_workspace_bytes(int64_t B, int64_t R, int64_t S, int64_t Hq, int64_t Hkv, int64_t P, int64_t span) {
-  if (!sizes_ok(B, R, S, Hq, Hkv, P, std::max<int64_t>(span, S)) || span < 0) return 0;
-  return bytes_for(plan_for(R, B / R, S, Hkv, Hq / Hkv, P, span), B * S * Hq);
+size_t q3_prefix_attention_workspace_bytes(int64_t B, int64_t R, int64_t S, int64_t Hq, int64_t Hkv, int64_t P, int64_t C,
+                                           int64_t span) {
+  if (!sizes_ok(B, R, S, Hq, Hkv, P, C) || span < 0 || span > C) return 0;
+  return bytes_for(plan_for(R, B / R, S, Hkv, Hq / Hkv, P, C, span), B * S * Hq);
 }
 
 int q3_prefix_attention(int dtype, const void* q, int64_t qsb, int64_t qss, int64_t qsh, const void* prefix_k, const void* prefix_v,
@@ -777,7 +792,7 @@ int q3_prefix_attention(int dtype, const void* q, int64_t qsb, int64_t qss, int6
   Q3_REQUIRE(out && al(out, 8) && osb % 4 == 0 && oss % 4 == 0 && osh % 4 == 0);
   Q3_REQUIRE(start_dev ? (starts == 1 || starts == B) : (start >= 0 && start + S <= C));
   const int64_t n = B / R, span = start_dev ? C : start + S, rows = B * S * Hq;
-  const Plan p = plan_for(R, n, S, Hkv, Hq / Hkv, P, span);
+  const Plan p = plan_for(R, n, S, Hkv, Hq / Hkv, P, C, span);
   const size_t need = bytes_for(p, rows);
   Q3_REQUIRE(p.pjobs + p.sjobs < (1ll << 31) && (need == 0 || (workspace && al(workspace, 16) && workspace_bytes >= need)));
   Args a{};

@@ -144,7 +144,7 @@ SIGNATURES: dict[str, tuple] = {
     "q3_gemm_nt_logprobs": (_i32, [_i32, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _f32, _p, _p, _p, _p, _i64, _p, _i64, _p]),
     "q3_head_logprobs_finish": (_i32, [_p, _p, _p, _i64, _p, _i64, _i64, _p, _i64, _f32, _p, _p, _p, _p, _p]),
     "q3_head_logprobs_bwd": (_i32, [_i32, _p, _i64, _i64, _i64, _p, _i64, _f32, _p, _i64, _p, _p, _p, _p, _p, _p, _p]),
-    "q3_prefix_attention_workspace_bytes": (_sz, [_i64] * 7),
+    "q3_prefix_attention_workspace_bytes": (_sz, [_i64] * 8),
     "q3_prefix_attention": (_i32, [_i32, _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _i64,
                                    _i64, _i64, _p, _sz, *[_i64] * 9, _p, _i64, _f32, _p]),
     "q3_gemm_strided": (_i32, [_i32, _i32, _p, _i64, _i64, _p, _i64, _i64, _p, _i64, _i64, _i64, _i64, _f32, _i32,

@@ -77,7 +77,7 @@ def attention(q, prefix_k, prefix_v, cache_k, cache_v, start, start_dev=None, *,
     if b * s * hq >= 1 << 31 or max(p, c) >= 1 << 30 or b >= 1 << 24:
         raise ValueError('fewer than 2^31 query rows, 2^30 positions and 2^24 rows required')
     out = q.new_empty((b, s, hq, d))
-    nbytes = H.query("q3_prefix_attention_workspace_bytes", b, r, s, hq, hkv, p, start + s if start_dev is None else c)
+    nbytes = H.query("q3_prefix_attention_workspace_bytes", b, r, s, hq, hkv, p, c, start + s if start_dev is None else c)
     ws = H.workspace(nbytes, q.device) if nbytes else None
     H.launch(q, "q3_prefix_attention", H.code(dt), q.data_ptr(), qb, qs, qh, prefix_k.data_ptr(), prefix_v.data_ptr(), *ps,
              cache_k.data_ptr(), cache_v.data_ptr(), *cs, out.data_ptr(), s * hq * d, hq * d, d,

@@ -37,14 +37,15 @@ def test_prefix_attention_refusals(bad):
 
 def test_prefix_workspace():
     q = lambda *a: H.query("q3_prefix_attention_workspace_bytes", *a)
-    assert q(0, 1, 1, 32, 8, 100, 10) == q(4, 3, 1, 32, 8, 100, 10) == q(4, 1, 1, 32, 5, 100, 10) == q(4, 1, 1, 32, 8, -1, 10) == 0
-    assert q(4, 1, 1, 32, 8, 100, -1) == 0
-    some = q(4, 1, 1, 32, 8, 1000, 10)
+    assert q(0, 1, 1, 32, 8, 1000, 90, 10) == q(4, 3, 1, 32, 8, 1000, 90, 10) == q(4, 1, 1, 32, 5, 1000, 90, 10) == q(4, 1, 1, 32, 8, -1, 90, 10) == 0
+    assert q(4, 1, 1, 32, 8, 1000, 90, -1) == q(4, 1, 1, 32, 8, 1000, 90, 91) == 0
+    some = q(4, 1, 1, 32, 8, 1000, 90, 10)
     assert some >= 2 * 128 * 130 * 4 and some % (128 * 130 * 4) == 0     # a slot of the prefix, a slot of its own, per query row
-    assert q(64, 1, 300, 32, 8, 4000, 300) == 0                          # many queries: no partials
+    assert q(64, 1, 300, 32, 8, 4000, 300, 300) == 0                     # many queries: no partials
+    assert q(4, 1, 1, 32, 8, 300, 90, 10) == 0                           # few positions: none either
     # no more for a longer prefix once its splits fill the chip; never more than the splits that fill it
-    assert q(32, 1, 1, 32, 8, 1 << 20, 10) <= 32 * 32 * 130 * 4 * 1024
-    for args in ((1, 1, 1, 8, 8, 0, 1 << 20), (1, 1, 1, 1, 1, 1 << 20, 1 << 20), (1 << 20, 1, 1, 1, 1, 1, 1)):
+    assert q(32, 1, 1, 32, 8, 1 << 20, 90, 10) <= 32 * 32 * 130 * 4 * 1024
+    for args in ((1, 1, 1, 8, 8, 0, 1 << 20, 1 << 20), (1, 1, 1, 1, 1, 1 << 20, 1 << 20, 1 << 20), (1 << 20, 1, 1, 1, 1, 1, 1, 1)):
         assert q(*args) >= 0
 
 

@@ -74,7 +74,9 @@ def check(got, q, pk, pv, ck, cv, starts, scale=None):
     (1, 33, 1, 4, 1, 257, 0), (3, 1, 1, 3, 1, 100, 100), (1, 4, 1, 14, 2, 70, 5),
     (1, 2, 2, 8, 2, 100, 0), (1, 3, 17, 8, 2, 64, 50), (2, 2, 33, 4, 4, 130, 64), (1, 1, 300, 8, 2, 77, 100), (1, 2, 65, 16, 2, 1, 1),
     (1, 8, 100, 32, 8, 333, 10), (1, 24, 40, 32, 8, 90, 3), (1, 1, 64, 4, 1, 64, 0), (2, 16, 130, 16, 8, 65, 77),
-    (1, 24, 56, 32, 8, 90, 3), (2, 16, 250, 16, 8, 65, 77), (1, 4, 2, 32, 8, 300, 9), (1, 1, 8, 32, 8, 700, 100)])
+    (1, 24, 56, 32, 8, 90, 3), (2, 16, 250, 16, 8, 65, 77), (1, 4, 2, 32, 8, 300, 9), (1, 1, 8, 32, 8, 700, 100),
+    (1, 4, 1, 32, 8, 1500, 7), (1, 8, 1, 32, 8, 2000, 300), (2, 5, 1, 6, 2, 1100, 64), (1, 4, 4, 8, 2, 1500, 60), (3, 11, 1, 8, 8, 600, 70),
+    (1, 65, 1, 32, 8, 200, 9), (1, 1, 1, 71, 1, 1000, 20), (1, 2, 4, 16, 4, 900, 600)])
 def test_against_64_bits(r, n, s, hq, hkv, p, start, dtype):
     print(f"prefix {r}x{n} S{s} {hq}/{hkv} P{p} start {start} {dtype}", flush=True)
     t = inputs(r, n, s, hq, hkv, p, start + s + 9, dtype)
@@ -125,14 +127,14 @@ def test_what_lies_behind_the_last_position_counts_for_nothing(s, n, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("n,s", [(2, 40), (24, 40), (2, 18), (24, 56)])
-def test_a_value_that_is_not_finite_stays_with_the_queries_that_see_it(n, s, dtype):
-    t = inputs(1, n, s, 32, 8, 70, 120, dtype)
+@pytest.mark.parametrize("n,s,start,p", [(2, 40, 20, 70), (24, 40, 20, 70), (2, 18, 20, 70), (24, 56, 20, 70), (2, 4, 28, 70), (2, 4, 28, 3000), (2, 4, 35, 70)])
+def test_a_value_that_is_not_finite_stays_with_the_queries_that_see_it(n, s, start, p, dtype):
+    t = inputs(1, n, s, 32, 8, p, 120, dtype)
     cv = t[4]
     cv[:, :, 30, 5], cv[:, :, 37, 8], cv[0, :, 33, :] = float('inf'), float('nan'), -float('inf')
-    got = PX.attention(*t, 20)
-    o, tol = expected(*t, [20] * n)
-    pos = 20 + torch.arange(s, device='cuda')
+    got = PX.attention(*t, start)
+    o, tol = expected(*t, [start] * n)
+    pos = start + torch.arange(s, device='cuda')
     bad = torch.zeros((n, s, 128), dtype=torch.bool, device='cuda')
     bad[:, pos >= 30, 5] = True
     bad[:, pos >= 37, 8] = True
