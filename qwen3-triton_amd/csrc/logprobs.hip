@@ -12,8 +12,9 @@
 //
 // Bound by the logits, read once (forward) or read and written once (backward).  A workgroup holds its slice of a row in
 // registers: the slice's maximum, then the sums, then the alternatives are taken from them.  Many rows take slices of 32 values (fp32: 16) a
-// thread; few rows small ones, so that one row's latency is spread over many CUs.  A second launch joins a row's slices.
-// On MI355X (kernels alone, 151936 logits a row): 4096 rows of bf16 197 + 5 us (6.3 TB/s), 777 of fp32 with 5 alternatives 75 + 7 (6.2 TB/s),
+// thread; few rows small ones, so that one row's latency is spread over many CUs.  A second launch joins a
+// row's slices, unless one workgroup goes through all of them (short rows; very many rows).
+// On MI355X (kernels alone, 151936 logits a row): 4096 rows of bf16 196 us (6.4 TB/s), 777 of fp32 with 5 alternatives 75 + 7 (6.2 TB/s),
 // one row with 20 alternatives 7.3 + 6.3; the gradient of 2048 bf16 rows 260 us (4.8 TB/s).
 #include <algorithm>
 
@@ -190,20 +191,53 @@ template <typename T, int C> Q3_DEV void unpack(float (&x)[C * T::vec], const i3
   }
 }
 
+// A row's results from its statistics.
+Q3_DEV void finish_row(const Fwd& a, int64_t r, const Part& p, float picked, bool valid) {
+  const float ls = log1pf(p.rest), d = picked - p.m;
+  const bool none = p.m == -INFINITY;
+  a.logprob[r] = valid ? fmaf(d, a.c, -ls) : NAN;
+  a.entropy[r] = none ? NAN : fmaf(-kLn2, p.u / (1.f + p.rest), ls);
+  a.m[r] = p.m;
+  a.ls[r] = none ? NAN : ls;
+}
+
+// The alternative of a rank, from its key.
+Q3_DEV void finish_top(const Fwd& a, int64_t r, int rank, uint64_t k, const Part& p) {
+  a.top_token[r * a.top + rank] = (int64_t)(uint32_t)~(uint32_t)k;
+  const float x = unorder32((uint32_t)(k >> 32));
+  a.top_logprob[r * a.top + rank] = p.m == -INFINITY ? NAN : fmaf(x - p.m, a.c, -log1pf(p.rest));
+}
+
+// Called by the row's threads 0 .. kMaxTop - 1 at least.
+Q3_DEV void left_out(const Fwd& a, int64_t r, int tid) {
+  if (tid == 0) a.logprob[r] = a.entropy[r] = a.m[r] = a.ls[r] = 0.f;
+  if (tid < a.top) {
+    a.top_logprob[r * a.top + tid] = 0.f;
+    a.top_token[r * a.top + tid] = 0;
+  }
+}
+
 // Bound by the logits where rows are many (the next slice is on its way beside the sums: with part_of's four chains of 32 values
 // these take about as long as the loads), by one trip to memory and the reductions where they are few.
-template <typename T, int C, bool TOP>
+// ONE: the workgroup's slices are the whole row, whose results it writes.
+template <typename T, int C, bool TOP, bool ONE>
 __global__ __launch_bounds__(kThreads) void slice_kernel(Fwd a) {
   typedef typename T::storage S;
   constexpr int V = T::vec;
   const int N = a.span;
-  const int64_t r = blockIdx.x / (unsigned)a.parts;
-  const int part = (int)(blockIdx.x - (unsigned)(r * a.parts)), tid = threadIdx.x;
-  if (a.tok[r] == a.ignore) return;  // the whole workgroup: nothing of the row is read
+  const int64_t r = ONE ? blockIdx.x : blockIdx.x / (unsigned)a.parts;
+  const int part = ONE ? 0 : (int)(blockIdx.x - (unsigned)(r * a.parts)), tid = threadIdx.x;
+  const int64_t t = a.tok[r];
+  if (t == a.ignore) {  // the whole workgroup: nothing of the row is read
+    if (ONE) left_out(a, r, tid);
+    return;
+  }
   const S* row = (const S*)a.z + r * a.ld;
   const int mis = misaligned<T>(row);
   const float c2 = a.c * kLog2e;
-  const int first = part * a.per, last = min(first + a.per, a.slices);
+  const int first = part * a.per, last = ONE ? a.slices : min(first + a.per, a.slices);
+  const bool valid = t >= 0 && t < a.vocab;
+  [[maybe_unused]] const float picked = ONE && tid == 0 && valid ? to_f32<T>(row[t]) : 0.f;
   Part p{-INFINITY, 0.f, 0.f};
   i32x4 raw[C];
   auto load = [&](int sl) {
@@ -218,43 +252,11 @@ __global__ __launch_bounds__(kThreads) void slice_kernel(Fwd a) {
     const Part q = part_of(x, c2);
     p = sl == first ? q : join(p, q, c2);
   }
+  [[maybe_unused]] uint32_t most = 0;  // the order of the thread's largest value
   if constexpr (TOP) {
-    __shared__ TopScratch sc;
-    __shared__ int who[kThreads], whos;
-    uint64_t* out = a.key + (r * a.parts + part) * a.top;
     const int64_t begin = (int64_t)first * N - mis + tid * V;  // of the thread's first vector
     const bool any = begin < a.vocab && begin + V > 0 && tid * V < N;
-    const uint32_t most = !any ? 0 : p.rest != p.rest ? order32(NAN) : order32(p.m);
-    if (tid == 0) whos = 0;
-    // The threads whose maximum reaches the bound are few, but one in most waves: all threads read a vector of theirs each (5 of 777 bf16
-    // rows 66 us, 10 of 2000 133; each such thread its own, one after the other, 100 and 225).
-    block_top(sc, a.top, most, [&](bool reaches, auto&& f) {
-      if (reaches) who[atomicAdd(&whos, 1)] = tid;
-      __syncthreads();
-      const int each = (last - first) * C, n = whos * each;
-      for (int j = tid; j < n; j += kThreads) {
-        const int v = j % each;
-        const int64_t base = (int64_t)(first + v / C) * N - mis, i0 = base + (v % C * kThreads + who[j / each]) * V, end = min(a.vocab, base + N);
-        const Vec<T> x = unpack_vec<T>(load_edge<T>(row, i0, end));
-#pragma unroll
-        for (int e = 0; e < V; ++e) f(i0 + e >= 0 && i0 + e < end ? order32(x.v[e]) : 0, (uint32_t)(i0 + e));
-      }
-    }, [&](auto&& f) {
-      for (int sl = last - 1; sl >= first; --sl) {
-        if (last - first > 1) load(sl);
-        float x[C * V];
-        unpack<T, C>(x, raw);
-        const int64_t base = (int64_t)sl * N - mis;
-        int lo = (int)max(-base, (int64_t)0);
-        const int n = max((int)min(a.vocab - base, (int64_t)N) - lo, 0);  // the row's part of the slice
-#pragma unroll
-        for (int i = 0; i < C * V; ++i) {
-          if (i % V == 0) asm volatile("" : "+v"(lo));  // compared as needed: masks kept for all values do not fit the scalars
-          const int at = (i / V * kThreads + tid) * V + i % V;
-          f((unsigned)(at - lo) < (unsigned)n ? order32(x[i]) : 0, (uint32_t)((int)base + at));
-        }
-      }
-    }, [&](int rank, uint64_t k) { out[rank] = k; });
+    most = !any ? 0 : p.rest != p.rest ? order32(NAN) : order32(p.m);
   }
   // over the wave: one lane that holds the maximum gives its rest, the others their totals
   const float wm = group_max<64>(p.m);
@@ -270,28 +272,48 @@ __global__ __launch_bounds__(kThreads) void slice_kernel(Fwd a) {
   __shared__ Part wave_part[kThreads / 64];
   if ((tid & 63) == 0) wave_part[tid >> 6] = p;
   __syncthreads();
+  [[maybe_unused]] __shared__ Part row_part;
   if (tid == 0) {
     p = wave_part[0];
 #pragma unroll
     for (int w = 1; w < kThreads / 64; ++w) p = join(p, wave_part[w], c2);
-    a.part[r * a.parts + part] = p;
+    if constexpr (ONE) {
+      finish_row(a, r, p, picked, valid);
+      row_part = p;
+    } else {
+      a.part[r * a.parts + part] = p;
+    }
+  }
+  if constexpr (TOP) {
+    __shared__ TopScratch sc;
+    __shared__ int who[kThreads], whos;
+    [[maybe_unused]] uint64_t* out = a.key + (r * a.parts + part) * a.top;
+    if (tid == 0) whos = 0;
+    const int each = (last - first) * C;  // vectors of a thread
+    auto look = [&](int thread, int v, auto&& f) {
+      const int64_t base = (int64_t)(first + v / C) * N - mis, i0 = base + (v % C * kThreads + thread) * V, end = min(a.vocab, base + N);
+      const Vec<T> x = unpack_vec<T>(load_edge<T>(row, i0, end));
+#pragma unroll
+      for (int e = 0; e < V; ++e) f(i0 + e >= 0 && i0 + e < end ? order32(x.v[e]) : 0, (uint32_t)(i0 + e));
+    };
+    // The threads whose maximum reaches the bound are few, but one in most waves: all threads look at a vector of theirs each (5 of 777 bf16
+    // rows 66 us, 10 of 2000 133; each such thread at its own, one after the other, 100 and 225).
+    block_top(sc, a.top, most, [&](bool reaches, auto&& f) {
+      if (reaches) who[atomicAdd(&whos, 1)] = tid;
+      __syncthreads();
+      const int n = whos * each;
+      for (int i = tid; i < n; i += kThreads) look(who[i / each], i % each, f);
+    }, [&](auto&& f) {
+#pragma unroll 1
+      for (int v = 0; v < each; ++v) look(tid, v, f);
+    }, [&](int rank, uint64_t k) {  // behind barriers: row_part is there
+      if constexpr (ONE) finish_top(a, r, rank, k, row_part);
+      else out[rank] = k;
+    });
   }
 }
 
 // ---------------------------------------------------------------- a row's slices joined
-Q3_DEV void finish_row(const Fwd& a, int64_t r, const Part& p, float picked, bool valid) {
-  const float ls = log1pf(p.rest), d = picked - p.m;
-  const bool none = p.m == -INFINITY;
-  a.logprob[r] = valid ? fmaf(d, a.c, -ls) : NAN;
-  a.entropy[r] = none ? NAN : fmaf(-kLn2, p.u / (1.f + p.rest), ls);
-  a.m[r] = p.m;
-  a.ls[r] = none ? NAN : ls;
-}
-
-Q3_DEV void left_out(const Fwd& a, int64_t r) {
-  a.logprob[r] = a.entropy[r] = a.m[r] = a.ls[r] = 0.f;
-}
-
 // One wave a row, no alternatives (4096 rows 5 us: a launch).
 template <typename T> __global__ __launch_bounds__(kThreads) void finish_kernel(Fwd a) {
   const int64_t r = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
@@ -299,7 +321,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void finish_kernel(
   if (r >= a.rows) return;
   const int64_t t = a.tok[r];
   if (t == a.ignore) {
-    if (lane == 0) left_out(a, r);
+    left_out(a, r, lane);
     return;
   }
   const bool valid = t >= 0 && t < a.vocab;
@@ -329,11 +351,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void finish_top_ker
     for (int i = 0; i < R; ++i) mine[i] = tid + i * kThreads < n ? key[tid + i * kThreads] : 0;
   }
   if (t == a.ignore) {
-    if (tid == 0) left_out(a, r);
-    if (tid < a.top) {
-      a.top_logprob[r * a.top + tid] = 0.f;
-      a.top_token[r * a.top + tid] = 0;
-    }
+    left_out(a, r, tid);
     return;
   }
   if (tid < 64) {
@@ -361,11 +379,7 @@ template <typename T> __global__ __launch_bounds__(kThreads) void finish_top_ker
   };
   block_top(sc, a.top, most, [&](bool reaches, auto&& f) {
     if (reaches) scan(f);
-  }, scan, [&](int rank, uint64_t k) {  // behind barriers: row_part is there
-    a.top_token[r * a.top + rank] = (int64_t)(uint32_t)~(uint32_t)k;
-    const float x = unorder32((uint32_t)(k >> 32));
-    a.top_logprob[r * a.top + rank] = row_part.m == -INFINITY ? NAN : fmaf(x - row_part.m, a.c, -log1pf(row_part.rest));
-  });
+  }, scan, [&](int rank, uint64_t k) { finish_top(a, r, rank, k, row_part); });  // behind barriers: row_part is there
 }
 
 // ---------------------------------------------------------------- gradient
@@ -527,7 +541,7 @@ template <int R, int NT> __global__ __launch_bounds__(NT) void head_finish_kerne
   for (int k = 1; k < W; ++k) p = join(p, part[k][lr], c2);
   const int64_t t = a.tok[r];
   if (t == a.ignore) {
-    left_out(a, r);
+    left_out(a, r, 0);
     return;
   }
   const bool valid = t >= 0 && t < a.vocab;
@@ -597,11 +611,15 @@ bool dtype_ok(int dt) { return dt == Q3_F32 || dt == Q3_F16 || dt == Q3_BF16; }
 int vec_of(int dtype) { return dtype == Q3_F32 ? 4 : 8; }
 int64_t cdiv(int64_t a, int64_t b) { return (a + b - 1) / b; }
 
+// Rows of up to 4 slices of 4 vectors a thread take a workgroup each and no second launch, however few they are (20 of one
+// row of 5000 9.0 us and 13.3 in two launches, of 32000 12.4 and 13.6, 10 of 256 rows of 32000 12.2 and 16.8; 500 rows of 5000 without
+// alternatives 6.1 and 9.3, one of 32000 7.3 and 7.1).
+bool one_launch(int dtype, int64_t vocab) { return vocab + vec_of(dtype) - 1 <= 4 * kThreads * vec_of(dtype) * 4; }
 // Vectors of a slice per thread: 4 where that leaves 1024 workgroups (or a row has very many values), else 1, which spreads the search
 // for alternatives (rows of 151936, 20 of one row 14.5 us and 17.1 with 4, 5 of 64 rows 25.8 and 22.3).  Without alternatives the
 // rule is the same, for the same bits with and without (one row 8.1 us and 7.6 with 4, 64 rows 13.7 and 10.7).
 int chunks_for(int dtype, int64_t rows, int64_t vocab) {
-  return vocab > (1 << 18) || rows * cdiv(vocab, (int64_t)kThreads * vec_of(dtype) * 4) >= 1024 ? 4 : 1;
+  return one_launch(dtype, vocab) || vocab > (1 << 18) || rows * cdiv(vocab, (int64_t)kThreads * vec_of(dtype) * 4) >= 1024 ? 4 : 1;
 }
 // A row may start up to a vector before its first element's boundary.
 int64_t slices_for(int dtype, int64_t rows, int64_t vocab) {
@@ -616,22 +634,25 @@ bool sizes_ok(int dtype, int64_t rows, int64_t vocab, int64_t top) {
 // Slices of a workgroup, dealt out evenly.  Without alternatives as many as leave 4096 workgroups (rows of 151936 bf16: 4096 of them 206
 // us, 229 with one slice each, 2048 108).  With them as many as leave 2048, at most 6, since each workgroup ends with a search (5 of
 // 777 rows 59 us, leaving 4096 66; 20 of 300 41 and 54; 5 of 777 fp32 rows 89, with up to 13 slices 93).
-int per_for(int64_t rows, int64_t slices, int64_t top) {
+int per_for(int dtype, int64_t rows, int64_t vocab, int64_t slices, int64_t top) {
+  if (one_launch(dtype, vocab)) return (int)slices;
   const int64_t most = top > 0 ? std::min<int64_t>(std::min<int64_t>(slices, 6), rows * slices / 2048) : std::min(slices, rows * slices / 4096);
   return (int)cdiv(slices, cdiv(slices, std::max<int64_t>(1, most)));
 }
 
-template <typename T, int C> void slices(const Fwd& a, hipStream_t s) {
+template <typename T, int C, bool ONE> void slices(const Fwd& a, hipStream_t s) {
   const unsigned n = (unsigned)(a.rows * a.parts);
-  if (a.top) slice_kernel<T, C, true><<<n, kThreads, 0, s>>>(a);
-  else slice_kernel<T, C, false><<<n, kThreads, 0, s>>>(a);
+  if (a.top) slice_kernel<T, C, true, ONE><<<n, kThreads, 0, s>>>(a);
+  else slice_kernel<T, C, false, ONE><<<n, kThreads, 0, s>>>(a);
 }
 
 template <typename T> int forward(const Fwd& a, int chunks, hipStream_t s) {
-  if (chunks == 4) slices<T, 4>(a, s);
-  else slices<T, 1>(a, s);
+  if (chunks == 4 && a.parts == 1) slices<T, 4, true>(a, s);
+  else if (chunks == 4) slices<T, 4, false>(a, s);
+  else slices<T, 1, false>(a, s);
   const int rc = (int)hipGetLastError();
   if (rc != 0) return rc;
+  if (chunks == 4 && a.parts == 1) return rc;
   if (a.top) {
     finish_top_kernel<T><<<(unsigned)a.rows, kThreads, 0, s>>>(a);
   } else {
@@ -669,7 +690,7 @@ int q3_token_logprobs(int dtype, const void* z, int64_t ld, int64_t rows, int64_
   Q3_REQUIRE((top == 0 || (top_logprob && top_token)) && inv_temperature > 0.f && inv_temperature < INFINITY);
   Q3_REQUIRE(((uintptr_t)z & (dtype == Q3_F32 ? 3 : 1)) == 0 && workspace && ((uintptr_t)workspace & 15) == 0 &&
              workspace_bytes >= q3_token_logprobs_workspace_bytes(dtype, rows, vocab, top));
-  const int n = (int)slices_for(dtype, rows, vocab), per = per_for(rows, n, top), c = chunks_for(dtype, rows, vocab), v = vec_of(dtype);
+  const int n = (int)slices_for(dtype, rows, vocab), per = per_for(dtype, rows, vocab, n, top), c = chunks_for(dtype, rows, vocab), v = vec_of(dtype);
   // one vector a thread: slices of a size (a short last one would have many candidates for its alternatives: T = 1, top 20
   // 19 -> 9 us)
   const int span = c == 1 ? (int)cdiv(cdiv(vocab + v - 1, v), n) * v : kThreads * v * c;

@@ -51,7 +51,8 @@ def near(got, want, tol):
     assert worst <= 1.0, f'{worst:.2f} times the tolerance'
 
 
-SHAPES = [(1, 1), (1, 2), (3, 7), (2, 1000), (5, 2047), (4, 2048), (3, 2049), (1, 16385), (2, 151936), (300, 4099), (1100, 2600), (130, 65537)]
+SHAPES = [(1, 1), (1, 2), (3, 7), (2, 1000), (5, 2047), (4, 2048), (3, 2049), (1, 16385), (2, 151936), (300, 4099), (1100, 2600), (130, 65537), (3, 32761), (3, 32762),
+          (3, 16381), (3, 16382)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -72,7 +73,8 @@ def test_against_64_bits(t, v, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("t,v,top", [(1, 1, 1), (2, 5, 5), (3, 33, 32), (1, 151936, 20), (2, 2049, 1), (700, 5001, 5), (5, 300001, 32), (1030, 2100, 3)])
+@pytest.mark.parametrize("t,v,top", [(1, 1, 1), (2, 5, 5), (3, 33, 32), (1, 151936, 20), (2, 2049, 1), (700, 5001, 5), (5, 300001, 32), (1030, 2100, 3),
+                                     (3, 32761, 20), (3, 32762, 20), (3, 16381, 7), (3, 16382, 7), (300, 33000, 4)])
 def test_alternatives(t, v, top, dtype):
     print(f"top {t} {v} {top} {dtype}", flush=True)
     z, ids = rows_of(t, v, dtype, masked=0.3 if v > 100 else 0.0)
@@ -86,20 +88,36 @@ def test_alternatives(t, v, top, dtype):
     near(out.top_logprobs, best, E * (160 + 4 * (best - lp.max(-1, keepdim=True).values).abs() + 4 * lp.max(-1, keepdim=True).values.abs()))
 
 
+@pytest.mark.parametrize("v", [40000, 30000, 9000])   # a row in several workgroups, in one
 @pytest.mark.parametrize("dtype", DTYPES)
-def test_alternatives_of_awkward_rows(dtype):
+def test_alternatives_of_awkward_rows(dtype, v):
     """Rows of equals, sorted rows either way, the largest all in one thread's values, few values that are not ruled out."""
-    v, top = 40000, 32
+    top = 32
     ramp = torch.linspace(-8, 8, v)
     rows = [torch.zeros(v), ramp, ramp.flip(0), torch.full((v,), -3.0), torch.zeros(v)]
-    rows[3][8 * 256 * torch.arange(16)[:, None] + torch.arange(8)] = 4.0 + torch.rand((16, 8), generator=seeded(1))
+    n = min(16, v // 2048)
+    rows[3][8 * 256 * torch.arange(n)[:, None] + torch.arange(8)] = 4.0 + torch.rand((n, 8), generator=seeded(1))
     rows[4] = torch.full((v,), float('-inf'))
-    rows[4][torch.tensor([5, 39999, 20000])] = torch.tensor([-0.0, 0.0, 1.0])
+    rows[4][torch.tensor([5, v - 1, v // 2])] = torch.tensor([-0.0, 0.0, 1.0])
     for reps in (1, 60):   # small slices and large ones
         z = torch.stack(rows).repeat(reps, 1).to(dtype).cuda()
         out = token_logprobs(z, torch.zeros(z.shape[0], dtype=torch.int64, device='cuda'), top=top)
         assert torch.equal(out.top_tokens, z.float().sort(dim=-1, descending=True, stable=True).indices[:, :top])
-        assert out.top_tokens[4, :4].tolist() == [20000, 5, 39999, 0] and float(out.top_logprobs[4, 3]) == -float('inf')
+        assert out.top_tokens[4, :4].tolist() == [v // 2, 5, v - 1, 0] and float(out.top_logprobs[4, 3]) == -float('inf')
+
+
+@pytest.mark.parametrize("v,top", [(5000, 0), (5000, 6), (40000, 0), (40000, 6)])
+def test_rows_left_out(v, top):
+    """Zeros, whatever the row holds, and the other rows as they are alone."""
+    z, ids = rows_of(6, v, torch.bfloat16)
+    ids[2], ids[5] = -100, -100
+    z[2], z[5] = float('nan'), float('inf')
+    out = token_logprobs(z, ids, top=top)
+    keep = torch.tensor([0, 1, 3, 4]).cuda()
+    alone = token_logprobs(z[keep], ids[keep], top=top)
+    for a, b in zip(out, alone):
+        if a is not None:
+            assert torch.equal(a[keep], b) and not bool(a[[2, 5]].any())
 
 
 def test_rows_without_a_distribution():
