@@ -564,9 +564,9 @@ int q3_kv8_attention(int dtype, const void* q, int64_t qsb, int64_t qss, int64_t
  * New: no counterpart in the reference.  Of rows z [rows, vocab] (row stride ld >= vocab, any alignment) at a temperature
  * (inv_temperature = 1 / it): logprob[r] = log softmax(z[r] / temperature)[tokens[r]], entropy[r] of that softmax, and the top
  * (0 .. 32) largest log probabilities with their tokens, [rows, top], in falling order (equal logits: the lower token first;
- * NaN first of all).  row_max and row_log [rows] keep what the gradient needs.  All results are fp32 / int64.
+ * NaN first of all).  row_max and row_log [rows] (both, or both NULL) keep what the gradient needs.  All results are fp32 / int64.
  * A row whose token is ignore_index is left out: zeros, and none of its logits is read.  Any other token outside
- * [0, vocab) gets NaN.  A row of -inf only, or with a NaN or +inf, gets NaN.  vocab < 2^30. */
+ * [0, vocab) gets NaN.  A row of -inf only, or with a NaN or +inf, gets NaN.  vocab < 2^30.  The workspace may be empty. */
 size_t q3_token_logprobs_workspace_bytes(int dtype, int64_t rows, int64_t vocab, int64_t top);
 int q3_token_logprobs(int dtype, const void* z, int64_t ld, int64_t rows, int64_t vocab, const int64_t* tokens,
                       int64_t ignore_index, float inv_temperature, int64_t top, float* logprob, float* entropy,

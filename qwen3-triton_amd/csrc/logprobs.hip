@@ -138,7 +138,7 @@ struct Fwd {
   int top, slices, span, per, parts;  // slices of a row, their elements, slices of a workgroup, workgroups of a row
   Part* part;   // [rows][parts]
   uint64_t* key;  // [rows][parts][top]
-  float *logprob, *entropy, *m, *ls;  // ls: log1p(rest)
+  float *logprob, *entropy, *m, *ls;  // ls: log1p(rest); m and ls: for the gradient, or null
   float* top_logprob;
   int64_t* top_token;
 };
@@ -197,6 +197,7 @@ Q3_DEV void finish_row(const Fwd& a, int64_t r, const Part& p, float picked, boo
   const bool none = p.m == -INFINITY;
   a.logprob[r] = valid ? fmaf(d, a.c, -ls) : NAN;
   a.entropy[r] = none ? NAN : fmaf(-kLn2, p.u / (1.f + p.rest), ls);
+  if (!a.m) return;
   a.m[r] = p.m;
   a.ls[r] = none ? NAN : ls;
 }
@@ -210,7 +211,8 @@ Q3_DEV void finish_top(const Fwd& a, int64_t r, int rank, uint64_t k, const Part
 
 // Called by the row's threads 0 .. kMaxTop - 1 at least.
 Q3_DEV void left_out(const Fwd& a, int64_t r, int tid) {
-  if (tid == 0) a.logprob[r] = a.entropy[r] = a.m[r] = a.ls[r] = 0.f;
+  if (tid == 0) a.logprob[r] = a.entropy[r] = 0.f;
+  if (tid == 0 && a.m) a.m[r] = a.ls[r] = 0.f;
   if (tid < a.top) {
     a.top_logprob[r * a.top + tid] = 0.f;
     a.top_token[r * a.top + tid] = 0;
@@ -640,6 +642,11 @@ int per_for(int dtype, int64_t rows, int64_t vocab, int64_t slices, int64_t top)
   return (int)cdiv(slices, cdiv(slices, std::max<int64_t>(1, most)));
 }
 
+// Whether each workgroup has a whole row, whose results it writes itself.
+bool writes_results(int dtype, int64_t rows, int64_t vocab, int64_t slices, int64_t top) {
+  return chunks_for(dtype, rows, vocab) == 4 && per_for(dtype, rows, vocab, slices, top) >= slices;
+}
+
 template <typename T, int C, bool ONE> void slices(const Fwd& a, hipStream_t s) {
   const unsigned n = (unsigned)(a.rows * a.parts);
   if (a.top) slice_kernel<T, C, true, ONE><<<n, kThreads, 0, s>>>(a);
@@ -647,12 +654,13 @@ template <typename T, int C, bool ONE> void slices(const Fwd& a, hipStream_t s) 
 }
 
 template <typename T> int forward(const Fwd& a, int chunks, hipStream_t s) {
-  if (chunks == 4 && a.parts == 1) slices<T, 4, true>(a, s);
+  const bool one = chunks == 4 && a.parts == 1;  // as writes_results
+  if (one) slices<T, 4, true>(a, s);
   else if (chunks == 4) slices<T, 4, false>(a, s);
   else slices<T, 1, false>(a, s);
   const int rc = (int)hipGetLastError();
   if (rc != 0) return rc;
-  if (chunks == 4 && a.parts == 1) return rc;
+  if (one) return rc;
   if (a.top) {
     finish_top_kernel<T><<<(unsigned)a.rows, kThreads, 0, s>>>(a);
   } else {
@@ -678,7 +686,9 @@ extern "C" {
 
 size_t q3_token_logprobs_workspace_bytes(int dtype, int64_t rows, int64_t vocab, int64_t top) {
   if (!sizes_ok(dtype, rows, vocab, top)) return 0;
-  const size_t n = (size_t)rows * (size_t)slices_for(dtype, rows, vocab);
+  const int64_t slices = slices_for(dtype, rows, vocab);
+  if (writes_results(dtype, rows, vocab, slices, top)) return 0;
+  const size_t n = (size_t)rows * (size_t)slices;
   return (n * sizeof(Part) + 7) / 8 * 8 + n * (size_t)top * sizeof(uint64_t);
 }
 
@@ -686,17 +696,18 @@ int q3_token_logprobs(int dtype, const void* z, int64_t ld, int64_t rows, int64_
                       int64_t ignore_index, float inv_temperature, int64_t top, float* logprob, float* entropy, float* row_max,
                       float* row_log, float* top_logprob, int64_t* top_token, void* workspace, size_t workspace_bytes,
                       hipStream_t stream) {
-  Q3_REQUIRE(sizes_ok(dtype, rows, vocab, top) && z && tokens && logprob && entropy && row_max && row_log && ld >= vocab);
+  Q3_REQUIRE(sizes_ok(dtype, rows, vocab, top) && z && tokens && logprob && entropy && !row_max == !row_log && ld >= vocab);
   Q3_REQUIRE((top == 0 || (top_logprob && top_token)) && inv_temperature > 0.f && inv_temperature < INFINITY);
-  Q3_REQUIRE(((uintptr_t)z & (dtype == Q3_F32 ? 3 : 1)) == 0 && workspace && ((uintptr_t)workspace & 15) == 0 &&
-             workspace_bytes >= q3_token_logprobs_workspace_bytes(dtype, rows, vocab, top));
+  const size_t need = q3_token_logprobs_workspace_bytes(dtype, rows, vocab, top);
+  Q3_REQUIRE(((uintptr_t)z & (dtype == Q3_F32 ? 3 : 1)) == 0 &&
+             (need == 0 || (workspace && ((uintptr_t)workspace & 15) == 0 && workspace_bytes >= need)));
   const int n = (int)slices_for(dtype, rows, vocab), per = per_for(dtype, rows, vocab, n, top), c = chunks_for(dtype, rows, vocab), v = vec_of(dtype);
   // one vector a thread: slices of a size (a short last one would have many candidates for its alternatives: T = 1, top 20
   // 19 -> 9 us)
   const int span = c == 1 ? (int)cdiv(cdiv(vocab + v - 1, v), n) * v : kThreads * v * c;
   Fwd a{z, ld, rows, vocab, tokens, ignore_index, inv_temperature, (int)top, n, span, per, (int)cdiv(n, per),
         (Part*)workspace, nullptr, logprob, entropy, row_max, row_log, top_logprob, top_token};
-  a.key = (uint64_t*)((char*)workspace + ((size_t)rows * n * sizeof(Part) + 7) / 8 * 8);
+  if (need > 0) a.key = (uint64_t*)((char*)workspace + ((size_t)rows * n * sizeof(Part) + 7) / 8 * 8);
   if (dtype == Q3_BF16) return forward<BF16>(a, c, stream);
   if (dtype == Q3_F16) return forward<F16>(a, c, stream);
   return forward<F32>(a, c, stream);

@@ -67,12 +67,12 @@ def _forward(z, rows, ld, v, tokens, ignore_index, temperature, top, keep, outs=
         outs = _outputs(z, rows, top, keep)
     lp, ent, tlp, tid, kept = outs
     nbytes = H.query("q3_token_logprobs_workspace_bytes", H.code(z.dtype), rows, v, top)
-    ws = H.workspace(nbytes + (0 if kept is not None else 8 * rows), z.device)
-    w = ws.data_ptr()
-    m, ls = (w + nbytes, w + nbytes + 4 * rows) if kept is None else (kept.data_ptr() + 4 * at, kept.data_ptr() + 4 * (kept.shape[1] + at))
+    ws = H.workspace(nbytes, z.device) if nbytes else None
+    m, ls = (None, None) if kept is None else (kept.data_ptr() + 4 * at, kept.data_ptr() + 4 * (kept.shape[1] + at))
     H.launch(z, "q3_token_logprobs", H.code(z.dtype), z.data_ptr(), ld, rows, v, tokens.data_ptr() + 8 * at, ignore_index,
              1.0 / temperature, top, lp.data_ptr() + 4 * at, ent.data_ptr() + 4 * at, m, ls,
-             None if tlp is None else tlp.data_ptr() + 4 * top * at, None if tid is None else tid.data_ptr() + 8 * top * at, w, nbytes)
+             None if tlp is None else tlp.data_ptr() + 4 * top * at, None if tid is None else tid.data_ptr() + 8 * top * at,
+             None if ws is None else ws.data_ptr(), nbytes)
     return outs
 
 

@@ -122,7 +122,8 @@ BOTH = [dict(dtype=3), dict(z=None), dict(z=P + 1), dict(ld=999), dict(rows=0), 
         dict(ent=None), dict(m=None), dict(ls=None), dict(rows=(1 << 31) - 1, vocab=100000, ld=100000)]
 
 
-@pytest.mark.parametrize("bad", BOTH + [dict(lp=None), dict(tlp=None), dict(tid=None), dict(ws=None), dict(ws=P + 8), dict(nbytes=8)])
+@pytest.mark.parametrize("bad", BOTH + [dict(lp=None), dict(tlp=None), dict(tid=None),
+                                        *(dict(vocab=100000, ld=100000, **x) for x in (dict(ws=None), dict(ws=P + 8), dict(nbytes=8)))])
 def test_token_logprobs_refusals(bad):
     assert logprob_call('fwd', **bad) == INVALID
 
@@ -138,6 +139,7 @@ def test_logprob_workspace():
     assert q(2, 0, 10, 0) == q(3, 1, 10, 0) == q(2, 1, 10, 11) == q(2, 1, 0, 0) == 0
     assert 0 < q(2, 1, 151936, 0) <= q(2, 1, 151936, 20) <= 1 << 20
     assert q(2, 4096, 151936, 0) <= 4096 * 24 * 12
+    assert q(2, 1, 1000, 5) == q(1, 3, 30000, 0) == q(0, 3, 16000, 9) == 0   # a row a workgroup: nothing to join
 
 
 def head_call(**kw):
