@@ -23,7 +23,8 @@ Q3_DEV Part join(const Part& a, const Part& b, float c2) {
 
 // Statistics of N values of a thread.  One element that is the maximum is taken out on the way to it (each step keeps the larger
 // and stores the smaller), in four chains.  d comes as fma(x, c2, -m c2): one rounding, and what the product m c2 lost to its own is
-// the same factor of every term.  Maxima and minima here hand NaN on.
+// the same factor of every term.  It is at most 1 in base 2 while |m c2| <= 2^24; beyond (finite masks, 1e-6 as the temperature) the
+// factor itself could leave the numbers, and d comes from the difference.  Maxima and minima here hand NaN on.
 template <int N> Q3_DEV Part part_of(const float (&v)[N], float c2) {
   static_assert(N % 4 == 0, "four chains");
   float x[N], top[4];
@@ -44,7 +45,7 @@ template <int N> Q3_DEV Part part_of(const float (&v)[N], float c2) {
   }
   const bool nan = p.m != p.m;
   if (nan) p.m = -INFINITY;
-  if (__any(fabsf(p.m) > 1e30f && p.m != -INFINITY)) {  // m c2 might overflow (rows of the type's lowest value)
+  if (__any(fabsf(p.m * c2) > 0x1p24f && p.m != -INFINITY)) {
     const float ref = p.m == -INFINITY ? 0.f : p.m;
 #pragma unroll
     for (int i = 1; i < N; ++i) {

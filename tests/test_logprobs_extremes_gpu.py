@@ -1,0 +1,81 @@
+"""Log probabilities where numbers are extreme: finite masks, temperatures near their bounds, infinite logits, gradients beyond fp16's
+range; and backward passes that are captured, offloaded or formed again.
+
+Tolerances are those of the plain cases (test_logprobs_gpu.py), and a probability below 2^-126 may come out of the exponential as 0."""
+import pytest
+import torch
+
+from _util import seeded
+from test_logprobs_gpu import E, grads, near, reference
+
+from qwen3_triton.kernels.logprobs import token_logprobs
+
+pytestmark = pytest.mark.gpu
+F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
+
+
+def close(got, want, tol):
+    """``near``, where equal infinities are near too and what fp32 rounds to an infinity (2^128 - 2^103 and more) is one."""
+    want = torch.where(want < -3.40282357e38, float('-inf'), want)
+    same = got.double() == want
+    near(torch.where(same, 0.0, got), torch.where(same, 0.0, want), torch.where(same, 1.0, tol))
+
+
+def check_rows(z, ids, temperature, top=5):
+    """Results, alternatives and gradients of rows against 64 bits."""
+    t, v = z.shape
+    gen = seeded(t)
+    g, gh = torch.randn(t, generator=gen).cuda(), torch.randn(t, generator=gen).cuda()
+    gtop = torch.randn((t, top), generator=gen).cuda()
+    zr = z.clone().requires_grad_()
+    out = token_logprobs(zr, ids, top=top, temperature=temperature)
+    lp, want, h, t_lp, t_h = reference(z, ids, temperature)
+    close(out.logprobs, want, t_lp)
+    near(out.entropy, h, t_h)
+    order = z.float().sort(dim=-1, descending=True, stable=True).indices[:, :top]
+    assert torch.equal(out.top_tokens, order)
+    best = lp.gather(-1, order)
+    close(out.top_logprobs, best, E * (160 + 4 * (best - lp.amax(-1, keepdim=True)).abs() + 4 * lp.amax(-1, keepdim=True).abs()))
+    plain = token_logprobs(z, ids, temperature=temperature)
+    assert torch.equal(plain.logprobs, out.logprobs) and torch.equal(plain.entropy, out.entropy)
+    (dz,) = torch.autograd.grad([out.logprobs, out.entropy, out.top_logprobs], zr, [g, gh, gtop])
+    want, tol = grads(z, ids, g, gh, gtop, out.top_tokens, temperature)
+    p_lp = torch.where(lp.exp() > 0, lp, 0.0).abs()
+    none = 2.0 ** -126 * (g.abs()[:, None] + gtop.abs().sum(-1, keepdim=True) + gh.abs()[:, None] * (p_lp + h[:, None] + 1)) / temperature
+    fin = torch.finfo(z.dtype)
+    near(dz, want, fin.eps / 2 * want.abs() + tol + none + fin.smallest_normal * fin.eps / 2)
+
+
+@pytest.mark.parametrize("dtype,mask", [*((d, m) for d in (F32, BF16) for m in (-1e4, -1e9, -1e10, -1e20, -1e29, -2e30, None)), (F16, -6e4), (F16, None)])
+@pytest.mark.parametrize("v", [700, 9000, 70001])   # one vector or less a thread, a row in one workgroup, in several
+def test_finite_masks(v, dtype, mask):
+    """Values ruled out by a finite number (None: the type's lowest): here and there, in blocks, all but a few, all."""
+    mask = torch.finfo(dtype).min if mask is None else mask
+    print(f"masks {v} {dtype} {mask}", flush=True)
+    gen = seeded(v)
+    z = torch.randn((8, v), generator=gen) * 2
+    ids = torch.randint(0, v, (8,), generator=gen)
+    z[1, torch.rand(v, generator=gen) < 0.3] = mask
+    z[2] = mask
+    z[2, ids[2]] = 1.5
+    z[3] = mask                                # a row of equals
+    z[4, :v // 2] = mask
+    z[5, 16:32] = mask
+    z[6, :-3] = mask
+    z[7], z[7, v // 3], ids[7] = mask, 2.0, v // 2   # the token is one of those ruled out
+    for reps in (1, 150):   # 1200 rows: large slices of a thread
+        zr, ir = z.repeat(reps, 1).to(dtype).cuda(), ids.repeat(reps).cuda()
+        for temperature in (1.0, 0.5, 0.1):
+            if reps == 1 or temperature == 0.5 and v < 10000:
+                check_rows(zr, ir, temperature)
+
+
+@pytest.mark.parametrize("dtype", [F32, BF16])
+@pytest.mark.parametrize("v", [700, 9000, 70001])
+def test_smallest_temperature(v, dtype):
+    """Large logits at a temperature of 1e-6: what counts is their difference to the largest."""
+    z = torch.full((3, v), 3000.3)
+    z[1, ::2] = 2999.0
+    z[2, v // 2] = 3100.0
+    check_rows(z.to(dtype).cuda(), torch.tensor([0, 1, v // 2]).cuda(), 1e-6)
+    check_rows(-z.to(dtype).cuda(), torch.tensor([0, 1, v // 2]).cuda(), 1e-6)
