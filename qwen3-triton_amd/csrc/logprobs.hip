@@ -43,9 +43,9 @@ Q3_DEV uint64_t key_xor(uint64_t x, int mask) {
 }
 
 // The k largest (k <= kMaxTop) of a workgroup's values in order, to emit(rank, key) by some thread each; ranks that no value
-// takes get key 0.  most: the order of the thread's largest value (0: it has none); scan(f) calls f(order, index) for each of
-// its values, order 0 for none, and may read them again; collect(reaches, f), called by all threads, does so for at least the values
-// of the threads for which `reaches`.
+// takes get key 0.  most: the order of the thread's largest value (0: it has none), and no higher, or ranks would stay empty;
+// scan(f) calls f(order, index) for each of its values, order 0 for none, and may read them again; collect(reaches, f), called by
+// all threads, does so for at least the values of the threads for which `reaches`.
 //  * The 64 maxima of groups of 4 threads: the k-th largest of those is a bound that at least k values reach.  Of random
 //    values about 1.3 k do; they are collected and ranked by counting the larger ones.
 //  * More than kCand may reach it (ties, a row that rises, few values that are not -inf): then k rounds, each the largest key
@@ -241,6 +241,7 @@ __global__ __launch_bounds__(kThreads) void slice_kernel(Fwd a) {
   const bool valid = t >= 0 && t < a.vocab;
   [[maybe_unused]] const float picked = ONE && tid == 0 && valid ? to_f32<T>(row[t]) : 0.f;
   Part p{-INFINITY, 0.f, 0.f};
+  [[maybe_unused]] bool nan = false;  // among the thread's values (p.rest is NaN for +inf too)
   i32x4 raw[C];
   auto load = [&](int sl) {
     const int64_t base = (int64_t)sl * N - mis;
@@ -252,13 +253,14 @@ __global__ __launch_bounds__(kThreads) void slice_kernel(Fwd a) {
     unpack<T, C>(x, raw);
     if (sl + 1 < last) load(sl + 1);  // in flight meanwhile
     const Part q = part_of(x, c2);
+    if constexpr (TOP) nan = nan || (q.m == -INFINITY && q.rest != q.rest);
     p = sl == first ? q : join(p, q, c2);
   }
   [[maybe_unused]] uint32_t most = 0;  // the order of the thread's largest value
   if constexpr (TOP) {
     const int64_t begin = (int64_t)first * N - mis + tid * V;  // of the thread's first vector
     const bool any = begin < a.vocab && begin + V > 0 && tid * V < N;
-    most = !any ? 0 : p.rest != p.rest ? order32(NAN) : order32(p.m);
+    most = !any ? 0 : nan ? order32(NAN) : order32(p.m);
   }
   // over the wave: one lane that holds the maximum gives its rest, the others their totals
   const float wm = group_max<64>(p.m);

@@ -79,3 +79,31 @@ def test_smallest_temperature(v, dtype):
     z[2, v // 2] = 3100.0
     check_rows(z.to(dtype).cuda(), torch.tensor([0, 1, v // 2]).cuda(), 1e-6)
     check_rows(-z.to(dtype).cuda(), torch.tensor([0, 1, v // 2]).cuda(), 1e-6)
+
+
+@pytest.mark.parametrize("dtype", [F32, F16, BF16])
+@pytest.mark.parametrize("v", [50, 5000, 30000, 70001, 151936])
+def test_alternatives_of_rows_with_infinite_logits(v, dtype):
+    """As many +inf as there are alternatives or more, alone and with NaN, all in different threads or in one: NaN first of all, then
+    +inf, equals by their tokens."""
+    gen = seeded(v)
+    z = torch.randn((6, v), generator=gen)
+    inf, nan = float('inf'), float('nan')
+    far = (torch.arange(12) * (v // 12) + 3) % v
+    z[0, v // 2] = inf
+    z[1, far] = inf
+    z[2, far], z[2, far[5]] = inf, nan
+    z[3, 8:16], z[3, 13] = inf, nan            # in one thread's values
+    z[4], z[4, 7] = -inf, inf
+    z[5] = inf
+    for reps in (1, 200):
+        if reps * v > 10 ** 7:
+            continue
+        zr = z.repeat(reps, 1).to(dtype).cuda()
+        ids = torch.zeros(zr.shape[0], dtype=torch.int64, device='cuda')
+        key = zr.double().nan_to_num(nan=3e300, posinf=2e300)
+        want = key.sort(dim=-1, descending=True, stable=True).indices
+        for top in (1, 2, 5, 12):
+            out = token_logprobs(zr, ids, top=top)
+            assert torch.equal(out.top_tokens, want[:, :top]), top
+            assert bool(out.logprobs.isnan().all()) and bool(out.entropy.isnan().all()) and bool(out.top_logprobs.isnan().all())
