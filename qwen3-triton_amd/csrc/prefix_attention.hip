@@ -202,9 +202,9 @@ Q3_DEV void softmax_block(Rows<U>& w, Step<U>& t, f32x4 (&S)[4][U], i32x4 (&P)[U
 // O^T += V^T P and the sums of P, V's tile at vb.  A value that is not finite would spoil the rows that do not see its position too
 // (0 times it is NaN): blocks that some row sees in part (LOOK; the last of a job, in a loop of their own, since the second way
 // through the product costs copies of O) are looked through first, and then such values are kept out of the product and
-// added to the rows that do see them.
+// added to the rows that do see them: all rows see a block of the prefix (pre), whose rows behind its end are zeros here.
 template <typename T, int U, bool LOOK>
-Q3_DEV void value_block(Rows<U>& w, const i32x4 (&P)[U][2], const char* vb, int key0, int g, int r16) {
+Q3_DEV void value_block(Rows<U>& w, const i32x4 (&P)[U][2], const char* vb, bool pre, int key0, int g, int r16) {
   const int lane = 16 * g + r16;
   const int voff[2] = {value_offset(g, r16, 0), value_offset(g, r16, 1)};
   bool clean = true;
@@ -251,7 +251,7 @@ Q3_DEV void value_block(Rows<U>& w, const i32x4 (&P)[U][2], const char* vb, int 
           const uint32_t bits = ((uint32_t)x[i >> 1] >> (16 * (i & 1))) & 0xffffu;
           const float bad = finite2<T>(bits) ? 0.f : to_f32<T>((u16)bits);
 #pragma unroll
-          for (int u = 0; u < U; ++u) w.o[dt][u][i] += key0 + key < w.lim[u] ? bad : 0.f;
+          for (int u = 0; u < U; ++u) w.o[dt][u][i] += pre || key0 + key < w.lim[u] ? bad : 0.f;
         }
       }
     }
@@ -383,7 +383,7 @@ template <typename T, int NW> Q3_DEV void tile_job(const Args& a, const Job& job
     Step<2> step;
     softmax_block<T, 2>(w, step, S, P, a.scale2, thr);
     rescale(w, step);
-    value_block<T, 2, decltype(look)::value>(w, P, kb + kKTile, key0, g, r16);
+    value_block<T, 2, decltype(look)::value>(w, P, kb + kKTile, pre, key0, g, r16);
   };
   issue(0);
   const int seen = first_partial(a, job, lim_w);
@@ -463,7 +463,7 @@ template <typename T, int U, bool LOOK> Q3_DEV void few_job(const Args& a, const
     if (EARLY && more) __builtin_amdgcn_s_waitcnt((16 & 15) | ((16 >> 4) << 14) | (7 << 4) | (15 << 8));
     else __builtin_amdgcn_s_waitcnt((0 & 15) | (7 << 4) | (15 << 8));
     fence();
-    value_block<T, U, LOOK>(w, P, vt, x.key0, g, r16);
+    value_block<T, U, LOOK>(w, P, vt, pre, x.key0, g, r16);
     if (more) {
       __builtin_amdgcn_s_waitcnt((15) | (3 << 14) | (7 << 4) | (0 << 8));  // the tile is read
       fence();

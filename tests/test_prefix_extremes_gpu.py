@@ -1,0 +1,31 @@
+"""Attention over a shared prefix where values or keys are not finite: what is seen counts, in every form of the kernel."""
+import pytest
+import torch
+
+from test_prefix_gpu import DTYPES, expected, inputs
+
+from qwen3_triton.inference import prefix as PX
+
+pytestmark = pytest.mark.gpu
+
+# single queries and short chunks in one pass over few positions, in jobs behind many, and tiles of longer chunks in either
+FORMS = [(1, 6, 1, 8, 2, 100, 9), (1, 6, 2, 8, 2, 100, 9), (1, 6, 4, 8, 2, 128, 0), (2, 3, 3, 8, 2, 70, 5), (1, 1, 4, 8, 2, 3000, 9), (1, 2, 2, 8, 2, 3000, 0),
+         (1, 1, 16, 4, 4, 2048, 70), (1, 9, 1, 8, 2, 3000, 5), (2, 2, 3, 8, 2, 1500, 0), (1, 4, 4, 8, 2, 3000, 3), (1, 3, 40, 8, 2, 100, 9),
+         (1, 3, 40, 8, 2, 3000, 9), (1, 24, 56, 32, 8, 200, 3)]
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("r,n,s,hq,hkv,p,start", FORMS)
+def test_values_of_the_prefix_that_are_not_finite(r, n, s, hq, hkv, p, start, dtype):
+    """Every query sees the whole prefix: infinite where a value is infinite, not a number where one is none, in every row."""
+    print(f"values {r}x{n} S{s} P{p} start {start} {dtype}", flush=True)
+    t = inputs(r, n, s, hq, hkv, p, start + s + 9, dtype)
+    pv = t[2]
+    pv[:, :, 60, 5], pv[:, :, p - 1, 8], pv[0, :, p // 2, 11] = float('inf'), float('nan'), -float('inf')
+    got = PX.attention(*t, start)
+    o, tol = expected(*t, [start] * (r * n))
+    bad = torch.zeros_like(got, dtype=torch.bool)
+    bad[..., 5], bad[..., 8], bad[:n, ..., 11] = True, True, True
+    assert bool((~got.isfinite() == bad).all())
+    assert bool(got[..., 8].isnan().all())
+    assert float(torch.where(bad, 0.0, (got.double() - o).abs() / tol).max()) <= 1.0
