@@ -653,8 +653,9 @@ template <typename T, int GR> __global__ __launch_bounds__(256) void prefix_join
     if (j0 != grp) load(j0);
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      if (j0 + k * GR >= used || m[k] == -INFINITY) continue;
-      const float w = __builtin_amdgcn_exp2f(m[k] - M);
+      if (j0 + k * GR >= used) continue;
+      // a slot without a maximum may hold a sum that is not a number (scores that are none beside hidden ones): times 0 it stays one
+      const float w = m[k] == -INFINITY ? 0.f : __builtin_amdgcn_exp2f(m[k] - M);
       sum = __builtin_fmaf(w, sj[k], sum);
       o += w * x[k];
     }

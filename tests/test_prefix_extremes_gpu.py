@@ -29,3 +29,29 @@ def test_values_of_the_prefix_that_are_not_finite(r, n, s, hq, hkv, p, start, dt
     assert bool((~got.isfinite() == bad).all())
     assert bool(got[..., 8].isnan().all())
     assert float(torch.where(bad, 0.0, (got.double() - o).abs() / tol).max()) <= 1.0
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("start", [0, 5, 61])
+@pytest.mark.parametrize("r,n,s,hq,hkv,p", sorted({f[:6] for f in FORMS}))
+def test_own_keys_that_are_not_numbers(r, n, s, hq, hkv, p, start, dtype):
+    """All of a row's own keys, beside positions that are not there yet: its queries are not numbers, the others' stay as they were."""
+    t = inputs(r, n, s, hq, hkv, p, 160, dtype)
+    want = PX.attention(*t, start)
+    row = r * n - 1
+    t[3][row, :, :start + s] = float('nan')
+    got = PX.attention(*t, start)
+    assert bool(got[row].isnan().all())
+    assert torch.equal(got[:row], want[:row])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("r,n,s,hq,hkv,p,start", FORMS)
+def test_keys_of_the_prefix_that_are_not_numbers(r, n, s, hq, hkv, p, start, dtype):
+    """The last part of a prefix, whose last block has positions that are not there: nobody behind it has a number."""
+    t = inputs(r, n, s, hq, hkv, p, start + s + 9, dtype)
+    want = PX.attention(*t, start)
+    t[1][0, :, p - p // 3:] = float('nan')
+    got = PX.attention(*t, start)
+    assert bool(got[:n].isnan().all())
+    assert torch.equal(got[n:], want[n:])
