@@ -73,7 +73,8 @@ template <int N> Q3_DEV Part part_of(const float (&v)[N], float c2) {
 // What the LM head keeps of a logit for its gradient: how far it lies below the maximum of its 128 columns, in base 2 at the
 // temperature, as 16 bits of a range of 64 (one conversion for two, which clamps).  A probability formed from it is off by at most
 // 0.034 % (half a step of 64 / 65535, times ln 2), a tenth of the rounding of a bf16 gradient and less than that of an fp16 one, at a
-// third of the memory and traffic of fp32 logits beside their gradient; below 2^-64 of the group's largest it is 2^-64 of it.
+// third of the memory and traffic of fp32 logits beside their gradient; below 2^-64 of the group's largest it is 0, as that of a
+// logit of -inf is.
 // (The distance in fp16 would be off by up to 0.4 % at e^-8, as much as the bf16 gradient's rounding.)
 constexpr float kGapRange = 64.f, kGapStep = kGapRange / 65535.f;
 Q3_DEV uint32_t gap2(float z0, float z1, float m, float c2) {

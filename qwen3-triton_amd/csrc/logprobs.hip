@@ -587,12 +587,13 @@ template <typename O> __global__ __launch_bounds__(kThreads) void head_grad_kern
     if (i0 >= vocab) continue;
     float o[8];
     if (live) {
-      const float at = fmaf(gm[i] - m, a.c, -ls) * kLog2e;
+      float at = fmaf(gm[i] - m, a.c, -ls) * kLog2e;
+      at = at < -1e30f ? -1e30f : at;  // a group of -inf only: its probabilities are 0
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        const float gap = (float)(((uint32_t)raw[i][e >> 1] >> (16 * (e & 1))) & 0xffffu);
-        const float l2 = fmaf(gap, -kGapStep, at);
-        o[e] = -a.c * __builtin_amdgcn_exp2f(l2) * fmaf(gh, fmaf(l2, kLn2, ent), g);
+        const uint32_t gap = ((uint32_t)raw[i][e >> 1] >> (16 * (e & 1))) & 0xffffu;
+        const float l2 = fmaf((float)gap, -kGapStep, at), p = gap == 0xffffu ? 0.f : __builtin_amdgcn_exp2f(l2);
+        o[e] = -a.c * p * fmaf(gh, fmaf(l2, kLn2, ent), g);
       }
       const int64_t mine = t - i0;
       if (mine >= 0 && mine < 8) {

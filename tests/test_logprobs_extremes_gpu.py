@@ -6,9 +6,9 @@ import pytest
 import torch
 
 from _util import seeded
-from test_logprobs_gpu import E, grads, near, reference
+from test_logprobs_gpu import E, grads, head, near, reference
 
-from qwen3_triton.kernels.logprobs import token_logprobs
+from qwen3_triton.kernels.logprobs import lm_head_logprobs, token_logprobs
 
 pytestmark = pytest.mark.gpu
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
@@ -107,3 +107,29 @@ def test_alternatives_of_rows_with_infinite_logits(v, dtype):
             out = token_logprobs(zr, ids, top=top)
             assert torch.equal(out.top_tokens, want[:, :top]), top
             assert bool(out.logprobs.isnan().all()) and bool(out.entropy.isnan().all()) and bool(out.top_logprobs.isnan().all())
+
+
+def test_lm_head_gradient_beside_ruled_out_tokens():
+    """Weights of -inf against a hidden feature of 1: whole groups of tokens whose logits are -inf.  Their probability is 0, and the
+    gradient of the weight is that of the others alone."""
+    t, h, v = 20, 64, 1024
+    x, w, ids = head(t, h, v, BF16)
+    x[:, 0], w[:, 0] = 1.0, 0.0
+    ids %= 256
+    keep = torch.ones(v, dtype=torch.bool)
+    keep[256:512], keep[700:] = False, False
+    w[~keep.cuda(), 0] = float('-inf')
+    g, gh = torch.randn(t, generator=seeded(1)).cuda(), torch.randn(t, generator=seeded(2)).cuda()
+    got = []
+    for weight in (w, w[keep.cuda()].contiguous()):
+        ids2 = torch.where(ids < 0, ids, ids)   # the first 256 tokens stand in both
+        wr = weight.clone().requires_grad_()
+        out = lm_head_logprobs(x, wr, ids2)
+        (dw,) = torch.autograd.grad([out.logprobs, out.entropy], wr, [g, gh])
+        got.append((out.logprobs, out.entropy, dw))
+    assert bool((got[0][2][~keep.cuda()] == 0).all())
+    for a, b in zip(got[0], got[1]):
+        a = a[keep.cuda()] if a.ndim == 2 else a
+        # the groups are others: sums in another order, and distances to other maxima (0.034 % of each probability, twice)
+        scale = float(b.double().abs().max())
+        assert bool(a.isfinite().all()) and float((a.double() - b.double()).abs().max()) <= (2.0 ** -7 + 7e-4) * scale
