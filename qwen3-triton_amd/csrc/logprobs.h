@@ -5,6 +5,9 @@
 namespace q3lp {
 
 constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
+// Logarithms of e^d as factors beside e^d itself: from here on down that is 0, and the product has to be (not 0 times infinity, nor
+// times what an upstream gradient makes of a larger number).
+constexpr float kDeep = -300.f;
 
 // Statistics of a part of a row: its maximum m, rest = the sum of e^d over all but one element that is m, and u = the sum of
 // e^d d, d counted from m in base 2.  m = -inf: nothing but -inf there (rest 0, or NaN where there is a NaN too).
@@ -18,7 +21,7 @@ Q3_DEV Part join(const Part& a, const Part& b, float c2) {
   const Part &hi = first ? a : b, &lo = first ? b : a;
   if (lo.m == -INFINITY) return Part{hi.m, hi.rest + lo.rest, hi.u};
   const float d = (lo.m - hi.m) * c2, w = __builtin_amdgcn_exp2f(d), t = 1.f + lo.rest;
-  return Part{hi.m, fmaf(t, w, hi.rest), fmaf(w, fmaf(t, fmaxf(d, -1e30f), lo.u), hi.u)};
+  return Part{hi.m, fmaf(t, w, hi.rest), fmaf(w, fmaf(t, fmaxf(d, kDeep), lo.u), hi.u)};
 }
 
 // Statistics of N values of a thread.  One element that is the maximum is taken out on the way to it (each step keeps the larger
@@ -51,7 +54,7 @@ template <int N> Q3_DEV Part part_of(const float (&v)[N], float c2) {
     for (int i = 1; i < N; ++i) {
       const float d = (x[i] - ref) * c2, e = __builtin_amdgcn_exp2f(d);
       p.rest += e;
-      p.u = fmaf(e, fmaxf(d, -1e30f), p.u);
+      p.u = fmaf(e, fmaxf(d, kDeep), p.u);
     }
   } else {
     const float mc = p.m == -INFINITY ? 0.f : p.m * c2, lost = p.m == -INFINITY ? 0.f : fmaf(p.m, c2, -mc);
@@ -60,7 +63,7 @@ template <int N> Q3_DEV Part part_of(const float (&v)[N], float c2) {
     for (int i = 1; i < N; ++i) {
       const float d = fmaf(x[i], c2, -mc), e = __builtin_amdgcn_exp2f(d);
       rest[i & 1] += e;
-      u[i & 1] = fmaf(e, fmaxf(d, -1e30f), u[i & 1]);
+      u[i & 1] = fmaf(e, fmaxf(d, kDeep), u[i & 1]);
     }
     const float k = __builtin_amdgcn_exp2f(-lost), r = rest[0] + rest[1];
     p.rest = r * k;

@@ -269,7 +269,7 @@ __global__ __launch_bounds__(kThreads) void slice_kernel(Fwd a) {
     const bool one = (threadIdx.x & 63) == (unsigned)__builtin_ctzll(at | (1ull << 63));
     const float d = (p.m - wm) * c2, w = p.m == -INFINITY ? 1.f : __builtin_amdgcn_exp2f(d);
     const float full = part_total(p), t = one ? p.rest : full;
-    p.u = group_sum<64>(p.m == -INFINITY ? 0.f : w * fmaf(full, fmaxf(d, -1e30f), p.u));
+    p.u = group_sum<64>(p.m == -INFINITY ? 0.f : w * fmaf(full, fmaxf(d, kDeep), p.u));
     p.rest = group_sum<64>(t * w);
     p.m = wm;
   }
@@ -477,7 +477,7 @@ template <typename T, typename O, bool FAR> __global__ __launch_bounds__(kThread
       for (int e = 0; e < V; ++e) {
         const float d = x.v[e] - m;
         const float p = __builtin_amdgcn_exp2f(fmaf(d, c2, -l2));
-        const float lp = fmaxf(fmaf(d, a.c, -ls), -1e30f);
+        const float lp = fmaxf(fmaf(d, a.c, -ls), kDeep);
         o[e] = -a.c * p * fmaf(gh, lp + ent, all);
       }
       // the given token, and the alternatives
@@ -491,7 +491,7 @@ template <typename T, typename O, bool FAR> __global__ __launch_bounds__(kThread
         for (int e = 0; e < V; ++e) {
           if (e != at) continue;
           const float lp = fmaf(x.v[e] - m, a.c, -ls), p = __builtin_amdgcn_exp2f(fmaf(x.v[e] - m, c2, -l2));
-          o[e] = a.c * (-expm1f(lp) * mine - p * fmaf(gh, fmaxf(lp, -1e30f) + ent, all - mine));
+          o[e] = a.c * (-expm1f(lp) * mine - p * fmaf(gh, fmaxf(lp, kDeep) + ent, all - mine));
         }
       }
     } else {
@@ -588,7 +588,7 @@ template <typename O> __global__ __launch_bounds__(kThreads) void head_grad_kern
     float o[8];
     if (live) {
       float at = fmaf(gm[i] - m, a.c, -ls) * kLog2e;
-      at = at < -1e30f ? -1e30f : at;  // a group of -inf only: its probabilities are 0
+      at = at < kDeep ? kDeep : at;  // a group of -inf only too
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const uint32_t gap = ((uint32_t)raw[i][e >> 1] >> (16 * (e & 1))) & 0xffffu;
@@ -598,7 +598,7 @@ template <typename O> __global__ __launch_bounds__(kThreads) void head_grad_kern
       const int64_t mine = t - i0;
       if (mine >= 0 && mine < 8) {
         const float p = __builtin_amdgcn_exp2f(tlp * kLog2e);
-        const float v = a.c * (-expm1f(tlp) * g - p * gh * (fmaxf(tlp, -1e30f) + ent));
+        const float v = a.c * (-expm1f(tlp) * g - p * gh * (fmaxf(tlp, kDeep) + ent));
 #pragma unroll
         for (int e = 0; e < 8; ++e)
           if (e == mine) o[e] = v;

@@ -109,6 +109,39 @@ def test_alternatives_of_rows_with_infinite_logits(v, dtype):
             assert bool(out.logprobs.isnan().all()) and bool(out.entropy.isnan().all()) and bool(out.top_logprobs.isnan().all())
 
 
+@pytest.mark.parametrize("size", [1.0, 1e12, 1e25])
+def test_large_gradients_of_entropies(size):
+    """Tokens of no probability add nothing to an entropy's gradient, however large it is."""
+    t, v = 6, 9000
+    gen = seeded(3)
+    z = torch.randn((t, v), generator=gen) * 2
+    z[:, ::3], z[2, 1::3], z[3, 5:] = float('-inf'), -1e20, -1e4
+    ids = torch.tensor([1, 2, 2, 0, 3, 8])   # some of them ruled out
+    z, ids = z.cuda(), ids.cuda()
+    g, gh = torch.zeros(t, device='cuda'), size * torch.randn(t, generator=gen).cuda()
+    zr = z.clone().requires_grad_()
+    (dz,) = torch.autograd.grad(token_logprobs(zr, ids).entropy, zr, gh)
+    none = torch.zeros((t, 0), device='cuda')
+    want, tol = grads(z, ids, g, gh, none, none.long(), 1.0)
+    near(dz, want, E * want.abs() + tol + 2.0 ** -126 * 1e3 * size)
+    # and from hidden states, some of whose logits are -inf, one group of 128 of them all
+    x, w, ids = head(t, 64, 1024, BF16)
+    x[:, 0], w[:, 0] = 1.0, 0.0
+    w[128:256, 0], w[300, 0] = float('-inf'), float('-inf')
+    wr = w.clone().requires_grad_()
+    (dw,) = torch.autograd.grad(lm_head_logprobs(x, wr, ids).entropy, wr, gh)
+    keep = w[:, 0] == 0
+    want, tol = grads(x.double() @ w.double().t(), ids, g, gh, none, none.long(), 1.0)
+    bound = (2.0 ** -7 * want.abs() + tol).t() @ x.double().abs()   # dz and dW round to bf16 once each
+    lp = (x.double() @ w.double().t()).log_softmax(-1)
+    p, span = lp.exp(), torch.where(lp.exp() > 0, lp.abs(), 0.0).amax(-1, keepdim=True)
+    off = 2 * 72 * E * (x.double().abs() @ w[keep].double().abs().t()).amax(-1, keepdim=True) + 3.5e-4   # a probability, of itself
+    bound += (p * gh.abs()[:, None] * (2 * span + 3) * off).t() @ x.double().abs()
+    exact = want.t() @ x.double()
+    assert bool((dw[~keep] == 0).all())
+    near(dw[keep], exact[keep], bound[keep] + 2.0 ** -8 * exact[keep].abs() + 2.0 ** -64 * size * 1e2)
+
+
 def test_lm_head_gradient_beside_ruled_out_tokens():
     """Weights of -inf against a hidden feature of 1: whole groups of tokens whose logits are -inf.  Their probability is 0, and the
     gradient of the weight is that of the others alone."""
