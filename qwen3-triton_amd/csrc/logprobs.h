@@ -78,11 +78,12 @@ template <int N> Q3_DEV Part part_of(const float (&v)[N], float c2) {
 // 0.034 % (half a step of 64 / 65535, times ln 2), a tenth of the rounding of a bf16 gradient and less than that of an fp16 one, at a
 // third of the memory and traffic of fp32 logits beside their gradient; below 2^-64 of the group's largest it is 0, as that of a
 // logit of -inf is.
-// (The distance in fp16 would be off by up to 0.4 % at e^-8, as much as the bf16 gradient's rounding.)
+// (The difference comes first: of m k, which is large at a small temperature, a rounding error would stay, 1 % of a probability for m
+// = 40 at 1e-4.  The distance in fp16 would be off by up to 0.4 % at e^-8, as much as the bf16 gradient's rounding.)
 constexpr float kGapRange = 64.f, kGapStep = kGapRange / 65535.f;
 Q3_DEV uint32_t gap2(float z0, float z1, float m, float c2) {
-  const float k = c2 * (1.f / kGapRange), mk = m * k;
-  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_u16(fmaf(z0, -k, mk), fmaf(z1, -k, mk)));
+  const float k = c2 * (1.f / kGapRange);
+  return __builtin_bit_cast(uint32_t, __builtin_amdgcn_cvt_pknorm_u16((m - z0) * k, (m - z1) * k));
 }
 
 }  // namespace q3lp

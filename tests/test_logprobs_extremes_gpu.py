@@ -142,6 +142,31 @@ def test_large_gradients_of_entropies(size):
     near(dw[keep], exact[keep], bound[keep] + 2.0 ** -8 * exact[keep].abs() + 2.0 ** -64 * size * 1e2)
 
 
+def test_lm_head_gradient_at_small_temperatures():
+    """Whole-number logits, exact in fp32, with several equal largest: each of k such tokens has the probability 1 / k.  A step of the
+    stored distance moves it by 3.4e-4; the gradient and the product round once each."""
+    gen = seeded(0)
+    h, v = 64, 1024
+    w = torch.randint(-2, 3, (v, h), generator=gen).float()
+    for seed in range(24):
+        x = torch.randint(-2, 3, (1, h), generator=seeded(seed)).float()
+        x[0, 0] = 1.0
+        best = int((x @ w.t()).argmax())
+        wr = w.clone()
+        wr[(torch.arange(4) * 250 + best + 1) % v] = w[best]
+        z = (x @ wr.t())[0].double()
+        for temperature in (0.01, 1e-3, 1e-4):
+            weight = wr.half().cuda().requires_grad_()
+            out = lm_head_logprobs(x.half().cuda(), weight, torch.tensor([best]).cuda(), temperature=temperature)
+            (dw,) = torch.autograd.grad(out.logprobs.sum(), weight)
+            p = (z / temperature).softmax(-1)
+            want = -p / temperature
+            want[best] += 1 / temperature
+            u = 2.0 ** -11
+            tol = want.abs() * (2 * u + 1.01 * 3.4e-4 + 400 * E) + 2.0 ** -24 + 2.0 ** -64 / temperature
+            near(dw[:, 0].cpu(), want, tol)
+
+
 def test_lm_head_gradient_beside_ruled_out_tokens():
     """Weights of -inf against a hidden feature of 1: whole groups of tokens whose logits are -inf.  Their probability is 0, and the
     gradient of the weight is that of the others alone."""
