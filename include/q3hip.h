@@ -303,6 +303,10 @@ int q3_gemm(const q3_gemm_desc* desc, void* workspace, size_t workspace_bytes, h
 /* The same plain product (no pieces, no epilogue) where k is far longer than m x n is large: k may be cut into up to 64 parts. */
 size_t q3_gemm_long_k_workspace_bytes(const q3_gemm_desc* desc);
 int q3_gemm_long_k(const q3_gemm_desc* desc, void* workspace, size_t workspace_bytes, hipStream_t stream);
+/* Either of the two (long_k) for fp16 operands, B K-major, and a plain product of one piece, times *scale (fp32 on the device) before it
+ * is rounded. */
+int q3_gemm_scaled(const q3_gemm_desc* desc, int long_k, const float* scale, void* workspace, size_t workspace_bytes,
+                   hipStream_t stream);
 /* Same product for arbitrary element strides: A(m,k) = A[m*sam + k*sak], B(k,n) = B[k*sbk + n*sbn];
  * any dtype (fp32 included).  SIMT path for shapes the matrix-core kernel does not take.
  * Replaces: kernels/linear.py:13-42 (_gemm with arbitrary strides). */
@@ -578,6 +582,18 @@ int q3_token_logprobs_bwd(int dtype, int out_dtype, const void* z, int64_t ld, i
                           int64_t ignore_index, float inv_temperature, int64_t top, const int64_t* top_token,
                           const float* row_max, const float* row_log, const float* entropy, const float* g,
                           const float* gh, const float* gtop, void* dz, int64_t ldo, hipStream_t stream);
+/* The same of dz times scale[0] (fp32 logits, fp16 gradient; null: 1).  scale [2] in fp32 on the device: a power of two and its
+ * inverse, which q3_logprobs_grad_scale chooses so that no value of dz passes 2^14, from the same upstream gradients (each or NULL).
+ * q3_gemm_scaled and q3_unscale_f16 (y [n] = x scale[1]) take it back from sums of products with dz before they round. */
+int q3_token_logprobs_bwd_scaled(int dtype, int out_dtype, const void* z, int64_t ld, int64_t rows, int64_t vocab,
+                                 const int64_t* tokens, int64_t ignore_index, float inv_temperature, int64_t top,
+                                 const int64_t* top_token, const float* row_max, const float* row_log, const float* entropy,
+                                 const float* g, const float* gh, const float* gtop, void* dz, int64_t ldo,
+                                 const float* scale, hipStream_t stream);
+int q3_logprobs_grad_scale(const float* g, const float* gh, const float* gtop, int64_t rows, int64_t vocab, int64_t top,
+                           const int64_t* tokens, int64_t ignore_index, float inv_temperature, float* scale,
+                           hipStream_t stream);
+int q3_unscale_f16(const float* x, void* y, int64_t n, const float* scale, hipStream_t stream);
 /* The same of the logits A . B^T (A [M, K] hidden states, B [N, K] the LM head's weight, N % 8 == 0, K % 64 == 0, 16-byte
  * aligned K-contiguous rows), which stay in fp32 registers: per row and group of 128 columns the maximum, rest and u of
  * csrc/logprobs.h to m_part, rest_part, u_part [ceil(N / 128)][ldp], and the logit of a row's token to pick [M].  z, or NULL: the
@@ -595,6 +611,11 @@ int q3_head_logprobs_bwd(int dtype, void* z, int64_t ldz, int64_t rows, int64_t 
                          int64_t ignore_index, float inv_temperature, const float* m_part, int64_t ldp,
                          const float* row_max, const float* row_log, const float* logprob, const float* entropy,
                          const float* g, const float* gh, hipStream_t stream);
+/* The same into dz [rows, vocab] (row stride ldo, a multiple of 8), which may be z, times scale[0] (fp16 only; null: 1). */
+int q3_head_logprobs_grad(int dtype, const void* z, int64_t ldz, void* dz, int64_t ldo, int64_t rows, int64_t vocab,
+                          const int64_t* tokens, int64_t ignore_index, float inv_temperature, const float* m_part,
+                          int64_t ldp, const float* row_max, const float* row_log, const float* logprob,
+                          const float* entropy, const float* g, const float* gh, const float* scale, hipStream_t stream);
 
 /* ------------------------------------------------------------------ attention over a shared prefix
  * New: no counterpart in the reference.  B rows in R groups of B / R; queries q [B, S, Hq, 128] of row b stand at its own

@@ -72,6 +72,7 @@ struct Args {
   const int64_t* tgt;
   float *m_part, *s_part, *pick;
   int64_t part0, ldp, col0;
+  const float* oscale;  // a plain product's factor, before it is rounded, or null
   float* u_part;  // log probability statistics: with m_part, s_part (rest) and log2(e) / temperature
   float c2;
   // Q8: scales of the A rows, and of the B rows of each piece (gate/up: of Wg and Wu)
@@ -117,7 +118,7 @@ Q3_DEV void work_coords(int bid, int tiles_m, int tiles_n, int splits, int& tm, 
 // (logprobs.h) of the fp32 logits per row and 128-column group, to m_part, s_part and u_part, with the logit of column tgt[row]
 // to pick[row], and where c[0] is set the logits' distances to their group's maximum in 16 bits (q3lp::kGapRange).  4096 x 151936 x 4096 takes 3.71 ms
 // with the statistics alone and 3.91 with the distances (1.30 PFLOP/s), as a plain product that writes its logits 3.76.  7: as 6, and B
-// is read past the caches (non-temporal).  KP: A and B in pieces along K.
+// is read past the caches (non-temporal).  8: as 0, times *oscale.  KP: A and B in pieces along K.
 template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool AT, bool BT, int EPI, bool KP, bool Q8>
 __global__ __launch_bounds__(WM * WN * 64) void gemm_tile_kernel(Args ar) {
   constexpr int NW = WM * WN;
@@ -443,6 +444,9 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile_kernel(Args ar) {
     }
     return;
   }
+  float by = 1.f;
+  if constexpr (EPI == 8) by = *ar.oscale;
+  auto scaled = [&](float x) { return EPI == 8 ? x * by : x; };
   u16* C = reinterpret_cast<u16*>(cp);
   if constexpr (Q8) {
     // One rounding: the product scaled, the residual (or SwiGLU) formed in fp32, then staged through LDS as below
@@ -508,7 +512,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile_kernel(Args ar) {
   } else {
     // 16-bit outputs: each wave rounds its tile into a private LDS block (16-byte chunks XOR-swizzled by row),
     // then works on whole rows with 16-byte accesses.
-    if (ar.vec || EPI != 0) {
+    if (ar.vec || (EPI != 0 && EPI != 8)) {
       constexpr int NC = EPI == 3 ? TNW / 2 : TNW, CH = NC / 8, RPI = 64 / CH;
       static_assert(CH == 2 || CH == 4 || CH == 8 || CH == 16, "16-byte chunks per staged row");
       char* wl = lds + wave * (TMW * NC * 2);
@@ -678,7 +682,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile_kernel(Args ar) {
         for (int i = 0; i < FM; ++i)
 #pragma unroll
           for (int j = 0; j < FN; ++j)
-            stage_out(i, j, pack2<T>(acc[i][j][0], acc[i][j][1]), pack2<T>(acc[i][j][2], acc[i][j][3]));
+            stage_out(i, j, pack2<T>(scaled(acc[i][j][0]), scaled(acc[i][j][1])), pack2<T>(scaled(acc[i][j][2]), scaled(acc[i][j][3])));
         const int64_t r0 = (int64_t)(ma + wm * TMW), c0 = nb + wn * TNW + c * 8;
         lds_wait();
         __builtin_amdgcn_wave_barrier();
@@ -732,7 +736,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile_kernel(Args ar) {
       }
     }
   }
-  if constexpr (EPI == 0 && !Q8) {
+  if constexpr ((EPI == 0 || EPI == 8) && !Q8) {
 #pragma unroll
     for (int i = 0; i < FM; ++i) {
       const int row = ma + wm * TMW + i * 16 + j16;
@@ -744,7 +748,7 @@ __global__ __launch_bounds__(WM * WN * 64) void gemm_tile_kernel(Args ar) {
 #pragma unroll
         for (int v = 0; v < 4; ++v)
           if (col + v < ncols) {
-            float x = to_f32<T>(from_f32<T>(acc[i][j][v]));
+            float x = to_f32<T>(from_f32<T>(scaled(acc[i][j][v])));
             if (ar.res) x += to_f32<T>(ar.res[(int64_t)row * ar.ldres + col + v]);
             crow[col + v] = from_f32<T>(x);
           }

@@ -6,7 +6,7 @@
 namespace q3gemm {
 int launch_tile_nt(int dtype, int cfg, int epi, const Args& a, hipStream_t s);
 int launch_tile_nn(int dtype, int cfg, int epi, const Args& a, hipStream_t s);
-int launch_tile_tn(int dtype, int cfg, const Args& a, hipStream_t s);
+int launch_tile_tn(int dtype, int cfg, int epi, const Args& a, hipStream_t s);
 int launch_tile_q8(int dtype, int cfg, int epi, const Args& a, hipStream_t s);
 int launch_rows_q8(int dtype, int epi, const Args& a, const RowIn& in, hipStream_t s);
 }  // namespace q3gemm
@@ -110,12 +110,16 @@ Plan plan_for(const Args& a, bool at, bool bt, int most, double combine) {
 
 // ---------------------------------------------------------------- combining passes
 // Sum of the fp32 partial products of one 8-column chunk, rounded to T.
-template <typename T> Q3_DEV Vec<T> sum_parts(const float* p, int splits, int64_t ld) {
+template <typename T> Q3_DEV Vec<T> sum_parts(const float* p, int splits, int64_t ld, const float* scale = nullptr) {
   f32x4 s0 = *reinterpret_cast<const f32x4*>(p), s1 = *reinterpret_cast<const f32x4*>(p + 4);
   for (int i = 1; i < splits; ++i) {
     p += ld;
     s0 += *reinterpret_cast<const f32x4*>(p);
     s1 += *reinterpret_cast<const f32x4*>(p + 4);
+  }
+  if (scale) {
+    s0 *= *scale;
+    s1 *= *scale;
   }
   Vec<T> r;
 #pragma unroll
@@ -135,7 +139,7 @@ template <typename T> __global__ __launch_bounds__(256) void combine_kernel(Args
   const int64_t cols = a.N / 8, i = (int64_t)blockIdx.x * 256 + threadIdx.x;
   if (i >= a.M * cols) return;
   int64_t r = i / cols, c = (i - r * cols) * 8;
-  Vec<T> v = sum_parts<T>(a.part + r * a.N + c, a.splits, a.M * a.N);
+  Vec<T> v = sum_parts<T>(a.part + r * a.N + c, a.splits, a.M * a.N, a.oscale);
   int s = 0;
   int64_t beg = 0;
   if (a.axis >= 2) {
@@ -164,7 +168,7 @@ template <typename T> __global__ __launch_bounds__(256) void combine_many_kernel
   for (int e = 0; e < 8; ++e) {
     float x = e < 4 ? s0[e] : s1[e - 4];
     for (int o = 1; o < 8; o <<= 1) x += __shfl_xor(x, o, 8);
-    v.v[e] = x;
+    v.v[e] = a.oscale ? x * *a.oscale : x;
   }
   if (on && (threadIdx.x & 7) == 0) store_vec<T>(reinterpret_cast<u16*>(a.c[0]) + r * a.ldc[0] + c, v);
 }
@@ -410,7 +414,7 @@ void set_grid(Launch& l) {
 
 int launch(const Call& c, const Launch& l, int dtype, hipStream_t s) {
   if (c.q8) return q3gemm::launch_tile_q8(dtype, l.p.cfg, c.epi, l.a, s);
-  if (c.at) return q3gemm::launch_tile_tn(dtype, l.p.cfg, l.a, s);
+  if (c.at) return q3gemm::launch_tile_tn(dtype, l.p.cfg, c.epi, l.a, s);
   if (c.bt) return q3gemm::launch_tile_nn(dtype, l.p.cfg, c.epi, l.a, s);
   return q3gemm::launch_tile_nt(dtype, l.p.cfg, c.epi, l.a, s);
 }
@@ -602,6 +606,15 @@ int q3_gemm(const q3_gemm_desc* d, void* workspace, size_t workspace_bytes, hipS
 int q3_gemm_long_k(const q3_gemm_desc* d, void* workspace, size_t workspace_bytes, hipStream_t stream) {
   Call c;
   Q3_REQUIRE(parse_long_k(d, c));
+  return run(d, c, workspace, workspace_bytes, stream);
+}
+
+int q3_gemm_scaled(const q3_gemm_desc* d, int long_k, const float* scale, void* workspace, size_t workspace_bytes, hipStream_t stream) {
+  Call c;
+  Q3_REQUIRE(d && d->dtype == Q3_F16 && scale && ((uintptr_t)scale & 3) == 0 && parse_long_k(d, c) && c.bt);
+  c.epi = 8;
+  if (!long_k && c.most > 1) c.most = kMost;
+  c.a.oscale = scale;
   return run(d, c, workspace, workspace_bytes, stream);
 }
 

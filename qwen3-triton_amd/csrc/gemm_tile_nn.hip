@@ -1,5 +1,5 @@
 // gemm_tile.h instantiated for a k-contiguous A and a K-major B: the input gradients dX = dY W, also with
-// the operands in pieces along k (several projections of one input) and with the SwiGLU backward.
+// the operands in pieces along k (several projections of one input) with the SwiGLU backward, and times a factor (fp16).
 #include "gemm_tile.h"
 
 namespace q3gemm {
@@ -18,6 +18,7 @@ template <typename T, int EPI, bool KP> static int nn(int cfg, const Args& a, hi
 
 int launch_tile_nn(int dtype, int cfg, int epi, const Args& a, hipStream_t s) {
   if (epi == 5) return dtype == Q3_BF16 ? nn<BF16, 5, false>(cfg, a, s) : nn<F16, 5, false>(cfg, a, s);
+  if (epi == 8) return nn<F16, 8, false>(cfg, a, s);
   if (a.axis == 1) return dtype == Q3_BF16 ? nn<BF16, 0, true>(cfg, a, s) : nn<F16, 0, true>(cfg, a, s);
   return dtype == Q3_BF16 ? nn<BF16, 0, false>(cfg, a, s) : nn<F16, 0, false>(cfg, a, s);
 }

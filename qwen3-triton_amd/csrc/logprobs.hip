@@ -414,7 +414,43 @@ struct Bwd {
   const float *m, *ls, *entropy, *g, *gh, *gtop;
   void* dz;
   int64_t ldo;
+  const float* scale;  // fp16 gradients: a power of two that they are multiplied with (scale_kernel), or null
 };
+Q3_DEV float scale_of(const Bwd& a) { return a.scale ? *a.scale : 1.f; }
+
+// A gradient in fp16 that products are formed from is scaled into the type's range, and the products take the scale back before they
+// round: with a mean of 4096 rows and 151936 tokens, single values (1e-9) would be below its smallest number and add up to nothing.
+// scale[0] = 2^e such that no value passes 2^14, scale[1] = 2^-e: what |dz| is at most, c (|g| + sum |g_j| + |h| (1 + log V)), from all
+// rows that are not left out and have a number for it (p |log p| <= 1 / e, p entropy <= log V).  One value for all rows, since dW sums over
+// them.  One workgroup (4096 rows 5 us).
+constexpr int kScaleThreads = 1024;
+__global__ __launch_bounds__(kScaleThreads) void scale_kernel(Bwd a, float log_v, float* __restrict__ scale) {
+  __shared__ float wave_most[kScaleThreads / 64];
+  float most = 0.f;
+  for (int64_t r = threadIdx.x; r < a.rows; r += kScaleThreads) {
+    float x = (a.g ? fabsf(a.g[r]) : 0.f) + (a.gh ? fabsf(a.gh[r]) * (1.f + log_v) : 0.f);
+    if (a.gtop)
+      for (int j = 0; j < a.top; ++j) x += fabsf(a.gtop[r * a.top + j]);
+    x *= a.c;
+    if (a.tok[r] != a.ignore && x < INFINITY) most = fmaxf(most, x);
+  }
+  most = group_max<64>(most);
+  if ((threadIdx.x & 63) == 0) wave_most[threadIdx.x >> 6] = most;
+  __syncthreads();
+  if (threadIdx.x != 0) return;
+  for (int w = 1; w < kScaleThreads / 64; ++w) most = fmaxf(most, wave_most[w]);
+  int x = 14;
+  if (most > 0.f) frexpf(most, &x);  // most <= 2^x
+  const int e = max(-110, min(14 - x, 110));
+  scale[0] = ldexpf(1.f, e);
+  scale[1] = ldexpf(1.f, -e);
+}
+
+// 16-bit results of sums in fp32, times scale[1].
+__global__ __launch_bounds__(kThreads) void unscale_kernel(const float* __restrict__ x, u16* __restrict__ y, int64_t n, const float* __restrict__ scale) {
+  const float s = scale[1];
+  for (int64_t i = (int64_t)blockIdx.x * kThreads + threadIdx.x; i < n; i += (int64_t)gridDim.x * kThreads) y[i] = from_f32<F16>(x[i] * s);
+}
 
 // 32 (fp32: 16) values a thread, all loads before the first use; bound by the logits' read and the gradient's write (2048 x 151936
 // bf16: 1.24 GB in 260 us).  Rows left out are zeros, and nothing of them is read.
@@ -455,15 +491,16 @@ template <typename T, typename O, bool FAR> __global__ __launch_bounds__(kThread
     }
   }
   float m = 0.f, ls = 0.f, g = 0.f, gh = 0.f, ent = 0.f, all = 0.f;
+  const float by = O::code == Q3_F16 && T::code == Q3_F32 ? scale_of(a) : 1.f;
   if (live) {
     m = a.m[r];
     ls = a.ls[r];
     ent = a.entropy[r];
-    g = a.g ? (t >= 0 && t < a.vocab ? a.g[r] : NAN) : 0.f;
-    gh = a.gh ? a.gh[r] : 0.f;
+    g = a.g ? (t >= 0 && t < a.vocab ? a.g[r] * by : NAN) : 0.f;
+    gh = a.gh ? a.gh[r] * by : 0.f;
     all = g;
     if (a.gtop)
-      for (int j = 0; j < a.top; ++j) all += a.gtop[r * a.top + j];
+      for (int j = 0; j < a.top; ++j) all += a.gtop[r * a.top + j] * by;
   }
   const float c2 = a.c * kLog2e, l2 = ls * kLog2e;
 #pragma unroll
@@ -486,7 +523,7 @@ template <typename T, typename O, bool FAR> __global__ __launch_bounds__(kThread
         if (at < 0 || at >= V) continue;
         float mine = i0 + at == t ? g : 0.f;
         if (a.gtop)
-          for (int k = 0; k < a.top; ++k) mine += a.top_token[r * a.top + k] == i0 + at ? a.gtop[r * a.top + k] : 0.f;
+          for (int k = 0; k < a.top; ++k) mine += a.top_token[r * a.top + k] == i0 + at ? a.gtop[r * a.top + k] * by : 0.f;
 #pragma unroll
         for (int e = 0; e < V; ++e) {
           if (e != at) continue;
@@ -552,7 +589,7 @@ template <int R, int NT> __global__ __launch_bounds__(NT) void head_finish_kerne
   finish_row(a, r, p, valid ? h.pick[r] : 0.f, valid);
 }
 
-// dz in the place of what the product left of the logits (their distances to their group's maximum): as grad_kernel, with
+// dz from what the product left of the logits (their distances to their group's maximum), in its place or elsewhere: as grad_kernel, with
 // log2 p = (c2 (m_group - M) - ls log2(e)) - distance; the given token's log p is the result itself.  Bound by z, read and written
 // (4096 x 151936: 2.5 GB in 442 us, 5.6 TB/s).
 template <typename O> __global__ __launch_bounds__(kThreads) void head_grad_kernel(Head h, Bwd a, const float* logprob, int slices) {
@@ -560,7 +597,8 @@ template <typename O> __global__ __launch_bounds__(kThreads) void head_grad_kern
   const int64_t r = blockIdx.x / (unsigned)slices;
   const int base = (int)(blockIdx.x - (unsigned)(r * slices)) * N + (int)threadIdx.x * 8, vocab = (int)a.vocab;
   const int64_t t = a.tok[r];
-  u16* row = (u16*)a.dz + r * a.ldo;
+  const u16* row = (const u16*)a.z + r * a.ld;
+  u16* out = (u16*)a.dz + r * a.ldo;
   const bool live = t != a.ignore;
   i32x4 raw[C];
   float gm[C];
@@ -578,8 +616,9 @@ template <typename O> __global__ __launch_bounds__(kThreads) void head_grad_kern
     ls = a.ls[r];
     ent = a.entropy[r];
     tlp = logprob[r];
-    g = a.g ? (t >= 0 && t < vocab ? a.g[r] : NAN) : 0.f;
-    gh = a.gh ? a.gh[r] : 0.f;
+    const float by = O::code == Q3_F16 ? scale_of(a) : 1.f;
+    g = a.g ? (t >= 0 && t < vocab ? a.g[r] * by : NAN) : 0.f;
+    gh = a.gh ? a.gh[r] * by : 0.f;
   }
 #pragma unroll
   for (int i = 0; i < C; ++i) {
@@ -607,7 +646,7 @@ template <typename O> __global__ __launch_bounds__(kThreads) void head_grad_kern
 #pragma unroll
       for (int e = 0; e < 8; ++e) o[e] = 0.f;
     }
-    store_values<O, 8, false>(row + i0, o);
+    store_values<O, 8, false>(out + i0, o);
   }
 }
 
@@ -716,21 +755,54 @@ int q3_token_logprobs(int dtype, const void* z, int64_t ld, int64_t rows, int64_
   return forward<F32>(a, c, stream);
 }
 
-int q3_token_logprobs_bwd(int dtype, int out_dtype, const void* z, int64_t ld, int64_t rows, int64_t vocab, const int64_t* tokens,
-                          int64_t ignore_index, float inv_temperature, int64_t top, const int64_t* top_token,
-                          const float* row_max, const float* row_log, const float* entropy, const float* g, const float* gh,
-                          const float* gtop, void* dz, int64_t ldo, hipStream_t stream) {
+int q3_token_logprobs_bwd_scaled(int dtype, int out_dtype, const void* z, int64_t ld, int64_t rows, int64_t vocab, const int64_t* tokens,
+                                 int64_t ignore_index, float inv_temperature, int64_t top, const int64_t* top_token,
+                                 const float* row_max, const float* row_log, const float* entropy, const float* g, const float* gh,
+                                 const float* gtop, void* dz, int64_t ldo, const float* scale,
+                                 hipStream_t stream) {
   Q3_REQUIRE(sizes_ok(dtype, rows, vocab, top) && z && tokens && row_max && row_log && entropy && dz && ld >= vocab &&
              ldo >= vocab && (!gtop || (top > 0 && top_token)) && inv_temperature > 0.f && inv_temperature < INFINITY);
+  Q3_REQUIRE(!scale || (dtype == Q3_F32 && out_dtype == Q3_F16 && ((uintptr_t)scale & 3) == 0));
   Q3_REQUIRE(out_dtype == dtype || (dtype == Q3_F32 && dtype_ok(out_dtype)));
   Q3_REQUIRE(((uintptr_t)z & (dtype == Q3_F32 ? 3 : 1)) == 0 && ((uintptr_t)dz & (out_dtype == Q3_F32 ? 3 : 1)) == 0 && dz != z);
   const Bwd a{z, ld, rows, vocab, tokens, ignore_index, inv_temperature, (int)top, top_token, row_max, row_log, entropy, g, gh,
-              gtop, dz, ldo};
+              gtop, dz, ldo, scale};
   if (dtype == Q3_BF16) return backward<BF16, BF16>(a, stream);
   if (dtype == Q3_F16) return backward<F16, F16>(a, stream);
   if (out_dtype == Q3_BF16) return backward<F32, BF16>(a, stream);
   if (out_dtype == Q3_F16) return backward<F32, F16>(a, stream);
   return backward<F32, F32>(a, stream);
+}
+
+int q3_token_logprobs_bwd(int dtype, int out_dtype, const void* z, int64_t ld, int64_t rows, int64_t vocab, const int64_t* tokens,
+                          int64_t ignore_index, float inv_temperature, int64_t top, const int64_t* top_token,
+                          const float* row_max, const float* row_log, const float* entropy, const float* g, const float* gh,
+                          const float* gtop, void* dz, int64_t ldo, hipStream_t stream) {
+  return q3_token_logprobs_bwd_scaled(dtype, out_dtype, z, ld, rows, vocab, tokens, ignore_index, inv_temperature, top, top_token,
+                                      row_max, row_log, entropy, g, gh, gtop, dz, ldo, nullptr, stream);
+}
+
+int q3_logprobs_grad_scale(const float* g, const float* gh, const float* gtop, int64_t rows, int64_t vocab, int64_t top,
+                           const int64_t* tokens, int64_t ignore_index, float inv_temperature, float* scale, hipStream_t stream) {
+  Q3_REQUIRE(rows > 0 && rows < (1ll << 31) && vocab > 0 && vocab < (1ll << 30) && top >= 0 && top <= kMaxTop && tokens && scale &&
+             ((uintptr_t)scale & 3) == 0 && (!gtop || top > 0) && inv_temperature > 0.f && inv_temperature < INFINITY);
+  Bwd a{};
+  a.rows = rows;
+  a.tok = tokens;
+  a.ignore = ignore_index;
+  a.c = inv_temperature;
+  a.top = (int)top;
+  a.g = g;
+  a.gh = gh;
+  a.gtop = gtop;
+  scale_kernel<<<1, kScaleThreads, 0, stream>>>(a, logf((float)vocab), scale);
+  return (int)hipGetLastError();
+}
+
+int q3_unscale_f16(const float* x, void* y, int64_t n, const float* scale, hipStream_t stream) {
+  Q3_REQUIRE(x && y && scale && n > 0 && ((uintptr_t)x & 3) == 0 && ((uintptr_t)y & 1) == 0 && ((uintptr_t)scale & 3) == 0);
+  unscale_kernel<<<(unsigned)std::min<int64_t>(cdiv(n, kThreads), 4096), kThreads, 0, stream>>>(x, (u16*)y, n, scale);
+  return (int)hipGetLastError();
 }
 
 int q3_head_logprobs_finish(const float* m_part, const float* rest_part, const float* u_part, int64_t ldp, const float* pick,
@@ -754,19 +826,29 @@ int q3_head_logprobs_finish(const float* m_part, const float* rest_part, const f
   return (int)hipGetLastError();
 }
 
-int q3_head_logprobs_bwd(int dtype, void* z, int64_t ldz, int64_t rows, int64_t vocab, const int64_t* tokens, int64_t ignore_index,
-                         float inv_temperature, const float* m_part, int64_t ldp, const float* row_max, const float* row_log,
-                         const float* logprob, const float* entropy, const float* g, const float* gh, hipStream_t stream) {
+int q3_head_logprobs_grad(int dtype, const void* z, int64_t ldz, void* dz, int64_t ldo, int64_t rows, int64_t vocab, const int64_t* tokens,
+                          int64_t ignore_index, float inv_temperature, const float* m_part, int64_t ldp, const float* row_max,
+                          const float* row_log, const float* logprob, const float* entropy, const float* g, const float* gh,
+                          const float* scale, hipStream_t stream) {
   Q3_REQUIRE((dtype == Q3_BF16 || dtype == Q3_F16) && z && ((uintptr_t)z & 15) == 0 && vocab > 0 && vocab < (1ll << 30) - (1 << 16) &&
              vocab % 8 == 0 && ldz >= vocab && ldz % 8 == 0 && rows > 0 && rows < (1ll << 31) && ldp >= rows && tokens && m_part &&
              row_max && row_log && logprob && entropy && inv_temperature > 0.f && inv_temperature < INFINITY);
+  Q3_REQUIRE(dz && ((uintptr_t)dz & 15) == 0 && ldo >= vocab && ldo % 8 == 0 && (dz != z || ldo == ldz));
+  Q3_REQUIRE(!scale || (dtype == Q3_F16 && ((uintptr_t)scale & 3) == 0));
   const int64_t n = cdiv(vocab, (int64_t)kThreads * 8 * kGradVectors);
   Q3_REQUIRE(rows * n < (1ll << 31));
-  const Bwd a{nullptr, 0, rows, vocab, tokens, ignore_index, inv_temperature, 0, nullptr, row_max, row_log, entropy, g, gh, nullptr, z, ldz};
+  const Bwd a{z, ldz, rows, vocab, tokens, ignore_index, inv_temperature, 0, nullptr, row_max, row_log, entropy, g, gh, nullptr, dz, ldo, scale};
   const Head h{m_part, nullptr, nullptr, nullptr, ldp, 0};
   if (dtype == Q3_BF16) head_grad_kernel<BF16><<<(unsigned)(rows * n), kThreads, 0, stream>>>(h, a, logprob, (int)n);
   else head_grad_kernel<F16><<<(unsigned)(rows * n), kThreads, 0, stream>>>(h, a, logprob, (int)n);
   return (int)hipGetLastError();
+}
+
+int q3_head_logprobs_bwd(int dtype, void* z, int64_t ldz, int64_t rows, int64_t vocab, const int64_t* tokens, int64_t ignore_index,
+                         float inv_temperature, const float* m_part, int64_t ldp, const float* row_max, const float* row_log,
+                         const float* logprob, const float* entropy, const float* g, const float* gh, hipStream_t stream) {
+  return q3_head_logprobs_grad(dtype, z, ldz, z, ldz, rows, vocab, tokens, ignore_index, inv_temperature, m_part, ldp, row_max, row_log,
+                               logprob, entropy, g, gh, nullptr, stream);
 }
 
 }  // extern "C"

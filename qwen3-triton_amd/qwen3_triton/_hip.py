@@ -124,6 +124,7 @@ SIGNATURES: dict[str, tuple] = {
     "q3_gemm": (_i32, [_p, _p, _sz, _p]),
     "q3_gemm_long_k_workspace_bytes": (_sz, [_p]),
     "q3_gemm_long_k": (_i32, [_p, _p, _sz, _p]),
+    "q3_gemm_scaled": (_i32, [_p, _i32, _p, _p, _sz, _p]),
     "q3_quant_rows": (_i32, [_i32, _p, _i64, _p, _p, _i64, _i64, _p]),
     "q3_rmsnorm_quant": (_i32, [_i32, _p, _i64, _p, _i64, _p, _p, _p, _p, _i64, _i64, _f32, _p]),
     "q3_gemm_int8_workspace_bytes": (_sz, [_p]),
@@ -141,9 +142,14 @@ SIGNATURES: dict[str, tuple] = {
     "q3_token_logprobs": (_i32, [_i32, _p, _i64, _i64, _i64, _p, _i64, _f32, _i64, _p, _p, _p, _p, _p, _p, _p, _sz, _p]),
     "q3_token_logprobs_bwd": (_i32, [_i32, _i32, _p, _i64, _i64, _i64, _p, _i64, _f32, _i64, _p, _p, _p, _p, _p, _p, _p, _p, _i64,
                                      _p]),
+    "q3_token_logprobs_bwd_scaled": (_i32, [_i32, _i32, _p, _i64, _i64, _i64, _p, _i64, _f32, _i64, _p, _p, _p, _p, _p, _p, _p, _p,
+                                            _i64, _p, _p]),
+    "q3_logprobs_grad_scale": (_i32, [_p, _p, _p, _i64, _i64, _i64, _p, _i64, _f32, _p, _p]),
+    "q3_unscale_f16": (_i32, [_p, _p, _i64, _p, _p]),
     "q3_gemm_nt_logprobs": (_i32, [_i32, _p, _i64, _p, _i64, _i64, _i64, _i64, _p, _f32, _p, _p, _p, _p, _i64, _p, _i64, _p]),
     "q3_head_logprobs_finish": (_i32, [_p, _p, _p, _i64, _p, _i64, _i64, _p, _i64, _f32, _p, _p, _p, _p, _p]),
     "q3_head_logprobs_bwd": (_i32, [_i32, _p, _i64, _i64, _i64, _p, _i64, _f32, _p, _i64, _p, _p, _p, _p, _p, _p, _p]),
+    "q3_head_logprobs_grad": (_i32, [_i32, _p, _i64, _p, _i64, _i64, _i64, _p, _i64, _f32, _p, _i64, _p, _p, _p, _p, _p, _p, _p, _p]),
     "q3_prefix_attention_workspace_bytes": (_sz, [_i64] * 8),
     "q3_prefix_attention": (_i32, [_i32, _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _p, _i64, _i64, _i64, _p, _i64,
                                    _i64, _i64, _p, _sz, *[_i64] * 9, _p, _i64, _f32, _p]),

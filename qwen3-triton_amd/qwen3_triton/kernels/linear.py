@@ -67,11 +67,12 @@ def chunk_aligned(t):
 
 
 def gemm(a, b, c, m, n, k, *, kmajor=(False, False), axis=0, epilogue=H.GEMM_PLAIN, res=None, norm=None, g=None,
-         u=None, long_k=False):
+         u=None, long_k=False, scale=None):
     """``q3_gemm``: c = A B over ``m x n x k``.  ``a``, ``b``, ``c`` are lists of matrices: one each, or along
     ``axis`` (1: k, 2: n, 3: m) the pieces that lie side by side; gate/up takes both weights in ``b`` and the
     SwiGLU backward dg and du in ``c``.  ``norm`` = (weight, eps, y) for the residual + norm epilogue.
-    ``long_k``: a plain product whose k may be cut into more parts than eight (``q3_gemm_long_k``)."""
+    ``long_k``: a plain product whose k may be cut into more parts than eight (``q3_gemm_long_k``).  ``scale`` (fp16, a plain
+    product): the device address of an fp32 factor of the result, taken before it is rounded (``q3_gemm_scaled``)."""
     d = H.GemmDesc()
     d.dtype, d.a_kmajor, d.b_kmajor, d.axis, d.epilogue = H.code(a[0].dtype), kmajor[0], kmajor[1], axis, epilogue
     d.m, d.n, d.k = m, n, k
@@ -99,7 +100,10 @@ def gemm(a, b, c, m, n, k, *, kmajor=(False, False), axis=0, epilogue=H.GEMM_PLA
     entry = "q3_gemm_long_k" if long_k else "q3_gemm"
     nbytes = H.query(entry + "_workspace_bytes", ref)
     ws = H.workspace(nbytes, a[0].device) if nbytes else None
-    H.call(entry, ref, None if ws is None else ws.data_ptr(), nbytes, H.stream())
+    if scale is None:
+        H.call(entry, ref, None if ws is None else ws.data_ptr(), nbytes, H.stream())
+    else:
+        H.call("q3_gemm_scaled", ref, int(long_k), scale, None if ws is None else ws.data_ptr(), nbytes, H.stream())
 
 
 def gemm_nt_into(a, lda, bnk, ldb, out, m, n, k, *, alpha=1.0, accumulate=False):

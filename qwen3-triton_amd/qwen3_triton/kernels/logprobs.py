@@ -91,13 +91,16 @@ def _shaped(shape, top, lp, ent, tlp, tid, _=None):
     return lp, ent, tlp, tid
 
 
-def _backward(z, rows, ld, v, tokens, ignore_index, temperature, top, top_tokens, kept, ent, g, gh, gtop, dz, ldo, at=0):
-    """q3_token_logprobs_bwd of rows ``at`` .. ``at`` + rows - 1 (z and dz start there)."""
+def _backward(z, rows, ld, v, tokens, ignore_index, temperature, top, top_tokens, kept, ent, g, gh, gtop, dz, ldo, at=0, scale=None):
+    """q3_token_logprobs_bwd of rows ``at`` .. ``at`` + rows - 1 (z and dz start there), times ``scale``."""
     def p(t, width=4):
         return None if t is None else t.data_ptr() + at * width
-    H.launch(z, "q3_token_logprobs_bwd", H.code(z.dtype), H.code(dz.dtype), z.data_ptr(), ld, rows, v, p(tokens, 8), ignore_index,
-             1.0 / temperature, top, p(top_tokens, 8 * top), p(kept), p(kept[1]), p(ent), p(g), p(gh), p(gtop, 4 * top),
-             dz.data_ptr(), ldo)
+    args = (H.code(z.dtype), H.code(dz.dtype), z.data_ptr(), ld, rows, v, p(tokens, 8), ignore_index, 1.0 / temperature, top,
+            p(top_tokens, 8 * top), p(kept), p(kept[1]), p(ent), p(g), p(gh), p(gtop, 4 * top), dz.data_ptr(), ldo)
+    if scale is None:
+        H.launch(z, "q3_token_logprobs_bwd", *args)
+    else:
+        H.launch(z, "q3_token_logprobs_bwd_scaled", *args, scale.data_ptr())
 
 
 def _upstream(g):
@@ -240,45 +243,73 @@ class _LMHeadLogprobs(torch.autograd.Function):
         z, ctx.z = ctx.z, None   # consumed: the gradient takes the stored logits' place
         with H.on(x):
             dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
+            scale = _grad_scale(x, g, gh, gtop, v, top, tokens, ignore_index, temperature)
             if groups is not None:
                 if z is None:   # a second backward: the same logits again
                     z = _fused_product(x, weight, tokens, temperature, True)[2]
-                H.call("q3_head_logprobs_bwd", H.code(x.dtype), z.data_ptr(), v, t, v, tokens.data_ptr(), ignore_index, 1.0 / temperature,
-                       groups.data_ptr(), t, kept.data_ptr(), kept.data_ptr() + 4 * t, lp.data_ptr(), ent.data_ptr(),
-                       None if g is None else g.data_ptr(), None if gh is None else gh.data_ptr(), H.stream())
-                dw = _products(z, x, weight, dx, ctx.needs_input_grad[1])
+                H.call("q3_head_logprobs_grad", H.code(x.dtype), z.data_ptr(), v, z.data_ptr(), v, t, v, tokens.data_ptr(), ignore_index,
+                       1.0 / temperature, groups.data_ptr(), t, kept.data_ptr(), kept.data_ptr() + 4 * t, lp.data_ptr(), ent.data_ptr(),
+                       None if g is None else g.data_ptr(), None if gh is None else gh.data_ptr(), _address(scale), H.stream())
+                dw = _products(z, x, weight, dx, ctx.needs_input_grad[1], scale)
             else:
                 whole = gemm_ok(x, weight) and v % 8 == 0   # dW = dz^T x and dX = dz W from one dz [T, V]
                 chunks = _chunks(t, v)
                 z = torch.empty((chunks[0][1], v), device=x.device, dtype=torch.float32)
                 dz = torch.empty((t if whole else chunks[0][1], v), device=x.device, dtype=x.dtype)
-                dw = None
+                dw = part = None
                 if not whole and ctx.needs_input_grad[1]:
                     dw = torch.empty((v, h), device=x.device, dtype=torch.float32)
+                if not whole and dx is not None and scale is not None:
+                    part = torch.empty((chunks[0][1], h), device=x.device, dtype=torch.float32)
                 for r, end in chunks:
                     n, at = end - r, r if whole else 0
                     _logits(x[r:end], weight, z[:n])
-                    _backward(z, n, v, v, tokens, ignore_index, temperature, top, tid, kept, ent, g, gh, gtop, dz[at:], v, r)
+                    _backward(z, n, v, v, tokens, ignore_index, temperature, top, tid, kept, ent, g, gh, gtop, dz[at:], v, r, scale)
                     if not whole and dx is not None:
-                        matmul_into(dz[:n], weight, dx[r:end])
+                        matmul_into(dz[:n], weight, dx[r:end] if part is None else part[:n])
+                        if part is not None:
+                            _unscale(part[:n], dx[r:end], scale)
                     if dw is not None:
                         matmul_into(dz[:n].t(), x[r:end], dw, accumulate=r > 0)
                 if whole:
-                    dw = _products(dz, x, weight, dx, ctx.needs_input_grad[1])
+                    dw = _products(dz, x, weight, dx, ctx.needs_input_grad[1], scale)
+                elif dw is not None and scale is not None:
+                    dw = _unscale(dw, torch.empty_like(weight), scale)
                 elif dw is not None and dw.dtype != weight.dtype:
                     dw = cast(dw, weight.dtype)
         return None if dx is None else dx.view(hidden.shape), dw, None, None, None, None
 
 
-def _products(dz, x, weight, dx, need_dw):
-    """dX = dz W into ``dx`` (None: not wanted); returns dW = dz^T x or None."""
+def _address(t):
+    return None if t is None else t.data_ptr()
+
+
+def _grad_scale(x, g, gh, gtop, v, top, tokens, ignore_index, temperature):
+    """[factor, its inverse] of the logits' gradient in fp16, chosen on the device from the upstream gradients; None for types with
+    fp32's exponents.  Single values of it, p g, would be lost where dX and dW, which sum over them, are not."""
+    if x.dtype != torch.float16:
+        return None
+    scale = x.new_empty(2, dtype=torch.float32)
+    H.call("q3_logprobs_grad_scale", _address(g), _address(gh), _address(gtop), x.shape[0], v, top, tokens.data_ptr(), ignore_index,
+           1.0 / temperature, scale.data_ptr(), H.stream())
+    return scale
+
+
+def _unscale(x, out, scale):
+    H.call("q3_unscale_f16", x.data_ptr(), out.data_ptr(), x.numel(), scale.data_ptr(), H.stream())
+    return out
+
+
+def _products(dz, x, weight, dx, need_dw, scale):
+    """dX = dz W into ``dx`` (None: not wanted); returns dW = dz^T x or None.  ``scale``: that of dz."""
     (t, v), h = dz.shape, x.shape[1]
+    inverse = None if scale is None else scale.data_ptr() + 4
     if dx is not None:
-        gemm([dz], [weight], [dx], t, h, v, kmajor=(False, True), long_k=True)
+        gemm([dz], [weight], [dx], t, h, v, kmajor=(False, True), long_k=True, scale=inverse)
     if not need_dw:
         return None
     dw = torch.empty_like(weight)
-    gemm([dz], [x], [dw], v, h, t, kmajor=(True, True))
+    gemm([dz], [x], [dw], v, h, t, kmajor=(True, True), scale=inverse)
     return dw
 
 
@@ -288,7 +319,8 @@ def lm_head_logprobs(hidden, weight, tokens, *, top=0, temperature=1.0, ignore_i
 
     16-bit operands with H a multiple of 64 and V of 8, without alternatives: the results are formed beside the product, and no
     logits are written unless a gradient is wanted; then 16 bits of each are kept for it (their distance to the largest of 128),
-    which its own rounding takes the place of.  Otherwise the logits are written in fp32, 1 GiB of rows at a time."""
+    which its own rounding takes the place of.  Otherwise the logits are written in fp32, 1 GiB of rows at a time.  The products
+    that give the gradient take the logits' in the operands' type, in fp16 at a scale of its own: no loss scale is needed for it."""
     if hidden.ndim < 1 or weight.ndim != 2 or hidden.numel() < 1 or weight.numel() < 1 or hidden.shape[-1] != weight.shape[1]:
         raise ValueError('nonempty hidden [..., H] and weight [V, H] required')
     H.require_device(hidden, weight)

@@ -191,3 +191,48 @@ def test_lm_head_gradient_beside_ruled_out_tokens():
         # the groups are others: sums in another order, and distances to other maxima (0.034 % of each probability, twice)
         scale = float(b.double().abs().max())
         assert bool(a.isfinite().all()) and float((a.double() - b.double()).abs().max()) <= (2.0 ** -7 + 7e-4) * scale
+
+
+@pytest.mark.parametrize("top", [0, 3])
+@pytest.mark.parametrize("t,h,v", [(512, 64, 32000), (300, 72, 20000), (200, 64, 20001), (16, 256, 70000)])
+@pytest.mark.parametrize("size", [2.0 ** -14, 2.0 ** -24, 2.0 ** 18])
+def test_fp16_gradients_of_any_size(size, t, h, v, top):
+    """Upstream gradients that leave the gradient of single logits far below fp16's smallest number, or above its largest; dX and dW
+    are right wherever they fit the type themselves.  A logit's gradient may lose half a step of its own and 2^-38 of the largest that any could be, B."""
+    print(f"fp16 {size} {t} {h} {v} {top}", flush=True)
+    gen = seeded(t)
+    w = torch.randn((v, h), generator=gen) * 0.02
+    x = torch.randn((t, h), generator=gen)
+    up = 1.0 if size > 1 else 2.0 ** 6   # hidden states and weights that carry small gradients into fp16's range
+    w[:, 0], x[:, 1] = up, 8 * up
+    w[:, 1], x[:, 0] = 0.0, 0.0
+    x, w = x.half().cuda(), w.half().cuda()
+    ids = torch.randint(0, v, (t,), generator=gen).cuda()
+    ids[1] = -100
+    g, gh = size * torch.randn(t, generator=gen).cuda(), 0.1 * size * torch.randn(t, generator=gen).cuda()
+    g[1] = float('inf')   # a row that is left out
+    gtop = size * torch.randn((t, top), generator=gen).cuda()
+    xr, wr = x.clone().requires_grad_(), w.clone().requires_grad_()
+    out = lm_head_logprobs(xr, wr, ids, top=top)
+    dx, dw = torch.autograd.grad([o for o in out[:3] if o is not None], [xr, wr], [g, gh, gtop][:3 if top else 2])
+    g[1] = 0.0
+    gh[1] = 0.0
+    tid = out.top_tokens if top else torch.zeros((t, 0), dtype=torch.int64, device='cuda')
+    if top:
+        gtop[1] = 0.0
+    z = x.double() @ w.double().t()
+    e = 2 * ((h + 8) * E * (x.double().abs() @ w.double().abs().t())).amax(-1)
+    lp, _, ent, _, _ = reference(z, ids)
+    dz, tol = grads(z, ids, g, gh, gtop, tid, 1.0)
+    one = torch.zeros_like(z).scatter_(-1, ids.clamp(0)[:, None], 1.0).scatter_(-1, tid, 1.0)
+    wide = g.abs()[:, None] + gtop.abs().sum(-1, keepdim=True) + gh.abs()[:, None] * (3 + lp.abs() + ent[:, None])
+    largest = float((g.abs() + gtop.abs().sum(-1) + gh.abs() * (1 + torch.log(torch.tensor(float(v))))).max())
+    p = lp.exp()
+    tol = tol + 2.0 ** -11 * dz.abs() + (p + one * (1 - p)) * wide * e[:, None] + p * wide * 3.5e-4 + 2.0 ** -64 * wide + 2.0 ** -38 * largest
+    tol = torch.where((ids == -100)[:, None], 0.0, tol)
+    for got, exact, bound in ((dx, dz @ w.double(), tol @ w.double().abs() + (v + 8) * E * (dz.abs() @ w.double().abs())),
+                              (dw, dz.t() @ x.double(), tol.t() @ x.double().abs() + (t + 8) * E * (dz.abs().t() @ x.double().abs()))):
+        bound = bound + 2.0 ** -11 * exact.abs() + 2.0 ** -25
+        fits, over = exact.abs() + bound < 65504, exact.abs() - bound >= 65520   # fp16's largest, and from where on it rounds to infinity
+        near(torch.where(fits, got, 0.0), torch.where(fits, exact, 0.0), bound)
+        assert bool(fits.any()) and bool((got[over] == exact[over].sign() * float('inf')).all())
