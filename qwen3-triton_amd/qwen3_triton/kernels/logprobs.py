@@ -221,9 +221,9 @@ def _head_forward(x, weight, tokens, ignore_index, temperature, top, keep):
 class _LMHeadLogprobs(torch.autograd.Function):
     @staticmethod
     def forward(ctx, hidden, weight, tokens, ignore_index, temperature, top):
-        outs, (groups, ctx.z) = _head_forward(hidden.view(-1, weight.shape[1]), weight, tokens, ignore_index, temperature, top, True)
-        ctx.save_for_backward(hidden, weight, tokens, outs[4], outs[1], outs[3], groups, outs[0] if groups is not None else None)
-        ctx.rest = ignore_index, temperature, top
+        outs, (groups, z) = _head_forward(hidden.view(-1, weight.shape[1]), weight, tokens, ignore_index, temperature, top, True)
+        ctx.save_for_backward(hidden, weight, tokens, outs[4], outs[1], outs[3], groups, outs[0] if groups is not None else None, z)
+        ctx.rest, ctx.consumed = (ignore_index, temperature, top), False
         ctx.set_materialize_grads(False)
         lp, ent, tlp, tid = _shaped(hidden.shape[:-1], top, *outs)
         if not top:
@@ -234,18 +234,18 @@ class _LMHeadLogprobs(torch.autograd.Function):
     @staticmethod
     @once_differentiable
     def backward(ctx, g, gh, gtop=None, _=None):
-        hidden, weight, tokens, kept, ent, tid, groups, lp = ctx.saved_tensors
+        hidden, weight, tokens, kept, ent, tid, groups, lp, z = ctx.saved_tensors
         ignore_index, temperature, top = ctx.rest
         v, h = weight.shape
         x = hidden.view(-1, h)
         t = x.shape[0]
         g, gh, gtop = _upstream(g), _upstream(gh), _upstream(gtop)
-        z, ctx.z = ctx.z, None   # consumed: the gradient takes the stored logits' place
+        again, ctx.consumed = ctx.consumed, True   # the gradient takes the stored logits' place
         with H.on(x):
             dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
             scale = _grad_scale(x, g, gh, gtop, v, top, tokens, ignore_index, temperature)
             if groups is not None:
-                if z is None:   # a second backward: the same logits again
+                if again:   # a second backward: the same logits once more
                     z = _fused_product(x, weight, tokens, temperature, True)[2]
                 H.call("q3_head_logprobs_grad", H.code(x.dtype), z.data_ptr(), v, z.data_ptr(), v, t, v, tokens.data_ptr(), ignore_index,
                        1.0 / temperature, groups.data_ptr(), t, kept.data_ptr(), kept.data_ptr() + 4 * t, lp.data_ptr(), ent.data_ptr(),

@@ -236,3 +236,26 @@ def test_fp16_gradients_of_any_size(size, t, h, v, top):
         fits, over = exact.abs() + bound < 65504, exact.abs() - bound >= 65520   # fp16's largest, and from where on it rounds to infinity
         near(torch.where(fits, got, 0.0), torch.where(fits, exact, 0.0), bound)
         assert bool(fits.any()) and bool((got[over] == exact[over].sign() * float('inf')).all())
+
+
+# ------------------------------------------------------------------------------------------ backward passes
+def step(x, w, ids, g):
+    xr, wr = x.clone().requires_grad_(), w.clone().requires_grad_()
+    out = lm_head_logprobs(xr, wr, ids)
+    return torch.autograd.grad([out.logprobs, out.entropy], (xr, wr), [g, g])
+
+
+def test_saved_tensor_hooks_see_the_stored_logits():
+    """Offloading and recomputation work on all that the forward keeps: the 16 bits of each logit too."""
+    t, h, v = 70, 128, 1000
+    x, w, ids = head(t, h, v, BF16)
+    g = torch.randn(t, generator=seeded(1)).cuda()
+    want = step(x, w, ids, g)
+    seen = []
+    with torch.autograd.graph.saved_tensors_hooks(lambda s: (seen.append(s.numel() * s.element_size()), s.cpu())[1], lambda s: s.cuda()):
+        got = step(x, w, ids, g)
+    assert 2 * t * v in seen and all(torch.equal(a, b) for a, b in zip(got, want))
+    xr, wr = x.clone().requires_grad_(), w.clone().requires_grad_()
+    out = torch.utils.checkpoint.checkpoint(lambda a, b: lm_head_logprobs(a, b, ids)[:2], xr, wr, use_reentrant=False)
+    got = torch.autograd.grad(out, (xr, wr), [g, g])
+    assert all(torch.equal(a, b) for a, b in zip(got, want))
