@@ -223,7 +223,7 @@ class _LMHeadLogprobs(torch.autograd.Function):
     def forward(ctx, hidden, weight, tokens, ignore_index, temperature, top):
         outs, (groups, z) = _head_forward(hidden.view(-1, weight.shape[1]), weight, tokens, ignore_index, temperature, top, True)
         ctx.save_for_backward(hidden, weight, tokens, outs[4], outs[1], outs[3], groups, outs[0] if groups is not None else None, z)
-        ctx.rest, ctx.consumed = (ignore_index, temperature, top), False
+        ctx.rest, ctx.consumed, ctx.captured = (ignore_index, temperature, top), False, False
         ctx.set_materialize_grads(False)
         lp, ent, tlp, tid = _shaped(hidden.shape[:-1], top, *outs)
         if not top:
@@ -240,17 +240,21 @@ class _LMHeadLogprobs(torch.autograd.Function):
         x = hidden.view(-1, h)
         t = x.shape[0]
         g, gh, gtop = _upstream(g), _upstream(gh), _upstream(gtop)
-        again, ctx.consumed = ctx.consumed, True   # the gradient takes the stored logits' place
+        again = ctx.consumed
+        ctx.captured = ctx.captured or torch.cuda.is_current_stream_capturing()
+        ctx.consumed = again or not ctx.captured
         with H.on(x):
             dx = torch.empty_like(x) if ctx.needs_input_grad[0] else None
             scale = _grad_scale(x, g, gh, gtop, v, top, tokens, ignore_index, temperature)
             if groups is not None:
                 if again:   # a second backward: the same logits once more
                     z = _fused_product(x, weight, tokens, temperature, True)[2]
-                H.call("q3_head_logprobs_grad", H.code(x.dtype), z.data_ptr(), v, z.data_ptr(), v, t, v, tokens.data_ptr(), ignore_index,
+                # The gradient takes the stored logits' place, except where replays of a captured pass read them again.
+                dz = z if ctx.consumed else torch.empty_like(z)
+                H.call("q3_head_logprobs_grad", H.code(x.dtype), z.data_ptr(), v, dz.data_ptr(), v, t, v, tokens.data_ptr(), ignore_index,
                        1.0 / temperature, groups.data_ptr(), t, kept.data_ptr(), kept.data_ptr() + 4 * t, lp.data_ptr(), ent.data_ptr(),
                        None if g is None else g.data_ptr(), None if gh is None else gh.data_ptr(), _address(scale), H.stream())
-                dw = _products(z, x, weight, dx, ctx.needs_input_grad[1], scale)
+                dw = _products(dz, x, weight, dx, ctx.needs_input_grad[1], scale)
             else:
                 whole = gemm_ok(x, weight) and v % 8 == 0   # dW = dz^T x and dX = dz W from one dz [T, V]
                 chunks = _chunks(t, v)

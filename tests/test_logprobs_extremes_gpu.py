@@ -259,3 +259,35 @@ def test_saved_tensor_hooks_see_the_stored_logits():
     out = torch.utils.checkpoint.checkpoint(lambda a, b: lm_head_logprobs(a, b, ids)[:2], xr, wr, use_reentrant=False)
     got = torch.autograd.grad(out, (xr, wr), [g, g])
     assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("before", [0, 1])   # eager backward passes before the captured one
+def test_captured_backward_of_an_eager_forward(before):
+    """Replays of a backward pass alone, with other upstream gradients, beside eager work that takes and frees memory."""
+    t, h, v = 70, 128, 1000
+    x, w, ids = head(t, h, v, BF16)
+    up = torch.zeros(t, device='cuda')
+    stream = torch.cuda.Stream()
+    stream.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(stream):
+        xr, wr = x.clone().requires_grad_(), w.clone().requires_grad_()
+        out = lm_head_logprobs(xr, wr, ids)
+        for _ in range(before):
+            torch.autograd.grad([out.logprobs, out.entropy], (xr, wr), [up, up], retain_graph=True)
+    torch.cuda.current_stream().wait_stream(stream)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=stream):
+        got = torch.autograd.grad([out.logprobs, out.entropy], (xr, wr), [up, up], retain_graph=True)
+    torch.cuda.current_stream().wait_stream(stream)
+    for i in range(4):
+        g = torch.randn(t, generator=seeded(i)).cuda()
+        want = step(x, w, ids, g)
+        junk = [torch.full((t, v), float('nan'), dtype=BF16, device='cuda') for _ in range(4)]
+        up.copy_(g)
+        graph.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(got, want)), i
+        if i:   # an eager one between the replays
+            eager = torch.autograd.grad([out.logprobs, out.entropy], (xr, wr), [g, g], retain_graph=True)
+            assert all(torch.equal(a, b) for a, b in zip(eager, want)), i
+        del junk, want
