@@ -16,6 +16,7 @@ from ._ops import cast, ce_shift_labels
 from .linear import MAX_LD, gemm, gemm_nt_into, gemm_ok, matmul_into
 
 MAX_TOP = 32
+MAX_GRAD_VOCAB = MAX_LD - 64   # of lm_head_logprobs: what the products with the logits' gradient take, whichever of them run
 IGNORE_INDEX = -100
 _FLOATS = (torch.float32, torch.bfloat16, torch.float16)
 
@@ -319,7 +320,7 @@ def _products(dz, x, weight, dx, need_dw, scale):
 
 def lm_head_logprobs(hidden, weight, tokens, *, top=0, temperature=1.0, ignore_index=IGNORE_INDEX):
     """``token_logprobs`` of the logits ``hidden @ weight.T`` (hidden [..., H], weight [V, H], both fp32, bf16 or fp16), which
-    are formed in fp32; the gradient reaches hidden and weight.
+    are formed in fp32; the gradient reaches hidden and weight (V up to 2^22 - 64).
 
     16-bit operands with H a multiple of 64 and V of 8, without alternatives: the results are formed beside the product, and no
     logits are written unless a gradient is wanted; then 16 bits of each are kept for it (their distance to the largest of 128),
@@ -336,6 +337,8 @@ def lm_head_logprobs(hidden, weight, tokens, *, top=0, temperature=1.0, ignore_i
     _check_options(weight.shape[0], top, temperature, ignore_index)
     _check_tokens(tokens, hidden.shape[:-1], hidden)
     if _recorded(hidden, weight):
+        if weight.shape[0] > MAX_GRAD_VOCAB:
+            raise ValueError(f'a gradient takes at most {MAX_GRAD_VOCAB} tokens')
         return TokenLogprobs(*_LMHeadLogprobs.apply(hidden, weight, tokens, ignore_index, temperature, top))
     return TokenLogprobs(*_shaped(hidden.shape[:-1], top, *_head_forward(hidden.view(-1, weight.shape[1]), weight, tokens, ignore_index,
                                                                          temperature, top, False)[0]))

@@ -6,9 +6,10 @@ import pytest
 import torch
 
 from _util import seeded
-from test_logprobs_gpu import E, grads, head, near, reference
+from test_logprobs_gpu import E, check_head, grads, head, near, reference
 
-from qwen3_triton.kernels.logprobs import lm_head_logprobs, token_logprobs
+from qwen3_triton.kernels.linear import MAX_LD
+from qwen3_triton.kernels.logprobs import MAX_GRAD_VOCAB, lm_head_logprobs, token_logprobs
 
 pytestmark = pytest.mark.gpu
 F32, F16, BF16 = torch.float32, torch.float16, torch.bfloat16
@@ -236,6 +237,26 @@ def test_fp16_gradients_of_any_size(size, t, h, v, top):
         fits, over = exact.abs() + bound < 65504, exact.abs() - bound >= 65520   # fp16's largest, and from where on it rounds to infinity
         near(torch.where(fits, got, 0.0), torch.where(fits, exact, 0.0), bound)
         assert bool(fits.any()) and bool((got[over] == exact[over].sign() * float('inf')).all())
+
+
+def test_lm_head_of_a_very_long_vocabulary():
+    """The most tokens that a gradient takes, and more: log probabilities still, but no gradient, which is refused before any work."""
+    t, h = 3, 64
+    for v in (MAX_GRAD_VOCAB, MAX_GRAD_VOCAB - 1, MAX_LD + 8):
+        w = (torch.randn((v, h), generator=seeded(0)) * 0.1).bfloat16().cuda()
+        x = torch.randn((t, h), generator=seeded(1)).bfloat16().cuda()
+        ids = torch.randint(0, v, (t,), generator=seeded(2)).cuda()
+        for top in (0, 2):
+            if v <= MAX_GRAD_VOCAB:
+                check_head(x, w, ids, torch.ones(t, device='cuda'), torch.ones(t, device='cuda'), 1.0, t, top)
+                continue
+            out = lm_head_logprobs(x, w, ids, top=top)
+            dot = 72 * E * (x.double().abs() @ w.double().abs().t()).amax(-1)
+            _, lp, _, t_lp, _ = reference(x.double() @ w.double().t(), ids)
+            near(out.logprobs, lp, t_lp + 2 * dot)
+            for need in (0, 1):
+                with pytest.raises(ValueError, match='gradient'):
+                    lm_head_logprobs(x.clone().requires_grad_(need == 0), w.detach().requires_grad_(need == 1), ids, top=top)
 
 
 # ------------------------------------------------------------------------------------------ backward passes
