@@ -83,6 +83,8 @@ class KVCache:
     length: int = 0
     valid: bool = True
     resets: int = field(default=0, init=False)
+    forked: int = field(default=0, init=False)                    # positions that forks share
+    rewritten: list = field(default_factory=list, init=False)     # where forwards began below that
 
     prefix_length = 0   # of the positions, those that are another cache's
 
@@ -97,7 +99,7 @@ class KVCache:
     def fork(self, rows, max_length):
         """A cache for ``rows`` continuations of each of this cache's rows (row b continues row b // rows), of up to ``max_length``
         positions of their own.  The positions that this cache holds now are shared, not copied: it has to keep them (it may
-        grow)."""
+        grow; once it has been reset, or set back and written again, the fork refuses to go on)."""
         if type(rows) is not int or rows < 1 or type(max_length) is not int or max_length < 1:
             raise ValueError('a positive number of rows and of positions required')
         if not self.valid:
@@ -110,8 +112,15 @@ class KVCache:
 
         def layer_buffers(like):
             return [t.new_empty((self.batch_size * rows, h, max_length, d)) for t in like]
+        self.forked = max(self.forked, self.length)
         return SharedPrefixCache(layer_buffers(self.keys), layer_buffers(self.values), self.length + max_length,
                                  self.batch_size * rows, self.owner, self.length, prefix=self)
+
+    def write_from(self, start):
+        """Positions from ``start`` on are about to be written: forks that share some of them no longer can."""
+        if start < self.forked:
+            self.rewritten.append(start)
+            self.forked = start
 
     def quantized(self):
         """An ``Int8KVCache`` of the same positions (prefilled in 16 bits, decoded in 8)."""
@@ -137,11 +146,12 @@ class SharedPrefixCache(KVCache):
     prefix: Optional[KVCache] = None
 
     def __post_init__(self):
-        self.prefix_length, self._prefix_resets = self.length, self.prefix.resets
+        self.prefix_length, self._prefix_resets, self._prefix_rewritten = self.length, self.prefix.resets, len(self.prefix.rewritten)
 
     def admit(self, owner, batch, tokens):
         super().admit(owner, batch, tokens)
-        if self.prefix.resets != self._prefix_resets or not self.prefix.valid or self.prefix.length < self.prefix_length:
+        lost = any(start < self.prefix_length for start in self.prefix.rewritten[self._prefix_rewritten:])
+        if lost or self.prefix.resets != self._prefix_resets or not self.prefix.valid or self.prefix.length < self.prefix_length:
             raise ValueError('the cache that holds the shared positions no longer does')
 
     def shared(self, i):
@@ -490,6 +500,7 @@ class TritonQwen3Inference(nn.Module):
                 x = embedding(input_ids, table)
             except IdRangeError:
                 raise ValueError('Token ID outside vocabulary') from None
+        cache.write_from(start)
         pos = _ops.positions(b, s, start if start_dev is None else cache.prefix_length, self.device, start_dev)
         try:
             if x is None:
