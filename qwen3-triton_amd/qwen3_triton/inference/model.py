@@ -467,6 +467,11 @@ class TritonQwen3Inference(nn.Module):
             down = int8.linear(*int8.quantize_rows(y), *w.down)
         return residual_add(x, down)
 
+    def _check_positions(self, cache, tokens):
+        """Raise unless the model has ``tokens`` more positions (forked caches may be longer than it; others are made no longer)."""
+        if cache.prefix_length and cache.length + tokens > self.config.max_position_embeddings:
+            raise ValueError(f'the model has {self.config.max_position_embeddings} positions')
+
     def _forward(self, input_ids, cache, logits_to_keep, *, validate_ids=True, start_dev=None, head=True):
         """``start_dev``: the positions of the rows' own that are there before this step's, on the device.  Without ``head`` the
         normed hidden states take the logits' place."""
@@ -483,8 +488,7 @@ class TritonQwen3Inference(nn.Module):
         if self._int8 is not None:
             self._int8.check()
         start = cache.length
-        if cache.prefix_length and start + s > self.config.max_position_embeddings:   # other caches are made no longer
-            raise ValueError(f'the model has {self.config.max_position_embeddings} positions')
+        self._check_positions(cache, s)
         if start_dev is not None and s != 1:
             raise ValueError('device-resident positions are for single-token decode steps')
         x = None
@@ -640,6 +644,7 @@ class TritonQwen3Inference(nn.Module):
             if cache_dtype == torch.int8 and not isinstance(cache, Int8KVCache):
                 raise ValueError('past_key_values is not in int8')
             cache.admit(self._cache_owner, b, s + max_new_tokens - 1)
+            self._check_positions(cache, s + max_new_tokens - 1)
         output = torch.empty((b, s + max_new_tokens), device=self.device, dtype=torch.int64)
         output[:, :s].copy_(input_ids)
         done = torch.zeros((b,), device=self.device, dtype=torch.bool)
