@@ -192,6 +192,19 @@ Q3_DEV void softmax_block(Rows<U>& w, Step<U>& t, f32x4 (&S)[4][U], i32x4 (&P)[U
 #pragma unroll
   for (int u = 0; u < U; ++u) x[u] = row_max<U>(S, u);
   move_max(w, t, x, scale2, thr);
+  // A product of the maximum and the scale that passes 2^24 is off by more than 1: differences first there.
+  bool far = false;
+#pragma unroll
+  for (int u = 0; u < U; ++u) far = far || fabsf(t.ms[u]) > 0x1p24f;
+  if (__builtin_expect(__any(far), 0)) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const float m = w.m[u] == -INFINITY ? 0.f : w.m[u];
+#pragma unroll
+      for (int kt = 0; kt < 4; ++kt) S[kt][u] -= m;
+      t.ms[u] = 0.f;
+    }
+  }
 #pragma unroll
   for (int u = 0; u < U; ++u)
 #pragma unroll

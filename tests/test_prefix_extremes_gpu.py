@@ -2,6 +2,7 @@
 import pytest
 import torch
 
+from _util import seeded
 from test_prefix_gpu import DTYPES, expected, inputs
 
 from qwen3_triton.inference import prefix as PX
@@ -55,3 +56,21 @@ def test_keys_of_the_prefix_that_are_not_numbers(r, n, s, hq, hkv, p, start, dty
     got = PX.attention(*t, start)
     assert bool(got[:n].isnan().all())
     assert torch.equal(got[n:], want[n:])
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("r,n,s,hq,hkv,p,start", FORMS)
+def test_very_large_scores(r, n, s, hq, hkv, p, start, dtype):
+    """Scores of 2^34 and more, exact in fp32 and at least 2^30 apart where they differ: each query's output is the mean of the values at
+    its largest one."""
+    t = inputs(r, n, s, hq, hkv, p, start + s + 9, dtype)
+    gen = seeded(p + s)
+    t[0].copy_((2 ** 15 * (1 - 2 * torch.randint(0, 2, t[0].shape[:3], generator=gen)))[..., None])
+    for k in (t[1], t[3]):
+        k.copy_((2 ** 12 * torch.randint(-8, 9, k.shape[:3], generator=gen))[..., None])
+    got = PX.attention(*t, start)
+    o, _ = expected(*t, [start] * (r * n))
+    a, _ = expected(t[0], t[1], t[2].abs(), t[3], t[4].abs(), [start] * (r * n))
+    u = torch.finfo(dtype).eps / 2   # the output's rounding; weights of 2^x, equal ones alike, and their sum in fp32
+    tol = u * o.abs() + (u + 2.0 ** -14) * a + 2.0 ** -24
+    assert float(((got.double() - o).abs() / tol).nan_to_num(nan=1e9).max()) <= 1.0
