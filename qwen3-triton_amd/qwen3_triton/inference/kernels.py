@@ -11,10 +11,10 @@ from ..kernels import _ops
 from ..kernels.linear import matmul
 
 
-def positions(batch, sequence, start, device, start_dev=None):
+def positions(batch, sequence, start, device, start_dev=None, before=0):
     """``inference/kernels.py:18``: [B,S] int64 positions start..start+S-1 (offset by the device
-    int64 ``start_dev`` when given)."""
-    return _ops.positions(batch, sequence, start if start_dev is None else 0, device, start_dev)
+    int64 ``start_dev`` when given, which counts the positions that follow the first ``before``)."""
+    return _ops.positions(batch, sequence, start if start_dev is None else before, device, start_dev)
 
 
 def append(k, v, cache_k, cache_v, start, start_dev=None):

@@ -505,7 +505,7 @@ class TritonQwen3Inference(nn.Module):
             except IdRangeError:
                 raise ValueError('Token ID outside vocabulary') from None
         cache.write_from(start)
-        pos = _ops.positions(b, s, start if start_dev is None else cache.prefix_length, self.device, start_dev)
+        pos = kernels.positions(b, s, start, self.device, start_dev, cache.prefix_length)
         try:
             if x is None:
                 x = embedding(input_ids, self.model.embed_tokens.weight)

@@ -93,9 +93,12 @@ def norm_rope_qk_cache_fwd(q, k, v, wq, wk, cos, sin, cache_k, cache_v, start, e
     b, s, hq, d = q.shape
     hk = k.shape[2]
     yq = torch.empty_like(q)
-    H.call("q3_norm_rope_qk_cache_dev_fwd", H.code(q.dtype), q.data_ptr(), k.data_ptr(), v.data_ptr(), wq.data_ptr(),
-           wk.data_ptr(), cos.data_ptr(), sin.data_ptr(), yq.data_ptr(), cache_k.data_ptr(), cache_v.data_ptr(), b, s,
-           hq, hk, d, cache_k.shape[2], start, None if start_dev is None else start_dev.data_ptr(), float(eps), H.stream())
+    args = (H.code(q.dtype), q.data_ptr(), k.data_ptr(), v.data_ptr(), wq.data_ptr(), wk.data_ptr(), cos.data_ptr(), sin.data_ptr(),
+            yq.data_ptr(), cache_k.data_ptr(), cache_v.data_ptr(), b, s, hq, hk, d, cache_k.shape[2], start)
+    if start_dev is None:
+        H.call("q3_norm_rope_qk_cache_fwd", *args, float(eps), H.stream())
+    else:
+        H.call("q3_norm_rope_qk_cache_dev_fwd", *args, start_dev.data_ptr(), float(eps), H.stream())
     return yq
 
 
