@@ -696,8 +696,8 @@ int q3_gemm_nt_ce_stats_store(int dtype, const void* A, int64_t lda, const void*
   return q3gemm::launch_tile_nt(dtype, big ? 0 : 1, 2, a, stream);
 }
 
-// LM-head logits A B^T and their log probability statistics (q3hip.h), stored less their groups' maxima where z is set: 256 x 256
-// tiles, 128 x 256 as above, 32 x 256 with a deeper ring for few rows, which wait for the weight.
+// LM-head logits A B^T and their log probability statistics (q3hip.h), with the logits' distances to their groups' maxima where z is set, in
+// the tiles of logprob_plan: one launch, or a second one for the last columns.
 int q3_gemm_nt_logprobs(int dtype, const void* A, int64_t lda, const void* B, int64_t ldb, int64_t M, int64_t N, int64_t K,
                         const int64_t* tokens, float inv_temperature, float* m_part, float* rest_part, float* u_part, float* pick,
                         int64_t ldp, void* z, int64_t ldz, hipStream_t stream) {

@@ -318,7 +318,7 @@ __global__ __launch_bounds__(kThreads) void slice_kernel(Fwd a) {
 }
 
 // ---------------------------------------------------------------- a row's slices joined
-// One wave a row, no alternatives (4096 rows 5 us: a launch).
+// One wave a row, no alternatives (2048 rows of three parts 4 us: a launch).
 template <typename T> __global__ __launch_bounds__(kThreads) void finish_kernel(Fwd a) {
   const int64_t r = (int64_t)blockIdx.x * (kThreads / 64) + (threadIdx.x >> 6);
   const int lane = threadIdx.x & 63;

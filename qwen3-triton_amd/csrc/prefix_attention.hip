@@ -283,7 +283,7 @@ struct Job {
   int b0, hk, tile, slot;  // first row b of the job's query rows
   int rows;                // query rows from b0's first on
   int pb, npre, sb, nblk;
-  int own, all, start;     // own positions that the job's last query row sees
+  int own, start;          // own positions that the job's last query row sees
   const u16 *pk, *pv, *ck, *cv;
 };
 struct Block {  // one of them: 64 positions from key0 on, `count` of them there

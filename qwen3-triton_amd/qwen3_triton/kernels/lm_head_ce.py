@@ -82,7 +82,7 @@ class _LMHeadCE(torch.autograd.Function):
         loss = st.finish(tgt, v, ignore_index)
         ctx.save_for_backward(hidden, weight, tgt, st.lse, st.count)
         ctx.ignore, ctx.chunk = ignore_index, chunk
-        ctx.z = z
+        ctx.z = z   # not a saved tensor: hooks (offloading, checkpointing) do not see it
         return loss.clone()
 
     @staticmethod
