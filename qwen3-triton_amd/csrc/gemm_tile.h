@@ -117,7 +117,7 @@ Q3_DEV void work_coords(int bid, int tiles_m, int tiles_n, int splits, int& tm, 
 // the rounded logits, which are stored too; 3: gate/up SwiGLU; 5: SwiGLU backward; 6: log probability statistics
 // (logprobs.h) of the fp32 logits per row and 128-column group, to m_part, s_part and u_part, with the logit of column tgt[row]
 // to pick[row], and where c[0] is set the logits' distances to their group's maximum in 16 bits (q3lp::kGapRange).  4096 x 151936 x 4096 takes 3.71 ms
-// with the statistics alone and 3.91 with the distances (1.30 PFLOP/s), as a plain product that writes its logits 3.76.  7: as 6, and B
+// with the statistics alone and 3.93 with the distances (1.29 PFLOP/s), as a plain product that writes its logits 3.76.  7: as 6, and B
 // is read past the caches (non-temporal).  8: as 0, times *oscale.  KP: A and B in pieces along K.
 template <typename T, int BM, int BN, int WM, int WN, int STAGES, bool AT, bool BT, int EPI, bool KP, bool Q8>
 __global__ __launch_bounds__(WM * WN * 64) void gemm_tile_kernel(Args ar) {

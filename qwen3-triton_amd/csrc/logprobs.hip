@@ -422,7 +422,7 @@ Q3_DEV float scale_of(const Bwd& a) { return a.scale ? *a.scale : 1.f; }
 // round: with a mean of 4096 rows and 151936 tokens, single values (1e-9) would be below its smallest number and add up to nothing.
 // scale[0] = 2^e such that no value passes 2^14, scale[1] = 2^-e: what |dz| is at most, c (|g| + sum |g_j| + |h| (1 + log V)), from all
 // rows that are not left out and have a number for it (p |log p| <= 1 / e, p entropy <= log V).  One value for all rows, since dW sums over
-// them.  One workgroup (4096 rows 5 us).
+// them.  One workgroup (4096 rows 7.6 us).
 constexpr int kScaleThreads = 1024;
 __global__ __launch_bounds__(kScaleThreads) void scale_kernel(Bwd a, float log_v, float* __restrict__ scale) {
   __shared__ float wave_most[kScaleThreads / 64];
@@ -591,7 +591,7 @@ template <int R, int NT> __global__ __launch_bounds__(NT) void head_finish_kerne
 
 // dz from what the product left of the logits (their distances to their group's maximum), in its place or elsewhere: as grad_kernel, with
 // log2 p = (c2 (m_group - M) - ls log2(e)) - distance; the given token's log p is the result itself.  Bound by z, read and written
-// (4096 x 151936: 2.5 GB in 442 us, 5.6 TB/s).
+// (4096 x 151936: 2.5 GB in 446 us, 5.6 TB/s).
 template <typename O> __global__ __launch_bounds__(kThreads) void head_grad_kernel(Head h, Bwd a, const float* logprob, int slices) {
   constexpr int C = kGradVectors, N = kThreads * 8 * C;
   const int64_t r = blockIdx.x / (unsigned)slices;

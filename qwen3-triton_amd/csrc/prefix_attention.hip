@@ -334,7 +334,7 @@ template <typename T> Q3_DEV void store4(const Args& a, int64_t part, int64_t ou
 }
 
 // More query rows: 32 a wave.  Bound by the matrix cores and the softmax between them: 8 x 200 queries of 32 heads behind 4001 (256
-// tiles, 78 % full) 125 us, 0.87 PFLOP/s; 64 single queries behind 32768, with up to 1000 positions of the rows' own in jobs beside,
+// tiles, 78 % full) 131 us, 0.82 PFLOP/s; 64 single queries behind 32768, with up to 1000 positions of the rows' own in jobs beside,
 // 67 us (265 MB, 4.0 TB/s).  A third K and V tile in flight, or the softmax of one block beside the products of the next, gave
 // nothing more (138 and 134 us where this took 134).
 template <typename T, int NW> Q3_DEV void tile_job(const Args& a, const Job& job, char* lds, int wave, int g, int r16) {
